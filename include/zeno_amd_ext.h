@@ -2,14 +2,16 @@
  * zeno_amd_ext.h — extension entry points of libzeno (MI355X build).
  *
  * None of these exist in the reference's C ABI (Lulzx/zeno); they sit beside the reference
- * ABI of zeno.h and serve four callers:
+ * ABI of zeno.h and serve five callers:
  *   - inspection of the model a world was built from (tests and the CPU oracle read the
  *     constraint templates, colours and records the kernels use), without a GPU;
  *   - device-resident stepping and timing for benchmarks and graph capture;
  *   - solver state that the reference keeps but never exposes (lambda, previous contact
  *     count, spatial-hash cells), used by parity tests;
  *   - the reference's Zig-level collision routine (narrow_phase.detectCollision) for C
- *     callers, batched on the GPU.
+ *     callers, batched on the GPU;
+ *   - policies with memory that act on the environments: their memory layer (one token per
+ *     environment, and whole rollouts with gradients) and the update of their matrices.
  */
 #ifndef ZENO_AMD_EXT_H
 #define ZENO_AMD_EXT_H
@@ -222,6 +224,78 @@ int zeno_amd_selfcheck_sqrt(const float* x, float* y, uint32_t n);
  * the correctly rounded fp32 a / b when this is below about 2^-49.1. Runs on the current
  * device (2^32 divisors, well under a second) and waits. */
 int zeno_amd_selfcheck_reciprocal_error(double* max_err);
+
+/* ---- Operators of policies with memory ------------------------------------------------
+ * No counterpart in the reference. A policy that acts on partial observations keeps a state
+ * for each environment and head beside the simulation. Its memory layer here is the gated
+ * delta rule: per sequence (environment) and value head, S [key_dim, value_dim],
+ *
+ *     S <- exp(g) S                          (S <- 0 at a token whose reset flag is set)
+ *     S <- S + k (beta (v - S^T k))^T
+ *     o  = scale S^T q
+ *
+ * with q and k of key head (value head / (value_heads / key_heads)), divided by
+ * sqrt(sum of squares + 1e-6) first where `normalize` is set. A token with g < -104, whose
+ * exp is 0 in fp32, counts as a reset: nothing before it, NaN or infinity included, reaches
+ * what follows. q, k, v and o have one element type; g, beta and every state are fp32, and
+ * all sums are.
+ *
+ * All pointers are device pointers of the current device. Strides are in elements (sequence,
+ * token, head); the last dimension of q, k, v and o is contiguous; strides may be anything
+ * else, 0 included for inputs, and outputs must not overlap. Calls return after enqueueing on
+ * `stream` (a hipStream_t; null = the default stream). */
+#define ZENO_AMD_FLOAT32 0u
+#define ZENO_AMD_FLOAT16 1u
+#define ZENO_AMD_BFLOAT16 2u
+#define ZENO_AMD_DELTA_MAX_DIM 128u /* of key_dim and value_dim */
+
+typedef struct {
+    uint32_t dtype;                   /* of q, k, v, o and their gradients */
+    uint32_t batch, length;           /* sequences, tokens */
+    uint32_t key_heads, value_heads;  /* value_heads is a multiple of key_heads */
+    uint32_t key_dim, value_dim;      /* 1 to ZENO_AMD_DELTA_MAX_DIM */
+    uint32_t normalize;
+    float scale;
+    const void *q, *k, *v;
+    const float *g, *beta;            /* log of the decay; strength of the correction */
+    const uint8_t* reset;             /* [sequence, token], nonzero: the state is cleared before it; null: none */
+    const float* state;               /* [batch, value_heads, key_dim, value_dim] before the first token; null: zeros */
+    int64_t q_stride[3], k_stride[3], v_stride[3];
+    int64_t g_stride[3], beta_stride[3];
+    int64_t reset_stride[2];
+} ZenoAmdDeltaInputs;
+
+/* Gradients: of o and of the last state (null: zeros) in; of the inputs out. d_state may be
+ * null. Strides as above. */
+typedef struct {
+    const void* d_o;
+    int64_t d_o_stride[3];
+    const float* d_last;
+    void *d_q, *d_k, *d_v;
+    float *d_g, *d_beta;
+    float* d_state;
+    int64_t d_q_stride[3], d_k_stride[3], d_v_stride[3], d_g_stride[3], d_beta_stride[3];
+} ZenoAmdDeltaGradients;
+
+/* Whole sequences. o [batch, length, value_heads, value_dim] by o_stride; last [batch,
+ * value_heads, key_dim, value_dim], contiguous, the state after the last token (it may not be
+ * `in->state`). `saved`: null, or zeno_amd_delta_saved_bytes(in) bytes that the gradients of
+ * this call read. */
+int zeno_amd_delta_forward(const ZenoAmdDeltaInputs* in, void* o, const int64_t* o_stride, float* last, void* saved, void* stream);
+
+/* Gradients of a zeno_amd_delta_forward call with the same inputs, whose `last` and `saved`
+ * it left. `workspace`: zeno_amd_delta_workspace_bytes(in) bytes (null where that is 0).
+ * Gradients of key heads that several value heads share are summed in a fixed order: results
+ * are bitwise reproducible. */
+int zeno_amd_delta_backward(const ZenoAmdDeltaInputs* in, const float* last, const void* saved, const ZenoAmdDeltaGradients* grad,
+                            void* workspace, void* stream);
+
+uint64_t zeno_amd_delta_saved_bytes(const ZenoAmdDeltaInputs* in);      /* 0 also for invalid inputs */
+uint64_t zeno_amd_delta_workspace_bytes(const ZenoAmdDeltaInputs* in);
+
+/* One token (length 1) for every sequence: `state` is advanced in place (in->state is not
+ * read). What runs beside a step of the simulation. */
+int zeno_amd_delta_step(const ZenoAmdDeltaInputs* in, void* o, const int64_t* o_stride, float* state, void* stream);
 
 #ifdef __cplusplus
 }

@@ -84,10 +84,38 @@ class ZenoAmdModelView(C.Structure):
     ]
 
 
+class ZenoAmdDeltaInputs(C.Structure):
+    """include/zeno_amd_ext.h"""
+
+    _fields_ = [
+        ("dtype", C.c_uint32), ("batch", C.c_uint32), ("length", C.c_uint32),
+        ("key_heads", C.c_uint32), ("value_heads", C.c_uint32), ("key_dim", C.c_uint32), ("value_dim", C.c_uint32),
+        ("normalize", C.c_uint32), ("scale", C.c_float),
+        ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("g", C.c_void_p), ("beta", C.c_void_p),
+        ("reset", C.c_void_p), ("state", C.c_void_p),
+        ("q_stride", C.c_int64 * 3), ("k_stride", C.c_int64 * 3), ("v_stride", C.c_int64 * 3),
+        ("g_stride", C.c_int64 * 3), ("beta_stride", C.c_int64 * 3), ("reset_stride", C.c_int64 * 2),
+    ]
+
+
+class ZenoAmdDeltaGradients(C.Structure):
+    """include/zeno_amd_ext.h"""
+
+    _fields_ = [
+        ("d_o", C.c_void_p), ("d_o_stride", C.c_int64 * 3), ("d_last", C.c_void_p),
+        ("d_q", C.c_void_p), ("d_k", C.c_void_p), ("d_v", C.c_void_p), ("d_g", C.c_void_p), ("d_beta", C.c_void_p),
+        ("d_state", C.c_void_p),
+        ("d_q_stride", C.c_int64 * 3), ("d_k_stride", C.c_int64 * 3), ("d_v_stride", C.c_int64 * 3),
+        ("d_g_stride", C.c_int64 * 3), ("d_beta_stride", C.c_int64 * 3),
+    ]
+
+
 _vp = C.c_void_p
 _fp = C.POINTER(C.c_float)
 _u8p = C.POINTER(C.c_uint8)
 _u32p = C.POINTER(C.c_uint32)
+_i64p = C.POINTER(C.c_int64)
+_delta = C.POINTER(ZenoAmdDeltaInputs)
 
 # name: (restype, argtypes)
 SIGNATURES = {
@@ -175,6 +203,11 @@ SIGNATURES = {
     "zeno_amd_selfcheck_divide": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint32]),
     "zeno_amd_selfcheck_sqrt": (C.c_int, [C.c_void_p, C.c_void_p, C.c_uint32]),
     "zeno_amd_selfcheck_reciprocal_error": (C.c_int, [C.c_void_p]),
+    "zeno_amd_delta_forward": (C.c_int, [_delta, _vp, _i64p, _vp, _vp, _vp]),
+    "zeno_amd_delta_backward": (C.c_int, [_delta, _vp, _vp, C.POINTER(ZenoAmdDeltaGradients), _vp, _vp]),
+    "zeno_amd_delta_saved_bytes": (C.c_uint64, [_delta]),
+    "zeno_amd_delta_workspace_bytes": (C.c_uint64, [_delta]),
+    "zeno_amd_delta_step": (C.c_int, [_delta, _vp, _i64p, _vp, _vp]),
     "zeno_amd_world_waves_per_group": (C.c_uint32, [C.c_void_p]),
     "zeno_amd_world_split_groups": (C.c_int, [C.c_void_p]),
 }

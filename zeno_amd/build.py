@@ -37,6 +37,14 @@ HIP_FLAGS = [
 # instructions by up to 7% either way (110 swimmers of four substeps 111 or 119 us with identical code
 # in their loops, 114 aligned; a 32-step schedule of 4096 Ants 1362, 1381 and 1366); 128 bytes gain nothing more.
 STEP_FLAGS = ["-Rpass-analysis=kernel-resource-usage", "-mllvm", "-align-all-nofallthru-blocks=6"]
+# The operators of policies are compared with tolerances, not bit for bit: products and sums may
+# contract. No packed fp32 instructions here either.
+POLICY_SOURCES = ("delta.hip", "delta_f32.hip", "delta_f16.hip", "delta_bf16.hip")
+POLICY_FLAGS = [
+    f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-fno-fast-math",
+    "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
+    "-Wall", "-Wno-unused-result",
+]
 CXX_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-ffp-contract=off", "-fno-fast-math", "-Wall", "-Wextra"]
 ORACLE_FLAGS = ["-O2", "-std=c11", "-fPIC", "-shared", "-ffp-contract=off", "-fno-fast-math", "-fopenmp", "-Wall"]
 
@@ -100,6 +108,8 @@ def build_library() -> Path:
         obj = BUILD / (src + ".o")
         extra = STEP_FLAGS if src == "step.hip" else []
         jobs.append([hipcc, *HIP_FLAGS, *extra, "-c", str(CSRC / src), "-o", str(obj)])
+    for src in POLICY_SOURCES:
+        jobs.append([hipcc, *POLICY_FLAGS, "-c", str(CSRC / src), "-o", str(BUILD / (src + ".o"))])
     with ThreadPoolExecutor(max_workers=min(len(jobs), os.cpu_count() or 4)) as ex:
         outs = list(ex.map(_run, jobs))
     remarks = outs[2]
@@ -107,7 +117,7 @@ def build_library() -> Path:
     occ = step_occupancy(remarks)
     print("step_kernel waves per SIMD (EPW,PL,HASH): " + " ".join(f"{k}={v}" for k, v in sorted(occ.items())),
           file=sys.stderr)
-    objs = [str(BUILD / (s + ".o")) for s in ("mjcf.cpp", "model.cpp", "step.hip", "world.hip", "capi.hip", "collide.hip")]
+    objs = [str(BUILD / (s + ".o")) for s in ("mjcf.cpp", "model.cpp", "step.hip", "world.hip", "capi.hip", "collide.hip", *POLICY_SOURCES)]
     tmp = LIB.with_suffix(".so.tmp")
     _run([hipcc, f"--offload-arch={ARCH}", "-shared", "-fPIC", *objs, "-o", str(tmp)])
     os.replace(tmp, LIB)

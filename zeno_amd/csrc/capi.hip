@@ -10,6 +10,7 @@
 #include "../../include/zeno.h"
 #include "../../include/zeno_amd_ext.h"
 #include "collide.h"
+#include "delta.h"
 #include "world.h"
 
 using za::World;
@@ -539,6 +540,46 @@ int zeno_amd_selfcheck_sqrt(const float* x, float* y, uint32_t n) {
 int zeno_amd_selfcheck_reciprocal_error(double* max_err) {
     if (!max_err) return ZENO_INVALID_ARGUMENT;
     return hip_status(za::selfcheck_rcp_error_host(max_err), "selfcheck_reciprocal_error");
+}
+
+// ---- Operators of policies with memory ---------------------------------------------------
+static int delta_refused(const char* what, const std::string& why) {
+    set_error(std::string(what) + ": " + why);
+    return ZENO_INVALID_ARGUMENT;
+}
+
+int zeno_amd_delta_forward(const ZenoAmdDeltaInputs* in, void* o, const int64_t* o_stride, float* last, void* saved, void* stream) {
+    const std::string why = za::delta::check(in, false);
+    if (!why.empty()) return delta_refused("delta_forward", why);
+    if (!o || !o_stride || !last) return delta_refused("delta_forward", "null output");
+    if (last == in->state) return delta_refused("delta_forward", "the last state would overwrite the first");
+    return hip_status(za::delta::forward(*in, o, o_stride, last, (float*)saved, (hipStream_t)stream), "delta_forward");
+}
+
+int zeno_amd_delta_backward(const ZenoAmdDeltaInputs* in, const float* last, const void* saved, const ZenoAmdDeltaGradients* grad,
+                            void* workspace, void* stream) {
+    const std::string why = za::delta::check(in, false);
+    if (!why.empty()) return delta_refused("delta_backward", why);
+    if (!grad || !grad->d_o || !grad->d_q || !grad->d_k || !grad->d_v || !grad->d_g || !grad->d_beta)
+        return delta_refused("delta_backward", "null gradient");
+    if (!last || (!saved && za::delta::saved_floats(*in))) return delta_refused("delta_backward", "null state of the forward call");
+    if (!workspace && za::delta::workspace_floats(*in)) return delta_refused("delta_backward", "null workspace");
+    return hip_status(za::delta::backward(*in, last, (const float*)saved, *grad, (float*)workspace, (hipStream_t)stream), "delta_backward");
+}
+
+uint64_t zeno_amd_delta_saved_bytes(const ZenoAmdDeltaInputs* in) {
+    return in && za::delta::check_sizes(*in).empty() ? 4 * za::delta::saved_floats(*in) : 0;
+}
+
+uint64_t zeno_amd_delta_workspace_bytes(const ZenoAmdDeltaInputs* in) {
+    return in && za::delta::check_sizes(*in).empty() ? 4 * za::delta::workspace_floats(*in) : 0;
+}
+
+int zeno_amd_delta_step(const ZenoAmdDeltaInputs* in, void* o, const int64_t* o_stride, float* state, void* stream) {
+    const std::string why = za::delta::check(in, true);
+    if (!why.empty()) return delta_refused("delta_step", why);
+    if (!o || !o_stride || !state) return delta_refused("delta_step", "null output or state");
+    return hip_status(za::delta::step(*in, o, o_stride, state, (hipStream_t)stream), "delta_step");
 }
 
 }  // extern "C"

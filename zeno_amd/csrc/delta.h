@@ -1,0 +1,61 @@
+// The gated delta rule: host side (argument checks, launch shapes) and the kernels' arguments.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <string>
+
+#include "../../include/zeno_amd_ext.h"
+
+namespace za {
+namespace delta {
+
+// What a kernel reads and writes. Strides are in elements: sequence, token, head.
+struct Args {
+    ZenoAmdDeltaInputs in;
+    void* o;
+    int64_t o_stride[3];
+    float* last;                 // [batch, value_heads, key_dim, value_dim]
+    float* saved;                // states inside the sequences (training), see saved_floats
+    uint32_t chunks;             // chunks of the grid that a sequence has
+    uint32_t share;              // value heads per key head
+    bool q_vec, k_vec, v_vec, o_vec, s_vec;  // 16-byte accesses are aligned
+    // backward
+    const void* d_o;
+    int64_t d_o_stride[3];
+    bool d_o_vec;
+    const float* d_last;         // null: zeros
+    void *dq, *dk, *dv;
+    int64_t dq_stride[3], dk_stride[3], dv_stride[3];
+    bool dq_vec, dk_vec, dv_vec;
+    float *dg, *dbeta;
+    int64_t dg_stride[3], dbeta_stride[3];
+    float* d_state;              // null: not wanted
+    float *part_q, *part_k;      // gradients per value head where heads share keys: [batch, length, value_heads, key_dim]
+};
+
+// Launch shape of the chunked kernels, by sizes and type alone.
+struct Shape {
+    int dk;      // key columns held: 64 or 128
+    int waves;   // of 16 value columns each: 4 or 8
+    int tiles;   // chunk of 16 or 32 tokens
+};
+Shape shape_of(const ZenoAmdDeltaInputs& in);
+uint64_t saved_floats(const ZenoAmdDeltaInputs& in);
+
+// One translation unit per element type.
+template <int TY> hipError_t launch_forward(const Args& a, const Shape& s, hipStream_t stream);
+template <int TY> hipError_t launch_backward(const Args& a, const Shape& s, hipStream_t stream);
+template <int TY> hipError_t launch_step(const Args& a, float* state, hipStream_t stream);
+
+// Entry points behind the C ABI. A non-empty message means that nothing was launched.
+std::string check_sizes(const ZenoAmdDeltaInputs& in);
+std::string check(const ZenoAmdDeltaInputs* in, bool step);
+hipError_t forward(const ZenoAmdDeltaInputs& in, void* o, const int64_t* o_stride, float* last, float* saved, hipStream_t stream);
+hipError_t backward(const ZenoAmdDeltaInputs& in, const float* last, const float* saved, const ZenoAmdDeltaGradients& grad, float* workspace,
+                    hipStream_t stream);
+hipError_t step(const ZenoAmdDeltaInputs& in, void* o, const int64_t* o_stride, float* state, hipStream_t stream);
+uint64_t workspace_floats(const ZenoAmdDeltaInputs& in);
+
+}  // namespace delta
+}  // namespace za

@@ -1,0 +1,150 @@
+// The gated delta rule: argument checks, launch shapes and dispatch by element type.
+#include "delta.h"
+
+#include <cmath>
+
+#include "mma.h"
+
+namespace za {
+namespace delta {
+
+using mma::T_BF16;
+using mma::T_F16;
+using mma::T_F32;
+
+namespace {
+
+uint32_t element_bytes(uint32_t dtype) { return dtype == T_F32 ? 4 : 2; }
+
+// Whether eight elements along a row can move in 16-byte accesses: the base and every stride
+// that is used are multiples of 16 bytes.
+bool vectors(const void* p, const int64_t* stride, uint32_t batch, uint32_t length, uint32_t heads, uint32_t bytes) {
+    const int64_t n[3] = {batch, length, heads};
+    if ((uintptr_t)p % 16) return false;
+    for (int i = 0; i < 3; ++i)
+        if (n[i] > 1 && stride[i] * bytes % 16) return false;
+    return true;
+}
+
+hipError_t by_type(uint32_t dtype, hipError_t (*f32)(const Args&, const Shape&, hipStream_t), hipError_t (*f16)(const Args&, const Shape&, hipStream_t),
+                   hipError_t (*bf16)(const Args&, const Shape&, hipStream_t), const Args& a, const Shape& s, hipStream_t stream) {
+    return (dtype == T_F32 ? f32 : dtype == T_F16 ? f16 : bf16)(a, s, stream);
+}
+
+Args common(const ZenoAmdDeltaInputs& in, const Shape& s) {
+    Args a{};
+    a.in = in;
+    a.share = in.value_heads / in.key_heads;
+    a.chunks = (in.length + 16 * s.tiles - 1) / (16 * s.tiles);
+    const uint32_t eb = element_bytes(in.dtype);
+    a.q_vec = vectors(in.q, in.q_stride, in.batch, in.length, in.key_heads, eb);
+    a.k_vec = vectors(in.k, in.k_stride, in.batch, in.length, in.key_heads, eb);
+    a.v_vec = vectors(in.v, in.v_stride, in.batch, in.length, in.value_heads, eb);
+    a.s_vec = in.value_dim % 4 == 0 && (uintptr_t)in.state % 16 == 0;
+    return a;
+}
+
+void set_strides(int64_t* to, const int64_t* from) {
+    for (int i = 0; i < 3; ++i) to[i] = from[i];
+}
+
+}  // namespace
+
+// 16 tokens a chunk where 32 do not fit the 160 KB of a CU in the gradients' kernel.
+Shape shape_of(const ZenoAmdDeltaInputs& in) {
+    Shape s;
+    s.dk = in.key_dim <= 64 ? 64 : 128;
+    s.waves = s.dk == 128 || in.value_dim > 64 ? 8 : 4;
+    s.tiles = s.waves == 8 && (in.dtype == T_F32 || (in.dtype == T_F16 && s.dk == 128)) ? 1 : 2;
+    return s;
+}
+
+uint64_t saved_floats(const ZenoAmdDeltaInputs& in) {
+    const Shape s = shape_of(in);
+    const uint64_t chunks = (in.length + 16 * s.tiles - 1) / (16 * s.tiles);
+    return chunks < 2 ? 0 : (uint64_t)in.batch * in.value_heads * (chunks - 1) * s.dk * (16 * s.waves);
+}
+
+uint64_t workspace_floats(const ZenoAmdDeltaInputs& in) {
+    return in.key_heads == in.value_heads ? 0 : 2ull * in.batch * in.length * in.value_heads * in.key_dim;
+}
+
+std::string check_sizes(const ZenoAmdDeltaInputs& in) {
+    if (in.dtype > T_BF16) return "dtype is none of float32, float16, bfloat16";
+    if (!in.batch || !in.length || !in.key_heads || !in.value_heads) return "batch, length and head counts must be positive";
+    if (in.value_heads % in.key_heads) return "value_heads is not a multiple of key_heads";
+    if (!in.key_dim || in.key_dim > ZENO_AMD_DELTA_MAX_DIM || !in.value_dim || in.value_dim > ZENO_AMD_DELTA_MAX_DIM)
+        return "key_dim and value_dim must be 1 to " + std::to_string(ZENO_AMD_DELTA_MAX_DIM);
+    if (in.length > 0x7fffff00u || (uint64_t)in.batch * in.value_heads > 0x7fffffffull / 64) return "too many sequences or tokens";
+    if ((uint64_t)in.batch * in.length * in.key_heads > 0x7fffffffull) return "too many tokens";  // blocks of the sum over shared heads
+    return "";
+}
+
+std::string check(const ZenoAmdDeltaInputs* p, bool step) {
+    if (!p) return "null arguments";
+    const ZenoAmdDeltaInputs& in = *p;
+    const std::string why = check_sizes(in);
+    if (!why.empty()) return why;
+    if (step && in.length != 1) return "a step takes one token";
+    if (!in.q || !in.k || !in.v || !in.g || !in.beta) return "null input";
+    if (!std::isfinite(in.scale)) return "scale is not finite";
+    return "";
+}
+
+hipError_t forward(const ZenoAmdDeltaInputs& in, void* o, const int64_t* o_stride, float* last, float* saved, hipStream_t stream) {
+    Shape s = shape_of(in);
+    if (!saved) s.tiles = 2;
+    Args a = common(in, s);
+    a.o = o;
+    set_strides(a.o_stride, o_stride);
+    a.o_vec = vectors(o, o_stride, in.batch, in.length, in.value_heads, element_bytes(in.dtype));
+    a.last = last;
+    a.saved = saved;
+    return by_type(in.dtype, launch_forward<T_F32>, launch_forward<T_F16>, launch_forward<T_BF16>, a, s, stream);
+}
+
+hipError_t backward(const ZenoAmdDeltaInputs& in, const float* last, const float* saved, const ZenoAmdDeltaGradients& grad, float* workspace,
+                    hipStream_t stream) {
+    const Shape s = shape_of(in);
+    Args a = common(in, s);
+    const uint32_t eb = element_bytes(in.dtype);
+    a.last = const_cast<float*>(last);
+    a.saved = const_cast<float*>(saved);
+    a.d_o = grad.d_o;
+    set_strides(a.d_o_stride, grad.d_o_stride);
+    a.d_o_vec = vectors(grad.d_o, grad.d_o_stride, in.batch, in.length, in.value_heads, eb);
+    a.d_last = grad.d_last;
+    a.dq = grad.d_q;
+    a.dk = grad.d_k;
+    a.dv = grad.d_v;
+    set_strides(a.dq_stride, grad.d_q_stride);
+    set_strides(a.dk_stride, grad.d_k_stride);
+    set_strides(a.dv_stride, grad.d_v_stride);
+    a.dq_vec = vectors(grad.d_q, grad.d_q_stride, in.batch, in.length, in.key_heads, eb);
+    a.dk_vec = vectors(grad.d_k, grad.d_k_stride, in.batch, in.length, in.key_heads, eb);
+    a.dv_vec = vectors(grad.d_v, grad.d_v_stride, in.batch, in.length, in.value_heads, eb);
+    a.dg = grad.d_g;
+    a.dbeta = grad.d_beta;
+    set_strides(a.dg_stride, grad.d_g_stride);
+    set_strides(a.dbeta_stride, grad.d_beta_stride);
+    a.d_state = grad.d_state;
+    if (a.share > 1) {
+        a.part_q = workspace;
+        a.part_k = workspace + workspace_floats(in) / 2;
+    }
+    return by_type(in.dtype, launch_backward<T_F32>, launch_backward<T_F16>, launch_backward<T_BF16>, a, s, stream);
+}
+
+hipError_t step(const ZenoAmdDeltaInputs& in, void* o, const int64_t* o_stride, float* state, hipStream_t stream) {
+    Args a{};
+    a.in = in;
+    a.share = in.value_heads / in.key_heads;
+    a.o = o;
+    set_strides(a.o_stride, o_stride);
+    return in.dtype == T_F32   ? launch_step<T_F32>(a, state, stream)
+           : in.dtype == T_F16 ? launch_step<T_F16>(a, state, stream)
+                               : launch_step<T_BF16>(a, state, stream);
+}
+
+}  // namespace delta
+}  // namespace za

@@ -1,0 +1,10 @@
+// The gated delta rule's kernels for one element type.
+#include "delta_kernels.h"
+
+namespace za {
+namespace delta {
+template hipError_t launch_forward<T_BF16>(const Args&, const Shape&, hipStream_t);
+template hipError_t launch_backward<T_BF16>(const Args&, const Shape&, hipStream_t);
+template hipError_t launch_step<T_BF16>(const Args&, float*, hipStream_t);
+}  // namespace delta
+}  // namespace za

@@ -1,0 +1,203 @@
+"""The memory layer of policies that act on partial observations: the gated delta rule.
+
+Each environment (or recorded sequence) and head keeps a state S [key_dim, value_dim]. A token
+brings a query, a key, a value, the log of a decay and a strength, and
+
+    S <- exp(g) S                       (S <- 0 where an episode begins)
+    S <- S + k (beta (v - S^T k))^T
+    o  = scale S^T q
+
+``gated_delta_step`` advances every environment's state by one token in place, beside a step of
+the simulation; ``gated_delta`` runs whole sequences (rollouts, recorded episodes) and has
+gradients for every input. Both take torch tensors on the GPU and run on torch's current stream.
+
+Arguments, for B sequences (environments) of T tokens, Hk key heads and Hv value heads (a
+multiple of Hk; value head h reads key head h // (Hv // Hk)):
+
+    q, k       [B, T, Hk, key_dim]    float32, float16 or bfloat16
+    v          [B, T, Hv, value_dim]  the same type
+    g, beta    [B, T, Hv]             float32
+    reset      [B, T]                 bool or uint8, or None: this token begins an episode
+    state      [B, Hv, key_dim, value_dim] float32, or None for zeros
+
+without T for a step. Dimensions are 1 to 128. Any strides will do where the last dimension of
+q, k and v is contiguous, so views of one projection and time-major rollouts
+(``x.transpose(0, 1)``) need no copy. scale defaults to key_dim ** -0.5; with ``normalize``,
+queries and keys are divided by sqrt(sum of squares + 1e-6) first. All sums and states are 32-bit;
+a token with g < -104 (its decay is 0 in fp32) counts as a reset. What lies before a reset, NaN
+and infinity included, has no effect on what follows.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import Optional, Tuple
+
+import torch
+
+from . import _lib as L
+
+_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_S2, _S3 = C.c_int64 * 2, C.c_int64 * 3
+
+
+def _fail(rc: int, what: str) -> None:
+    if rc == -6:
+        raise ValueError(L.last_error())
+    raise RuntimeError(f"{what} failed: {rc}: {L.last_error()}")
+
+
+def _check(q, k, v, g, beta, reset, state, lead: int) -> None:
+    """Shapes, types and devices; `lead` is the number of dimensions before the heads."""
+    if q.dtype not in _DTYPES:
+        raise TypeError(f"q, k and v must be float32, float16 or bfloat16, not {q.dtype}")
+    if q.dim() != lead + 2 or v.dim() != lead + 2:
+        raise ValueError(f"q and v must have {lead + 2} dimensions, not {q.dim()} and {v.dim()}")
+    if k.shape != q.shape or v.shape[:lead] != q.shape[:lead] or g.shape != v.shape[:-1] or beta.shape != g.shape:
+        raise ValueError(f"shapes do not agree: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}, "
+                         f"g {tuple(g.shape)}, beta {tuple(beta.shape)}")
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError(f"q, k and v must have one type, not {q.dtype}, {k.dtype}, {v.dtype}")
+    if g.dtype != torch.float32 or beta.dtype != torch.float32:
+        raise TypeError(f"g and beta must be float32, not {g.dtype} and {beta.dtype}")
+    if not q.is_cuda:
+        raise ValueError("the operands must be on the GPU (there is no CPU fallback)")
+    others = [k, v, g, beta]
+    if reset is not None:
+        if reset.shape != q.shape[:lead]:
+            raise ValueError(f"reset must have the shape {tuple(q.shape[:lead])}, not {tuple(reset.shape)}")
+        if reset.dtype not in (torch.bool, torch.uint8):
+            raise TypeError(f"reset must be bool or uint8, not {reset.dtype}")
+        others.append(reset)
+    if state is not None:
+        want = (q.shape[0], v.shape[lead], q.shape[-1], v.shape[-1])
+        if state.shape != want:
+            raise ValueError(f"state must have the shape {want}, not {tuple(state.shape)}")
+        if state.dtype != torch.float32:
+            raise TypeError(f"state must be float32, not {state.dtype}")
+        others.append(state)
+    if any(x.device != q.device for x in others):
+        raise ValueError("the operands must be on one device")
+
+
+def _row(x: torch.Tensor) -> torch.Tensor:
+    return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
+
+
+def _inputs(q, k, v, g, beta, reset, state, scale, normalize) -> L.ZenoAmdDeltaInputs:
+    if q.dim() == 4:
+        b, t, hk, dk = q.shape
+        qs, ks, vs = q.stride()[:3], k.stride()[:3], v.stride()[:3]
+        gs, bs = g.stride(), beta.stride()
+        rs = (0, 0) if reset is None else reset.stride()
+    else:
+        (b, hk, dk), t = q.shape, 1
+        qs, ks, vs = ((x.stride(0), 0, x.stride(1)) for x in (q, k, v))
+        gs, bs = ((x.stride(0), 0, x.stride(1)) for x in (g, beta))
+        rs = (0, 0) if reset is None else (reset.stride(0), 0)
+    return L.ZenoAmdDeltaInputs(
+        _DTYPES[q.dtype], b, t, hk, v.shape[-2], dk, v.shape[-1], bool(normalize), scale,
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(),
+        None if reset is None else reset.data_ptr(), None if state is None else state.data_ptr(),
+        _S3(*qs), _S3(*ks), _S3(*vs), _S3(*gs), _S3(*bs), _S2(*rs))
+
+
+def _stream(x: torch.Tensor) -> int:
+    return torch.cuda.current_stream(x.device).cuda_stream
+
+
+class _GatedDelta(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, g, beta, reset, state, scale, normalize, train):
+        with torch.cuda.device(q.device):
+            lib = L.load()
+            a = _inputs(q, k, v, g, beta, reset, state, scale, normalize)
+            o = torch.empty_like(v)  # v's order of dimensions: time-major in, time-major out
+            if o.stride(-1) != 1 and o.shape[-1] != 1:
+                o = torch.empty(v.shape, dtype=v.dtype, device=v.device)
+            last = torch.empty((q.shape[0], v.shape[2], q.shape[3], v.shape[3]), dtype=torch.float32, device=q.device)
+            saved = None
+            if train:
+                n = lib.zeno_amd_delta_saved_bytes(a)
+                saved = torch.empty(max(n, 1), dtype=torch.uint8, device=q.device)
+            rc = lib.zeno_amd_delta_forward(a, o.data_ptr(), _S3(*o.stride()[:3]), last.data_ptr(),
+                                            None if saved is None else saved.data_ptr(), _stream(q))
+            if rc:
+                _fail(rc, "gated_delta")
+        if train:
+            ctx.save_for_backward(q, k, v, g, beta, reset, state, last, saved)
+            ctx.scale, ctx.normalize = scale, normalize
+            ctx.set_materialize_grads(False)
+        return o, last
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_o, d_last):
+        q, k, v, g, beta, reset, state, last, saved = ctx.saved_tensors
+        if d_o is None and d_last is None:
+            return (None,) * 10
+        with torch.cuda.device(q.device):
+            lib = L.load()
+            a = _inputs(q, k, v, g, beta, reset, state, ctx.scale, ctx.normalize)
+            d_o = torch.zeros_like(v) if d_o is None else _row(d_o)
+            d_last = None if d_last is None else d_last.contiguous()
+            d_q, d_k, d_v = (_dense_like(x) for x in (q, k, v))
+            d_g, d_beta = _dense_like(g), _dense_like(beta)
+            d_state = torch.empty_like(state) if state is not None and ctx.needs_input_grad[6] else None
+            n = lib.zeno_amd_delta_workspace_bytes(a)
+            space = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
+            grads = L.ZenoAmdDeltaGradients(
+                d_o.data_ptr(), _S3(*d_o.stride()[:3]), None if d_last is None else d_last.data_ptr(),
+                d_q.data_ptr(), d_k.data_ptr(), d_v.data_ptr(), d_g.data_ptr(), d_beta.data_ptr(),
+                None if d_state is None else d_state.data_ptr(),
+                *(_S3(*x.stride()[:3]) for x in (d_q, d_k, d_v, d_g, d_beta)))
+            rc = lib.zeno_amd_delta_backward(a, last.data_ptr(), saved.data_ptr(), grads, None if space is None else space.data_ptr(),
+                                             _stream(q))
+            if rc:
+                _fail(rc, "gated_delta's gradients")
+        return d_q, d_k, d_v, d_g, d_beta, None, d_state, None, None, None
+
+
+def _dense_like(x: torch.Tensor) -> torch.Tensor:
+    """Memory for x's gradient in x's order of dimensions, each value at a place of its own."""
+    y = torch.empty_like(x)
+    return y if y.stride(-1) == 1 or x.shape[-1] == 1 or x.dim() == 3 else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+
+
+def gated_delta(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, beta: torch.Tensor,
+                reset: Optional[torch.Tensor] = None, state: Optional[torch.Tensor] = None, *,
+                scale: Optional[float] = None, normalize: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The rule over whole sequences. Returns o [B, T, Hv, value_dim] in the type of v and the
+    state after the last token, a new tensor. Differentiable in q, k, v, g, beta and state."""
+    _check(q, k, v, g, beta, reset, state, 2)
+    if min(q.shape) < 1 or min(v.shape) < 1:
+        raise ValueError(f"empty operands: q {tuple(q.shape)}, v {tuple(v.shape)}")
+    scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
+    q, k, v = _row(q), _row(k), _row(v)
+    state = None if state is None else state.contiguous()
+    train = torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in (q, k, v, g, beta, state))
+    return _GatedDelta.apply(q, k, v, g, beta, reset, state, scale, bool(normalize), train)
+
+
+@torch.no_grad()
+def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, beta: torch.Tensor,
+                     state: torch.Tensor, reset: Optional[torch.Tensor] = None, *, scale: Optional[float] = None,
+                     normalize: bool = False, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """One token for every sequence: q, k [B, Hk, key_dim], v [B, Hv, value_dim], g, beta
+    [B, Hv], reset [B]. `state` (contiguous) is advanced in place; returns o [B, Hv, value_dim]
+    (`out` if given). Without gradients: training runs gated_delta on the recorded rollout."""
+    _check(q, k, v, g, beta, reset, state, 1)
+    if min(q.shape) < 1 or min(v.shape) < 1:
+        raise ValueError(f"empty operands: q {tuple(q.shape)}, v {tuple(v.shape)}")
+    if not state.is_contiguous():
+        raise ValueError("state must be contiguous: it is advanced in place")
+    q, k, v = _row(q), _row(k), _row(v)
+    if out is None:
+        out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
+    elif out.shape != v.shape or out.dtype != v.dtype or out.device != v.device or (out.stride(-1) != 1 and out.shape[-1] != 1):
+        raise ValueError(f"out must be like v: {tuple(v.shape)}, {v.dtype}, on {v.device}, its last dimension contiguous")
+    with torch.cuda.device(q.device):
+        a = _inputs(q, k, v, g, beta, reset, state, q.shape[-1] ** -0.5 if scale is None else float(scale), normalize)
+        rc = L.load().zeno_amd_delta_step(a, out.data_ptr(), _S3(out.stride(0), 0, out.stride(1)), state.data_ptr(), _stream(q))
+        if rc:
+            _fail(rc, "gated_delta_step")
+    return out
