@@ -297,6 +297,31 @@ uint64_t zeno_amd_delta_workspace_bytes(const ZenoAmdDeltaInputs* in);
  * read). What runs beside a step of the simulation. */
 int zeno_amd_delta_step(const ZenoAmdDeltaInputs* in, void* o, const int64_t* o_stride, float* state, void* stream);
 
+/* An orthogonalised update: `count` matrices of one shape (a momentum, say), each divided by
+ * its Frobenius norm plus eps and then, `steps` times, with rows <= cols (else transposed),
+ *     A = X X^T,   X <- a X + (b A + c A A) X,
+ * which drives all its singular values towards 1. Products are summed in fp32 (the norm in
+ * fp64); for float32 and float16 their operands carry 22 bits, for bfloat16 11. Coefficients
+ * that let a singular value of X, or an entry of the products, exceed 32 are refused: the
+ * operands are 16-bit numbers at a fixed scale. Strides are in elements (matrix, row, column)
+ * and may be anything; out must not overlap x unless it is the same memory with the same
+ * strides. */
+typedef struct {
+    uint32_t dtype;               /* of x and out, as above */
+    uint32_t count, rows, cols;   /* at most 65535 matrices of 65536 x 65536 */
+    uint32_t steps;               /* 1 to 100 */
+    float a, b, c;                /* 3.4445, -4.7750, 2.0315 is usual, with 5 steps */
+    float eps;
+    const void* x;
+    int64_t x_stride[3];
+    void* out;
+    int64_t out_stride[3];
+} ZenoAmdOrthogonalize;
+
+uint64_t zeno_amd_orthogonalize_workspace_bytes(const ZenoAmdOrthogonalize* args); /* 0 for refused arguments */
+/* `workspace`: that many bytes, aligned to 256. Returns after enqueueing on `stream`. */
+int zeno_amd_orthogonalize(const ZenoAmdOrthogonalize* args, void* workspace, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

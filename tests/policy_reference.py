@@ -46,3 +46,17 @@ def assert_near(got, want, tol, what=""):
     assert torch.equal(fine, torch.isfinite(got)), f"{what}: finite values in other places"
     err, norm = float((got - want)[fine].norm()), float(want[fine].norm())
     assert err <= tol * norm + 1e-30, f"{what}: off by {err / max(norm, 1e-300):.3g} of its norm, {tol:.3g} allowed"
+
+
+def orthogonalize(x, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7):
+    """Newton-Schulz in float64, matrix by matrix, from the definition."""
+    a, b, c = coefficients
+    out = torch.empty(x.shape, dtype=torch.float64)
+    for i, g in enumerate(x.double().reshape(-1, *x.shape[-2:])):
+        y = g.T if g.shape[0] > g.shape[1] else g
+        y = y / (torch.linalg.norm(y) + eps)
+        for _ in range(steps):
+            s = y @ y.T
+            y = a * y + (b * s + c * s @ s) @ y
+        out.view(-1, *x.shape[-2:])[i] = y.T if g.shape[0] > g.shape[1] else y
+    return out

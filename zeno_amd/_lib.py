@@ -110,6 +110,16 @@ class ZenoAmdDeltaGradients(C.Structure):
     ]
 
 
+class ZenoAmdOrthogonalize(C.Structure):
+    """include/zeno_amd_ext.h"""
+
+    _fields_ = [
+        ("dtype", C.c_uint32), ("count", C.c_uint32), ("rows", C.c_uint32), ("cols", C.c_uint32), ("steps", C.c_uint32),
+        ("a", C.c_float), ("b", C.c_float), ("c", C.c_float), ("eps", C.c_float),
+        ("x", C.c_void_p), ("x_stride", C.c_int64 * 3), ("out", C.c_void_p), ("out_stride", C.c_int64 * 3),
+    ]
+
+
 _vp = C.c_void_p
 _fp = C.POINTER(C.c_float)
 _u8p = C.POINTER(C.c_uint8)
@@ -208,6 +218,8 @@ SIGNATURES = {
     "zeno_amd_delta_saved_bytes": (C.c_uint64, [_delta]),
     "zeno_amd_delta_workspace_bytes": (C.c_uint64, [_delta]),
     "zeno_amd_delta_step": (C.c_int, [_delta, _vp, _i64p, _vp, _vp]),
+    "zeno_amd_orthogonalize_workspace_bytes": (C.c_uint64, [C.POINTER(ZenoAmdOrthogonalize)]),
+    "zeno_amd_orthogonalize": (C.c_int, [C.POINTER(ZenoAmdOrthogonalize), _vp, _vp]),
     "zeno_amd_world_waves_per_group": (C.c_uint32, [C.c_void_p]),
     "zeno_amd_world_split_groups": (C.c_int, [C.c_void_p]),
 }

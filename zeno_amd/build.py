@@ -39,7 +39,7 @@ HIP_FLAGS = [
 STEP_FLAGS = ["-Rpass-analysis=kernel-resource-usage", "-mllvm", "-align-all-nofallthru-blocks=6"]
 # The operators of policies are compared with tolerances, not bit for bit: products and sums may
 # contract. No packed fp32 instructions here either.
-POLICY_SOURCES = ("delta.hip", "delta_f32.hip", "delta_f16.hip", "delta_bf16.hip")
+POLICY_SOURCES = ("delta.hip", "delta_f32.hip", "delta_f16.hip", "delta_bf16.hip", "orth.hip")
 POLICY_FLAGS = [
     f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-fno-fast-math",
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",

@@ -11,6 +11,7 @@
 #include "../../include/zeno_amd_ext.h"
 #include "collide.h"
 #include "delta.h"
+#include "orth.h"
 #include "world.h"
 
 using za::World;
@@ -580,6 +581,20 @@ int zeno_amd_delta_step(const ZenoAmdDeltaInputs* in, void* o, const int64_t* o_
     if (!why.empty()) return delta_refused("delta_step", why);
     if (!o || !o_stride || !state) return delta_refused("delta_step", "null output or state");
     return hip_status(za::delta::step(*in, o, o_stride, state, (hipStream_t)stream), "delta_step");
+}
+
+uint64_t zeno_amd_orthogonalize_workspace_bytes(const ZenoAmdOrthogonalize* args) {
+    return za::orth::check(args).empty() ? za::orth::workspace_bytes(*args) : 0;
+}
+
+int zeno_amd_orthogonalize(const ZenoAmdOrthogonalize* args, void* workspace, void* stream) {
+    std::string why = za::orth::check(args);
+    if (why.empty() && (!workspace || (uintptr_t)workspace % 256)) why = "workspace is null or not aligned to 256 bytes";
+    if (!why.empty()) {
+        set_error("orthogonalize: " + why);
+        return ZENO_INVALID_ARGUMENT;
+    }
+    return hip_status(za::orth::run(*args, workspace, (hipStream_t)stream), "orthogonalize");
 }
 
 }  // extern "C"

@@ -1,0 +1,443 @@
+// Newton-Schulz orthogonalisation: X = G / (|G| + eps), then `steps` times
+//     A = X X^T,  B = b A + c A A,  X <- a X + B X          (rows <= columns, else G^T)
+// which drives every singular value towards 1.
+//
+// Everything is a matrix product, (m m n + m m m + 2 m m n) operations a step with the symmetric
+// ones done by half, on the fp16 matrix units. Their operands are bounded: no singular value of X
+// exceeds about 1.2 (the host checks the coefficients), so X, A and B are held in fp16 at fixed
+// scales far from either end of its range. X itself stays in fp32 and is what a X adds: a small
+// singular value grows 3.4-fold a step by that term, and with it every rounding of X that the
+// term would carry (results 4.8e-3 off instead of 5e-4 with fp16 there). Operands of two parts
+// carry 22 bits, three of the four part products give fp32's accuracy at a third of the units'
+// rate, five times the fp32 units'. Results of bfloat16, which carry 8 bits, are content with one
+// part of 11 where the roundings average out over enough terms: a smaller dimension of 256 moves
+// them by 2e-4 to 1.6e-3 of their norm (momenta with strong directions to Gaussian matrices; their
+// own rounding is 1.7e-3), 37 by 2.8e-3. Sums are fp32, the norm's fp64.
+//
+// Layout. X and X^T are both kept as operands (every product then reads two operands along their
+// rows); rows and columns are padded with zeros to the tile. Two parts alternate every 32 columns,
+// so a row's 128 bytes are 64 columns of one part or 32 of two, and both run through the same loop.
+#include <cmath>
+#include <utility>
+
+#include "mma.h"
+#include "orth.h"
+
+namespace za {
+namespace orth {
+namespace {
+
+using namespace mma;
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+
+constexpr float kScale = 1024.0f;   // of X, A and B in fp16
+constexpr float kLargest = 32.0f;   // entries that the scale leaves room for, twice over
+constexpr int kNormBlocks = 64;
+
+struct Args {
+    ZenoAmdOrthogonalize in;
+    int m, n;             // of X
+    int mp, np;           // padded
+    bool flip;            // X = G^T
+    double* partial;      // [count][kNormBlocks]
+    float* master;        // X^T in fp32, each value read and written by one thread
+    float* sums;          // of the slices of a product
+    int slices;
+    bool out_vec;         // four values along out's dense dimension are aligned
+    _Float16 *x, *xt, *gram, *poly;  // [count][...]
+    _Float16* xt2;        // the next X^T (X is no operand of the product that makes the next one)
+};
+
+template <int P> __device__ __forceinline__ int64_t place(int64_t row, int col, int ld) {
+    return row * ld * P + (P == 1 ? col : (col >> 5) * 64 + (col & 31));
+}
+template <int P> __device__ __forceinline__ void put(_Float16* at, float x) {
+    const _Float16 h = (_Float16)x;
+    at[0] = h;
+    if (P == 2) at[32] = (_Float16)(x - (float)h);
+}
+
+template <int TY> __device__ __forceinline__ float input(const Args& a, int64_t k, int row, int col) {  // of G
+    typedef typename Elem<TY>::type E;
+    return Elem<TY>::get(((const E*)a.in.x)[k * a.in.x_stride[0] + row * a.in.x_stride[1] + col * a.in.x_stride[2]]);
+}
+
+// Sums of squares, a grid-stride share of the matrix a block, along whichever dimension is dense.
+template <int TY> __global__ __launch_bounds__(256) void norm_kernel(const Args a) {
+    __shared__ double part[4];
+    const int64_t k = blockIdx.y;
+    const bool by_col = a.in.x_stride[2] <= a.in.x_stride[1];
+    const int inner = by_col ? a.in.cols : a.in.rows;
+    const int64_t all = (int64_t)a.in.rows * a.in.cols;
+    double sum = 0.0;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
+        const int u = (int)(i / inner), w = (int)(i % inner);
+        const double v = by_col ? input<TY>(a, k, u, w) : input<TY>(a, k, w, u);
+        sum += v * v;
+    }
+#pragma unroll
+    for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) a.partial[k * kNormBlocks + blockIdx.x] = part[0] + part[1] + part[2] + part[3];
+}
+
+// X and X^T in fp16 from G, a 64x64 tile a block.
+template <int TY, int P> __global__ __launch_bounds__(256) void load_kernel(const Args a) {
+    __shared__ float tile[64][65];
+    const int64_t k = blockIdx.z;
+    const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;  // of X
+    double s = a.partial[k * kNormBlocks + (threadIdx.x & (kNormBlocks - 1))];
+#pragma unroll
+    for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d);
+    const float f = (float)((double)kScale / (sqrt(s) + (double)a.in.eps));
+    const bool dense_cols = a.flip ? a.in.x_stride[1] <= a.in.x_stride[2] : a.in.x_stride[2] <= a.in.x_stride[1];
+    const int w = threadIdx.x & 63, u = threadIdx.x >> 6;
+#pragma unroll
+    for (int i = u; i < 64; i += 4) {
+        const int r = dense_cols ? i : w, c = dense_cols ? w : i;
+        float v = 0.0f;
+        if (r0 + r < a.m && c0 + c < a.n) v = a.flip ? input<TY>(a, k, c0 + c, r0 + r) : input<TY>(a, k, r0 + r, c0 + c);
+        tile[r][c] = v * f;
+    }
+    __syncthreads();
+    _Float16* x = a.x + k * a.mp * a.np * P;
+    _Float16* xt = a.xt + k * a.mp * a.np * P;
+#pragma unroll
+    for (int i = u; i < 64; i += 4) {
+        a.master[(k * a.np + c0 + i) * a.mp + r0 + w] = tile[w][i];
+        put<P>(x + place<P>(r0 + i, c0 + w, a.np), tile[i][w]);
+        put<P>(xt + place<P>(c0 + i, r0 + w, a.mp), tile[w][i]);
+    }
+}
+
+// Four values of a row-major operand row that start at a multiple of four.
+template <int P> __device__ __forceinline__ void put4(_Float16* at, f4 x) {
+    h4 h;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) h[r] = (_Float16)x[r];
+    *reinterpret_cast<h4*>(at) = h;
+    if constexpr (P == 2) {
+        h4 l;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) l[r] = (_Float16)(x[r] - (float)h[r]);
+        *reinterpret_cast<h4*>(at + 32) = l;
+    }
+}
+template <int P> __device__ __forceinline__ f4 get4(const _Float16* at) {
+    const h4 h = *reinterpret_cast<const h4*>(at);
+    f4 x = {(float)h[0], (float)h[1], (float)h[2], (float)h[3]};
+    if constexpr (P == 2) {
+        const h4 l = *reinterpret_cast<const h4*>(at + 32);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[r] += (float)l[r];
+    }
+    return x;
+}
+
+template <int CTRL> __device__ __forceinline__ float quad(float x) {  // from another lane of four
+    return __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(x), CTRL, 0xf, 0xf, true));
+}
+// Transposes 4x4 values across four lanes: register r of lane q becomes register q of lane r. Of a
+// result tile, lane n then holds row 4 g + n % 4, columns 4 (n / 4) + 0..3.
+__device__ __forceinline__ f4 turn(f4 x, int lane) {
+    const bool a = lane & 1, b = lane & 2;
+    const float s0 = quad<0xb1>(a ? x[0] : x[1]), s1 = quad<0xb1>(a ? x[2] : x[3]);  // lanes 1 0 3 2
+    f4 y = a ? f4{s0, x[1], s1, x[3]} : f4{x[0], s0, x[2], s1};
+    const float t0 = quad<0x4e>(b ? y[0] : y[2]), t1 = quad<0x4e>(b ? y[1] : y[3]);  // lanes 2 3 0 1
+    return b ? f4{t0, t1, y[2], y[3]} : f4{y[0], y[1], t0, t1};
+}
+
+enum Kind { GRAM, POLY, NEXT, LAST };
+enum Share { WHOLE, SLICE, JOIN };  // of the contraction: all of it; a slice, sums kept; the sum of the slices
+
+// C = L R^T of rows along the contraction, and what follows from it. A block computes BM x BN; its
+// WR x WC waves hold their part in registers. 128 bytes of every row of both operands are in LDS
+// at a time, twice (the next ones arrive while these are multiplied), written by the loads
+// themselves; their 16-byte pieces are permuted by half the row number, which leaves the operand
+// reads without bank conflicts. Few tiles with a long contraction are cut into slices along it
+// (SLICE), whose sums another launch adds in their order (JOIN).
+template <int TY, int P, int BM, int BN, int WR, int WC, int KIND, int SHARE>
+__global__ __launch_bounds__(64 * WR * WC) void product_kernel(const Args a) {
+    constexpr int threads = 64 * WR * WC, waves = WR * WC;
+    constexpr int TM = BM / WR / 16, TN = BN / WC / 16;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
+    const int64_t k = blockIdx.y;
+    constexpr bool half = KIND == GRAM || KIND == POLY;  // symmetric: tiles on and below the diagonal
+    int ti, tj;
+    {
+        // Consecutive blocks go to the eight dies in turn: each die gets a run of tiles, whose operands its L2 shares.
+        const int all = gridDim.x, per = all / 8, rest = all % 8, die = blockIdx.x % 8;
+        const int id = die * per + min(die, rest) + blockIdx.x / 8;
+        if (half) {
+            ti = (int)((sqrtf(8.0f * id + 1.0f) - 1.0f) * 0.5f);
+            while ((ti + 1) * (ti + 2) / 2 <= id) ++ti;
+            while (ti * (ti + 1) / 2 > id) --ti;
+            tj = id - ti * (ti + 1) / 2;
+        } else {
+            const int cols = a.np / BN;
+            ti = id / cols;
+            tj = id % cols;
+        }
+    }
+    f4 acc[TM][TN];
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) acc[i][j] = f4{0, 0, 0, 0};
+    // The sums of slice s of this tile: [matrix][slice][tile][value][thread].
+    auto sums = [&](int s) { return (f4*)a.sums + (((k * a.slices + s) * gridDim.x + blockIdx.x) * (TM * TN)) * threads + threadIdx.x; };
+
+    if constexpr (SHARE == JOIN) {
+        for (int s = 0; s < a.slices; ++s) {
+            const f4* from = sums(s);
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < TN; ++j) acc[i][j] += from[(i * TN + j) * threads];
+        }
+    } else {
+        __shared__ __attribute__((aligned(128))) char lds[2][(BM + BN) * 128];
+        const int ld = KIND == GRAM ? a.np : a.mp;  // of the contraction
+        const _Float16* left = (KIND == GRAM ? a.x + k * a.mp * a.np * P : KIND == POLY ? a.gram + k * a.mp * a.mp * P : a.poly + k * a.mp * a.mp * P);
+        const _Float16* right = KIND == NEXT || KIND == LAST ? a.xt + k * a.mp * a.np * P : left;
+        left += (int64_t)ti * BM * ld * P;
+        right += (int64_t)tj * BN * ld * P;
+        int b0 = 0, blocks = ld * P / 64;
+        if constexpr (SHARE == SLICE) {
+            const int s = blockIdx.z, all = blocks;
+            b0 = (int)((int64_t)all * s / a.slices);
+            blocks = (int)((int64_t)all * (s + 1) / a.slices);
+        }
+        auto fetch = [&](int block, int buf) {
+#pragma unroll
+            for (int i = wave; i < (BM + BN) / 8; i += waves) {  // eight rows of 128 bytes an instruction
+                const int row = 8 * i + (lane >> 3), piece = (lane & 7) ^ ((row >> 1) & 7);
+                const _Float16* from = (row < BM ? left + (int64_t)row * ld * P : right + (int64_t)(row - BM) * ld * P) + 64 * (int64_t)block + 8 * piece;
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
+                                                 (__attribute__((address_space(3))) void*)(lds[buf] + 1024 * i), 16, 0, 0);
+            }
+        };
+        const int row_l = (wave / WC) * (BM / WR) + n, row_r = BM + (wave % WC) * (BN / WC) + n;
+        fetch(b0, b0 & 1);
+        __syncthreads();
+        for (int b = b0; b < blocks; ++b) {
+            if (b + 1 < blocks) fetch(b + 1, (b + 1) & 1);
+            const char* at = lds[b & 1];
+            auto piece = [&](int row, int c) { return *reinterpret_cast<const h8*>(at + row * 128 + ((c ^ ((row >> 1) & 7)) << 4)); };
+#pragma unroll
+            for (int s = 0; s < (P == 1 ? 2 : 1); ++s) {
+                h8 l[P][TM], r[P][TN];
+#pragma unroll
+                for (int p = 0; p < P; ++p) {
+                    const int c = 4 * (P == 1 ? s : p) + g;
+#pragma unroll
+                    for (int i = 0; i < TM; ++i) l[p][i] = piece(row_l + 16 * i, c);
+#pragma unroll
+                    for (int j = 0; j < TN; ++j) r[p][j] = piece(row_r + 16 * j, c);
+                }
+#pragma unroll
+                for (int i = 0; i < TM; ++i)
+#pragma unroll
+                    for (int j = 0; j < TN; ++j) {
+                        if constexpr (P == 2) {
+                            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(l[1][i], r[0][j], acc[i][j], 0, 0, 0);
+                            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(l[0][i], r[1][j], acc[i][j], 0, 0, 0);
+                        }
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(l[0][i], r[0][j], acc[i][j], 0, 0, 0);
+                    }
+            }
+            __syncthreads();
+        }
+    }
+
+    if constexpr (SHARE == SLICE) {
+        f4* to = sums(blockIdx.z);
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j) to[(i * TN + j) * threads] = acc[i][j];
+        return;
+    }
+    // Products of two numbers at kScale: once too much.
+    const float down = 1.0f / kScale;
+    const int q = n & 3, qc = n & 12;
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+            const int row0 = ti * BM + (wave / WC) * (BM / WR) + 16 * i + 4 * g, col0 = tj * BN + (wave % WC) * (BN / WC) + 16 * j;
+            f4 v = acc[i][j] * down;
+            if constexpr (half) {
+                _Float16* to = (KIND == GRAM ? a.gram : a.poly) + k * a.mp * a.mp * P;
+                if constexpr (KIND == POLY) v = a.in.b * get4<P>(a.gram + k * a.mp * a.mp * P + place<P>(col0 + n, row0, a.mp)) + a.in.c * v;
+                put4<P>(to + place<P>(col0 + n, row0, a.mp), v);  // the mirrored tile (of a diagonal tile, the same)
+                if (ti != tj) put4<P>(to + place<P>(row0 + q, col0 + qc, a.mp), turn(v, lane));
+            } else {
+                f4* x = reinterpret_cast<f4*>(a.master + (k * a.np + col0 + n) * a.mp + row0);
+                v += a.in.a * *x;
+                if constexpr (KIND == NEXT) {
+                    *x = v;
+                    put4<P>(a.xt2 + k * a.mp * a.np * P + place<P>(col0 + n, row0, a.mp), v);
+                    put4<P>(a.x + k * a.mp * a.np * P + place<P>(row0 + q, col0 + qc, a.np), turn(v, lane));
+                } else {
+                    typedef typename Elem<TY>::type E;
+                    // Four consecutive values along the dimension of out that is dense.
+                    const bool along_rows = a.flip ? a.in.out_stride[2] == 1 : a.in.out_stride[1] == 1;
+                    const f4 w = (along_rows ? v : turn(v, lane)) * down;
+                    const int row = along_rows ? row0 : row0 + q, col = along_rows ? col0 + n : col0 + qc;
+                    const int64_t sr = a.in.out_stride[a.flip ? 2 : 1], sc = a.in.out_stride[a.flip ? 1 : 2];
+                    E* to = (E*)a.in.out + k * a.in.out_stride[0] + row * sr + col * sc;
+                    const int64_t step = along_rows ? sr : sc;
+                    const int left = along_rows ? (col < a.n ? a.m - row : 0) : (row < a.m ? a.n - col : 0);
+                    if (a.out_vec && left >= 4) {
+                        if constexpr (TY == T_F32) *reinterpret_cast<f4*>(to) = w;
+                        else {
+                            u2 e;
+#pragma unroll
+                            for (int r = 0; r < 2; ++r)
+                                e[r] = (uint32_t)__builtin_bit_cast(uint16_t, Elem<TY>::put(w[2 * r])) |
+                                       (uint32_t)__builtin_bit_cast(uint16_t, Elem<TY>::put(w[2 * r + 1])) << 16;
+                            *reinterpret_cast<u2*>(to) = e;
+                        }
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (r < left) to[r * step] = Elem<TY>::put(w[r]);
+                    }
+                }
+            }
+        }
+}
+
+struct Plan {
+    int m, n, mp, np, parts;
+    int slices;  // of X X^T
+    uint64_t norm, master, x, square, sums;  // bytes: partial norms, X in fp32, X as an operand, m x m as an operand, slices' sums
+};
+
+// Tiles of 64, 128 or (one part) 256 squared: the largest that still makes a block for every CU.
+int tile_of(const Plan& p, uint32_t count, bool half) {
+    auto tiles = [&](int t) {
+        const int64_t r = p.mp / t, c = p.np / t;
+        return (half ? r * (r + 1) / 2 : r * c) * count;
+    };
+    if (p.parts == 1 && p.mp % 256 == 0 && p.np % 256 == 0 && tiles(256) >= 256) return 256;
+    return tiles(128) > 256 ? 128 : 64;
+}
+
+Plan plan_of(const ZenoAmdOrthogonalize& a) {
+    Plan p;
+    p.m = (int)(a.rows < a.cols ? a.rows : a.cols);
+    p.n = (int)(a.rows < a.cols ? a.cols : a.rows);
+    p.parts = a.dtype == T_BF16 && p.m >= 256 ? 1 : 2;
+    const int pad = p.m <= 512 ? 64 : 128;
+    p.mp = (p.m + pad - 1) / pad * pad;
+    p.np = (p.n + pad - 1) / pad * pad;
+    p.norm = (uint64_t)a.count * kNormBlocks * sizeof(double);
+    p.master = (uint64_t)a.count * p.mp * p.np * 4;
+    p.x = (uint64_t)a.count * p.mp * p.np * p.parts * 2;
+    p.square = (uint64_t)a.count * p.mp * p.mp * p.parts * 2;
+    const int t = tile_of(p, a.count, true);
+    const uint64_t r = p.mp / t, tiles = r * (r + 1) / 2 * a.count, blocks = (uint64_t)p.np * p.parts / 64;
+    // Two blocks a CU, at least eight steps of the contraction each.
+    p.slices = 1;
+    while (p.slices < 16 && tiles * p.slices * 2 <= 512 && blocks / (p.slices * 2) >= 8) p.slices *= 2;
+    p.sums = p.slices > 1 ? tiles * p.slices * t * t * 4 : 0;
+    return p;
+}
+
+template <int TY, int P, int KIND, int SHARE> void product(const Args& a, int tile, int slices, hipStream_t stream) {
+    const int rows = a.mp / tile, cols = a.np / tile;
+    const dim3 grid(KIND == GRAM || KIND == POLY ? rows * (rows + 1) / 2 : rows * cols, a.in.count, slices);
+    if (tile == 64) product_kernel<TY, P, 64, 64, 2, 2, KIND, SHARE><<<grid, 256, 0, stream>>>(a);
+    else if (tile == 128) product_kernel<TY, P, 128, 128, 2, 2, KIND, SHARE><<<grid, 256, 0, stream>>>(a);
+    else if constexpr (P == 1 && SHARE == WHOLE) product_kernel<TY, P, 256, 256, 2, 4, KIND, SHARE><<<grid, 512, 0, stream>>>(a);
+}
+
+template <int TY, int P> hipError_t launch(Args a, const Plan& p, hipStream_t stream) {
+    const int square = tile_of(p, a.in.count, true), whole = tile_of(p, a.in.count, false);
+    norm_kernel<TY><<<dim3(kNormBlocks, a.in.count), 256, 0, stream>>>(a);
+    load_kernel<TY, P><<<dim3(a.np / 64, a.mp / 64, a.in.count), 256, 0, stream>>>(a);
+    for (uint32_t s = 0; s < a.in.steps; ++s) {
+        if (p.slices == 1) {
+            product<TY, P, GRAM, WHOLE>(a, square, 1, stream);
+        } else {
+            product<TY, P, GRAM, SLICE>(a, square, p.slices, stream);
+            product<TY, P, GRAM, JOIN>(a, square, 1, stream);
+        }
+        product<TY, P, POLY, WHOLE>(a, square, 1, stream);
+        if (s + 1 < a.in.steps) product<TY, P, NEXT, WHOLE>(a, whole, 1, stream);
+        else product<TY, P, LAST, WHOLE>(a, whole, 1, stream);
+        std::swap(a.xt, a.xt2);
+    }
+    return hipGetLastError();
+}
+
+}  // namespace
+
+std::string check(const ZenoAmdOrthogonalize* p) {
+    if (!p) return "null arguments";
+    const ZenoAmdOrthogonalize& a = *p;
+    if (a.dtype > T_BF16) return "dtype is none of float32, float16, bfloat16";
+    if (!a.count || !a.rows || !a.cols) return "count, rows and cols must be positive";
+    if (a.count > 65535) return "more than 65535 matrices";
+    if (a.rows > 65536 || a.cols > 65536) return "more than 65536 rows or columns";
+    if (!a.steps || a.steps > 100) return "steps must be 1 to 100";
+    if (!(a.eps > 0.0f) || !std::isfinite(a.eps)) return "eps must be positive";
+    if (!std::isfinite(a.a) || !std::isfinite(a.b) || !std::isfinite(a.c)) return "coefficients must be finite";
+    if (!a.x || !a.out) return "null matrix";
+    // What the coefficients make of singular values up to 1, on a grid of them.
+    double top = 1.0;
+    for (uint32_t s = 0; s < a.steps; ++s) {
+        double next = 0.0, poly = 0.0;
+        for (int i = 0; i <= 2048; ++i) {
+            const double v = top * i / 2048, w = v * v, f = a.b * w + a.c * w * w;
+            poly = std::fmax(poly, std::fabs(f));
+            next = std::fmax(next, std::fabs(v * (a.a + f)));
+        }
+        if (top * top > kLargest || poly > kLargest || next > kLargest) return "coefficients let singular values grow out of the range of 16-bit operands";
+        top = next;
+    }
+    return "";
+}
+
+uint64_t workspace_bytes(const ZenoAmdOrthogonalize& a) {
+    const Plan p = plan_of(a);
+    return p.norm + p.master + 3 * p.x + 2 * p.square + p.sums;
+}
+
+hipError_t run(const ZenoAmdOrthogonalize& in, void* workspace, hipStream_t stream) {
+    const Plan p = plan_of(in);
+    Args a{};
+    a.in = in;
+    a.m = p.m;
+    a.n = p.n;
+    a.mp = p.mp;
+    a.np = p.np;
+    a.flip = in.rows > in.cols;
+    char* at = (char*)workspace;
+    a.partial = (double*)at;
+    at += p.norm;
+    a.master = (float*)at;
+    at += p.master;
+    a.x = (_Float16*)at;
+    a.xt = (_Float16*)(at + p.x);
+    a.xt2 = (_Float16*)(at + 2 * p.x);
+    a.gram = (_Float16*)(at + 3 * p.x);
+    a.poly = (_Float16*)(at + 3 * p.x + p.square);
+    a.sums = (float*)(at + 3 * p.x + 2 * p.square);
+    a.slices = p.slices;
+    const uint64_t four = in.dtype == T_F32 ? 16 : 8;
+    const int64_t* s = in.out_stride;
+    const int other = (a.flip ? s[2] : s[1]) == 1 ? (a.flip ? 1 : 2) : (a.flip ? 2 : 1);  // the dimension that the stores do not run along
+    a.out_vec = s[3 - other] == 1 && (uintptr_t)in.out % four == 0 && s[other] % 4 == 0 && (in.count == 1 || s[0] % 4 == 0);
+    return in.dtype == T_F32   ? launch<T_F32, 2>(a, p, stream)
+           : in.dtype == T_F16 ? launch<T_F16, 2>(a, p, stream)
+           : p.parts == 2      ? launch<T_BF16, 2>(a, p, stream)
+                               : launch<T_BF16, 1>(a, p, stream);
+}
+
+}  // namespace orth
+}  // namespace za
