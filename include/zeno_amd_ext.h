@@ -280,8 +280,11 @@ typedef struct {
 /* Whole sequences. o [batch, length, value_heads, value_dim] by o_stride; last [batch,
  * value_heads, key_dim, value_dim], contiguous, the state after the last token (it may not be
  * `in->state`). `saved`: null, or zeno_amd_delta_saved_bytes(in) bytes that the gradients of
- * this call read. */
-int zeno_amd_delta_forward(const ZenoAmdDeltaInputs* in, void* o, const int64_t* o_stride, float* last, void* saved, void* stream);
+ * this call read. `workspace`: zeno_amd_delta_workspace_bytes(in) bytes (null where that is
+ * 0). Both aligned to 16 bytes. A long sequence with few heads is cut into segments that run
+ * side by side. */
+int zeno_amd_delta_forward(const ZenoAmdDeltaInputs* in, void* o, const int64_t* o_stride, float* last, void* saved, void* workspace,
+                           void* stream);
 
 /* Gradients of a zeno_amd_delta_forward call with the same inputs, whose `last` and `saved`
  * it left. `workspace`: zeno_amd_delta_workspace_bytes(in) bytes (null where that is 0).
@@ -291,7 +294,7 @@ int zeno_amd_delta_backward(const ZenoAmdDeltaInputs* in, const float* last, con
                             void* workspace, void* stream);
 
 uint64_t zeno_amd_delta_saved_bytes(const ZenoAmdDeltaInputs* in);      /* 0 also for invalid inputs */
-uint64_t zeno_amd_delta_workspace_bytes(const ZenoAmdDeltaInputs* in);
+uint64_t zeno_amd_delta_workspace_bytes(const ZenoAmdDeltaInputs* in);  /* of either call */
 
 /* One token (length 1) for every sequence: `state` is advanced in place (in->state is not
  * read). What runs beside a step of the simulation. */

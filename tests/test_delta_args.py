@@ -24,7 +24,7 @@ def lib():
     ({"scale": float("inf")}, "scale"), ({"batch": 1 << 31}, "too many")])
 def test_refused_before_any_gpu_work(lib, change, words):
     a, strides = args(**change), (C.c_int64 * 3)()
-    assert lib.zeno_amd_delta_forward(a, 16, strides, 16, None, None) == -6
+    assert lib.zeno_amd_delta_forward(a, 16, strides, 16, None, None, None) == -6
     assert words in _lib.last_error()
     assert lib.zeno_amd_delta_backward(a, 16, 16, _lib.ZenoAmdDeltaGradients(), 16, None) == -6
     assert lib.zeno_amd_delta_step(a, 16, strides, 16, None) == -6
@@ -32,9 +32,9 @@ def test_refused_before_any_gpu_work(lib, change, words):
 
 def test_null_results_are_refused(lib):
     strides = (C.c_int64 * 3)()
-    assert lib.zeno_amd_delta_forward(None, 16, strides, 16, None, None) == -6
-    assert lib.zeno_amd_delta_forward(args(), None, strides, 16, None, None) == -6
-    assert lib.zeno_amd_delta_forward(args(state=64), 16, strides, 64, None, None) == -6
+    assert lib.zeno_amd_delta_forward(None, 16, strides, 16, None, None, None) == -6
+    assert lib.zeno_amd_delta_forward(args(), None, strides, 16, None, None, None) == -6
+    assert lib.zeno_amd_delta_forward(args(state=64), 16, strides, 64, None, None, None) == -6
     assert "overwrite" in _lib.last_error()
     assert lib.zeno_amd_delta_backward(args(), 16, 16, _lib.ZenoAmdDeltaGradients(), None, None) == -6
     assert lib.zeno_amd_delta_step(args(), 16, strides, 16, None) == -6  # 70 tokens
@@ -63,3 +63,14 @@ def test_python_refuses_cpu_tensors_and_wrong_shapes():
         memory.gated_delta_step(*good, z(1, 1, 4, 4))
     with pytest.raises(TypeError, match="float32, float16 or bfloat16"):
         memory.gated_delta(good[0].double(), *good[1:])
+
+
+def test_segments_of_long_sequences(lib):
+    """One head over 4096 tokens: 128 chunks, 16 segments of 8, states and matrices between them."""
+    long = args(batch=1, key_heads=1, value_heads=1, length=4096)
+    assert lib.zeno_amd_delta_workspace_bytes(long) == 4 * 15 * (64 * 64 + 64 * 64 + 4)
+    assert lib.zeno_amd_delta_saved_bytes(long) == 4 * (127 * 64 * 64 + 15 * (64 * 64 + 4))
+    assert lib.zeno_amd_delta_forward(long, 16, (C.c_int64 * 3)(), 16, None, None, None) == -6
+    assert "workspace" in _lib.last_error()
+    assert lib.zeno_amd_delta_forward(long, 16, (C.c_int64 * 3)(), 16, None, 8, None) == -6
+    assert lib.zeno_amd_delta_workspace_bytes(args(batch=512, length=4096, key_heads=4)) == 0

@@ -278,3 +278,43 @@ def test_refusals():
         gated_delta_step(*token, x["state"].mT.contiguous().mT)
     with pytest.raises(ValueError, match="out must be"):
         gated_delta_step(*token, x["state"], out=torch.empty(1, device="cuda"))
+
+
+# (batch, length, key heads, value heads, key_dim, value_dim): few heads and long axes, cut into
+# segments, the last of them partial
+LONG = [(1, 800, 1, 1, 64, 64), (1, 1111, 1, 2, 40, 100), (2, 770, 1, 1, 128, 128), (1, 900, 2, 2, 100, 33)]
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("shape", LONG, ids=str)
+def test_long_sequences(shape, dtype):
+    x = inputs(*shape, dtype, seed=sum(shape), resets=0.003)
+    x["g"] *= 0.05  # states that reach over several segments
+    check_train(x, normalize=True)
+
+
+def test_long_sequence_without_state_and_one_reset_in_a_segment():
+    x = inputs(1, 1500, 1, 1, 32, 64, torch.float32, seed=31, resets=0.0)
+    x["g"] *= 0.01
+    x["state"] = None
+    x["reset"][:, 700] = True
+    check_train(x, normalize=True)
+
+
+def test_nothing_passes_a_reset_between_segments():
+    """NaN in one segment, cleared in a later one: the matrices over segments are cleared too."""
+    from zeno_amd.memory import gated_delta as ours
+
+    x = on_gpu(inputs(1, 2000, 1, 1, 64, 64, torch.float32, seed=12, resets=0.0))
+    x["reset"][:, 1300] = True
+    clean = {n: y.clone() for n, y in x.items()}
+    for at, n in ((3, "v"), (260, "k"), (520, "q"), (780, "g"), (1290, "beta")):
+        x[n][:, at] = float("nan")
+    results = []
+    for d in (clean, x):
+        d = {n: (y.clone().requires_grad_() if n in NAMES else y) for n, y in d.items()}
+        o, s = ours(**d, normalize=True)
+        grads = torch.autograd.grad((o[:, 1300:].square().sum(), s.square().sum()), [d[n] for n in NAMES[:5]])
+        results.append([o[:, 1300:], s, *(y[:, 1300:] for y in grads)])
+    for a, b in zip(*results):
+        assert torch.isfinite(a).all() and torch.equal(a, b)

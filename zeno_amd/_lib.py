@@ -213,7 +213,7 @@ SIGNATURES = {
     "zeno_amd_selfcheck_divide": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint32]),
     "zeno_amd_selfcheck_sqrt": (C.c_int, [C.c_void_p, C.c_void_p, C.c_uint32]),
     "zeno_amd_selfcheck_reciprocal_error": (C.c_int, [C.c_void_p]),
-    "zeno_amd_delta_forward": (C.c_int, [_delta, _vp, _i64p, _vp, _vp, _vp]),
+    "zeno_amd_delta_forward": (C.c_int, [_delta, _vp, _i64p, _vp, _vp, _vp, _vp]),
     "zeno_amd_delta_backward": (C.c_int, [_delta, _vp, _vp, C.POINTER(ZenoAmdDeltaGradients), _vp, _vp]),
     "zeno_amd_delta_saved_bytes": (C.c_uint64, [_delta]),
     "zeno_amd_delta_workspace_bytes": (C.c_uint64, [_delta]),

@@ -549,12 +549,15 @@ static int delta_refused(const char* what, const std::string& why) {
     return ZENO_INVALID_ARGUMENT;
 }
 
-int zeno_amd_delta_forward(const ZenoAmdDeltaInputs* in, void* o, const int64_t* o_stride, float* last, void* saved, void* stream) {
+int zeno_amd_delta_forward(const ZenoAmdDeltaInputs* in, void* o, const int64_t* o_stride, float* last, void* saved, void* workspace,
+                           void* stream) {
     const std::string why = za::delta::check(in, false);
     if (!why.empty()) return delta_refused("delta_forward", why);
     if (!o || !o_stride || !last) return delta_refused("delta_forward", "null output");
     if (last == in->state) return delta_refused("delta_forward", "the last state would overwrite the first");
-    return hip_status(za::delta::forward(*in, o, o_stride, last, (float*)saved, (hipStream_t)stream), "delta_forward");
+    if ((uintptr_t)saved % 16 || (uintptr_t)workspace % 16 || (!workspace && za::delta::workspace_floats(*in)))
+        return delta_refused("delta_forward", "saved or workspace is not aligned to 16 bytes, or workspace is null");
+    return hip_status(za::delta::forward(*in, o, o_stride, last, (float*)saved, (float*)workspace, (hipStream_t)stream), "delta_forward");
 }
 
 int zeno_amd_delta_backward(const ZenoAmdDeltaInputs* in, const float* last, const void* saved, const ZenoAmdDeltaGradients* grad,
@@ -564,7 +567,8 @@ int zeno_amd_delta_backward(const ZenoAmdDeltaInputs* in, const float* last, con
     if (!grad || !grad->d_o || !grad->d_q || !grad->d_k || !grad->d_v || !grad->d_g || !grad->d_beta)
         return delta_refused("delta_backward", "null gradient");
     if (!last || (!saved && za::delta::saved_floats(*in))) return delta_refused("delta_backward", "null state of the forward call");
-    if (!workspace && za::delta::workspace_floats(*in)) return delta_refused("delta_backward", "null workspace");
+    if ((uintptr_t)saved % 16 || (uintptr_t)workspace % 16 || (!workspace && za::delta::workspace_floats(*in)))
+        return delta_refused("delta_backward", "saved or workspace is not aligned to 16 bytes, or workspace is null");
     return hip_status(za::delta::backward(*in, last, (const float*)saved, *grad, (float*)workspace, (hipStream_t)stream), "delta_backward");
 }
 

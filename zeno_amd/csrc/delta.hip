@@ -1,6 +1,7 @@
 // The gated delta rule: argument checks, launch shapes and dispatch by element type.
 #include "delta.h"
 
+#include <algorithm>
 #include <cmath>
 
 #include "mma.h"
@@ -16,15 +17,15 @@ namespace {
 
 uint32_t element_bytes(uint32_t dtype) { return dtype == T_F32 ? 4 : 2; }
 
-// Whether eight elements along a row can move in 16-byte accesses: the base and every stride
-// that is used are multiples of 16 bytes.
-bool vectors(const void* p, const int64_t* stride, uint32_t batch, uint32_t length, uint32_t heads, uint32_t bytes) {
+// Whether every row begins at a multiple of `unit` bytes: the base and every stride that is used.
+bool vectors(const void* p, const int64_t* stride, uint32_t batch, uint32_t length, uint32_t heads, uint32_t bytes, uint32_t unit) {
     const int64_t n[3] = {batch, length, heads};
-    if ((uintptr_t)p % 16) return false;
+    if ((uintptr_t)p % unit) return false;
     for (int i = 0; i < 3; ++i)
-        if (n[i] > 1 && stride[i] * bytes % 16) return false;
+        if (n[i] > 1 && stride[i] * bytes % unit) return false;
     return true;
 }
+bool state_vectors(const void* state, const ZenoAmdDeltaInputs& in) { return in.value_dim % 4 == 0 && (uintptr_t)state % 16 == 0; }
 
 hipError_t by_type(uint32_t dtype, hipError_t (*f32)(const Args&, const Shape&, hipStream_t), hipError_t (*f16)(const Args&, const Shape&, hipStream_t),
                    hipError_t (*bf16)(const Args&, const Shape&, hipStream_t), const Args& a, const Shape& s, hipStream_t stream) {
@@ -36,11 +37,13 @@ Args common(const ZenoAmdDeltaInputs& in, const Shape& s) {
     a.in = in;
     a.share = in.value_heads / in.key_heads;
     a.chunks = (in.length + 16 * s.tiles - 1) / (16 * s.tiles);
+    a.segments = s.segments;
+    a.segment_length = s.segment_length;
     const uint32_t eb = element_bytes(in.dtype);
-    a.q_vec = vectors(in.q, in.q_stride, in.batch, in.length, in.key_heads, eb);
-    a.k_vec = vectors(in.k, in.k_stride, in.batch, in.length, in.key_heads, eb);
-    a.v_vec = vectors(in.v, in.v_stride, in.batch, in.length, in.value_heads, eb);
-    a.s_vec = in.value_dim % 4 == 0 && (uintptr_t)in.state % 16 == 0;
+    a.q_vec = vectors(in.q, in.q_stride, in.batch, in.length, in.key_heads, eb, 16);
+    a.k_vec = vectors(in.k, in.k_stride, in.batch, in.length, in.key_heads, eb, 16);
+    a.v_vec = vectors(in.v, in.v_stride, in.batch, in.length, in.value_heads, eb, 4 * eb);
+    a.s_vec = state_vectors(in.state, in);
     return a;
 }
 
@@ -50,23 +53,48 @@ void set_strides(int64_t* to, const int64_t* from) {
 
 }  // namespace
 
-// 16 tokens a chunk where 32 do not fit the 160 KB of a CU in the gradients' kernel.
-Shape shape_of(const ZenoAmdDeltaInputs& in) {
+// 16 tokens a chunk where 32 do not fit the 160 KB of a CU in the gradients' kernel. Segments:
+// with fewer heads than the GPU holds workgroups (one of eight waves a CU, two of four), as many as
+// fill it, of at least eight chunks. The additional pass over the tokens costs as much as it
+// saves where fewer than three segments come of it.
+Shape shape_of(const ZenoAmdDeltaInputs& in, bool train) {
     Shape s;
     s.dk = in.key_dim <= 64 ? 64 : 128;
     s.waves = s.dk == 128 || in.value_dim > 64 ? 8 : 4;
-    s.tiles = s.waves == 8 && (in.dtype == T_F32 || (in.dtype == T_F16 && s.dk == 128)) ? 1 : 2;
+    s.tiles = train && s.waves == 8 && (in.dtype == T_F32 || (in.dtype == T_F16 && s.dk == 128)) ? 1 : 2;
+    const int64_t chunk = 16 * s.tiles, chunks = (in.length + chunk - 1) / chunk;
+    const int64_t heads = (int64_t)in.batch * in.value_heads, room = s.waves == 8 ? 256 : 512;
+    int64_t want = room / heads;
+    if (want > chunks / 8) want = chunks / 8;
+    if (want < 3) want = 1;
+    const int64_t each = (chunks + want - 1) / want;
+    s.segment_length = (int)(each * chunk);
+    s.segments = (int)((chunks + each - 1) / each);
     return s;
 }
 
-uint64_t saved_floats(const ZenoAmdDeltaInputs& in) {
-    const Shape s = shape_of(in);
-    const uint64_t chunks = (in.length + 16 * s.tiles - 1) / (16 * s.tiles);
-    return chunks < 2 ? 0 : (uint64_t)in.batch * in.value_heads * (chunks - 1) * s.dk * (16 * s.waves);
+namespace {
+uint64_t heads_of(const ZenoAmdDeltaInputs& in) { return (uint64_t)in.batch * in.value_heads; }
+uint64_t states_floats(const ZenoAmdDeltaInputs& in, const Shape& s) {  // between segments
+    return heads_of(in) * (s.segments - 1) * s.dk * (16 * s.waves);
 }
+uint64_t jumps_floats(const ZenoAmdDeltaInputs& in, const Shape& s) { return heads_of(in) * (s.segments - 1) * (s.dk * s.dk + 4); }
+uint64_t inner_floats(const ZenoAmdDeltaInputs& in, const Shape& s) {
+    const uint64_t chunks = (in.length + 16 * s.tiles - 1) / (16 * s.tiles);
+    return heads_of(in) * (chunks - 1) * s.dk * (16 * s.waves);
+}
+uint64_t share_floats(const ZenoAmdDeltaInputs& in) {
+    return in.key_heads == in.value_heads ? 0 : (2ull * in.batch * in.length * in.value_heads * in.key_dim + 3) / 4 * 4;
+}
+}  // namespace
 
+uint64_t saved_floats(const ZenoAmdDeltaInputs& in) {
+    const Shape s = shape_of(in, true);
+    return inner_floats(in, s) + jumps_floats(in, s);
+}
 uint64_t workspace_floats(const ZenoAmdDeltaInputs& in) {
-    return in.key_heads == in.value_heads ? 0 : 2ull * in.batch * in.length * in.value_heads * in.key_dim;
+    const Shape run = shape_of(in, false), train = shape_of(in, true);
+    return std::max(states_floats(in, run) + jumps_floats(in, run), share_floats(in) + states_floats(in, train));
 }
 
 std::string check_sizes(const ZenoAmdDeltaInputs& in) {
@@ -91,46 +119,57 @@ std::string check(const ZenoAmdDeltaInputs* p, bool step) {
     return "";
 }
 
-hipError_t forward(const ZenoAmdDeltaInputs& in, void* o, const int64_t* o_stride, float* last, float* saved, hipStream_t stream) {
-    Shape s = shape_of(in);
-    if (!saved) s.tiles = 2;
+hipError_t forward(const ZenoAmdDeltaInputs& in, void* o, const int64_t* o_stride, float* last, float* saved, float* workspace,
+                   hipStream_t stream) {
+    const Shape s = shape_of(in, saved != nullptr);
     Args a = common(in, s);
     a.o = o;
     set_strides(a.o_stride, o_stride);
-    a.o_vec = vectors(o, o_stride, in.batch, in.length, in.value_heads, element_bytes(in.dtype));
+    a.o_vec = vectors(o, o_stride, in.batch, in.length, in.value_heads, element_bytes(in.dtype), 4 * element_bytes(in.dtype));
     a.last = last;
+    a.last_vec = state_vectors(last, in);
     a.saved = saved;
+    a.starts = workspace;
+    a.jumps = saved ? saved + inner_floats(in, s) : workspace + states_floats(in, s);
+    a.full = in.key_dim == (uint32_t)s.dk && in.value_dim == 16u * s.waves && a.q_vec && a.k_vec && a.v_vec && a.o_vec && a.s_vec && a.last_vec;
     return by_type(in.dtype, launch_forward<T_F32>, launch_forward<T_F16>, launch_forward<T_BF16>, a, s, stream);
 }
 
 hipError_t backward(const ZenoAmdDeltaInputs& in, const float* last, const float* saved, const ZenoAmdDeltaGradients& grad, float* workspace,
                     hipStream_t stream) {
-    const Shape s = shape_of(in);
+    const Shape s = shape_of(in, true);
     Args a = common(in, s);
     const uint32_t eb = element_bytes(in.dtype);
     a.last = const_cast<float*>(last);
+    a.last_vec = state_vectors(last, in);
     a.saved = const_cast<float*>(saved);
+    a.jumps = a.saved + inner_floats(in, s);
+    a.d_starts = workspace + share_floats(in);
     a.d_o = grad.d_o;
     set_strides(a.d_o_stride, grad.d_o_stride);
-    a.d_o_vec = vectors(grad.d_o, grad.d_o_stride, in.batch, in.length, in.value_heads, eb);
+    a.d_o_vec = vectors(grad.d_o, grad.d_o_stride, in.batch, in.length, in.value_heads, eb, 16);
     a.d_last = grad.d_last;
+    a.d_last_vec = state_vectors(grad.d_last, in);
     a.dq = grad.d_q;
     a.dk = grad.d_k;
     a.dv = grad.d_v;
     set_strides(a.dq_stride, grad.d_q_stride);
     set_strides(a.dk_stride, grad.d_k_stride);
     set_strides(a.dv_stride, grad.d_v_stride);
-    a.dq_vec = vectors(grad.d_q, grad.d_q_stride, in.batch, in.length, in.key_heads, eb);
-    a.dk_vec = vectors(grad.d_k, grad.d_k_stride, in.batch, in.length, in.key_heads, eb);
-    a.dv_vec = vectors(grad.d_v, grad.d_v_stride, in.batch, in.length, in.value_heads, eb);
+    a.dq_vec = vectors(grad.d_q, grad.d_q_stride, in.batch, in.length, in.key_heads, eb, 16);
+    a.dk_vec = vectors(grad.d_k, grad.d_k_stride, in.batch, in.length, in.key_heads, eb, 16);
+    a.dv_vec = vectors(grad.d_v, grad.d_v_stride, in.batch, in.length, in.value_heads, eb, 4 * eb);
     a.dg = grad.d_g;
     a.dbeta = grad.d_beta;
     set_strides(a.dg_stride, grad.d_g_stride);
     set_strides(a.dbeta_stride, grad.d_beta_stride);
     a.d_state = grad.d_state;
+    a.d_state_vec = state_vectors(grad.d_state, in);
+    a.full = in.key_dim == (uint32_t)s.dk && in.value_dim == 16u * s.waves && a.q_vec && a.k_vec && a.v_vec && a.s_vec && a.last_vec && a.d_o_vec &&
+             a.dv_vec && a.d_last_vec && a.d_state_vec;
     if (a.share > 1) {
         a.part_q = workspace;
-        a.part_k = workspace + workspace_floats(in) / 2;
+        a.part_k = workspace + (uint64_t)in.batch * in.length * in.value_heads * in.key_dim;
     }
     return by_type(in.dtype, launch_backward<T_F32>, launch_backward<T_F16>, launch_backward<T_BF16>, a, s, stream);
 }

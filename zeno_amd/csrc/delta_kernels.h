@@ -17,6 +17,8 @@
 // it and no value from before a reset is ever multiplied by a zero. Partial chunks are filled
 // with zero keys, zero beta and zero g, which change nothing.
 #pragma once
+#include <type_traits>
+
 #include "delta.h"
 #include "mma.h"
 
@@ -65,31 +67,40 @@ template <int TILES> struct Scalars {  // one float a token
     alignas(16) float beta[C], rk[C], rq[C], gam[C], end[C];
 };
 
-// Rows of q or k into LDS: row-major in `slot` order along the head's dimension, and (cols not
-// null) transposed. norm: 1 / sqrt(sum of squares + eps) of each row, or 1.
-template <int TY, int DK, int NW, int TILES>
-__device__ __forceinline__ void load_rows(const typename Elem<TY>::type* base, int64_t stride, int len, int dim, bool vec, bool normalize,
-                                          uint16_t* rows, uint16_t* cols, float* norm) {
+__device__ __forceinline__ f4 row4(const float* s, int tile, int g) { return *reinterpret_cast<const f4*>(s + 16 * tile + 4 * g); }
+
+// One thread's eight values of a chunk's rows of q or k (or of rows as wide as DK).
+template <int TY, int DK, int NW, int TILES> struct Rows {
     typedef Geo<TY, DK, NW, TILES> G;
-    constexpr int per = DK / 8;
-#pragma unroll 1
-    for (int it = threadIdx.x; it < G::C * per; it += G::threads) {
-        const int row = it / per, e = 8 * (it % per);
-        float x[8];
-        load8<TY>(base + row * stride + e, row < len ? dim - e : 0, vec, x);
+    static constexpr int per = DK / 8;
+    static_assert(G::C * per <= G::threads, "one piece a thread");
+    Raw<TY> raw;
+    static __device__ __forceinline__ bool mine() { return G::C * per == G::threads || threadIdx.x < G::C * per; }
+    // The first `rows` rows (others repeat the last one). FULL: the head has DK dimensions, aligned.
+    template <bool FULL> __device__ __forceinline__ void fetch(const typename Elem<TY>::type* base, int64_t stride, int rows, int dim, bool vec) {
+        const int row = min((int)threadIdx.x / per, rows - 1), e = 8 * (threadIdx.x % per);
+        if (mine()) raw.template load<FULL>(base + row * stride + e, dim - e, vec);
+    }
+    // The first `len` rows and zeros into LDS: row-major in `slot` order along the head's
+    // dimension, and (cols not null) transposed. norm: 1 / sqrt(sum of squares + eps) of each row, or 1.
+    __device__ __forceinline__ void store(int len, bool normalize, uint16_t* rows, uint16_t* cols, float* norm) {
+        const int row = threadIdx.x / per, e = 8 * (threadIdx.x % per);
+        if (!mine()) return;
+        raw.keep(row < len);
+        float ss = 0.0f;
         if (normalize) {
-            float ss = 0.0f;
+            float x[8];
+            raw.get(x);
 #pragma unroll
             for (int j = 0; j < 8; ++j) ss += x[j] * x[j];
-#pragma unroll
-            for (int d = 1; d < per; d <<= 1) ss += __shfl_xor(ss, d);
-            if (e == 0) norm[row] = 1.0f / sqrtf(ss + kNormEps);
-        } else if (e == 0) {
-            norm[row] = 1.0f;
+            if (per > 8) ss += dpp<0x128>(ss);  // rotation by 8 within 16 lanes: sums of 8 in either half
+            ss += dpp<0x141>(ss);               // the half's mirror image, and so on
+            ss += dpp<0x1b>(ss);                // lanes 3 2 1 0 of four
+            ss += dpp<0xb1>(ss);                // lanes 1 0 3 2
         }
+        if (e == 0) norm[row] = normalize ? __builtin_amdgcn_rsqf(ss + kNormEps) : 1.0f;
         uint32_t w[4][G::NP];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) split_pair<G::NP>(x[2 * j], x[2 * j + 1], w[j]);
+        raw.parts(w);
         const int ts = Tok<TILES>::slot_of(row);
 #pragma unroll
         for (int p = 0; p < G::NP; ++p) {
@@ -103,7 +114,7 @@ __device__ __forceinline__ void load_rows(const typename Elem<TY>::type* base, i
             }
         }
     }
-}
+};
 
 // g and beta of a chunk (one lane a token, wave 0): sums in 64 bits.
 template <int TILES>
@@ -138,32 +149,48 @@ __device__ __forceinline__ f4 decayed(const uint16_t* rows_i, const uint16_t* ro
                      frag_at<G::NP>(rows_j + (16 * tj + n) * G::KS + 32 * ks + 8 * g, G::C * G::KS), acc);
     const int j = 16 * tj + n;
     const float hj = s.hi[j], lj = s.lo[j], rj = s.rk[j];
+    const f4 hi = row4(s.hi, ti, g), lo = row4(s.lo, ti, g), nr = row4(ri, ti, g);
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        const int i = 16 * ti + 4 * g + r;
-        acc[r] *= __expf((s.hi[i] - hj) + (s.lo[i] - lj)) * (ri[i] * rj);
-    }
+    for (int r = 0; r < 4; ++r) acc[r] *= __expf((hi[r] - hj) + (lo[r] - lj)) * (nr[r] * rj);
     return acc;
 }
 
-// Column c (of 16) of the inverse of a unit lower triangular 16x16 matrix whose strict part is
-// `at`, by forward substitution.
-__device__ __forceinline__ void inverse_column(const float* at, int c, float* t) {
+// Row r (of 16) of the inverse of I + N, N strictly lower triangular and row-major: of t (I + N) =
+// e_r, from the last column to the first, each value taken out of all sums that still need it.
+__device__ __forceinline__ void inverse_row(const float* N, int r, float* t) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        float s = i == c ? 1.0f : 0.0f;
+    for (int j = 0; j < 16; ++j) t[j] = j == r ? 1.0f : 0.0f;
 #pragma unroll
-        for (int j = 0; j < i; ++j) s -= at[i * kInvStride + j] * t[j];
-        t[i] = s;
+    for (int j = 15; j > 0; --j) {
+#pragma unroll
+        for (int c = 0; c < j; c += 4) {
+            const f4 w = *reinterpret_cast<const f4*>(N + j * kInvStride + c);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (c + i < j) t[c + i] -= t[j] * w[i];
+        }
     }
 }
-
-__device__ __forceinline__ void put_parts3(uint16_t* to, int part, float x) {
-    uint32_t w[3];
-    split_pair<3>(x, 0.0f, w);
+// Column c of the same, from N transposed.
+__device__ __forceinline__ void inverse_column(const float* NT, int c, float* t) {
 #pragma unroll
-    for (int p = 0; p < 3; ++p) to[p * part] = (uint16_t)w[p];
+    for (int j = 0; j < 16; ++j) t[j] = j == c ? 1.0f : 0.0f;
+#pragma unroll
+    for (int j = 0; j < 15; ++j) {
+#pragma unroll
+        for (int b = (j + 1) & ~3; b < 16; b += 4) {
+            const f4 w = *reinterpret_cast<const f4*>(NT + j * kInvStride + b);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (b + i > j) t[b + i] -= t[j] * w[i];
+        }
+    }
 }
+__device__ __forceinline__ void put_row(uint16_t* to, const float* t) {  // 16 values in three parts
+#pragma unroll
+    for (int b = 0; b < 16; b += 4) put4<3>(to + b, 16 * kInvStride, f4{t[b], t[b + 1], t[b + 2], t[b + 3]});
+}
+
 template <int P> __device__ __forceinline__ void put_parts(uint16_t* to, int part, float x) {
     uint32_t w[P];
     split_pair<P>(x, 0.0f, w);
@@ -171,7 +198,6 @@ template <int P> __device__ __forceinline__ void put_parts(uint16_t* to, int par
     for (int p = 0; p < P; ++p) to[p * part] = (uint16_t)w[p];
 }
 
-__device__ __forceinline__ f4 row4(const float* s, int tile, int g) { return *reinterpret_cast<const f4*>(s + 16 * tile + 4 * g); }
 
 // The matrices inside a chunk that both directions use.
 template <int TILES> struct Inner {
@@ -189,87 +215,121 @@ template <int TILES> struct InnerBack : Inner<TILES> {
     alignas(16) float diag2[TILES * 16 * kInvStride];         // B Z, diagonal tiles
 };
 
-// Fills Inner (and InnerBack) from the rows in LDS: K K^T and Q K^T by all waves. The caller
-// synchronises before and after; invert() follows.
-template <int TY, int DK, int NW, int TILES, bool BACK, class M>
+// A result tile (rows from i0 = 16 ti + 4 g, this lane's column j) into a matrix along tokens,
+// [row][slot of column], and its transpose.
+template <int P, int TILES> __device__ __forceinline__ void put_rows(uint16_t* m, f4 v, int ti, int tj, int lane) {
+    typedef Tok<TILES> K;
+    const int n = lane & 15, g = lane >> 4;
+    put4<P>(m + (16 * ti + 4 * g + (n & 3)) * K::stride + K::slot_of(16 * tj + (n & 12)), 16 * TILES * K::stride, turn(v, lane));
+}
+template <int P, int TILES> __device__ __forceinline__ void put_cols(uint16_t* m, f4 v, int ti, int tj, int lane) {
+    typedef Tok<TILES> K;
+    const int n = lane & 15, g = lane >> 4;
+    put4<P>(m + (16 * tj + n) * K::stride + K::slot_of(16 * ti + 4 * g), 16 * TILES * K::stride, v);
+}
+
+// Fills Inner (and InnerBack) from the rows in LDS, the tiles spread over the waves; a wave that
+// makes a diagonal tile of Z inverts it. USED tiles of 16 tokens are in use. The caller
+// synchronises before and after.
+enum Want { W_P = 1, W_PT = 2, W_INV = 4, W_INVT = 8 };  // the latter two with Z below the diagonal
+template <int TY, int DK, int NW, int TILES, int USED, int WANT, class M>
 __device__ __forceinline__ void fill_inner(const uint16_t* K, const uint16_t* Q, const Scalars<TILES>& s, float scale, M& m) {
-    typedef Geo<TY, DK, NW, TILES> G;
-    constexpr int pairs = TILES * (TILES + 1) / 2;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
-    for (int job = wave; job < 2 * pairs; job += NW) {
-        const int pair = job % pairs, ti = pair > 0 ? 1 : 0, tj = pair > 1 ? 1 : 0, j = 16 * tj + n;
-        if (job < pairs) {
+    // Jobs by wave of four (of two tiles): Z00 and its inverse, Z11 and its inverse, Z10 and P00,
+    // P10 and P11; eight waves take one each.
+#pragma unroll
+    for (int job = 0; job < 3 * TILES; ++job) {
+        constexpr int order[6][3] = {{0, 0, 0}, {0, 1, 1}, {0, 1, 0}, {1, 1, 0}, {1, 0, 0}, {1, 1, 1}};  // product, tile
+        const int what = TILES == 2 ? order[job][0] : job, ti = TILES == 2 ? order[job][1] : 0, tj = TILES == 2 ? order[job][2] : 0;
+        const int by = NW >= 6 ? job : job < 4 ? job : job - 2;
+        if ((TILES == 1 && job > 1) || ti >= USED || by != wave || (what == 1 && !(WANT & (W_P | W_PT)))) continue;
+        const int j = 16 * tj + n;
+        if (what == 0) {
             const f4 z = decayed<TY, DK, NW, TILES>(K, K, s.rk, ti, tj, n, g, s);
             if (ti == tj) {
                 const float bj = s.beta[j];
+                const f4 bi = row4(s.beta, ti, g);
+                f4 zb, bz;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const int i = 4 * g + r;
-                    const float v = n < i ? z[r] : 0.0f;
-                    m.diag[(ti * 16 + i) * kInvStride + n] = v * bj;
-                    if constexpr (BACK) m.diag2[(ti * 16 + i) * kInvStride + n] = v * s.beta[16 * ti + i];
+                    const float v = n < 4 * g + r ? z[r] : 0.0f;
+                    zb[r] = v * bj;
+                    bz[r] = v * bi[r];
                 }
+                if constexpr (WANT & W_INV) *reinterpret_cast<f4*>(m.diag + (ti * 16 + 4 * g + (n & 3)) * kInvStride + (n & 12)) = turn(zb, lane);
+                if constexpr (WANT & W_INVT) *reinterpret_cast<f4*>(m.diag2 + (ti * 16 + n) * kInvStride + 4 * g) = bz;
+                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+                float t[16];
+                if constexpr (WANT & W_INV)
+                    if (lane < 16) {
+                        inverse_row(m.diag + ti * 16 * kInvStride, n, t);
+                        put_row(m.inv + (ti * 3 * 16 + n) * kInvStride, t);
+                    }
+                if constexpr (WANT & W_INVT)
+                    if (lane >= 48) {
+                        inverse_column(m.diag2 + ti * 16 * kInvStride, n, t);
+                        put_row(m.invT + (ti * 3 * 16 + n) * kInvStride, t);
+                    }
             } else {
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    put_parts3(m.off + (4 * g + r) * kInvStride + n, 16 * kInvStride, z[r]);
-                    if constexpr (BACK) put_parts3(m.offT + n * kInvStride + 4 * g + r, 16 * kInvStride, z[r]);
-                }
+                if constexpr (WANT & W_INV) put4<3>(m.off + (4 * g + (n & 3)) * kInvStride + (n & 12), 16 * kInvStride, turn(z, lane));
+                if constexpr (WANT & W_INVT) put4<3>(m.offT + n * kInvStride + 4 * g, 16 * kInvStride, z);
             }
         } else {
-            const f4 p = decayed<TY, DK, NW, TILES>(Q, K, s.rq, ti, tj, n, g, s);
-            const int sj = Tok<TILES>::slot_of(j);
+            f4 p = decayed<TY, DK, NW, TILES>(Q, K, s.rq, ti, tj, n, g, s);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int i = 16 * ti + 4 * g + r;
-                const float v = j <= i ? p[r] * scale : 0.0f;
-                put_parts3(m.P + i * G::TS + sj, G::C * G::TS, v);
-                if constexpr (BACK) put_parts3(m.PT + j * G::TS + Tok<TILES>::slot_of(i), G::C * G::TS, v);
-            }
+            for (int r = 0; r < 4; ++r) p[r] = j <= 16 * ti + 4 * g + r ? p[r] * scale : 0.0f;
+            if constexpr (WANT & W_P) put_rows<3, TILES>(m.P, p, ti, tj, lane);
+            if constexpr (WANT & W_PT) put_cols<3, TILES>(m.PT, p, ti, tj, lane);
         }
     }
 }
 
-// One wave: the inverses of the diagonal tiles, 16 lanes each.
-template <int TILES, bool BACK, class M> __device__ __forceinline__ void invert(int lane, M& m) {
-    const int which = lane >> 4, c = lane & 15;
-    float t[16];
-    if (which < TILES) {
-        inverse_column(m.diag + which * 16 * kInvStride, c, t);
-        uint16_t* to = m.inv + which * 3 * 16 * kInvStride + c;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) put_parts3(to + i * kInvStride, 16 * kInvStride, t[i]);
-    }
-    if constexpr (BACK) {
-        if (which >= TILES && which < 2 * TILES) {
-            inverse_column(m.diag2 + (which - TILES) * 16 * kInvStride, c, t);
-            uint16_t* to = m.invT + (which - TILES) * 3 * 16 * kInvStride + c * kInvStride;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) put_parts3(to + i, 16 * kInvStride, t[i]);
-        }
-    }
-}
-
-// E (and U = beta E) from X, in place in registers.
-template <int TILES, class M> __device__ __forceinline__ void solve(const M& m, const Scalars<TILES>& s, int n, int g, f4* x, f4* u) {
+// E (and U = beta E, and its parts) from X, in place in registers.
+template <int TILES, int USED, class M>
+__device__ __forceinline__ void solve(const M& m, const Scalars<TILES>& s, int n, int g, f4* x, f4* u, Half<3>* up) {
     constexpr int tile = 16 * kInvStride;
     const f4 zero = {0, 0, 0, 0};
     const uint16_t* row = m.inv + n * kInvStride + 4 * g;
     x[0] = mul<2>(half_at<3>(row, tile), split<3>(x[0]), zero);
     u[0] = x[0] * row4(s.beta, 0, g);
-    if constexpr (TILES == 2) {
-        const f4 d = mul<2>(half_at<3>(m.off + n * kInvStride + 4 * g, tile), split<3>(u[0]), zero);
+    up[0] = split<3>(u[0]);
+    if constexpr (USED == 2) {
+        const f4 d = mul<2>(half_at<3>(m.off + n * kInvStride + 4 * g, tile), up[0], zero);
         x[1] = mul<2>(half_at<3>(row + 3 * tile, tile), split<3>(x[1] - d), zero);
         u[1] = x[1] * row4(s.beta, 1, g);
+        up[1] = split<3>(u[1]);
     }
 }
 
 // acc += lower(D Q K^T) scale U
-template <int TY, int DK, int NW, int TILES, class M>
-__device__ __forceinline__ void add_PU(const M& m, int n, int g, const f4* u, f4* acc) {
-    typedef Geo<TY, DK, NW, TILES> G;
-    acc[0] = mul<2>(half_at<3>(m.P + n * G::TS + Tok<TILES>::tile_at(g, 0), G::C * G::TS), split<3>(u[0]), acc[0]);
-    if constexpr (TILES == 2) acc[1] = mul<2>(frag_at<3>(m.P + (16 + n) * G::TS + 8 * g, G::C * G::TS), split<3>(u[0], u[1]), acc[1]);
+template <int TILES, int USED, class M>
+__device__ __forceinline__ void add_PU(const M& m, int n, int g, const Half<3>* up, f4* acc) {
+    constexpr int TS = Tok<TILES>::stride, part = 16 * TILES * TS;
+    acc[0] = mul<2>(half_at<3>(m.P + n * TS + Tok<TILES>::tile_at(g, 0), part), up[0], acc[0]);
+    if constexpr (USED == 2) acc[1] = mul<2>(frag_at<3>(m.P + (16 + n) * TS + 8 * g, part), join<3>(up[0], up[1]), acc[1]);
+}
+
+// This wave's columns of a state [rows, cols] in memory (leading dimension ld), as result tiles:
+// a lane reads four columns of a row, and four lanes exchange them.
+template <int DK, bool FULL> __device__ __forceinline__ void load_state(const float* at, int rows, int cols, int ld, bool vec, int col0, int lane, f4* S) {
+    const int row = 4 * (lane >> 4) + (lane & 3), col = col0 + (lane & 12);
+    if (at) {
+        const float* from = at + row * ld + col;
+#pragma unroll
+        for (int i = 0; i < DK / 16; ++i) S[i] = load4<T_F32, FULL>(from + 16 * i * ld, 16 * i + row < rows ? cols - col : 0, vec);
+#pragma unroll
+        for (int i = 0; i < DK / 16; ++i) S[i] = turn(S[i], lane);
+    } else {
+#pragma unroll
+        for (int i = 0; i < DK / 16; ++i) S[i] = f4{0, 0, 0, 0};
+    }
+}
+template <int DK, bool FULL> __device__ __forceinline__ void store_state(float* at, int rows, int cols, int ld, bool vec, int col0, int lane, const f4* S) {
+    const int row = 4 * (lane >> 4) + (lane & 3), col = col0 + (lane & 12);
+    float* to = at + row * ld + col;
+#pragma unroll
+    for (int i = 0; i < DK / 16; ++i) store4<T_F32, FULL>(to + 16 * i * ld, 16 * i + row < rows ? cols - col : 0, vec, turn(S[i], lane));
 }
 
 // ---- forward -------------------------------------------------------------------------------
@@ -280,7 +340,11 @@ template <int TY, int DK, int NW, int TILES> struct ForwardLds {
     Scalars<TILES> s;
 };
 
-template <int TY, int DK, int NW, int TILES>
+// FULL: heads of exactly DK and 16 NW dimensions, aligned, need no masks (a fifth of the instructions).
+// STATES: no outputs; of each segment but the last, N, the state after it from zeros (from the
+// caller's state in the first segment), and M, the same without values from the unit matrix: with
+// S the state before the segment, the state after it is M S + N.
+template <int TY, int DK, int NW, int TILES, bool FULL, bool STATES>
 __global__ __launch_bounds__(64 * NW) void delta_forward_kernel(const Args a) {
     typedef Geo<TY, DK, NW, TILES> G;
     typedef typename Elem<TY>::type E;
@@ -288,9 +352,11 @@ __global__ __launch_bounds__(64 * NW) void delta_forward_kernel(const Args a) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
     const ZenoAmdDeltaInputs& in = a.in;
     const int64_t b = blockIdx.x / in.value_heads, h = blockIdx.x % in.value_heads, hk = h / a.share;
-    const int dk = in.key_dim, dv = in.value_dim, T = in.length;
-    const int col = (blockIdx.y * NW + wave) * 16 + n;
-    const bool live = col < dv;
+    const int dk = in.key_dim, dv = in.value_dim, segment = blockIdx.y;
+    const int begin = segment * a.segment_length, T = min((int)in.length, begin + a.segment_length);  // this segment's tokens
+    const bool unit = STATES && blockIdx.z;
+    if (unit && segment == 0) return;
+    const int col0 = wave * 16, row0 = 4 * g + (n & 3), col = col0 + (n & 12);  // memory: four columns of a row
     const E* q = (const E*)in.q + b * in.q_stride[0] + hk * in.q_stride[2];
     const E* k = (const E*)in.k + b * in.k_stride[0] + hk * in.k_stride[2];
     const E* v = (const E*)in.v + b * in.v_stride[0] + h * in.v_stride[2] + col;
@@ -301,97 +367,185 @@ __global__ __launch_bounds__(64 * NW) void delta_forward_kernel(const Args a) {
     const int64_t bh = b * in.value_heads + h;
 
     f4 S[DK / 16];
+    if (segment == 0) {
+        load_state<DK, FULL>(in.state ? in.state + bh * dk * dv : nullptr, dk, dv, dv, a.s_vec, col0, lane, S);
+    } else if (STATES) {
 #pragma unroll
-    for (int i = 0; i < DK / 16; ++i)
+        for (int i = 0; i < DK / 16; ++i)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int row = 16 * i + 4 * g + r;
-            S[i][r] = in.state && live && row < dk ? in.state[(bh * dk + row) * dv + col] : 0.0f;
-        }
+            for (int r = 0; r < 4; ++r) S[i][r] = unit && 16 * i + 4 * g + r == col0 + n ? 1.0f : 0.0f;
+    } else {
+        load_state<DK, true>(a.starts + (bh * (a.segments - 1) + segment - 1) * (DK * G::DV), DK, G::DV, G::DV, true, col0, lane, S);
+    }
 
-    for (int t = 0; t < T;) {
-        const int lim = min(T, (t / G::C + 1) * G::C);
-        const int tok = t + lane;
-        const bool mine = lane < G::C && tok < lim;
-        float gv = mine ? gp[tok * in.g_stride[1]] : 0.0f;
-        const uint64_t cuts = __ballot(mine && (gv < kClears || (rp && rp[tok * in.reset_stride[1]])));
-        const bool first = cuts & 1;
-        const uint64_t later = cuts & ~1ull;
-        const int len = later ? __ffsll((unsigned long long)later) - 1 : lim - t;
-        f4 x[TILES];
+    // What a chunk reads from memory, fetched one chunk ahead: up to the grid, as where the chunk
+    // ends is known only when its resets are here.
+    Rows<TY, DK, NW, TILES> kr, qr;
+    f4 vr[TILES];
+    float gv, bv;
+    bool cut, any_cut = false;
+    auto fetch = [&](int t) {
+        const int rows = min(T, (t / G::C + 1) * G::C) - t;
+        const int tok = t + min(lane, rows - 1);
+        gv = gp[tok * in.g_stride[1]];
+        bv = bp[tok * in.beta_stride[1]];
+        cut = lane < rows && ((rp && rp[tok * in.reset_stride[1]]) || gv < kClears);
+        kr.template fetch<FULL>(k + t * in.k_stride[1], in.k_stride[1], rows, dk, a.k_vec);
+        if (!STATES) qr.template fetch<FULL>(q + t * in.q_stride[1], in.q_stride[1], rows, dk, a.q_vec);
 #pragma unroll
         for (int i = 0; i < TILES; ++i)
+            vr[i] = unit ? f4{0, 0, 0, 0} : load4<TY, FULL>(v + (t + min(16 * i + row0, rows - 1)) * in.v_stride[1], dv - col, a.v_vec);
+    };
+    // The chunk of tokens t to t + len, in USED tiles (len <= 16 needs but one of two). No branch is
+    // inside: where one lies between a matrix instruction and the use of its result, the compiler
+    // has been seen to leave out the wait.
+    auto chunk = [&](auto used, int t, int len, f4* x) {
+        constexpr int USED = decltype(used)::value;
+        fill_inner<TY, DK, NW, TILES, USED, STATES ? W_INV : W_INV | W_P>(lds.K, lds.Q, lds.s, in.scale, lds.m);
+        f4 ks[USED], o4[USED], u[USED];
+        Half<3> up[USED];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int row = 16 * i + 4 * g + r;
-                x[i][r] = live && row < len ? Elem<TY>::get(v[(t + row) * in.v_stride[1]]) : 0.0f;
-            }
-        if (a.saved && t && t % G::C == 0) {
-            float* to = a.saved + ((bh * (a.chunks - 1) + t / G::C - 1) * DK) * (16 * NW) + 16 * wave + n;
-#pragma unroll
-            for (int i = 0; i < DK / 16; ++i)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) to[(16 * i + 4 * g + r) * (16 * NW)] = S[i][r];
-        }
-        if (first)
-#pragma unroll
-            for (int i = 0; i < DK / 16; ++i) S[i] = f4{0, 0, 0, 0};
-
-        __syncthreads();  // the last chunk's operands are read
-        if (wave == 0) load_scalars<TILES>(lane < len ? gv : 0.0f, lane < len ? bp[tok * in.beta_stride[1]] : 0.0f, lane, first, lds.s);
-        load_rows<TY, DK, NW, TILES>(k + t * in.k_stride[1], in.k_stride[1], len, dk, a.k_vec, in.normalize, lds.K, lds.KT, lds.s.rk);
-        load_rows<TY, DK, NW, TILES>(q + t * in.q_stride[1], in.q_stride[1], len, dk, a.q_vec, in.normalize, lds.Q, nullptr, lds.s.rq);
-        __syncthreads();
-        fill_inner<TY, DK, NW, TILES, false>(lds.K, lds.Q, lds.s, in.scale, lds.m);
-        __syncthreads();
-        if (wave == 0) invert<TILES, false>(lane, lds.m);
-        f4 ks[TILES], o4[TILES];
-#pragma unroll
-        for (int i = 0; i < TILES; ++i) ks[i] = o4[i] = f4{0, 0, 0, 0};
+        for (int i = 0; i < USED; ++i) ks[i] = o4[i] = f4{0, 0, 0, 0};
 #pragma unroll
         for (int c = 0; c < DK / 32; ++c) {
             const Frag<3> sb = split<3>(S[2 * c], S[2 * c + 1]);
 #pragma unroll
-            for (int i = 0; i < TILES; ++i) {
+            for (int i = 0; i < USED; ++i) {
                 const int at = (16 * i + n) * G::KS + 32 * c + 8 * g;
                 ks[i] = mul<2>(frag_at<G::NP>(lds.K + at, G::C * G::KS), sb, ks[i]);
-                o4[i] = mul<2>(frag_at<G::NP>(lds.Q + at, G::C * G::KS), sb, o4[i]);
+                if constexpr (!STATES) o4[i] = mul<2>(frag_at<G::NP>(lds.Q + at, G::C * G::KS), sb, o4[i]);
             }
         }
 #pragma unroll
-        for (int i = 0; i < TILES; ++i) {
+        for (int i = 0; i < USED; ++i) {
             const f4 gam = row4(lds.s.gam, i, g);
             x[i] -= gam * row4(lds.s.rk, i, g) * ks[i];
             o4[i] *= gam * row4(lds.s.rq, i, g) * in.scale;
         }
         __syncthreads();
-        f4 u[TILES];
-        solve<TILES>(lds.m, lds.s, n, g, x, u);
-        add_PU<TY, DK, NW, TILES>(lds.m, n, g, u, o4);
+        solve<TILES, USED>(lds.m, lds.s, n, g, x, u, up);
+        if constexpr (!STATES) {
+            add_PU<TILES, USED>(lds.m, n, g, up, o4);
 #pragma unroll
-        for (int i = 0; i < TILES; ++i) {
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int row = 16 * i + 4 * g + r;
-                if (live && row < len) o[(t + row) * a.o_stride[1]] = Elem<TY>::put(o4[i][r]);
+            for (int i = 0; i < USED; ++i) {
+                const f4 y = turn(o4[i], lane);
+                if (16 * i + row0 < len) store4<TY, FULL>(o + (t + 16 * i + row0) * a.o_stride[1], dv - col, a.o_vec, y);
             }
-            u[i] *= row4(lds.s.end, i, g) * row4(lds.s.rk, i, g);
         }
-        const auto ub = Tok<TILES>::template make<3>(u);
-        const float all = lds.s.gam[G::C - 1];
 #pragma unroll
-        for (int i = 0; i < DK / 16; ++i)
-            S[i] = mul<2>(Tok<TILES>::template at<G::NP>(lds.KT + (16 * i + n) * G::TS, g, DK * G::TS), ub, S[i] * all);
+        for (int i = 0; i < USED; ++i) u[i] *= row4(lds.s.end, i, g) * row4(lds.s.rk, i, g);
+        const float all = lds.s.gam[G::C - 1];
+        if constexpr (USED == TILES) {
+            const auto ub = Tok<TILES>::template make<3>(u);
+#pragma unroll
+            for (int i = 0; i < DK / 16; ++i)
+                S[i] = mul<2>(Tok<TILES>::template at<G::NP>(lds.KT + (16 * i + n) * G::TS, g, DK * G::TS), ub, S[i] * all);
+        } else {
+            const Half<3> ub = split<3>(u[0]);
+#pragma unroll
+            for (int i = 0; i < DK / 16; ++i)
+                S[i] = mul<2>(half_at<G::NP>(lds.KT + (16 * i + n) * G::TS + Tok<TILES>::tile_at(g, 0), DK * G::TS), ub, S[i] * all);
+        }
+    };
+    fetch(begin);
+    for (int t = begin; t < T;) {
+        const int lim = min(T, (t / G::C + 1) * G::C);
+        const uint64_t cuts = __ballot(cut);
+        const bool first = cuts & 1;
+        const uint64_t later = cuts & ~1ull;
+        const int len = later ? __ffsll((unsigned long long)later) - 1 : lim - t;
+        f4 x[TILES];
+#pragma unroll
+        for (int i = 0; i < TILES; ++i) x[i] = turn(16 * i + row0 < len ? vr[i] : f4{0, 0, 0, 0}, lane);
+        if (!STATES && a.saved && t && t % G::C == 0)
+            store_state<DK, true>(a.saved + (bh * (a.chunks - 1) + t / G::C - 1) * (DK * G::DV), DK, G::DV, G::DV, true, col0, lane, S);
+        if (first) {
+            any_cut = true;
+#pragma unroll
+            for (int i = 0; i < DK / 16; ++i) S[i] = f4{0, 0, 0, 0};
+        }
+
+        __syncthreads();  // the last chunk's operands are read
+        if (wave == 0) load_scalars<TILES>(lane < len ? gv : 0.0f, lane < len ? bv : 0.0f, lane, first, lds.s);
+        kr.store(len, in.normalize, lds.K, lds.KT, lds.s.rk);
+        if (!STATES) qr.store(len, in.normalize, lds.Q, nullptr, lds.s.rq);
+        if (t + len < T) fetch(t + len);
+        __syncthreads();
+        if (TILES == 2 && len <= 16) chunk(std::integral_constant<int, 1>{}, t, len, x);
+        else chunk(std::integral_constant<int, TILES>{}, t, len, x);
         t += len;
     }
-    if (live)
+    if constexpr (STATES) {
+        if (unit) {
+            float* to = a.jumps + (bh * (a.segments - 1) + segment) * (DK * DK + 4);
+            if (col0 < DK) store_state<DK, true>(to, DK, DK, DK, true, col0, lane, S);
+            if (threadIdx.x == 0) to[DK * DK] = any_cut ? 0.0f : 1.0f;  // whether anything passes the segment
+        } else {
+            store_state<DK, true>(a.starts + (bh * (a.segments - 1) + segment) * (DK * G::DV), DK, G::DV, G::DV, true, col0, lane, S);
+        }
+    } else if (segment == (int)a.segments - 1)
+        store_state<DK, FULL>(a.last + bh * dk * dv, dk, dv, dv, a.last_vec, col0, lane, S);
+}
+
+// ---- joining segments ------------------------------------------------------------------------
+// The states between the segments from M and N of each: S_{p+1} = M_p S_p + N_p, in place of N.
+// BACK: the same for the state's gradient from the last segment to the first, with M transposed.
+// A workgroup joins one head; its waves hold 16 columns each, M goes through LDS in three parts.
+template <int DK, int NW, bool BACK> __global__ __launch_bounds__(64 * NW) void delta_join_kernel(float* states, const float* jumps, int segments) {
+    constexpr int KS = DK + 8, DV = 16 * NW, pieces = DK * DK / 8 / (64 * NW);
+    __shared__ __attribute__((aligned(16))) uint16_t lds[3 * DK * KS];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4, col0 = 16 * wave;
+    const int64_t bh = blockIdx.x, between = segments - 1;
+    // Between segments p and p + 1 lies state p; jump p leads from state p - 1 to state p.
+    const int first = BACK ? segments - 2 : 0, last = BACK ? 0 : segments - 2, step = BACK ? -1 : 1;
+    float* at = states + bh * between * (DK * DV);
+    const float* jump = jumps + bh * between * (DK * DK + 4);
+    Raw<T_F32> raw[pieces];
+    auto fetch = [&](int p) {
 #pragma unroll
-        for (int i = 0; i < DK / 16; ++i)
+        for (int i = 0; i < pieces; ++i) raw[i].template load<true>(jump + (int64_t)p * (DK * DK + 4) + 8 * (threadIdx.x + 64 * NW * i), 8, true);
+    };
+    f4 S[DK / 16];
+    load_state<DK, true>(at + (int64_t)first * (DK * DV), DK, DV, DV, true, col0, lane, S);
+    for (int p = first; p != last; p += step) {
+        // Forward: from state p to p + 1 by jump p + 1. Back: from state p to p - 1 by jump p.
+        const int j = BACK ? p : p + 1, to = p + step;
+        if (p == first) fetch(j);
+        __syncthreads();
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int row = 16 * i + 4 * g + r;
-                if (row < dk) a.last[(bh * dk + row) * dv + col] = S[i][r];
+        for (int i = 0; i < pieces; ++i) {
+            const int piece = threadIdx.x + 64 * NW * i, row = piece / (DK / 8), e = 8 * (piece % (DK / 8));
+            uint32_t w[4][3];
+            raw[i].parts(w);
+#pragma unroll
+            for (int q = 0; q < 3; ++q) {
+                if (BACK) {
+#pragma unroll
+                    for (int x = 0; x < 8; ++x) lds[(q * DK + e + x) * KS + slot(row)] = (uint16_t)(w[x >> 1][q] >> (16 * (x & 1)));
+                } else {
+                    uint16_t* y = lds + (q * DK + row) * KS;
+                    *reinterpret_cast<u2*>(y + slot(e)) = u2{w[0][q], w[1][q]};
+                    *reinterpret_cast<u2*>(y + slot(e + 4)) = u2{w[2][q], w[3][q]};
+                }
             }
+        }
+        if (to != last) fetch(j + step);
+        f4 N[DK / 16];
+        load_state<DK, true>(at + (int64_t)to * (DK * DV), DK, DV, DV, true, col0, lane, N);
+        __syncthreads();
+        if (jump[(int64_t)j * (DK * DK + 4) + DK * DK] == 0.0f)  // a reset: NaN times a zero matrix would pass it
+#pragma unroll
+            for (int i = 0; i < DK / 16; ++i) S[i] = f4{0, 0, 0, 0};
+#pragma unroll
+        for (int c = 0; c < DK / 32; ++c) {
+            const Frag<3> sb = split<3>(S[2 * c], S[2 * c + 1]);
+#pragma unroll
+            for (int i = 0; i < DK / 16; ++i) N[i] = mul<2>(frag_at<3>(lds + (16 * i + n) * KS + 32 * c + 8 * g, DK * KS), sb, N[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < DK / 16; ++i) S[i] = N[i];
+        store_state<DK, true>(at + (int64_t)to * (DK * DV), DK, DV, DV, true, col0, lane, S);
+    }
 }
 
 // ---- backward ------------------------------------------------------------------------------
@@ -439,8 +593,133 @@ __device__ __forceinline__ void state8(const float* at, int n, bool vec, f4& x, 
     y = f4{v[4], v[5], v[6], v[7]};
 }
 
-template <int TY, int DK, int NW, int TILES>
-__global__ __launch_bounds__(64 * NW) void delta_backward_kernel(const Args a) {
+// dR and dX = beta dR of dU + P^T dO, dU in du.
+template <int TY, int TILES, class M>
+__device__ __forceinline__ void solve_back(const M& m, const Scalars<TILES>& s, int n, int g, const f4* d_o, f4* du, f4* dr, f4* dx) {
+    constexpr int tile = 16 * kInvStride, NP = Elem<TY>::parts, TS = Tok<TILES>::stride, part = 16 * TILES * TS;
+    const f4 zero = {0, 0, 0, 0};
+    const uint16_t* invT = m.invT + n * kInvStride + 4 * g;
+    du[0] = mul<2>(Tok<TILES>::template at<3>(m.PT + n * TS, g, part), Tok<TILES>::template make<NP>(d_o), du[0]);
+    if constexpr (TILES == 2) {
+        du[1] = mul<2>(half_at<3>(m.PT + (16 + n) * TS + Tok<TILES>::tile_at(g, 1), part), split<NP>(d_o[1]), du[1]);
+        dr[1] = mul<2>(half_at<3>(invT + 3 * tile, tile), split<3>(du[1]), zero);
+        dx[1] = dr[1] * row4(s.beta, 1, g);
+        du[0] -= mul<2>(half_at<3>(m.offT + n * kInvStride + 4 * g, tile), split<3>(dx[1]), zero);
+    }
+    dr[0] = mul<2>(half_at<3>(invT, tile), split<3>(du[0]), zero);
+    dx[0] = dr[0] * row4(s.beta, 0, g);
+}
+
+// dS = gam_C dS' + scale (gam Q)^T dO - K^T (gam dX)
+template <int TY, int DK, int TILES>
+__device__ __forceinline__ void pull_state(const uint16_t* KT, const uint16_t* QT, const Scalars<TILES>& s, float scale, int n, int g, const f4* d_o,
+                                           const f4* dx, f4* dS) {
+    constexpr int NP = Elem<TY>::parts, TS = Tok<TILES>::stride;
+    f4 so[TILES], sx[TILES];
+#pragma unroll
+    for (int i = 0; i < TILES; ++i) {
+        const f4 gam = row4(s.gam, i, g);
+        sx[i] = dx[i] * gam * row4(s.rk, i, g) * -1.0f;
+        so[i] = d_o[i] * gam * row4(s.rq, i, g) * scale;
+    }
+    const auto xb = Tok<TILES>::template make<3>(sx);
+    const auto ob = Tok<TILES>::template make<3>(so);
+    const float all = s.gam[16 * TILES - 1];
+#pragma unroll
+    for (int i = 0; i < DK / 16; ++i) {
+        f4 y = dS[i] * all;
+        y = mul<2>(Tok<TILES>::template at<NP>(KT + (16 * i + n) * TS, g, DK * TS), xb, y);
+        dS[i] = mul<2>(Tok<TILES>::template at<NP>(QT + (16 * i + n) * TS, g, DK * TS), ob, y);
+    }
+}
+
+// The gradient of the state alone, for the segments: of every segment but the first, what its
+// outputs (and, of the last, d_last) add to the gradient of the state before it. It needs neither
+// states nor values.
+template <int TY, int DK, int NW, int TILES> struct PullLds {
+    typedef Geo<TY, DK, NW, TILES> G;
+    alignas(16) uint16_t K[G::NP * G::C * G::KS], Q[G::NP * G::C * G::KS], KT[G::NP * DK * G::TS], QT[G::NP * DK * G::TS];
+    InnerBack<TILES> m;
+    Scalars<TILES> s;
+};
+
+// Where the chunk that ends before token te begins: at the grid, or at the last reset since.
+struct Cut {
+    int t;
+    bool first;
+};
+template <int C> __device__ __forceinline__ Cut chunk_before(int te, int lane, const float* gp, int64_t g_stride, const uint8_t* rp, int64_t r_stride) {
+    const int t0 = (te - 1) / C * C;
+    const bool inside = lane < C && t0 + lane < te;
+    const uint64_t cuts = __ballot(inside && (gp[(t0 + lane) * g_stride] < kClears || (rp && rp[(t0 + lane) * r_stride])));
+    return Cut{cuts ? t0 + 63 - __clzll((long long)cuts) : t0, cuts != 0};
+}
+
+template <int TY, int DK, int NW, int TILES, bool FULL>
+__global__ __launch_bounds__(64 * NW) void delta_pull_kernel(const Args a) {
+    typedef Geo<TY, DK, NW, TILES> G;
+    typedef typename Elem<TY>::type E;
+    __shared__ PullLds<TY, DK, NW, TILES> lds;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
+    const ZenoAmdDeltaInputs& in = a.in;
+    const int64_t b = blockIdx.x / in.value_heads, h = blockIdx.x % in.value_heads, hk = h / a.share;
+    const int dk = in.key_dim, dv = in.value_dim, segment = blockIdx.y + 1;
+    const int begin = segment * a.segment_length, T = min((int)in.length, begin + a.segment_length);
+    const int col0 = wave * 16, row0 = 4 * g + (n & 3), col = col0 + (n & 12);
+    const E* q = (const E*)in.q + b * in.q_stride[0] + hk * in.q_stride[2];
+    const E* k = (const E*)in.k + b * in.k_stride[0] + hk * in.k_stride[2];
+    const float* gp = in.g + b * in.g_stride[0] + h * in.g_stride[2];
+    const float* bp = in.beta + b * in.beta_stride[0] + h * in.beta_stride[2];
+    const uint8_t* rp = in.reset ? in.reset + b * in.reset_stride[0] : nullptr;
+    const E* d_o = (const E*)a.d_o + b * a.d_o_stride[0] + h * a.d_o_stride[2] + col;
+    const int64_t bh = b * in.value_heads + h;
+    f4 dS[DK / 16];
+    load_state<DK, FULL>(a.d_last && segment == (int)a.segments - 1 ? a.d_last + bh * dk * dv : nullptr, dk, dv, dv, a.d_last_vec, col0, lane, dS);
+    for (int te = T; te > begin;) {
+        const Cut cut = chunk_before<G::C>(te, lane, gp, in.g_stride[1], rp, in.reset_stride[1]);
+        const int t = cut.t, len = te - t;
+        Rows<TY, DK, NW, TILES> kr, qr;
+        kr.template fetch<FULL>(k + t * in.k_stride[1], in.k_stride[1], len, dk, a.k_vec);
+        qr.template fetch<FULL>(q + t * in.q_stride[1], in.q_stride[1], len, dk, a.q_vec);
+        f4 d4[TILES];
+#pragma unroll
+        for (int i = 0; i < TILES; ++i) {
+            const f4 x = load4<TY, FULL>(d_o + (t + min(16 * i + row0, len - 1)) * a.d_o_stride[1], dv - col, a.d_o_vec);
+            d4[i] = turn(16 * i + row0 < len ? x : f4{0, 0, 0, 0}, lane);
+        }
+        __syncthreads();
+        if (wave == 0)
+            load_scalars<TILES>(lane < len ? gp[(t + lane) * in.g_stride[1]] : 0.0f, lane < len ? bp[(t + lane) * in.beta_stride[1]] : 0.0f, lane,
+                                cut.first, lds.s);
+        kr.store(len, in.normalize, lds.K, lds.KT, lds.s.rk);
+        qr.store(len, in.normalize, lds.Q, lds.QT, lds.s.rq);
+        __syncthreads();
+        fill_inner<TY, DK, NW, TILES, TILES, W_PT | W_INVT>(lds.K, lds.Q, lds.s, in.scale, lds.m);
+        f4 du[TILES], dr[TILES], dx[TILES];
+#pragma unroll
+        for (int i = 0; i < TILES; ++i) du[i] = f4{0, 0, 0, 0};
+#pragma unroll
+        for (int c = 0; c < DK / 32; ++c) {
+            const Frag<3> db = split<3>(dS[2 * c], dS[2 * c + 1]);
+#pragma unroll
+            for (int i = 0; i < TILES; ++i)
+                du[i] = mul<2>(frag_at<G::NP>(lds.K + (16 * i + n) * G::KS + 32 * c + 8 * g, G::C * G::KS), db, du[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < TILES; ++i) du[i] *= row4(lds.s.end, i, g) * row4(lds.s.rk, i, g);
+        __syncthreads();
+        solve_back<TY, TILES>(lds.m, lds.s, n, g, d4, du, dr, dx);
+        pull_state<TY, DK, TILES>(lds.KT, lds.QT, lds.s, in.scale, n, g, d4, dx, dS);
+        if (cut.first)
+#pragma unroll
+            for (int i = 0; i < DK / 16; ++i) dS[i] = f4{0, 0, 0, 0};
+        te = t;
+    }
+    store_state<DK, true>(a.d_starts + (bh * (a.segments - 1) + segment - 1) * (DK * G::DV), DK, G::DV, G::DV, true, col0, lane, dS);
+}
+
+template <int TY, int DK, int NW, int TILES, bool FULL>
+__global__ __launch_bounds__(64 * NW, NW == 8 || sizeof(BackwardLds<TY, DK, NW, TILES>) <= 80 * 1024 ? 2 : 1) void delta_backward_kernel(const Args a) {
     typedef Geo<TY, DK, NW, TILES> G;
     typedef BackwardLds<TY, DK, NW, TILES> L;
     typedef typename Elem<TY>::type E;
@@ -449,9 +728,9 @@ __global__ __launch_bounds__(64 * NW) void delta_backward_kernel(const Args a) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
     const ZenoAmdDeltaInputs& in = a.in;
     const int64_t b = blockIdx.x / in.value_heads, h = blockIdx.x % in.value_heads, hk = h / a.share;
-    const int dk = in.key_dim, dv = in.value_dim, T = in.length;
-    const int col = wave * 16 + n;
-    const bool live = col < dv;
+    const int dk = in.key_dim, dv = in.value_dim, segment = blockIdx.y;
+    const int begin = segment * a.segment_length, T = min((int)in.length, begin + a.segment_length);  // this segment's tokens
+    const int col0 = wave * 16, row0 = 4 * g + (n & 3), col = col0 + (n & 12);  // memory: four columns of a row
     const E* q = (const E*)in.q + b * in.q_stride[0] + hk * in.q_stride[2];
     const E* k = (const E*)in.k + b * in.k_stride[0] + hk * in.k_stride[2];
     const E* v = (const E*)in.v + b * in.v_stride[0] + h * in.v_stride[2] + col;
@@ -463,23 +742,18 @@ __global__ __launch_bounds__(64 * NW) void delta_backward_kernel(const Args a) {
     const int64_t bh = b * in.value_heads + h;
 
     f4 dS[DK / 16], Sn[DK / 16];  // the gradient of the state, and the state, after the chunk
-#pragma unroll
-    for (int i = 0; i < DK / 16; ++i)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int row = 16 * i + 4 * g + r;
-            const int64_t at = (bh * dk + row) * dv + col;
-            const bool ok = live && row < dk;
-            dS[i][r] = ok && a.d_last ? a.d_last[at] : 0.0f;
-            Sn[i][r] = ok ? a.last[at] : 0.0f;
-        }
+    if (segment == (int)a.segments - 1) {
+        load_state<DK, FULL>(a.d_last ? a.d_last + bh * dk * dv : nullptr, dk, dv, dv, a.d_last_vec, col0, lane, dS);
+        load_state<DK, FULL>(a.last + bh * dk * dv, dk, dv, dv, a.last_vec, col0, lane, Sn);
+    } else {
+        load_state<DK, true>(a.d_starts + (bh * (a.segments - 1) + segment) * (DK * G::DV), DK, G::DV, G::DV, true, col0, lane, dS);
+        load_state<DK, true>(a.saved + (bh * (a.chunks - 1) + T / C - 1) * (DK * G::DV), DK, G::DV, G::DV, true, col0, lane, Sn);
+    }
 
-    for (int te = T; te > 0;) {
-        const int t0 = (te - 1) / C * C;
-        const bool inside = lane < C && t0 + lane < te;
-        const uint64_t cuts = __ballot(inside && (gp[(t0 + lane) * in.g_stride[1]] < kClears || (rp && rp[(t0 + lane) * in.reset_stride[1]])));
-        const bool first = cuts != 0;
-        const int t = first ? t0 + 63 - __clzll((long long)cuts) : t0;
+    for (int te = T; te > begin;) {
+        const Cut cut = chunk_before<C>(te, lane, gp, in.g_stride[1], rp, in.reset_stride[1]);
+        const int t = cut.t;
+        const bool first = cut.first;
         const int len = te - t;
         // The state before the chunk: nothing, the caller's, or a saved one.
         const float* sp = nullptr;
@@ -498,51 +772,45 @@ __global__ __launch_bounds__(64 * NW) void delta_backward_kernel(const Args a) {
         if (wave == 0)
             load_scalars<TILES>(lane < len ? gp[(t + lane) * in.g_stride[1]] : 0.0f, lane < len ? bp[(t + lane) * in.beta_stride[1]] : 0.0f, lane,
                                 first, lds.s);
-        load_rows<TY, DK, NW, TILES>(k + t * in.k_stride[1], in.k_stride[1], len, dk, a.k_vec, in.normalize, lds.K, lds.KT, lds.s.rk);
-        load_rows<TY, DK, NW, TILES>(q + t * in.q_stride[1], in.q_stride[1], len, dk, a.q_vec, in.normalize, lds.Q, lds.QT, lds.s.rq);
-        for (int it = threadIdx.x; it < C * G::DV / 8; it += G::threads) {
-            const int row = it / (G::DV / 8), e = 8 * (it % (G::DV / 8));
-            float x[8];
-            load8<TY>(d_o + (t + row) * a.d_o_stride[1] + e, row < len ? dv - e : 0, a.d_o_vec, x);
-            uint32_t w[4][NP];
+        Rows<TY, DK, NW, TILES> kr, qr;
+        kr.template fetch<FULL>(k + t * in.k_stride[1], in.k_stride[1], len, dk, a.k_vec);
+        qr.template fetch<FULL>(q + t * in.q_stride[1], in.q_stride[1], len, dk, a.q_vec);
+        kr.store(len, in.normalize, lds.K, lds.KT, lds.s.rk);
+        qr.store(len, in.normalize, lds.Q, lds.QT, lds.s.rq);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) split_pair<NP>(x[2 * j], x[2 * j + 1], w[j]);
+        for (int it0 = 0; it0 < C * G::DV / 8; it0 += G::threads) {
+            const int it = it0 + threadIdx.x, row = it / (G::DV / 8), e = 8 * (it % (G::DV / 8));
+            if (C * G::DV / 8 % G::threads && it >= C * G::DV / 8) break;
+            Raw<TY> x;
+            x.template load<FULL>(d_o + (t + min(row, len - 1)) * a.d_o_stride[1] + e, dv - e, a.d_o_vec);
+            x.keep(row < len);
+            uint32_t w[4][NP];
+            x.parts(w);
 #pragma unroll
             for (int p = 0; p < NP; ++p) *reinterpret_cast<u4*>(lds.DO + (p * C + row) * G::VS + e) = u4{w[0][p], w[1][p], w[2][p], w[3][p]};
         }
         f4 S[DK / 16];
-#pragma unroll
-        for (int i = 0; i < DK / 16; ++i)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int row = 16 * i + 4 * g + r;
-                S[i][r] = sp && row < s_rows && col < s_cols ? sp[row * s_ld + col] : 0.0f;
-            }
+        load_state<DK, FULL>(sp, s_rows, s_cols, s_ld, s_vec, col0, lane, S);
         f4 vv[TILES];
 #pragma unroll
         for (int i = 0; i < TILES; ++i)
+            vv[i] = turn(load4<TY, FULL>(v + (t + min(16 * i + row0, len - 1)) * in.v_stride[1], dv - col, a.v_vec), lane);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int row = 16 * i + 4 * g + r;
-                vv[i][r] = live && row < len ? Elem<TY>::get(v[(t + row) * in.v_stride[1]]) : 0.0f;
-            }
+        for (int i = 0; i < TILES; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) vv[i][r] = 16 * i + 4 * g + r < len ? vv[i][r] : 0.0f;
         __syncthreads();
-        fill_inner<TY, DK, NW, TILES, true>(lds.K, lds.Q, lds.s, in.scale, lds.m);
-        __syncthreads();
+        fill_inner<TY, DK, NW, TILES, TILES, W_P | W_PT | W_INV | W_INVT>(lds.K, lds.Q, lds.s, in.scale, lds.m);
 
         // ---- phase A: this wave's columns
-        if (wave == 0) invert<TILES, true>(lane, lds.m);
         f4 ks[TILES], o4[TILES], du[TILES], d4[TILES];
 #pragma unroll
         for (int i = 0; i < TILES; ++i) {
             ks[i] = o4[i] = du[i] = f4{0, 0, 0, 0};
+            f4 x = {0, 0, 0, 0};
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                float x = 0.0f;
-#pragma unroll
-                for (int p = NP - 1; p >= 0; --p) x += __uint_as_float((uint32_t)lds.DO[(p * C + 16 * i + 4 * g + r) * G::VS + col] << 16);
-                d4[i][r] = x;
-            }
+            for (int p = NP - 1; p >= 0; --p) x += load4<T_BF16>(lds.DO + (p * C + 16 * i + row0) * G::VS + col, 4, true);
+            d4[i] = turn(x, lane);
         }
 #pragma unroll
         for (int c = 0; c < DK / 32; ++c) {
@@ -573,36 +841,31 @@ __global__ __launch_bounds__(64 * NW) void delta_backward_kernel(const Args a) {
         edge = sum64(edge);
         if (lane == 0) lds.edge[wave] = edge;
         __syncthreads();
-        solve<TILES>(lds.m, lds.s, n, g, x, u);
-        add_PU<TY, DK, NW, TILES>(lds.m, n, g, u, o4);
-        // dU += P^T dO, the transposed solve
-        constexpr int tile = 16 * kInvStride;
+        Half<3> up[TILES];
+        solve<TILES, TILES>(lds.m, lds.s, n, g, x, u, up);
+        add_PU<TILES, TILES>(lds.m, n, g, up, o4);
         const f4 zero = {0, 0, 0, 0};
         f4 dr[TILES], dx[TILES];
-        const uint16_t* invT = lds.m.invT + n * kInvStride + 4 * g;
-        du[0] = mul<2>(Tok<TILES>::template at<3>(lds.m.PT + n * G::TS, g, C * G::TS), Tok<TILES>::template make<NP>(d4), du[0]);
-        if constexpr (TILES == 2) {
-            du[1] = mul<2>(half_at<3>(lds.m.PT + (16 + n) * G::TS + Tok<TILES>::tile_at(g, 1), C * G::TS), split<NP>(d4[1]), du[1]);
-            dr[1] = mul<2>(half_at<3>(invT + 3 * tile, tile), split<3>(du[1]), zero);
-            dx[1] = dr[1] * row4(lds.s.beta, 1, g);
-            du[0] -= mul<2>(half_at<3>(lds.m.offT + n * kInvStride + 4 * g, tile), split<3>(dx[1]), zero);
-        }
-        dr[0] = mul<2>(half_at<3>(invT, tile), split<3>(du[0]), zero);
-        dx[0] = dr[0] * row4(lds.s.beta, 0, g);
+        solve_back<TY, TILES>(lds.m, lds.s, n, g, d4, du, dr, dx);
 #pragma unroll
         for (int i = 0; i < TILES; ++i)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int row = 16 * i + 4 * g + r;
-                if (live && row < len) d_v[(t + row) * a.dv_stride[1]] = Elem<TY>::put(dx[i][r]);
                 const float de = sum16(d4[i][r] * o4[i][r] - dx[i][r] * vv[i][r]), be = sum16(dr[i][r] * x[i][r]);
                 if (n == 0) {
                     lds.decay[wave][row] = de;
                     lds.beta[wave][row] = be;
                 }
-                put_parts<NO>(lds.c.U + row * G::VS + col, C * G::VS, u[i][r]);
-                put_parts<NO>(lds.c.X + row * G::VS + col, C * G::VS, dx[i][r]);
             }
+#pragma unroll
+        for (int i = 0; i < TILES; ++i) {
+            const int at = (16 * i + row0) * G::VS + col;
+            const f4 y = turn(dx[i], lane);
+            put4<NO>(lds.c.U + at, C * G::VS, turn(u[i], lane));
+            put4<NO>(lds.c.X + at, C * G::VS, y);
+            if (16 * i + row0 < len) store4<TY, FULL>(d_v + (t + 16 * i + row0) * a.dv_stride[1], dv - col, a.dv_vec, y);
+        }
         __syncthreads();
 
         // ---- phase B: gradients of q and k
@@ -640,21 +903,30 @@ __global__ __launch_bounds__(64 * NW) void delta_backward_kernel(const Args a) {
                 else acc = mul<SO>(frag_at<NO>(lds.c.X + ai, C * G::VS), uf, acc);
             }
             const float hj = lds.s.hi[j], lj = lds.s.lo[j], rj = lds.s.rk[j];
-            const int sj = Tok<TILES>::slot_of(j);
+            f4 by_col, by_row;  // times the norm of the column's token, and of the row's
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int i = 16 * ti + 4 * g + r, si = Tok<TILES>::slot_of(i);
+                const int i = 16 * ti + 4 * g + r;
                 const float w = acc[r] * __expf((lds.s.hi[i] - hj) + (lds.s.lo[i] - lj));
-                if (job < pairs) {
-                    const float y = j <= i ? w * in.scale : 0.0f;
-                    put_parts<NO>(lds.b.W + i * G::TS + sj, C * G::TS, y * rj);
-                    put_parts<NO>(lds.b.WT + j * G::TS + si, C * G::TS, y * lds.s.rq[i]);
-                } else if (ti != tj || j < i) {
-                    put_parts<NO>(lds.b.Y + i * G::TS + sj, C * G::TS, -w * rj);
-                    put_parts<NO>(lds.b.Y + j * G::TS + si, C * G::TS, -w * lds.s.rk[i]);
-                } else if (j == i) {
-                    put_parts<NO>(lds.b.Y + i * G::TS + sj, C * G::TS, 0.0f);
-                }
+                const float y = job < pairs ? (j <= i ? w * in.scale : 0.0f) : (j < i ? -w : 0.0f);
+                by_col[r] = y * rj;
+                by_row[r] = y * (job < pairs ? lds.s.rq[i] : lds.s.rk[i]);
+            }
+            if (job < pairs) {
+                put_rows<NO, TILES>(lds.b.W, by_col, ti, tj, lane);
+                put_cols<NO, TILES>(lds.b.WT, by_row, ti, tj, lane);
+            } else if (ti != tj) {
+                put_rows<NO, TILES>(lds.b.Y, by_col, ti, tj, lane);
+                put_cols<NO, TILES>(lds.b.Y, by_row, ti, tj, lane);
+            } else {
+                // A diagonal tile of Y + Y^T: the mirrored values come through LDS.
+                put_rows<NO, TILES>(lds.b.Y, by_col, ti, tj, lane);
+                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (j < 16 * ti + 4 * g + r)
+                        put_parts<NO>(lds.b.Y + j * G::TS + Tok<TILES>::slot_of(16 * ti + 4 * g + r), C * G::TS, by_row[r]);
             }
         }
         constexpr int blocks = L::slab / 16, slabs = DK / L::slab;
@@ -667,7 +939,7 @@ __global__ __launch_bounds__(64 * NW) void delta_backward_kernel(const Args a) {
 #pragma unroll
             for (int i = 0; i < L::slab / 16; ++i)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) lds.b.dS[(16 * i + 4 * g + r) * L::SS + col] = dS[sl * (L::slab / 16) + i][r];
+                for (int r = 0; r < 4; ++r) lds.b.dS[(16 * i + 4 * g + r) * L::SS + col0 + n] = dS[sl * (L::slab / 16) + i][r];
             __syncthreads();
 #pragma unroll
             for (int rd = 0; rd < rounds; ++rd) {
@@ -723,25 +995,11 @@ __global__ __launch_bounds__(64 * NW) void delta_backward_kernel(const Args a) {
             }
         }
         // the state's gradient, from this wave's columns
-        f4 sx[TILES];
+        pull_state<TY, DK, TILES>(lds.KT, lds.QT, lds.s, in.scale, n, g, d4, dx, dS);
 #pragma unroll
-        for (int i = 0; i < TILES; ++i) {
-            const f4 gam = row4(lds.s.gam, i, g);
-            sx[i] = dx[i] * gam * row4(lds.s.rk, i, g) * -1.0f;
-            d4[i] *= gam * row4(lds.s.rq, i, g) * in.scale;
-        }
-        {
-            const auto xb = Tok<TILES>::template make<3>(sx);
-            const auto ob = Tok<TILES>::template make<3>(d4);
-            const float all = lds.s.gam[C - 1];
-#pragma unroll
-            for (int i = 0; i < DK / 16; ++i) {
-                f4 y = dS[i] * all;
-                y = mul<2>(Tok<TILES>::template at<NP>(lds.KT + (16 * i + n) * G::TS, g, DK * G::TS), xb, y);
-                y = mul<2>(Tok<TILES>::template at<NP>(lds.QT + (16 * i + n) * G::TS, g, DK * G::TS), ob, y);
-                dS[i] = first ? zero : y;
-                Sn[i] = S[i];
-            }
+        for (int i = 0; i < DK / 16; ++i) {
+            if (first) dS[i] = zero;
+            Sn[i] = S[i];
         }
         __syncthreads();  // U and dX are read
 #pragma unroll
@@ -802,14 +1060,7 @@ __global__ __launch_bounds__(64 * NW) void delta_backward_kernel(const Args a) {
         }
         te = t;
     }
-    if (a.d_state && live)
-#pragma unroll
-        for (int i = 0; i < DK / 16; ++i)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int row = 16 * i + 4 * g + r;
-                if (row < dk) a.d_state[(bh * dk + row) * dv + col] = dS[i][r];
-            }
+    if (a.d_state && segment == 0) store_state<DK, FULL>(a.d_state + bh * dk * dv, dk, dv, dv, a.d_state_vec, col0, lane, dS);
 }
 
 // Sums the value heads of each key head, in their order; one thread a value.
@@ -931,25 +1182,46 @@ __global__ __launch_bounds__(256) void delta_step_kernel(const Args a, float* st
 }
 
 // ---- launches ------------------------------------------------------------------------------
+template <int TY, int DK, int NW, int TILES, bool FULL> void forward_shape(const Args& a, hipStream_t stream) {
+    const uint32_t heads = a.in.batch * a.in.value_heads;
+    if (a.segments > 1) {
+        delta_forward_kernel<TY, DK, NW, TILES, FULL, true><<<dim3(heads, a.segments - 1, 2), 64 * NW, 0, stream>>>(a);
+        if (a.segments > 2) delta_join_kernel<DK, NW, false><<<heads, 64 * NW, 0, stream>>>(a.starts, a.jumps, a.segments);
+    }
+    delta_forward_kernel<TY, DK, NW, TILES, FULL, false><<<dim3(heads, a.segments), 64 * NW, 0, stream>>>(a);
+}
+template <int TY, int DK, int NW, int TILES, bool FULL> void backward_shape(const Args& a, hipStream_t stream) {
+    const uint32_t heads = a.in.batch * a.in.value_heads;
+    if (a.segments > 1) {
+        delta_pull_kernel<TY, DK, NW, TILES, FULL><<<dim3(heads, a.segments - 1), 64 * NW, 0, stream>>>(a);
+        if (a.segments > 2) delta_join_kernel<DK, NW, true><<<heads, 64 * NW, 0, stream>>>(a.d_starts, a.jumps, a.segments);
+    }
+    delta_backward_kernel<TY, DK, NW, TILES, FULL><<<dim3(heads, a.segments), 64 * NW, 0, stream>>>(a);
+}
+template <int TY, int DK, int NW, int TILES> void forward_shape(const Args& a, hipStream_t stream) {
+    a.full ? forward_shape<TY, DK, NW, TILES, true>(a, stream) : forward_shape<TY, DK, NW, TILES, false>(a, stream);
+}
+template <int TY, int DK, int NW, int TILES> void backward_shape(const Args& a, hipStream_t stream) {
+    a.full ? backward_shape<TY, DK, NW, TILES, true>(a, stream) : backward_shape<TY, DK, NW, TILES, false>(a, stream);
+}
+
 template <int TY> hipError_t launch_forward(const Args& a, const Shape& s, hipStream_t stream) {
-    const dim3 grid(a.in.batch * a.in.value_heads);
-    if (s.dk == 64 && s.waves == 4) delta_forward_kernel<TY, 64, 4, 2><<<grid, 256, 0, stream>>>(a);
-    else if (s.dk == 64 && s.tiles == 2) delta_forward_kernel<TY, 64, 8, 2><<<grid, 512, 0, stream>>>(a);
-    else if (s.tiles == 2) delta_forward_kernel<TY, 128, 8, 2><<<grid, 512, 0, stream>>>(a);
+    if (s.dk == 64 && s.waves == 4) forward_shape<TY, 64, 4, 2>(a, stream);
+    else if (s.dk == 64 && s.tiles == 2) forward_shape<TY, 64, 8, 2>(a, stream);
+    else if (s.tiles == 2) forward_shape<TY, 128, 8, 2>(a, stream);
     else if constexpr (TY == T_F32) {
-        if (s.dk == 64) delta_forward_kernel<TY, 64, 8, 1><<<grid, 512, 0, stream>>>(a);
-        else delta_forward_kernel<TY, 128, 8, 1><<<grid, 512, 0, stream>>>(a);
+        if (s.dk == 64) forward_shape<TY, 64, 8, 1>(a, stream);
+        else forward_shape<TY, 128, 8, 1>(a, stream);
     } else if constexpr (TY == T_F16) {
-        delta_forward_kernel<TY, 128, 8, 1><<<grid, 512, 0, stream>>>(a);
+        forward_shape<TY, 128, 8, 1>(a, stream);
     }
     return hipGetLastError();
 }
 
 template <int TY> hipError_t launch_backward(const Args& a, const Shape& s, hipStream_t stream) {
-    const dim3 grid(a.in.batch * a.in.value_heads);
-    if (s.dk == 64 && s.waves == 4) delta_backward_kernel<TY, 64, 4, 2><<<grid, 256, 0, stream>>>(a);
-    else if (s.dk == 64) delta_backward_kernel<TY, 64, 8, TY == T_F32 ? 1 : 2><<<grid, 512, 0, stream>>>(a);
-    else delta_backward_kernel<TY, 128, 8, TY == T_BF16 ? 2 : 1><<<grid, 512, 0, stream>>>(a);
+    if (s.dk == 64 && s.waves == 4) backward_shape<TY, 64, 4, 2>(a, stream);
+    else if (s.dk == 64) backward_shape<TY, 64, 8, TY == T_F32 ? 1 : 2>(a, stream);
+    else backward_shape<TY, 128, 8, TY == T_BF16 ? 2 : 1>(a, stream);
     if (a.part_q) {
         const int64_t all = (int64_t)a.in.batch * a.in.length * a.in.key_heads * a.in.key_dim;
         delta_share_kernel<TY><<<dim3((uint32_t)((all + 255) / 256)), 256, 0, stream>>>(a);

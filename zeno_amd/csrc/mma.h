@@ -133,6 +133,65 @@ template <> struct Elem<T_BF16> {
     static __device__ __forceinline__ uint16_t put(float x) { return (uint16_t)round_pair(x, x); }
 };
 
+// Eight consecutive elements as they are in memory, the first `n` of them in bounds (the rest are
+// zero). `vec`: the address is a multiple of 16 bytes whenever n is 8. FULL: n is 8, and so it is.
+template <int TY> struct Raw {
+    static constexpr int words = TY == T_F32 ? 8 : 4;
+    u4 a[words / 4];
+    template <bool FULL> __device__ __forceinline__ void load(const typename Elem<TY>::type* at, int n, bool vec) {
+        typedef typename Elem<TY>::type E;
+        if (FULL || (vec && n >= 8)) {
+#pragma unroll
+            for (int i = 0; i < words / 4; ++i) a[i] = reinterpret_cast<const u4*>(at)[i];
+        } else if constexpr (TY == T_F32) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) a[j / 4][j % 4] = j < n ? __float_as_uint(at[j]) : 0u;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t lo = 2 * j < n ? __builtin_bit_cast(uint16_t, at[2 * j]) : 0u;
+                const uint32_t hi = 2 * j + 1 < n ? __builtin_bit_cast(uint16_t, (E)at[2 * j + 1]) : 0u;
+                a[0][j] = lo | hi << 16;
+            }
+        }
+    }
+    __device__ __forceinline__ void keep(bool yes) {
+#pragma unroll
+        for (int i = 0; i < words; ++i) a[i / 4][i % 4] = yes ? a[i / 4][i % 4] : 0u;
+    }
+    __device__ __forceinline__ void get(float* x) const {
+        typedef typename Elem<TY>::type E;
+        if constexpr (TY == T_F32) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = __uint_as_float(a[j / 4][j % 4]);
+        } else if constexpr (TY == T_BF16) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                x[2 * j] = __uint_as_float(a[0][j] << 16);
+                x[2 * j + 1] = __uint_as_float(a[0][j] & 0xffff0000u);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                x[2 * j] = Elem<TY>::get(__builtin_bit_cast(E, (uint16_t)(a[0][j] & 0xffffu)));
+                x[2 * j + 1] = Elem<TY>::get(__builtin_bit_cast(E, (uint16_t)(a[0][j] >> 16)));
+            }
+        }
+    }
+    // The bf16 parts, pairs of values by pair.
+    __device__ __forceinline__ void parts(uint32_t w[4][Elem<TY>::parts]) const {
+        if constexpr (TY == T_BF16) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j][0] = a[0][j];
+        } else {
+            float x[8];
+            get(x);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) split_pair<Elem<TY>::parts>(x[2 * j], x[2 * j + 1], w[j]);
+        }
+    }
+};
+
 // Eight consecutive elements, the first `n` of them in bounds (the rest are zero). `vec`: the
 // address is a multiple of 16 bytes whenever n is 8.
 template <int TY> __device__ __forceinline__ void load8(const typename Elem<TY>::type* at, int n, bool vec, float* x) {
@@ -176,11 +235,71 @@ template <int TY> __device__ __forceinline__ void store8(typename Elem<TY>::type
     }
 }
 
+// Four consecutive elements, the first `n` of them in bounds. `vec`: the address is a multiple of
+// the four elements' bytes whenever n is 4. FULL: n is 4, and so it is.
+template <int TY, bool FULL = false> __device__ __forceinline__ f4 load4(const typename Elem<TY>::type* at, int n, bool vec) {
+    typedef typename Elem<TY>::type E;
+    f4 x = {0, 0, 0, 0};
+    if (FULL || (vec && n >= 4)) {
+        if constexpr (TY == T_F32) {
+            x = *reinterpret_cast<const f4*>(at);
+        } else {
+            const u2 a = *reinterpret_cast<const u2*>(at);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] = Elem<TY>::get(__builtin_bit_cast(E, (uint16_t)(a[j >> 1] >> (16 * (j & 1)))));
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (j < n) x[j] = Elem<TY>::get(at[j]);
+    }
+    return x;
+}
+template <int TY, bool FULL = false> __device__ __forceinline__ void store4(typename Elem<TY>::type* at, int n, bool vec, f4 x) {
+    if (FULL || (vec && n >= 4)) {
+        if constexpr (TY == T_F32) {
+            *reinterpret_cast<f4*>(at) = x;
+        } else {
+            u2 a;
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+                a[j] = TY == T_BF16 ? round_pair(x[2 * j], x[2 * j + 1])
+                                    : (uint32_t)__builtin_bit_cast(uint16_t, Elem<TY>::put(x[2 * j])) |
+                                          (uint32_t)__builtin_bit_cast(uint16_t, Elem<TY>::put(x[2 * j + 1])) << 16;
+            *reinterpret_cast<u2*>(at) = a;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (j < n) at[j] = Elem<TY>::put(x[j]);
+    }
+}
+
+// A value from another lane of the same 16 (or of the same four).
+template <int CTRL> __device__ __forceinline__ float dpp(float x) {
+    return __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(x), CTRL, 0xf, 0xf, true));
+}
 // Sum over the 16 lanes that hold one row of a result tile; every lane gets it.
 __device__ __forceinline__ float sum16(float x) {
+    x += dpp<0x128>(x);  // rotations within 16 lanes by 8, 4, 2 and 1
+    x += dpp<0x124>(x);
+    x += dpp<0x122>(x);
+    return x + dpp<0x121>(x);
+}
+// Transposes 4x4 values across four lanes: register r of lane q becomes register q of lane r. Of a
+// result tile, lane n then holds row 4 g + n % 4, columns 4 (n / 4) + 0..3.
+__device__ __forceinline__ f4 turn(f4 x, int lane) {
+    const bool a = lane & 1, b = lane & 2;
+    const float s0 = dpp<0xb1>(a ? x[0] : x[1]), s1 = dpp<0xb1>(a ? x[2] : x[3]);  // lanes 1 0 3 2
+    const f4 y = a ? f4{s0, x[1], s1, x[3]} : f4{x[0], s0, x[2], s1};
+    const float t0 = dpp<0x4e>(b ? y[0] : y[2]), t1 = dpp<0x4e>(b ? y[1] : y[3]);  // lanes 2 3 0 1
+    return b ? f4{t0, t1, y[2], y[3]} : f4{y[0], y[1], t0, t1};
+}
+// The parts of four values that are consecutive in LDS.
+template <int P> __device__ __forceinline__ void put4(uint16_t* at, int part, f4 x) {
+    const Half<P> h = split<P>(x);
 #pragma unroll
-    for (int d = 1; d < 16; d <<= 1) x += __shfl_xor(x, d);
-    return x;
+    for (int p = 0; p < P; ++p) *reinterpret_cast<u2*>(at + p * part) = h.p[p];
 }
 __device__ __forceinline__ float sum64(float x) {
 #pragma unroll

@@ -136,19 +136,6 @@ template <int P> __device__ __forceinline__ f4 get4(const _Float16* at) {
     return x;
 }
 
-template <int CTRL> __device__ __forceinline__ float quad(float x) {  // from another lane of four
-    return __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(x), CTRL, 0xf, 0xf, true));
-}
-// Transposes 4x4 values across four lanes: register r of lane q becomes register q of lane r. Of a
-// result tile, lane n then holds row 4 g + n % 4, columns 4 (n / 4) + 0..3.
-__device__ __forceinline__ f4 turn(f4 x, int lane) {
-    const bool a = lane & 1, b = lane & 2;
-    const float s0 = quad<0xb1>(a ? x[0] : x[1]), s1 = quad<0xb1>(a ? x[2] : x[3]);  // lanes 1 0 3 2
-    f4 y = a ? f4{s0, x[1], s1, x[3]} : f4{x[0], s0, x[2], s1};
-    const float t0 = quad<0x4e>(b ? y[0] : y[2]), t1 = quad<0x4e>(b ? y[1] : y[3]);  // lanes 2 3 0 1
-    return b ? f4{t0, t1, y[2], y[3]} : f4{y[0], y[1], t0, t1};
-}
-
 enum Kind { GRAM, POLY, NEXT, LAST };
 enum Share { WHOLE, SLICE, JOIN };  // of the contraction: all of it; a slice, sums kept; the sum of the slices
 

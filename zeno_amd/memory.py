@@ -101,6 +101,10 @@ def _inputs(q, k, v, g, beta, reset, state, scale, normalize) -> L.ZenoAmdDeltaI
         _S3(*qs), _S3(*ks), _S3(*vs), _S3(*gs), _S3(*bs), _S2(*rs))
 
 
+def _space(n: int, x: torch.Tensor) -> Optional[torch.Tensor]:
+    return torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
+
+
 def _stream(x: torch.Tensor) -> int:
     return torch.cuda.current_stream(x.device).cuda_stream
 
@@ -115,12 +119,10 @@ class _GatedDelta(torch.autograd.Function):
             if o.stride(-1) != 1 and o.shape[-1] != 1:
                 o = torch.empty(v.shape, dtype=v.dtype, device=v.device)
             last = torch.empty((q.shape[0], v.shape[2], q.shape[3], v.shape[3]), dtype=torch.float32, device=q.device)
-            saved = None
-            if train:
-                n = lib.zeno_amd_delta_saved_bytes(a)
-                saved = torch.empty(max(n, 1), dtype=torch.uint8, device=q.device)
+            saved = torch.empty(max(lib.zeno_amd_delta_saved_bytes(a), 1), dtype=torch.uint8, device=q.device) if train else None
+            space = _space(lib.zeno_amd_delta_workspace_bytes(a), q)
             rc = lib.zeno_amd_delta_forward(a, o.data_ptr(), _S3(*o.stride()[:3]), last.data_ptr(),
-                                            None if saved is None else saved.data_ptr(), _stream(q))
+                                            None if saved is None else saved.data_ptr(), None if space is None else space.data_ptr(), _stream(q))
             if rc:
                 _fail(rc, "gated_delta")
         if train:
@@ -143,8 +145,7 @@ class _GatedDelta(torch.autograd.Function):
             d_q, d_k, d_v = (_dense_like(x) for x in (q, k, v))
             d_g, d_beta = _dense_like(g), _dense_like(beta)
             d_state = torch.empty_like(state) if state is not None and ctx.needs_input_grad[6] else None
-            n = lib.zeno_amd_delta_workspace_bytes(a)
-            space = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
+            space = _space(lib.zeno_amd_delta_workspace_bytes(a), q)
             grads = L.ZenoAmdDeltaGradients(
                 d_o.data_ptr(), _S3(*d_o.stride()[:3]), None if d_last is None else d_last.data_ptr(),
                 d_q.data_ptr(), d_k.data_ptr(), d_v.data_ptr(), d_g.data_ptr(), d_beta.data_ptr(),
