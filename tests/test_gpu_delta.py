@@ -282,7 +282,7 @@ def test_refusals():
 
 # (batch, length, key heads, value heads, key_dim, value_dim): few heads and long axes, cut into
 # segments, the last of them partial
-LONG = [(1, 800, 1, 1, 64, 64), (1, 1111, 1, 2, 40, 100), (2, 770, 1, 1, 128, 128), (1, 900, 2, 2, 100, 33)]
+LONG = [(1, 800, 1, 1, 64, 64), (1, 1111, 1, 2, 40, 100), (2, 770, 1, 1, 128, 128), (1, 900, 2, 2, 100, 33), (2, 800, 1, 2, 64, 64)]
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)

@@ -20,8 +20,8 @@ struct Args {
     uint32_t chunks;             // chunks of the grid that a sequence has
     // A long sequence is cut into segments that run side by side. Between them: the states and
     // their gradients [batch, value_heads, segments - 1, DK, 16 waves], and of each segment but the
-    // last (unused for the first) the matrix that takes the state over it [.., DK, DK] and a zero
-    // where a reset lies in it (one float of four).
+    // last (unused for the first) the matrix that takes the state over it, as operands of three
+    // 16-bit parts, and its transpose (3 DK DK + 4 floats).
     uint32_t segments;
     int segment_length;          // tokens, whole chunks
     float *starts, *jumps, *d_starts;

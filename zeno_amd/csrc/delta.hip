@@ -78,7 +78,7 @@ uint64_t heads_of(const ZenoAmdDeltaInputs& in) { return (uint64_t)in.batch * in
 uint64_t states_floats(const ZenoAmdDeltaInputs& in, const Shape& s) {  // between segments
     return heads_of(in) * (s.segments - 1) * s.dk * (16 * s.waves);
 }
-uint64_t jumps_floats(const ZenoAmdDeltaInputs& in, const Shape& s) { return heads_of(in) * (s.segments - 1) * (s.dk * s.dk + 4); }
+uint64_t jumps_floats(const ZenoAmdDeltaInputs& in, const Shape& s) { return heads_of(in) * (s.segments - 1) * (3 * s.dk * s.dk + 4); }
 uint64_t inner_floats(const ZenoAmdDeltaInputs& in, const Shape& s) {
     const uint64_t chunks = (in.length + 16 * s.tiles - 1) / (16 * s.tiles);
     return heads_of(in) * (chunks - 1) * s.dk * (16 * s.waves);
@@ -166,7 +166,7 @@ hipError_t backward(const ZenoAmdDeltaInputs& in, const float* last, const float
     a.d_state = grad.d_state;
     a.d_state_vec = state_vectors(grad.d_state, in);
     a.full = in.key_dim == (uint32_t)s.dk && in.value_dim == 16u * s.waves && a.q_vec && a.k_vec && a.v_vec && a.s_vec && a.last_vec && a.d_o_vec &&
-             a.dv_vec && a.d_last_vec && a.d_state_vec;
+             a.dq_vec && a.dk_vec && a.dv_vec && a.d_last_vec && a.d_state_vec;
     if (a.share > 1) {
         a.part_q = workspace;
         a.part_k = workspace + (uint64_t)in.batch * in.length * in.value_heads * in.key_dim;

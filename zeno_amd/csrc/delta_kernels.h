@@ -155,23 +155,8 @@ __device__ __forceinline__ f4 decayed(const uint16_t* rows_i, const uint16_t* ro
     return acc;
 }
 
-// Row r (of 16) of the inverse of I + N, N strictly lower triangular and row-major: of t (I + N) =
-// e_r, from the last column to the first, each value taken out of all sums that still need it.
-__device__ __forceinline__ void inverse_row(const float* N, int r, float* t) {
-#pragma unroll
-    for (int j = 0; j < 16; ++j) t[j] = j == r ? 1.0f : 0.0f;
-#pragma unroll
-    for (int j = 15; j > 0; --j) {
-#pragma unroll
-        for (int c = 0; c < j; c += 4) {
-            const f4 w = *reinterpret_cast<const f4*>(N + j * kInvStride + c);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (c + i < j) t[c + i] -= t[j] * w[i];
-        }
-    }
-}
-// Column c of the same, from N transposed.
+// Column c (of 16) of the inverse of I + N, N strictly lower triangular and kept transposed: each
+// value, once it is final, is taken out of all sums that still need it.
 __device__ __forceinline__ void inverse_column(const float* NT, int c, float* t) {
 #pragma unroll
     for (int j = 0; j < 16; ++j) t[j] = j == c ? 1.0f : 0.0f;
@@ -186,33 +171,32 @@ __device__ __forceinline__ void inverse_column(const float* NT, int c, float* t)
         }
     }
 }
-__device__ __forceinline__ void put_row(uint16_t* to, const float* t) {  // 16 values in three parts
+// 16 values in three parts, from last to first where `flip`.
+__device__ __forceinline__ void put_row(uint16_t* to, const float* t, bool flip) {
 #pragma unroll
-    for (int b = 0; b < 16; b += 4) put4<3>(to + b, 16 * kInvStride, f4{t[b], t[b + 1], t[b + 2], t[b + 3]});
+    for (int b = 0; b < 16; b += 4) {
+        const float v0 = t[b], v1 = t[b + 1], v2 = t[b + 2], v3 = t[b + 3];
+        put4<3>(to + (flip ? 12 - b : b), 16 * kInvStride, f4{flip ? v3 : v0, flip ? v2 : v1, flip ? v1 : v2, flip ? v0 : v3});
+    }
 }
 
-template <int P> __device__ __forceinline__ void put_parts(uint16_t* to, int part, float x) {
-    uint32_t w[P];
-    split_pair<P>(x, 0.0f, w);
-#pragma unroll
-    for (int p = 0; p < P; ++p) to[p * part] = (uint16_t)w[p];
-}
-
-
-// The matrices inside a chunk that both directions use.
+// The matrices inside a chunk. Of the diagonal tiles: 0, Z B with rows and columns from last to
+// first, and the inverse of I + Z B; 1 (gradients), B Z transposed, and the transposed inverse of I + B Z.
 template <int TILES> struct Inner {
-    static constexpr int C = 16 * TILES, TS = Tok<TILES>::stride;
-    alignas(16) uint16_t P[3 * C * TS];                     // lower(D * Q K^T) scale
-    alignas(16) uint16_t off[3 * 16 * kInvStride];          // Z, lower left tile
-    alignas(16) uint16_t inv[TILES * 3 * 16 * kInvStride];  // of I + Z B, diagonal tiles
-    alignas(16) float diag[TILES * 16 * kInvStride];        // Z B, diagonal tiles
+    static constexpr int C = 16 * TILES, TS = Tok<TILES>::stride, sides = 1;
+    static constexpr int tile = 16 * kInvStride;                // of one 16x16 tile
+    alignas(16) uint16_t P[3 * C * TS];                         // lower(D * Q K^T) scale
+    alignas(16) uint16_t off[3 * tile];                         // Z, lower left tile
+    alignas(16) uint16_t inv[TILES * 3 * tile];
+    alignas(16) float diag[TILES * tile];
 };
-template <int TILES> struct InnerBack : Inner<TILES> {
-    typedef Inner<TILES> I;
-    alignas(16) uint16_t PT[3 * I::C * I::TS];                // transposed
-    alignas(16) uint16_t offT[3 * 16 * kInvStride];
-    alignas(16) uint16_t invT[TILES * 3 * 16 * kInvStride];   // of I + B Z, transposed
-    alignas(16) float diag2[TILES * 16 * kInvStride];         // B Z, diagonal tiles
+template <int TILES> struct InnerBack {
+    static constexpr int C = 16 * TILES, TS = Tok<TILES>::stride, sides = 2;
+    static constexpr int tile = 16 * kInvStride;
+    alignas(16) uint16_t P[3 * C * TS], PT[3 * C * TS];         // and transposed
+    alignas(16) uint16_t off[3 * tile], offT[3 * tile];
+    alignas(16) uint16_t inv[2 * TILES * 3 * tile];
+    alignas(16) float diag[2 * TILES * tile];
 };
 
 // A result tile (rows from i0 = 16 ti + 4 g, this lane's column j) into a matrix along tokens,
@@ -256,21 +240,24 @@ __device__ __forceinline__ void fill_inner(const uint16_t* K, const uint16_t* Q,
                     zb[r] = v * bj;
                     bz[r] = v * bi[r];
                 }
-                if constexpr (WANT & W_INV) *reinterpret_cast<f4*>(m.diag + (ti * 16 + 4 * g + (n & 3)) * kInvStride + (n & 12)) = turn(zb, lane);
-                if constexpr (WANT & W_INVT) *reinterpret_cast<f4*>(m.diag2 + (ti * 16 + n) * kInvStride + 4 * g) = bz;
+                // A row of an inverse is a column of it once rows and columns are taken from last to
+                // first: lanes 0 to 15 make the rows of (I + Z B)^-1, lanes 16 to 31 the columns of (I + B Z)^-1.
+                constexpr bool row = WANT & W_INV, col = WANT & W_INVT;
+                constexpr int second = M::sides == 2 ? TILES : 0;  // tiles before those of side 1
+                if constexpr (row) {
+                    const f4 y = turn(zb, lane);
+                    *reinterpret_cast<f4*>(m.diag + (ti * 16 + 15 - 4 * g - (n & 3)) * kInvStride + 12 - (n & 12)) = f4{y[3], y[2], y[1], y[0]};
+                }
+                if constexpr (col) *reinterpret_cast<f4*>(m.diag + ((second + ti) * 16 + n) * kInvStride + 4 * g) = bz;
                 __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
                 __builtin_amdgcn_wave_barrier();
-                float t[16];
-                if constexpr (WANT & W_INV)
-                    if (lane < 16) {
-                        inverse_row(m.diag + ti * 16 * kInvStride, n, t);
-                        put_row(m.inv + (ti * 3 * 16 + n) * kInvStride, t);
-                    }
-                if constexpr (WANT & W_INVT)
-                    if (lane >= 48) {
-                        inverse_column(m.diag2 + ti * 16 * kInvStride, n, t);
-                        put_row(m.invT + (ti * 3 * 16 + n) * kInvStride, t);
-                    }
+                if (lane < (row && col ? 32 : 16)) {
+                    const bool side = row && col ? lane >= 16 : col;
+                    const int at = (side ? second : 0) + ti;
+                    float t[16];
+                    inverse_column(m.diag + at * M::tile, side ? n : 15 - n, t);
+                    put_row(m.inv + at * 3 * M::tile + n * kInvStride, t, !side);
+                }
             } else {
                 if constexpr (WANT & W_INV) put4<3>(m.off + (4 * g + (n & 3)) * kInvStride + (n & 12), 16 * kInvStride, turn(z, lane));
                 if constexpr (WANT & W_INVT) put4<3>(m.offT + n * kInvStride + 4 * g, 16 * kInvStride, z);
@@ -310,26 +297,51 @@ __device__ __forceinline__ void add_PU(const M& m, int n, int g, const Half<3>* 
     if constexpr (USED == 2) acc[1] = mul<2>(frag_at<3>(m.P + (16 + n) * TS + 8 * g, part), join<3>(up[0], up[1]), acc[1]);
 }
 
-// This wave's columns of a state [rows, cols] in memory (leading dimension ld), as result tiles:
-// a lane reads four columns of a row, and four lanes exchange them.
-template <int DK, bool FULL> __device__ __forceinline__ void load_state(const float* at, int rows, int cols, int ld, bool vec, int col0, int lane, f4* S) {
+// This wave's columns of a state [rows, cols] in memory (leading dimension ld; null: zeros). A lane
+// reads four columns of a row; four lanes exchange them (turn) to make result tiles of it.
+template <int DK, bool FULL> __device__ __forceinline__ void fetch_state(const float* at, int rows, int cols, int ld, bool vec, int col0, int lane, f4* S) {
     const int row = 4 * (lane >> 4) + (lane & 3), col = col0 + (lane & 12);
-    if (at) {
-        const float* from = at + row * ld + col;
+    const float* from = at + row * ld + col;
 #pragma unroll
-        for (int i = 0; i < DK / 16; ++i) S[i] = load4<T_F32, FULL>(from + 16 * i * ld, 16 * i + row < rows ? cols - col : 0, vec);
-#pragma unroll
-        for (int i = 0; i < DK / 16; ++i) S[i] = turn(S[i], lane);
-    } else {
-#pragma unroll
-        for (int i = 0; i < DK / 16; ++i) S[i] = f4{0, 0, 0, 0};
+    for (int i = 0; i < DK / 16; ++i) {
+        S[i] = f4{0, 0, 0, 0};
+        if (at) S[i] = load4<T_F32, FULL>(from + 16 * i * ld, 16 * i + row < rows ? cols - col : 0, vec);
     }
+}
+template <int DK, bool FULL> __device__ __forceinline__ void load_state(const float* at, int rows, int cols, int ld, bool vec, int col0, int lane, f4* S) {
+    fetch_state<DK, FULL>(at, rows, cols, ld, vec, col0, lane, S);
+#pragma unroll
+    for (int i = 0; i < DK / 16; ++i) S[i] = turn(S[i], lane);
 }
 template <int DK, bool FULL> __device__ __forceinline__ void store_state(float* at, int rows, int cols, int ld, bool vec, int col0, int lane, const f4* S) {
     const int row = 4 * (lane >> 4) + (lane & 3), col = col0 + (lane & 12);
     float* to = at + row * ld + col;
 #pragma unroll
     for (int i = 0; i < DK / 16; ++i) store4<T_F32, FULL>(to + 16 * i * ld, 16 * i + row < rows ? cols - col : 0, vec, turn(S[i], lane));
+}
+
+// The matrices over segments are kept in the parts and the order in which a lane holds them as
+// left operands: [row tile][32 of the contraction][part][lane][8]; M and, behind it, M transposed.
+template <int DK> struct Jump {
+    static constexpr int steps = DK / 32, part = 64 * 8, row = steps * 3 * part, size = DK / 16 * row;  // in bf16
+    static constexpr int floats = size + 4;  // of both, and whether anything passes the segment at all
+};
+// M's columns from the 16 that this wave holds as result tiles.
+template <int DK> __device__ __forceinline__ void store_jump(uint16_t* to, int wave, int lane, const f4* S) {
+    typedef Jump<DK> J;
+    const int n = lane & 15, g = lane >> 4;
+    // Row 16 i + 4 g + n % 4, columns 16 wave + 4 (n / 4) + 0..3 of M: half of a lane's eight values.
+    uint16_t* m = to + (wave >> 1) * 3 * J::part + (4 * g + (n & 3) + 16 * (n >> 2)) * 8 + 4 * (wave & 1);
+#pragma unroll
+    for (int i = 0; i < DK / 16; ++i) put4<3>(m + i * J::row, J::part, turn(S[i], lane));
+    // Of M transposed these registers are the operand already.
+    uint16_t* t = to + J::size + wave * J::row + lane * 8;
+#pragma unroll
+    for (int c = 0; c < J::steps; ++c) {
+        const Frag<3> f = split<3>(S[2 * c], S[2 * c + 1]);
+#pragma unroll
+        for (int p = 0; p < 3; ++p) *reinterpret_cast<u4*>(t + (c * 3 + p) * J::part) = f.p[p];
+    }
 }
 
 // ---- forward -------------------------------------------------------------------------------
@@ -345,7 +357,7 @@ template <int TY, int DK, int NW, int TILES> struct ForwardLds {
 // caller's state in the first segment), and M, the same without values from the unit matrix: with
 // S the state before the segment, the state after it is M S + N.
 template <int TY, int DK, int NW, int TILES, bool FULL, bool STATES>
-__global__ __launch_bounds__(64 * NW) void delta_forward_kernel(const Args a) {
+__global__ __launch_bounds__(64 * NW, NW == 4 && sizeof(ForwardLds<TY, DK, NW, TILES>) * 3 <= 160 * 1024 ? 3 : 2) void delta_forward_kernel(const Args a) {
     typedef Geo<TY, DK, NW, TILES> G;
     typedef typename Elem<TY>::type E;
     __shared__ ForwardLds<TY, DK, NW, TILES> lds;
@@ -477,9 +489,9 @@ __global__ __launch_bounds__(64 * NW) void delta_forward_kernel(const Args a) {
     }
     if constexpr (STATES) {
         if (unit) {
-            float* to = a.jumps + (bh * (a.segments - 1) + segment) * (DK * DK + 4);
-            if (col0 < DK) store_state<DK, true>(to, DK, DK, DK, true, col0, lane, S);
-            if (threadIdx.x == 0) to[DK * DK] = any_cut ? 0.0f : 1.0f;  // whether anything passes the segment
+            float* to = a.jumps + (bh * (a.segments - 1) + segment) * Jump<DK>::floats;
+            if (col0 < DK) store_jump<DK>(reinterpret_cast<uint16_t*>(to), wave, lane, S);
+            if (threadIdx.x == 0) to[Jump<DK>::size] = any_cut ? 0.0f : 1.0f;
         } else {
             store_state<DK, true>(a.starts + (bh * (a.segments - 1) + segment) * (DK * G::DV), DK, G::DV, G::DV, true, col0, lane, S);
         }
@@ -490,61 +502,58 @@ __global__ __launch_bounds__(64 * NW) void delta_forward_kernel(const Args a) {
 // ---- joining segments ------------------------------------------------------------------------
 // The states between the segments from M and N of each: S_{p+1} = M_p S_p + N_p, in place of N.
 // BACK: the same for the state's gradient from the last segment to the first, with M transposed.
-// A workgroup joins one head; its waves hold 16 columns each, M goes through LDS in three parts.
-template <int DK, int NW, bool BACK> __global__ __launch_bounds__(64 * NW) void delta_join_kernel(float* states, const float* jumps, int segments) {
-    constexpr int KS = DK + 8, DV = 16 * NW, pieces = DK * DK / 8 / (64 * NW);
-    __shared__ __attribute__((aligned(16))) uint16_t lds[3 * DK * KS];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4, col0 = 16 * wave;
+// A workgroup joins 16 value columns of a head. Its four waves share the rows of the result; each
+// step's state reaches them as a right operand through LDS, the matrices come from memory a step
+// ahead. One step is DK / 64 x DK / 32 x 6 dependent-free matrix instructions a wave.
+template <int DK, bool BACK>
+__global__ __launch_bounds__(256) void delta_join_kernel(float* states, const float* jumps, int segments, int DV) {
+    typedef Jump<DK> J;
+    constexpr int TR = DK / 64;  // row tiles a wave
+    __shared__ __attribute__((aligned(16))) uint16_t lds[2][J::steps * 3 * J::part];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col0 = 16 * blockIdx.y;
     const int64_t bh = blockIdx.x, between = segments - 1;
     // Between segments p and p + 1 lies state p; jump p leads from state p - 1 to state p.
     const int first = BACK ? segments - 2 : 0, last = BACK ? 0 : segments - 2, step = BACK ? -1 : 1;
-    float* at = states + bh * between * (DK * DV);
-    const float* jump = jumps + bh * between * (DK * DK + 4);
-    Raw<T_F32> raw[pieces];
-    auto fetch = [&](int p) {
+    float* at = states + bh * between * (DK * DV) + (int64_t)wave * TR * 16 * DV;  // this wave's rows
+    const float* jump = jumps + bh * between * J::floats;
+    Frag<3> m[TR][J::steps];
+    f4 N[TR];
+    float passes;
+    auto fetch = [&](int j, int to) {  // what leads to state `to`
+        const float* from = jump + (int64_t)j * J::floats;
+        const uint16_t* f = reinterpret_cast<const uint16_t*>(from) + (BACK ? J::size : 0) + wave * TR * J::row + lane * 8;
 #pragma unroll
-        for (int i = 0; i < pieces; ++i) raw[i].template load<true>(jump + (int64_t)p * (DK * DK + 4) + 8 * (threadIdx.x + 64 * NW * i), 8, true);
+        for (int i = 0; i < TR; ++i)
+#pragma unroll
+            for (int c = 0; c < J::steps; ++c) m[i][c] = frag_at<3>(f + i * J::row + c * 3 * J::part, J::part);
+        load_state<16 * TR, true>(at + (int64_t)to * (DK * DV), 16 * TR, DV, DV, true, col0, lane, N);
+        passes = from[J::size];
     };
-    f4 S[DK / 16];
-    load_state<DK, true>(at + (int64_t)first * (DK * DV), DK, DV, DV, true, col0, lane, S);
+    f4 S[TR];
+    load_state<16 * TR, true>(at + (int64_t)first * (DK * DV), 16 * TR, DV, DV, true, col0, lane, S);
+    // Forward: from state p to p + 1 by jump p + 1. Back: from state p to p - 1 by jump p.
+    fetch(BACK ? first : first + 1, first + step);
     for (int p = first; p != last; p += step) {
-        // Forward: from state p to p + 1 by jump p + 1. Back: from state p to p - 1 by jump p.
-        const int j = BACK ? p : p + 1, to = p + step;
-        if (p == first) fetch(j);
+        uint16_t* buf = lds[p & 1];
+#pragma unroll
+        for (int i = 0; i < TR; ++i) {
+            // Over a reset nothing passes, not even NaN times a zero matrix.
+            const f4 x = passes == 0.0f ? f4{0, 0, 0, 0} : S[i];
+            const int tile = wave * TR + i;
+            put4<3>(buf + (tile >> 1) * 3 * J::part + lane * 8 + 4 * (tile & 1), J::part, x);
+        }
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < pieces; ++i) {
-            const int piece = threadIdx.x + 64 * NW * i, row = piece / (DK / 8), e = 8 * (piece % (DK / 8));
-            uint32_t w[4][3];
-            raw[i].parts(w);
+        for (int i = 0; i < TR; ++i) S[i] = N[i];
 #pragma unroll
-            for (int q = 0; q < 3; ++q) {
-                if (BACK) {
+        for (int c = 0; c < J::steps; ++c) {
+            const Frag<3> sb = frag_at<3>(buf + c * 3 * J::part + lane * 8, J::part);
 #pragma unroll
-                    for (int x = 0; x < 8; ++x) lds[(q * DK + e + x) * KS + slot(row)] = (uint16_t)(w[x >> 1][q] >> (16 * (x & 1)));
-                } else {
-                    uint16_t* y = lds + (q * DK + row) * KS;
-                    *reinterpret_cast<u2*>(y + slot(e)) = u2{w[0][q], w[1][q]};
-                    *reinterpret_cast<u2*>(y + slot(e + 4)) = u2{w[2][q], w[3][q]};
-                }
-            }
+            for (int i = 0; i < TR; ++i) S[i] = mul<2>(m[i][c], sb, S[i]);
         }
-        if (to != last) fetch(j + step);
-        f4 N[DK / 16];
-        load_state<DK, true>(at + (int64_t)to * (DK * DV), DK, DV, DV, true, col0, lane, N);
-        __syncthreads();
-        if (jump[(int64_t)j * (DK * DK + 4) + DK * DK] == 0.0f)  // a reset: NaN times a zero matrix would pass it
-#pragma unroll
-            for (int i = 0; i < DK / 16; ++i) S[i] = f4{0, 0, 0, 0};
-#pragma unroll
-        for (int c = 0; c < DK / 32; ++c) {
-            const Frag<3> sb = split<3>(S[2 * c], S[2 * c + 1]);
-#pragma unroll
-            for (int i = 0; i < DK / 16; ++i) N[i] = mul<2>(frag_at<3>(lds + (16 * i + n) * KS + 32 * c + 8 * g, DK * KS), sb, N[i]);
-        }
-#pragma unroll
-        for (int i = 0; i < DK / 16; ++i) S[i] = N[i];
-        store_state<DK, true>(at + (int64_t)to * (DK * DV), DK, DV, DV, true, col0, lane, S);
+        const int to = p + step;
+        if (to != last) fetch(BACK ? to : to + 1, to + step);
+        store_state<16 * TR, true>(at + (int64_t)to * (DK * DV), 16 * TR, DV, DV, true, col0, lane, S);
     }
 }
 
@@ -585,20 +594,12 @@ template <int TY, int DK, int NW, int TILES> struct BackwardLds {
     float decay[NW][G::C], beta[NW][G::C], edge[NW];  // sums over each wave's columns
 };
 
-// Eight values of a row of a state [dk, dv] in memory (zero outside).
-__device__ __forceinline__ void state8(const float* at, int n, bool vec, f4& x, f4& y) {
-    float v[8];
-    load8<T_F32>(at, n, vec, v);
-    x = f4{v[0], v[1], v[2], v[3]};
-    y = f4{v[4], v[5], v[6], v[7]};
-}
-
 // dR and dX = beta dR of dU + P^T dO, dU in du.
 template <int TY, int TILES, class M>
 __device__ __forceinline__ void solve_back(const M& m, const Scalars<TILES>& s, int n, int g, const f4* d_o, f4* du, f4* dr, f4* dx) {
     constexpr int tile = 16 * kInvStride, NP = Elem<TY>::parts, TS = Tok<TILES>::stride, part = 16 * TILES * TS;
     const f4 zero = {0, 0, 0, 0};
-    const uint16_t* invT = m.invT + n * kInvStride + 4 * g;
+    const uint16_t* invT = m.inv + TILES * 3 * tile + n * kInvStride + 4 * g;
     du[0] = mul<2>(Tok<TILES>::template at<3>(m.PT + n * TS, g, part), Tok<TILES>::template make<NP>(d_o), du[0]);
     if constexpr (TILES == 2) {
         du[1] = mul<2>(half_at<3>(m.PT + (16 + n) * TS + Tok<TILES>::tile_at(g, 1), part), split<NP>(d_o[1]), du[1]);
@@ -719,97 +720,117 @@ __global__ __launch_bounds__(64 * NW) void delta_pull_kernel(const Args a) {
 }
 
 template <int TY, int DK, int NW, int TILES, bool FULL>
-__global__ __launch_bounds__(64 * NW, NW == 8 || sizeof(BackwardLds<TY, DK, NW, TILES>) <= 80 * 1024 ? 2 : 1) void delta_backward_kernel(const Args a) {
+__global__ __launch_bounds__(64 * NW, NW == 8 || sizeof(BackwardLds<TY, DK, NW, TILES>) <= 80 * 1024 ? 2 : 1) void delta_backward_kernel(const Args) {
     typedef Geo<TY, DK, NW, TILES> G;
     typedef BackwardLds<TY, DK, NW, TILES> L;
     typedef typename Elem<TY>::type E;
     constexpr int NP = G::NP, NO = L::NO, SO = NO - 1, C = G::C;
     __shared__ L lds;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
-    const ZenoAmdDeltaInputs& in = a.in;
-    const int64_t b = blockIdx.x / in.value_heads, h = blockIdx.x % in.value_heads, hk = h / a.share;
-    const int dk = in.key_dim, dv = in.value_dim, segment = blockIdx.y;
-    const int begin = segment * a.segment_length, T = min((int)in.length, begin + a.segment_length);  // this segment's tokens
+    // The arguments are read where they are used: as values held over the loop they would not fit
+    // the scalar registers (two hundred spills, a tenth of the instructions).
+    typedef const __attribute__((address_space(4))) Args* ArgsAt;
+    ArgsAt ap = (ArgsAt)__builtin_amdgcn_kernarg_segment_ptr();
+    const int64_t b = blockIdx.x / ap->in.value_heads, h = blockIdx.x % ap->in.value_heads, hk = h / ap->share;
+    const int dk = ap->in.key_dim, dv = ap->in.value_dim, segment = blockIdx.y;
+    const int begin = segment * ap->segment_length, T = min((int)ap->in.length, begin + ap->segment_length);  // this segment's tokens
     const int col0 = wave * 16, row0 = 4 * g + (n & 3), col = col0 + (n & 12);  // memory: four columns of a row
-    const E* q = (const E*)in.q + b * in.q_stride[0] + hk * in.q_stride[2];
-    const E* k = (const E*)in.k + b * in.k_stride[0] + hk * in.k_stride[2];
-    const E* v = (const E*)in.v + b * in.v_stride[0] + h * in.v_stride[2] + col;
-    const float* gp = in.g + b * in.g_stride[0] + h * in.g_stride[2];
-    const float* bp = in.beta + b * in.beta_stride[0] + h * in.beta_stride[2];
-    const uint8_t* rp = in.reset ? in.reset + b * in.reset_stride[0] : nullptr;
-    const E* d_o = (const E*)a.d_o + b * a.d_o_stride[0] + h * a.d_o_stride[2];
-    E* d_v = (E*)a.dv + b * a.dv_stride[0] + h * a.dv_stride[2] + col;
-    const int64_t bh = b * in.value_heads + h;
+    const int64_t bh = b * ap->in.value_heads + h;
 
     f4 dS[DK / 16], Sn[DK / 16];  // the gradient of the state, and the state, after the chunk
-    if (segment == (int)a.segments - 1) {
-        load_state<DK, FULL>(a.d_last ? a.d_last + bh * dk * dv : nullptr, dk, dv, dv, a.d_last_vec, col0, lane, dS);
-        load_state<DK, FULL>(a.last + bh * dk * dv, dk, dv, dv, a.last_vec, col0, lane, Sn);
+    if (segment == (int)ap->segments - 1) {
+        load_state<DK, FULL>(ap->d_last ? ap->d_last + bh * dk * dv : nullptr, dk, dv, dv, ap->d_last_vec, col0, lane, dS);
+        load_state<DK, FULL>(ap->last + bh * dk * dv, dk, dv, dv, ap->last_vec, col0, lane, Sn);
     } else {
-        load_state<DK, true>(a.d_starts + (bh * (a.segments - 1) + segment) * (DK * G::DV), DK, G::DV, G::DV, true, col0, lane, dS);
-        load_state<DK, true>(a.saved + (bh * (a.chunks - 1) + T / C - 1) * (DK * G::DV), DK, G::DV, G::DV, true, col0, lane, Sn);
+        load_state<DK, true>(ap->d_starts + (bh * (ap->segments - 1) + segment) * (DK * G::DV), DK, G::DV, G::DV, true, col0, lane, dS);
+        load_state<DK, true>(ap->saved + (bh * (ap->chunks - 1) + T / C - 1) * (DK * G::DV), DK, G::DV, G::DV, true, col0, lane, Sn);
     }
 
+    // What a chunk reads from memory.
+    Rows<TY, DK, NW, TILES> kr, qr;
+    Raw<TY> dor;
+    f4 vr[TILES];
+    float gv, bv;
+    bool cut;
+    constexpr int pieces_o = G::DV / 8;
+    static_assert(C * pieces_o <= G::threads, "one piece a thread");
+    const int row_o = threadIdx.x / pieces_o, e_o = 8 * (threadIdx.x % pieces_o);
+    auto fetch = [&](int t, int te) {
+        const ZenoAmdDeltaInputs __attribute__((address_space(4)))& in = ap->in;
+        const E* q = (const E*)in.q + b * in.q_stride[0] + hk * in.q_stride[2];
+        const E* k = (const E*)in.k + b * in.k_stride[0] + hk * in.k_stride[2];
+        const E* v = (const E*)in.v + b * in.v_stride[0] + h * in.v_stride[2] + col;
+        const E* d_o = (const E*)ap->d_o + b * ap->d_o_stride[0] + h * ap->d_o_stride[2];
+        const float* gp = in.g + b * in.g_stride[0] + h * in.g_stride[2];
+        const float* bp = in.beta + b * in.beta_stride[0] + h * in.beta_stride[2];
+        const uint8_t* rp = in.reset ? in.reset + b * in.reset_stride[0] : nullptr;
+        const int rows = te - t;
+        const int64_t tok = t + min(lane, rows - 1);
+        gv = gp[tok * in.g_stride[1]];
+        bv = bp[tok * in.beta_stride[1]];
+        cut = lane < rows && ((rp && rp[tok * in.reset_stride[1]]) || gv < kClears);
+        kr.template fetch<FULL>(k + t * in.k_stride[1], in.k_stride[1], rows, dk, ap->k_vec);
+        qr.template fetch<FULL>(q + t * in.q_stride[1], in.q_stride[1], rows, dk, ap->q_vec);
+        if (C * pieces_o == G::threads || row_o < C) dor.template load<FULL>(d_o + (t + min(row_o, rows - 1)) * ap->d_o_stride[1] + e_o, dv - e_o, ap->d_o_vec);
+#pragma unroll
+        for (int i = 0; i < TILES; ++i) vr[i] = load4<TY, FULL>(v + (t + min(16 * i + row0, rows - 1)) * in.v_stride[1], dv - col, ap->v_vec);
+    };
     for (int te = T; te > begin;) {
-        const Cut cut = chunk_before<C>(te, lane, gp, in.g_stride[1], rp, in.reset_stride[1]);
-        const int t = cut.t;
-        const bool first = cut.first;
+        asm volatile("" : "+s"(ap));
+        // From the grid, and where a reset lies inside, once more from the last one.
+        int t = (te - 1) / C * C;
+        uint64_t cuts;
+        for (;;) {
+            fetch(t, te);
+            cuts = __ballot(cut);
+            if (cuts <= 1) break;
+            t += 63 - __clzll((long long)cuts);
+        }
+        const bool first = cuts != 0;
         const int len = te - t;
         // The state before the chunk: nothing, the caller's, or a saved one.
         const float* sp = nullptr;
         int s_rows = dk, s_cols = dv, s_ld = dv;
-        bool s_vec = a.s_vec;
+        bool s_vec = ap->s_vec;
         if (!first) {
             if (t == 0) {
-                if (in.state) sp = in.state + bh * dk * dv;
+                if (ap->in.state) sp = ap->in.state + bh * dk * dv;
             } else {
-                sp = a.saved + (bh * (a.chunks - 1) + t / C - 1) * (DK * G::DV);
+                sp = ap->saved + (bh * (ap->chunks - 1) + t / C - 1) * (DK * G::DV);
                 s_rows = DK, s_cols = s_ld = G::DV, s_vec = true;
             }
         }
+        f4 S[DK / 16];
+        fetch_state<DK, FULL>(sp, s_rows, s_cols, s_ld, s_vec, col0, lane, S);
 
         __syncthreads();
-        if (wave == 0)
-            load_scalars<TILES>(lane < len ? gp[(t + lane) * in.g_stride[1]] : 0.0f, lane < len ? bp[(t + lane) * in.beta_stride[1]] : 0.0f, lane,
-                                first, lds.s);
-        Rows<TY, DK, NW, TILES> kr, qr;
-        kr.template fetch<FULL>(k + t * in.k_stride[1], in.k_stride[1], len, dk, a.k_vec);
-        qr.template fetch<FULL>(q + t * in.q_stride[1], in.q_stride[1], len, dk, a.q_vec);
-        kr.store(len, in.normalize, lds.K, lds.KT, lds.s.rk);
-        qr.store(len, in.normalize, lds.Q, lds.QT, lds.s.rq);
-#pragma unroll
-        for (int it0 = 0; it0 < C * G::DV / 8; it0 += G::threads) {
-            const int it = it0 + threadIdx.x, row = it / (G::DV / 8), e = 8 * (it % (G::DV / 8));
-            if (C * G::DV / 8 % G::threads && it >= C * G::DV / 8) break;
-            Raw<TY> x;
-            x.template load<FULL>(d_o + (t + min(row, len - 1)) * a.d_o_stride[1] + e, dv - e, a.d_o_vec);
-            x.keep(row < len);
+        if (wave == 0) load_scalars<TILES>(lane < len ? gv : 0.0f, lane < len ? bv : 0.0f, lane, first, lds.s);
+        kr.store(len, ap->in.normalize, lds.K, lds.KT, lds.s.rk);
+        qr.store(len, ap->in.normalize, lds.Q, lds.QT, lds.s.rq);
+        if (C * pieces_o == G::threads || row_o < C) {
+            dor.keep(row_o < len);
             uint32_t w[4][NP];
-            x.parts(w);
+            dor.parts(w);
 #pragma unroll
-            for (int p = 0; p < NP; ++p) *reinterpret_cast<u4*>(lds.DO + (p * C + row) * G::VS + e) = u4{w[0][p], w[1][p], w[2][p], w[3][p]};
+            for (int p = 0; p < NP; ++p) *reinterpret_cast<u4*>(lds.DO + (p * C + row_o) * G::VS + e_o) = u4{w[0][p], w[1][p], w[2][p], w[3][p]};
         }
-        f4 S[DK / 16];
-        load_state<DK, FULL>(sp, s_rows, s_cols, s_ld, s_vec, col0, lane, S);
         f4 vv[TILES];
 #pragma unroll
-        for (int i = 0; i < TILES; ++i)
-            vv[i] = turn(load4<TY, FULL>(v + (t + min(16 * i + row0, len - 1)) * in.v_stride[1], dv - col, a.v_vec), lane);
-#pragma unroll
-        for (int i = 0; i < TILES; ++i)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) vv[i][r] = 16 * i + 4 * g + r < len ? vv[i][r] : 0.0f;
+        for (int i = 0; i < TILES; ++i) vv[i] = turn(16 * i + row0 < len ? vr[i] : f4{0, 0, 0, 0}, lane);
         __syncthreads();
-        fill_inner<TY, DK, NW, TILES, TILES, W_P | W_PT | W_INV | W_INVT>(lds.K, lds.Q, lds.s, in.scale, lds.m);
+        fill_inner<TY, DK, NW, TILES, TILES, W_P | W_PT | W_INV | W_INVT>(lds.K, lds.Q, lds.s, ap->in.scale, lds.m);
 
         // ---- phase A: this wave's columns
+        asm volatile("" : "+s"(ap));
+#pragma unroll
+        for (int i = 0; i < DK / 16; ++i) S[i] = turn(S[i], lane);
         f4 ks[TILES], o4[TILES], du[TILES], d4[TILES];
 #pragma unroll
         for (int i = 0; i < TILES; ++i) {
             ks[i] = o4[i] = du[i] = f4{0, 0, 0, 0};
             f4 x = {0, 0, 0, 0};
 #pragma unroll
-            for (int p = NP - 1; p >= 0; --p) x += load4<T_BF16>(lds.DO + (p * C + 16 * i + row0) * G::VS + col, 4, true);
+            for (int p = NP - 1; p >= 0; --p) x += load4<T_BF16, true>(lds.DO + (p * C + 16 * i + row0) * G::VS + col, 4, true);
             d4[i] = turn(x, lane);
         }
 #pragma unroll
@@ -829,16 +850,14 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || sizeof(BackwardLds<TY, DK, NW, 
         for (int i = 0; i < TILES; ++i) {
             const f4 gam = row4(lds.s.gam, i, g), rk = row4(lds.s.rk, i, g);
             x[i] = vv[i] - gam * rk * ks[i];
-            o4[i] *= gam * row4(lds.s.rq, i, g) * in.scale;
+            o4[i] *= gam * row4(lds.s.rq, i, g) * ap->in.scale;
             du[i] *= row4(lds.s.end, i, g) * rk;
         }
         // <dS', S'>, the decay's gradient from all that passes the chunk's end.
-        float edge = 0.0f;
+        f4 edge4 = {0, 0, 0, 0};
 #pragma unroll
-        for (int i = 0; i < DK / 16; ++i)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) edge += dS[i][r] * Sn[i][r];
-        edge = sum64(edge);
+        for (int i = 0; i < DK / 16; ++i) edge4 += dS[i] * Sn[i];
+        const float edge = sum64(edge4[0] + edge4[1] + edge4[2] + edge4[3]);
         if (lane == 0) lds.edge[wave] = edge;
         __syncthreads();
         Half<3> up[TILES];
@@ -848,27 +867,47 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || sizeof(BackwardLds<TY, DK, NW, 
         f4 dr[TILES], dx[TILES];
         solve_back<TY, TILES>(lds.m, lds.s, n, g, d4, du, dr, dx);
 #pragma unroll
-        for (int i = 0; i < TILES; ++i)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int row = 16 * i + 4 * g + r;
-                const float de = sum16(d4[i][r] * o4[i][r] - dx[i][r] * vv[i][r]), be = sum16(dr[i][r] * x[i][r]);
-                if (n == 0) {
-                    lds.decay[wave][row] = de;
-                    lds.beta[wave][row] = be;
-                }
-            }
-#pragma unroll
         for (int i = 0; i < TILES; ++i) {
+            f4 de = d4[i] * o4[i] - dx[i] * vv[i], be = dr[i] * x[i];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) de[r] = sum16(de[r]), be[r] = sum16(be[r]);
+            if (n == 0) {
+                *reinterpret_cast<f4*>(lds.decay[wave] + 16 * i + 4 * g) = de;
+                *reinterpret_cast<f4*>(lds.beta[wave] + 16 * i + 4 * g) = be;
+            }
             const int at = (16 * i + row0) * G::VS + col;
             const f4 y = turn(dx[i], lane);
             put4<NO>(lds.c.U + at, C * G::VS, turn(u[i], lane));
             put4<NO>(lds.c.X + at, C * G::VS, y);
-            if (16 * i + row0 < len) store4<TY, FULL>(d_v + (t + 16 * i + row0) * a.dv_stride[1], dv - col, a.dv_vec, y);
+            if (16 * i + row0 < len) store4<TY, FULL>((E*)ap->dv + b * ap->dv_stride[0] + h * ap->dv_stride[2] + col + (t + 16 * i + row0) * ap->dv_stride[1], dv - col, ap->dv_vec, y);
         }
         __syncthreads();
 
         // ---- phase B: gradients of q and k
+        asm volatile("" : "+s"(ap));
+        constexpr int blocks = L::slab / 16, slabs = DK / L::slab;
+        constexpr bool spread = NW >= 2 * blocks && TILES == 2;  // one tile a wave
+        constexpr int rounds = spread ? 1 : (blocks + NW - 1) / NW, per = spread ? 1 : TILES;
+        static_assert(rounds == 1, "one block of the slab a wave");
+        const int blk = spread ? wave % blocks : wave, tile0 = spread ? wave / blocks : 0;
+        const bool busy = blk < blocks && tile0 < TILES;
+        // S transposed as a right operand: this lane's row of the key dimension, from memory. Rows and
+        // columns outside the head are zero.
+        f4 st[G::DV / 32][2];
+        auto fetch_rows = [&](int sl) {
+            const int row = sl * L::slab + 16 * blk + n;
+            const bool ok = busy && sp && row < s_rows;
+#pragma unroll
+            for (int c = 0; c < G::DV / 32; ++c) {
+                const int e = 32 * c + 8 * g;
+                st[c][0] = st[c][1] = zero;
+                if (ok) {
+                    st[c][0] = load4<T_F32, FULL>(sp + row * s_ld + e, s_cols - e, s_vec);
+                    st[c][1] = load4<T_F32, FULL>(sp + row * s_ld + e + 4, s_cols - e - 4, s_vec);
+                }
+            }
+        };
+        fetch_rows(0);
         if (wave == NW - 1) {
             double sum = 0.0;
             float bsum = 0.0f;
@@ -887,52 +926,52 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || sizeof(BackwardLds<TY, DK, NW, 
                 if (lane + d < C) sum += dn;
             }
             if (lane < len) {
-                a.dg[b * a.dg_stride[0] + (t + lane) * a.dg_stride[1] + h * a.dg_stride[2]] = first && lane == 0 ? 0.0f : (float)sum;
-                a.dbeta[b * a.dbeta_stride[0] + (t + lane) * a.dbeta_stride[1] + h * a.dbeta_stride[2]] = bsum;
+                ap->dg[b * ap->dg_stride[0] + (t + lane) * ap->dg_stride[1] + h * ap->dg_stride[2]] = first && lane == 0 ? 0.0f : (float)sum;
+                ap->dbeta[b * ap->dbeta_stride[0] + (t + lane) * ap->dbeta_stride[1] + h * ap->dbeta_stride[2]] = bsum;
             }
         }
+        // W and Y + Y^T (times the norms of the rows that they multiply), a tile a wave.
         constexpr int pairs = TILES * (TILES + 1) / 2;
-        for (int job = wave; job < 2 * pairs; job += NW) {
+#pragma unroll
+        for (int job = 0; job < 2 * pairs; ++job) {
             const int pair = job % pairs, ti = pair > 0 ? 1 : 0, tj = pair > 1 ? 1 : 0, j = 16 * tj + n;
-            f4 acc = zero;
+            if (wave != (NW >= 2 * pairs ? job : pair)) continue;
+            f4 acc = zero, mirror = zero;
 #pragma unroll
             for (int c = 0; c < G::DV / 32; ++c) {
                 const int ai = (16 * ti + n) * G::VS + 32 * c + 8 * g, aj = (16 * tj + n) * G::VS + 32 * c + 8 * g;
                 const Frag<NO> uf = frag_at<NO>(lds.c.U + aj, C * G::VS);
-                if (job < pairs) acc = mul<SO>(frag_at<NP>(lds.DO + ai, C * G::VS), uf, acc);
-                else acc = mul<SO>(frag_at<NO>(lds.c.X + ai, C * G::VS), uf, acc);
+                if (job < pairs) {
+                    acc = mul<SO>(frag_at<NP>(lds.DO + ai, C * G::VS), uf, acc);
+                } else {
+                    const Frag<NO> xf = frag_at<NO>(lds.c.X + ai, C * G::VS);
+                    acc = mul<SO>(xf, uf, acc);
+                    if (ti == tj) mirror = mul<SO>(uf, xf, mirror);  // the tile's transpose
+                }
             }
             const float hj = lds.s.hi[j], lj = lds.s.lo[j], rj = lds.s.rk[j];
+            const f4 hi = row4(lds.s.hi, ti, g), lo = row4(lds.s.lo, ti, g), nr = row4(job < pairs ? lds.s.rq : lds.s.rk, ti, g);
             f4 by_col, by_row;  // times the norm of the column's token, and of the row's
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int i = 16 * ti + 4 * g + r;
-                const float w = acc[r] * __expf((lds.s.hi[i] - hj) + (lds.s.lo[i] - lj));
-                const float y = job < pairs ? (j <= i ? w * in.scale : 0.0f) : (j < i ? -w : 0.0f);
+                const float d = (hi[r] - hj) + (lo[r] - lj);
+                float y;
+                if (job < pairs) y = j <= i ? acc[r] * __expf(d) * ap->in.scale : 0.0f;
+                else if (ti != tj) y = -acc[r] * __expf(d);
+                else y = j == i ? 0.0f : -(j < i ? acc[r] : mirror[r]) * __expf(j < i ? d : -d);
                 by_col[r] = y * rj;
-                by_row[r] = y * (job < pairs ? lds.s.rq[i] : lds.s.rk[i]);
+                by_row[r] = y * nr[r];
             }
-            if (job < pairs) {
-                put_rows<NO, TILES>(lds.b.W, by_col, ti, tj, lane);
-                put_cols<NO, TILES>(lds.b.WT, by_row, ti, tj, lane);
-            } else if (ti != tj) {
-                put_rows<NO, TILES>(lds.b.Y, by_col, ti, tj, lane);
-                put_cols<NO, TILES>(lds.b.Y, by_row, ti, tj, lane);
-            } else {
-                // A diagonal tile of Y + Y^T: the mirrored values come through LDS.
-                put_rows<NO, TILES>(lds.b.Y, by_col, ti, tj, lane);
-                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-                __builtin_amdgcn_wave_barrier();
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (j < 16 * ti + 4 * g + r)
-                        put_parts<NO>(lds.b.Y + j * G::TS + Tok<TILES>::slot_of(16 * ti + 4 * g + r), C * G::TS, by_row[r]);
+            put_rows<NO, TILES>(job < pairs ? lds.b.W : lds.b.Y, by_col, ti, tj, lane);
+            if (job < pairs) put_cols<NO, TILES>(lds.b.WT, by_row, ti, tj, lane);
+            if (job < pairs && ti != tj) {  // above the diagonal
+                put_rows<NO, TILES>(lds.b.W, zero, tj, ti, lane);
+                put_rows<NO, TILES>(lds.b.WT, zero, ti, tj, lane);
             }
+            else if (ti != tj) put_cols<NO, TILES>(lds.b.Y, by_row, ti, tj, lane);
         }
-        constexpr int blocks = L::slab / 16, slabs = DK / L::slab;
-        constexpr bool spread = NW >= 2 * blocks && TILES == 2;  // one tile a wave
-        constexpr int rounds = spread ? 1 : (blocks + NW - 1) / NW, per = spread ? 1 : TILES;
-        f4 dq[slabs * rounds * per], dkk[slabs * rounds * per];
+        f4 dq[slabs * per], dkk[slabs * per];
 #pragma unroll
         for (int sl = 0; sl < slabs; ++sl) {
             if (sl) __syncthreads();
@@ -941,128 +980,112 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || sizeof(BackwardLds<TY, DK, NW, 
 #pragma unroll
                 for (int r = 0; r < 4; ++r) lds.b.dS[(16 * i + 4 * g + r) * L::SS + col0 + n] = dS[sl * (L::slab / 16) + i][r];
             __syncthreads();
+            // Waves without a block multiply what they hold and drop it: no branch around matrix instructions.
+            const int row = sl * L::slab + 16 * (blk % blocks) + n;  // of the key dimension: this lane's column of the results
+            const int t1 = tile0 % TILES;
+            f4 aq[per], ar[per], ac[per];
 #pragma unroll
-            for (int rd = 0; rd < rounds; ++rd) {
-                const int blk = spread ? wave % blocks : wave + rd * NW;
-                const int tile0 = spread ? wave / blocks : 0;
-                if (blk < blocks && tile0 < TILES) {
-                    const int row = sl * L::slab + 16 * blk + n;  // of the key dimension: this lane's column of the results
-                    f4 aq[per], ar[per], ac[per];
+            for (int i = 0; i < per; ++i) aq[i] = ar[i] = ac[i] = zero;
 #pragma unroll
-                    for (int i = 0; i < per; ++i) aq[i] = ar[i] = ac[i] = zero;
+            for (int c = 0; c < G::DV / 32; ++c) {
+                const int e = 32 * c + 8 * g;
+                const Frag<NO> sf = split<NO>(st[c][0], st[c][1]);
+                const float* ds = lds.b.dS + (16 * (blk % blocks) + n) * L::SS + e;
+                const Frag<NO> df = split<NO>(*reinterpret_cast<const f4*>(ds), *reinterpret_cast<const f4*>(ds + 4));
 #pragma unroll
-                    for (int c = 0; c < G::DV / 32; ++c) {
-                        const int e = 32 * c + 8 * g;
-                        f4 s0 = zero, s1 = zero;
-                        if (sp && row < s_rows) state8(sp + row * s_ld + e, s_cols - e, s_vec, s0, s1);
-                        const Frag<NO> sf = split<NO>(s0, s1);
-                        const float* ds = lds.b.dS + (16 * blk + n) * L::SS + e;
-                        const Frag<NO> df = split<NO>(*reinterpret_cast<const f4*>(ds), *reinterpret_cast<const f4*>(ds + 4));
-#pragma unroll
-                        for (int i = 0; i < per; ++i) {
-                            const int at = (16 * (tile0 + i) + n) * G::VS + e;
-                            if (sp) {
-                                aq[i] = mul<SO>(frag_at<NP>(lds.DO + at, C * G::VS), sf, aq[i]);
-                                ar[i] = mul<SO>(frag_at<NO>(lds.c.X + at, C * G::VS), sf, ar[i]);
-                            }
-                            ac[i] = mul<SO>(frag_at<NO>(lds.c.U + at, C * G::VS), df, ac[i]);
-                        }
-                    }
-                    const auto kt = Tok<TILES>::template at<NP>(lds.KT + row * G::TS, g, DK * G::TS);
-                    const auto qt = Tok<TILES>::template at<NP>(lds.QT + row * G::TS, g, DK * G::TS);
-#pragma unroll
-                    for (int i = 0; i < per; ++i) {
-                        const int ti = tile0 + i, at = (16 * ti + n) * G::TS, to = (sl * rounds + rd) * per + i;
-                        const f4 gam = row4(lds.s.gam, ti, g);
-                        f4 yq = aq[i] * gam * in.scale, yk = ac[i] * row4(lds.s.end, ti, g) - ar[i] * gam;
-                        yk = mul<SO>(Tok<TILES>::template at<NO>(lds.b.Y + at, g, C * G::TS), kt, yk);
-                        if (TILES == 2 && ti == 0) {  // the upper right tile of W is not written
-                            yq = mul<SO>(half_at<NO>(lds.b.W + at + Tok<TILES>::tile_at(g, 0), C * G::TS),
-                                         half_at<NP>(lds.KT + row * G::TS + Tok<TILES>::tile_at(g, 0), DK * G::TS), yq);
-                            yk = mul<SO>(Tok<TILES>::template at<NO>(lds.b.WT + at, g, C * G::TS), qt, yk);
-                        } else if (TILES == 2) {
-                            yq = mul<SO>(Tok<TILES>::template at<NO>(lds.b.W + at, g, C * G::TS), kt, yq);
-                            yk = mul<SO>(half_at<NO>(lds.b.WT + at + Tok<TILES>::tile_at(g, 1), C * G::TS),
-                                         half_at<NP>(lds.QT + row * G::TS + Tok<TILES>::tile_at(g, 1), DK * G::TS), yk);
-                        } else {
-                            yq = mul<SO>(Tok<TILES>::template at<NO>(lds.b.W + at, g, C * G::TS), kt, yq);
-                            yk = mul<SO>(Tok<TILES>::template at<NO>(lds.b.WT + at, g, C * G::TS), qt, yk);
-                        }
-                        dq[to] = yq;
-                        dkk[to] = yk;
-                    }
+                for (int i = 0; i < per; ++i) {
+                    const int at = (16 * (t1 + i) + n) * G::VS + e;
+                    aq[i] = mul<SO>(frag_at<NP>(lds.DO + at, C * G::VS), sf, aq[i]);
+                    ar[i] = mul<SO>(frag_at<NO>(lds.c.X + at, C * G::VS), sf, ar[i]);
+                    ac[i] = mul<SO>(frag_at<NO>(lds.c.U + at, C * G::VS), df, ac[i]);
                 }
+            }
+            if (sl + 1 < slabs) fetch_rows(sl + 1);
+            const auto kt = Tok<TILES>::template at<NP>(lds.KT + row * G::TS, g, DK * G::TS);
+            const auto qt = Tok<TILES>::template at<NP>(lds.QT + row * G::TS, g, DK * G::TS);
+#pragma unroll
+            for (int i = 0; i < per; ++i) {
+                const int ti = t1 + i, at = (16 * ti + n) * G::TS;
+                const f4 gam = row4(lds.s.gam, ti, g);
+                f4 yq = aq[i] * gam * ap->in.scale, yk = ac[i] * row4(lds.s.end, ti, g) - ar[i] * gam;
+                yk = mul<SO>(Tok<TILES>::template at<NO>(lds.b.Y + at, g, C * G::TS), kt, yk);
+                yq = mul<SO>(Tok<TILES>::template at<NO>(lds.b.W + at, g, C * G::TS), kt, yq);
+                yk = mul<SO>(Tok<TILES>::template at<NO>(lds.b.WT + at, g, C * G::TS), qt, yk);
+                dq[sl * per + i] = yq;
+                dkk[sl * per + i] = yk;
             }
         }
         // the state's gradient, from this wave's columns
-        pull_state<TY, DK, TILES>(lds.KT, lds.QT, lds.s, in.scale, n, g, d4, dx, dS);
+        pull_state<TY, DK, TILES>(lds.KT, lds.QT, lds.s, ap->in.scale, n, g, d4, dx, dS);
 #pragma unroll
         for (int i = 0; i < DK / 16; ++i) {
-            if (first) dS[i] = zero;
+            dS[i] = first ? zero : dS[i];
             Sn[i] = S[i];
         }
         __syncthreads();  // U and dX are read
+        if (busy)
 #pragma unroll
-        for (int sl = 0; sl < slabs; ++sl)
+            for (int sl = 0; sl < slabs; ++sl)
 #pragma unroll
-            for (int rd = 0; rd < rounds; ++rd) {
-                const int blk = spread ? wave % blocks : wave + rd * NW;
-                const int tile0 = spread ? wave / blocks : 0;
-                if (blk < blocks && tile0 < TILES)
+                for (int i = 0; i < per; ++i)
 #pragma unroll
-                    for (int i = 0; i < per; ++i)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            const int at = (16 * (tile0 + i) + 4 * g + r) * L::OS + sl * L::slab + 16 * blk + n, from = (sl * rounds + rd) * per + i;
-                            lds.out.q[at] = dq[from][r];
-                            lds.out.k[at] = dkk[from][r];
-                        }
-            }
+                    for (int r = 0; r < 4; ++r) {
+                        const int at = (16 * (tile0 + i) + 4 * g + r) * L::OS + sl * L::slab + 16 * blk + n;
+                        lds.out.q[at] = dq[sl * per + i][r];
+                        lds.out.k[at] = dkk[sl * per + i][r];
+                    }
         __syncthreads();
+        asm volatile("" : "+s"(ap));
         // rows out, through the norms: d(x / |x|) = (d - x^ (x^ . d)) / |x|, |x|^2 with its eps; of
         // one dimension alone that is d eps / |x|^3, which the difference would lose to rounding
         constexpr int pieces = DK / 8;
-        for (int it = threadIdx.x; it < C * pieces; it += G::threads) {
-            const int row = it / pieces, e = 8 * (it % pieces);
+        const int row = threadIdx.x / pieces, e = 8 * (threadIdx.x % pieces);
+        if (C * pieces == G::threads || row < C) {
 #pragma unroll
             for (int w = 0; w < 2; ++w) {
                 const float* from = (w ? lds.out.k : lds.out.q) + row * L::OS + e;
-                const f4 x0 = *reinterpret_cast<const f4*>(from), x1 = *reinterpret_cast<const f4*>(from + 4);
-                float y[8] = {x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]};
-                if (in.normalize) {
+                f4 y0 = *reinterpret_cast<const f4*>(from), y1 = *reinterpret_cast<const f4*>(from + 4);
+                if (ap->in.normalize) {
                     const float nr = w ? lds.s.rk[row] : lds.s.rq[row];
                     const uint16_t* src = (w ? lds.K : lds.Q) + row * G::KS;
-                    float xs[8], dot = 0.0f;
+                    f4 x0 = zero, x1 = zero;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        float z = 0.0f;
-#pragma unroll
-                        for (int p = NP - 1; p >= 0; --p) z += __uint_as_float((uint32_t)src[p * C * G::KS + slot(e + j)] << 16);
-                        xs[j] = z * nr;
-                        dot += xs[j] * y[j];
+                    for (int p = NP - 1; p >= 0; --p) {
+                        x0 += load4<T_BF16, true>(src + p * C * G::KS + slot(e), 4, true);
+                        x1 += load4<T_BF16, true>(src + p * C * G::KS + slot(e + 4), 4, true);
                     }
-#pragma unroll
-                    for (int d = 1; d < pieces; d <<= 1) dot += __shfl_xor(dot, d);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) y[j] = dk == 1 ? y[j] * kNormEps * nr * nr * nr : nr * (y[j] - xs[j] * dot);
+                    x0 *= nr;
+                    x1 *= nr;
+                    const f4 d = x0 * y0 + x1 * y1;
+                    float dot = d[0] + d[1] + d[2] + d[3];
+                    if (pieces > 8) dot += dpp<0x128>(dot);
+                    dot += dpp<0x141>(dot);
+                    dot += dpp<0x1b>(dot);
+                    dot += dpp<0xb1>(dot);
+                    if (dk == 1) {
+                        y0 *= kNormEps * nr * nr * nr;
+                    } else {
+                        y0 = (y0 - x0 * dot) * nr;
+                        y1 = (y1 - x1 * dot) * nr;
+                    }
                 }
                 if (row < len) {
-                    if (a.part_q) {
-                        float* to = (w ? a.part_k : a.part_q) + ((b * T + t + row) * in.value_heads + h) * dk + e;
-                        store8<T_F32>(to, dk - e, dk % 8 == 0, y);
+                    const float y[8] = {y0[0], y0[1], y0[2], y0[3], y1[0], y1[1], y1[2], y1[3]};
+                    if (ap->part_q) {
+                        float* to = (w ? ap->part_k : ap->part_q) + ((b * ap->in.length + t + row) * ap->in.value_heads + h) * dk + e;
+                        store8<T_F32, FULL>(to, dk - e, dk % 8 == 0, y);
                     } else if (w) {
-                        store8<TY>((E*)a.dk + b * a.dk_stride[0] + (t + row) * a.dk_stride[1] + hk * a.dk_stride[2] + e, dk - e, a.dk_vec, y);
+                        store8<TY, FULL>((E*)ap->dk + b * ap->dk_stride[0] + (t + row) * ap->dk_stride[1] + hk * ap->dk_stride[2] + e, dk - e, ap->dk_vec, y);
                     } else {
-                        store8<TY>((E*)a.dq + b * a.dq_stride[0] + (t + row) * a.dq_stride[1] + hk * a.dq_stride[2] + e, dk - e, a.dq_vec, y);
+                        store8<TY, FULL>((E*)ap->dq + b * ap->dq_stride[0] + (t + row) * ap->dq_stride[1] + hk * ap->dq_stride[2] + e, dk - e, ap->dq_vec, y);
                     }
                 }
             }
         }
         te = t;
     }
-    if (a.d_state && segment == 0) store_state<DK, FULL>(a.d_state + bh * dk * dv, dk, dv, dv, a.d_state_vec, col0, lane, dS);
+    if (ap->d_state && segment == 0) store_state<DK, FULL>(ap->d_state + bh * dk * dv, dk, dv, dv, ap->d_state_vec, col0, lane, dS);
 }
-
 // Sums the value heads of each key head, in their order; one thread a value.
 template <int TY> __global__ __launch_bounds__(256) void delta_share_kernel(const Args a) {
     typedef typename Elem<TY>::type E;
@@ -1186,7 +1209,7 @@ template <int TY, int DK, int NW, int TILES, bool FULL> void forward_shape(const
     const uint32_t heads = a.in.batch * a.in.value_heads;
     if (a.segments > 1) {
         delta_forward_kernel<TY, DK, NW, TILES, FULL, true><<<dim3(heads, a.segments - 1, 2), 64 * NW, 0, stream>>>(a);
-        if (a.segments > 2) delta_join_kernel<DK, NW, false><<<heads, 64 * NW, 0, stream>>>(a.starts, a.jumps, a.segments);
+        if (a.segments > 2) delta_join_kernel<DK, false><<<dim3(heads, NW), 256, 0, stream>>>(a.starts, a.jumps, a.segments, 16 * NW);
     }
     delta_forward_kernel<TY, DK, NW, TILES, FULL, false><<<dim3(heads, a.segments), 64 * NW, 0, stream>>>(a);
 }
@@ -1194,7 +1217,7 @@ template <int TY, int DK, int NW, int TILES, bool FULL> void backward_shape(cons
     const uint32_t heads = a.in.batch * a.in.value_heads;
     if (a.segments > 1) {
         delta_pull_kernel<TY, DK, NW, TILES, FULL><<<dim3(heads, a.segments - 1), 64 * NW, 0, stream>>>(a);
-        if (a.segments > 2) delta_join_kernel<DK, NW, true><<<heads, 64 * NW, 0, stream>>>(a.d_starts, a.jumps, a.segments);
+        if (a.segments > 2) delta_join_kernel<DK, true><<<dim3(heads, NW), 256, 0, stream>>>(a.d_starts, a.jumps, a.segments, 16 * NW);
     }
     delta_backward_kernel<TY, DK, NW, TILES, FULL><<<dim3(heads, a.segments), 64 * NW, 0, stream>>>(a);
 }

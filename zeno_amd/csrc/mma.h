@@ -192,31 +192,9 @@ template <int TY> struct Raw {
     }
 };
 
-// Eight consecutive elements, the first `n` of them in bounds (the rest are zero). `vec`: the
-// address is a multiple of 16 bytes whenever n is 8.
-template <int TY> __device__ __forceinline__ void load8(const typename Elem<TY>::type* at, int n, bool vec, float* x) {
-    typedef typename Elem<TY>::type E;
-    if (vec && n >= 8) {
-        if constexpr (TY == T_F32) {
-            const f4 a = reinterpret_cast<const f4*>(at)[0], b = reinterpret_cast<const f4*>(at)[1];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) { x[j] = a[j]; x[4 + j] = b[j]; }
-        } else {
-            const u4 a = *reinterpret_cast<const u4*>(at);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const E e[2] = {__builtin_bit_cast(E, (uint16_t)(a[j] & 0xffffu)), __builtin_bit_cast(E, (uint16_t)(a[j] >> 16))};
-                x[2 * j] = Elem<TY>::get(e[0]);
-                x[2 * j + 1] = Elem<TY>::get(e[1]);
-            }
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = j < n ? Elem<TY>::get(at[j]) : 0.0f;
-    }
-}
-template <int TY> __device__ __forceinline__ void store8(typename Elem<TY>::type* at, int n, bool vec, const float* x) {
-    if (vec && n >= 8) {
+// The same, out.
+template <int TY, bool FULL = false> __device__ __forceinline__ void store8(typename Elem<TY>::type* at, int n, bool vec, const float* x) {
+    if (FULL || (vec && n >= 8)) {
         if constexpr (TY == T_F32) {
             reinterpret_cast<f4*>(at)[0] = f4{x[0], x[1], x[2], x[3]};
             reinterpret_cast<f4*>(at)[1] = f4{x[4], x[5], x[6], x[7]};
