@@ -297,27 +297,29 @@ __device__ __forceinline__ void add_PU(const M& m, int n, int g, const Half<3>* 
     if constexpr (USED == 2) acc[1] = mul<2>(frag_at<3>(m.P + (16 + n) * TS + 8 * g, part), join<3>(up[0], up[1]), acc[1]);
 }
 
-// This wave's columns of a state [rows, cols] in memory (leading dimension ld; null: zeros). A lane
-// reads four columns of a row; four lanes exchange them (turn) to make result tiles of it.
-template <int DK, bool FULL> __device__ __forceinline__ void fetch_state(const float* at, int rows, int cols, int ld, bool vec, int col0, int lane, f4* S) {
-    const int row = 4 * (lane >> 4) + (lane & 3), col = col0 + (lane & 12);
-    const float* from = at + row * ld + col;
+// This wave's columns of a state [rows, cols] in memory (leading dimension ld; null: zeros) as
+// result tiles, one value an access: 64 bytes of four rows at a time, and no exchange between lanes.
+// FULL: [DK, LD].
+template <int DK, int LD, bool FULL> __device__ __forceinline__ void load_state(const float* at, int rows, int cols, int ld, int col0, int lane, f4* S) {
+    const int row = 4 * (lane >> 4), col = col0 + (lane & 15), stride = FULL ? LD : ld;
+    const float* from = at + row * stride + col;
 #pragma unroll
-    for (int i = 0; i < DK / 16; ++i) {
-        S[i] = f4{0, 0, 0, 0};
-        if (at) S[i] = load4<T_F32, FULL>(from + 16 * i * ld, 16 * i + row < rows ? cols - col : 0, vec);
-    }
+    for (int i = 0; i < DK / 16; ++i) S[i] = f4{0, 0, 0, 0};
+    if (at)
+#pragma unroll
+        for (int i = 0; i < DK / 16; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (FULL || (16 * i + r + row < rows && col < cols)) S[i][r] = from[(16 * i + r) * stride];
 }
-template <int DK, bool FULL> __device__ __forceinline__ void load_state(const float* at, int rows, int cols, int ld, bool vec, int col0, int lane, f4* S) {
-    fetch_state<DK, FULL>(at, rows, cols, ld, vec, col0, lane, S);
+template <int DK, int LD, bool FULL> __device__ __forceinline__ void store_state(float* at, int rows, int cols, int ld, int col0, int lane, const f4* S) {
+    const int row = 4 * (lane >> 4), col = col0 + (lane & 15), stride = FULL ? LD : ld;
+    float* to = at + row * stride + col;
 #pragma unroll
-    for (int i = 0; i < DK / 16; ++i) S[i] = turn(S[i], lane);
-}
-template <int DK, bool FULL> __device__ __forceinline__ void store_state(float* at, int rows, int cols, int ld, bool vec, int col0, int lane, const f4* S) {
-    const int row = 4 * (lane >> 4) + (lane & 3), col = col0 + (lane & 12);
-    float* to = at + row * ld + col;
+    for (int i = 0; i < DK / 16; ++i)
 #pragma unroll
-    for (int i = 0; i < DK / 16; ++i) store4<T_F32, FULL>(to + 16 * i * ld, 16 * i + row < rows ? cols - col : 0, vec, turn(S[i], lane));
+        for (int r = 0; r < 4; ++r)
+            if (FULL || (16 * i + r + row < rows && col < cols)) to[(16 * i + r) * stride] = S[i][r];
 }
 
 // The matrices over segments are kept in the parts and the order in which a lane holds them as
@@ -380,14 +382,14 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && sizeof(ForwardLds<TY, DK, NW, T
 
     f4 S[DK / 16];
     if (segment == 0) {
-        load_state<DK, FULL>(in.state ? in.state + bh * dk * dv : nullptr, dk, dv, dv, a.s_vec, col0, lane, S);
+        load_state<DK, G::DV, FULL>(in.state ? in.state + bh * dk * dv : nullptr, dk, dv, dv, col0, lane, S);
     } else if (STATES) {
 #pragma unroll
         for (int i = 0; i < DK / 16; ++i)
 #pragma unroll
             for (int r = 0; r < 4; ++r) S[i][r] = unit && 16 * i + 4 * g + r == col0 + n ? 1.0f : 0.0f;
     } else {
-        load_state<DK, true>(a.starts + (bh * (a.segments - 1) + segment - 1) * (DK * G::DV), DK, G::DV, G::DV, true, col0, lane, S);
+        load_state<DK, G::DV, true>(a.starts + (bh * (a.segments - 1) + segment - 1) * (DK * G::DV), DK, G::DV, G::DV, col0, lane, S);
     }
 
     // What a chunk reads from memory, fetched one chunk ahead: up to the grid, as where the chunk
@@ -470,7 +472,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && sizeof(ForwardLds<TY, DK, NW, T
 #pragma unroll
         for (int i = 0; i < TILES; ++i) x[i] = turn(16 * i + row0 < len ? vr[i] : f4{0, 0, 0, 0}, lane);
         if (!STATES && a.saved && t && t % G::C == 0)
-            store_state<DK, true>(a.saved + (bh * (a.chunks - 1) + t / G::C - 1) * (DK * G::DV), DK, G::DV, G::DV, true, col0, lane, S);
+            store_state<DK, G::DV, true>(a.saved + (bh * (a.chunks - 1) + t / G::C - 1) * (DK * G::DV), DK, G::DV, G::DV, col0, lane, S);
         if (first) {
             any_cut = true;
 #pragma unroll
@@ -478,7 +480,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && sizeof(ForwardLds<TY, DK, NW, T
         }
 
         __syncthreads();  // the last chunk's operands are read
-        if (wave == 0) load_scalars<TILES>(lane < len ? gv : 0.0f, lane < len ? bv : 0.0f, lane, first, lds.s);
+        if (wave == NW - 1) load_scalars<TILES>(lane < len ? gv : 0.0f, lane < len ? bv : 0.0f, lane, first, lds.s);
         kr.store(len, in.normalize, lds.K, lds.KT, lds.s.rk);
         if (!STATES) qr.store(len, in.normalize, lds.Q, nullptr, lds.s.rq);
         if (t + len < T) fetch(t + len);
@@ -493,10 +495,10 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && sizeof(ForwardLds<TY, DK, NW, T
             if (col0 < DK) store_jump<DK>(reinterpret_cast<uint16_t*>(to), wave, lane, S);
             if (threadIdx.x == 0) to[Jump<DK>::size] = any_cut ? 0.0f : 1.0f;
         } else {
-            store_state<DK, true>(a.starts + (bh * (a.segments - 1) + segment) * (DK * G::DV), DK, G::DV, G::DV, true, col0, lane, S);
+            store_state<DK, G::DV, true>(a.starts + (bh * (a.segments - 1) + segment) * (DK * G::DV), DK, G::DV, G::DV, col0, lane, S);
         }
     } else if (segment == (int)a.segments - 1)
-        store_state<DK, FULL>(a.last + bh * dk * dv, dk, dv, dv, a.last_vec, col0, lane, S);
+        store_state<DK, G::DV, FULL>(a.last + bh * dk * dv, dk, dv, dv, col0, lane, S);
 }
 
 // ---- joining segments ------------------------------------------------------------------------
@@ -505,8 +507,8 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && sizeof(ForwardLds<TY, DK, NW, T
 // A workgroup joins 16 value columns of a head. Its four waves share the rows of the result; each
 // step's state reaches them as a right operand through LDS, the matrices come from memory a step
 // ahead. One step is DK / 64 x DK / 32 x 6 dependent-free matrix instructions a wave.
-template <int DK, bool BACK>
-__global__ __launch_bounds__(256) void delta_join_kernel(float* states, const float* jumps, int segments, int DV) {
+template <int DK, int DV, bool BACK>
+__global__ __launch_bounds__(256) void delta_join_kernel(float* states, const float* jumps, int segments) {
     typedef Jump<DK> J;
     constexpr int TR = DK / 64;  // row tiles a wave
     __shared__ __attribute__((aligned(16))) uint16_t lds[2][J::steps * 3 * J::part];
@@ -526,11 +528,11 @@ __global__ __launch_bounds__(256) void delta_join_kernel(float* states, const fl
         for (int i = 0; i < TR; ++i)
 #pragma unroll
             for (int c = 0; c < J::steps; ++c) m[i][c] = frag_at<3>(f + i * J::row + c * 3 * J::part, J::part);
-        load_state<16 * TR, true>(at + (int64_t)to * (DK * DV), 16 * TR, DV, DV, true, col0, lane, N);
+        load_state<16 * TR, DV, true>(at + (int64_t)to * (DK * DV), 16 * TR, DV, DV, col0, lane, N);
         passes = from[J::size];
     };
     f4 S[TR];
-    load_state<16 * TR, true>(at + (int64_t)first * (DK * DV), 16 * TR, DV, DV, true, col0, lane, S);
+    load_state<16 * TR, DV, true>(at + (int64_t)first * (DK * DV), 16 * TR, DV, DV, col0, lane, S);
     // Forward: from state p to p + 1 by jump p + 1. Back: from state p to p - 1 by jump p.
     fetch(BACK ? first : first + 1, first + step);
     for (int p = first; p != last; p += step) {
@@ -553,7 +555,7 @@ __global__ __launch_bounds__(256) void delta_join_kernel(float* states, const fl
         }
         const int to = p + step;
         if (to != last) fetch(BACK ? to : to + 1, to + step);
-        store_state<16 * TR, true>(at + (int64_t)to * (DK * DV), 16 * TR, DV, DV, true, col0, lane, S);
+        store_state<16 * TR, DV, true>(at + (int64_t)to * (DK * DV), 16 * TR, DV, DV, col0, lane, S);
     }
 }
 
@@ -675,7 +677,7 @@ __global__ __launch_bounds__(64 * NW) void delta_pull_kernel(const Args a) {
     const E* d_o = (const E*)a.d_o + b * a.d_o_stride[0] + h * a.d_o_stride[2] + col;
     const int64_t bh = b * in.value_heads + h;
     f4 dS[DK / 16];
-    load_state<DK, FULL>(a.d_last && segment == (int)a.segments - 1 ? a.d_last + bh * dk * dv : nullptr, dk, dv, dv, a.d_last_vec, col0, lane, dS);
+    load_state<DK, G::DV, FULL>(a.d_last && segment == (int)a.segments - 1 ? a.d_last + bh * dk * dv : nullptr, dk, dv, dv, col0, lane, dS);
     for (int te = T; te > begin;) {
         const Cut cut = chunk_before<G::C>(te, lane, gp, in.g_stride[1], rp, in.reset_stride[1]);
         const int t = cut.t, len = te - t;
@@ -689,7 +691,7 @@ __global__ __launch_bounds__(64 * NW) void delta_pull_kernel(const Args a) {
             d4[i] = turn(16 * i + row0 < len ? x : f4{0, 0, 0, 0}, lane);
         }
         __syncthreads();
-        if (wave == 0)
+        if (wave == NW - 1)
             load_scalars<TILES>(lane < len ? gp[(t + lane) * in.g_stride[1]] : 0.0f, lane < len ? bp[(t + lane) * in.beta_stride[1]] : 0.0f, lane,
                                 cut.first, lds.s);
         kr.store(len, in.normalize, lds.K, lds.KT, lds.s.rk);
@@ -716,7 +718,7 @@ __global__ __launch_bounds__(64 * NW) void delta_pull_kernel(const Args a) {
             for (int i = 0; i < DK / 16; ++i) dS[i] = f4{0, 0, 0, 0};
         te = t;
     }
-    store_state<DK, true>(a.d_starts + (bh * (a.segments - 1) + segment - 1) * (DK * G::DV), DK, G::DV, G::DV, true, col0, lane, dS);
+    store_state<DK, G::DV, true>(a.d_starts + (bh * (a.segments - 1) + segment - 1) * (DK * G::DV), DK, G::DV, G::DV, col0, lane, dS);
 }
 
 template <int TY, int DK, int NW, int TILES, bool FULL>
@@ -737,14 +739,24 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || sizeof(BackwardLds<TY, DK, NW, 
     const int col0 = wave * 16, row0 = 4 * g + (n & 3), col = col0 + (n & 12);  // memory: four columns of a row
     const int64_t bh = b * ap->in.value_heads + h;
 
-    f4 dS[DK / 16], Sn[DK / 16];  // the gradient of the state, and the state, after the chunk
+    f4 dS[DK / 16];     // the gradient of the state after the chunk
+    float edge = 0.0f;  // this lane's share of <dS', S'>, the decay's gradient from all that passes the chunk's end
+    auto meet = [&](const f4* S) {
+        f4 y = {0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < DK / 16; ++i) y += dS[i] * S[i];
+        edge = (y[0] + y[1]) + (y[2] + y[3]);
+    };
+    f4 Sn[DK / 16];
     if (segment == (int)ap->segments - 1) {
-        load_state<DK, FULL>(ap->d_last ? ap->d_last + bh * dk * dv : nullptr, dk, dv, dv, ap->d_last_vec, col0, lane, dS);
-        load_state<DK, FULL>(ap->last + bh * dk * dv, dk, dv, dv, ap->last_vec, col0, lane, Sn);
+        load_state<DK, G::DV, FULL>(ap->d_last ? ap->d_last + bh * dk * dv : nullptr, dk, dv, dv, col0, lane, dS);
+        load_state<DK, G::DV, FULL>(ap->last + bh * dk * dv, dk, dv, dv, col0, lane, Sn);
     } else {
-        load_state<DK, true>(ap->d_starts + (bh * (ap->segments - 1) + segment) * (DK * G::DV), DK, G::DV, G::DV, true, col0, lane, dS);
-        load_state<DK, true>(ap->saved + (bh * (ap->chunks - 1) + T / C - 1) * (DK * G::DV), DK, G::DV, G::DV, true, col0, lane, Sn);
+        load_state<DK, G::DV, true>(ap->d_starts + (bh * (ap->segments - 1) + segment) * (DK * G::DV), DK, G::DV, G::DV, col0, lane, dS);
+        load_state<DK, G::DV, true>(ap->saved + (bh * (ap->chunks - 1) + T / C - 1) * (DK * G::DV), DK, G::DV, G::DV, col0, lane, Sn);
     }
+
+    meet(Sn);
 
     // What a chunk reads from memory.
     Rows<TY, DK, NW, TILES> kr, qr;
@@ -801,10 +813,10 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || sizeof(BackwardLds<TY, DK, NW, 
             }
         }
         f4 S[DK / 16];
-        fetch_state<DK, FULL>(sp, s_rows, s_cols, s_ld, s_vec, col0, lane, S);
+        load_state<DK, G::DV, FULL>(sp, s_rows, s_cols, s_ld, col0, lane, S);
 
         __syncthreads();
-        if (wave == 0) load_scalars<TILES>(lane < len ? gv : 0.0f, lane < len ? bv : 0.0f, lane, first, lds.s);
+        if (wave == NW - 1) load_scalars<TILES>(lane < len ? gv : 0.0f, lane < len ? bv : 0.0f, lane, first, lds.s);
         kr.store(len, ap->in.normalize, lds.K, lds.KT, lds.s.rk);
         qr.store(len, ap->in.normalize, lds.Q, lds.QT, lds.s.rq);
         if (C * pieces_o == G::threads || row_o < C) {
@@ -822,8 +834,6 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || sizeof(BackwardLds<TY, DK, NW, 
 
         // ---- phase A: this wave's columns
         asm volatile("" : "+s"(ap));
-#pragma unroll
-        for (int i = 0; i < DK / 16; ++i) S[i] = turn(S[i], lane);
         f4 ks[TILES], o4[TILES], du[TILES], d4[TILES];
 #pragma unroll
         for (int i = 0; i < TILES; ++i) {
@@ -853,11 +863,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || sizeof(BackwardLds<TY, DK, NW, 
             o4[i] *= gam * row4(lds.s.rq, i, g) * ap->in.scale;
             du[i] *= row4(lds.s.end, i, g) * rk;
         }
-        // <dS', S'>, the decay's gradient from all that passes the chunk's end.
-        f4 edge4 = {0, 0, 0, 0};
-#pragma unroll
-        for (int i = 0; i < DK / 16; ++i) edge4 += dS[i] * Sn[i];
-        const float edge = sum64(edge4[0] + edge4[1] + edge4[2] + edge4[3]);
+        edge = sum64(edge);
         if (lane == 0) lds.edge[wave] = edge;
         __syncthreads();
         Half<3> up[TILES];
@@ -1018,10 +1024,8 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || sizeof(BackwardLds<TY, DK, NW, 
         // the state's gradient, from this wave's columns
         pull_state<TY, DK, TILES>(lds.KT, lds.QT, lds.s, ap->in.scale, n, g, d4, dx, dS);
 #pragma unroll
-        for (int i = 0; i < DK / 16; ++i) {
-            dS[i] = first ? zero : dS[i];
-            Sn[i] = S[i];
-        }
+        for (int i = 0; i < DK / 16; ++i) dS[i] = first ? zero : dS[i];
+        meet(S);
         __syncthreads();  // U and dX are read
         if (busy)
 #pragma unroll
@@ -1084,7 +1088,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || sizeof(BackwardLds<TY, DK, NW, 
         }
         te = t;
     }
-    if (ap->d_state && segment == 0) store_state<DK, FULL>(ap->d_state + bh * dk * dv, dk, dv, dv, ap->d_state_vec, col0, lane, dS);
+    if (ap->d_state && segment == 0) store_state<DK, G::DV, FULL>(ap->d_state + bh * dk * dv, dk, dv, dv, col0, lane, dS);
 }
 // Sums the value heads of each key head, in their order; one thread a value.
 template <int TY> __global__ __launch_bounds__(256) void delta_share_kernel(const Args a) {
@@ -1209,7 +1213,7 @@ template <int TY, int DK, int NW, int TILES, bool FULL> void forward_shape(const
     const uint32_t heads = a.in.batch * a.in.value_heads;
     if (a.segments > 1) {
         delta_forward_kernel<TY, DK, NW, TILES, FULL, true><<<dim3(heads, a.segments - 1, 2), 64 * NW, 0, stream>>>(a);
-        if (a.segments > 2) delta_join_kernel<DK, false><<<dim3(heads, NW), 256, 0, stream>>>(a.starts, a.jumps, a.segments, 16 * NW);
+        if (a.segments > 2) delta_join_kernel<DK, 16 * NW, false><<<dim3(heads, NW), 256, 0, stream>>>(a.starts, a.jumps, a.segments);
     }
     delta_forward_kernel<TY, DK, NW, TILES, FULL, false><<<dim3(heads, a.segments), 64 * NW, 0, stream>>>(a);
 }
@@ -1217,7 +1221,7 @@ template <int TY, int DK, int NW, int TILES, bool FULL> void backward_shape(cons
     const uint32_t heads = a.in.batch * a.in.value_heads;
     if (a.segments > 1) {
         delta_pull_kernel<TY, DK, NW, TILES, FULL><<<dim3(heads, a.segments - 1), 64 * NW, 0, stream>>>(a);
-        if (a.segments > 2) delta_join_kernel<DK, true><<<dim3(heads, NW), 256, 0, stream>>>(a.d_starts, a.jumps, a.segments, 16 * NW);
+        if (a.segments > 2) delta_join_kernel<DK, 16 * NW, true><<<dim3(heads, NW), 256, 0, stream>>>(a.d_starts, a.jumps, a.segments);
     }
     delta_backward_kernel<TY, DK, NW, TILES, FULL><<<dim3(heads, a.segments), 64 * NW, 0, stream>>>(a);
 }
