@@ -63,6 +63,19 @@ def test_large(shape):
     assert_near(orthogonalize(x.cuda()), y.T if shape[0] > shape[1] else y, tolerance(x))
 
 
+def test_largest_tiles():
+    """Enough tiles of 256 squared for every product: four matrices of 2048 x 2304."""
+    from zeno_amd.optim import orthogonalize
+
+    x = matrices((4, 2048, 2304), torch.bfloat16, seed=2, rank=8).cuda()
+    y = x.double()
+    y = y / (torch.linalg.matrix_norm(y)[:, None, None] + 1e-7)
+    for _ in range(5):
+        s = y @ y.mT.contiguous()
+        y = 3.4445 * y + (-4.7750 * s + 2.0315 * (s @ s)) @ y
+    assert_near(orthogonalize(x), y, tolerance(x))
+
+
 def test_singular_values_come_near_one():
     from zeno_amd.optim import orthogonalize
 

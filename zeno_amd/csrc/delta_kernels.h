@@ -355,11 +355,18 @@ template <int TY, int DK, int NW, int TILES> struct ForwardLds {
 };
 
 // FULL: heads of exactly DK and 16 NW dimensions, aligned, need no masks (a fifth of the instructions).
+// Waves a SIMD that the registers are cut down to: as many workgroups as fit the LDS, but not more
+// than the registers bear (128 of four waves spill in the wide kernel with outputs).
+constexpr int forward_waves(int waves, bool states, size_t lds) {
+    const int groups = (int)(160 * 1024 / lds), fit = groups * waves / 4;
+    return waves == 8 && !states ? 2 : fit >= 4 ? 4 : fit == 3 ? 3 : 2;
+}
+
 // STATES: no outputs; of each segment but the last, N, the state after it from zeros (from the
 // caller's state in the first segment), and M, the same without values from the unit matrix: with
 // S the state before the segment, the state after it is M S + N.
 template <int TY, int DK, int NW, int TILES, bool FULL, bool STATES>
-__global__ __launch_bounds__(64 * NW, NW == 4 && sizeof(ForwardLds<TY, DK, NW, TILES>) * 3 <= 160 * 1024 ? 3 : 2) void delta_forward_kernel(const Args a) {
+__global__ __launch_bounds__(64 * NW, forward_waves(NW, STATES, sizeof(ForwardLds<TY, DK, NW, TILES>))) void delta_forward_kernel(const Args a) {
     typedef Geo<TY, DK, NW, TILES> G;
     typedef typename Elem<TY>::type E;
     __shared__ ForwardLds<TY, DK, NW, TILES> lds;

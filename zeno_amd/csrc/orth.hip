@@ -33,7 +33,7 @@ typedef _Float16 h4 __attribute__((ext_vector_type(4)));
 
 constexpr float kScale = 1024.0f;   // of X, A and B in fp16
 constexpr float kLargest = 32.0f;   // entries that the scale leaves room for, twice over
-constexpr int kNormBlocks = 64;
+constexpr int kNormBlocks = 256;
 
 struct Args {
     ZenoAmdOrthogonalize in;
@@ -44,6 +44,7 @@ struct Args {
     float* master;        // X^T in fp32, each value read and written by one thread
     float* sums;          // of the slices of a product
     int slices;
+    bool x_vec;           // eight values along x's dense dimension are 16 bytes aligned (32 of fp32)
     bool out_vec;         // four values along out's dense dimension are aligned
     _Float16 *x, *xt, *gram, *poly;  // [count][...]
     _Float16* xt2;        // the next X^T (X is no operand of the product that makes the next one)
@@ -63,18 +64,31 @@ template <int TY> __device__ __forceinline__ float input(const Args& a, int64_t 
     return Elem<TY>::get(((const E*)a.in.x)[k * a.in.x_stride[0] + row * a.in.x_stride[1] + col * a.in.x_stride[2]]);
 }
 
-// Sums of squares, a grid-stride share of the matrix a block, along whichever dimension is dense.
+// Sums of squares: pieces of eight values along the dense dimension, spread over the blocks.
 template <int TY> __global__ __launch_bounds__(256) void norm_kernel(const Args a) {
+    typedef typename Elem<TY>::type E;
     __shared__ double part[4];
     const int64_t k = blockIdx.y;
     const bool by_col = a.in.x_stride[2] <= a.in.x_stride[1];
-    const int inner = by_col ? a.in.cols : a.in.rows;
-    const int64_t all = (int64_t)a.in.rows * a.in.cols;
+    const uint32_t inner = by_col ? a.in.cols : a.in.rows, pieces = (inner + 7) / 8;
+    const int64_t step = a.in.x_stride[by_col ? 2 : 1], ld = a.in.x_stride[by_col ? 1 : 2];
+    const uint32_t all = pieces * (by_col ? a.in.rows : a.in.cols);
+    const E* x = (const E*)a.in.x + k * a.in.x_stride[0];
     double sum = 0.0;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
-        const int u = (int)(i / inner), w = (int)(i % inner);
-        const double v = by_col ? input<TY>(a, k, u, w) : input<TY>(a, k, w, u);
-        sum += v * v;
+    for (uint32_t i = blockIdx.x * 256 + threadIdx.x; i < all; i += gridDim.x * 256) {
+        const uint32_t row = i / pieces, e = 8 * (i % pieces);
+        const E* at = x + row * ld + e * step;
+        float v[8];
+        if (a.x_vec && e + 8 <= inner) {
+            Raw<TY> raw;
+            raw.template load<true>(at, 8, true);
+            raw.get(v);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = e + j < inner ? Elem<TY>::get(at[j * step]) : 0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum += (double)v[j] * (double)v[j];
     }
 #pragma unroll
     for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
@@ -88,7 +102,9 @@ template <int TY, int P> __global__ __launch_bounds__(256) void load_kernel(cons
     __shared__ float tile[64][65];
     const int64_t k = blockIdx.z;
     const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;  // of X
-    double s = a.partial[k * kNormBlocks + (threadIdx.x & (kNormBlocks - 1))];
+    double s = 0.0;
+#pragma unroll
+    for (int i = 0; i < kNormBlocks; i += 64) s += a.partial[k * kNormBlocks + i + (threadIdx.x & 63)];
 #pragma unroll
     for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d);
     const float f = (float)((double)kScale / (sqrt(s) + (double)a.in.eps));
@@ -136,6 +152,35 @@ template <int P> __device__ __forceinline__ f4 get4(const _Float16* at) {
     return x;
 }
 
+// Which tile a block computes. Consecutive blocks go to the eight dies in turn; each die gets a run
+// of tiles, in bands of eight rows and column by column within a band, so that the tiles which
+// run at once on a die share as many operand rows as they can in its L2. cols 0: the tiles on and
+// below the diagonal.
+__device__ __forceinline__ void tile_at(int block, int blocks, int cols, int rows, int& ti, int& tj) {
+    constexpr int band = 8;
+    const int per = blocks / 8, rest = blocks % 8, die = block % 8;
+    int id = die * per + min(die, rest) + block / 8;
+    for (int r0 = 0;; r0 += band) {
+        const int high = min(band, rows - r0);
+        const int left = cols ? cols : r0, count = left * high + (cols ? 0 : high * (high + 1) / 2);
+        if (id >= count) {
+            id -= count;
+            continue;
+        }
+        if (id < left * high) {
+            ti = r0 + id % high;
+            tj = id / high;
+        } else {  // the band's own triangle
+            id -= left * high;
+            int i = 0;
+            while (id > i) id -= ++i;
+            ti = r0 + i;
+            tj = r0 + id;
+        }
+        return;
+    }
+}
+
 enum Kind { GRAM, POLY, NEXT, LAST };
 enum Share { WHOLE, SLICE, JOIN };  // of the contraction: all of it; a slice, sums kept; the sum of the slices
 
@@ -145,7 +190,7 @@ enum Share { WHOLE, SLICE, JOIN };  // of the contraction: all of it; a slice, s
 // themselves; their 16-byte pieces are permuted by half the row number, which leaves the operand
 // reads without bank conflicts. Few tiles with a long contraction are cut into slices along it
 // (SLICE), whose sums another launch adds in their order (JOIN).
-template <int TY, int P, int BM, int BN, int WR, int WC, int KIND, int SHARE>
+template <int TY, int P, int BM, int BN, int WR, int WC, int STAGES, int KIND, int SHARE>
 __global__ __launch_bounds__(64 * WR * WC) void product_kernel(const Args a) {
     constexpr int threads = 64 * WR * WC, waves = WR * WC;
     constexpr int TM = BM / WR / 16, TN = BN / WC / 16;
@@ -153,21 +198,7 @@ __global__ __launch_bounds__(64 * WR * WC) void product_kernel(const Args a) {
     const int64_t k = blockIdx.y;
     constexpr bool half = KIND == GRAM || KIND == POLY;  // symmetric: tiles on and below the diagonal
     int ti, tj;
-    {
-        // Consecutive blocks go to the eight dies in turn: each die gets a run of tiles, whose operands its L2 shares.
-        const int all = gridDim.x, per = all / 8, rest = all % 8, die = blockIdx.x % 8;
-        const int id = die * per + min(die, rest) + blockIdx.x / 8;
-        if (half) {
-            ti = (int)((sqrtf(8.0f * id + 1.0f) - 1.0f) * 0.5f);
-            while ((ti + 1) * (ti + 2) / 2 <= id) ++ti;
-            while (ti * (ti + 1) / 2 > id) --ti;
-            tj = id - ti * (ti + 1) / 2;
-        } else {
-            const int cols = a.np / BN;
-            ti = id / cols;
-            tj = id % cols;
-        }
-    }
+    tile_at(blockIdx.x, gridDim.x, half ? 0 : a.np / BN, a.mp / BM, ti, tj);
     f4 acc[TM][TN];
 #pragma unroll
     for (int i = 0; i < TM; ++i)
@@ -185,7 +216,8 @@ __global__ __launch_bounds__(64 * WR * WC) void product_kernel(const Args a) {
                 for (int j = 0; j < TN; ++j) acc[i][j] += from[(i * TN + j) * threads];
         }
     } else {
-        __shared__ __attribute__((aligned(128))) char lds[2][(BM + BN) * 128];
+        constexpr int stages = STAGES;
+        __shared__ __attribute__((aligned(128))) char lds[stages][(BM + BN) * 128];
         const int ld = KIND == GRAM ? a.np : a.mp;  // of the contraction
         const _Float16* left = (KIND == GRAM ? a.x + k * a.mp * a.np * P : KIND == POLY ? a.gram + k * a.mp * a.mp * P : a.poly + k * a.mp * a.mp * P);
         const _Float16* right = KIND == NEXT || KIND == LAST ? a.xt + k * a.mp * a.np * P : left;
@@ -197,45 +229,98 @@ __global__ __launch_bounds__(64 * WR * WC) void product_kernel(const Args a) {
             b0 = (int)((int64_t)all * s / a.slices);
             blocks = (int)((int64_t)all * (s + 1) / a.slices);
         }
+        // A load instruction of a wave brings eight rows of 128 bytes.
+        constexpr int loads = (BM + BN) / 8 / waves;
+        static_assert(BM / 8 % waves == 0 && BN / 8 % waves == 0, "whole loads of either operand a wave");
+        uint32_t from[loads];
+#pragma unroll
+        for (int i = 0; i < loads; ++i) {
+            const int row = 8 * (wave + i * waves) + (lane >> 3), piece = (lane & 7) ^ ((row >> 1) & 7);
+            from[i] = (uint32_t)(row < BM ? row : row - BM) * (uint32_t)(ld * P) + 8 * piece;
+        }
         auto fetch = [&](int block, int buf) {
 #pragma unroll
-            for (int i = wave; i < (BM + BN) / 8; i += waves) {  // eight rows of 128 bytes an instruction
-                const int row = 8 * i + (lane >> 3), piece = (lane & 7) ^ ((row >> 1) & 7);
-                const _Float16* from = (row < BM ? left + (int64_t)row * ld * P : right + (int64_t)(row - BM) * ld * P) + 64 * (int64_t)block + 8 * piece;
-                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
-                                                 (__attribute__((address_space(3))) void*)(lds[buf] + 1024 * i), 16, 0, 0);
-            }
+            for (int i = 0; i < loads; ++i)
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)((i * waves * 8 < BM ? left : right) + 64 * (int64_t)block + from[i]),
+                                                 (__attribute__((address_space(3))) void*)(lds[buf] + 1024 * (wave + i * waves)), 16, 0, 0);
         };
         const int row_l = (wave / WC) * (BM / WR) + n, row_r = BM + (wave % WC) * (BN / WC) + n;
-        fetch(b0, b0 & 1);
-        __syncthreads();
-        for (int b = b0; b < blocks; ++b) {
-            if (b + 1 < blocks) fetch(b + 1, (b + 1) & 1);
-            const char* at = lds[b & 1];
-            auto piece = [&](int row, int c) { return *reinterpret_cast<const h8*>(at + row * 128 + ((c ^ ((row >> 1) & 7)) << 4)); };
+        if constexpr (BM == 256) {
+            static_assert(P == 1, "two parts would not fit the registers");
+            // Operands of 32 of the contraction are read while those before them are multiplied.
+            h8 l0[TM], r0[TN], l1[TM], r1[TN];
+            auto read = [&](int b, int s, h8* l, h8* r) {
+                const char* at = lds[b & 1];
 #pragma unroll
-            for (int s = 0; s < (P == 1 ? 2 : 1); ++s) {
-                h8 l[P][TM], r[P][TN];
-#pragma unroll
-                for (int p = 0; p < P; ++p) {
-                    const int c = 4 * (P == 1 ? s : p) + g;
-#pragma unroll
-                    for (int i = 0; i < TM; ++i) l[p][i] = piece(row_l + 16 * i, c);
-#pragma unroll
-                    for (int j = 0; j < TN; ++j) r[p][j] = piece(row_r + 16 * j, c);
+                for (int i = 0; i < TM; ++i) {
+                    const int row = row_l + 16 * i;
+                    l[i] = *reinterpret_cast<const h8*>(at + row * 128 + (((4 * s + g) ^ ((row >> 1) & 7)) << 4));
                 }
+#pragma unroll
+                for (int j = 0; j < TN; ++j) {
+                    const int row = row_r + 16 * j;
+                    r[j] = *reinterpret_cast<const h8*>(at + row * 128 + (((4 * s + g) ^ ((row >> 1) & 7)) << 4));
+                }
+            };
+            auto multiply = [&](const h8* l, const h8* r) {
 #pragma unroll
                 for (int i = 0; i < TM; ++i)
 #pragma unroll
-                    for (int j = 0; j < TN; ++j) {
-                        if constexpr (P == 2) {
-                            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(l[1][i], r[0][j], acc[i][j], 0, 0, 0);
-                            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(l[0][i], r[1][j], acc[i][j], 0, 0, 0);
-                        }
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(l[0][i], r[0][j], acc[i][j], 0, 0, 0);
-                    }
-            }
+                    for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(l[i], r[j], acc[i][j], 0, 0, 0);
+#pragma unroll
+                for (int i = 0; i < TM + TN; ++i) {
+                    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);                    // an LDS read,
+                    __builtin_amdgcn_sched_group_barrier(0x008, TM * TN / (TM + TN), 0);  // and some products
+                }
+            };
+            fetch(b0, b0 & 1);
             __syncthreads();
+            if (b0 + 1 < blocks) fetch(b0 + 1, (b0 + 1) & 1);
+            read(b0, 0, l0, r0);
+            for (int b = b0; b < blocks; ++b) {
+                read(b, 1, l1, r1);
+                multiply(l0, r0);
+                __syncthreads();  // the next 64 have arrived, these are read
+                if (b + 2 < blocks) fetch(b + 2, b & 1);
+                read(b + 1, 0, l0, r0);  // past the end: read and not used
+                multiply(l1, r1);
+            }
+        } else {
+            // Every step fetches, past the end the last 64 again, so that the number of loads under
+            // way is the same at every wait.
+#pragma unroll
+            for (int i = 0; i + 1 < stages; ++i) fetch(min(b0 + i, blocks - 1), i);
+            for (int b = b0, buf = 0; b < blocks; ++b, buf = buf + 1 == stages ? 0 : buf + 1) {
+                // This step's operands are here, and the last step's are read: all waves' after the barrier.
+                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((stages - 2) * loads) : "memory");
+                const char* at = lds[buf];
+                auto piece = [&](int row, int c) { return *reinterpret_cast<const h8*>(at + row * 128 + ((c ^ ((row >> 1) & 7)) << 4)); };
+#pragma unroll
+                for (int s = 0; s < (P == 1 ? 2 : 1); ++s) {
+                    h8 l[P][TM], r[P][TN];
+#pragma unroll
+                    for (int p = 0; p < P; ++p) {
+                        const int c = 4 * (P == 1 ? s : p) + g;
+#pragma unroll
+                        for (int i = 0; i < TM; ++i) l[p][i] = piece(row_l + 16 * i, c);
+#pragma unroll
+                        for (int j = 0; j < TN; ++j) r[p][j] = piece(row_r + 16 * j, c);
+                    }
+                    if (s == 0) fetch(min(b + stages - 1, blocks - 1), buf == 0 ? stages - 1 : buf - 1);
+#pragma unroll
+                    for (int i = 0; i < TM; ++i)
+#pragma unroll
+                        for (int j = 0; j < TN; ++j) {
+                            if constexpr (P == 2) {
+                                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(l[1][i], r[0][j], acc[i][j], 0, 0, 0);
+                                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(l[0][i], r[1][j], acc[i][j], 0, 0, 0);
+                            }
+                            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(l[0][i], r[0][j], acc[i][j], 0, 0, 0);
+                        }
+                }
+            }
+            // No load may still write the LDS when the workgroup's share of it is handed on.
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         }
     }
 
@@ -304,14 +389,17 @@ struct Plan {
     uint64_t norm, master, x, square, sums;  // bytes: partial norms, X in fp32, X as an operand, m x m as an operand, slices' sums
 };
 
-// Tiles of 64, 128 or (one part) 256 squared: the largest that still makes a block for every CU.
+// Tiles of 64, 128 or (one part) 256 squared, the largest that makes enough blocks: one a CU of 128
+// squared (2048 x 2048, one part: B X 36 us with 128, 38 with 64; two parts, whose steps are three
+// times as long, need two to overlap: 82 us with 128, 68 with 64); half the CUs of 256 squared (4096
+// x 4096: the symmetric products have 136 such blocks and take 90 us, 103 with 128; B X 128 and 149).
 int tile_of(const Plan& p, uint32_t count, bool half) {
     auto tiles = [&](int t) {
         const int64_t r = p.mp / t, c = p.np / t;
         return (half ? r * (r + 1) / 2 : r * c) * count;
     };
-    if (p.parts == 1 && p.mp % 256 == 0 && p.np % 256 == 0 && tiles(256) >= 256) return 256;
-    return tiles(128) > 256 ? 128 : 64;
+    if (p.parts == 1 && p.mp % 256 == 0 && p.np % 256 == 0 && tiles(256) >= 128) return 256;
+    return tiles(128) >= (p.parts == 1 ? 256 : 512) ? 128 : 64;
 }
 
 Plan plan_of(const ZenoAmdOrthogonalize& a) {
@@ -328,9 +416,9 @@ Plan plan_of(const ZenoAmdOrthogonalize& a) {
     p.square = (uint64_t)a.count * p.mp * p.mp * p.parts * 2;
     const int t = tile_of(p, a.count, true);
     const uint64_t r = p.mp / t, tiles = r * (r + 1) / 2 * a.count, blocks = (uint64_t)p.np * p.parts / 64;
-    // Two blocks a CU, at least eight steps of the contraction each.
+    // Two blocks a CU, at least eight steps of the contraction each; tiles of 256 are enough as they are.
     p.slices = 1;
-    while (p.slices < 16 && tiles * p.slices * 2 <= 512 && blocks / (p.slices * 2) >= 8) p.slices *= 2;
+    while (t < 256 && p.slices < 16 && tiles * p.slices * 2 <= 512 && blocks / (p.slices * 2) >= 8) p.slices *= 2;
     p.sums = p.slices > 1 ? tiles * p.slices * t * t * 4 : 0;
     return p;
 }
@@ -338,9 +426,13 @@ Plan plan_of(const ZenoAmdOrthogonalize& a) {
 template <int TY, int P, int KIND, int SHARE> void product(const Args& a, int tile, int slices, hipStream_t stream) {
     const int rows = a.mp / tile, cols = a.np / tile;
     const dim3 grid(KIND == GRAM || KIND == POLY ? rows * (rows + 1) / 2 : rows * cols, a.in.count, slices);
-    if (tile == 64) product_kernel<TY, P, 64, 64, 2, 2, KIND, SHARE><<<grid, 256, 0, stream>>>(a);
-    else if (tile == 128) product_kernel<TY, P, 128, 128, 2, 2, KIND, SHARE><<<grid, 256, 0, stream>>>(a);
-    else if constexpr (P == 1 && SHARE == WHOLE) product_kernel<TY, P, 256, 256, 2, 4, KIND, SHARE><<<grid, 512, 0, stream>>>(a);
+    // Small tiles do little between two barriers. Where they do not fill the GPU twice, their operands
+    // are on their way for three steps (1000 x 4000: X X^T 31 us, 39 with one step); where they do, four
+    // blocks a CU instead of two serve better (B X 45, 48).
+    if (tile == 64 && (int64_t)grid.x * grid.y * grid.z <= 768) product_kernel<TY, P, 64, 64, 2, 2, 4, KIND, SHARE><<<grid, 256, 0, stream>>>(a);
+    else if (tile == 64) product_kernel<TY, P, 64, 64, 2, 2, 2, KIND, SHARE><<<grid, 256, 0, stream>>>(a);
+    else if (tile == 128) product_kernel<TY, P, 128, 128, 2, 2, 2, KIND, SHARE><<<grid, 256, 0, stream>>>(a);
+    else if constexpr (P == 1 && SHARE == WHOLE) product_kernel<TY, P, 256, 256, 2, 4, 2, KIND, SHARE><<<grid, 512, 0, stream>>>(a);
 }
 
 template <int TY, int P> hipError_t launch(Args a, const Plan& p, hipStream_t stream) {
@@ -419,6 +511,10 @@ hipError_t run(const ZenoAmdOrthogonalize& in, void* workspace, hipStream_t stre
     const uint64_t four = in.dtype == T_F32 ? 16 : 8;
     const int64_t* s = in.out_stride;
     const int other = (a.flip ? s[2] : s[1]) == 1 ? (a.flip ? 1 : 2) : (a.flip ? 2 : 1);  // the dimension that the stores do not run along
+    const int64_t* xs = in.x_stride;
+    const int dense = xs[2] <= xs[1] ? 2 : 1;
+    const uint64_t eb = in.dtype == T_F32 ? 4 : 2;
+    a.x_vec = xs[dense] == 1 && (uintptr_t)in.x % 16 == 0 && xs[3 - dense] * eb % 16 == 0 && (in.count == 1 || xs[0] * eb % 16 == 0);
     a.out_vec = s[3 - other] == 1 && (uintptr_t)in.out % four == 0 && s[other] % 4 == 0 && (in.count == 1 || s[0] % 4 == 0);
     return in.dtype == T_F32   ? launch<T_F32, 2>(a, p, stream)
            : in.dtype == T_F16 ? launch<T_F16, 2>(a, p, stream)
