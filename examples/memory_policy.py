@@ -1,0 +1,119 @@
+"""Trains a policy with memory on the Cartpole scene from positions alone.
+
+The scene's sensors give positions and velocities of the cart and the pole; the policy sees the
+two positions, so it has to remember what it saw to know how fast they move. Its memory layer is
+the gated delta rule: `gated_delta_step` advances every environment's state beside each step of
+the simulation, `gated_delta` runs the recorded rollout and its gradients, and `orthogonalize`
+makes the update of the policy's matrices.
+
+    python examples/memory_policy.py --envs 1024 --updates 40
+"""
+import argparse
+import os
+import sys
+
+import numpy as np
+import torch
+
+sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+from zeno_amd import make  # noqa: E402
+from zeno_amd.memory import gated_delta, gated_delta_step  # noqa: E402
+from zeno_amd.optim import orthogonalize  # noqa: E402
+
+HEADS, DIM, HIDDEN = 2, 32, 64
+SEEN = [0, 2]           # of the scene's sensors: slider position, hinge angle
+FALLEN, OFF_RAIL = 0.6, 4.0
+
+
+class Policy:
+    """Positions -> features -> memory -> mean action, as plain tensors."""
+
+    def __init__(self, seed: int):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+
+        def matrix(rows, cols, gain=1.0):
+            return (gain * torch.randn(rows, cols, generator=g, device="cuda") / rows ** 0.5).requires_grad_()
+
+        wide = HEADS * DIM
+        self.matrices = {"seen": matrix(len(SEEN), HIDDEN, 2.0), "qkv": matrix(HIDDEN, 3 * wide), "gates": matrix(HIDDEN, 2 * HEADS),
+                         "act": matrix(HIDDEN + wide, 1, 0.1)}
+        self.momenta = {n: torch.zeros_like(w) for n, w in self.matrices.items()}
+
+    def project(self, seen):
+        """What the memory layer takes, for one token or a whole rollout."""
+        x = torch.tanh(seen @ self.matrices["seen"])
+        q, k, v = (y.unflatten(-1, (HEADS, DIM)) for y in (x @ self.matrices["qkv"]).split(HEADS * DIM, -1))
+        g, beta = (x @ self.matrices["gates"]).split(HEADS, -1)
+        return x, q, k, v, torch.nn.functional.logsigmoid(g + 3.0), torch.sigmoid(beta)
+
+    def mean(self, x, o):
+        return (torch.cat([x, o.flatten(-2)], -1) @ self.matrices["act"])[..., 0]
+
+    def update(self, grads, rate):
+        for (n, w), grad in zip(self.matrices.items(), grads):
+            m = self.momenta[n].mul_(0.9).add_(grad)
+            with torch.no_grad():
+                w.sub_(rate * max(1.0, w.shape[0] / w.shape[1]) ** 0.5 * orthogonalize(m))
+
+
+def train(envs: int, updates: int, length: int, seed: int = 0, rate: float = 0.02, noise: float = 0.3, log=print):
+    """Returns the mean length of the episodes that ended during each update, and how far the
+    rollout's outputs, as they were acted, are from those the training pass computes."""
+    torch.manual_seed(seed)
+    rng = torch.Generator(device="cuda").manual_seed(seed + 1)
+    policy, env = Policy(seed), make("cartpole", num_envs=envs)
+    obs = env.reset()
+    state = torch.zeros(envs, HEADS, DIM, DIM, device="cuda")
+    began = np.ones(envs, dtype=bool)  # this step begins an episode
+    age, history, apart = np.zeros(envs), [], 0.0
+    for step in range(updates):
+        seen, actions, begins, rewards, outputs, lengths = [], [], [], [], [], []
+        first = state.clone()
+        with torch.no_grad():
+            for _ in range(length):
+                s = torch.from_numpy(obs[:, SEEN]).cuda()
+                reset = torch.from_numpy(began).cuda()
+                x, *token = policy.project(s)
+                o = gated_delta_step(*token, state, reset, normalize=True)
+                act = policy.mean(x, o) + noise * torch.randn(envs, generator=rng, device="cuda")
+                seen.append(s), begins.append(reset), actions.append(act), outputs.append(o)
+                obs = env.step(act.clamp(-1, 1).cpu().numpy()[:, None])[0]
+                age += 1
+                fell = (np.abs(obs[:, 2]) > FALLEN) | (np.abs(obs[:, 0]) > OFF_RAIL) | ~np.isfinite(obs).all(1)
+                rewards.append(torch.from_numpy(np.where(fell, 0.0, 1.0 - np.nan_to_num(obs[:, 2]) ** 2 - 0.05 * np.nan_to_num(obs[:, 0]) ** 2)).float().cuda())
+                began = fell | (age >= 500)
+                if began.any():
+                    lengths.extend(age[began])
+                    age[began] = 0
+                    obs = env.reset(began.astype(np.uint8))
+        seen, actions, begins, rewards = (torch.stack(y) for y in (seen, actions, begins, rewards))  # time-major, as recorded
+        # Discounted returns to the end of each episode (or of the rollout), against their mean.
+        returns, total = torch.empty_like(rewards), torch.zeros(envs, device="cuda")
+        last = torch.from_numpy(began).cuda()
+        for t in reversed(range(length)):
+            ends = last if t + 1 == length else begins[t + 1]
+            total = rewards[t] + 0.97 * torch.where(ends, torch.zeros_like(total), total)
+            returns[t] = total
+        advantage = (returns - returns.mean(1, keepdim=True)) / (returns.std() + 1e-6)
+
+        x, *tokens = policy.project(seen)
+        o, _ = gated_delta(*(y.transpose(0, 1) for y in tokens), begins.transpose(0, 1), first, normalize=True)
+        o = o.transpose(0, 1)
+        apart = max(apart, float((o.detach() - torch.stack(outputs)).abs().max()))
+        loss = (0.5 * ((actions - policy.mean(x, o)) / noise).square() * advantage).mean()
+        policy.update(torch.autograd.grad(loss, list(policy.matrices.values())), rate * (1.0 - step / updates))
+        history.append(float(np.mean(lengths)) if lengths else float(age.mean()))
+        if step % 10 == 9:
+            log(f"update {step + 1}: episodes that ended lasted {history[-1]:.1f} steps, mean reward {float(rewards.mean()):.3f}")
+    env.close()
+    return history, apart
+
+
+if __name__ == "__main__":
+    ap = argparse.ArgumentParser(description=__doc__, formatter_class=argparse.RawDescriptionHelpFormatter)
+    ap.add_argument("--envs", type=int, default=1024)
+    ap.add_argument("--updates", type=int, default=60)
+    ap.add_argument("--length", type=int, default=64)
+    ap.add_argument("--seed", type=int, default=0)
+    a = ap.parse_args()
+    train(a.envs, a.updates, a.length, a.seed)
