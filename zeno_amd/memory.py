@@ -29,6 +29,7 @@ and infinity included, has no effect on what follows.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 from typing import Optional, Tuple
 
@@ -37,7 +38,8 @@ import torch
 from . import _lib as L
 
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
-_S2, _S3 = C.c_int64 * 2, C.c_int64 * 3
+_S3 = C.c_int64 * 3
+_HERE = contextlib.nullcontext()
 
 
 def _fail(rc: int, what: str) -> None:
@@ -48,34 +50,37 @@ def _fail(rc: int, what: str) -> None:
 
 def _check(q, k, v, g, beta, reset, state, lead: int) -> None:
     """Shapes, types and devices; `lead` is the number of dimensions before the heads."""
-    if q.dtype not in _DTYPES:
-        raise TypeError(f"q, k and v must be float32, float16 or bfloat16, not {q.dtype}")
-    if q.dim() != lead + 2 or v.dim() != lead + 2:
-        raise ValueError(f"q and v must have {lead + 2} dimensions, not {q.dim()} and {v.dim()}")
-    if k.shape != q.shape or v.shape[:lead] != q.shape[:lead] or g.shape != v.shape[:-1] or beta.shape != g.shape:
-        raise ValueError(f"shapes do not agree: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}, "
-                         f"g {tuple(g.shape)}, beta {tuple(beta.shape)}")
-    if k.dtype != q.dtype or v.dtype != q.dtype:
-        raise TypeError(f"q, k and v must have one type, not {q.dtype}, {k.dtype}, {v.dtype}")
-    if g.dtype != torch.float32 or beta.dtype != torch.float32:
+    dtype, device, qs, vs, gs = q.dtype, q.device, q.shape, v.shape, g.shape
+    if dtype not in _DTYPES:
+        raise TypeError(f"q, k and v must be float32, float16 or bfloat16, not {dtype}")
+    if len(qs) != lead + 2 or len(vs) != lead + 2:
+        raise ValueError(f"q and v must have {lead + 2} dimensions, not {len(qs)} and {len(vs)}")
+    if k.shape != qs or vs[:lead] != qs[:lead] or gs != vs[:-1] or beta.shape != gs:
+        raise ValueError(f"shapes do not agree: q {tuple(qs)}, k {tuple(k.shape)}, v {tuple(vs)}, "
+                         f"g {tuple(gs)}, beta {tuple(beta.shape)}")
+    if 0 in qs or 0 in vs:
+        raise ValueError(f"empty operands: q {tuple(qs)}, v {tuple(vs)}")
+    if k.dtype is not dtype or v.dtype is not dtype:
+        raise TypeError(f"q, k and v must have one type, not {dtype}, {k.dtype}, {v.dtype}")
+    if g.dtype is not torch.float32 or beta.dtype is not torch.float32:
         raise TypeError(f"g and beta must be float32, not {g.dtype} and {beta.dtype}")
     if not q.is_cuda:
         raise ValueError("the operands must be on the GPU (there is no CPU fallback)")
-    others = [k, v, g, beta]
+    apart = k.device != device or v.device != device or g.device != device or beta.device != device
     if reset is not None:
-        if reset.shape != q.shape[:lead]:
-            raise ValueError(f"reset must have the shape {tuple(q.shape[:lead])}, not {tuple(reset.shape)}")
+        if reset.shape != qs[:lead]:
+            raise ValueError(f"reset must have the shape {tuple(qs[:lead])}, not {tuple(reset.shape)}")
         if reset.dtype not in (torch.bool, torch.uint8):
             raise TypeError(f"reset must be bool or uint8, not {reset.dtype}")
-        others.append(reset)
+        apart = apart or reset.device != device
     if state is not None:
-        want = (q.shape[0], v.shape[lead], q.shape[-1], v.shape[-1])
+        want = (qs[0], vs[lead], qs[-1], vs[-1])
         if state.shape != want:
             raise ValueError(f"state must have the shape {want}, not {tuple(state.shape)}")
-        if state.dtype != torch.float32:
+        if state.dtype is not torch.float32:
             raise TypeError(f"state must be float32, not {state.dtype}")
-        others.append(state)
-    if any(x.device != q.device for x in others):
+        apart = apart or state.device != device
+    if apart:
         raise ValueError("the operands must be on one device")
 
 
@@ -84,21 +89,20 @@ def _row(x: torch.Tensor) -> torch.Tensor:
 
 
 def _inputs(q, k, v, g, beta, reset, state, scale, normalize) -> L.ZenoAmdDeltaInputs:
-    if q.dim() == 4:
+    qs, ks, vs, gs, bs = q.stride(), k.stride(), v.stride(), g.stride(), beta.stride()
+    rs = (0, 0) if reset is None else reset.stride()
+    if len(qs) == 4:
         b, t, hk, dk = q.shape
-        qs, ks, vs = q.stride()[:3], k.stride()[:3], v.stride()[:3]
-        gs, bs = g.stride(), beta.stride()
-        rs = (0, 0) if reset is None else reset.stride()
+        qs, ks, vs = qs[:3], ks[:3], vs[:3]
     else:
         (b, hk, dk), t = q.shape, 1
-        qs, ks, vs = ((x.stride(0), 0, x.stride(1)) for x in (q, k, v))
-        gs, bs = ((x.stride(0), 0, x.stride(1)) for x in (g, beta))
-        rs = (0, 0) if reset is None else (reset.stride(0), 0)
+        qs, ks, vs, gs, bs = (qs[0], 0, qs[1]), (ks[0], 0, ks[1]), (vs[0], 0, vs[1]), (gs[0], 0, gs[1]), (bs[0], 0, bs[1])
+        rs = (rs[0], 0)
+    _, hv, dv = v.shape[-3:]
     return L.ZenoAmdDeltaInputs(
-        _DTYPES[q.dtype], b, t, hk, v.shape[-2], dk, v.shape[-1], bool(normalize), scale,
+        _DTYPES[q.dtype], b, t, hk, hv, dk, dv, normalize, scale,
         q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(),
-        None if reset is None else reset.data_ptr(), None if state is None else state.data_ptr(),
-        _S3(*qs), _S3(*ks), _S3(*vs), _S3(*gs), _S3(*bs), _S2(*rs))
+        None if reset is None else reset.data_ptr(), None if state is None else state.data_ptr(), qs, ks, vs, gs, bs, rs)
 
 
 def _space(n: int, x: torch.Tensor) -> Optional[torch.Tensor]:
@@ -109,10 +113,15 @@ def _stream(x: torch.Tensor) -> int:
     return torch.cuda.current_stream(x.device).cuda_stream
 
 
+def _on(x: torch.Tensor):
+    """The context in which x's device is the current one, as the library's calls need it."""
+    return _HERE if torch.cuda.current_device() == x.device.index else torch.cuda.device(x.device)
+
+
 class _GatedDelta(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, g, beta, reset, state, scale, normalize, train):
-        with torch.cuda.device(q.device):
+        with _on(q):
             lib = L.load()
             a = _inputs(q, k, v, g, beta, reset, state, scale, normalize)
             o = torch.empty_like(v)  # v's order of dimensions: time-major in, time-major out
@@ -137,7 +146,7 @@ class _GatedDelta(torch.autograd.Function):
         q, k, v, g, beta, reset, state, last, saved = ctx.saved_tensors
         if d_o is None and d_last is None:
             return (None,) * 10
-        with torch.cuda.device(q.device):
+        with _on(q):
             lib = L.load()
             a = _inputs(q, k, v, g, beta, reset, state, ctx.scale, ctx.normalize)
             d_o = torch.zeros_like(v) if d_o is None else _row(d_o)
@@ -170,8 +179,6 @@ def gated_delta(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tens
     """The rule over whole sequences. Returns o [B, T, Hv, value_dim] in the type of v and the
     state after the last token, a new tensor. Differentiable in q, k, v, g, beta and state."""
     _check(q, k, v, g, beta, reset, state, 2)
-    if min(q.shape) < 1 or min(v.shape) < 1:
-        raise ValueError(f"empty operands: q {tuple(q.shape)}, v {tuple(v.shape)}")
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
     q, k, v = _row(q), _row(k), _row(v)
     state = None if state is None else state.contiguous()
@@ -179,26 +186,25 @@ def gated_delta(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tens
     return _GatedDelta.apply(q, k, v, g, beta, reset, state, scale, bool(normalize), train)
 
 
-@torch.no_grad()
 def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, beta: torch.Tensor,
                      state: torch.Tensor, reset: Optional[torch.Tensor] = None, *, scale: Optional[float] = None,
                      normalize: bool = False, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """One token for every sequence: q, k [B, Hk, key_dim], v [B, Hv, value_dim], g, beta
     [B, Hv], reset [B]. `state` (contiguous) is advanced in place; returns o [B, Hv, value_dim]
-    (`out` if given). Without gradients: training runs gated_delta on the recorded rollout."""
+    (`out` if given). Without gradients, even where an operand asks for them: training runs
+    gated_delta on the recorded rollout."""
     _check(q, k, v, g, beta, reset, state, 1)
-    if min(q.shape) < 1 or min(v.shape) < 1:
-        raise ValueError(f"empty operands: q {tuple(q.shape)}, v {tuple(v.shape)}")
     if not state.is_contiguous():
         raise ValueError("state must be contiguous: it is advanced in place")
     q, k, v = _row(q), _row(k), _row(v)
     if out is None:
-        out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
+        out = torch.empty_like(v, memory_format=torch.contiguous_format)
     elif out.shape != v.shape or out.dtype != v.dtype or out.device != v.device or (out.stride(-1) != 1 and out.shape[-1] != 1):
         raise ValueError(f"out must be like v: {tuple(v.shape)}, {v.dtype}, on {v.device}, its last dimension contiguous")
-    with torch.cuda.device(q.device):
-        a = _inputs(q, k, v, g, beta, reset, state, q.shape[-1] ** -0.5 if scale is None else float(scale), normalize)
-        rc = L.load().zeno_amd_delta_step(a, out.data_ptr(), _S3(out.stride(0), 0, out.stride(1)), state.data_ptr(), _stream(q))
+    with _on(q):
+        a = _inputs(q, k, v, g, beta, reset, state, q.shape[-1] ** -0.5 if scale is None else float(scale), bool(normalize))
+        os = out.stride()
+        rc = L.load().zeno_amd_delta_step(a, out.data_ptr(), _S3(os[0], 0, os[1]), state.data_ptr(), _stream(q))
         if rc:
             _fail(rc, "gated_delta_step")
     return out
