@@ -66,10 +66,10 @@ def test_python_refuses_cpu_tensors_and_wrong_shapes():
 
 
 def test_segments_of_long_sequences(lib):
-    """One head over 4096 tokens: 128 chunks, 16 segments of 8, states and matrices between them."""
+    """One head over 4096 tokens: 128 chunks, 32 segments of 4, states and matrices between them."""
     long = args(batch=1, key_heads=1, value_heads=1, length=4096)
-    assert lib.zeno_amd_delta_workspace_bytes(long) == 4 * 15 * (64 * 64 + 3 * 64 * 64 + 4)
-    assert lib.zeno_amd_delta_saved_bytes(long) == 4 * (127 * 64 * 64 + 15 * (3 * 64 * 64 + 4))
+    assert lib.zeno_amd_delta_workspace_bytes(long) == 4 * 31 * (64 * 64 + 3 * 64 * 64 + 4)
+    assert lib.zeno_amd_delta_saved_bytes(long) == 4 * (127 * 64 * 64 + 31 * (3 * 64 * 64 + 4))
     assert lib.zeno_amd_delta_forward(long, 16, (C.c_int64 * 3)(), 16, None, None, None) == -6
     assert "workspace" in _lib.last_error()
     assert lib.zeno_amd_delta_forward(long, 16, (C.c_int64 * 3)(), 16, None, 8, None) == -6
