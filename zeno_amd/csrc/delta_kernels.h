@@ -49,7 +49,7 @@ template <> struct Tok<1> {
     static constexpr int stride = 24;
 };
 
-constexpr int kInvStride = 20;  // of 16x16 tiles in LDS, bf16 or float
+constexpr int kInvStride = 20;  // of 16x16 tiles in LDS
 
 template <int TY, int DK, int NW, int TILES> struct Geo {
     static constexpr int NP = Elem<TY>::parts;        // parts of an input value
@@ -116,17 +116,29 @@ template <int TY, int DK, int NW, int TILES> struct Rows {
     }
 };
 
-// g and beta of a chunk (one lane a token, wave 0): sums in 64 bits.
+// A double from other lanes: shifted up by CTRL - 0x110 lanes within each 16 (zeros come in), or
+// (0x142) the last lane of the 16 before, in every second 16.
+template <int CTRL> __device__ __forceinline__ double dpp64(double x) {
+    constexpr int rows = CTRL == 0x142 ? 0xa : 0xf;
+    const uint64_t b = __builtin_bit_cast(uint64_t, x);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, rows, 0xf, CTRL != 0x142);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), CTRL, rows, 0xf, CTRL != 0x142);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+
+// g and beta of a chunk (one lane a token, one wave): sums in 64 bits.
 template <int TILES>
 __device__ __forceinline__ void load_scalars(float g, float beta, int lane, bool first, Scalars<TILES>& s) {
     constexpr int C = 16 * TILES;
     double sum = (first && lane == 0) ? 0.0 : (double)g;
-#pragma unroll
-    for (int d = 1; d < C; d <<= 1) {
-        const double up = __shfl_up(sum, d);
-        if (lane >= d) sum += up;
-    }
-    const double all = __shfl(sum, C - 1);
+    sum += dpp64<0x111>(sum);
+    sum += dpp64<0x112>(sum);
+    sum += dpp64<0x114>(sum);
+    sum += dpp64<0x118>(sum);
+    if constexpr (TILES == 2) sum += dpp64<0x142>(sum);
+    const uint64_t b = __builtin_bit_cast(uint64_t, sum);
+    const double all = __builtin_bit_cast(double, (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(b >> 32), C - 1) << 32 |
+                                                      (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)b, C - 1));
     if (lane < C) {
         const float hi = (float)sum;
         s.hi[lane] = hi;
@@ -155,40 +167,52 @@ __device__ __forceinline__ f4 decayed(const uint16_t* rows_i, const uint16_t* ro
     return acc;
 }
 
-// Column c (of 16) of the inverse of I + N, N strictly lower triangular and kept transposed: each
-// value, once it is final, is taken out of all sums that still need it.
-__device__ __forceinline__ void inverse_column(const float* NT, int c, float* t) {
+// A value of row group G (lanes 16 G to 16 G + 15) in all four groups.
+template <int G> __device__ __forceinline__ float from_group(float x) {
+    const uint32_t b = __float_as_uint(x);
+    const uint32_t pair = __builtin_amdgcn_permlane16_swap(b, b, false, false)[G & 1];
+    return __uint_as_float(__builtin_amdgcn_permlane32_swap(pair, pair, false, false)[G >> 1]);
+}
+// Rows 4 G to 4 G + 3 of W = Z - Z B W, and what they take from the rows below; zb is -Z B. Rows
+// that are final take only zeros.
+template <int G> __device__ __forceinline__ void solve_rows(f4 zb, int g, f4& w) {
+    constexpr int lane = 0x150 + 4 * G;  // the first of these rows' columns, from within each 16 lanes
+    f4 u = w;
+    u[1] += dpp<lane>(zb[1]) * u[0];
+    u[2] += dpp<lane>(zb[2]) * u[0];
+    u[3] += dpp<lane>(zb[3]) * u[0];
+    u[2] += dpp<lane + 1>(zb[2]) * u[1];
+    u[3] += dpp<lane + 1>(zb[3]) * u[1];
+    u[3] += dpp<lane + 2>(zb[3]) * u[2];
+    if constexpr (G == 3) {
+        w = g == 3 ? u : w;
+    } else {
+        const f4 y = {from_group<G>(u[0]), from_group<G>(u[1]), from_group<G>(u[2]), from_group<G>(u[3])};
 #pragma unroll
-    for (int j = 0; j < 16; ++j) t[j] = j == c ? 1.0f : 0.0f;
-#pragma unroll
-    for (int j = 0; j < 15; ++j) {
-#pragma unroll
-        for (int b = (j + 1) & ~3; b < 16; b += 4) {
-            const f4 w = *reinterpret_cast<const f4*>(NT + j * kInvStride + b);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (b + i > j) t[b + i] -= t[j] * w[i];
-        }
+        for (int r = 0; r < 4; ++r)
+            w[r] += dpp<lane>(zb[r]) * y[0] + dpp<lane + 1>(zb[r]) * y[1] + dpp<lane + 2>(zb[r]) * y[2] + dpp<lane + 3>(zb[r]) * y[3];
     }
 }
-// 16 values in three parts, from last to first where `flip`.
-__device__ __forceinline__ void put_row(uint16_t* to, const float* t, bool flip) {
-#pragma unroll
-    for (int b = 0; b < 16; b += 4) {
-        const float v0 = t[b], v1 = t[b + 1], v2 = t[b + 2], v3 = t[b + 3];
-        put4<3>(to + (flip ? 12 - b : b), 16 * kInvStride, f4{flip ? v3 : v0, flip ? v2 : v1, flip ? v1 : v2, flip ? v0 : v3});
-    }
+// W = (I + Z B)^-1 Z of a strictly lower 16x16 tile, by forward substitution of four rows at a time,
+// in registers: with Z read from LDS, one lane a column, latency was three quarters of the time.
+// The inverses of I + Z B and I + B Z are I - W B and I - B W.
+__device__ __forceinline__ f4 solve_tile(f4 z, float beta, int g) {
+    const f4 zb = z * -beta;
+    solve_rows<0>(zb, g, z);
+    solve_rows<1>(zb, g, z);
+    solve_rows<2>(zb, g, z);
+    solve_rows<3>(zb, g, z);
+    return z;
 }
 
-// The matrices inside a chunk. Of the diagonal tiles: 0, Z B with rows and columns from last to
-// first, and the inverse of I + Z B; 1 (gradients), B Z transposed, and the transposed inverse of I + B Z.
+// The matrices inside a chunk. Of the diagonal tiles: the inverse of I + Z B, and for gradients
+// behind it the transposed inverse of I + B Z.
 template <int TILES> struct Inner {
     static constexpr int C = 16 * TILES, TS = Tok<TILES>::stride, sides = 1;
     static constexpr int tile = 16 * kInvStride;                // of one 16x16 tile
     alignas(16) uint16_t P[3 * C * TS];                         // lower(D * Q K^T) scale
     alignas(16) uint16_t off[3 * tile];                         // Z, lower left tile
     alignas(16) uint16_t inv[TILES * 3 * tile];
-    alignas(16) float diag[TILES * tile];
 };
 template <int TILES> struct InnerBack {
     static constexpr int C = 16 * TILES, TS = Tok<TILES>::stride, sides = 2;
@@ -196,7 +220,6 @@ template <int TILES> struct InnerBack {
     alignas(16) uint16_t P[3 * C * TS], PT[3 * C * TS];         // and transposed
     alignas(16) uint16_t off[3 * tile], offT[3 * tile];
     alignas(16) uint16_t inv[2 * TILES * 3 * tile];
-    alignas(16) float diag[2 * TILES * tile];
 };
 
 // A result tile (rows from i0 = 16 ti + 4 g, this lane's column j) into a matrix along tokens,
@@ -231,33 +254,21 @@ __device__ __forceinline__ void fill_inner(const uint16_t* K, const uint16_t* Q,
         if (what == 0) {
             const f4 z = decayed<TY, DK, NW, TILES>(K, K, s.rk, ti, tj, n, g, s);
             if (ti == tj) {
+                constexpr int second = M::sides == 2 ? TILES : 0;  // tiles before the transposed ones
                 const float bj = s.beta[j];
                 const f4 bi = row4(s.beta, ti, g);
-                f4 zb, bz;
+                f4 lower, t, tt;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) lower[r] = n < 4 * g + r ? z[r] : 0.0f;
+                const f4 w = solve_tile(lower, bj, g);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const float v = n < 4 * g + r ? z[r] : 0.0f;
-                    zb[r] = v * bj;
-                    bz[r] = v * bi[r];
+                    const float one = n == 4 * g + r ? 1.0f : 0.0f;
+                    t[r] = one - w[r] * bj;
+                    tt[r] = one - bi[r] * w[r];
                 }
-                // A row of an inverse is a column of it once rows and columns are taken from last to
-                // first: lanes 0 to 15 make the rows of (I + Z B)^-1, lanes 16 to 31 the columns of (I + B Z)^-1.
-                constexpr bool row = WANT & W_INV, col = WANT & W_INVT;
-                constexpr int second = M::sides == 2 ? TILES : 0;  // tiles before those of side 1
-                if constexpr (row) {
-                    const f4 y = turn(zb, lane);
-                    *reinterpret_cast<f4*>(m.diag + (ti * 16 + 15 - 4 * g - (n & 3)) * kInvStride + 12 - (n & 12)) = f4{y[3], y[2], y[1], y[0]};
-                }
-                if constexpr (col) *reinterpret_cast<f4*>(m.diag + ((second + ti) * 16 + n) * kInvStride + 4 * g) = bz;
-                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-                __builtin_amdgcn_wave_barrier();
-                if (lane < (row && col ? 32 : 16)) {
-                    const bool side = row && col ? lane >= 16 : col;
-                    const int at = (side ? second : 0) + ti;
-                    float t[16];
-                    inverse_column(m.diag + at * M::tile, side ? n : 15 - n, t);
-                    put_row(m.inv + at * 3 * M::tile + n * kInvStride, t, !side);
-                }
+                if constexpr (WANT & W_INV) put4<3>(m.inv + ti * 3 * M::tile + (4 * g + (n & 3)) * kInvStride + (n & 12), M::tile, turn(t, lane));
+                if constexpr (WANT & W_INVT) put4<3>(m.inv + (second + ti) * 3 * M::tile + n * kInvStride + 4 * g, M::tile, tt);
             } else {
                 if constexpr (WANT & W_INV) put4<3>(m.off + (4 * g + (n & 3)) * kInvStride + (n & 12), 16 * kInvStride, turn(z, lane));
                 if constexpr (WANT & W_INVT) put4<3>(m.offT + n * kInvStride + 4 * g, 16 * kInvStride, z);
