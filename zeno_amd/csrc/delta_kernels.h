@@ -189,8 +189,12 @@ template <int G> __device__ __forceinline__ void solve_rows(f4 zb, int g, f4& w)
     } else {
         const f4 y = {from_group<G>(u[0]), from_group<G>(u[1]), from_group<G>(u[2]), from_group<G>(u[3])};
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-            w[r] += dpp<lane>(zb[r]) * y[0] + dpp<lane + 1>(zb[r]) * y[1] + dpp<lane + 2>(zb[r]) * y[2] + dpp<lane + 3>(zb[r]) * y[3];
+        for (int r = 0; r < 4; ++r) {
+            w[r] += dpp<lane>(zb[r]) * y[0];
+            w[r] += dpp<lane + 1>(zb[r]) * y[1];
+            w[r] += dpp<lane + 2>(zb[r]) * y[2];
+            w[r] += dpp<lane + 3>(zb[r]) * y[3];
+        }
     }
 }
 // W = (I + Z B)^-1 Z of a strictly lower 16x16 tile, by forward substitution of four rows at a time,
