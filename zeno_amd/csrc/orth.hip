@@ -17,6 +17,7 @@
 // Layout. X and X^T are both kept as operands (every product then reads two operands along their
 // rows); rows and columns are padded with zeros to the tile. Two parts alternate every 32 columns,
 // so a row's 128 bytes are 64 columns of one part or 32 of two, and both run through the same loop.
+#include <algorithm>
 #include <cmath>
 #include <utility>
 
@@ -111,7 +112,7 @@ template <int TY, int P> __global__ __launch_bounds__(256) void load_kernel(cons
     const bool dense_cols = a.flip ? a.in.x_stride[1] <= a.in.x_stride[2] : a.in.x_stride[2] <= a.in.x_stride[1];
     const int w = threadIdx.x & 63, u = threadIdx.x >> 6;
 #pragma unroll
-    for (int i = u; i < 64; i += 4) {
+    for (int i = u, t = 0; t < 16; ++t, i += 4) {
         const int r = dense_cols ? i : w, c = dense_cols ? w : i;
         float v = 0.0f;
         if (r0 + r < a.m && c0 + c < a.n) v = a.flip ? input<TY>(a, k, c0 + c, r0 + r) : input<TY>(a, k, r0 + r, c0 + c);
@@ -121,7 +122,7 @@ template <int TY, int P> __global__ __launch_bounds__(256) void load_kernel(cons
     _Float16* x = a.x + k * a.mp * a.np * P;
     _Float16* xt = a.xt + k * a.mp * a.np * P;
 #pragma unroll
-    for (int i = u; i < 64; i += 4) {
+    for (int i = u, t = 0; t < 16; ++t, i += 4) {
         a.master[(k * a.np + c0 + i) * a.mp + r0 + w] = tile[w][i];
         put<P>(x + place<P>(r0 + i, c0 + w, a.np), tile[i][w]);
         put<P>(xt + place<P>(c0 + i, r0 + w, a.mp), tile[w][i]);
@@ -152,14 +153,16 @@ template <int P> __device__ __forceinline__ f4 get4(const _Float16* at) {
     return x;
 }
 
-// Which tile a block computes. Consecutive blocks go to the eight dies in turn; each die gets a run
-// of tiles, in bands of eight rows and column by column within a band, so that the tiles which
-// run at once on a die share as many operand rows as they can in its L2. cols 0: the tiles on and
-// below the diagonal.
-__device__ __forceinline__ void tile_at(int block, int blocks, int cols, int rows, int& ti, int& tj) {
-    constexpr int band = 8;
+// Consecutive blocks go to the eight dies in turn; each die gets a run of the work.
+__device__ __forceinline__ int run_at(int block, int blocks) {
     const int per = blocks / 8, rest = blocks % 8, die = block % 8;
-    int id = die * per + min(die, rest) + block / 8;
+    return die * per + min(die, rest) + block / 8;
+}
+// Which tile that is: in bands of eight rows and column by column within a band, so that the tiles
+// which run at once on a die share as many operand rows as they can in its L2. cols 0: the tiles on
+// and below the diagonal.
+__device__ __forceinline__ void tile_at(int id, int cols, int rows, int& ti, int& tj) {
+    constexpr int band = 8;
     for (int r0 = 0;; r0 += band) {
         const int high = min(band, rows - r0);
         const int left = cols ? cols : r0, count = left * high + (cols ? 0 : high * (high + 1) / 2);
@@ -185,29 +188,37 @@ enum Kind { GRAM, POLY, NEXT, LAST };
 enum Share { WHOLE, SLICE, JOIN };  // of the contraction: all of it; a slice, sums kept; the sum of the slices
 
 // C = L R^T of rows along the contraction, and what follows from it. A block computes BM x BN; its
-// WR x WC waves hold their part in registers. 128 bytes of every row of both operands are in LDS
-// at a time, twice (the next ones arrive while these are multiplied), written by the loads
-// themselves; their 16-byte pieces are permuted by half the row number, which leaves the operand
-// reads without bank conflicts. Few tiles with a long contraction are cut into slices along it
-// (SLICE), whose sums another launch adds in their order (JOIN).
+// WR x WC waves hold their part in registers. 128 bytes of every row of both operands are a step;
+// steps come into LDS by loads that write it themselves, their 16-byte pieces permuted by half the
+// row number, which leaves the operand reads without bank conflicts. Few tiles with a long
+// contraction are cut into slices along it (SLICE), whose sums another launch adds in their order (JOIN).
+// Bound by the matrix units and the operands' way from L2 together, and at its end by memory: X, X^T and
+// the fp32 X are written at once by all blocks. 4096 x 4096, one part: B X 147 us (0.93 PFLOP/s), the
+// symmetric products 110 and 114 (half the operations; 0.62); 1000 x 4000, two parts: B X 38 us (0.65
+// PFLOP/s of part products, of which 14 are the end), X X^T 18 and 7 for the join.
 template <int TY, int P, int BM, int BN, int WR, int WC, int STAGES, int KIND, int SHARE>
 __global__ __launch_bounds__(64 * WR * WC) void product_kernel(const Args a) {
     constexpr int threads = 64 * WR * WC, waves = WR * WC;
-    constexpr int TM = BM / WR / 16, TN = BN / WC / 16;
+    constexpr int rows = BM / WR / 16, TM = SHARE == JOIN ? 1 : rows, TN = BN / WC / 16;  // a join: one row of result tiles a wave
+    const int i0 = SHARE == JOIN ? blockIdx.z : 0;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
     const int64_t k = blockIdx.y;
     constexpr bool half = KIND == GRAM || KIND == POLY;  // symmetric: tiles on and below the diagonal
+    // Slices are the outer order: a die then reads little more than a slice of the operands.
+    const int tiles = SHARE == SLICE ? gridDim.x / a.slices : gridDim.x, run = run_at(blockIdx.x, gridDim.x);
+    const int slice = SHARE == SLICE ? run / tiles : 0, tile = run - slice * tiles;
     int ti, tj;
-    tile_at(blockIdx.x, gridDim.x, half ? 0 : a.np / BN, a.mp / BM, ti, tj);
+    tile_at(tile, half ? 0 : a.np / BN, a.mp / BM, ti, tj);
     f4 acc[TM][TN];
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
         for (int j = 0; j < TN; ++j) acc[i][j] = f4{0, 0, 0, 0};
     // The sums of slice s of this tile: [matrix][slice][tile][value][thread].
-    auto sums = [&](int s) { return (f4*)a.sums + (((k * a.slices + s) * gridDim.x + blockIdx.x) * (TM * TN)) * threads + threadIdx.x; };
+    auto sums = [&](int s) { return (f4*)a.sums + (((k * a.slices + s) * tiles + tile) * (rows * TN) + i0 * TN) * threads + threadIdx.x; };
 
     if constexpr (SHARE == JOIN) {
+#pragma unroll 4
         for (int s = 0; s < a.slices; ++s) {
             const f4* from = sums(s);
 #pragma unroll
@@ -225,9 +236,9 @@ __global__ __launch_bounds__(64 * WR * WC) void product_kernel(const Args a) {
         right += (int64_t)tj * BN * ld * P;
         int b0 = 0, blocks = ld * P / 64;
         if constexpr (SHARE == SLICE) {
-            const int s = blockIdx.z, all = blocks;
-            b0 = (int)((int64_t)all * s / a.slices);
-            blocks = (int)((int64_t)all * (s + 1) / a.slices);
+            const int all = blocks;
+            b0 = (int)((int64_t)all * slice / a.slices);
+            blocks = (int)((int64_t)all * (slice + 1) / a.slices);
         }
         // A load instruction of a wave brings eight rows of 128 bytes.
         constexpr int loads = (BM + BN) / 8 / waves;
@@ -236,12 +247,12 @@ __global__ __launch_bounds__(64 * WR * WC) void product_kernel(const Args a) {
 #pragma unroll
         for (int i = 0; i < loads; ++i) {
             const int row = 8 * (wave + i * waves) + (lane >> 3), piece = (lane & 7) ^ ((row >> 1) & 7);
-            from[i] = (uint32_t)(row < BM ? row : row - BM) * (uint32_t)(ld * P) + 8 * piece;
+            from[i] = (uint32_t)(row < BM ? row : row - BM) * (uint32_t)(ld * P * 2) + 16 * piece;  // in bytes
         }
         auto fetch = [&](int block, int buf) {
 #pragma unroll
             for (int i = 0; i < loads; ++i)
-                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)((i * waves * 8 < BM ? left : right) + 64 * (int64_t)block + from[i]),
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)((const char*)((i * waves * 8 < BM ? left : right) + 64 * (int64_t)block) + from[i]),
                                                  (__attribute__((address_space(3))) void*)(lds[buf] + 1024 * (wave + i * waves)), 16, 0, 0);
         };
         const int row_l = (wave / WC) * (BM / WR) + n, row_r = BM + (wave % WC) * (BN / WC) + n;
@@ -286,38 +297,71 @@ __global__ __launch_bounds__(64 * WR * WC) void product_kernel(const Args a) {
                 multiply(l1, r1);
             }
         } else {
-            // Every step fetches, past the end the last 64 again, so that the number of loads under
-            // way is the same at every wait.
-#pragma unroll
-            for (int i = 0; i + 1 < stages; ++i) fetch(min(b0 + i, blocks - 1), i);
-            for (int b = b0, buf = 0; b < blocks; ++b, buf = buf + 1 == stages ? 0 : buf + 1) {
-                // This step's operands are here, and the last step's are read: all waves' after the barrier.
-                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((stages - 2) * loads) : "memory");
+            // A step is 64 of the contraction of one part, or 32 of two. Its operands are read while the
+            // step before is multiplied, and `stages` more steps are in LDS or on their way. Every step
+            // fetches, past the end the last one again, so that the number of loads under way is the same at
+            // every wait. The products are spread between the LDS reads, then between the loads (1000 x 4000
+            // 438 us with the reads of a step before its products, 361 so).
+            constexpr int products = (P == 1 ? 2 : 3) * TM * TN, reads = 2 * (TM + TN);
+            struct Operands {
+                h8 l[2][TM], r[2][TN];
+            } now, next;
+            auto read = [&](int buf, Operands& o) {
                 const char* at = lds[buf];
-                auto piece = [&](int row, int c) { return *reinterpret_cast<const h8*>(at + row * 128 + ((c ^ ((row >> 1) & 7)) << 4)); };
 #pragma unroll
-                for (int s = 0; s < (P == 1 ? 2 : 1); ++s) {
-                    h8 l[P][TM], r[P][TN];
+                for (int p = 0; p < 2; ++p) {
+                    const int c = 4 * p + g;
 #pragma unroll
-                    for (int p = 0; p < P; ++p) {
-                        const int c = 4 * (P == 1 ? s : p) + g;
-#pragma unroll
-                        for (int i = 0; i < TM; ++i) l[p][i] = piece(row_l + 16 * i, c);
-#pragma unroll
-                        for (int j = 0; j < TN; ++j) r[p][j] = piece(row_r + 16 * j, c);
+                    for (int i = 0; i < TM; ++i) {
+                        const int row = row_l + 16 * i;
+                        o.l[p][i] = *reinterpret_cast<const h8*>(at + row * 128 + ((c ^ ((row >> 1) & 7)) << 4));
                     }
-                    if (s == 0) fetch(min(b + stages - 1, blocks - 1), buf == 0 ? stages - 1 : buf - 1);
+#pragma unroll
+                    for (int j = 0; j < TN; ++j) {
+                        const int row = row_r + 16 * j;
+                        o.r[p][j] = *reinterpret_cast<const h8*>(at + row * 128 + ((c ^ ((row >> 1) & 7)) << 4));
+                    }
+                }
+            };
+            int buf = 0;  // of this step
+            auto step = [&](int b, Operands& x, Operands& y) {
+                // The next step's operands are here, and this step's are read: all waves' after the barrier.
+                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((stages - 2) * loads) : "memory");
+                const int other = buf + 1 == stages ? 0 : buf + 1;
+                read(other, y);  // past the end: read and not used
+                fetch(min(b + stages, blocks - 1), buf);
+                buf = other;
+#pragma unroll
+                for (int p = P == 1 ? 1 : 2; p >= 0; --p)  // two parts: second by first, first by second, first by first
 #pragma unroll
                     for (int i = 0; i < TM; ++i)
 #pragma unroll
-                        for (int j = 0; j < TN; ++j) {
-                            if constexpr (P == 2) {
-                                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(l[1][i], r[0][j], acc[i][j], 0, 0, 0);
-                                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(l[0][i], r[1][j], acc[i][j], 0, 0, 0);
-                            }
-                            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(l[0][i], r[0][j], acc[i][j], 0, 0, 0);
-                        }
+                        for (int j = 0; j < TN; ++j)
+                            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x.l[P == 1 ? p : p >> 1][i], x.r[P == 1 ? p : p & 1][j], acc[i][j], 0, 0, 0);
+#pragma unroll
+                for (int i = 0; i < reads; ++i) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // a product,
+                    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // an LDS read
                 }
+#pragma unroll
+                for (int i = 0; i < loads; ++i) {
+                    if constexpr (products - reads >= loads) __builtin_amdgcn_sched_group_barrier(0x008, (products - reads) / loads, 0);  // some products,
+                    __builtin_amdgcn_sched_group_barrier(0x010, 1, 0);                                                                   // a load
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            };
+#pragma unroll
+            for (int i = 0; i < stages; ++i) fetch(min(b0 + i, blocks - 1), i);
+            asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((stages - 1) * loads) : "memory");
+            read(0, now);
+            int b = b0;
+            if ((blocks - b0) & 1) {
+                step(b++, now, next);
+                now = next;
+            }
+            for (; b < blocks; b += 2) {
+                step(b, now, next);
+                step(b + 1, next, now);
             }
             // No load may still write the LDS when the workgroup's share of it is handed on.
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -325,7 +369,7 @@ __global__ __launch_bounds__(64 * WR * WC) void product_kernel(const Args a) {
     }
 
     if constexpr (SHARE == SLICE) {
-        f4* to = sums(blockIdx.z);
+        f4* to = sums(slice);
 #pragma unroll
         for (int i = 0; i < TM; ++i)
 #pragma unroll
@@ -335,71 +379,108 @@ __global__ __launch_bounds__(64 * WR * WC) void product_kernel(const Args a) {
     // Products of two numbers at kScale: once too much.
     const float down = 1.0f / kScale;
     const int q = n & 3, qc = n & 12;
+    // What the results are added to is read for `batch` rows of tiles before any of them is stored: a
+    // read behind a store waits for memory each time (B X of 4096 x 4096: 165 us so, 147 in batches).
+    constexpr int batch = TM < 4 ? TM : 4;
 #pragma unroll
-    for (int i = 0; i < TM; ++i)
+    for (int i1 = 0; i1 < TM; i1 += batch) {
+        f4 old[batch][TN];
+        auto row_of = [&](int i) { return ti * BM + (wave / WC) * (BM / WR) + 16 * (i0 + i1 + i) + 4 * g; };
+        auto col_of = [&](int j) { return tj * BN + (wave % WC) * (BN / WC) + 16 * j; };
+        auto master = [&](int i, int j) { return reinterpret_cast<f4*>(a.master + (k * a.np + col_of(j) + n) * a.mp + row_of(i)); };
 #pragma unroll
-        for (int j = 0; j < TN; ++j) {
-            const int row0 = ti * BM + (wave / WC) * (BM / WR) + 16 * i + 4 * g, col0 = tj * BN + (wave % WC) * (BN / WC) + 16 * j;
-            f4 v = acc[i][j] * down;
-            if constexpr (half) {
-                _Float16* to = (KIND == GRAM ? a.gram : a.poly) + k * a.mp * a.mp * P;
-                if constexpr (KIND == POLY) v = a.in.b * get4<P>(a.gram + k * a.mp * a.mp * P + place<P>(col0 + n, row0, a.mp)) + a.in.c * v;
-                put4<P>(to + place<P>(col0 + n, row0, a.mp), v);  // the mirrored tile (of a diagonal tile, the same)
-                if (ti != tj) put4<P>(to + place<P>(row0 + q, col0 + qc, a.mp), turn(v, lane));
-            } else {
-                f4* x = reinterpret_cast<f4*>(a.master + (k * a.np + col0 + n) * a.mp + row0);
-                v += a.in.a * *x;
-                if constexpr (KIND == NEXT) {
-                    *x = v;
-                    put4<P>(a.xt2 + k * a.mp * a.np * P + place<P>(col0 + n, row0, a.mp), v);
-                    put4<P>(a.x + k * a.mp * a.np * P + place<P>(row0 + q, col0 + qc, a.np), turn(v, lane));
+        for (int i = 0; i < batch; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j) {
+                if constexpr (KIND == POLY) old[i][j] = get4<P>(a.gram + k * a.mp * a.mp * P + place<P>(col_of(j) + n, row_of(i), a.mp));
+                if constexpr (!half) old[i][j] = *master(i, j);
+            }
+#pragma unroll
+        for (int i = 0; i < batch; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j) {
+                const int row0 = row_of(i), col0 = col_of(j);
+                f4 v = acc[i1 + i][j] * down;
+                if constexpr (half) {
+                    _Float16* to = (KIND == GRAM ? a.gram : a.poly) + k * a.mp * a.mp * P;
+                    if constexpr (KIND == POLY) v = a.in.b * old[i][j] + a.in.c * v;
+                    put4<P>(to + place<P>(col0 + n, row0, a.mp), v);  // the mirrored tile (of a diagonal tile, the same)
+                    if (ti != tj) put4<P>(to + place<P>(row0 + q, col0 + qc, a.mp), turn(v, lane));
                 } else {
-                    typedef typename Elem<TY>::type E;
-                    // Four consecutive values along the dimension of out that is dense.
-                    const bool along_rows = a.flip ? a.in.out_stride[2] == 1 : a.in.out_stride[1] == 1;
-                    const f4 w = (along_rows ? v : turn(v, lane)) * down;
-                    const int row = along_rows ? row0 : row0 + q, col = along_rows ? col0 + n : col0 + qc;
-                    const int64_t sr = a.in.out_stride[a.flip ? 2 : 1], sc = a.in.out_stride[a.flip ? 1 : 2];
-                    E* to = (E*)a.in.out + k * a.in.out_stride[0] + row * sr + col * sc;
-                    const int64_t step = along_rows ? sr : sc;
-                    const int left = along_rows ? (col < a.n ? a.m - row : 0) : (row < a.m ? a.n - col : 0);
-                    if (a.out_vec && left >= 4) {
-                        if constexpr (TY == T_F32) *reinterpret_cast<f4*>(to) = w;
-                        else {
-                            u2 e;
-#pragma unroll
-                            for (int r = 0; r < 2; ++r)
-                                e[r] = (uint32_t)__builtin_bit_cast(uint16_t, Elem<TY>::put(w[2 * r])) |
-                                       (uint32_t)__builtin_bit_cast(uint16_t, Elem<TY>::put(w[2 * r + 1])) << 16;
-                            *reinterpret_cast<u2*>(to) = e;
-                        }
+                    v += a.in.a * old[i][j];
+                    if constexpr (KIND == NEXT) {
+                        *master(i, j) = v;
+                        put4<P>(a.xt2 + k * a.mp * a.np * P + place<P>(col0 + n, row0, a.mp), v);
+                        put4<P>(a.x + k * a.mp * a.np * P + place<P>(row0 + q, col0 + qc, a.np), turn(v, lane));
                     } else {
+                        typedef typename Elem<TY>::type E;
+                        // Four consecutive values along the dimension of out that is dense.
+                        const bool along_rows = a.flip ? a.in.out_stride[2] == 1 : a.in.out_stride[1] == 1;
+                        const f4 w = (along_rows ? v : turn(v, lane)) * down;
+                        const int row = along_rows ? row0 : row0 + q, col = along_rows ? col0 + n : col0 + qc;
+                        const int64_t sr = a.in.out_stride[a.flip ? 2 : 1], sc = a.in.out_stride[a.flip ? 1 : 2];
+                        E* to = (E*)a.in.out + k * a.in.out_stride[0] + row * sr + col * sc;
+                        const int64_t step = along_rows ? sr : sc;
+                        const int left = along_rows ? (col < a.n ? a.m - row : 0) : (row < a.m ? a.n - col : 0);
+                        if (a.out_vec && left >= 4) {
+                            if constexpr (TY == T_F32) *reinterpret_cast<f4*>(to) = w;
+                            else {
+                                u2 e;
 #pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            if (r < left) to[r * step] = Elem<TY>::put(w[r]);
+                                for (int r = 0; r < 2; ++r)
+                                    e[r] = (uint32_t)__builtin_bit_cast(uint16_t, Elem<TY>::put(w[2 * r])) |
+                                           (uint32_t)__builtin_bit_cast(uint16_t, Elem<TY>::put(w[2 * r + 1])) << 16;
+                                *reinterpret_cast<u2*>(to) = e;
+                            }
+                        } else {
+#pragma unroll
+                            for (int r = 0; r < 4; ++r)
+                                if (r < left) to[r * step] = Elem<TY>::put(w[r]);
+                        }
                     }
                 }
             }
-        }
+    }
 }
 
 struct Plan {
     int m, n, mp, np, parts;
-    int slices;  // of X X^T
+    int gram, slices;  // X X^T: tile, slices
     uint64_t norm, master, x, square, sums;  // bytes: partial norms, X in fp32, X as an operand, m x m as an operand, slices' sums
 };
 
-// Tiles of 64, 128 or (one part) 256 squared, the largest that makes enough blocks: one a CU of 128
-// squared (2048 x 2048, one part: B X 36 us with 128, 38 with 64; two parts, whose steps are three
-// times as long, need two to overlap: 82 us with 128, 68 with 64); half the CUs of 256 squared (4096
-// x 4096: the symmetric products have 136 such blocks and take 90 us, 103 with 128; B X 128 and 149).
+// Tiles of 64, 128 or (one part) 256 squared, the largest that makes enough blocks. 256: half the
+// CUs (4096 x 4096, whose symmetric products have 136 such tiles: 1657 us, 1932 with 128). 128 of one
+// part: two blocks a CU (1536 x 6144 588 us, 600 with 64; 2048 x 2048, one block a CU, 434 and 422).
+// 128 of two parts, which do three products for two: half the CUs (2048 x 2048 715 us, 773 with 64).
+int64_t tiles_of(const Plan& p, uint32_t count, bool half, int t) {
+    const int64_t r = p.mp / t, c = p.np / t;
+    return (half ? r * (r + 1) / 2 : r * c) * count;
+}
 int tile_of(const Plan& p, uint32_t count, bool half) {
-    auto tiles = [&](int t) {
-        const int64_t r = p.mp / t, c = p.np / t;
-        return (half ? r * (r + 1) / 2 : r * c) * count;
-    };
-    if (p.parts == 1 && p.mp % 256 == 0 && p.np % 256 == 0 && tiles(256) >= 128) return 256;
-    return tiles(128) >= (p.parts == 1 ? 256 : 512) ? 128 : 64;
+    if (p.mp % 128) return 64;
+    if (p.parts == 1 && p.mp % 256 == 0 && p.np % 256 == 0 && tiles_of(p, count, half, 256) >= 128) return 256;
+    return tiles_of(p, count, half, 128) >= (p.parts == 1 ? 512 : 128) ? 128 : 64;
+}
+// Of X X^T, whose contraction is the longer dimension, also the slices. With tiles of 128 as many as
+// fill the CUs once, of at least 16 steps (1000 x 4000 361 us, 382 without; 640 x 4000, which would
+// come to 105 blocks, 275 so and 251 with 64). With tiles of 64 up to one block a CU, where that spares a
+// block 24 steps, more than the join costs (512 x 2048 162 us, 193 without; four of 512 x 512, 8 of 16
+// steps spared, 170 and 153).
+void slice(Plan& p, uint32_t count) {
+    const int64_t steps = (int64_t)p.np * p.parts / 64;
+    p.slices = 1;
+    if (p.parts == 2 && p.mp % 128 == 0) {
+        const int64_t tiles = tiles_of(p, count, true, 128);
+        p.gram = 128;
+        p.slices = (int)std::max<int64_t>(1, std::min(256 / tiles, steps / 16));
+        if (tiles * p.slices >= 128) return;
+    }
+    p.gram = tile_of(p, count, true);
+    const int64_t tiles = tiles_of(p, count, true, p.gram);
+    p.slices = 1;
+    while (p.gram < 256 && p.slices < 16 && tiles * p.slices * 2 <= 256 && steps / (p.slices * 2) >= 8) p.slices *= 2;
+    if (steps - steps / p.slices < 24) p.slices = 1;
 }
 
 Plan plan_of(const ZenoAmdOrthogonalize& a) {
@@ -414,25 +495,19 @@ Plan plan_of(const ZenoAmdOrthogonalize& a) {
     p.master = (uint64_t)a.count * p.mp * p.np * 4;
     p.x = (uint64_t)a.count * p.mp * p.np * p.parts * 2;
     p.square = (uint64_t)a.count * p.mp * p.mp * p.parts * 2;
-    const int t = tile_of(p, a.count, true);
-    const uint64_t r = p.mp / t, tiles = r * (r + 1) / 2 * a.count, blocks = (uint64_t)p.np * p.parts / 64;
-    // Two blocks a CU, at least eight steps of the contraction each; tiles of 256 are enough as they are.
-    p.slices = 1;
-    while (t < 256 && p.slices < 16 && tiles * p.slices * 2 <= 512 && blocks / (p.slices * 2) >= 8) p.slices *= 2;
-    p.sums = p.slices > 1 ? tiles * p.slices * t * t * 4 : 0;
+    slice(p, a.count);
+    p.sums = p.slices > 1 ? (uint64_t)tiles_of(p, a.count, true, p.gram) * p.slices * p.gram * p.gram * 4 : 0;
     return p;
 }
 
-template <int TY, int P, int KIND, int SHARE> void product(const Args& a, int tile, int slices, hipStream_t stream) {
-    const int rows = a.mp / tile, cols = a.np / tile;
-    const dim3 grid(KIND == GRAM || KIND == POLY ? rows * (rows + 1) / 2 : rows * cols, a.in.count, slices);
-    // Small tiles do little between two barriers. Where they do not fill the GPU twice, their operands
-    // are on their way for three steps (1000 x 4000: X X^T 31 us, 39 with one step); where they do, four
-    // blocks a CU instead of two serve better (B X 45, 48).
-    if (tile == 64 && (int64_t)grid.x * grid.y * grid.z <= 768) product_kernel<TY, P, 64, 64, 2, 2, 4, KIND, SHARE><<<grid, 256, 0, stream>>>(a);
-    else if (tile == 64) product_kernel<TY, P, 64, 64, 2, 2, 2, KIND, SHARE><<<grid, 256, 0, stream>>>(a);
-    else if (tile == 128) product_kernel<TY, P, 128, 128, 2, 2, 2, KIND, SHARE><<<grid, 256, 0, stream>>>(a);
-    else if constexpr (P == 1 && SHARE == WHOLE) product_kernel<TY, P, 256, 256, 2, 4, 2, KIND, SHARE><<<grid, 512, 0, stream>>>(a);
+template <int TY, int P, int KIND, int SHARE> void product(const Args& a, int tile, hipStream_t stream) {
+    const int rows = a.mp / tile, cols = a.np / tile, tiles = KIND == GRAM || KIND == POLY ? rows * (rows + 1) / 2 : rows * cols;
+    const dim3 grid(SHARE == SLICE ? tiles * a.slices : tiles, a.in.count, SHARE == JOIN ? tile / 32 : 1);  // a join: a block for each row of result tiles of a wave
+    if (tile == 64) product_kernel<TY, P, 64, 64, 2, 2, 4, KIND, SHARE><<<grid, 256, 0, stream>>>(a);
+    if constexpr (P == 2 || SHARE == WHOLE)
+        if (tile == 128) product_kernel<TY, P, 128, 128, 2, 2, 3, KIND, SHARE><<<grid, 256, 0, stream>>>(a);
+    if constexpr (P == 1 && SHARE == WHOLE)
+        if (tile == 256) product_kernel<TY, P, 256, 256, 2, 4, 2, KIND, SHARE><<<grid, 512, 0, stream>>>(a);
 }
 
 template <int TY, int P> hipError_t launch(Args a, const Plan& p, hipStream_t stream) {
@@ -441,14 +516,14 @@ template <int TY, int P> hipError_t launch(Args a, const Plan& p, hipStream_t st
     load_kernel<TY, P><<<dim3(a.np / 64, a.mp / 64, a.in.count), 256, 0, stream>>>(a);
     for (uint32_t s = 0; s < a.in.steps; ++s) {
         if (p.slices == 1) {
-            product<TY, P, GRAM, WHOLE>(a, square, 1, stream);
+            product<TY, P, GRAM, WHOLE>(a, p.gram, stream);
         } else {
-            product<TY, P, GRAM, SLICE>(a, square, p.slices, stream);
-            product<TY, P, GRAM, JOIN>(a, square, 1, stream);
+            product<TY, P, GRAM, SLICE>(a, p.gram, stream);
+            product<TY, P, GRAM, JOIN>(a, p.gram, stream);
         }
-        product<TY, P, POLY, WHOLE>(a, square, 1, stream);
-        if (s + 1 < a.in.steps) product<TY, P, NEXT, WHOLE>(a, whole, 1, stream);
-        else product<TY, P, LAST, WHOLE>(a, whole, 1, stream);
+        product<TY, P, POLY, WHOLE>(a, square, stream);
+        if (s + 1 < a.in.steps) product<TY, P, NEXT, WHOLE>(a, whole, stream);
+        else product<TY, P, LAST, WHOLE>(a, whole, stream);
         std::swap(a.xt, a.xt2);
     }
     return hipGetLastError();
@@ -504,10 +579,10 @@ hipError_t run(const ZenoAmdOrthogonalize& in, void* workspace, hipStream_t stre
     a.x = (_Float16*)at;
     a.xt = (_Float16*)(at + p.x);
     a.xt2 = (_Float16*)(at + 2 * p.x);
+    a.slices = p.slices;
     a.gram = (_Float16*)(at + 3 * p.x);
     a.poly = (_Float16*)(at + 3 * p.x + p.square);
     a.sums = (float*)(at + 3 * p.x + 2 * p.square);
-    a.slices = p.slices;
     const uint64_t four = in.dtype == T_F32 ? 16 : 8;
     const int64_t* s = in.out_stride;
     const int other = (a.flip ? s[2] : s[1]) == 1 ? (a.flip ? 1 : 2) : (a.flip ? 2 : 1);  // the dimension that the stores do not run along
