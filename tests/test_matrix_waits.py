@@ -98,10 +98,9 @@ def test_the_check_sees_a_missing_wait():
 @pytest.mark.skipif(not (shutil.which("hipcc") or shutil.which("/opt/rocm/bin/hipcc")), reason="no hipcc")
 def test_every_kernel_of_the_policy_operators_waits():
     sources = [s for s in build.POLICY_SOURCES if s != "delta.hip"]
-    flags = [f for f in build.POLICY_FLAGS if f not in ("-fPIC", "-Wall")]
 
     def assembly(source):
-        return subprocess.run([build._hipcc(), *flags, "-w", "--cuda-device-only", "-S", "-o", "-", str(build.CSRC / source)],
+        return subprocess.run([build._hipcc(), *(f for f in build.policy_flags(source) if f not in ("-fPIC", "-Wall")), "-w", "--cuda-device-only", "-S", "-o", "-", str(build.CSRC / source)],
                               capture_output=True, text=True, check=True).stdout
 
     with ThreadPoolExecutor(len(sources)) as pool:

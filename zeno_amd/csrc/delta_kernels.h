@@ -116,14 +116,20 @@ template <int TY, int DK, int NW, int TILES> struct Rows {
     }
 };
 
-// A double from other lanes: shifted up by CTRL - 0x110 lanes within each 16 (zeros come in), or
-// (0x142) the last lane of the 16 before, in every second 16.
+// A double from other lanes: shifted up by CTRL - 0x110 lanes or down by CTRL - 0x100 within each 16
+// (zeros come in), or (0x142) the last lane of the 16 before, in every second 16.
 template <int CTRL> __device__ __forceinline__ double dpp64(double x) {
     constexpr int rows = CTRL == 0x142 ? 0xa : 0xf;
     const uint64_t b = __builtin_bit_cast(uint64_t, x);
     const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, rows, 0xf, CTRL != 0x142);
     const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), CTRL, rows, 0xf, CTRL != 0x142);
     return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+
+__device__ __forceinline__ double from_lane(double x, int lane) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, x);
+    return __builtin_bit_cast(double, (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(b >> 32), lane) << 32 |
+                                          (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)b, lane));
 }
 
 // g and beta of a chunk (one lane a token, one wave): sums in 64 bits.
@@ -136,9 +142,7 @@ __device__ __forceinline__ void load_scalars(float g, float beta, int lane, bool
     sum += dpp64<0x114>(sum);
     sum += dpp64<0x118>(sum);
     if constexpr (TILES == 2) sum += dpp64<0x142>(sum);
-    const uint64_t b = __builtin_bit_cast(uint64_t, sum);
-    const double all = __builtin_bit_cast(double, (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(b >> 32), C - 1) << 32 |
-                                                      (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)b, C - 1));
+    const double all = from_lane(sum, C - 1);
     if (lane < C) {
         const float hi = (float)sum;
         s.hi[lane] = hi;
@@ -948,10 +952,13 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || sizeof(BackwardLds<TY, DK, NW, 
             if (lane == C - 1)
 #pragma unroll
                 for (int w = 0; w < NW; ++w) sum += (double)lds.edge[w];
-#pragma unroll
-            for (int d = 1; d < C; d <<= 1) {
-                const double dn = __shfl_down(sum, d);
-                if (lane + d < C) sum += dn;
+            sum += dpp64<0x101>(sum);
+            sum += dpp64<0x102>(sum);
+            sum += dpp64<0x104>(sum);
+            sum += dpp64<0x108>(sum);
+            if constexpr (TILES == 2) {
+                const double behind = from_lane(sum, 16);
+                if (lane < 16) sum += behind;
             }
             if (lane < len) {
                 ap->dg[b * ap->dg_stride[0] + (t + lane) * ap->dg_stride[1] + h * ap->dg_stride[2]] = first && lane == 0 ? 0.0f : (float)sum;

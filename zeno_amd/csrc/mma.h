@@ -279,10 +279,15 @@ template <int P> __device__ __forceinline__ void put4(uint16_t* at, int part, f4
 #pragma unroll
     for (int p = 0; p < P; ++p) *reinterpret_cast<u2*>(at + p * part) = h.p[p];
 }
+// Sum over the wave; every lane gets it.
 __device__ __forceinline__ float sum64(float x) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d);
-    return x;
+    x = sum16(x);
+    uint32_t b = __float_as_uint(x);
+    auto rows = __builtin_amdgcn_permlane16_swap(b, b, false, false);  // the 16 lanes before and after, in pairs
+    x = __uint_as_float(rows[0]) + __uint_as_float(rows[1]);
+    b = __float_as_uint(x);
+    rows = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+    return __uint_as_float(rows[0]) + __uint_as_float(rows[1]);
 }
 
 }  // namespace mma
