@@ -4,6 +4,8 @@ The step runs as hand-written HIP kernels behind libzeno.so, whose C ABI matches
 reference's (include/zeno.h). This package holds the build script, the ctypes bindings,
 the ZenoWorld mirror of the reference's python/zeno/_ffi.py, the batched ZenoEnv / make of
 python/zeno/env.py and the Gymnasium-style environments of python/zeno/gym (zeno_amd.gym).
+zeno_amd.memory and zeno_amd.optim (imported on their own: they need torch) hold the operators of
+policies with memory and of their updates.
 """
 from pathlib import Path
 

@@ -55,9 +55,9 @@ void set_strides(int64_t* to, const int64_t* from) {
 
 // 16 tokens a chunk where 32 do not fit the 160 KB of a CU in the gradients' kernel. Segments:
 // with fewer heads than the GPU holds workgroups (one of eight waves a CU, two of four), as many as
-// fill it, of at least three chunks (4 heads of 1000 tokens forward: 47 us with three, 77 with eight;
-// 76 heads of 333 with gradients 281 and 393). The additional pass over the tokens costs as much as
-// it saves where fewer than three segments come of it.
+// fill it, of at least three chunks (4 heads of 1000 tokens forward: 40 us with three, 64 with eight, 125
+// in one segment; 76 heads of 333 with gradients 251 and 352). The additional pass over the tokens costs as
+// much as it saves where fewer than three segments come of it (111 heads of 211: 48 us in one, 53 in two).
 Shape shape_of(const ZenoAmdDeltaInputs& in, bool train) {
     Shape s;
     s.dk = in.key_dim <= 64 ? 64 : 128;

@@ -9,9 +9,9 @@
 // value columns and keeps their state in registers as result tiles; every right operand is its
 // own registers' content (mma.h), and the waves of a workgroup share only the left operands, in
 // LDS: K, Q, K^T, the decayed Q K^T, Z below the diagonal tile, and the inverses of the 16x16
-// diagonal tiles of I + Z B. Those come from forward substitution, 16 columns in 16 lanes: the
-// cheaper product of powers (I - N)(I + N^2)... loses all digits where keys repeat, as they do
-// for an environment that stands still.
+// diagonal tiles of I + Z B. Those come from forward substitution in registers: the cheaper
+// product of powers (I - N)(I + N^2)... loses all digits where keys repeat, as they do for an
+// environment that stands still.
 //
 // A chunk ends at a token of the grid of C and before every reset, so nothing is masked inside
 // it and no value from before a reset is ever multiplied by a zero. Partial chunks are filled
@@ -373,7 +373,12 @@ template <int TY, int DK, int NW, int TILES> struct ForwardLds {
     Scalars<TILES> s;
 };
 
-// FULL: heads of exactly DK and 16 NW dimensions, aligned, need no masks (a fifth of the instructions).
+// What bounds it: of many short sequences memory (16384 of 16 tokens, 4 heads of 64 x 64, bfloat16:
+// 320 us, 4.1 TB/s of inputs, outputs and states; a large copy reaches 5.1), else a chunk's chain of
+// dependent products and exchanges, about 10,000 cycles with two workgroups a CU taking turns (4096
+// of 32 tokens, four heads, with the states for the gradients: 248 us).
+// FULL: heads of exactly DK and 16 NW dimensions, aligned, need no masks: a quarter of the
+// instructions less (3345 and 4595 of 64 x 64, bfloat16).
 // Waves a SIMD that the registers are cut down to: as many workgroups as fit the LDS, but not more
 // than the registers bear (128 of four waves spill in the wide kernel with outputs).
 constexpr int forward_waves(int waves, bool states, size_t lds) {
@@ -532,7 +537,9 @@ __global__ __launch_bounds__(64 * NW, forward_waves(NW, STATES, sizeof(ForwardLd
 // BACK: the same for the state's gradient from the last segment to the first, with M transposed.
 // A workgroup joins 16 value columns of a head. Its four waves share the rows of the result; each
 // step's state reaches them as a right operand through LDS, the matrices come from memory a step
-// ahead. One step is DK / 64 x DK / 32 x 6 dependent-free matrix instructions a wave.
+// ahead. One step is DK / 64 x DK / 32 x 6 dependent-free matrix instructions a wave. Bound by how fast
+// one CU draws the matrices in: 106 KB in 1.9 us of 128 x 128, the same with loads two steps ahead (8
+// heads, 32 segments: 56 us). More workgroups would each read all of a head's matrices again.
 template <int DK, int DV, bool BACK>
 __global__ __launch_bounds__(256) void delta_join_kernel(float* states, const float* jumps, int segments) {
     typedef Jump<DK> J;
@@ -600,6 +607,9 @@ __global__ __launch_bounds__(256) void delta_join_kernel(float* states, const fl
 // transposed) go through LDS (phase B). Phase A feeds fp32 results and takes three parts; phase
 // B feeds results of the element type alone and takes `NO` parts: two for 16-bit types, 2^-17 of
 // each operand against the 2^-9 or 2^-12 of the results' own rounding.
+// What bounds it: two workgroups a CU, as LDS and registers allow, each going through some 30,000
+// cycles a chunk between barriers, half of them waiting on LDS and products (4096 sequences of 32,
+// four heads of 64 x 64, bfloat16: 840 us, about 1.3 TB/s; 2 of 4096, 8 heads of 128 x 128: 231).
 template <int TY, int DK, int NW, int TILES> struct BackwardLds {
     typedef Geo<TY, DK, NW, TILES> G;
     static constexpr int NO = TY == T_F32 ? 3 : 2;
@@ -664,7 +674,8 @@ __device__ __forceinline__ void pull_state(const uint16_t* KT, const uint16_t* Q
 
 // The gradient of the state alone, for the segments: of every segment but the first, what its
 // outputs (and, of the last, d_last) add to the gradient of the state before it. It needs neither
-// states nor values.
+// states nor values: 71 us where the gradients' own pass takes 231 (2 sequences of 4096, 8 heads of
+// 128 x 128, bfloat16).
 template <int TY, int DK, int NW, int TILES> struct PullLds {
     typedef Geo<TY, DK, NW, TILES> G;
     alignas(16) uint16_t K[G::NP * G::C * G::KS], Q[G::NP * G::C * G::KS], KT[G::NP * DK * G::TS], QT[G::NP * DK * G::TS];
@@ -1119,7 +1130,9 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || sizeof(BackwardLds<TY, DK, NW, 
     }
     if (ap->d_state && segment == 0) store_state<DK, G::DV, FULL>(ap->d_state + bh * dk * dv, dk, dv, dv, col0, lane, dS);
 }
-// Sums the value heads of each key head, in their order; one thread a value.
+
+// Sums the value heads of each key head, in their order; one thread a value. Memory-bound and small: 4 us
+// of 250 (19 sequences of 333 tokens, two value heads a key head, fp32).
 template <int TY> __global__ __launch_bounds__(256) void delta_share_kernel(const Args a) {
     typedef typename Elem<TY>::type E;
     const ZenoAmdDeltaInputs& in = a.in;
