@@ -1,11 +1,16 @@
 """The gated delta rule's entry points on the CPU: argument checks that come before any GPU
 work, and the sizes of what training keeps."""
 import ctypes as C
+import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 import torch
 
 from zeno_amd import _lib, memory
+
+ROOT = Path(__file__).resolve().parent.parent
 
 
 def args(**change):
@@ -74,3 +79,16 @@ def test_segments_of_long_sequences(lib):
     assert "workspace" in _lib.last_error()
     assert lib.zeno_amd_delta_forward(long, 16, (C.c_int64 * 3)(), 16, None, 8, None) == -6
     assert lib.zeno_amd_delta_workspace_bytes(args(batch=512, length=4096, key_heads=4)) == 0
+
+
+@pytest.mark.parametrize("module", ["memory", "optim"])
+def test_torch_has_to_come_before_the_library(module):
+    """Two HIP runtimes in one process are refused by name, one shared by both is not."""
+    def run(first, then):
+        return subprocess.run([sys.executable, "-c", f"{first}; {then}"], cwd=ROOT, capture_output=True, text=True)
+
+    load, use = "from zeno_amd import _lib; _lib.load()", f"import zeno_amd.{module}"
+    late = run(load, use)
+    assert late.returncode == 1 and "import torch before" in late.stderr, late.stderr
+    early = run("import torch", f"{load}; {use}")
+    assert early.returncode == 0, early.stderr

@@ -245,5 +245,16 @@ def load() -> C.CDLL:
     return lib
 
 
+def one_runtime() -> None:
+    """Raises where libzeno.so was loaded before torch. Torch's packages bring a HIP runtime of
+    their own: loaded first it is the one that libzeno.so uses too, loaded later it is a second
+    one in the process, which sees no GPU."""
+    with open("/proc/self/maps") as maps:
+        files = {line.split()[-1] for line in maps if "/libamdhip64.so" in line}
+    if len(files) > 1:
+        raise ImportError("two HIP runtimes are loaded (" + ", ".join(sorted(files)) +
+                          "): import torch before the first use of zeno_amd's library")
+
+
 def last_error() -> str:
     return load().zeno_amd_last_error().decode()

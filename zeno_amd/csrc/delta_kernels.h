@@ -373,7 +373,7 @@ template <int TY, int DK, int NW, int TILES> struct ForwardLds {
     Scalars<TILES> s;
 };
 
-// What bounds it: of many short sequences memory (16384 of 16 tokens, 4 heads of 64 x 64, bfloat16:
+// What bounds it: of many short sequences memory (16384 of 16 tokens, two heads of 64 x 64, bfloat16:
 // 320 us, 4.1 TB/s of inputs, outputs and states; a large copy reaches 5.1), else a chunk's chain of
 // dependent products and exchanges, about 10,000 cycles with two workgroups a CU taking turns (4096
 // of 32 tokens, four heads, with the states for the gradients: 248 us).

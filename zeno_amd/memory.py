@@ -37,6 +37,8 @@ import torch
 
 from . import _lib as L
 
+L.one_runtime()
+
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _S3 = C.c_int64 * 3
 _HERE = contextlib.nullcontext()
