@@ -318,3 +318,19 @@ def test_nothing_passes_a_reset_between_segments():
         results.append([o[:, 1300:], s, *(y[:, 1300:] for y in grads)])
     for a, b in zip(*results):
         assert torch.isfinite(a).all() and torch.equal(a, b)
+
+
+@pytest.mark.parametrize("advanced", ["last", "state"])
+def test_a_state_advanced_before_the_backward_pass_is_noticed(advanced):
+    """Steps write the state in place, outside of torch: gradients that would read it are refused."""
+    from zeno_amd.memory import gated_delta as ours, gated_delta_step
+
+    x = torch.randn(2, 9, 3, 16, device="cuda")
+    g = torch.zeros(2, 9, 3, device="cuda")
+    beta = torch.full_like(g, 0.5).requires_grad_()
+    state = torch.randn(2, 3, 16, 16, device="cuda")
+    o, last = ours(x, x, x, g, beta, state=state, normalize=True)
+    token = x[:, 0], x[:, 0], x[:, 0], g[:, 0], beta[:, 0].detach()
+    gated_delta_step(*token, last.detach() if advanced == "last" else state, normalize=True)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        o.sum().backward()

@@ -161,3 +161,14 @@ def test_refusals():
             orthogonalize(*bad)
     with pytest.raises(ValueError, match="out must be"):
         orthogonalize(x, out=x.half())
+
+
+def test_a_matrix_written_in_place_is_noticed():
+    from zeno_amd.optim import orthogonalize
+
+    w = torch.randn(8, 8, device="cuda")
+    x = torch.randn(8, 8, device="cuda", requires_grad=True)
+    y = (x * w).sum()
+    orthogonalize(w, out=w)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()

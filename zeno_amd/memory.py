@@ -42,6 +42,7 @@ L.one_runtime()
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _S3 = C.c_int64 * 3
 _HERE = contextlib.nullcontext()
+_written = torch.autograd.graph.increment_version
 
 
 def _fail(rc: int, what: str) -> None:
@@ -209,4 +210,6 @@ def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
         rc = L.load().zeno_amd_delta_step(a, out.data_ptr(), _S3(os[0], 0, os[1]), state.data_ptr(), _stream(q))
         if rc:
             _fail(rc, "gated_delta_step")
+    _written(state)  # autograd refuses a backward pass that needs what was here
+    _written(out)
     return out

@@ -54,4 +54,5 @@ def orthogonalize(update: torch.Tensor, steps: int = 5, coefficients: Tuple[floa
         raise ValueError(L.last_error())
     if rc:
         raise RuntimeError(f"orthogonalize failed: {rc}: {L.last_error()}")
+    torch.autograd.graph.increment_version(out)  # autograd refuses a backward pass that needs what was here
     return out
