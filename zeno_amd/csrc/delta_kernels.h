@@ -375,7 +375,7 @@ template <int TY, int DK, int NW, int TILES> struct ForwardLds {
 
 // What bounds it: of many short sequences memory (16384 of 16 tokens, two heads of 64 x 64, bfloat16:
 // 320 us, 4.1 TB/s of inputs, outputs and states; a large copy reaches 5.1), else a chunk's chain of
-// dependent products and exchanges, about 10,000 cycles with two workgroups a CU taking turns (4096
+// dependent products and exchanges, of which the workgroups of a CU (four of four waves) take turns (4096
 // of 32 tokens, four heads, with the states for the gradients: 248 us).
 // FULL: heads of exactly DK and 16 NW dimensions, aligned, need no masks: a quarter of the
 // instructions less (3345 and 4595 of 64 x 64, bfloat16).
@@ -398,7 +398,7 @@ __global__ __launch_bounds__(64 * NW, forward_waves(NW, STATES, sizeof(ForwardLd
     const ZenoAmdDeltaInputs& in = a.in;
     const int64_t b = blockIdx.x / in.value_heads, h = blockIdx.x % in.value_heads, hk = h / a.share;
     const int dk = in.key_dim, dv = in.value_dim, segment = blockIdx.y;
-    const int begin = segment * a.segment_length, T = min((int)in.length, begin + a.segment_length);  // this segment's tokens
+    const int begin = segment * a.segment_length, T = begin + min((int)in.length - begin, (int)a.segment_length);  // this segment's tokens
     const bool unit = STATES && blockIdx.z;
     if (unit && segment == 0) return;
     const int col0 = wave * 16, row0 = 4 * g + (n & 3), col = col0 + (n & 12);  // memory: four columns of a row
@@ -704,7 +704,7 @@ __global__ __launch_bounds__(64 * NW) void delta_pull_kernel(const Args a) {
     const ZenoAmdDeltaInputs& in = a.in;
     const int64_t b = blockIdx.x / in.value_heads, h = blockIdx.x % in.value_heads, hk = h / a.share;
     const int dk = in.key_dim, dv = in.value_dim, segment = blockIdx.y + 1;
-    const int begin = segment * a.segment_length, T = min((int)in.length, begin + a.segment_length);
+    const int begin = segment * a.segment_length, T = begin + min((int)in.length - begin, (int)a.segment_length);
     const int col0 = wave * 16, row0 = 4 * g + (n & 3), col = col0 + (n & 12);
     const E* q = (const E*)in.q + b * in.q_stride[0] + hk * in.q_stride[2];
     const E* k = (const E*)in.k + b * in.k_stride[0] + hk * in.k_stride[2];
@@ -772,7 +772,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || sizeof(BackwardLds<TY, DK, NW, 
     ArgsAt ap = (ArgsAt)__builtin_amdgcn_kernarg_segment_ptr();
     const int64_t b = blockIdx.x / ap->in.value_heads, h = blockIdx.x % ap->in.value_heads, hk = h / ap->share;
     const int dk = ap->in.key_dim, dv = ap->in.value_dim, segment = blockIdx.y;
-    const int begin = segment * ap->segment_length, T = min((int)ap->in.length, begin + ap->segment_length);  // this segment's tokens
+    const int begin = segment * ap->segment_length, T = begin + min((int)ap->in.length - begin, (int)ap->segment_length);  // this segment's tokens
     const int col0 = wave * 16, row0 = 4 * g + (n & 3), col = col0 + (n & 12);  // memory: four columns of a row
     const int64_t bh = b * ap->in.value_heads + h;
 
