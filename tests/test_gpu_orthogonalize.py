@@ -172,3 +172,12 @@ def test_a_matrix_written_in_place_is_noticed():
     orthogonalize(w, out=w)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.backward()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("shape", [(40, 250, 310), (50, 320, 250), (64, 380, 450), (130, 100, 180), (70, 128, 192)], ids=str)
+def test_many_matrices_whose_sides_are_odd_numbers_of_small_tiles(shape, dtype):
+    from zeno_amd.optim import orthogonalize
+
+    x = matrices(shape, dtype, seed=7, rank=4)
+    assert_near(orthogonalize(x.cuda()), reference(x), tolerance(x))

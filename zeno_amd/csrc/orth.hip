@@ -459,7 +459,7 @@ int64_t tiles_of(const Plan& p, uint32_t count, bool half, int t) {
     return (half ? r * (r + 1) / 2 : r * c) * count;
 }
 int tile_of(const Plan& p, uint32_t count, bool half) {
-    if (p.mp % 128) return 64;
+    if (p.mp % 128 || (!half && p.np % 128)) return 64;  // sizes are multiples of 64
     if (p.parts == 1 && p.mp % 256 == 0 && p.np % 256 == 0 && tiles_of(p, count, half, 256) >= 128) return 256;
     return tiles_of(p, count, half, 128) >= (p.parts == 1 ? 512 : 128) ? 128 : 64;
 }
