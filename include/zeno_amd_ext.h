@@ -304,9 +304,9 @@ int zeno_amd_delta_step(const ZenoAmdDeltaInputs* in, void* o, const int64_t* o_
  * its Frobenius norm plus eps and then, `steps` times, with rows <= cols (else transposed),
  *     A = X X^T,   X <- a X + (b A + c A A) X,
  * which drives all its singular values towards 1. Products are summed in fp32 (the norm in
- * fp64); for float32 and float16 their operands carry 22 bits, for bfloat16 11. Coefficients
- * that let a singular value of X, or an entry of the products, exceed 32 are refused: the
- * operands are 16-bit numbers at a fixed scale. Strides are in elements (matrix, row, column)
+ * fp64) and their operands carry 22 bits. Coefficients that let a singular value of X, or an
+ * entry of the products, exceed 32 are refused: the operands are pairs of 16-bit numbers at a
+ * fixed scale. Strides are in elements (matrix, row, column)
  * and may be anything; out must not overlap x unless it is the same memory with the same
  * strides. */
 typedef struct {

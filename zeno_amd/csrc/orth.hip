@@ -5,18 +5,17 @@
 // Everything is a matrix product, (m m n + m m m + 2 m m n) operations a step with the symmetric
 // ones done by half, on the fp16 matrix units. Their operands are bounded: no singular value of X
 // exceeds about 1.2 (the host checks the coefficients), so X, A and B are held in fp16 at fixed
-// scales far from either end of its range. X itself stays in fp32 and is what a X adds: a small
-// singular value grows 3.4-fold a step by that term, and with it every rounding of X that the
-// term would carry (results 4.8e-3 off instead of 5e-4 with fp16 there). Operands of two parts
-// carry 22 bits, three of the four part products give fp32's accuracy at a third of the units'
-// rate, five times the fp32 units'. Results of bfloat16, which carry 8 bits, are content with one
-// part of 11 where the roundings average out over enough terms: a smaller dimension of 256 moves
-// them by 2e-4 to 1.6e-3 of their norm (momenta with strong directions to Gaussian matrices; their
-// own rounding is 1.7e-3), 37 by 2.8e-3. Sums are fp32, the norm's fp64.
+// scales far from either end of its range, in two parts that carry 22 bits: three of the four part
+// products give fp32's accuracy at a third of the units' rate, five times the fp32 units'. X itself
+// stays in fp32 and is what a X adds: a small singular value grows 3.4-fold a step by that term, and
+// with it every rounding of X that the term would carry (results 4.8e-3 off instead of 5e-4 with fp16
+// there). bfloat16 takes two parts as well: with one of 11 bits a result of 256 x 512 with 37 rows
+// that are not zero is off by 3.3e-3 of its norm and one of 1024 x 1024 Gaussian values by 1.3e-3,
+// where its own rounding is 1.7e-3; with two, 4e-6. Sums are fp32, the norm's fp64.
 //
 // Layout. X and X^T are both kept as operands (every product then reads two operands along their
-// rows); rows and columns are padded with zeros to the tile. Two parts alternate every 32 columns,
-// so a row's 128 bytes are 64 columns of one part or 32 of two, and both run through the same loop.
+// rows); rows and columns are padded with zeros to the tile. The two parts alternate every 32 columns,
+// so 128 bytes of a row are 32 columns.
 #include <algorithm>
 #include <cmath>
 #include <utility>
@@ -51,13 +50,13 @@ struct Args {
     _Float16* xt2;        // the next X^T (X is no operand of the product that makes the next one)
 };
 
-template <int P> __device__ __forceinline__ int64_t place(int64_t row, int col, int ld) {
-    return row * ld * P + (P == 1 ? col : (col >> 5) * 64 + (col & 31));
-}
-template <int P> __device__ __forceinline__ void put(_Float16* at, float x) {
+constexpr int kParts = 2;           // fp16 numbers that hold a value
+
+__device__ __forceinline__ int64_t place(int64_t row, int col, int ld) { return row * ld * kParts + (col >> 5) * 64 + (col & 31); }
+__device__ __forceinline__ void put(_Float16* at, float x) {
     const _Float16 h = (_Float16)x;
     at[0] = h;
-    if (P == 2) at[32] = (_Float16)(x - (float)h);
+    at[32] = (_Float16)(x - (float)h);
 }
 
 template <int TY> __device__ __forceinline__ float input(const Args& a, int64_t k, int row, int col) {  // of G
@@ -99,8 +98,8 @@ template <int TY> __global__ __launch_bounds__(256) void norm_kernel(const Args 
     if (threadIdx.x == 0) a.partial[k * kNormBlocks + blockIdx.x] = part[0] + part[1] + part[2] + part[3];
 }
 
-// X and X^T in fp16 from G, a 64x64 tile a block. Bound by memory: 4096 x 4096 bfloat16 36 us, 4.6 TB/s.
-template <int TY, int P> __global__ __launch_bounds__(256) void load_kernel(const Args a) {
+// X and X^T in fp16 from G, a 64x64 tile a block. Bound by memory: 4096 x 4096 bfloat16 60 us, 3.9 TB/s.
+template <int TY> __global__ __launch_bounds__(256) void load_kernel(const Args a) {
     __shared__ float tile[64][65];
     const int64_t k = blockIdx.z;
     const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;  // of X
@@ -120,37 +119,32 @@ template <int TY, int P> __global__ __launch_bounds__(256) void load_kernel(cons
         tile[r][c] = v * f;
     }
     __syncthreads();
-    _Float16* x = a.x + k * a.mp * a.np * P;
-    _Float16* xt = a.xt + k * a.mp * a.np * P;
+    _Float16* x = a.x + k * a.mp * a.np * kParts;
+    _Float16* xt = a.xt + k * a.mp * a.np * kParts;
 #pragma unroll
     for (int i = u, t = 0; t < 16; ++t, i += 4) {
         a.master[(k * a.np + c0 + i) * a.mp + r0 + w] = tile[w][i];
-        put<P>(x + place<P>(r0 + i, c0 + w, a.np), tile[i][w]);
-        put<P>(xt + place<P>(c0 + i, r0 + w, a.mp), tile[w][i]);
+        put(x + place(r0 + i, c0 + w, a.np), tile[i][w]);
+        put(xt + place(c0 + i, r0 + w, a.mp), tile[w][i]);
     }
 }
 
 // Four values of a row-major operand row that start at a multiple of four.
-template <int P> __device__ __forceinline__ void put4(_Float16* at, f4 x) {
-    h4 h;
+__device__ __forceinline__ void put4(_Float16* at, f4 x) {
+    h4 h, l;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) h[r] = (_Float16)x[r];
+    for (int r = 0; r < 4; ++r) {
+        h[r] = (_Float16)x[r];
+        l[r] = (_Float16)(x[r] - (float)h[r]);
+    }
     *reinterpret_cast<h4*>(at) = h;
-    if constexpr (P == 2) {
-        h4 l;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) l[r] = (_Float16)(x[r] - (float)h[r]);
-        *reinterpret_cast<h4*>(at + 32) = l;
-    }
+    *reinterpret_cast<h4*>(at + 32) = l;
 }
-template <int P> __device__ __forceinline__ f4 get4(const _Float16* at) {
-    const h4 h = *reinterpret_cast<const h4*>(at);
-    f4 x = {(float)h[0], (float)h[1], (float)h[2], (float)h[3]};
-    if constexpr (P == 2) {
-        const h4 l = *reinterpret_cast<const h4*>(at + 32);
+__device__ __forceinline__ f4 get4(const _Float16* at) {
+    const h4 h = *reinterpret_cast<const h4*>(at), l = *reinterpret_cast<const h4*>(at + 32);
+    f4 x;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) x[r] += (float)l[r];
-    }
+    for (int r = 0; r < 4; ++r) x[r] = (float)h[r] + (float)l[r];
     return x;
 }
 
@@ -194,10 +188,10 @@ enum Share { WHOLE, SLICE, JOIN };  // of the contraction: all of it; a slice, s
 // row number, which leaves the operand reads without bank conflicts. Few tiles with a long
 // contraction are cut into slices along it (SLICE), whose sums another launch adds in their order (JOIN).
 // Bound by the matrix units and the operands' way from L2 together, and at its end by memory: X, X^T and
-// the fp32 X are written at once by all blocks. 4096 x 4096, one part: B X 147 us (0.93 PFLOP/s), the
-// symmetric products 110 and 114 (half the operations; 0.62); 1000 x 4000, two parts: B X 38 us (0.65
-// PFLOP/s of part products, of which 14 are the end), X X^T 18 and 7 for the join.
-template <int TY, int P, int BM, int BN, int WR, int WC, int STAGES, int KIND, int SHARE>
+// the fp32 X are written at once by all blocks. Rates of part products: 4096 x 4096 B X 390 us (1.06
+// PFLOP/s; a large library product of fp16 1.18), the symmetric products 252 and 264 (half the operations;
+// 0.82); 1000 x 4000 B X 37 us (0.65, of which 14 are the end), X X^T 18 and 7 for the join.
+template <int TY, int BM, int BN, int WR, int WC, int STAGES, int KIND, int SHARE>
 __global__ __launch_bounds__(64 * WR * WC) void product_kernel(const Args a) {
     constexpr int threads = 64 * WR * WC, waves = WR * WC;
     constexpr int rows = BM / WR / 16, TM = SHARE == JOIN ? 1 : rows, TN = BN / WC / 16;  // a join: one row of result tiles a wave
@@ -231,11 +225,11 @@ __global__ __launch_bounds__(64 * WR * WC) void product_kernel(const Args a) {
         constexpr int stages = STAGES;
         __shared__ __attribute__((aligned(128))) char lds[stages][(BM + BN) * 128];
         const int ld = KIND == GRAM ? a.np : a.mp;  // of the contraction
-        const _Float16* left = (KIND == GRAM ? a.x + k * a.mp * a.np * P : KIND == POLY ? a.gram + k * a.mp * a.mp * P : a.poly + k * a.mp * a.mp * P);
-        const _Float16* right = KIND == NEXT || KIND == LAST ? a.xt + k * a.mp * a.np * P : left;
-        left += (int64_t)ti * BM * ld * P;
-        right += (int64_t)tj * BN * ld * P;
-        int b0 = 0, blocks = ld * P / 64;
+        const _Float16* left = (KIND == GRAM ? a.x + k * a.mp * a.np * kParts : KIND == POLY ? a.gram + k * a.mp * a.mp * kParts : a.poly + k * a.mp * a.mp * kParts);
+        const _Float16* right = KIND == NEXT || KIND == LAST ? a.xt + k * a.mp * a.np * kParts : left;
+        left += (int64_t)ti * BM * ld * kParts;
+        right += (int64_t)tj * BN * ld * kParts;
+        int b0 = 0, blocks = ld * kParts / 64;
         if constexpr (SHARE == SLICE) {
             const int all = blocks;
             b0 = (int)((int64_t)all * slice / a.slices);
@@ -248,7 +242,7 @@ __global__ __launch_bounds__(64 * WR * WC) void product_kernel(const Args a) {
 #pragma unroll
         for (int i = 0; i < loads; ++i) {
             const int row = 8 * (wave + i * waves) + (lane >> 3), piece = (lane & 7) ^ ((row >> 1) & 7);
-            from[i] = (uint32_t)(row < BM ? row : row - BM) * (uint32_t)(ld * P * 2) + 16 * piece;  // in bytes
+            from[i] = (uint32_t)(row < BM ? row : row - BM) * (uint32_t)(ld * kParts * 2) + 16 * piece;  // in bytes
         }
         auto fetch = [&](int block, int buf) {
 #pragma unroll
@@ -257,116 +251,73 @@ __global__ __launch_bounds__(64 * WR * WC) void product_kernel(const Args a) {
                                                  (__attribute__((address_space(3))) void*)(lds[buf] + 1024 * (wave + i * waves)), 16, 0, 0);
         };
         const int row_l = (wave / WC) * (BM / WR) + n, row_r = BM + (wave % WC) * (BN / WC) + n;
-        if constexpr (BM == 256) {
-            static_assert(P == 1, "two parts would not fit the registers");
-            // Operands of 32 of the contraction are read while those before them are multiplied.
-            h8 l0[TM], r0[TN], l1[TM], r1[TN];
-            auto read = [&](int b, int s, h8* l, h8* r) {
-                const char* at = lds[b & 1];
+        // A step is 32 of the contraction. Its operands are read while the step before is multiplied, and
+        // `stages` more steps are in LDS or on their way. Every step fetches, past the end the last one
+        // again, so that the number of loads under way is the same at every wait. The products are spread between the LDS reads, then between the loads (1000 x 4000
+        // 438 us with the reads of a step before its products, 361 so).
+        constexpr int products = 3 * TM * TN, reads = 2 * (TM + TN);
+        struct Operands {
+            h8 l[2][TM], r[2][TN];
+        } now, next;
+        auto read = [&](int buf, Operands& o) {
+            const char* at = lds[buf];
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+                const int c = 4 * p + g;
 #pragma unroll
                 for (int i = 0; i < TM; ++i) {
                     const int row = row_l + 16 * i;
-                    l[i] = *reinterpret_cast<const h8*>(at + row * 128 + (((4 * s + g) ^ ((row >> 1) & 7)) << 4));
+                    o.l[p][i] = *reinterpret_cast<const h8*>(at + row * 128 + ((c ^ ((row >> 1) & 7)) << 4));
                 }
 #pragma unroll
                 for (int j = 0; j < TN; ++j) {
                     const int row = row_r + 16 * j;
-                    r[j] = *reinterpret_cast<const h8*>(at + row * 128 + (((4 * s + g) ^ ((row >> 1) & 7)) << 4));
+                    o.r[p][j] = *reinterpret_cast<const h8*>(at + row * 128 + ((c ^ ((row >> 1) & 7)) << 4));
                 }
-            };
-            auto multiply = [&](const h8* l, const h8* r) {
+            }
+        };
+        int buf = 0;  // of this step
+        auto step = [&](int b, Operands& x, Operands& y) {
+            // The next step's operands are here, and this step's are read: all waves' after the barrier.
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((stages - 2) * loads) : "memory");
+            const int other = buf + 1 == stages ? 0 : buf + 1;
+            read(other, y);  // past the end: read and not used
+            fetch(min(b + stages, blocks - 1), buf);
+            buf = other;
+#pragma unroll
+            for (int p = 2; p >= 0; --p)  // second part by first, first by second, first by first
 #pragma unroll
                 for (int i = 0; i < TM; ++i)
 #pragma unroll
-                    for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(l[i], r[j], acc[i][j], 0, 0, 0);
+                    for (int j = 0; j < TN; ++j)
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x.l[p >> 1][i], x.r[p & 1][j], acc[i][j], 0, 0, 0);
 #pragma unroll
-                for (int i = 0; i < TM + TN; ++i) {
-                    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);                    // an LDS read,
-                    __builtin_amdgcn_sched_group_barrier(0x008, TM * TN / (TM + TN), 0);  // and some products
-                }
-            };
-            fetch(b0, b0 & 1);
-            __syncthreads();
-            if (b0 + 1 < blocks) fetch(b0 + 1, (b0 + 1) & 1);
-            read(b0, 0, l0, r0);
-            for (int b = b0; b < blocks; ++b) {
-                read(b, 1, l1, r1);
-                multiply(l0, r0);
-                __syncthreads();  // the next 64 have arrived, these are read
-                if (b + 2 < blocks) fetch(b + 2, b & 1);
-                read(b + 1, 0, l0, r0);  // past the end: read and not used
-                multiply(l1, r1);
+            for (int i = 0; i < reads; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // a product,
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // an LDS read
             }
-        } else {
-            // A step is 64 of the contraction of one part, or 32 of two. Its operands are read while the
-            // step before is multiplied, and `stages` more steps are in LDS or on their way. Every step
-            // fetches, past the end the last one again, so that the number of loads under way is the same at
-            // every wait. The products are spread between the LDS reads, then between the loads (1000 x 4000
-            // 438 us with the reads of a step before its products, 361 so).
-            constexpr int products = (P == 1 ? 2 : 3) * TM * TN, reads = 2 * (TM + TN);
-            struct Operands {
-                h8 l[2][TM], r[2][TN];
-            } now, next;
-            auto read = [&](int buf, Operands& o) {
-                const char* at = lds[buf];
 #pragma unroll
-                for (int p = 0; p < 2; ++p) {
-                    const int c = 4 * p + g;
-#pragma unroll
-                    for (int i = 0; i < TM; ++i) {
-                        const int row = row_l + 16 * i;
-                        o.l[p][i] = *reinterpret_cast<const h8*>(at + row * 128 + ((c ^ ((row >> 1) & 7)) << 4));
-                    }
-#pragma unroll
-                    for (int j = 0; j < TN; ++j) {
-                        const int row = row_r + 16 * j;
-                        o.r[p][j] = *reinterpret_cast<const h8*>(at + row * 128 + ((c ^ ((row >> 1) & 7)) << 4));
-                    }
-                }
-            };
-            int buf = 0;  // of this step
-            auto step = [&](int b, Operands& x, Operands& y) {
-                // The next step's operands are here, and this step's are read: all waves' after the barrier.
-                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((stages - 2) * loads) : "memory");
-                const int other = buf + 1 == stages ? 0 : buf + 1;
-                read(other, y);  // past the end: read and not used
-                fetch(min(b + stages, blocks - 1), buf);
-                buf = other;
-#pragma unroll
-                for (int p = P == 1 ? 1 : 2; p >= 0; --p)  // two parts: second by first, first by second, first by first
-#pragma unroll
-                    for (int i = 0; i < TM; ++i)
-#pragma unroll
-                        for (int j = 0; j < TN; ++j)
-                            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x.l[P == 1 ? p : p >> 1][i], x.r[P == 1 ? p : p & 1][j], acc[i][j], 0, 0, 0);
-#pragma unroll
-                for (int i = 0; i < reads; ++i) {
-                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // a product,
-                    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // an LDS read
-                }
-#pragma unroll
-                for (int i = 0; i < loads; ++i) {
-                    if constexpr (products - reads >= loads) __builtin_amdgcn_sched_group_barrier(0x008, (products - reads) / loads, 0);  // some products,
-                    __builtin_amdgcn_sched_group_barrier(0x010, 1, 0);                                                                   // a load
-                }
-                __builtin_amdgcn_sched_barrier(0);
-            };
-#pragma unroll
-            for (int i = 0; i < stages; ++i) fetch(min(b0 + i, blocks - 1), i);
-            asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((stages - 1) * loads) : "memory");
-            read(0, now);
-            int b = b0;
-            if ((blocks - b0) & 1) {
-                step(b++, now, next);
-                now = next;
+            for (int i = 0; i < loads; ++i) {
+                if constexpr (products - reads >= loads) __builtin_amdgcn_sched_group_barrier(0x008, (products - reads) / loads, 0);  // some products,
+                __builtin_amdgcn_sched_group_barrier(0x010, 1, 0);                                                                   // a load
             }
-            for (; b < blocks; b += 2) {
-                step(b, now, next);
-                step(b + 1, next, now);
-            }
-            // No load may still write the LDS when the workgroup's share of it is handed on.
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __builtin_amdgcn_sched_barrier(0);
+        };
+#pragma unroll
+        for (int i = 0; i < stages; ++i) fetch(min(b0 + i, blocks - 1), i);
+        asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((stages - 1) * loads) : "memory");
+        read(0, now);
+        int b = b0;
+        if ((blocks - b0) & 1) {
+            step(b++, now, next);
+            now = next;
         }
+        for (; b < blocks; b += 2) {
+            step(b, now, next);
+            step(b + 1, next, now);
+        }
+        // No load may still write the LDS when the workgroup's share of it is handed on.
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
 
     if constexpr (SHARE == SLICE) {
@@ -393,7 +344,7 @@ __global__ __launch_bounds__(64 * WR * WC) void product_kernel(const Args a) {
         for (int i = 0; i < batch; ++i)
 #pragma unroll
             for (int j = 0; j < TN; ++j) {
-                if constexpr (KIND == POLY) old[i][j] = get4<P>(a.gram + k * a.mp * a.mp * P + place<P>(col_of(j) + n, row_of(i), a.mp));
+                if constexpr (KIND == POLY) old[i][j] = get4(a.gram + k * a.mp * a.mp * kParts + place(col_of(j) + n, row_of(i), a.mp));
                 if constexpr (!half) old[i][j] = *master(i, j);
             }
 #pragma unroll
@@ -403,16 +354,16 @@ __global__ __launch_bounds__(64 * WR * WC) void product_kernel(const Args a) {
                 const int row0 = row_of(i), col0 = col_of(j);
                 f4 v = acc[i1 + i][j] * down;
                 if constexpr (half) {
-                    _Float16* to = (KIND == GRAM ? a.gram : a.poly) + k * a.mp * a.mp * P;
+                    _Float16* to = (KIND == GRAM ? a.gram : a.poly) + k * a.mp * a.mp * kParts;
                     if constexpr (KIND == POLY) v = a.in.b * old[i][j] + a.in.c * v;
-                    put4<P>(to + place<P>(col0 + n, row0, a.mp), v);  // the mirrored tile (of a diagonal tile, the same)
-                    if (ti != tj) put4<P>(to + place<P>(row0 + q, col0 + qc, a.mp), turn(v, lane));
+                    put4(to + place(col0 + n, row0, a.mp), v);  // the mirrored tile (of a diagonal tile, the same)
+                    if (ti != tj) put4(to + place(row0 + q, col0 + qc, a.mp), turn(v, lane));
                 } else {
                     v += a.in.a * old[i][j];
                     if constexpr (KIND == NEXT) {
                         *master(i, j) = v;
-                        put4<P>(a.xt2 + k * a.mp * a.np * P + place<P>(col0 + n, row0, a.mp), v);
-                        put4<P>(a.x + k * a.mp * a.np * P + place<P>(row0 + q, col0 + qc, a.np), turn(v, lane));
+                        put4(a.xt2 + k * a.mp * a.np * kParts + place(col0 + n, row0, a.mp), v);
+                        put4(a.x + k * a.mp * a.np * kParts + place(row0 + q, col0 + qc, a.np), turn(v, lane));
                     } else {
                         typedef typename Elem<TY>::type E;
                         // Four consecutive values along the dimension of out that is dense.
@@ -445,23 +396,19 @@ __global__ __launch_bounds__(64 * WR * WC) void product_kernel(const Args a) {
 }
 
 struct Plan {
-    int m, n, mp, np, parts;
+    int m, n, mp, np;
     int gram, slices;  // X X^T: tile, slices
     uint64_t norm, master, x, square, sums;  // bytes: partial norms, X in fp32, X as an operand, m x m as an operand, slices' sums
 };
 
-// Tiles of 64, 128 or (one part) 256 squared, the largest that makes enough blocks. 256: half the
-// CUs (4096 x 4096, whose symmetric products have 136 such tiles: 1657 us, 1932 with 128). 128 of one
-// part: two blocks a CU (1536 x 6144 588 us, 600 with 64; 2048 x 2048, one block a CU, 434 and 422).
-// 128 of two parts, which do three products for two: half the CUs (2048 x 2048 715 us, 773 with 64).
+// Tiles of 64 or 128 squared, 128 where they make a block for half the CUs (2048 x 2048 715 us, 773 with 64).
 int64_t tiles_of(const Plan& p, uint32_t count, bool half, int t) {
     const int64_t r = p.mp / t, c = p.np / t;
     return (half ? r * (r + 1) / 2 : r * c) * count;
 }
 int tile_of(const Plan& p, uint32_t count, bool half) {
     if (p.mp % 128 || (!half && p.np % 128)) return 64;  // sizes are multiples of 64
-    if (p.parts == 1 && p.mp % 256 == 0 && p.np % 256 == 0 && tiles_of(p, count, half, 256) >= 128) return 256;
-    return tiles_of(p, count, half, 128) >= (p.parts == 1 ? 512 : 128) ? 128 : 64;
+    return tiles_of(p, count, half, 128) >= 128 ? 128 : 64;
 }
 // Of X X^T, whose contraction is the longer dimension, also the slices. With tiles of 128 as many as
 // fill the CUs once, of at least 16 steps (1000 x 4000 361 us, 382 without; 640 x 4000, which would
@@ -469,9 +416,9 @@ int tile_of(const Plan& p, uint32_t count, bool half) {
 // block 24 steps, more than the join costs (512 x 2048 162 us, 193 without; four of 512 x 512, 8 of 16
 // steps spared, 170 and 153).
 void slice(Plan& p, uint32_t count) {
-    const int64_t steps = (int64_t)p.np * p.parts / 64;
+    const int64_t steps = (int64_t)p.np * kParts / 64;
     p.slices = 1;
-    if (p.parts == 2 && p.mp % 128 == 0) {
+    if (p.mp % 128 == 0) {
         const int64_t tiles = tiles_of(p, count, true, 128);
         p.gram = 128;
         p.slices = (int)std::max<int64_t>(1, std::min(256 / tiles, steps / 16));
@@ -480,7 +427,7 @@ void slice(Plan& p, uint32_t count) {
     p.gram = tile_of(p, count, true);
     const int64_t tiles = tiles_of(p, count, true, p.gram);
     p.slices = 1;
-    while (p.gram < 256 && p.slices < 16 && tiles * p.slices * 2 <= 256 && steps / (p.slices * 2) >= 8) p.slices *= 2;
+    while (p.slices < 16 && tiles * p.slices * 2 <= 256 && steps / (p.slices * 2) >= 8) p.slices *= 2;
     if (steps - steps / p.slices < 24) p.slices = 1;
 }
 
@@ -488,43 +435,39 @@ Plan plan_of(const ZenoAmdOrthogonalize& a) {
     Plan p;
     p.m = (int)(a.rows < a.cols ? a.rows : a.cols);
     p.n = (int)(a.rows < a.cols ? a.cols : a.rows);
-    p.parts = a.dtype == T_BF16 && p.m >= 256 ? 1 : 2;
     const int pad = p.m <= 512 ? 64 : 128;
     p.mp = (p.m + pad - 1) / pad * pad;
     p.np = (p.n + pad - 1) / pad * pad;
     p.norm = (uint64_t)a.count * kNormBlocks * sizeof(double);
     p.master = (uint64_t)a.count * p.mp * p.np * 4;
-    p.x = (uint64_t)a.count * p.mp * p.np * p.parts * 2;
-    p.square = (uint64_t)a.count * p.mp * p.mp * p.parts * 2;
+    p.x = (uint64_t)a.count * p.mp * p.np * kParts * 2;
+    p.square = (uint64_t)a.count * p.mp * p.mp * kParts * 2;
     slice(p, a.count);
     p.sums = p.slices > 1 ? (uint64_t)tiles_of(p, a.count, true, p.gram) * p.slices * p.gram * p.gram * 4 : 0;
     return p;
 }
 
-template <int TY, int P, int KIND, int SHARE> void product(const Args& a, int tile, hipStream_t stream) {
+template <int TY, int KIND, int SHARE> void product(const Args& a, int tile, hipStream_t stream) {
     const int rows = a.mp / tile, cols = a.np / tile, tiles = KIND == GRAM || KIND == POLY ? rows * (rows + 1) / 2 : rows * cols;
     const dim3 grid(SHARE == SLICE ? tiles * a.slices : tiles, a.in.count, SHARE == JOIN ? tile / 32 : 1);  // a join: a block for each row of result tiles of a wave
-    if (tile == 64) product_kernel<TY, P, 64, 64, 2, 2, 4, KIND, SHARE><<<grid, 256, 0, stream>>>(a);
-    if constexpr (P == 2 || SHARE == WHOLE)
-        if (tile == 128) product_kernel<TY, P, 128, 128, 2, 2, 3, KIND, SHARE><<<grid, 256, 0, stream>>>(a);
-    if constexpr (P == 1 && SHARE == WHOLE)
-        if (tile == 256) product_kernel<TY, P, 256, 256, 2, 4, 2, KIND, SHARE><<<grid, 512, 0, stream>>>(a);
+    if (tile == 64) product_kernel<TY, 64, 64, 2, 2, 4, KIND, SHARE><<<grid, 256, 0, stream>>>(a);
+    else product_kernel<TY, 128, 128, 2, 2, 3, KIND, SHARE><<<grid, 256, 0, stream>>>(a);
 }
 
-template <int TY, int P> hipError_t launch(Args a, const Plan& p, hipStream_t stream) {
+template <int TY> hipError_t launch(Args a, const Plan& p, hipStream_t stream) {
     const int square = tile_of(p, a.in.count, true), whole = tile_of(p, a.in.count, false);
     norm_kernel<TY><<<dim3(kNormBlocks, a.in.count), 256, 0, stream>>>(a);
-    load_kernel<TY, P><<<dim3(a.np / 64, a.mp / 64, a.in.count), 256, 0, stream>>>(a);
+    load_kernel<TY><<<dim3(a.np / 64, a.mp / 64, a.in.count), 256, 0, stream>>>(a);
     for (uint32_t s = 0; s < a.in.steps; ++s) {
         if (p.slices == 1) {
-            product<TY, P, GRAM, WHOLE>(a, p.gram, stream);
+            product<TY, GRAM, WHOLE>(a, p.gram, stream);
         } else {
-            product<TY, P, GRAM, SLICE>(a, p.gram, stream);
-            product<TY, P, GRAM, JOIN>(a, p.gram, stream);
+            product<TY, GRAM, SLICE>(a, p.gram, stream);
+            product<TY, GRAM, JOIN>(a, p.gram, stream);
         }
-        product<TY, P, POLY, WHOLE>(a, square, stream);
-        if (s + 1 < a.in.steps) product<TY, P, NEXT, WHOLE>(a, whole, stream);
-        else product<TY, P, LAST, WHOLE>(a, whole, stream);
+        product<TY, POLY, WHOLE>(a, square, stream);
+        if (s + 1 < a.in.steps) product<TY, NEXT, WHOLE>(a, whole, stream);
+        else product<TY, LAST, WHOLE>(a, whole, stream);
         std::swap(a.xt, a.xt2);
     }
     return hipGetLastError();
@@ -592,10 +535,9 @@ hipError_t run(const ZenoAmdOrthogonalize& in, void* workspace, hipStream_t stre
     const uint64_t eb = in.dtype == T_F32 ? 4 : 2;
     a.x_vec = xs[dense] == 1 && (uintptr_t)in.x % 16 == 0 && xs[3 - dense] * eb % 16 == 0 && (in.count == 1 || xs[0] * eb % 16 == 0);
     a.out_vec = s[3 - other] == 1 && (uintptr_t)in.out % four == 0 && s[other] % 4 == 0 && (in.count == 1 || s[0] % 4 == 0);
-    return in.dtype == T_F32   ? launch<T_F32, 2>(a, p, stream)
-           : in.dtype == T_F16 ? launch<T_F16, 2>(a, p, stream)
-           : p.parts == 2      ? launch<T_BF16, 2>(a, p, stream)
-                               : launch<T_BF16, 1>(a, p, stream);
+    return in.dtype == T_F32   ? launch<T_F32>(a, p, stream)
+           : in.dtype == T_F16 ? launch<T_F16>(a, p, stream)
+                               : launch<T_BF16>(a, p, stream);
 }
 
 }  // namespace orth

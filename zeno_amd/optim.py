@@ -28,8 +28,8 @@ def orthogonalize(update: torch.Tensor, steps: int = 5, coefficients: Tuple[floa
                   eps: float = 1e-7, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """`update` [..., rows, cols]: one matrix or several of one shape, float32, float16 or
     bfloat16, on the GPU, of any strides. Returns matrices of its shape and type (`out` if given;
-    out=update works in place). Results of float32 and float16 are as exact as fp32 products give
-    them, those of bfloat16 to its own rounding. Runs on torch's current stream."""
+    out=update works in place). Results of every type are as exact as fp32 products give them,
+    rounded once. Runs on torch's current stream."""
     if update.dtype not in _DTYPES:
         raise TypeError(f"update must be float32, float16 or bfloat16, not {update.dtype}")
     if update.dim() < 2 or update.numel() == 0:
