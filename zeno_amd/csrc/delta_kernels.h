@@ -604,33 +604,42 @@ __global__ __launch_bounds__(256) void delta_join_kernel(float* states, const fl
 //     dG_i = dO_i . O_i - dV_i . V_i,  dG_C += <dS', S'>,  dg_t = sum over i >= t of dG_i
 // (every other term cancels against its partner). The first line is column-local like the
 // forward pass (phase A); dQ and dK sum over the value columns, whose operands (U, dX, dO, dS'
-// transposed) go through LDS (phase B). Phase A feeds fp32 results and takes three parts; phase
-// B feeds results of the element type alone and takes `NO` parts: two for 16-bit types, 2^-17 of
-// each operand against the 2^-9 or 2^-12 of the results' own rounding.
+// transposed) go through LDS (phase B). What phase B multiplies lies in LDS in fp32 and is split
+// into its three parts as it is read: two thirds of the room of the parts, and no digit of fp32 is lost
+// before dQ and dK are rounded (behind the norms they may be a small rest of large terms).
 // What bounds it: two workgroups a CU, as LDS and registers allow, each going through some 30,000
 // cycles a chunk between barriers, half of them waiting on LDS and products (4096 sequences of 32,
 // four heads of 64 x 64, bfloat16: 840 us, about 1.3 TB/s; 2 of 4096, 8 heads of 128 x 128: 231).
 template <int TY, int DK, int NW, int TILES> struct BackwardLds {
     typedef Geo<TY, DK, NW, TILES> G;
-    static constexpr int NO = TY == T_F32 ? 3 : 2;
     static constexpr int slab = DK < 64 ? DK : 64;  // rows of dS' that are in LDS at once
-    static constexpr int SS = G::DV + 4, OS = DK + 4;
+    static constexpr int SS = G::DV + 4, OS = DK + 4, WS = G::C + 4;
     alignas(16) uint16_t K[G::NP * G::C * G::KS], Q[G::NP * G::C * G::KS], KT[G::NP * DK * G::TS], QT[G::NP * DK * G::TS];
     alignas(16) uint16_t DO[G::NP * G::C * G::VS];
     union {
         InnerBack<TILES> m;  // phase A
         struct {             // phase B
-            alignas(16) uint16_t W[NO * G::C * G::TS], WT[NO * G::C * G::TS], Y[NO * G::C * G::TS];
+            alignas(16) float W[G::C * WS], WT[G::C * WS], Y[G::C * WS];
             alignas(16) float dS[slab * SS];
         } b;
     };
     union {
-        struct { alignas(16) uint16_t U[NO * G::C * G::VS], X[NO * G::C * G::VS]; } c;
+        struct { alignas(16) float U[G::C * SS], X[G::C * SS]; } c;
         struct { alignas(16) float q[G::C * OS], k[G::C * OS]; } out;
     };
     Scalars<TILES> s;
     float decay[NW][G::C], beta[NW][G::C], edge[NW];  // sums over each wave's columns
 };
+
+// Operands from rows of fp32 in LDS: eight consecutive values along the head, or (Tok) a lane's
+// values along the tokens of a chunk.
+__device__ __forceinline__ Frag<3> frag_of(const float* at) { return split<3>(*reinterpret_cast<const f4*>(at), *reinterpret_cast<const f4*>(at + 4)); }
+template <int TILES> __device__ __forceinline__ auto tokens_of(const float* row, int g) {
+    f4 x[TILES];
+#pragma unroll
+    for (int i = 0; i < TILES; ++i) x[i] = *reinterpret_cast<const f4*>(row + 16 * i + 4 * g);
+    return Tok<TILES>::template make<3>(x);
+}
 
 // dR and dX = beta dR of dU + P^T dO, dU in du.
 template <int TY, int TILES, class M>
@@ -763,7 +772,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || sizeof(BackwardLds<TY, DK, NW, 
     typedef Geo<TY, DK, NW, TILES> G;
     typedef BackwardLds<TY, DK, NW, TILES> L;
     typedef typename Elem<TY>::type E;
-    constexpr int NP = G::NP, NO = L::NO, SO = NO - 1, C = G::C;
+    constexpr int NP = G::NP, C = G::C;
     __shared__ L lds;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
     // The arguments are read where they are used: as values held over the loop they would not fit
@@ -918,10 +927,10 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || sizeof(BackwardLds<TY, DK, NW, 
                 *reinterpret_cast<f4*>(lds.decay[wave] + 16 * i + 4 * g) = de;
                 *reinterpret_cast<f4*>(lds.beta[wave] + 16 * i + 4 * g) = be;
             }
-            const int at = (16 * i + row0) * G::VS + col;
+            const int at = (16 * i + row0) * L::SS + col;
             const f4 y = turn(dx[i], lane);
-            put4<NO>(lds.c.U + at, C * G::VS, turn(u[i], lane));
-            put4<NO>(lds.c.X + at, C * G::VS, y);
+            *reinterpret_cast<f4*>(lds.c.U + at) = turn(u[i], lane);
+            *reinterpret_cast<f4*>(lds.c.X + at) = y;
             if (16 * i + row0 < len) store4<TY, FULL>((E*)ap->dv + b * ap->dv_stride[0] + h * ap->dv_stride[2] + col + (t + 16 * i + row0) * ap->dv_stride[1], dv - col, ap->dv_vec, y);
         }
         __syncthreads();
@@ -985,14 +994,14 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || sizeof(BackwardLds<TY, DK, NW, 
             f4 acc = zero, mirror = zero;
 #pragma unroll
             for (int c = 0; c < G::DV / 32; ++c) {
-                const int ai = (16 * ti + n) * G::VS + 32 * c + 8 * g, aj = (16 * tj + n) * G::VS + 32 * c + 8 * g;
-                const Frag<NO> uf = frag_at<NO>(lds.c.U + aj, C * G::VS);
+                const int e = 32 * c + 8 * g;
+                const Frag<3> uf = frag_of(lds.c.U + (16 * tj + n) * L::SS + e);
                 if (job < pairs) {
-                    acc = mul<SO>(frag_at<NP>(lds.DO + ai, C * G::VS), uf, acc);
+                    acc = mul<2>(frag_at<NP>(lds.DO + (16 * ti + n) * G::VS + e, C * G::VS), uf, acc);
                 } else {
-                    const Frag<NO> xf = frag_at<NO>(lds.c.X + ai, C * G::VS);
-                    acc = mul<SO>(xf, uf, acc);
-                    if (ti == tj) mirror = mul<SO>(uf, xf, mirror);  // the tile's transpose
+                    const Frag<3> xf = frag_of(lds.c.X + (16 * ti + n) * L::SS + e);
+                    acc = mul<2>(xf, uf, acc);
+                    if (ti == tj) mirror = mul<2>(uf, xf, mirror);  // the tile's transpose
                 }
             }
             const float hj = lds.s.hi[j], lj = lds.s.lo[j], rj = lds.s.rk[j];
@@ -1009,13 +1018,15 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || sizeof(BackwardLds<TY, DK, NW, 
                 by_col[r] = y * rj;
                 by_row[r] = y * nr[r];
             }
-            put_rows<NO, TILES>(job < pairs ? lds.b.W : lds.b.Y, by_col, ti, tj, lane);
-            if (job < pairs) put_cols<NO, TILES>(lds.b.WT, by_row, ti, tj, lane);
+            // Rows of a matrix along tokens, and of its transpose.
+            auto rows_out = [&](float* m, f4 v, int ti, int tj) { *reinterpret_cast<f4*>(m + (16 * ti + row0) * L::WS + 16 * tj + (n & 12)) = turn(v, lane); };
+            auto cols_out = [&](float* m, f4 v, int ti, int tj) { *reinterpret_cast<f4*>(m + (16 * tj + n) * L::WS + 16 * ti + 4 * g) = v; };
+            rows_out(job < pairs ? lds.b.W : lds.b.Y, by_col, ti, tj);
+            if (job < pairs) cols_out(lds.b.WT, by_row, ti, tj);
             if (job < pairs && ti != tj) {  // above the diagonal
-                put_rows<NO, TILES>(lds.b.W, zero, tj, ti, lane);
-                put_rows<NO, TILES>(lds.b.WT, zero, ti, tj, lane);
-            }
-            else if (ti != tj) put_cols<NO, TILES>(lds.b.Y, by_row, ti, tj, lane);
+                rows_out(lds.b.W, zero, tj, ti);
+                rows_out(lds.b.WT, zero, ti, tj);
+            } else if (ti != tj) cols_out(lds.b.Y, by_row, ti, tj);
         }
         f4 dq[slabs * per], dkk[slabs * per];
 #pragma unroll
@@ -1035,15 +1046,13 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || sizeof(BackwardLds<TY, DK, NW, 
 #pragma unroll
             for (int c = 0; c < G::DV / 32; ++c) {
                 const int e = 32 * c + 8 * g;
-                const Frag<NO> sf = split<NO>(st[c][0], st[c][1]);
-                const float* ds = lds.b.dS + (16 * (blk % blocks) + n) * L::SS + e;
-                const Frag<NO> df = split<NO>(*reinterpret_cast<const f4*>(ds), *reinterpret_cast<const f4*>(ds + 4));
+                const Frag<3> sf = split<3>(st[c][0], st[c][1]), df = frag_of(lds.b.dS + (16 * (blk % blocks) + n) * L::SS + e);
 #pragma unroll
                 for (int i = 0; i < per; ++i) {
-                    const int at = (16 * (t1 + i) + n) * G::VS + e;
-                    aq[i] = mul<SO>(frag_at<NP>(lds.DO + at, C * G::VS), sf, aq[i]);
-                    ar[i] = mul<SO>(frag_at<NO>(lds.c.X + at, C * G::VS), sf, ar[i]);
-                    ac[i] = mul<SO>(frag_at<NO>(lds.c.U + at, C * G::VS), df, ac[i]);
+                    const int row = 16 * (t1 + i) + n;
+                    aq[i] = mul<2>(frag_at<NP>(lds.DO + row * G::VS + e, C * G::VS), sf, aq[i]);
+                    ar[i] = mul<2>(frag_of(lds.c.X + row * L::SS + e), sf, ar[i]);
+                    ac[i] = mul<2>(frag_of(lds.c.U + row * L::SS + e), df, ac[i]);
                 }
             }
             if (sl + 1 < slabs) fetch_rows(sl + 1);
@@ -1051,12 +1060,12 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || sizeof(BackwardLds<TY, DK, NW, 
             const auto qt = Tok<TILES>::template at<NP>(lds.QT + row * G::TS, g, DK * G::TS);
 #pragma unroll
             for (int i = 0; i < per; ++i) {
-                const int ti = t1 + i, at = (16 * ti + n) * G::TS;
+                const int ti = t1 + i, at = (16 * ti + n) * L::WS;
                 const f4 gam = row4(lds.s.gam, ti, g);
                 f4 yq = aq[i] * gam * ap->in.scale, yk = ac[i] * row4(lds.s.end, ti, g) - ar[i] * gam;
-                yk = mul<SO>(Tok<TILES>::template at<NO>(lds.b.Y + at, g, C * G::TS), kt, yk);
-                yq = mul<SO>(Tok<TILES>::template at<NO>(lds.b.W + at, g, C * G::TS), kt, yq);
-                yk = mul<SO>(Tok<TILES>::template at<NO>(lds.b.WT + at, g, C * G::TS), qt, yk);
+                yk = mul<2>(tokens_of<TILES>(lds.b.Y + at, g), kt, yk);
+                yq = mul<2>(tokens_of<TILES>(lds.b.W + at, g), kt, yq);
+                yk = mul<2>(tokens_of<TILES>(lds.b.WT + at, g), qt, yk);
                 dq[sl * per + i] = yq;
                 dkk[sl * per + i] = yk;
             }
