@@ -286,8 +286,9 @@ typedef struct {
 int zeno_amd_delta_forward(const ZenoAmdDeltaInputs* in, void* o, const int64_t* o_stride, float* last, void* saved, void* workspace,
                            void* stream);
 
-/* Gradients of a zeno_amd_delta_forward call with the same inputs, whose `last` and `saved`
- * it left. `workspace`: zeno_amd_delta_workspace_bytes(in) bytes (null where that is 0).
+/* Gradients of a zeno_amd_delta_forward call with the same inputs, which left `last` (not null,
+ * not read) and `saved`. The gradient of g keeps fp32's digits relative to its own size, exp(g),
+ * for heads that forget fast too. `workspace`: zeno_amd_delta_workspace_bytes(in) bytes (null where that is 0).
  * Gradients of key heads that several value heads share are summed in a fixed order: results
  * are bitwise reproducible. */
 int zeno_amd_delta_backward(const ZenoAmdDeltaInputs* in, const float* last, const void* saved, const ZenoAmdDeltaGradients* grad,

@@ -569,7 +569,7 @@ int zeno_amd_delta_backward(const ZenoAmdDeltaInputs* in, const float* last, con
     if (!last || (!saved && za::delta::saved_floats(*in))) return delta_refused("delta_backward", "null state of the forward call");
     if ((uintptr_t)saved % 16 || (uintptr_t)workspace % 16 || (!workspace && za::delta::workspace_floats(*in)))
         return delta_refused("delta_backward", "saved or workspace is not aligned to 16 bytes, or workspace is null");
-    return hip_status(za::delta::backward(*in, last, (const float*)saved, *grad, (float*)workspace, (hipStream_t)stream), "delta_backward");
+    return hip_status(za::delta::backward(*in, (const float*)saved, *grad, (float*)workspace, (hipStream_t)stream), "delta_backward");
 }
 
 uint64_t zeno_amd_delta_saved_bytes(const ZenoAmdDeltaInputs* in) {

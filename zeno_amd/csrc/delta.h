@@ -66,7 +66,7 @@ std::string check_sizes(const ZenoAmdDeltaInputs& in);
 std::string check(const ZenoAmdDeltaInputs* in, bool step);
 hipError_t forward(const ZenoAmdDeltaInputs& in, void* o, const int64_t* o_stride, float* last, float* saved, float* workspace,
                    hipStream_t stream);
-hipError_t backward(const ZenoAmdDeltaInputs& in, const float* last, const float* saved, const ZenoAmdDeltaGradients& grad, float* workspace,
+hipError_t backward(const ZenoAmdDeltaInputs& in, const float* saved, const ZenoAmdDeltaGradients& grad, float* workspace,
                     hipStream_t stream);
 hipError_t step(const ZenoAmdDeltaInputs& in, void* o, const int64_t* o_stride, float* state, hipStream_t stream);
 

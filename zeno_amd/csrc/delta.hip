@@ -136,13 +136,11 @@ hipError_t forward(const ZenoAmdDeltaInputs& in, void* o, const int64_t* o_strid
     return by_type(in.dtype, launch_forward<T_F32>, launch_forward<T_F16>, launch_forward<T_BF16>, a, s, stream);
 }
 
-hipError_t backward(const ZenoAmdDeltaInputs& in, const float* last, const float* saved, const ZenoAmdDeltaGradients& grad, float* workspace,
+hipError_t backward(const ZenoAmdDeltaInputs& in, const float* saved, const ZenoAmdDeltaGradients& grad, float* workspace,
                     hipStream_t stream) {
     const Shape s = shape_of(in, true);
     Args a = common(in, s);
     const uint32_t eb = element_bytes(in.dtype);
-    a.last = const_cast<float*>(last);
-    a.last_vec = state_vectors(last, in);
     a.saved = const_cast<float*>(saved);
     a.jumps = a.saved + inner_floats(in, s);
     a.d_starts = workspace + share_floats(in);
@@ -166,7 +164,7 @@ hipError_t backward(const ZenoAmdDeltaInputs& in, const float* last, const float
     set_strides(a.dbeta_stride, grad.d_beta_stride);
     a.d_state = grad.d_state;
     a.d_state_vec = state_vectors(grad.d_state, in);
-    a.full = in.key_dim == (uint32_t)s.dk && in.value_dim == 16u * s.waves && a.q_vec && a.k_vec && a.v_vec && a.s_vec && a.last_vec && a.d_o_vec &&
+    a.full = in.key_dim == (uint32_t)s.dk && in.value_dim == 16u * s.waves && a.q_vec && a.k_vec && a.v_vec && a.s_vec && a.d_o_vec &&
              a.dq_vec && a.dk_vec && a.dv_vec && a.d_last_vec && a.d_state_vec;
     if (a.share > 1) {
         a.part_q = workspace;

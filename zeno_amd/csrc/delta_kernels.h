@@ -225,7 +225,7 @@ template <int TILES> struct Inner {
 template <int TILES> struct InnerBack {
     static constexpr int C = 16 * TILES, TS = Tok<TILES>::stride, sides = 2;
     static constexpr int tile = 16 * kInvStride;
-    alignas(16) uint16_t P[3 * C * TS], PT[3 * C * TS];         // and transposed
+    alignas(16) uint16_t PT[3 * C * TS];                        // transposed
     alignas(16) uint16_t off[3 * tile], offT[3 * tile];
     alignas(16) uint16_t inv[2 * TILES * 3 * tile];
 };
@@ -599,17 +599,21 @@ __global__ __launch_bounds__(256) void delta_join_kernel(float* states, const fl
 //     dS = gam_C dS' + scale (gam Q)^T dO - K^T (gam dX)
 //     W = lower(D * dO U^T) scale;  Y = -strict_lower(D * dX U^T)
 //     dQ = scale gam dO S^T + W K;  dK = D_C U dS'^T - gam dX S^T + W^T Q + (Y + Y^T) K
-// O and V enter the chunk's result only through products with decays, so each decay's gradient
-// follows from the others: with dG_i the gradient of G_i,
-//     dG_i = dO_i . O_i - dV_i . V_i,  dG_C += <dS', S'>,  dg_t = sum over i >= t of dG_i
-// (every other term cancels against its partner). The first line is column-local like the
-// forward pass (phase A); dQ and dK sum over the value columns, whose operands (U, dX, dO, dS'
-// transposed) go through LDS (phase B). What phase B multiplies lies in LDS in fp32 and is split
-// into its three parts as it is read: two thirds of the room of the parts, and no digit of fp32 is lost
-// before dQ and dK are rounded (behind the norms they may be a small rest of large terms).
+// The decay of token t is in every term that passes it, from a token before t (or the state) to t or
+// a later token (or the end): with w_ij = W_ij (q_i . k_j) + Y_ij (k_i . k_j) between two tokens,
+// f_i = scale gam_i q_i S . dO_i - gam_i k_i S . dX_i, e_j = D_Cj k_j dS' . U_j,
+//     dg_t = sum over j < t <= i of w_ij + sum over i >= t of f_i + sum over j < t of e_j + gam_C <dS', S>
+// Nothing in it cancels but what the signs make cancel: each term carries the decay itself, so the
+// gradients of heads that forget fast, which are as small as exp(g), keep their digits. (dO_i . O_i - dV_i .
+// V_i summed over i >= t, the same in exact numbers, left 1e-2 of them at g = -8 and nothing at -16.)
+// f, e, dU and dX are column-local like the forward pass (phase A); w, dQ and dK sum over the value
+// columns, whose operands (U, dX, dO, dS' transposed) go through LDS (phase B). What phase B multiplies
+// lies in LDS in fp32 and is split into its three parts as it is read: two thirds of the room of the
+// parts, and no digit of fp32 is lost before dQ and dK are rounded (behind the norms they may be a small
+// rest of large terms).
 // What bounds it: two workgroups a CU, as LDS and registers allow, each going through some 30,000
 // cycles a chunk between barriers, half of them waiting on LDS and products (4096 sequences of 32,
-// four heads of 64 x 64, bfloat16: 840 us, about 1.3 TB/s; 2 of 4096, 8 heads of 128 x 128: 231).
+// four heads of 64 x 64, bfloat16: 960 us, about 1.1 TB/s; 2 of 4096, 8 heads of 128 x 128: 262).
 template <int TY, int DK, int NW, int TILES> struct BackwardLds {
     typedef Geo<TY, DK, NW, TILES> G;
     static constexpr int slab = DK < 64 ? DK : 64;  // rows of dS' that are in LDS at once
@@ -628,7 +632,8 @@ template <int TY, int DK, int NW, int TILES> struct BackwardLds {
         struct { alignas(16) float q[G::C * OS], k[G::C * OS]; } out;
     };
     Scalars<TILES> s;
-    float decay[NW][G::C], beta[NW][G::C], edge[NW];  // sums over each wave's columns
+    float from[NW][G::C], end[NW][G::C], beta[NW][G::C], past[NW];  // sums over each wave's columns: f, e, of beta, <dS', S>
+    alignas(16) float cross[2][TILES][G::C];  // sums of w over j < t <= i: W's and Y's, inside the 16 tokens of t and between the two 16
 };
 
 // Operands from rows of fp32 in LDS: eight consecutive values along the head, or (Tok) a lane's
@@ -639,6 +644,47 @@ template <int TILES> __device__ __forceinline__ auto tokens_of(const float* row,
 #pragma unroll
     for (int i = 0; i < TILES; ++i) x[i] = *reinterpret_cast<const f4*>(row + 16 * i + 4 * g);
     return Tok<TILES>::template make<3>(x);
+}
+
+// Of a 16x16 result tile of terms between tokens (row i, column j): the sum over all columns before
+// token t of the rows from t on (ALL: of all rows), for t = n + 1 in lane n; 0 in lane 15, where t is the next tile's.
+template <bool ALL> __device__ __forceinline__ float sum_over(f4 w, int n, int g) {
+    float y = 0.0f;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        float x = w[r];
+        if constexpr (!ALL) {
+            x += dpp<0x111>(x);  // from 1, 2, 4 and 8 lanes before, within 16
+            x += dpp<0x112>(x);
+            x += dpp<0x114>(x);
+            x += dpp<0x118>(x);
+        }
+        y += ALL || 4 * g + r > n ? x : 0.0f;
+    }
+    uint32_t b = __float_as_uint(y);
+    auto rows = __builtin_amdgcn_permlane16_swap(b, b, false, false);
+    y = __uint_as_float(rows[0]) + __uint_as_float(rows[1]);
+    b = __float_as_uint(y);
+    rows = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+    y = __uint_as_float(rows[0]) + __uint_as_float(rows[1]);
+    if constexpr (ALL) {
+        y += dpp<0x111>(y);
+        y += dpp<0x112>(y);
+        y += dpp<0x114>(y);
+        y += dpp<0x118>(y);
+    }
+    return n == 15 ? 0.0f : y;
+}
+// The sum of all columns over each of this lane's rows and those below it.
+__device__ __forceinline__ f4 sum_below(f4 w, int g) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) w[r] = sum16(w[r]);
+    w[2] += w[3];
+    w[1] += w[2];
+    w[0] += w[1];
+    const float y1 = from_group<1>(w[0]), y2 = from_group<2>(w[0]), y3 = from_group<3>(w[0]);
+    const float y = g == 0 ? (y3 + y2) + y1 : g == 1 ? y3 + y2 : g == 2 ? y3 : 0.0f;
+    return w + y;
 }
 
 // dR and dX = beta dR of dU + P^T dO, dU in du.
@@ -683,7 +729,7 @@ __device__ __forceinline__ void pull_state(const uint16_t* KT, const uint16_t* Q
 
 // The gradient of the state alone, for the segments: of every segment but the first, what its
 // outputs (and, of the last, d_last) add to the gradient of the state before it. It needs neither
-// states nor values: 71 us where the gradients' own pass takes 231 (2 sequences of 4096, 8 heads of
+// states nor values: 72 us where the gradients' own pass takes 262 (2 sequences of 4096, 8 heads of
 // 128 x 128, bfloat16).
 template <int TY, int DK, int NW, int TILES> struct PullLds {
     typedef Geo<TY, DK, NW, TILES> G;
@@ -785,24 +831,12 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || sizeof(BackwardLds<TY, DK, NW, 
     const int col0 = wave * 16, row0 = 4 * g + (n & 3), col = col0 + (n & 12);  // memory: four columns of a row
     const int64_t bh = b * ap->in.value_heads + h;
 
-    f4 dS[DK / 16];     // the gradient of the state after the chunk
-    float edge = 0.0f;  // this lane's share of <dS', S'>, the decay's gradient from all that passes the chunk's end
-    auto meet = [&](const f4* S) {
-        f4 y = {0, 0, 0, 0};
-#pragma unroll
-        for (int i = 0; i < DK / 16; ++i) y += dS[i] * S[i];
-        edge = (y[0] + y[1]) + (y[2] + y[3]);
-    };
-    f4 Sn[DK / 16];
+    f4 dS[DK / 16];  // the gradient of the state after the chunk
     if (segment == (int)ap->segments - 1) {
         load_state<DK, G::DV, FULL>(ap->d_last ? ap->d_last + bh * dk * dv : nullptr, dk, dv, dv, col0, lane, dS);
-        load_state<DK, G::DV, FULL>(ap->last + bh * dk * dv, dk, dv, dv, col0, lane, Sn);
     } else {
         load_state<DK, G::DV, true>(ap->d_starts + (bh * (ap->segments - 1) + segment) * (DK * G::DV), DK, G::DV, G::DV, col0, lane, dS);
-        load_state<DK, G::DV, true>(ap->saved + (bh * (ap->chunks - 1) + T / C - 1) * (DK * G::DV), DK, G::DV, G::DV, col0, lane, Sn);
     }
-
-    meet(Sn);
 
     // What a chunk reads from memory.
     Rows<TY, DK, NW, TILES> kr, qr;
@@ -876,7 +910,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || sizeof(BackwardLds<TY, DK, NW, 
 #pragma unroll
         for (int i = 0; i < TILES; ++i) vv[i] = turn(16 * i + row0 < len ? vr[i] : f4{0, 0, 0, 0}, lane);
         __syncthreads();
-        fill_inner<TY, DK, NW, TILES, TILES, W_P | W_PT | W_INV | W_INVT>(lds.K, lds.Q, lds.s, ap->in.scale, lds.m);
+        fill_inner<TY, DK, NW, TILES, TILES, W_PT | W_INV | W_INVT>(lds.K, lds.Q, lds.s, ap->in.scale, lds.m);
 
         // ---- phase A: this wave's columns
         asm volatile("" : "+s"(ap));
@@ -901,30 +935,35 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || sizeof(BackwardLds<TY, DK, NW, 
                 o4[i] = mul<2>(frag_at<NP>(lds.Q + at, C * G::KS), sb, o4[i]);
             }
         }
-        f4 x[TILES], u[TILES];
+        f4 x[TILES], u[TILES], meet = {0, 0, 0, 0};
 #pragma unroll
         for (int i = 0; i < TILES; ++i) {
             const f4 gam = row4(lds.s.gam, i, g), rk = row4(lds.s.rk, i, g);
-            x[i] = vv[i] - gam * rk * ks[i];
+            ks[i] *= gam * rk;
+            x[i] = vv[i] - ks[i];
             o4[i] *= gam * row4(lds.s.rq, i, g) * ap->in.scale;
             du[i] *= row4(lds.s.end, i, g) * rk;
         }
-        edge = sum64(edge);
-        if (lane == 0) lds.edge[wave] = edge;
+#pragma unroll
+        for (int i = 0; i < DK / 16; ++i) meet += dS[i] * S[i];
+        const float met = sum64((meet[0] + meet[1]) + (meet[2] + meet[3]));
+        if (lane == 0) lds.past[wave] = met;
         __syncthreads();
         Half<3> up[TILES];
         solve<TILES, TILES>(lds.m, lds.s, n, g, x, u, up);
-        add_PU<TILES, TILES>(lds.m, n, g, up, o4);
         const f4 zero = {0, 0, 0, 0};
-        f4 dr[TILES], dx[TILES];
+        f4 dr[TILES], dx[TILES], en[TILES];
+#pragma unroll
+        for (int i = 0; i < TILES; ++i) en[i] = du[i] * u[i];
         solve_back<TY, TILES>(lds.m, lds.s, n, g, d4, du, dr, dx);
 #pragma unroll
         for (int i = 0; i < TILES; ++i) {
-            f4 de = d4[i] * o4[i] - dx[i] * vv[i], be = dr[i] * x[i];
+            f4 fr = d4[i] * o4[i] - dx[i] * ks[i], be = dr[i] * x[i];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) de[r] = sum16(de[r]), be[r] = sum16(be[r]);
+            for (int r = 0; r < 4; ++r) fr[r] = sum16(fr[r]), en[i][r] = sum16(en[i][r]), be[r] = sum16(be[r]);
             if (n == 0) {
-                *reinterpret_cast<f4*>(lds.decay[wave] + 16 * i + 4 * g) = de;
+                *reinterpret_cast<f4*>(lds.from[wave] + 16 * i + 4 * g) = fr;
+                *reinterpret_cast<f4*>(lds.end[wave] + 16 * i + 4 * g) = en[i];
                 *reinterpret_cast<f4*>(lds.beta[wave] + 16 * i + 4 * g) = be;
             }
             const int at = (16 * i + row0) * L::SS + col;
@@ -960,38 +999,17 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || sizeof(BackwardLds<TY, DK, NW, 
             }
         };
         fetch_rows(0);
-        if (wave == NW - 1) {
-            double sum = 0.0;
-            float bsum = 0.0f;
-            if (lane < C)
-#pragma unroll
-                for (int w = 0; w < NW; ++w) {
-                    sum += (double)lds.decay[w][lane];
-                    bsum += lds.beta[w][lane];
-                }
-            if (lane == C - 1)
-#pragma unroll
-                for (int w = 0; w < NW; ++w) sum += (double)lds.edge[w];
-            sum += dpp64<0x101>(sum);
-            sum += dpp64<0x102>(sum);
-            sum += dpp64<0x104>(sum);
-            sum += dpp64<0x108>(sum);
-            if constexpr (TILES == 2) {
-                const double behind = from_lane(sum, 16);
-                if (lane < 16) sum += behind;
-            }
-            if (lane < len) {
-                ap->dg[b * ap->dg_stride[0] + (t + lane) * ap->dg_stride[1] + h * ap->dg_stride[2]] = first && lane == 0 ? 0.0f : (float)sum;
-                ap->dbeta[b * ap->dbeta_stride[0] + (t + lane) * ap->dbeta_stride[1] + h * ap->dbeta_stride[2]] = bsum;
-            }
-        }
-        // W and Y + Y^T (times the norms of the rows that they multiply), a tile a wave.
+        // W and Y + Y^T (times the norms of the rows that they multiply), a tile a wave; and w's sums.
         constexpr int pairs = TILES * (TILES + 1) / 2;
 #pragma unroll
         for (int job = 0; job < 2 * pairs; ++job) {
             const int pair = job % pairs, ti = pair > 0 ? 1 : 0, tj = pair > 1 ? 1 : 0, j = 16 * tj + n;
             if (wave != (NW >= 2 * pairs ? job : pair)) continue;
-            f4 acc = zero, mirror = zero;
+            f4 acc = zero, mirror = zero, dot = zero;
+#pragma unroll
+            for (int c = 0; c < DK / 32; ++c)
+                dot = mul<2>(frag_at<NP>((job < pairs ? lds.Q : lds.K) + (16 * ti + n) * G::KS + 32 * c + 8 * g, C * G::KS),
+                             frag_at<NP>(lds.K + j * G::KS + 32 * c + 8 * g, C * G::KS), dot);
 #pragma unroll
             for (int c = 0; c < G::DV / 32; ++c) {
                 const int e = 32 * c + 8 * g;
@@ -1006,7 +1024,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || sizeof(BackwardLds<TY, DK, NW, 
             }
             const float hj = lds.s.hi[j], lj = lds.s.lo[j], rj = lds.s.rk[j];
             const f4 hi = row4(lds.s.hi, ti, g), lo = row4(lds.s.lo, ti, g), nr = row4(job < pairs ? lds.s.rq : lds.s.rk, ti, g);
-            f4 by_col, by_row;  // times the norm of the column's token, and of the row's
+            f4 by_col, by_row, w;  // times the norm of the column's token, of the row's, and times the product
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int i = 16 * ti + 4 * g + r;
@@ -1017,6 +1035,16 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || sizeof(BackwardLds<TY, DK, NW, 
                 else y = j == i ? 0.0f : -(j < i ? acc[r] : mirror[r]) * __expf(j < i ? d : -d);
                 by_col[r] = y * rj;
                 by_row[r] = y * nr[r];
+                w[r] = j < i ? by_col[r] * nr[r] * dot[r] : 0.0f;
+            }
+            if (ti == tj) {
+                const float y = sum_over<false>(w, n, g);
+                if (g == 0) lds.cross[job >= pairs][0][16 * ti + ((n + 1) & 15)] = y;
+            } else {
+                const float y = sum_over<true>(w, n, g);
+                if (g == 0) lds.cross[job >= pairs][TILES - 1][(n + 1) & 15] = y;
+                const f4 z = sum_below(w, g);
+                if (n == 0) *reinterpret_cast<f4*>(lds.cross[job >= pairs][TILES - 1] + 16 + 4 * g) = z;
             }
             // Rows of a matrix along tokens, and of its transpose.
             auto rows_out = [&](float* m, f4 v, int ti, int tj) { *reinterpret_cast<f4*>(m + (16 * ti + row0) * L::WS + 16 * tj + (n & 12)) = turn(v, lane); };
@@ -1074,8 +1102,41 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || sizeof(BackwardLds<TY, DK, NW, 
         pull_state<TY, DK, TILES>(lds.KT, lds.QT, lds.s, ap->in.scale, n, g, d4, dx, dS);
 #pragma unroll
         for (int i = 0; i < DK / 16; ++i) dS[i] = first ? zero : dS[i];
-        meet(S);
         __syncthreads();  // U and dX are read
+        if (wave == NW - 1) {
+            // f of this token and the later ones, e of those before it, in 64 bits
+            double later = 0.0, before = 0.0, past = 0.0;
+            float bsum = 0.0f, w = 0.0f;
+            if (lane < C) {
+#pragma unroll
+                for (int v = 0; v < NW; ++v) {
+                    later += (double)lds.from[v][lane];
+                    if (lane) before += (double)lds.end[v][lane - 1];
+                    past += (double)lds.past[v];
+                    bsum += lds.beta[v][lane];
+                }
+#pragma unroll
+                for (int i = 0; i < TILES; ++i) w += lds.cross[0][i][lane] + lds.cross[1][i][lane];
+            }
+            later += dpp64<0x101>(later);
+            later += dpp64<0x102>(later);
+            later += dpp64<0x104>(later);
+            later += dpp64<0x108>(later);
+            before += dpp64<0x111>(before);
+            before += dpp64<0x112>(before);
+            before += dpp64<0x114>(before);
+            before += dpp64<0x118>(before);
+            if constexpr (TILES == 2) {
+                const double behind = from_lane(later, 16);
+                if (lane < 16) later += behind;
+                before += dpp64<0x142>(before);
+            }
+            if (lane < len) {
+                const float sum = (float)(later + before + (double)lds.s.gam[C - 1] * past + (double)w);
+                ap->dg[b * ap->dg_stride[0] + (t + lane) * ap->dg_stride[1] + h * ap->dg_stride[2]] = first && lane == 0 ? 0.0f : sum;
+                ap->dbeta[b * ap->dbeta_stride[0] + (t + lane) * ap->dbeta_stride[1] + h * ap->dbeta_stride[2]] = bsum;
+            }
+        }
         if (busy)
 #pragma unroll
             for (int sl = 0; sl < slabs; ++sl)
