@@ -14,8 +14,9 @@
 // environment that stands still.
 //
 // A chunk ends at a token of the grid of C and before every reset, so nothing is masked inside
-// it and no value from before a reset is ever multiplied by a zero. Partial chunks are filled
-// with zero keys, zero beta and zero g, which change nothing.
+// it and no value from before a reset is ever multiplied by a zero. Nor may an output meet a NaN or an
+// infinity of a later token by way of the zeros above a diagonal: a chunk that holds one goes token by
+// token. Partial chunks are filled with zero keys, zero beta and zero g, which change nothing.
 #pragma once
 #include <type_traits>
 
@@ -371,12 +372,13 @@ template <int TY, int DK, int NW, int TILES> struct ForwardLds {
     alignas(16) uint16_t K[G::NP * G::C * G::KS], Q[G::NP * G::C * G::KS], KT[G::NP * DK * G::TS];
     Inner<TILES> m;
     Scalars<TILES> s;
+    alignas(16) uint32_t odd[NW];  // whether a wave has fetched a value that is not finite
 };
 
 // What bounds it: of many short sequences memory (16384 of 16 tokens, two heads of 64 x 64, bfloat16:
-// 320 us, 4.1 TB/s of inputs, outputs and states; a large copy reaches 5.1), else a chunk's chain of
+// 335 us, 3.9 TB/s of inputs, outputs and states; a large copy reaches 5.1), else a chunk's chain of
 // dependent products and exchanges, of which the workgroups of a CU (four of four waves) take turns (4096
-// of 32 tokens, four heads, with the states for the gradients: 248 us).
+// of 32 tokens, four heads, with the states for the gradients: 253 us). The look for values that are not finite takes 4%.
 // FULL: heads of exactly DK and 16 NW dimensions, aligned, need no masks: a quarter of the
 // instructions less (3345 and 4595 of 64 x 64, bfloat16).
 // Waves a SIMD that the registers are cut down to: as many workgroups as fit the LDS, but not more
@@ -498,10 +500,7 @@ __global__ __launch_bounds__(64 * NW, forward_waves(NW, STATES, sizeof(ForwardLd
         const uint64_t cuts = __ballot(cut);
         const bool first = cuts & 1;
         const uint64_t later = cuts & ~1ull;
-        const int len = later ? __ffsll((unsigned long long)later) - 1 : lim - t;
-        f4 x[TILES];
-#pragma unroll
-        for (int i = 0; i < TILES; ++i) x[i] = turn(16 * i + row0 < len ? vr[i] : f4{0, 0, 0, 0}, lane);
+        int len = later ? __ffsll((unsigned long long)later) - 1 : lim - t;
         if (!STATES && a.saved && t && t % G::C == 0)
             store_state<DK, G::DV, true>(a.saved + (bh * (a.chunks - 1) + t / G::C - 1) * (DK * G::DV), DK, G::DV, G::DV, col0, lane, S);
         if (first) {
@@ -510,7 +509,22 @@ __global__ __launch_bounds__(64 * NW, forward_waves(NW, STATES, sizeof(ForwardLd
             for (int i = 0; i < DK / 16; ++i) S[i] = f4{0, 0, 0, 0};
         }
 
+        if constexpr (!STATES) {
+            bool fine = (gv < __builtin_inff()) & finite(bv) & (!kr.mine() | (kr.raw.finite() & qr.raw.finite()));
+#pragma unroll
+            for (int i = 0; i < TILES; ++i) fine &= finite(vr[i]);
+            lds.odd[wave] = __ballot(!fine) != 0;
+        }
         __syncthreads();  // the last chunk's operands are read
+        if constexpr (!STATES) {
+            uint32_t odd = 0;
+#pragma unroll
+            for (int w = 0; w < NW; ++w) odd |= lds.odd[w];
+            len = __builtin_amdgcn_readfirstlane(odd) ? 1 : len;
+        }
+        f4 x[TILES];
+#pragma unroll
+        for (int i = 0; i < TILES; ++i) x[i] = turn(16 * i + row0 < len ? vr[i] : f4{0, 0, 0, 0}, lane);
         if (wave == NW - 1) load_scalars<TILES>(lane < len ? gv : 0.0f, lane < len ? bv : 0.0f, lane, first, lds.s);
         kr.store(len, in.normalize, lds.K, lds.KT, lds.s.rk);
         if (!STATES) qr.store(len, in.normalize, lds.Q, nullptr, lds.s.rq);

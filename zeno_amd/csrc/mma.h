@@ -159,6 +159,21 @@ template <int TY> struct Raw {
 #pragma unroll
         for (int i = 0; i < words; ++i) a[i / 4][i % 4] = yes ? a[i / 4][i % 4] : 0u;
     }
+    __device__ __forceinline__ bool finite() const {
+        if constexpr (TY == T_F32) {
+            uint32_t top = 0;
+#pragma unroll
+            for (int i = 0; i < words; ++i) top = max(top, a[i / 4][i % 4] & 0x7fffffffu);
+            return top < 0x7f800000u;
+        } else {
+            typedef uint16_t h2 __attribute__((ext_vector_type(2)));
+            constexpr uint32_t inf = TY == T_BF16 ? 0x7f80u : 0x7c00u;
+            h2 top = {0, 0};
+#pragma unroll
+            for (int i = 0; i < words; ++i) top = __builtin_elementwise_max(top, __builtin_bit_cast(h2, a[0][i] & 0x7fff7fffu));
+            return top[0] < inf && top[1] < inf;
+        }
+    }
     __device__ __forceinline__ void get(float* x) const {
         typedef typename Elem<TY>::type E;
         if constexpr (TY == T_F32) {
@@ -252,6 +267,9 @@ template <int TY, bool FULL = false> __device__ __forceinline__ void store4(type
             if (j < n) at[j] = Elem<TY>::put(x[j]);
     }
 }
+
+__device__ __forceinline__ bool finite(float x) { return (__float_as_uint(x) & 0x7fffffffu) < 0x7f800000u; }
+__device__ __forceinline__ bool finite(f4 x) { return finite(x[0]) & finite(x[1]) & finite(x[2]) & finite(x[3]); }
 
 // A value from another lane of the same 16 (or of the same four).
 template <int CTRL> __device__ __forceinline__ float dpp(float x) {
