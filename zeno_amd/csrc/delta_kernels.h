@@ -510,7 +510,11 @@ __global__ __launch_bounds__(64 * NW, forward_waves(NW, STATES, sizeof(ForwardLd
         }
 
         if constexpr (!STATES) {
-            bool fine = (gv < __builtin_inff()) & finite(bv) & (!kr.mine() | (kr.raw.finite() & qr.raw.finite()));
+            bool fine = kr.raw.finite();  // no branch here either
+            fine &= qr.raw.finite();
+            fine |= !kr.mine();
+            fine &= gv < __builtin_inff();
+            fine &= finite(bv);
 #pragma unroll
             for (int i = 0; i < TILES; ++i) fine &= finite(vr[i]);
             lds.odd[wave] = __ballot(!fine) != 0;

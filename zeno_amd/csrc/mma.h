@@ -268,8 +268,11 @@ template <int TY, bool FULL = false> __device__ __forceinline__ void store4(type
     }
 }
 
-__device__ __forceinline__ bool finite(float x) { return (__float_as_uint(x) & 0x7fffffffu) < 0x7f800000u; }
-__device__ __forceinline__ bool finite(f4 x) { return finite(x[0]) & finite(x[1]) & finite(x[2]) & finite(x[3]); }
+__device__ __forceinline__ uint32_t bits_of_size(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+__device__ __forceinline__ bool finite(float x) { return bits_of_size(x) < 0x7f800000u; }
+__device__ __forceinline__ bool finite(f4 x) {
+    return max(max(bits_of_size(x[0]), bits_of_size(x[1])), max(bits_of_size(x[2]), bits_of_size(x[3]))) < 0x7f800000u;
+}
 
 // A value from another lane of the same 16 (or of the same four).
 template <int CTRL> __device__ __forceinline__ float dpp(float x) {
