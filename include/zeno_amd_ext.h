@@ -82,7 +82,9 @@ int zeno_amd_world_get_prev_contact_counts(ZenoWorldHandle world, uint32_t* out 
 int zeno_amd_world_set_contact_counts(ZenoWorldHandle world, const uint32_t* counts /* [E] */);
 
 /* Step with actions already in device memory (d_actions: [E*A] floats on the world's
- * device). Same semantics as zeno_world_step. */
+ * device). Same semantics as zeno_world_step. A world runs on a stream of its own: what writes
+ * the actions on another stream has to have ended before the call, and nothing may change them
+ * until the step has (zeno_amd_world_synchronize). */
 int zeno_amd_world_step_device(ZenoWorldHandle world, const float* d_actions, uint32_t substeps);
 
 /* Waits for all work queued on the world's stream. */

@@ -374,7 +374,8 @@ class ZenoWorld:
 
     def step_device(self, d_actions: int, substeps: int = 0) -> None:
         """One step with actions already in device memory (address d_actions, E x action_dim
-        f32); returns after enqueueing."""
+        f32); returns after enqueueing on the world's own stream: what writes the actions on another
+        stream has to have ended (torch.cuda.current_stream().synchronize())."""
         rc = self._lib.zeno_amd_world_step_device(self._handle, C.c_void_p(d_actions or None), substeps)
         if rc != 0:
             raise RuntimeError(f"step_device failed: {rc}: {L.last_error()}")
