@@ -244,7 +244,8 @@ int zeno_amd_selfcheck_reciprocal_error(double* max_err);
  *
  * All pointers are device pointers of the current device. Strides are in elements (sequence,
  * token, head); the last dimension of q, k, v and o is contiguous; strides may be anything
- * else, 0 included for inputs, and outputs must not overlap. Calls return after enqueueing on
+ * else, 0 included for inputs. Outputs may not overlap themselves, one another or an input (o may
+ * be v itself, with the same strides); a step and a forward call refuse what does. Calls return after enqueueing on
  * `stream` (a hipStream_t; null = the default stream). */
 #define ZENO_AMD_FLOAT32 0u
 #define ZENO_AMD_FLOAT16 1u
@@ -310,8 +311,8 @@ int zeno_amd_delta_step(const ZenoAmdDeltaInputs* in, void* o, const int64_t* o_
  * fp64) and their operands carry 22 bits. Coefficients that let a singular value of X, or an
  * entry of the products, exceed 32 are refused: the operands are pairs of 16-bit numbers at a
  * fixed scale. Strides are in elements (matrix, row, column)
- * and may be anything; out must not overlap x unless it is the same memory with the same
- * strides. */
+ * and may be anything, but for an out that overlaps itself, which is refused. out may overlap
+ * x: all of x is read before any of out is written. */
 typedef struct {
     uint32_t dtype;               /* of x and out, as above */
     uint32_t count, rows, cols;   /* at most 65535 matrices of 65536 x 65536 */

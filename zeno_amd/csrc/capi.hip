@@ -557,6 +557,8 @@ int zeno_amd_delta_forward(const ZenoAmdDeltaInputs* in, void* o, const int64_t*
     if (last == in->state) return delta_refused("delta_forward", "the last state would overwrite the first");
     if ((uintptr_t)saved % 16 || (uintptr_t)workspace % 16 || (!workspace && za::delta::workspace_floats(*in)))
         return delta_refused("delta_forward", "saved or workspace is not aligned to 16 bytes, or workspace is null");
+    const std::string shared = za::delta::check_overlap(*in, o, o_stride, last, false);
+    if (!shared.empty()) return delta_refused("delta_forward", shared);
     return hip_status(za::delta::forward(*in, o, o_stride, last, (float*)saved, (float*)workspace, (hipStream_t)stream), "delta_forward");
 }
 
@@ -584,6 +586,8 @@ int zeno_amd_delta_step(const ZenoAmdDeltaInputs* in, void* o, const int64_t* o_
     const std::string why = za::delta::check(in, true);
     if (!why.empty()) return delta_refused("delta_step", why);
     if (!o || !o_stride || !state) return delta_refused("delta_step", "null output or state");
+    const std::string shared = za::delta::check_overlap(*in, o, o_stride, state, true);
+    if (!shared.empty()) return delta_refused("delta_step", shared);
     return hip_status(za::delta::step(*in, o, o_stride, state, (hipStream_t)stream), "delta_step");
 }
 
@@ -594,6 +598,7 @@ uint64_t zeno_amd_orthogonalize_workspace_bytes(const ZenoAmdOrthogonalize* args
 int zeno_amd_orthogonalize(const ZenoAmdOrthogonalize* args, void* workspace, void* stream) {
     std::string why = za::orth::check(args);
     if (why.empty() && (!workspace || (uintptr_t)workspace % 256)) why = "workspace is null or not aligned to 256 bytes";
+    if (why.empty() && za::orth::out_overlaps(*args)) why = "out overlaps itself";
     if (!why.empty()) {
         set_error("orthogonalize: " + why);
         return ZENO_INVALID_ARGUMENT;

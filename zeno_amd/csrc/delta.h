@@ -64,6 +64,9 @@ template <int TY> hipError_t launch_step(const Args& a, float* state, hipStream_
 // Entry points behind the C ABI. A non-empty message means that nothing was launched.
 std::string check_sizes(const ZenoAmdDeltaInputs& in);
 std::string check(const ZenoAmdDeltaInputs* in, bool step);
+// Outputs of a step or a forward call (`state`: of either) that overlap themselves, each other or an
+// input. o may be v itself, value by value: the wave that writes a value has read it.
+std::string check_overlap(const ZenoAmdDeltaInputs& in, const void* o, const int64_t* o_stride, const float* state, bool step);
 hipError_t forward(const ZenoAmdDeltaInputs& in, void* o, const int64_t* o_stride, float* last, float* saved, float* workspace,
                    hipStream_t stream);
 hipError_t backward(const ZenoAmdDeltaInputs& in, const float* saved, const ZenoAmdDeltaGradients& grad, float* workspace,

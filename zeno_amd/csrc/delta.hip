@@ -5,6 +5,7 @@
 #include <cmath>
 
 #include "mma.h"
+#include "overlap.h"
 
 namespace za {
 namespace delta {
@@ -118,6 +119,35 @@ std::string check(const ZenoAmdDeltaInputs* p, bool step) {
     if (!in.q || !in.k || !in.v || !in.g || !in.beta) return "null input";
     if (!std::isfinite(in.scale)) return "scale is not finite";
     return "";
+}
+
+std::string check_overlap(const ZenoAmdDeltaInputs& in, const void* o, const int64_t* o_stride, const float* state, bool step) {
+    const int64_t eb = element_bytes(in.dtype), keys[3] = {in.batch, in.length, in.key_heads}, values[3] = {in.batch, in.length, in.value_heads};
+    const int64_t none[1] = {0}, one[1] = {1}, states = (int64_t)in.batch * in.value_heads * in.key_dim * in.value_dim;
+    const Memory out(o, o_stride, values, 3, in.value_dim, eb), kept(state, none, one, 1, states, 4), v(in.v, in.v_stride, values, 3, in.value_dim, eb);
+    const Memory inputs[] = {Memory(in.q, in.q_stride, keys, 3, in.key_dim, eb), Memory(in.k, in.k_stride, keys, 3, in.key_dim, eb),
+                             Memory(in.g, in.g_stride, values, 3, 1, 4), Memory(in.beta, in.beta_stride, values, 3, 1, 4)};
+    if (!out.apart_from_itself()) return "o overlaps itself";
+    if (!apart(out, kept)) return "o overlaps the state";
+    bool same = o == in.v;
+    for (int i = 0; i < 3; ++i) same = same && (values[i] == 1 || o_stride[i] == in.v_stride[i]);
+    if (!same && !apart(out, v)) return "o overlaps v and is not v itself";
+    bool clear = apart(kept, v);
+    for (const Memory& x : inputs) {
+        if (!apart(out, x)) return "o overlaps an input";
+        clear = clear && apart(kept, x);
+    }
+    if (in.reset) {
+        const Memory reset(in.reset, in.reset_stride, values, 2, 1, 1);
+        if (!apart(out, reset)) return "o overlaps an input";
+        clear = clear && apart(kept, reset);
+    }
+    if (!step && in.state) {
+        const Memory before(in.state, none, one, 1, states, 4);
+        if (!apart(out, before)) return "o overlaps an input";
+        clear = clear && apart(kept, before);
+    }
+    return clear ? "" : "the state overlaps an input";
 }
 
 hipError_t forward(const ZenoAmdDeltaInputs& in, void* o, const int64_t* o_stride, float* last, float* saved, float* workspace,

@@ -22,6 +22,7 @@
 
 #include "mma.h"
 #include "orth.h"
+#include "overlap.h"
 
 namespace za {
 namespace orth {
@@ -499,6 +500,11 @@ std::string check(const ZenoAmdOrthogonalize* p) {
         top = next;
     }
     return "";
+}
+
+bool out_overlaps(const ZenoAmdOrthogonalize& a) {
+    const int64_t sizes[3] = {a.count, a.rows, a.cols};
+    return !Memory(a.out, a.out_stride, sizes, 3, 1, a.dtype == T_F32 ? 4 : 2).apart_from_itself();
 }
 
 uint64_t workspace_bytes(const ZenoAmdOrthogonalize& a) {

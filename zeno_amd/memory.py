@@ -196,7 +196,7 @@ def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
                      normalize: bool = False, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """One token for every sequence: q, k [B, Hk, key_dim], v [B, Hv, value_dim], g, beta
     [B, Hv], reset [B]. `state` (contiguous) is advanced in place; returns o [B, Hv, value_dim]
-    (`out` if given). Without gradients, even where an operand asks for them: training runs
+    (`out` if given; it may be v, but overlap nothing else that the step reads or writes). Without gradients, even where an operand asks for them: training runs
     gated_delta on the recorded rollout."""
     _check(q, k, v, g, beta, reset, state, 1)
     if not state.is_contiguous():
