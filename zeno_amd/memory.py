@@ -195,12 +195,14 @@ def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
                      state: torch.Tensor, reset: Optional[torch.Tensor] = None, *, scale: Optional[float] = None,
                      normalize: bool = False, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """One token for every sequence: q, k [B, Hk, key_dim], v [B, Hv, value_dim], g, beta
-    [B, Hv], reset [B]. `state` (contiguous) is advanced in place; returns o [B, Hv, value_dim]
+    [B, Hv], reset [B]. `state` (contiguous, refused if autograd follows it) is advanced in place; returns o [B, Hv, value_dim]
     (`out` if given; it may be v, but overlap nothing else that the step reads or writes). Without gradients, even where an operand asks for them: training runs
     gated_delta on the recorded rollout."""
     _check(q, k, v, g, beta, reset, state, 1)
     if not state.is_contiguous():
         raise ValueError("state must be contiguous: it is advanced in place")
+    if (state.requires_grad or (out is not None and out.requires_grad)) and torch.is_grad_enabled():
+        raise ValueError("state and out are written in place, which autograd does not see: give detached ones, or step under torch.no_grad()")
     q, k, v = _row(q), _row(k), _row(v)
     if out is None:
         out = torch.empty_like(v, memory_format=torch.contiguous_format)
