@@ -109,7 +109,7 @@ template <int TY> __global__ __launch_bounds__(256) void load_kernel(const Args 
     for (int i = 0; i < kNormBlocks; i += 64) s += a.partial[k * kNormBlocks + i + (threadIdx.x & 63)];
 #pragma unroll
     for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d);
-    const float f = (float)((double)kScale / (sqrt(s) + (double)a.in.eps));
+    const double f = (double)kScale / (sqrt(s) + (double)a.in.eps);  // beyond fp32's range where both are small
     const bool dense_cols = a.flip ? a.in.x_stride[1] <= a.in.x_stride[2] : a.in.x_stride[2] <= a.in.x_stride[1];
     const int w = threadIdx.x & 63, u = threadIdx.x >> 6;
 #pragma unroll
@@ -117,7 +117,7 @@ template <int TY> __global__ __launch_bounds__(256) void load_kernel(const Args 
         const int r = dense_cols ? i : w, c = dense_cols ? w : i;
         float v = 0.0f;
         if (r0 + r < a.m && c0 + c < a.n) v = a.flip ? input<TY>(a, k, c0 + c, r0 + r) : input<TY>(a, k, r0 + r, c0 + c);
-        tile[r][c] = v * f;
+        tile[r][c] = (float)((double)v * f);
     }
     __syncthreads();
     _Float16* x = a.x + k * a.mp * a.np * kParts;
