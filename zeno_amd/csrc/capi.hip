@@ -575,11 +575,11 @@ int zeno_amd_delta_backward(const ZenoAmdDeltaInputs* in, const float* last, con
 }
 
 uint64_t zeno_amd_delta_saved_bytes(const ZenoAmdDeltaInputs* in) {
-    return in && za::delta::check_sizes(*in).empty() ? 4 * za::delta::saved_floats(*in) : 0;
+    return in && za::delta::check_sizes(*in, false).empty() ? 4 * za::delta::saved_floats(*in) : 0;
 }
 
 uint64_t zeno_amd_delta_workspace_bytes(const ZenoAmdDeltaInputs* in) {
-    return in && za::delta::check_sizes(*in).empty() ? 4 * za::delta::workspace_floats(*in) : 0;
+    return in && za::delta::check_sizes(*in, false).empty() ? 4 * za::delta::workspace_floats(*in) : 0;
 }
 
 int zeno_amd_delta_step(const ZenoAmdDeltaInputs* in, void* o, const int64_t* o_stride, float* state, void* stream) {

@@ -61,8 +61,16 @@ template <int TY> hipError_t launch_forward(const Args& a, const Shape& s, hipSt
 template <int TY> hipError_t launch_backward(const Args& a, const Shape& s, hipStream_t stream);
 template <int TY> hipError_t launch_step(const Args& a, float* state, hipStream_t stream);
 
+// Of the single step: a wave holds all rows of 4 `lanes` columns of a head.
+inline int step_lanes(const ZenoAmdDeltaInputs& in) { return in.key_dim <= 32 || in.key_dim > 64 ? 8 : 16; }
+inline uint64_t step_waves(const ZenoAmdDeltaInputs& in) {
+    const uint32_t cols = 4 * step_lanes(in);
+    return (uint64_t)in.batch * in.value_heads * ((in.value_dim + cols - 1) / cols);
+}
+inline uint64_t step_threads(const ZenoAmdDeltaInputs& in) { return (step_waves(in) + 3) / 4 * 256; }
+
 // Entry points behind the C ABI. A non-empty message means that nothing was launched.
-std::string check_sizes(const ZenoAmdDeltaInputs& in);
+std::string check_sizes(const ZenoAmdDeltaInputs& in, bool step);
 std::string check(const ZenoAmdDeltaInputs* in, bool step);
 // Outputs of a step or a forward call (`state`: of either) that overlap themselves, each other or an
 // input. o may be v itself, value by value: the wave that writes a value has read it.

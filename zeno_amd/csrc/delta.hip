@@ -99,21 +99,24 @@ uint64_t workspace_floats(const ZenoAmdDeltaInputs& in) {
     return std::max(states_floats(in, run) + jumps_floats(in, run), share_floats(in) + states_floats(in, train));
 }
 
-std::string check_sizes(const ZenoAmdDeltaInputs& in) {
+std::string check_sizes(const ZenoAmdDeltaInputs& in, bool step) {
     if (in.dtype > T_BF16) return "dtype is none of float32, float16, bfloat16";
     if (!in.batch || !in.length || !in.key_heads || !in.value_heads) return "batch, length and head counts must be positive";
     if (in.value_heads % in.key_heads) return "value_heads is not a multiple of key_heads";
     if (!in.key_dim || in.key_dim > ZENO_AMD_DELTA_MAX_DIM || !in.value_dim || in.value_dim > ZENO_AMD_DELTA_MAX_DIM)
         return "key_dim and value_dim must be 1 to " + std::to_string(ZENO_AMD_DELTA_MAX_DIM);
-    if (in.length > 0x7fffff00u || (uint64_t)in.batch * in.value_heads > 0x7fffffffull / 64) return "too many sequences or tokens";
-    if ((uint64_t)in.batch * in.length * in.key_heads > 0x7fffffffull) return "too many tokens";  // blocks of the sum over shared heads
+    // A launch takes less than 2^32 threads: 64 to 512 for each sequence and head (step_threads: see there).
+    const uint64_t heads = (uint64_t)in.batch * in.value_heads;
+    if (in.length > 0x7fffff00u || heads > 0x7fffffffull / 64 || (step ? step_threads(in) : heads * 64 * shape_of(in, false).waves) > 0xffffffffull)
+        return "too many sequences or tokens";
+    if ((uint64_t)in.batch * in.length * in.key_heads > 0x7fffffffull) return "too many tokens";
     return "";
 }
 
 std::string check(const ZenoAmdDeltaInputs* p, bool step) {
     if (!p) return "null arguments";
     const ZenoAmdDeltaInputs& in = *p;
-    const std::string why = check_sizes(in);
+    const std::string why = check_sizes(in, step);
     if (!why.empty()) return why;
     if (step && in.length != 1) return "a step takes one token";
     if (!in.q || !in.k || !in.v || !in.g || !in.beta) return "null input";

@@ -1219,24 +1219,25 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || sizeof(BackwardLds<TY, DK, NW, 
     if (ap->d_state && segment == 0) store_state<DK, G::DV, FULL>(ap->d_state + bh * dk * dv, dk, dv, dv, col0, lane, dS);
 }
 
-// Sums the value heads of each key head, in their order; one thread a value. Memory-bound and small: 4 us
+// Sums the value heads of each key head, in their order; a thread a value, several where there are more
+// than 2^28 (a launch takes less than 2^32 threads). Memory-bound and small: 4 us
 // of 250 (19 sequences of 333 tokens, two value heads a key head, fp32).
 template <int TY> __global__ __launch_bounds__(256) void delta_share_kernel(const Args a) {
     typedef typename Elem<TY>::type E;
     const ZenoAmdDeltaInputs& in = a.in;
     const int64_t all = (int64_t)in.batch * in.length * in.key_heads * in.key_dim;
-    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (id >= all) return;
-    const int64_t x = id % in.key_dim, hk = id / in.key_dim % in.key_heads, bt = id / in.key_dim / in.key_heads;
-    const int64_t t = bt % in.length, b = bt / in.length;
-    const int64_t from = (bt * in.value_heads + hk * a.share) * in.key_dim + x;
-    float sq = 0.0f, sk = 0.0f;
-    for (uint32_t s = 0; s < a.share; ++s) {
-        sq += a.part_q[from + s * in.key_dim];
-        sk += a.part_k[from + s * in.key_dim];
+    for (int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x; id < all; id += (int64_t)gridDim.x * 256) {
+        const int64_t x = id % in.key_dim, hk = id / in.key_dim % in.key_heads, bt = id / in.key_dim / in.key_heads;
+        const int64_t t = bt % in.length, b = bt / in.length;
+        const int64_t from = (bt * in.value_heads + hk * a.share) * in.key_dim + x;
+        float sq = 0.0f, sk = 0.0f;
+        for (uint32_t s = 0; s < a.share; ++s) {
+            sq += a.part_q[from + s * in.key_dim];
+            sk += a.part_k[from + s * in.key_dim];
+        }
+        ((E*)a.dq)[b * a.dq_stride[0] + t * a.dq_stride[1] + hk * a.dq_stride[2] + x] = Elem<TY>::put(sq);
+        ((E*)a.dk)[b * a.dk_stride[0] + t * a.dk_stride[1] + hk * a.dk_stride[2] + x] = Elem<TY>::put(sk);
     }
-    ((E*)a.dq)[b * a.dq_stride[0] + t * a.dq_stride[1] + hk * a.dq_stride[2] + x] = Elem<TY>::put(sq);
-    ((E*)a.dk)[b * a.dk_stride[0] + t * a.dk_stride[1] + hk * a.dk_stride[2] + x] = Elem<TY>::put(sk);
 }
 
 // ---- one token -----------------------------------------------------------------------------
@@ -1382,18 +1383,16 @@ template <int TY> hipError_t launch_backward(const Args& a, const Shape& s, hipS
     else backward_shape<TY, 128, 8, TY == T_BF16 ? 2 : 1>(a, stream);
     if (a.part_q) {
         const int64_t all = (int64_t)a.in.batch * a.in.length * a.in.key_heads * a.in.key_dim;
-        delta_share_kernel<TY><<<dim3((uint32_t)((all + 255) / 256)), 256, 0, stream>>>(a);
+        const int64_t blocks = (all + 255) / 256, most = 1 << 20;
+        delta_share_kernel<TY><<<dim3((uint32_t)(blocks < most ? blocks : most)), 256, 0, stream>>>(a);
     }
     return hipGetLastError();
 }
 
 template <int TY> hipError_t launch_step(const Args& a, float* state, hipStream_t stream) {
     const ZenoAmdDeltaInputs& in = a.in;
-    const int64_t heads = (int64_t)in.batch * in.value_heads;
     const bool vec = in.value_dim % 4 == 0 && (uintptr_t)state % 16 == 0;
-    const int lanes = in.key_dim <= 32 || in.key_dim > 64 ? 8 : 16;
-    const int64_t waves = heads * ((in.value_dim + 4 * lanes - 1) / (4 * lanes));
-    const dim3 grid((uint32_t)((waves + 3) / 4));
+    const dim3 grid((uint32_t)((step_waves(in) + 3) / 4));
     if (in.key_dim <= 32) {
         if (vec) delta_step_kernel<TY, 8, 4, true><<<grid, 256, 0, stream>>>(a, state);
         else delta_step_kernel<TY, 8, 4, false><<<grid, 256, 0, stream>>>(a, state);
