@@ -36,6 +36,8 @@ def orthogonalize(update: torch.Tensor, steps: int = 5, coefficients: Tuple[floa
         raise ValueError(f"update must hold matrices, not {tuple(update.shape)}")
     if not update.is_cuda:
         raise ValueError("update must be on the GPU (there is no CPU fallback)")
+    if not 1 <= steps <= 100:  # before it is cut to 32 bits
+        raise ValueError(f"steps must be 1 to 100, not {steps}")
     if len(coefficients) != 3:
         raise ValueError("coefficients are three numbers")
     if out is None:
