@@ -45,8 +45,10 @@ POLICY_FLAGS = [
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
     "-Wall", "-Wno-unused-result",
 ]
-# The scheduler's exact register counts spare the gradients' kernels spills (heads of 128x128: 254 us
-# without, 231 with); orth.hip's kernels, which spill nothing, lose 3% by them.
+# The scheduler's exact register counts spare the delta kernels some of their spills (2 sequences of 4096
+# with gradients, 8 heads of 128x128: float32 835 us, 863 without; bfloat16 494 and 499; none remain in the
+# gradients' kernel of 64x64, up to 18 registers of 128x128 and 28 of the segments' pass of 128x128 in float16
+# do); orth.hip's kernels, which spill nothing, lose 3% by them.
 DELTA_FLAGS = ["-mllvm", "-amdgpu-use-amdgpu-trackers=1"]
 
 

@@ -55,10 +55,14 @@ void set_strides(int64_t* to, const int64_t* from) {
 }  // namespace
 
 // 16 tokens a chunk where 32 do not fit the 160 KB of a CU in the gradients' kernel. Segments:
-// with fewer heads than the GPU holds workgroups (one of eight waves a CU, two of four), as many as
-// fill it, of at least three chunks (4 heads of 1000 tokens forward: 40 us with three, 64 with eight, 125
-// in one segment; 76 heads of 333 with gradients 251 and 352). The additional pass over the tokens costs as
-// much as it saves where fewer than three segments come of it (111 heads of 211: 48 us in one, 53 in two).
+// with fewer heads than 256 workgroups of eight waves or 512 of four, as many as make up those, of at least
+// three chunks (4 heads of 1000 tokens forward: 40 us with three, 64 with eight, 125 in one segment; 76 heads
+// of 333 with gradients 251 and 352). The gradients' kernel of four waves fits a CU twice in bfloat16 (76 KB)
+// and once in float16 (119) and float32 (143), where the other kernels' gain still pays for segments that
+// take turns (128 heads of 1024 x 64 x 64 with gradients: bfloat16 278 us, 560 with room for 256; float16 410
+// and 635; float32 475 and 670). The additional pass over the tokens costs more than it saves where fewer than
+// three segments come of it (111 heads of 211 tokens of 40 x 72, float32, inputs in cache: 48 us in one, 53 in
+// two; of 64 x 64, bfloat16, 34 and 43).
 Shape shape_of(const ZenoAmdDeltaInputs& in, bool train) {
     Shape s;
     s.dk = in.key_dim <= 64 ? 64 : 128;

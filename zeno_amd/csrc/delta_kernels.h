@@ -382,7 +382,9 @@ template <int TY, int DK, int NW, int TILES> struct ForwardLds {
 // FULL: heads of exactly DK and 16 NW dimensions, aligned, need no masks: a quarter of the
 // instructions less (3345 and 4595 of 64 x 64, bfloat16).
 // Waves a SIMD that the registers are cut down to: as many workgroups as fit the LDS, but not more
-// than the registers bear (128 of four waves spill in the wide kernel with outputs).
+// than the registers bear (128 of four waves spill in the wide kernel with outputs: 107 us, 130 so). The
+// segments' pass of 128x128 spills a few too and is faster all the same (one sequence of 16384, 8 heads: bfloat16
+// 4 registers, 277 us a pass, 309 without; float16 28, 362 and 392).
 constexpr int forward_waves(int waves, bool states, size_t lds) {
     const int groups = (int)(160 * 1024 / lds), fit = groups * waves / 4;
     return waves == 8 && !states ? 2 : fit >= 4 ? 4 : fit == 3 ? 3 : 2;
@@ -555,9 +557,11 @@ __global__ __launch_bounds__(64 * NW, forward_waves(NW, STATES, sizeof(ForwardLd
 // BACK: the same for the state's gradient from the last segment to the first, with M transposed.
 // A workgroup joins 16 value columns of a head. Its four waves share the rows of the result; each
 // step's state reaches them as a right operand through LDS, the matrices come from memory a step
-// ahead. One step is DK / 64 x DK / 32 x 6 dependent-free matrix instructions a wave. Bound by how fast
-// one CU draws the matrices in: 106 KB in 1.9 us of 128 x 128, the same with loads two steps ahead (8
-// heads, 32 segments: 56 us). More workgroups would each read all of a head's matrices again.
+// ahead. A wave has DK / 64 chains of DK / 32 x 6 matrix instructions a step, each behind the one before.
+// Bound by the steps in a row: of 128 x 128 one takes 1.9 us (8 heads, 32 segments: 57 us), in which a CU
+// draws 106 KB in; by the counters a wave waits for memory and LDS a quarter of that, its products take a
+// sixth and the rest goes to their order. Loads two steps ahead gained 3%. More workgroups would each read all
+// of a head's matrices again.
 template <int DK, int DV, bool BACK>
 __global__ __launch_bounds__(256) void delta_join_kernel(float* states, const float* jumps, int segments) {
     typedef Jump<DK> J;
@@ -625,44 +629,71 @@ __global__ __launch_bounds__(256) void delta_join_kernel(float* states, const fl
 // gradients of heads that forget fast, which are as small as exp(g), keep their digits. (dO_i . O_i - dV_i .
 // V_i summed over i >= t, the same in exact numbers, left 1e-2 of them at g = -8 and nothing at -16.)
 // f, e, dU and dX are column-local like the forward pass (phase A); w, dQ and dK sum over the value
-// columns, whose operands (U, dX, dO, dS' transposed) go through LDS (phase B). What phase B multiplies
-// lies in LDS in fp32 and is split into its three parts as it is read: two thirds of the room of the
-// parts, and no digit of fp32 is lost before dQ and dK are rounded (behind the norms they may be a small
-// rest of large terms).
-// What bounds it: two workgroups a CU, as LDS and registers allow, each going through some 30,000
-// cycles a chunk between barriers, half of them waiting on LDS and products (4096 sequences of 32,
-// four heads of 64 x 64, bfloat16: 960 us, about 1.1 TB/s; 2 of 4096, 8 heads of 128 x 128: 262).
+// columns, whose operands (U, dX, dO, dS' transposed) go through LDS (phase B). No digit of fp32 is lost
+// before dQ and dK are rounded: behind the norms they may be a small rest of large terms.
+// What bounds it: instructions, and two workgroups a CU, as LDS and registers allow (in float16 and
+// float32 one). Of a wave's 54,000 cycles a chunk 35% issue its 4,700 vector instructions and 37% wait for
+// LDS, barriers and memory; the matrix units are busy 18% of two such waves' time (4096 sequences of 32,
+// four heads of 64 x 64, bfloat16: 950 us, about 1.1 TB/s; 2 of 4096, 8 heads of 128 x 128: 260).
+
+// What phase B multiplies, in LDS: as three parts, or in fp32 and split as it is read, which takes two thirds
+// of the room and some time more (4096 sequences of 32 with gradients, four heads of 64 x 64: float32 1210 and
+// 1272 us, float16 1086 and 1156). bfloat16 has it in fp32, with which two workgroups of four waves fit a
+// CU, and float16 where 32 tokens of 128 columns would not fit at all as parts; the other kernels fit a CU
+// once either way.
+template <int TY, int C, int DV, int TILES> struct Held {
+    static constexpr bool parts = TY == T_F32 || (TY == T_F16 && C * DV <= 2048);
+    typedef std::conditional_t<parts, uint16_t, float> T;
+    static constexpr int RS = parts ? DV + 8 : DV + 4, rows = (parts ? 3 : 1) * C * RS;               // along the head
+    static constexpr int TS = parts ? Tok<TILES>::stride : C + 4, tokens = (parts ? 3 : 1) * C * TS;  // along the tokens
+    // Four consecutive values of a row, from a multiple of four on.
+    static __device__ __forceinline__ void put_row(T* m, int row, int col, f4 v) {
+        if constexpr (parts) put4<3>(m + row * RS + col, C * RS, v);
+        else *reinterpret_cast<f4*>(m + row * RS + col) = v;
+    }
+    static __device__ __forceinline__ void put_tokens(T* m, int row, int col, f4 v) {
+        if constexpr (parts) put4<3>(m + row * TS + Tok<TILES>::slot_of(col), C * TS, v);
+        else *reinterpret_cast<f4*>(m + row * TS + col) = v;
+    }
+    // Operands: eight consecutive values of a row, or a lane's values along the tokens.
+    static __device__ __forceinline__ Frag<3> along_row(const T* m, int row, int col) {
+        if constexpr (parts) return frag_at<3>(m + row * RS + col, C * RS);
+        else return frag_of(m + row * RS + col);
+    }
+    static __device__ __forceinline__ auto along_tokens(const T* m, int row, int g) {
+        if constexpr (parts) {
+            return Tok<TILES>::template at<3>(m + row * TS, g, C * TS);
+        } else {
+            f4 x[TILES];
+#pragma unroll
+            for (int i = 0; i < TILES; ++i) x[i] = *reinterpret_cast<const f4*>(m + row * TS + 16 * i + 4 * g);
+            return Tok<TILES>::template make<3>(x);
+        }
+    }
+};
+
 template <int TY, int DK, int NW, int TILES> struct BackwardLds {
     typedef Geo<TY, DK, NW, TILES> G;
     static constexpr int slab = DK < 64 ? DK : 64;  // rows of dS' that are in LDS at once
-    static constexpr int SS = G::DV + 4, OS = DK + 4, WS = G::C + 4;
+    static constexpr int SS = G::DV + 4, OS = DK + 4;
+    typedef Held<TY, G::C, G::DV, TILES> H;
     alignas(16) uint16_t K[G::NP * G::C * G::KS], Q[G::NP * G::C * G::KS], KT[G::NP * DK * G::TS], QT[G::NP * DK * G::TS];
     alignas(16) uint16_t DO[G::NP * G::C * G::VS];
     union {
         InnerBack<TILES> m;  // phase A
         struct {             // phase B
-            alignas(16) float W[G::C * WS], WT[G::C * WS], Y[G::C * WS];
+            alignas(16) typename H::T W[H::tokens], WT[H::tokens], Y[H::tokens];
             alignas(16) float dS[slab * SS];
         } b;
     };
     union {
-        struct { alignas(16) float U[G::C * SS], X[G::C * SS]; } c;
+        struct { alignas(16) typename H::T U[H::rows], X[H::rows]; } c;
         struct { alignas(16) float q[G::C * OS], k[G::C * OS]; } out;
     };
     Scalars<TILES> s;
     float from[NW][G::C], end[NW][G::C], beta[NW][G::C], past[NW];  // sums over each wave's columns: f, e, of beta, <dS', S>
     alignas(16) float cross[2][TILES][G::C];  // sums of w over j < t <= i: W's and Y's, inside the 16 tokens of t and between the two 16
 };
-
-// Operands from rows of fp32 in LDS: eight consecutive values along the head, or (Tok) a lane's
-// values along the tokens of a chunk.
-__device__ __forceinline__ Frag<3> frag_of(const float* at) { return split<3>(*reinterpret_cast<const f4*>(at), *reinterpret_cast<const f4*>(at + 4)); }
-template <int TILES> __device__ __forceinline__ auto tokens_of(const float* row, int g) {
-    f4 x[TILES];
-#pragma unroll
-    for (int i = 0; i < TILES; ++i) x[i] = *reinterpret_cast<const f4*>(row + 16 * i + 4 * g);
-    return Tok<TILES>::template make<3>(x);
-}
 
 // Of a 16x16 result tile of terms between tokens (row i, column j): the sum over all columns before
 // token t of the rows from t on (ALL: of all rows), for t = n + 1 in lane n; 0 in lane 15, where t is the next tile's.
@@ -835,6 +866,7 @@ template <int TY, int DK, int NW, int TILES, bool FULL>
 __global__ __launch_bounds__(64 * NW, NW == 8 || sizeof(BackwardLds<TY, DK, NW, TILES>) <= 80 * 1024 ? 2 : 1) void delta_backward_kernel(const Args) {
     typedef Geo<TY, DK, NW, TILES> G;
     typedef BackwardLds<TY, DK, NW, TILES> L;
+    typedef typename L::H H;
     typedef typename Elem<TY>::type E;
     constexpr int NP = G::NP, C = G::C;
     __shared__ L lds;
@@ -984,10 +1016,9 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || sizeof(BackwardLds<TY, DK, NW, 
                 *reinterpret_cast<f4*>(lds.end[wave] + 16 * i + 4 * g) = en[i];
                 *reinterpret_cast<f4*>(lds.beta[wave] + 16 * i + 4 * g) = be;
             }
-            const int at = (16 * i + row0) * L::SS + col;
             const f4 y = turn(dx[i], lane);
-            *reinterpret_cast<f4*>(lds.c.U + at) = turn(u[i], lane);
-            *reinterpret_cast<f4*>(lds.c.X + at) = y;
+            H::put_row(lds.c.U, 16 * i + row0, col, turn(u[i], lane));
+            H::put_row(lds.c.X, 16 * i + row0, col, y);
             if (16 * i + row0 < len) store4<TY, FULL>((E*)ap->dv + b * ap->dv_stride[0] + h * ap->dv_stride[2] + col + (t + 16 * i + row0) * ap->dv_stride[1], dv - col, ap->dv_vec, y);
         }
         __syncthreads();
@@ -1031,11 +1062,11 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || sizeof(BackwardLds<TY, DK, NW, 
 #pragma unroll
             for (int c = 0; c < G::DV / 32; ++c) {
                 const int e = 32 * c + 8 * g;
-                const Frag<3> uf = frag_of(lds.c.U + (16 * tj + n) * L::SS + e);
+                const Frag<3> uf = H::along_row(lds.c.U, 16 * tj + n, e);
                 if (job < pairs) {
                     acc = mul<2>(frag_at<NP>(lds.DO + (16 * ti + n) * G::VS + e, C * G::VS), uf, acc);
                 } else {
-                    const Frag<3> xf = frag_of(lds.c.X + (16 * ti + n) * L::SS + e);
+                    const Frag<3> xf = H::along_row(lds.c.X, 16 * ti + n, e);
                     acc = mul<2>(xf, uf, acc);
                     if (ti == tj) mirror = mul<2>(uf, xf, mirror);  // the tile's transpose
                 }
@@ -1065,8 +1096,8 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || sizeof(BackwardLds<TY, DK, NW, 
                 if (n == 0) *reinterpret_cast<f4*>(lds.cross[job >= pairs][TILES - 1] + 16 + 4 * g) = z;
             }
             // Rows of a matrix along tokens, and of its transpose.
-            auto rows_out = [&](float* m, f4 v, int ti, int tj) { *reinterpret_cast<f4*>(m + (16 * ti + row0) * L::WS + 16 * tj + (n & 12)) = turn(v, lane); };
-            auto cols_out = [&](float* m, f4 v, int ti, int tj) { *reinterpret_cast<f4*>(m + (16 * tj + n) * L::WS + 16 * ti + 4 * g) = v; };
+            auto rows_out = [&](typename H::T* m, f4 v, int ti, int tj) { H::put_tokens(m, 16 * ti + row0, 16 * tj + (n & 12), turn(v, lane)); };
+            auto cols_out = [&](typename H::T* m, f4 v, int ti, int tj) { H::put_tokens(m, 16 * tj + n, 16 * ti + 4 * g, v); };
             rows_out(job < pairs ? lds.b.W : lds.b.Y, by_col, ti, tj);
             if (job < pairs) cols_out(lds.b.WT, by_row, ti, tj);
             if (job < pairs && ti != tj) {  // above the diagonal
@@ -1097,8 +1128,8 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || sizeof(BackwardLds<TY, DK, NW, 
                 for (int i = 0; i < per; ++i) {
                     const int row = 16 * (t1 + i) + n;
                     aq[i] = mul<2>(frag_at<NP>(lds.DO + row * G::VS + e, C * G::VS), sf, aq[i]);
-                    ar[i] = mul<2>(frag_of(lds.c.X + row * L::SS + e), sf, ar[i]);
-                    ac[i] = mul<2>(frag_of(lds.c.U + row * L::SS + e), df, ac[i]);
+                    ar[i] = mul<2>(H::along_row(lds.c.X, row, e), sf, ar[i]);
+                    ac[i] = mul<2>(H::along_row(lds.c.U, row, e), df, ac[i]);
                 }
             }
             if (sl + 1 < slabs) fetch_rows(sl + 1);
@@ -1106,12 +1137,12 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || sizeof(BackwardLds<TY, DK, NW, 
             const auto qt = Tok<TILES>::template at<NP>(lds.QT + row * G::TS, g, DK * G::TS);
 #pragma unroll
             for (int i = 0; i < per; ++i) {
-                const int ti = t1 + i, at = (16 * ti + n) * L::WS;
+                const int ti = t1 + i, at = 16 * ti + n;
                 const f4 gam = row4(lds.s.gam, ti, g);
                 f4 yq = aq[i] * gam * ap->in.scale, yk = ac[i] * row4(lds.s.end, ti, g) - ar[i] * gam;
-                yk = mul<2>(tokens_of<TILES>(lds.b.Y + at, g), kt, yk);
-                yq = mul<2>(tokens_of<TILES>(lds.b.W + at, g), kt, yq);
-                yk = mul<2>(tokens_of<TILES>(lds.b.WT + at, g), qt, yk);
+                yk = mul<2>(H::along_tokens(lds.b.Y, at, g), kt, yk);
+                yq = mul<2>(H::along_tokens(lds.b.W, at, g), kt, yq);
+                yk = mul<2>(H::along_tokens(lds.b.WT, at, g), qt, yk);
                 dq[sl * per + i] = yq;
                 dkk[sl * per + i] = yk;
             }

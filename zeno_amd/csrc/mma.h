@@ -110,6 +110,8 @@ template <int P> __device__ __forceinline__ Half<P> half_at(const uint16_t* at, 
     return f;
 }
 
+__device__ __forceinline__ Frag<3> frag_of(const float* at) { return split<3>(*reinterpret_cast<const f4*>(at), *reinterpret_cast<const f4*>(at + 4)); }
+
 // ---- element types ------------------------------------------------------------------------
 enum Type : uint32_t { T_F32 = 0, T_F16 = 1, T_BF16 = 2 };
 template <int TY> struct Elem;
