@@ -8,8 +8,8 @@
 // scales far from either end of its range, in two parts that carry 22 bits: three of the four part
 // products give fp32's accuracy at a third of the units' rate, five times the fp32 units'. X itself
 // stays in fp32 and is what a X adds: a small singular value grows 3.4-fold a step by that term, and
-// with it every rounding of X that the term would carry (results 4.8e-3 off instead of 5e-4 with fp16
-// there). bfloat16 takes two parts as well: with one of 11 bits a result of 256 x 512 with 37 rows
+// with it every rounding of X that the term would carry (momenta with strong directions 4.3e-3 off with 11
+// bits there; emulated, the operand's 22 bits would do as well as 32). bfloat16 takes two parts as well: with one of 11 bits a result of 256 x 512 with 37 rows
 // that are not zero is off by 3.3e-3 of its norm and one of 1024 x 1024 Gaussian values by 1.3e-3,
 // where its own rounding is 1.7e-3; with two, 4e-6. Sums are fp32, the norm's fp64.
 //
@@ -189,9 +189,9 @@ enum Share { WHOLE, SLICE, JOIN };  // of the contraction: all of it; a slice, s
 // row number, which leaves the operand reads without bank conflicts. Few tiles with a long
 // contraction are cut into slices along it (SLICE), whose sums another launch adds in their order (JOIN).
 // Bound by the matrix units and the operands' way from L2 together, and at its end by memory: X, X^T and
-// the fp32 X are written at once by all blocks. Rates of part products: 4096 x 4096 B X 390 us (1.06
-// PFLOP/s; a large library product of fp16 1.18), the symmetric products 252 and 264 (half the operations;
-// 0.82); 1000 x 4000 B X 37 us (0.65, of which 14 are the end), X X^T 18 and 7 for the join.
+// the fp32 X are written at once by all blocks. Rates of part products: 4096 x 4096 B X 387 us (1.07
+// PFLOP/s; a large library product of fp16 1.18), the symmetric products 247 and 259 (half the operations;
+// 0.8); 1000 x 4000 B X 37 us (0.65, of which 14 are the end), X X^T 18 and 7 for the join.
 template <int TY, int BM, int BN, int WR, int WC, int STAGES, int KIND, int SHARE>
 __global__ __launch_bounds__(64 * WR * WC) void product_kernel(const Args a) {
     constexpr int threads = 64 * WR * WC, waves = WR * WC;
