@@ -25,9 +25,10 @@ q, k and v is contiguous, so views of one projection and time-major rollouts
 (``x.transpose(0, 1)``) need no copy. scale defaults to key_dim ** -0.5; with ``normalize``,
 queries and keys are divided by sqrt(sum of squares + 1e-6) first. All sums and states are 32-bit;
 a token with g < -104 (its decay is 0 in fp32) counts as a reset. What lies before a reset, NaN
-and infinity included, has no effect on what follows. A NaN or an infinity has none on outputs before
-its token either (an infinity makes NaN of what it meets, and results that pass the type's range on
-the way may do so from 32 tokens before); gradients of up to 32 tokens around it may all be NaN.
+and infinity included, has no effect on what follows. A NaN or an infinity in an operand has
+none on outputs before its token either; an infinity may make NaN of what it meets. Two limits:
+gradients of up to 31 tokens on either side of it may be NaN too, and so may up to 31 outputs before
+a token whose own sums overflow fp32.
 """
 from __future__ import annotations
 
