@@ -329,6 +329,42 @@ uint64_t zeno_amd_orthogonalize_workspace_bytes(const ZenoAmdOrthogonalize* args
 /* `workspace`: that many bytes, aligned to 256. Returns after enqueueing on `stream`. */
 int zeno_amd_orthogonalize(const ZenoAmdOrthogonalize* args, void* workspace, void* stream);
 
+/* Layer norm of rows of `dim` features: y = (s - mean) / sqrt(variance + eps) * weight + bias, with
+ * s = x, or x + residual rounded to its type, which goes to `sum`. Statistics and sums are fp32
+ * (the mean to its last digit, for rows far off zero too), y is rounded once. Rows lie along up to
+ * three dimensions of any stride (the first changes slowest; unused ones have size 1); the features
+ * of a row are contiguous, at any address of their type. Outputs may not overlap themselves, one
+ * another or an input, which is refused. Calls return after enqueueing on `stream`, allocate nothing
+ * and use device pointers of the current device. */
+#define ZENO_AMD_NORM_MAX_DIM 16384u
+
+typedef struct {
+    uint32_t dtype;              /* of x, residual, sum, y and their gradients */
+    uint32_t weight_dtype;       /* of weight, bias and their gradients: dtype or ZENO_AMD_FLOAT32 */
+    uint32_t rows[3];            /* at most 2^31 - 1 in all */
+    uint32_t dim;                /* 1 to ZENO_AMD_NORM_MAX_DIM */
+    float eps;
+    const void *x, *residual;    /* residual: null for none */
+    const void *weight, *bias;   /* [dim], contiguous; null: 1 and 0 */
+    int64_t x_stride[3], residual_stride[3];
+} ZenoAmdNormInputs;
+
+/* Gradients: of y, and of the sum (null: zeros), in; of x (and of the residual, which is the same),
+ * the weight and the bias out, each of which may be null. */
+typedef struct {
+    const void *d_y, *d_sum;
+    void *d_x, *d_weight, *d_bias;
+    int64_t d_y_stride[3], d_sum_stride[3], d_x_stride[3];
+} ZenoAmdNormGradients;
+
+/* `sum` (with `sum_stride`) where there is a residual, else null. */
+int zeno_amd_norm_forward(const ZenoAmdNormInputs* in, void* y, const int64_t* y_stride, void* sum, const int64_t* sum_stride, void* stream);
+/* `in` as in the forward call, but for x, which is what was normalised: the sum where there was a
+ * residual (residual and bias are not read). `workspace`: zeno_amd_norm_workspace_bytes(in) bytes,
+ * aligned to 16; null where neither d_weight nor d_bias is wanted. Bitwise reproducible. */
+int zeno_amd_norm_backward(const ZenoAmdNormInputs* in, const ZenoAmdNormGradients* grad, void* workspace, void* stream);
+uint64_t zeno_amd_norm_workspace_bytes(const ZenoAmdNormInputs* in); /* 0 for refused arguments */
+
 #ifdef __cplusplus
 }
 #endif

@@ -120,12 +120,32 @@ class ZenoAmdOrthogonalize(C.Structure):
     ]
 
 
+class ZenoAmdNormInputs(C.Structure):
+    """include/zeno_amd_ext.h"""
+
+    _fields_ = [
+        ("dtype", C.c_uint32), ("weight_dtype", C.c_uint32), ("rows", C.c_uint32 * 3), ("dim", C.c_uint32), ("eps", C.c_float),
+        ("x", C.c_void_p), ("residual", C.c_void_p), ("weight", C.c_void_p), ("bias", C.c_void_p),
+        ("x_stride", C.c_int64 * 3), ("residual_stride", C.c_int64 * 3),
+    ]
+
+
+class ZenoAmdNormGradients(C.Structure):
+    """include/zeno_amd_ext.h"""
+
+    _fields_ = [
+        ("d_y", C.c_void_p), ("d_sum", C.c_void_p), ("d_x", C.c_void_p), ("d_weight", C.c_void_p), ("d_bias", C.c_void_p),
+        ("d_y_stride", C.c_int64 * 3), ("d_sum_stride", C.c_int64 * 3), ("d_x_stride", C.c_int64 * 3),
+    ]
+
+
 _vp = C.c_void_p
 _fp = C.POINTER(C.c_float)
 _u8p = C.POINTER(C.c_uint8)
 _u32p = C.POINTER(C.c_uint32)
 _i64p = C.POINTER(C.c_int64)
 _delta = C.POINTER(ZenoAmdDeltaInputs)
+_norm = C.POINTER(ZenoAmdNormInputs)
 
 # name: (restype, argtypes)
 SIGNATURES = {
@@ -220,6 +240,9 @@ SIGNATURES = {
     "zeno_amd_delta_step": (C.c_int, [_delta, _vp, _i64p, _vp, _vp]),
     "zeno_amd_orthogonalize_workspace_bytes": (C.c_uint64, [C.POINTER(ZenoAmdOrthogonalize)]),
     "zeno_amd_orthogonalize": (C.c_int, [C.POINTER(ZenoAmdOrthogonalize), _vp, _vp]),
+    "zeno_amd_norm_forward": (C.c_int, [_norm, _vp, _i64p, _vp, _i64p, _vp]),
+    "zeno_amd_norm_backward": (C.c_int, [_norm, C.POINTER(ZenoAmdNormGradients), _vp, _vp]),
+    "zeno_amd_norm_workspace_bytes": (C.c_uint64, [_norm]),
     "zeno_amd_world_waves_per_group": (C.c_uint32, [C.c_void_p]),
     "zeno_amd_world_split_groups": (C.c_int, [C.c_void_p]),
 }

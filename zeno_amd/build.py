@@ -40,6 +40,8 @@ STEP_FLAGS = ["-Rpass-analysis=kernel-resource-usage", "-mllvm", "-align-all-nof
 # The operators of policies are compared with tolerances, not bit for bit: products and sums may
 # contract. No packed fp32 instructions here either.
 POLICY_SOURCES = ("delta.hip", "delta_f32.hip", "delta_f16.hip", "delta_bf16.hip", "orth.hip")
+# Those of them without matrix instructions, whose waits the tests read in the others' assembly.
+ROW_SOURCES = ("norm.hip", "norm_f32.hip", "norm_f16.hip", "norm_bf16.hip")
 POLICY_FLAGS = [
     f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-fno-fast-math",
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
@@ -119,7 +121,7 @@ def build_library() -> Path:
         obj = BUILD / (src + ".o")
         extra = STEP_FLAGS if src == "step.hip" else []
         jobs.append([hipcc, *HIP_FLAGS, *extra, "-c", str(CSRC / src), "-o", str(obj)])
-    for src in POLICY_SOURCES:
+    for src in POLICY_SOURCES + ROW_SOURCES:
         jobs.append([hipcc, *policy_flags(src), "-c", str(CSRC / src), "-o", str(BUILD / (src + ".o"))])
     with ThreadPoolExecutor(max_workers=min(len(jobs), os.cpu_count() or 4)) as ex:
         outs = list(ex.map(_run, jobs))
@@ -128,7 +130,7 @@ def build_library() -> Path:
     occ = step_occupancy(remarks)
     print("step_kernel waves per SIMD (EPW,PL,HASH): " + " ".join(f"{k}={v}" for k, v in sorted(occ.items())),
           file=sys.stderr)
-    objs = [str(BUILD / (s + ".o")) for s in ("mjcf.cpp", "model.cpp", "step.hip", "world.hip", "capi.hip", "collide.hip", *POLICY_SOURCES)]
+    objs = [str(BUILD / (s + ".o")) for s in ("mjcf.cpp", "model.cpp", "step.hip", "world.hip", "capi.hip", "collide.hip", *POLICY_SOURCES, *ROW_SOURCES)]
     tmp = LIB.with_suffix(".so.tmp")
     _run([hipcc, f"--offload-arch={ARCH}", "-shared", "-fPIC", *objs, "-o", str(tmp)])
     os.replace(tmp, LIB)

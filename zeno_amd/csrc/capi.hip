@@ -11,6 +11,7 @@
 #include "../../include/zeno_amd_ext.h"
 #include "collide.h"
 #include "delta.h"
+#include "norm.h"
 #include "orth.h"
 #include "world.h"
 
@@ -604,6 +605,32 @@ int zeno_amd_orthogonalize(const ZenoAmdOrthogonalize* args, void* workspace, vo
         return ZENO_INVALID_ARGUMENT;
     }
     return hip_status(za::orth::run(*args, workspace, (hipStream_t)stream), "orthogonalize");
+}
+
+static int norm_refused(const char* what, const std::string& why) {
+    set_error(std::string(what) + ": " + why);
+    return ZENO_INVALID_ARGUMENT;
+}
+
+int zeno_amd_norm_forward(const ZenoAmdNormInputs* in, void* y, const int64_t* y_stride, void* sum, const int64_t* sum_stride, void* stream) {
+    std::string why = za::norm::check(in);
+    if (why.empty()) why = za::norm::check_forward(*in, y, y_stride, sum, sum_stride);
+    if (!why.empty()) return norm_refused("norm_forward", why);
+    return hip_status(za::norm::forward(*in, y, y_stride, sum, sum_stride, (hipStream_t)stream), "norm_forward");
+}
+
+int zeno_amd_norm_backward(const ZenoAmdNormInputs* in, const ZenoAmdNormGradients* grad, void* workspace, void* stream) {
+    std::string why = za::norm::check(in);
+    if (why.empty() && !grad) why = "null gradient";
+    if (why.empty()) why = za::norm::check_backward(*in, *grad);
+    if (why.empty() && ((uintptr_t)workspace % 16 || (!workspace && (grad->d_weight || grad->d_bias))))
+        why = "workspace is null or not aligned to 16 bytes";
+    if (!why.empty()) return norm_refused("norm_backward", why);
+    return hip_status(za::norm::backward(*in, *grad, (float*)workspace, (hipStream_t)stream), "norm_backward");
+}
+
+uint64_t zeno_amd_norm_workspace_bytes(const ZenoAmdNormInputs* in) {
+    return za::norm::check(in).empty() ? 4 * za::norm::workspace_floats(*in) : 0;
 }
 
 }  // extern "C"
