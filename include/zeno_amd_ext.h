@@ -365,6 +365,62 @@ int zeno_amd_norm_forward(const ZenoAmdNormInputs* in, void* y, const int64_t* y
 int zeno_amd_norm_backward(const ZenoAmdNormInputs* in, const ZenoAmdNormGradients* grad, void* workspace, void* stream);
 uint64_t zeno_amd_norm_workspace_bytes(const ZenoAmdNormInputs* in); /* 0 for refused arguments */
 
+/* Linear attention with a decay for each head, a memory layer without the delta rule's correction: per
+ * sequence and value head, S [key_dim, value_dim],
+ *
+ *     S <- exp(g) S + k v^T        (S <- k v^T at a token whose reset flag is set)
+ *     o  = scale S^T q
+ *
+ * with q and k of key head (value head / (value_heads / key_heads)) and one g a value head. Nothing
+ * before a reset, NaN or infinity included, reaches what follows. q, k, v and o have one element type; g and
+ * every state are fp32, and all sums are. Pointers, strides, streams and what outputs may overlap are as
+ * above, but that only a step's o may be v. */
+#define ZENO_AMD_LINEAR_MAX_DIM 128u /* of key_dim and value_dim */
+
+typedef struct {
+    uint32_t dtype;                   /* of q, k, v, o and their gradients */
+    uint32_t batch, length;           /* sequences, tokens */
+    uint32_t key_heads, value_heads;  /* value_heads is a multiple of key_heads */
+    uint32_t key_dim, value_dim;      /* 1 to ZENO_AMD_LINEAR_MAX_DIM */
+    uint32_t decay_gradient;          /* the gradient of g is (or will be) wanted */
+    float scale;
+    const void *q, *k, *v;
+    const float* g;                   /* [value_heads]: log of the decay */
+    const uint8_t* reset;             /* [sequence, token], nonzero: the state is cleared before it; null: none */
+    const float* state;               /* [batch, value_heads, key_dim, value_dim] before the first token; null: zeros */
+    int64_t q_stride[3], k_stride[3], v_stride[3];
+    int64_t reset_stride[2];
+} ZenoAmdLinearInputs;
+
+/* Gradients: of o and of the last state (null: zeros) in; of the inputs out. d_g is wanted where
+ * decay_gradient is set, d_state may be null. */
+typedef struct {
+    const void* d_o;
+    int64_t d_o_stride[3];
+    const float* d_last;
+    void *d_q, *d_k, *d_v;
+    float* d_g;
+    float* d_state;
+    int64_t d_q_stride[3], d_k_stride[3], d_v_stride[3];
+} ZenoAmdLinearGradients;
+
+/* Whole sequences. o [batch, length, value_heads, value_dim] by o_stride; last [batch, value_heads,
+ * key_dim, value_dim], contiguous, the state after the last token. `saved`: null, or
+ * zeno_amd_linear_saved_bytes(in) bytes that the gradients of this call read. `workspace`:
+ * zeno_amd_linear_workspace_bytes(in, 0) bytes. Both aligned to 16 bytes, null where 0 bytes are needed. */
+int zeno_amd_linear_forward(const ZenoAmdLinearInputs* in, void* o, const int64_t* o_stride, float* last, void* saved, void* workspace, void* stream);
+
+/* Gradients of a zeno_amd_linear_forward call with the same inputs, which left `saved`. `workspace`:
+ * zeno_amd_linear_workspace_bytes(in, 1) bytes. The gradient of g keeps fp32's digits relative to its own
+ * size for heads that forget fast too. All sums are in a fixed order: results are bitwise reproducible. */
+int zeno_amd_linear_backward(const ZenoAmdLinearInputs* in, const void* saved, const ZenoAmdLinearGradients* grad, void* workspace, void* stream);
+
+uint64_t zeno_amd_linear_saved_bytes(const ZenoAmdLinearInputs* in);  /* 0 also for invalid inputs */
+uint64_t zeno_amd_linear_workspace_bytes(const ZenoAmdLinearInputs* in, uint32_t backward);
+
+/* One token (length 1) for every sequence: `state` is advanced in place (in->state is not read). */
+int zeno_amd_linear_step(const ZenoAmdLinearInputs* in, void* o, const int64_t* o_stride, float* state, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -139,6 +139,28 @@ class ZenoAmdNormGradients(C.Structure):
     ]
 
 
+class ZenoAmdLinearInputs(C.Structure):
+    """include/zeno_amd_ext.h"""
+
+    _fields_ = [
+        ("dtype", C.c_uint32), ("batch", C.c_uint32), ("length", C.c_uint32),
+        ("key_heads", C.c_uint32), ("value_heads", C.c_uint32), ("key_dim", C.c_uint32), ("value_dim", C.c_uint32),
+        ("decay_gradient", C.c_uint32), ("scale", C.c_float),
+        ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("g", C.c_void_p), ("reset", C.c_void_p), ("state", C.c_void_p),
+        ("q_stride", C.c_int64 * 3), ("k_stride", C.c_int64 * 3), ("v_stride", C.c_int64 * 3), ("reset_stride", C.c_int64 * 2),
+    ]
+
+
+class ZenoAmdLinearGradients(C.Structure):
+    """include/zeno_amd_ext.h"""
+
+    _fields_ = [
+        ("d_o", C.c_void_p), ("d_o_stride", C.c_int64 * 3), ("d_last", C.c_void_p),
+        ("d_q", C.c_void_p), ("d_k", C.c_void_p), ("d_v", C.c_void_p), ("d_g", C.c_void_p), ("d_state", C.c_void_p),
+        ("d_q_stride", C.c_int64 * 3), ("d_k_stride", C.c_int64 * 3), ("d_v_stride", C.c_int64 * 3),
+    ]
+
+
 _vp = C.c_void_p
 _fp = C.POINTER(C.c_float)
 _u8p = C.POINTER(C.c_uint8)
@@ -146,6 +168,7 @@ _u32p = C.POINTER(C.c_uint32)
 _i64p = C.POINTER(C.c_int64)
 _delta = C.POINTER(ZenoAmdDeltaInputs)
 _norm = C.POINTER(ZenoAmdNormInputs)
+_linear = C.POINTER(ZenoAmdLinearInputs)
 
 # name: (restype, argtypes)
 SIGNATURES = {
@@ -240,6 +263,11 @@ SIGNATURES = {
     "zeno_amd_delta_step": (C.c_int, [_delta, _vp, _i64p, _vp, _vp]),
     "zeno_amd_orthogonalize_workspace_bytes": (C.c_uint64, [C.POINTER(ZenoAmdOrthogonalize)]),
     "zeno_amd_orthogonalize": (C.c_int, [C.POINTER(ZenoAmdOrthogonalize), _vp, _vp]),
+    "zeno_amd_linear_forward": (C.c_int, [_linear, _vp, _i64p, _vp, _vp, _vp, _vp]),
+    "zeno_amd_linear_backward": (C.c_int, [_linear, _vp, C.POINTER(ZenoAmdLinearGradients), _vp, _vp]),
+    "zeno_amd_linear_saved_bytes": (C.c_uint64, [_linear]),
+    "zeno_amd_linear_workspace_bytes": (C.c_uint64, [_linear, C.c_uint32]),
+    "zeno_amd_linear_step": (C.c_int, [_linear, _vp, _i64p, _vp, _vp]),
     "zeno_amd_norm_forward": (C.c_int, [_norm, _vp, _i64p, _vp, _i64p, _vp]),
     "zeno_amd_norm_backward": (C.c_int, [_norm, C.POINTER(ZenoAmdNormGradients), _vp, _vp]),
     "zeno_amd_norm_workspace_bytes": (C.c_uint64, [_norm]),

@@ -39,9 +39,9 @@ HIP_FLAGS = [
 STEP_FLAGS = ["-Rpass-analysis=kernel-resource-usage", "-mllvm", "-align-all-nofallthru-blocks=6"]
 # The operators of policies are compared with tolerances, not bit for bit: products and sums may
 # contract. No packed fp32 instructions here either.
-POLICY_SOURCES = ("delta.hip", "delta_f32.hip", "delta_f16.hip", "delta_bf16.hip", "orth.hip")
+POLICY_SOURCES = ("delta.hip", "delta_f32.hip", "delta_f16.hip", "delta_bf16.hip", "orth.hip", "linear_f32.hip", "linear_f16.hip", "linear_bf16.hip")
 # Those of them without matrix instructions, whose waits the tests read in the others' assembly.
-ROW_SOURCES = ("norm.hip", "norm_f32.hip", "norm_f16.hip", "norm_bf16.hip")
+ROW_SOURCES = ("linear.hip", "norm.hip", "norm_f32.hip", "norm_f16.hip", "norm_bf16.hip")
 POLICY_FLAGS = [
     f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-fno-fast-math",
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",

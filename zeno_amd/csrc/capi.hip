@@ -11,6 +11,7 @@
 #include "../../include/zeno_amd_ext.h"
 #include "collide.h"
 #include "delta.h"
+#include "linear.h"
 #include "norm.h"
 #include "orth.h"
 #include "world.h"
@@ -631,6 +632,48 @@ int zeno_amd_norm_backward(const ZenoAmdNormInputs* in, const ZenoAmdNormGradien
 
 uint64_t zeno_amd_norm_workspace_bytes(const ZenoAmdNormInputs* in) {
     return za::norm::check(in).empty() ? 4 * za::norm::workspace_floats(*in) : 0;
+}
+
+static int linear_refused(const char* what, const std::string& why) {
+    set_error(std::string(what) + ": " + why);
+    return ZENO_INVALID_ARGUMENT;
+}
+static const char* const kLinearBuffers = "saved or workspace is not aligned to 16 bytes, or is null";
+
+int zeno_amd_linear_forward(const ZenoAmdLinearInputs* in, void* o, const int64_t* o_stride, float* last, void* saved, void* workspace, void* stream) {
+    std::string why = za::linear::check(in, false);
+    if (why.empty() && (!o || !o_stride || !last)) why = "null output";
+    if (why.empty() && ((uintptr_t)saved % 16 || (uintptr_t)workspace % 16 || (!workspace && za::linear::workspace_floats(*in, false)))) why = kLinearBuffers;
+    if (why.empty()) why = za::linear::check_overlap(*in, o, o_stride, last, false);
+    if (!why.empty()) return linear_refused("linear_forward", why);
+    return hip_status(za::linear::forward(*in, o, o_stride, last, (float*)saved, (float*)workspace, (hipStream_t)stream), "linear_forward");
+}
+
+int zeno_amd_linear_backward(const ZenoAmdLinearInputs* in, const void* saved, const ZenoAmdLinearGradients* grad, void* workspace, void* stream) {
+    std::string why = za::linear::check(in, false);
+    if (why.empty() && !grad) why = "null gradient";
+    if (why.empty() && ((uintptr_t)saved % 16 || (uintptr_t)workspace % 16 || (!saved && za::linear::saved_floats(*in)) ||
+                        (!workspace && za::linear::workspace_floats(*in, true))))
+        why = kLinearBuffers;
+    if (why.empty()) why = za::linear::check_gradients(*in, *grad);
+    if (!why.empty()) return linear_refused("linear_backward", why);
+    return hip_status(za::linear::backward(*in, (const float*)saved, *grad, (float*)workspace, (hipStream_t)stream), "linear_backward");
+}
+
+uint64_t zeno_amd_linear_saved_bytes(const ZenoAmdLinearInputs* in) {
+    return in && za::linear::check_sizes(*in, false).empty() ? 4 * za::linear::saved_floats(*in) : 0;
+}
+
+uint64_t zeno_amd_linear_workspace_bytes(const ZenoAmdLinearInputs* in, uint32_t backward) {
+    return in && za::linear::check_sizes(*in, false).empty() ? 4 * za::linear::workspace_floats(*in, backward != 0) : 0;
+}
+
+int zeno_amd_linear_step(const ZenoAmdLinearInputs* in, void* o, const int64_t* o_stride, float* state, void* stream) {
+    std::string why = za::linear::check(in, true);
+    if (why.empty() && (!o || !o_stride || !state)) why = "null output or state";
+    if (why.empty()) why = za::linear::check_overlap(*in, o, o_stride, state, true);
+    if (!why.empty()) return linear_refused("linear_step", why);
+    return hip_status(za::linear::step(*in, o, o_stride, state, (hipStream_t)stream), "linear_step");
 }
 
 }  // extern "C"

@@ -1,0 +1,97 @@
+// Linear attention with a decay for each head: host side (argument checks, launch shapes) and the
+// kernels' arguments.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <string>
+
+#include "../../include/zeno_amd_ext.h"
+
+namespace za {
+namespace linear {
+
+constexpr int kChunk = 32;  // tokens of the grid that segments are cut on
+
+// Rows of one of the inputs. Strides are in elements: sequence, token, head.
+struct Rows {
+    const void* at;
+    int64_t stride[3];
+    uint32_t share;  // heads that read one of these
+};
+
+// One walk over the sequences, forward or back. With A, B and C three of the rows and S a state
+// [da, dc]: the outputs of a token are sums over the tokens behind it in the walk's direction,
+//     out_i = scale sum_j exp(g |i - j|) (A_i . B_j) C_j + A_i S,   S <- exp(g) S + B_i C_i^T
+// The operator itself is the walk forward of q, k, v; its gradients are those of d_o, v, k (forward:
+// d_q), of k, q, d_o (back: d_v) and of v, d_o, q (back: d_k).
+struct Walk {
+    Rows a, b, c, q;             // q: what the outputs of d_q are multiplied with for the gradient of g
+    int da, dc;
+    uint32_t batch, heads;       // value heads
+    int length;
+    float scale;
+    const float* g;
+    const uint8_t* reset;
+    int64_t reset_stride[2];
+    void* out;
+    int64_t out_stride[3];
+    uint32_t out_share;
+    bool out_f32;                // part sums per value head, where heads share one
+    const float* first;          // the state that the walk begins with; null: zeros
+    float* last;                 // the state that it ends with; null: not wanted
+    int row, col;                // strides of a state's rows and columns in memory
+    int64_t size;                // of a state
+    // A long sequence is cut into segments that are walked side by side. Between them: states (and
+    // slopes, see the kernels) [batch, heads, segments - 1, size], and whether a state passes the
+    // segment, [batch, heads, segments - 1].
+    uint32_t segments;
+    int segment_length;          // tokens, whole chunks
+    float *starts, *slopes, *passes;
+    const float* d_last;         // for the gradient of g; null: zeros
+    double* parts;               // of it: [walks]
+    uint32_t blocks;             // waves that share the columns
+    bool full;                   // dimensions as wide as the launch shape
+};
+
+// Launch shape: `steps` and `cols` times 32 rows and columns of the state a wave.
+struct Shape {
+    int steps, cols;
+    bool full;
+    uint32_t blocks;
+};
+Shape shape_of(uint32_t dtype, int da, int dc, bool slope);
+struct Segments {
+    uint32_t count;
+    int length;
+};
+Segments segments_of(const ZenoAmdLinearInputs& in);
+uint64_t saved_floats(const ZenoAmdLinearInputs& in);
+uint64_t workspace_floats(const ZenoAmdLinearInputs& in, bool train);
+
+enum Kind { OUTPUTS, OUTPUTS_SLOPE, STATES, STATES_SLOPE };  // SLOPE: with what the gradient of g needs
+
+// One translation unit per element type.
+template <int TY> hipError_t launch_walk(const Walk& w, const Shape& s, Kind kind, bool back, hipStream_t stream);
+template <int TY> hipError_t launch_share(const float* parts, void* out, const int64_t* stride, uint32_t batch, uint32_t length, uint32_t key_heads, uint32_t share,
+                                          uint32_t dim, hipStream_t stream);
+template <int TY> hipError_t launch_step(const ZenoAmdLinearInputs& in, void* o, const int64_t* o_stride, float* state, hipStream_t stream);
+
+// Of the single step: a wave holds all rows of 4 `lanes` columns of a head.
+inline int step_lanes(const ZenoAmdLinearInputs& in) { return in.key_dim <= 32 || in.key_dim > 64 ? 8 : 16; }
+inline uint64_t step_waves(const ZenoAmdLinearInputs& in) {
+    const uint32_t cols = 4 * step_lanes(in);
+    return (uint64_t)in.batch * in.value_heads * ((in.value_dim + cols - 1) / cols);
+}
+
+// Entry points behind the C ABI. A non-empty message means that nothing was launched.
+std::string check_sizes(const ZenoAmdLinearInputs& in, bool step);
+std::string check(const ZenoAmdLinearInputs* in, bool step);
+std::string check_overlap(const ZenoAmdLinearInputs& in, const void* o, const int64_t* o_stride, const float* state, bool step);
+std::string check_gradients(const ZenoAmdLinearInputs& in, const ZenoAmdLinearGradients& grad);
+hipError_t forward(const ZenoAmdLinearInputs& in, void* o, const int64_t* o_stride, float* last, float* saved, float* workspace, hipStream_t stream);
+hipError_t backward(const ZenoAmdLinearInputs& in, const float* saved, const ZenoAmdLinearGradients& grad, float* workspace, hipStream_t stream);
+hipError_t step(const ZenoAmdLinearInputs& in, void* o, const int64_t* o_stride, float* state, hipStream_t stream);
+
+}  // namespace linear
+}  // namespace za

@@ -1,0 +1,301 @@
+// Linear attention with a decay for each head: argument checks, launch shapes and dispatch by element type.
+#include "linear.h"
+
+#include <algorithm>
+#include <cmath>
+#include <vector>
+
+#include "mma.h"
+#include "overlap.h"
+
+namespace za {
+namespace linear {
+
+using mma::T_BF16;
+using mma::T_F16;
+using mma::T_F32;
+
+namespace {
+
+// The gradient of g: the walks' parts of each head, in order, in 64 bits.
+__global__ __launch_bounds__(256) void linear_decay_kernel(const double* parts, uint32_t batch, uint32_t heads, uint32_t each, float* d_g) {
+    __shared__ double all[256];
+    const uint32_t h = blockIdx.x;
+    const int64_t n = (int64_t)batch * each;
+    double sum = 0.0;
+    for (int64_t i = threadIdx.x; i < n; i += 256) sum += parts[(i / each * heads + h) * each + i % each];
+    all[threadIdx.x] = sum;
+    __syncthreads();
+    for (int d = 128; d; d >>= 1) {
+        if ((int)threadIdx.x < d) all[threadIdx.x] += all[threadIdx.x + d];
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) d_g[h] = (float)all[0];
+}
+
+int64_t bytes_of(uint32_t dtype) { return dtype == T_F32 ? 4 : 2; }
+uint64_t heads_of(const ZenoAmdLinearInputs& in) { return (uint64_t)in.batch * in.value_heads; }
+uint64_t even(uint64_t floats) { return (floats + 3) / 4 * 4; }  // 16 bytes
+int64_t state_size(const ZenoAmdLinearInputs& in) { return (int64_t)in.key_dim * in.value_dim; }
+uint64_t between(const ZenoAmdLinearInputs& in) { return heads_of(in) * (segments_of(in).count - 1); }
+uint64_t states_floats(const ZenoAmdLinearInputs& in) { return even(between(in) * state_size(in)); }
+uint64_t share_floats(const ZenoAmdLinearInputs& in) {  // gradients of q (or k) by value head
+    return in.key_heads == in.value_heads ? 0 : even((uint64_t)in.batch * in.length * in.value_heads * in.key_dim);
+}
+Shape slope_shape(const ZenoAmdLinearInputs& in) { return shape_of(in.dtype, in.value_dim, in.key_dim, true); }
+uint64_t parts_floats(const ZenoAmdLinearInputs& in) { return in.decay_gradient ? even(2 * heads_of(in) * segments_of(in).count * slope_shape(in).blocks) : 0; }
+
+void set_strides(int64_t* to, const int64_t* from) {
+    for (int i = 0; i < 3; ++i) to[i] = from[i];
+}
+Rows rows_of(const void* at, const int64_t* stride, uint32_t share) {
+    Rows r{};
+    r.at = at;
+    set_strides(r.stride, stride);
+    r.share = share;
+    return r;
+}
+
+hipError_t launch(uint32_t dtype, const Walk& w, const Shape& s, Kind kind, bool back, hipStream_t stream) {
+    return dtype == T_F32   ? launch_walk<T_F32>(w, s, kind, back, stream)
+           : dtype == T_F16 ? launch_walk<T_F16>(w, s, kind, back, stream)
+                            : launch_walk<T_BF16>(w, s, kind, back, stream);
+}
+
+// A walk over states [key_dim, value_dim], or (turned) over them transposed.
+Walk walk_of(const ZenoAmdLinearInputs& in, bool turned) {
+    Walk w{};
+    w.da = turned ? in.value_dim : in.key_dim;
+    w.dc = turned ? in.key_dim : in.value_dim;
+    w.row = turned ? 1 : in.value_dim;
+    w.col = turned ? in.value_dim : 1;
+    w.size = state_size(in);
+    w.batch = in.batch;
+    w.heads = in.value_heads;
+    w.length = in.length;
+    w.scale = in.scale;
+    w.g = in.g;
+    w.reset = in.reset;
+    w.reset_stride[0] = in.reset_stride[0];
+    w.reset_stride[1] = in.reset_stride[1];
+    const Segments s = segments_of(in);
+    w.segments = s.count;
+    w.segment_length = s.length;
+    return w;
+}
+void set_shape(Walk& w, const Shape& s) {
+    w.blocks = s.blocks;
+    w.full = s.full;
+}
+
+std::string check_outputs(const std::vector<Memory>& inputs, const std::vector<Memory>& outputs) {
+    for (size_t i = 0; i < outputs.size(); ++i) {
+        if (!outputs[i].apart_from_itself()) return "a gradient overlaps itself";
+        for (const Memory& x : inputs)
+            if (!apart(outputs[i], x)) return "a gradient overlaps an input";
+        for (size_t j = 0; j < i; ++j)
+            if (!apart(outputs[i], outputs[j])) return "gradients overlap";
+    }
+    return "";
+}
+
+}  // namespace
+
+// A wave holds 64 columns of the state in 16-bit types where that leaves room for the rows, else 32.
+Shape shape_of(uint32_t dtype, int da, int dc, bool slope) {
+    Shape s;
+    s.steps = da <= 32 ? 1 : da <= 64 ? 2 : 4;
+    s.cols = dtype != T_F32 && s.steps < 4 && dc > 32 && !slope ? 2 : 1;
+    s.blocks = (dc + 32 * s.cols - 1) / (32 * s.cols);
+    s.full = da == 32 * s.steps && dc == 32 * s.cols * (int)s.blocks;
+    return s;
+}
+
+// With fewer walks than two waves a SIMD, as many segments as make up those, of at least four chunks.
+Segments segments_of(const ZenoAmdLinearInputs& in) {
+    const int64_t chunks = ((int64_t)in.length + kChunk - 1) / kChunk;
+    const int64_t walks = (int64_t)heads_of(in) * shape_of(in.dtype, in.key_dim, in.value_dim, false).blocks;
+    int64_t want = std::min(2048 / walks, chunks / 4);
+    if (want < 2) want = 1;
+    const int64_t each = (chunks + want - 1) / want;
+    return Segments{(uint32_t)((chunks + each - 1) / each), (int)(each * kChunk)};
+}
+
+uint64_t saved_floats(const ZenoAmdLinearInputs& in) { return states_floats(in) * (in.decay_gradient ? 2 : 1); }
+uint64_t workspace_floats(const ZenoAmdLinearInputs& in, bool train) {
+    return even(between(in)) + states_floats(in) + (train ? 2 * share_floats(in) + parts_floats(in) : 0);
+}
+
+std::string check_sizes(const ZenoAmdLinearInputs& in, bool step) {
+    if (in.dtype > T_BF16) return "dtype is none of float32, float16, bfloat16";
+    if (!in.batch || !in.length || !in.key_heads || !in.value_heads) return "batch, length and head counts must be positive";
+    if (in.value_heads % in.key_heads) return "value_heads is not a multiple of key_heads";
+    if (!in.key_dim || in.key_dim > ZENO_AMD_LINEAR_MAX_DIM || !in.value_dim || in.value_dim > ZENO_AMD_LINEAR_MAX_DIM)
+        return "key_dim and value_dim must be 1 to " + std::to_string(ZENO_AMD_LINEAR_MAX_DIM);
+    // A launch takes less than 2^32 threads: up to four waves for each sequence and head.
+    if (in.length > 0x7fffff00u || heads_of(in) > 0xffffff00ull / 256) return "too many sequences or tokens";
+    if (step && in.length != 1) return "a step takes one token";
+    return "";
+}
+
+std::string check(const ZenoAmdLinearInputs* p, bool step) {
+    if (!p) return "null arguments";
+    const std::string why = check_sizes(*p, step);
+    if (!why.empty()) return why;
+    if (!p->q || !p->k || !p->v || !p->g) return "null input";
+    if (!std::isfinite(p->scale)) return "scale is not finite";
+    return "";
+}
+
+namespace {
+struct Places {  // what a call's arrays cover
+    int64_t eb, keys[3], values[3], states, none[1] = {0}, one[1] = {1};
+    explicit Places(const ZenoAmdLinearInputs& in)
+        : eb(bytes_of(in.dtype)), keys{in.batch, in.length, in.key_heads}, values{in.batch, in.length, in.value_heads}, states((int64_t)heads_of(in) * state_size(in)) {}
+    Memory key(const ZenoAmdLinearInputs& in, const void* p, const int64_t* stride) const { return Memory(p, stride, keys, 3, in.key_dim, eb); }
+    Memory value(const ZenoAmdLinearInputs& in, const void* p, const int64_t* stride) const { return Memory(p, stride, values, 3, in.value_dim, eb); }
+    Memory floats(const void* p, int64_t n) const { return Memory(p, none, one, 1, n, 4); }
+    std::vector<Memory> inputs(const ZenoAmdLinearInputs& in, bool with_state) const {
+        std::vector<Memory> m{key(in, in.q, in.q_stride), key(in, in.k, in.k_stride), floats(in.g, in.value_heads)};
+        if (in.reset) m.push_back(Memory(in.reset, in.reset_stride, values, 2, 1, 1));
+        if (with_state && in.state) m.push_back(floats(in.state, states));
+        return m;
+    }
+};
+}  // namespace
+
+std::string check_overlap(const ZenoAmdLinearInputs& in, const void* o, const int64_t* o_stride, const float* state, bool step) {
+    const Places at(in);
+    const Memory out = at.value(in, o, o_stride), kept = at.floats(state, at.states), v = at.value(in, in.v, in.v_stride);
+    if (!out.apart_from_itself()) return "o overlaps itself";
+    if (!apart(out, kept)) return "o overlaps the state";
+    // A step's o may be v itself, value by value: the wave that writes a value has read it.
+    bool same = step && o == in.v;
+    for (int i = 0; i < 3; ++i) same = same && (at.values[i] == 1 || o_stride[i] == in.v_stride[i]);
+    if (!same && !apart(out, v)) return "o overlaps v";
+    bool clear = apart(kept, v);
+    for (const Memory& x : at.inputs(in, !step)) {
+        if (!apart(out, x)) return "o overlaps an input";
+        clear = clear && apart(kept, x);
+    }
+    return clear ? "" : "the state overlaps an input";
+}
+
+std::string check_gradients(const ZenoAmdLinearInputs& in, const ZenoAmdLinearGradients& grad) {
+    if (!grad.d_o || !grad.d_q || !grad.d_k || !grad.d_v) return "null gradient";
+    if (!in.decay_gradient != !grad.d_g) return "d_g comes with decay_gradient";
+    const Places at(in);
+    std::vector<Memory> reads = at.inputs(in, true), writes{at.key(in, grad.d_q, grad.d_q_stride), at.key(in, grad.d_k, grad.d_k_stride), at.value(in, grad.d_v, grad.d_v_stride)};
+    reads.push_back(at.value(in, in.v, in.v_stride));
+    reads.push_back(at.value(in, grad.d_o, grad.d_o_stride));
+    if (grad.d_last) reads.push_back(at.floats(grad.d_last, at.states));
+    if (grad.d_g) writes.push_back(at.floats(grad.d_g, in.value_heads));
+    if (grad.d_state) writes.push_back(at.floats(grad.d_state, at.states));
+    return check_outputs(reads, writes);
+}
+
+hipError_t forward(const ZenoAmdLinearInputs& in, void* o, const int64_t* o_stride, float* last, float* saved, float* workspace, hipStream_t stream) {
+    const uint32_t share = in.value_heads / in.key_heads;
+    Walk w = walk_of(in, false);
+    w.a = rows_of(in.q, in.q_stride, share);
+    w.b = rows_of(in.k, in.k_stride, share);
+    w.c = rows_of(in.v, in.v_stride, 1);
+    w.out = o;
+    set_strides(w.out_stride, o_stride);
+    w.out_share = 1;
+    w.first = in.state;
+    w.last = last;
+    w.passes = workspace;
+    w.starts = saved ? saved : workspace + even(between(in));
+    if (w.segments > 1) {
+        const bool slope = saved && in.decay_gradient;
+        const Shape s = shape_of(in.dtype, w.da, w.dc, slope);
+        set_shape(w, s);
+        if (slope) w.slopes = saved + states_floats(in);
+        if (const hipError_t e = launch(in.dtype, w, s, slope ? STATES_SLOPE : STATES, false, stream)) return e;
+    }
+    const Shape s = shape_of(in.dtype, w.da, w.dc, false);
+    set_shape(w, s);
+    return launch(in.dtype, w, s, OUTPUTS, false, stream);
+}
+
+hipError_t backward(const ZenoAmdLinearInputs& in, const float* saved, const ZenoAmdLinearGradients& grad, float* workspace, hipStream_t stream) {
+    const uint32_t share = in.value_heads / in.key_heads;
+    const Rows q = rows_of(in.q, in.q_stride, share), k = rows_of(in.k, in.k_stride, share), v = rows_of(in.v, in.v_stride, 1),
+               d_o = rows_of(grad.d_o, grad.d_o_stride, 1);
+    float* passes = workspace;
+    float* d_starts = passes + even(between(in));
+    float* parts = d_starts + states_floats(in);
+    float* part_q = parts + parts_floats(in);
+    float* part_k = part_q + share_floats(in);
+    const int64_t part_stride[3] = {(int64_t)in.length * in.value_heads * in.key_dim, (int64_t)in.value_heads * in.key_dim, in.key_dim};
+    auto key_out = [&](Walk& w, void* to, const int64_t* stride, float* part) {
+        w.out = share > 1 ? part : to;
+        set_strides(w.out_stride, share > 1 ? part_stride : stride);
+        w.out_share = 1;
+        w.out_f32 = share > 1;
+    };
+    hipError_t e;
+
+    // d_v, and before it what it starts its segments with
+    Walk w = walk_of(in, false);
+    w.a = k;
+    w.b = q;
+    w.c = d_o;
+    w.out = grad.d_v;
+    set_strides(w.out_stride, grad.d_v_stride);
+    w.out_share = 1;
+    w.first = grad.d_last;
+    w.last = grad.d_state;
+    w.starts = d_starts;
+    w.passes = passes;
+    Shape s = shape_of(in.dtype, w.da, w.dc, false);
+    set_shape(w, s);
+    if (w.segments > 1 && (e = launch(in.dtype, w, s, STATES, true, stream))) return e;
+    if ((e = launch(in.dtype, w, s, OUTPUTS, true, stream))) return e;
+
+    // d_k
+    w = walk_of(in, true);
+    w.a = v;
+    w.b = d_o;
+    w.c = q;
+    key_out(w, grad.d_k, grad.d_k_stride, part_k);
+    w.first = grad.d_last;
+    w.starts = d_starts;
+    s = shape_of(in.dtype, w.da, w.dc, false);
+    set_shape(w, s);
+    if ((e = launch(in.dtype, w, s, OUTPUTS, true, stream))) return e;
+
+    // d_q and d_g
+    w = walk_of(in, true);
+    w.a = d_o;
+    w.b = v;
+    w.c = k;
+    w.q = q;
+    key_out(w, grad.d_q, grad.d_q_stride, part_q);
+    w.first = in.state;
+    w.starts = const_cast<float*>(saved);
+    w.slopes = w.starts + states_floats(in);
+    w.d_last = grad.d_last;
+    w.parts = reinterpret_cast<double*>(parts);
+    s = grad.d_g ? slope_shape(in) : shape_of(in.dtype, w.da, w.dc, false);
+    set_shape(w, s);
+    if ((e = launch(in.dtype, w, s, grad.d_g ? OUTPUTS_SLOPE : OUTPUTS, false, stream))) return e;
+    if (grad.d_g) linear_decay_kernel<<<in.value_heads, 256, 0, stream>>>(w.parts, in.batch, in.value_heads, w.segments * s.blocks, grad.d_g);
+
+    if (share > 1) {
+        auto add = in.dtype == T_F32 ? launch_share<T_F32> : in.dtype == T_F16 ? launch_share<T_F16> : launch_share<T_BF16>;
+        if ((e = add(part_q, grad.d_q, grad.d_q_stride, in.batch, in.length, in.key_heads, share, in.key_dim, stream))) return e;
+        if ((e = add(part_k, grad.d_k, grad.d_k_stride, in.batch, in.length, in.key_heads, share, in.key_dim, stream))) return e;
+    }
+    return hipGetLastError();
+}
+
+hipError_t step(const ZenoAmdLinearInputs& in, void* o, const int64_t* o_stride, float* state, hipStream_t stream) {
+    return in.dtype == T_F32   ? launch_step<T_F32>(in, o, o_stride, state, stream)
+           : in.dtype == T_F16 ? launch_step<T_F16>(in, o, o_stride, state, stream)
+                               : launch_step<T_BF16>(in, o, o_stride, state, stream);
+}
+
+}  // namespace linear
+}  // namespace za

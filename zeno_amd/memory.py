@@ -1,4 +1,4 @@
-"""The memory layer of policies that act on partial observations: the gated delta rule.
+"""Memory layers of policies that act on partial observations: the gated delta rule and linear attention.
 
 Each environment (or recorded sequence) and head keeps a state S [key_dim, value_dim]. A token
 brings a query, a key, a value, the log of a decay and a strength, and
@@ -29,6 +29,17 @@ and infinity included, has no effect on what follows. A NaN or an infinity in an
 none on outputs before its token either; an infinity may make NaN of what it meets. Two limits:
 gradients of up to 31 tokens on either side of it may be NaN too, and so may up to 31 outputs before
 a token whose own sums overflow fp32.
+
+Linear attention with a decay for each head is the same without the correction and with one decay a head:
+
+    S <- exp(g) S + k v^T      (S <- k v^T where an episode begins)
+    o  = scale S^T q
+
+``linear_attention_step`` and ``linear_attention`` take q, k, v, reset and state as above and g [Hv] float32. It
+costs less than the delta rule, as tokens do not wait for one another inside a sequence, but what is stored under a
+key is added to, not replaced. Its outputs grow with the state: ``zeno_amd.norm.layer_norm`` over each head's
+output usually follows. Values that are not finite are kept apart as above, in the gradients too: a NaN reaches
+gradients of tokens up to its own only, through o, and none beyond a reset.
 """
 from __future__ import annotations
 
@@ -88,6 +99,16 @@ def _check(q, k, v, g, beta, reset, state, lead: int) -> None:
         apart = apart or state.device != device
     if apart:
         raise ValueError("the operands must be on one device")
+
+
+def _check_step(v, state, out) -> None:
+    """What a step writes in place."""
+    if not state.is_contiguous():
+        raise ValueError("state must be contiguous: it is advanced in place")
+    if (state.requires_grad or (out is not None and out.requires_grad)) and torch.is_grad_enabled():
+        raise ValueError("state and out are written in place, which autograd does not see: give detached ones, or step under torch.no_grad()")
+    if out is not None and (out.shape != v.shape or out.dtype != v.dtype or out.device != v.device or (out.stride(-1) != 1 and out.shape[-1] != 1)):
+        raise ValueError(f"out must be like v: {tuple(v.shape)}, {v.dtype}, on {v.device}, its last dimension contiguous")
 
 
 def _row(x: torch.Tensor) -> torch.Tensor:
@@ -200,21 +221,118 @@ def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
     (`out` if given; it may be v, but overlap nothing else that the step reads or writes). Without gradients, even where an operand asks for them: training runs
     gated_delta on the recorded rollout."""
     _check(q, k, v, g, beta, reset, state, 1)
-    if not state.is_contiguous():
-        raise ValueError("state must be contiguous: it is advanced in place")
-    if (state.requires_grad or (out is not None and out.requires_grad)) and torch.is_grad_enabled():
-        raise ValueError("state and out are written in place, which autograd does not see: give detached ones, or step under torch.no_grad()")
+    _check_step(v, state, out)
     q, k, v = _row(q), _row(k), _row(v)
     if out is None:
         out = torch.empty_like(v, memory_format=torch.contiguous_format)
-    elif out.shape != v.shape or out.dtype != v.dtype or out.device != v.device or (out.stride(-1) != 1 and out.shape[-1] != 1):
-        raise ValueError(f"out must be like v: {tuple(v.shape)}, {v.dtype}, on {v.device}, its last dimension contiguous")
     with _on(q):
         a = _inputs(q, k, v, g, beta, reset, state, q.shape[-1] ** -0.5 if scale is None else float(scale), bool(normalize))
         os = out.stride()
         rc = L.load().zeno_amd_delta_step(a, out.data_ptr(), _S3(os[0], 0, os[1]), state.data_ptr(), _stream(q))
         if rc:
             _fail(rc, "gated_delta_step")
+    _written(state)  # autograd refuses a backward pass that needs what was here
+    _written(out)
+    return out
+
+
+# ---- linear attention ------------------------------------------------------------------------
+def _check_linear(q, k, v, g, reset, state, lead: int) -> None:
+    if g.shape != v.shape[lead:lead + 1]:
+        raise ValueError(f"g must have the shape {tuple(v.shape[lead:lead + 1])}, a decay for each head, not {tuple(g.shape)}")
+    each = g.expand(v.shape[:-1]) if v.dim() == lead + 2 else g
+    _check(q, k, v, each, each, reset, state, lead)
+
+
+def _linear_inputs(q, k, v, g, reset, state, scale, learned) -> L.ZenoAmdLinearInputs:
+    qs, ks, vs = q.stride(), k.stride(), v.stride()
+    rs = (0, 0) if reset is None else reset.stride()
+    if len(qs) == 4:
+        b, t, hk, dk = q.shape
+        qs, ks, vs = qs[:3], ks[:3], vs[:3]
+    else:
+        (b, hk, dk), t = q.shape, 1
+        qs, ks, vs = (qs[0], 0, qs[1]), (ks[0], 0, ks[1]), (vs[0], 0, vs[1])
+        rs = (rs[0], 0)
+    _, hv, dv = v.shape[-3:]
+    return L.ZenoAmdLinearInputs(
+        _DTYPES[q.dtype], b, t, hk, hv, dk, dv, learned, scale, q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(),
+        None if reset is None else reset.data_ptr(), None if state is None else state.data_ptr(), qs, ks, vs, rs)
+
+
+class _LinearAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, g, reset, state, scale, train):
+        learned = train and g.requires_grad
+        with _on(q):
+            lib = L.load()
+            a = _linear_inputs(q, k, v, g, reset, state, scale, learned)
+            o = _dense_like(v)  # v's order of dimensions: time-major in, time-major out
+            last = torch.empty((q.shape[0], v.shape[2], q.shape[3], v.shape[3]), dtype=torch.float32, device=q.device)
+            saved = _space(lib.zeno_amd_linear_saved_bytes(a), q) if train else None
+            space = _space(lib.zeno_amd_linear_workspace_bytes(a, 0), q)
+            rc = lib.zeno_amd_linear_forward(a, o.data_ptr(), _S3(*o.stride()[:3]), last.data_ptr(), None if saved is None else saved.data_ptr(),
+                                             None if space is None else space.data_ptr(), _stream(q))
+            if rc:
+                _fail(rc, "linear_attention")
+        if train:
+            ctx.save_for_backward(q, k, v, g, reset, state, saved)
+            ctx.scale, ctx.learned = scale, learned
+            ctx.set_materialize_grads(False)
+        return o, last
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_o, d_last):
+        q, k, v, g, reset, state, saved = ctx.saved_tensors
+        if d_o is None and d_last is None:
+            return (None,) * 8
+        with _on(q):
+            lib = L.load()
+            a = _linear_inputs(q, k, v, g, reset, state, ctx.scale, ctx.learned)
+            d_o = torch.zeros_like(v) if d_o is None else _row(d_o)
+            d_last = None if d_last is None else d_last.contiguous()
+            d_q, d_k, d_v = (_dense_like(x) for x in (q, k, v))
+            d_g = torch.empty_like(g) if ctx.learned else None
+            d_state = torch.empty_like(state) if state is not None and ctx.needs_input_grad[5] else None
+            space = _space(lib.zeno_amd_linear_workspace_bytes(a, 1), q)
+            grads = L.ZenoAmdLinearGradients(
+                d_o.data_ptr(), _S3(*d_o.stride()[:3]), None if d_last is None else d_last.data_ptr(), d_q.data_ptr(), d_k.data_ptr(), d_v.data_ptr(),
+                None if d_g is None else d_g.data_ptr(), None if d_state is None else d_state.data_ptr(),
+                *(_S3(*x.stride()[:3]) for x in (d_q, d_k, d_v)))
+            rc = lib.zeno_amd_linear_backward(a, None if saved is None else saved.data_ptr(), grads, None if space is None else space.data_ptr(), _stream(q))
+            if rc:
+                _fail(rc, "linear_attention's gradients")
+        return d_q, d_k, d_v, d_g, None, d_state, None, None
+
+
+def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, reset: Optional[torch.Tensor] = None,
+                     state: Optional[torch.Tensor] = None, *, scale: Optional[float] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Linear attention over whole sequences. Returns o [B, T, Hv, value_dim] in the type of v and the
+    state after the last token, a new tensor. Differentiable in q, k, v, g and state."""
+    _check_linear(q, k, v, g, reset, state, 2)
+    scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
+    q, k, v, g = _row(q), _row(k), _row(v), g.contiguous()
+    state = None if state is None else state.contiguous()
+    train = torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in (q, k, v, g, state))
+    return _LinearAttention.apply(q, k, v, g, reset, state, scale, train)
+
+
+def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, state: torch.Tensor,
+                          reset: Optional[torch.Tensor] = None, *, scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """One token of linear attention for every sequence: q, k [B, Hk, key_dim], v [B, Hv, value_dim], g [Hv],
+    reset [B]. `state`, `out` and gradients are as gated_delta_step has them."""
+    _check_linear(q, k, v, g, reset, state, 1)
+    _check_step(v, state, out)
+    q, k, v, g = _row(q), _row(k), _row(v), g.contiguous()
+    if out is None:
+        out = torch.empty_like(v, memory_format=torch.contiguous_format)
+    with _on(q):
+        a = _linear_inputs(q, k, v, g, reset, state, q.shape[-1] ** -0.5 if scale is None else float(scale), False)
+        os = out.stride()
+        rc = L.load().zeno_amd_linear_step(a, out.data_ptr(), _S3(os[0], 0, os[1]), state.data_ptr(), _stream(q))
+        if rc:
+            _fail(rc, "linear_attention_step")
     _written(state)  # autograd refuses a backward pass that needs what was here
     _written(out)
     return out
