@@ -54,13 +54,13 @@ struct Walk {
     bool full;                   // dimensions as wide as the launch shape
 };
 
-// Launch shape: `steps` and `cols` times 32 rows and columns of the state a wave.
+// Launch shape: 32 `steps` rows and 32 columns of the state a wave, `blocks` waves a head.
 struct Shape {
-    int steps, cols;
-    bool full;
+    int steps;
     uint32_t blocks;
+    bool full;
 };
-Shape shape_of(uint32_t dtype, int da, int dc, bool slope);
+Shape shape_of(int da, int dc);
 struct Segments {
     uint32_t count;
     int length;

@@ -42,8 +42,7 @@ uint64_t states_floats(const ZenoAmdLinearInputs& in) { return even(between(in) 
 uint64_t share_floats(const ZenoAmdLinearInputs& in) {  // gradients of q (or k) by value head
     return in.key_heads == in.value_heads ? 0 : even((uint64_t)in.batch * in.length * in.value_heads * in.key_dim);
 }
-Shape slope_shape(const ZenoAmdLinearInputs& in) { return shape_of(in.dtype, in.value_dim, in.key_dim, true); }
-uint64_t parts_floats(const ZenoAmdLinearInputs& in) { return in.decay_gradient ? even(2 * heads_of(in) * segments_of(in).count * slope_shape(in).blocks) : 0; }
+uint64_t parts_floats(const ZenoAmdLinearInputs& in) { return in.decay_gradient ? even(2 * heads_of(in) * segments_of(in).count * shape_of(in.value_dim, in.key_dim).blocks) : 0; }
 
 void set_strides(int64_t* to, const int64_t* from) {
     for (int i = 0; i < 3; ++i) to[i] = from[i];
@@ -101,20 +100,18 @@ std::string check_outputs(const std::vector<Memory>& inputs, const std::vector<M
 
 }  // namespace
 
-// A wave holds 64 columns of the state in 16-bit types where that leaves room for the rows, else 32.
-Shape shape_of(uint32_t dtype, int da, int dc, bool slope) {
+Shape shape_of(int da, int dc) {
     Shape s;
     s.steps = da <= 32 ? 1 : da <= 64 ? 2 : 4;
-    s.cols = dtype != T_F32 && s.steps < 4 && dc > 32 && !slope ? 2 : 1;
-    s.blocks = (dc + 32 * s.cols - 1) / (32 * s.cols);
-    s.full = da == 32 * s.steps && dc == 32 * s.cols * (int)s.blocks;
+    s.blocks = (dc + 31) / 32;
+    s.full = da == 32 * s.steps && dc % 32 == 0;
     return s;
 }
 
 // With fewer walks than two waves a SIMD, as many segments as make up those, of at least four chunks.
 Segments segments_of(const ZenoAmdLinearInputs& in) {
     const int64_t chunks = ((int64_t)in.length + kChunk - 1) / kChunk;
-    const int64_t walks = (int64_t)heads_of(in) * shape_of(in.dtype, in.key_dim, in.value_dim, false).blocks;
+    const int64_t walks = (int64_t)heads_of(in) * shape_of(in.key_dim, in.value_dim).blocks;
     int64_t want = std::min(2048 / walks, chunks / 4);
     if (want < 2) want = 1;
     const int64_t each = (chunks + want - 1) / want;
@@ -209,12 +206,12 @@ hipError_t forward(const ZenoAmdLinearInputs& in, void* o, const int64_t* o_stri
     w.starts = saved ? saved : workspace + even(between(in));
     if (w.segments > 1) {
         const bool slope = saved && in.decay_gradient;
-        const Shape s = shape_of(in.dtype, w.da, w.dc, slope);
+        const Shape s = shape_of(w.da, w.dc);
         set_shape(w, s);
         if (slope) w.slopes = saved + states_floats(in);
         if (const hipError_t e = launch(in.dtype, w, s, slope ? STATES_SLOPE : STATES, false, stream)) return e;
     }
-    const Shape s = shape_of(in.dtype, w.da, w.dc, false);
+    const Shape s = shape_of(w.da, w.dc);
     set_shape(w, s);
     return launch(in.dtype, w, s, OUTPUTS, false, stream);
 }
@@ -249,7 +246,7 @@ hipError_t backward(const ZenoAmdLinearInputs& in, const float* saved, const Zen
     w.last = grad.d_state;
     w.starts = d_starts;
     w.passes = passes;
-    Shape s = shape_of(in.dtype, w.da, w.dc, false);
+    Shape s = shape_of(w.da, w.dc);
     set_shape(w, s);
     if (w.segments > 1 && (e = launch(in.dtype, w, s, STATES, true, stream))) return e;
     if ((e = launch(in.dtype, w, s, OUTPUTS, true, stream))) return e;
@@ -262,7 +259,7 @@ hipError_t backward(const ZenoAmdLinearInputs& in, const float* saved, const Zen
     key_out(w, grad.d_k, grad.d_k_stride, part_k);
     w.first = grad.d_last;
     w.starts = d_starts;
-    s = shape_of(in.dtype, w.da, w.dc, false);
+    s = shape_of(w.da, w.dc);
     set_shape(w, s);
     if ((e = launch(in.dtype, w, s, OUTPUTS, true, stream))) return e;
 
@@ -278,7 +275,7 @@ hipError_t backward(const ZenoAmdLinearInputs& in, const float* saved, const Zen
     w.slopes = w.starts + states_floats(in);
     w.d_last = grad.d_last;
     w.parts = reinterpret_cast<double*>(parts);
-    s = grad.d_g ? slope_shape(in) : shape_of(in.dtype, w.da, w.dc, false);
+    s = shape_of(w.da, w.dc);
     set_shape(w, s);
     if ((e = launch(in.dtype, w, s, grad.d_g ? OUTPUTS_SLOPE : OUTPUTS, false, stream))) return e;
     if (grad.d_g) linear_decay_kernel<<<in.value_heads, 256, 0, stream>>>(w.parts, in.batch, in.value_heads, w.segments * s.blocks, grad.d_g);

@@ -8,7 +8,7 @@
 // and a walk back the same with the tokens' order reversed. The decays of a head are one number, so
 // they are a table in registers that is made once.
 //
-// A wave owns 32 or 64 columns of the state, all of its rows, and works alone: no LDS, no barrier.
+// A wave owns 32 columns of the state, all of its rows, and works alone: no LDS, no barrier.
 // Rows are read as they lie, 16 bytes a lane: lane (n, g) has row n's dimensions 8 g to 8 g + 7 of
 // every 32. That is an operand of the matrix units as it is, for contractions along the dimensions.
 // The other operands come from results without an exchange: a result tile has its rows in registers and
@@ -63,7 +63,26 @@ template <> struct Along<1> {
     template <int P> static __device__ __forceinline__ Half<P> make(const f4* x) { return split<P>(x[0]); }
 };
 
-template <int TY, int STEPS, int COLS, int TILES, bool BACK, int KIND, bool FULL>
+// Four floats at any address, the first `n` of them in bounds.
+template <bool FULL> __device__ __forceinline__ f4 load_floats(const float* at, int n) {
+    if (FULL || n >= 4) return __builtin_bit_cast(f4, reinterpret_cast<const Loose<T_F32>::U*>(at)->v);
+    f4 x = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < 3; ++i)
+        if (i < n) x[i] = at[i];
+    return x;
+}
+template <bool FULL> __device__ __forceinline__ void store_floats(float* at, int n, f4 x) {
+    if (FULL || n >= 4) {
+        reinterpret_cast<Loose<T_F32>::U*>(at)->v = __builtin_bit_cast(u4, x);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+            if (i < n) at[i] = x[i];
+    }
+}
+
+template <int TY, int STEPS, int TILES, bool AHEAD, bool BACK, int KIND, bool FULL>
 __global__ __launch_bounds__(256, 2) void linear_walk_kernel(const Walk a) {
     typedef typename Elem<TY>::type E;
     constexpr int NP = Elem<TY>::parts, C = 16 * TILES;
@@ -77,7 +96,7 @@ __global__ __launch_bounds__(256, 2) void linear_walk_kernel(const Walk a) {
     const int64_t b = bh / a.heads, h = bh % a.heads;
     const uint32_t segment = !OUT && BACK ? walk + 1 : walk;
     const int begin = segment * a.segment_length, T = begin + min(a.length - begin, a.segment_length);
-    const int col0 = block * 32 * COLS;
+    const int col0 = block * 32;
     const int da = a.da, dc = a.dc - col0;
     auto row_of = [&](const Rows& x, int e) { return (const E*)x.at + b * x.stride[0] + (h / x.share) * x.stride[2] + e + 8 * g; };
     const E* ap = OUT ? row_of(a.a, 0) : nullptr;
@@ -85,6 +104,83 @@ __global__ __launch_bounds__(256, 2) void linear_walk_kernel(const Walk a) {
     const E* cp = row_of(a.c, col0);
     const E* qp = GRAD ? row_of(a.q, col0) : nullptr;
     const uint8_t* rp = a.reset ? a.reset + b * a.reset_stride[0] : nullptr;
+
+    // ---- what a chunk reads
+    Eight<TY> ar[OUT ? TILES : 1][STEPS], br[TILES][STEPS], cr[TILES], qr[GRAD ? TILES : 1];
+    bool cut = false, any_cut = false;
+    auto fetch = [&](int t, int rows) {
+        cut = rp && lane < rows && rp[(t + lane) * a.reset_stride[1]];
+#pragma unroll
+        for (int i = 0; i < TILES; ++i) {
+            const int64_t tok = t + min(16 * i + n, rows - 1);
+            const E* x = bp + tok * a.b.stride[1];
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s) br[i][s].template load<FULL>(x + 32 * s, da - 32 * s - 8 * g);
+            if constexpr (OUT) {
+                x = ap + tok * a.a.stride[1];
+#pragma unroll
+                for (int s = 0; s < STEPS; ++s) ar[i][s].template load<FULL>(x + 32 * s, da - 32 * s - 8 * g);
+            }
+            cr[i].template load<FULL>(cp + tok * a.c.stride[1], dc - 8 * g);
+            if constexpr (GRAD) qr[i].template load<FULL>(qp + tok * a.q.stride[1], dc - 8 * g);
+        }
+    };
+    auto bounds = [&](int at, int& t, int& rows) {  // the chunk of the grid that `at` is in, from it (or up to it) on
+        if (BACK) {
+            t = begin + (at - 1 - begin) / C * C;
+            rows = at - t;
+        } else {
+            t = at;
+            rows = min(T, begin + ((at - begin) / C + 1) * C) - t;
+        }
+    };
+    int at = BACK ? T : begin, t, rows;
+    bounds(at, t, rows);
+    fetch(t, rows);
+
+    // ---- the state, by row tiles of 16 (pairs of them make 32 rows) and two column tiles
+    f4 S[2 * STEPS][2], N[SLOPE ? 2 * STEPS : 1][2];
+    // A lane takes four values that lie side by side: of one of four rows, which four lanes then exchange, or
+    // of a column, where columns lie side by side.
+    auto place = [&](int i, int j, int& left) {
+        const int row = 32 * (i >> 1) + 8 * g + 4 * (i & 1), col = 8 * (n >> 2) + 4 * j;
+        if (a.row == 1) {
+            left = FULL ? 4 : col + (n & 3) < dc ? da - row : 0;
+            return row + (int64_t)(col0 + col + (n & 3)) * a.col;
+        }
+        left = FULL ? 4 : row + (n & 3) < da ? dc - col : 0;
+        return (int64_t)(row + (n & 3)) * a.row + col0 + col;
+    };
+    auto load_state = [&](auto& X, const float* from) {
+#pragma unroll
+        for (int i = 0; i < 2 * STEPS; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                int left;
+                const int64_t at = place(i, j, left);
+                X[i][j] = f4{0, 0, 0, 0};
+                if (from) X[i][j] = load_floats<FULL>(from + at, left);
+            }
+        if (from && a.row != 1)
+#pragma unroll
+            for (int i = 0; i < 2 * STEPS; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) X[i][j] = turn(X[i][j], lane);
+    };
+    auto store_state = [&](const auto& X, float* to) {
+#pragma unroll
+        for (int i = 0; i < 2 * STEPS; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                int left;
+                const int64_t at = place(i, j, left);
+                store_floats<FULL>(to + at, left, a.row == 1 ? X[i][j] : turn(X[i][j], lane));
+            }
+    };
+    const bool at_first = BACK ? segment == a.segments - 1 : segment == 0;
+    const int64_t between = (int64_t)bh * (a.segments - 1) + (BACK ? segment : segment - 1);  // the start of this walk
+    load_state(S, at_first ? (a.first ? a.first + bh * a.size : nullptr) : OUT ? a.starts + between * a.size : nullptr);
+    if constexpr (SLOPE) load_state(N, OUT && !at_first ? a.slopes + between * a.size : nullptr);
 
     // ---- the head's decays. `read`: of the state to a token, `write`: of a token to the next state.
     float gh = a.g[h];
@@ -118,52 +214,7 @@ __global__ __launch_bounds__(256, 2) void linear_walk_kernel(const Walk a) {
         }
     };
 
-    // ---- the state, [pair of row tiles][tile][pair of column tiles][tile]
-    f4 S[STEPS][2][COLS][2], N[SLOPE ? STEPS : 1][2][COLS][2];
-    auto place = [&](int s, int i, int c, int j, int r, bool& inside) {
-        const int row = 32 * s + 8 * g + 4 * i + r, col = 32 * c + 8 * (n >> 2) + 4 * j + (n & 3);
-        inside = FULL || (row < da && col < dc);
-        return (int64_t)row * a.row + (int64_t)(col0 + col) * a.col;
-    };
-    auto load_state = [&](auto& X, const float* from) {
-#pragma unroll
-        for (int s = 0; s < STEPS; ++s)
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int c = 0; c < COLS; ++c)
-#pragma unroll
-                    for (int j = 0; j < 2; ++j)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            bool inside;
-                            const int64_t at = place(s, i, c, j, r, inside);
-                            X[s][i][c][j][r] = from && inside ? from[at] : 0.0f;
-                        }
-    };
-    auto store_state = [&](const auto& X, float* to) {
-#pragma unroll
-        for (int s = 0; s < STEPS; ++s)
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int c = 0; c < COLS; ++c)
-#pragma unroll
-                    for (int j = 0; j < 2; ++j)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            bool inside;
-                            const int64_t at = place(s, i, c, j, r, inside);
-                            if (inside) to[at] = X[s][i][c][j][r];
-                        }
-    };
-    const bool at_first = BACK ? segment == a.segments - 1 : segment == 0;
-    const int64_t between = (int64_t)bh * (a.segments - 1) + (BACK ? segment : segment - 1);  // the start of this walk
-    const float* from = at_first ? (a.first ? a.first + bh * a.size : nullptr) : OUT ? a.starts + between * a.size : nullptr;
-    load_state(S, from);
-    if (SLOPE) load_state(N, OUT && !at_first ? a.slopes + between * a.size : nullptr);
-
-    // ---- unit matrices as operands: eight of them pick dimension 8 (n / 4) + 4 i + n % 4 of a row's 32
+    // ---- unit matrices as operands: they pick dimension 8 (n / 4) + 4 i + n % 4 of a row's 32
     Frag<1> unit_of[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -172,45 +223,18 @@ __global__ __launch_bounds__(256, 2) void linear_walk_kernel(const Walk a) {
             const int e = 4 * i + (n & 3);
             unit_of[i].p[0][w] = g == (n >> 2) && (e >> 1) == w ? 0x3f80u << (16 * (e & 1)) : 0u;
         }
-
-    // ---- what a chunk reads
-    Eight<TY> ar[OUT ? TILES : 1][STEPS], br[TILES][STEPS], cr[TILES][COLS], qr[GRAD ? TILES : 1][COLS];
-    bool cut = false, any_cut = false;
-    auto fetch = [&](int t, int rows) {
-        cut = rp && lane < rows && rp[(t + lane) * a.reset_stride[1]];
-#pragma unroll
-        for (int i = 0; i < TILES; ++i) {
-            const int64_t tok = t + min(16 * i + n, rows - 1);
-            const E* x = bp + tok * a.b.stride[1];
-#pragma unroll
-            for (int s = 0; s < STEPS; ++s) br[i][s].template load<FULL>(x + 32 * s, da - 32 * s - 8 * g);
-            x = cp + tok * a.c.stride[1];
-#pragma unroll
-            for (int c = 0; c < COLS; ++c) cr[i][c].template load<FULL>(x + 32 * c, dc - 32 * c - 8 * g);
-            if constexpr (OUT) {
-                x = ap + tok * a.a.stride[1];
-#pragma unroll
-                for (int s = 0; s < STEPS; ++s) ar[i][s].template load<FULL>(x + 32 * s, da - 32 * s - 8 * g);
-            }
-            if constexpr (GRAD) {
-                x = qp + tok * a.q.stride[1];
-#pragma unroll
-                for (int c = 0; c < COLS; ++c) qr[i][c].template load<FULL>(x + 32 * c, dc - 32 * c - 8 * g);
-            }
-        }
-    };
     double dg = 0.0;
 
-    // The chunk of tokens t to t + len, in USED tiles. CUTS: resets inside, in `cuts`. ODD: one token, with
-    // values that are not finite: its operands along the tokens are read one by one. No branch is inside: where
-    // one lies between a matrix instruction and the use of its result, the compiler has been seen to leave out
-    // the wait.
+    // The chunk of tokens t to t + len, in USED tiles. CUTS: there may be resets inside, in `cuts`. ODD: one token,
+    // with values that are not finite: its operands along the tokens are read one by one. No branch is inside: where
+    // one lies between a matrix instruction and the use of its result, the compiler has been seen to leave out the
+    // wait. The scheduler is kept from starting everything at once, which takes more registers than there are.
     auto chunk = [&](auto used, auto with_cuts, auto is_odd, int t, int len, uint32_t cuts, auto&& next) {
         constexpr int USED = decltype(used)::value;
         constexpr bool CUTS = decltype(with_cuts)::value, ODD = decltype(is_odd)::value;
         const f4 zero = {0, 0, 0, 0};
-        Frag<NP> af[OUT ? USED : 1][STEPS], bf[USED][STEPS], cf[USED][COLS];
-        Eight<TY> qe[GRAD ? USED : 1][COLS];
+        Frag<NP> af[OUT ? USED : 1][STEPS], bf[USED][STEPS], cf[USED];
+        Eight<TY> qe[GRAD ? USED : 1];
 #pragma unroll
         for (int i = 0; i < USED; ++i) {
 #pragma unroll
@@ -218,32 +242,27 @@ __global__ __launch_bounds__(256, 2) void linear_walk_kernel(const Walk a) {
                 bf[i][s] = operand(br[i][s]);
                 if constexpr (OUT) af[i][s] = operand(ar[i][s]);
             }
-#pragma unroll
-            for (int c = 0; c < COLS; ++c) {
-                cf[i][c] = operand(cr[i][c]);
-                if constexpr (GRAD) qe[i][c] = qr[i][c];
-            }
+            cf[i] = operand(cr[i]);
+            if constexpr (GRAD) qe[i] = qr[i];
         }
-        f4 odd_b[ODD ? STEPS : 1][2], odd_c[ODD ? COLS : 1][2];
+        f4 odd_b[ODD ? 2 * STEPS : 1], odd_c[2];
         if constexpr (ODD) {
             const int e = 8 * (n >> 2) + (n & 3) - 8 * g;  // from this lane's place in its rows to the dimension that it stands for
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-#pragma unroll
-                for (int s = 0; s < STEPS; ++s)
-                    odd_b[s][i] = f4{g == 0 && 32 * s + 8 * g + e + 4 * i < da ? Elem<TY>::get(bp[t * a.b.stride[1] + 32 * s + e + 4 * i]) : 0.0f, 0, 0, 0};
-#pragma unroll
-                for (int c = 0; c < COLS; ++c)
-                    odd_c[c][i] = f4{g == 0 && 32 * c + 8 * g + e + 4 * i < dc ? Elem<TY>::get(cp[t * a.c.stride[1] + 32 * c + e + 4 * i]) : 0.0f, 0, 0, 0};
+            for (int i = 0; i < 2 * STEPS; ++i) {
+                const int x = 32 * (i >> 1) + 4 * (i & 1);
+                odd_b[i] = f4{g == 0 && x + e < da ? Elem<TY>::get(bp[t * a.b.stride[1] + x + e]) : 0.0f, 0, 0, 0};
             }
+#pragma unroll
+            for (int j = 0; j < 2; ++j) odd_c[j] = f4{g == 0 && 4 * j + e < dc ? Elem<TY>::get(cp[t * a.c.stride[1] + 4 * j + e]) : 0.0f, 0, 0, 0};
         }
-        next();
+        if (AHEAD) next();
 
         // Resets: the last one up to a token (this lane's, and those of its registers), and of the chunk.
         int mine[USED], theirs[USED][4], last_cut = -1, first_cut = 64;
         if constexpr (CUTS) {
-            last_cut = 31 - __builtin_clz(cuts);
-            first_cut = __builtin_ctz(cuts);
+            last_cut = cuts ? 31 - __builtin_clz(cuts) : -1;
+            first_cut = cuts ? __builtin_ctz(cuts) : 64;
 #pragma unroll
             for (int i = 0; i < USED; ++i) {
                 mine[i] = 31 - __clz((int)(cuts & (0xffffffffu >> (31 - 16 * i - n))));
@@ -252,10 +271,12 @@ __global__ __launch_bounds__(256, 2) void linear_walk_kernel(const Walk a) {
             }
         }
 
-        // ---- P transposed: row j = 16 tj + 4 g + r, column i = 16 ti + n
-        f4 pt[USED][USED];
+        // ---- P transposed (row j = 16 tj + 4 g + r, column i = 16 ti + n), as operands along j
+        Half<3> alone;  // of the tokens that see one tile
+        Frag<3> both;   // of those that see two
         float pairs = 0.0f;
         if constexpr (OUT) {
+            f4 pt[USED][USED];
 #pragma unroll
             for (int tj = 0; tj < USED; ++tj)
 #pragma unroll
@@ -264,9 +285,7 @@ __global__ __launch_bounds__(256, 2) void linear_walk_kernel(const Walk a) {
                     f4 x = zero, y = zero;
 #pragma unroll
                     for (int s = 0; s < STEPS; ++s) x = mul<2>(bf[tj][s], af[ti][s], x);
-                    if constexpr (GRAD)
-#pragma unroll
-                        for (int c = 0; c < COLS; ++c) y = mul<2>(cf[tj][c], operand(qe[ti][c]), y);
+                    if constexpr (GRAD) y = mul<2>(cf[tj], operand(qe[ti]), y);
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         const int i = 16 * ti + n, j = 16 * tj + 4 * g + r;
@@ -278,135 +297,113 @@ __global__ __launch_bounds__(256, 2) void linear_walk_kernel(const Walk a) {
                     }
                     pt[tj][ti] = x;
                 }
+            constexpr int one = BACK ? USED - 1 : 0;
+            alone = split<3>(pt[one][one]);
+            if constexpr (USED == 2) both = split<3>(pt[0][1 - one], pt[1][1 - one]);
         }
-        typename Along<USED>::template Op<NP> bt[STEPS][2];
+        typename Along<USED>::template Op<NP> bt[2 * STEPS];
 #pragma unroll
-        for (int s = 0; s < STEPS; ++s)
+        for (int i = 0; i < 2 * STEPS; ++i) {
+            f4 x[USED];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                f4 x[USED];
+            for (int k = 0; k < USED; ++k) x[k] = ODD ? odd_b[ODD ? i : 0] : mul<2>(bf[k][i >> 1], unit_of[i & 1], zero);
+            bt[i] = Along<USED>::template make<NP>(x);
+        }
+        f4 out[USED][2];
 #pragma unroll
-                for (int k = 0; k < USED; ++k) x[k] = ODD ? odd_b[ODD ? s : 0][i] : mul<2>(bf[k][s], unit_of[i], zero);
-                bt[s][i] = Along<USED>::template make<NP>(x);
-            }
+        for (int j = 0; j < 2; ++j) {
+            __builtin_amdgcn_sched_barrier(0);
+            f4 ct[USED], wc[USED];
 #pragma unroll
-        for (int c = 0; c < COLS; ++c) {
-            f4 out[USED][2];
+            for (int k = 0; k < USED; ++k) ct[k] = ODD ? odd_c[j] : mul<2>(cf[k], unit_of[j], zero);
+            if constexpr (OUT) {
+                f4 slope[USED];
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                f4 ct[USED], wc[USED];
+                for (int k = 0; k < USED; ++k) out[k][j] = slope[k] = zero;
 #pragma unroll
-                for (int k = 0; k < USED; ++k) ct[k] = ODD ? odd_c[ODD ? c : 0][j] : mul<2>(cf[k][c], unit_of[j], zero);
-                if constexpr (OUT) {
-                    f4 slope[USED];
+                for (int s = 0; s < STEPS; ++s) {
+                    const Frag<3> sf = split<3>(S[2 * s][j], S[2 * s + 1][j]);
 #pragma unroll
-                    for (int k = 0; k < USED; ++k) out[k][j] = slope[k] = zero;
+                    for (int k = 0; k < USED; ++k) out[k][j] = mul<2>(sf, af[k][s], out[k][j]);
+                    if constexpr (GRAD) {
+                        const Frag<3> nf = split<3>(N[2 * s][j], N[2 * s + 1][j]);
 #pragma unroll
-                    for (int s = 0; s < STEPS; ++s) {
-                        const Frag<3> sf = split<3>(S[s][0][c][j], S[s][1][c][j]);
-#pragma unroll
-                        for (int k = 0; k < USED; ++k) out[k][j] = mul<2>(sf, af[k][s], out[k][j]);
-                        if constexpr (GRAD) {
-                            const Frag<3> nf = split<3>(N[s][0][c][j], N[s][1][c][j]);
-#pragma unroll
-                            for (int k = 0; k < USED; ++k) slope[k] = mul<2>(nf, af[k][s], slope[k]);
-                        }
-                    }
-#pragma unroll
-                    for (int k = 0; k < USED; ++k) {
-                        const bool reach = !CUTS || (BACK ? 16 * k + n >= last_cut : mine[k] < 0);
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) out[k][j][r] = reach ? out[k][j][r] * read[k] : 0.0f;
-                        if constexpr (GRAD) {
-                            float q[8];
-                            qe[k][c].get(q);
-#pragma unroll
-                            for (int r = 0; r < 4; ++r) {
-                                const float x = (float)(16 * k + n + 1) * out[k][j][r] + (reach ? slope[k][r] * read[k] : 0.0f);
-                                pairs += x * q[4 * j + r];
-                            }
-                        }
-                    }
-                    Half<3> ph[USED][USED];
-                    const auto cop = [&](int k) { return split<NP>(ct[k]); };
-                    if constexpr (USED == 1) {
-                        out[0][j] = mul<2>(cop(0), split<3>(pt[0][0]), out[0][j]);
-                    } else {
-                        constexpr int alone = BACK ? 1 : 0;
-                        (void)ph;
-                        out[alone][j] = mul<2>(cop(alone), split<3>(pt[alone][alone]), out[alone][j]);
-                        out[1 - alone][j] = mul<2>(split<NP>(ct[0], ct[1]), split<3>(pt[0][1 - alone], pt[1][1 - alone]), out[1 - alone][j]);
+                        for (int k = 0; k < USED; ++k) slope[k] = mul<2>(nf, af[k][s], slope[k]);
                     }
                 }
-                // ---- the state behind the chunk
+#pragma unroll
+                for (int k = 0; k < USED; ++k) {
+                    const bool reach = !CUTS || (BACK ? 16 * k + n >= last_cut : mine[k] < 0);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) out[k][j][r] = reach ? out[k][j][r] * read[k] : 0.0f;
+                    if constexpr (GRAD) {
+                        float q[8];
+                        qe[k].get(q);
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const float x = (float)(16 * k + n + 1) * out[k][j][r] + (reach ? slope[k][r] * read[k] : 0.0f);
+                            pairs += x * q[4 * j + r];
+                        }
+                    }
+                }
+                constexpr int one = BACK ? USED - 1 : 0;
+                out[one][j] = mul<2>(split<NP>(ct[one]), alone, out[one][j]);
+                if constexpr (USED == 2) out[1 - one][j] = mul<2>(split<NP>(ct[0], ct[1]), both, out[1 - one][j]);
+            }
+            // ---- the state behind the chunk
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int k = 0; k < USED; ++k)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int at = 16 * k + 4 * g + r;
+                    wc[k][r] = !CUTS || (BACK ? at < first_cut : at >= last_cut) ? ct[k][r] * write[k][r] : 0.0f;
+                }
+            const auto wf = Along<USED>::template make<3>(wc);
+            if constexpr (SLOPE) {
 #pragma unroll
                 for (int k = 0; k < USED; ++k)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const int at = 16 * k + 4 * g + r;
-                        wc[k][r] = !CUTS || (BACK ? at < first_cut : at >= last_cut) ? ct[k][r] * write[k][r] : 0.0f;
-                    }
-                const auto wf = Along<USED>::template make<3>(wc);
-                if constexpr (SLOPE) {
+                    for (int r = 0; r < 4; ++r) wc[k][r] *= (float)max(len - 1 - 16 * k - 4 * g - r, 0);
+                const auto nf = Along<USED>::template make<3>(wc);
 #pragma unroll
-                    for (int k = 0; k < USED; ++k)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) wc[k][r] *= (float)max(len - 1 - 16 * k - 4 * g - r, 0);
-                    const auto nf = Along<USED>::template make<3>(wc);
-#pragma unroll
-                    for (int s = 0; s < STEPS; ++s)
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            f4 x = (N[s][i][c][j] + S[s][i][c][j] * (float)len) * all;
-                            if (CUTS) x = zero;
-                            N[s][i][c][j] = mul<2>(bt[s][i], nf, x);
-                        }
+                for (int i = 0; i < 2 * STEPS; ++i) {
+                    f4 x = (N[i][j] + S[i][j] * (float)len) * all;
+                    if (CUTS) x = cuts ? zero : x;
+                    N[i][j] = mul<2>(bt[i], nf, x);
                 }
-#pragma unroll
-                for (int s = 0; s < STEPS; ++s)
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        f4 x = S[s][i][c][j] * all;
-                        if (CUTS) x = zero;
-                        S[s][i][c][j] = mul<2>(bt[s][i], wf, x);
-                    }
             }
-            if constexpr (OUT) {
 #pragma unroll
-                for (int k = 0; k < USED; ++k) {
-                    const int row = 16 * k + n, e = 32 * c + 8 * g;
-                    const float y[8] = {out[k][0][0], out[k][0][1], out[k][0][2], out[k][0][3], out[k][1][0], out[k][1][1], out[k][1][2], out[k][1][3]};
-                    const int64_t to = b * a.out_stride[0] + (t + row) * a.out_stride[1] + (h / a.out_share) * a.out_stride[2] + col0 + e;
-                    if (row < len) {
-                        if (a.out_f32) {
-                            Eight<T_F32> x;
-                            x.set(y);
-                            x.template store<FULL>((float*)a.out + to, dc - e);
-                        } else {
-                            Eight<TY> x;
-                            x.set(y);
-                            x.template store<FULL>((E*)a.out + to, dc - e);
-                        }
+            for (int i = 0; i < 2 * STEPS; ++i) {
+                f4 x = S[i][j] * all;
+                if (CUTS) x = cuts ? zero : x;
+                S[i][j] = mul<2>(bt[i], wf, x);
+            }
+        }
+        if constexpr (OUT) {
+#pragma unroll
+            for (int k = 0; k < USED; ++k) {
+                const int row = 16 * k + n, e = 8 * g;
+                const float y[8] = {out[k][0][0], out[k][0][1], out[k][0][2], out[k][0][3], out[k][1][0], out[k][1][1], out[k][1][2], out[k][1][3]};
+                const int64_t to = b * a.out_stride[0] + (t + row) * a.out_stride[1] + (h / a.out_share) * a.out_stride[2] + col0 + e;
+                if (row < len) {
+                    if (a.out_f32) {
+                        Eight<T_F32> x;
+                        x.set(y);
+                        x.template store<FULL>((float*)a.out + to, dc - e);
+                    } else {
+                        Eight<TY> x;
+                        x.set(y);
+                        x.template store<FULL>((E*)a.out + to, dc - e);
                     }
                 }
             }
         }
         if (GRAD) dg += (double)pairs;
+        if (!AHEAD) next();
     };
 
     // ---- the walk
-    auto bounds = [&](int at, int& t, int& rows) {  // the chunk of the grid that `at` is in, from it (or up to it) on
-        if (BACK) {
-            t = begin + (at - 1 - begin) / C * C;
-            rows = at - t;
-        } else {
-            t = at;
-            rows = min(T, begin + ((at - begin) / C + 1) * C) - t;
-        }
-    };
-    int at = BACK ? T : begin, t, rows;
-    bounds(at, t, rows);
-    fetch(t, rows);
     while (BACK ? at > begin : at < T) {
         int len = rows, first = t;
         bool fine = true;
@@ -417,11 +414,8 @@ __global__ __launch_bounds__(256, 2) void linear_walk_kernel(const Walk a) {
                 fine &= br[i][s].finite();
                 if (OUT) fine &= ar[OUT ? i : 0][s].finite();
             }
-#pragma unroll
-            for (int c = 0; c < COLS; ++c) {
-                fine &= cr[i][c].finite();
-                if (GRAD) fine &= qr[GRAD ? i : 0][c].finite();
-            }
+            fine &= cr[i].finite();
+            if (GRAD) fine &= qr[GRAD ? i : 0].finite();
         }
         uint32_t cuts = (uint32_t)__ballot(cut);
         const bool odd = __ballot(!fine) != 0;
@@ -444,11 +438,8 @@ __global__ __launch_bounds__(256, 2) void linear_walk_kernel(const Walk a) {
                     br[i][s].keep(keep);
                     if (OUT) ar[OUT ? i : 0][s].keep(keep);
                 }
-#pragma unroll
-                for (int c = 0; c < COLS; ++c) {
-                    cr[i][c].keep(keep);
-                    if (GRAD) qr[GRAD ? i : 0][c].keep(keep);
-                }
+                cr[i].keep(keep);
+                if (GRAD) qr[GRAD ? i : 0].keep(keep);
             }
         }
         if (len != measured) measure(len);
@@ -466,8 +457,7 @@ __global__ __launch_bounds__(256, 2) void linear_walk_kernel(const Walk a) {
         constexpr std::true_type yes{};
         constexpr std::false_type no{};
         if (odd) {
-            if (cuts) chunk(one, yes, yes, now, len, cuts, next);
-            else chunk(one, no, yes, now, len, cuts, next);
+            chunk(one, yes, yes, now, len, cuts, next);
         } else if (TILES == 2 && len <= 16) {
             if (cuts) chunk(one, yes, no, now, len, cuts, next);
             else chunk(one, no, no, now, len, cuts, next);
@@ -485,18 +475,11 @@ __global__ __launch_bounds__(256, 2) void linear_walk_kernel(const Walk a) {
                 if (a.d_last) {
                     load_state(S, a.d_last + bh * a.size);
 #pragma unroll
-                    for (int s = 0; s < STEPS; ++s)
+                    for (int i = 0; i < 2 * STEPS; ++i)
 #pragma unroll
-                        for (int i = 0; i < 2; ++i)
+                        for (int j = 0; j < 2; ++j)
 #pragma unroll
-                            for (int c = 0; c < COLS; ++c)
-#pragma unroll
-                                for (int j = 0; j < 2; ++j)
-#pragma unroll
-                                    for (int r = 0; r < 4; ++r) {
-                                        const float x = S[s][i][c][j][r];
-                                        dg += x == 0.0f ? 0.0 : (double)(x * N[s][i][c][j][r]);
-                                    }
+                            for (int r = 0; r < 4; ++r) dg += S[i][j][r] == 0.0f ? 0.0 : (double)(S[i][j][r] * N[i][j][r]);
                 }
             }
         }
@@ -508,7 +491,7 @@ __global__ __launch_bounds__(256, 2) void linear_walk_kernel(const Walk a) {
     } else {
         const int64_t to = (int64_t)bh * (a.segments - 1) + walk;
         store_state(S, a.starts + to * a.size);
-        if (SLOPE) store_state(N, a.slopes + to * a.size);
+        if constexpr (SLOPE) store_state(N, a.slopes + to * a.size);
         if (block == 0 && lane == 0) a.passes[to] = any_cut ? 0.0f : 1.0f;
     }
 }
@@ -637,21 +620,28 @@ __global__ __launch_bounds__(256) void linear_step_kernel(const ZenoAmdLinearInp
 }
 
 // ---- launches ------------------------------------------------------------------------------
-template <int TY, int STEPS, int COLS, bool FULL> void walk_shape(const Walk& w, Kind kind, bool back, hipStream_t stream) {
-    constexpr int TILES = TY == T_F32 && STEPS == 4 ? 1 : 2;
+#ifndef TILES_OF
+#define TILES_OF(TY, STEPS) ((TY) == T_F32 ? 1 : 2)
+#endif
+#ifndef AHEAD_OF
+#define AHEAD_OF(TY, STEPS, KIND) ((STEPS) < 4 && (KIND) != OUTPUTS_SLOPE)
+#endif
+template <int TY, int STEPS, bool FULL> void walk_shape(const Walk& w, Kind kind, bool back, hipStream_t stream) {
+    constexpr int TILES = TILES_OF(TY, STEPS);
     const bool out = kind == OUTPUTS || kind == OUTPUTS_SLOPE;
     const uint32_t units = w.batch * w.heads * w.blocks * (out ? w.segments : w.segments - 1);
     const dim3 grid((units + 3) / 4);
     if (back) {
-        if (out) linear_walk_kernel<TY, STEPS, COLS, TILES, true, OUTPUTS, FULL><<<grid, 256, 0, stream>>>(w);
-        else linear_walk_kernel<TY, STEPS, COLS, TILES, true, STATES, FULL><<<grid, 256, 0, stream>>>(w);
+        if (out) linear_walk_kernel<TY, STEPS, TILES, AHEAD_OF(TY, STEPS, OUTPUTS), true, OUTPUTS, FULL><<<grid, 256, 0, stream>>>(w);
+        else linear_walk_kernel<TY, STEPS, TILES, AHEAD_OF(TY, STEPS, STATES), true, STATES, FULL><<<grid, 256, 0, stream>>>(w);
     } else if (kind == OUTPUTS) {
-        linear_walk_kernel<TY, STEPS, COLS, TILES, false, OUTPUTS, FULL><<<grid, 256, 0, stream>>>(w);
+        linear_walk_kernel<TY, STEPS, TILES, AHEAD_OF(TY, STEPS, OUTPUTS), false, OUTPUTS, FULL><<<grid, 256, 0, stream>>>(w);
     } else if (kind == STATES) {
-        linear_walk_kernel<TY, STEPS, COLS, TILES, false, STATES, FULL><<<grid, 256, 0, stream>>>(w);
-    } else if constexpr (COLS == 1) {
-        if (out) linear_walk_kernel<TY, STEPS, COLS, TILES, false, OUTPUTS_SLOPE, FULL><<<grid, 256, 0, stream>>>(w);
-        else linear_walk_kernel<TY, STEPS, COLS, TILES, false, STATES_SLOPE, FULL><<<grid, 256, 0, stream>>>(w);
+        linear_walk_kernel<TY, STEPS, TILES, AHEAD_OF(TY, STEPS, STATES), false, STATES, FULL><<<grid, 256, 0, stream>>>(w);
+    } else if (out) {
+        linear_walk_kernel<TY, STEPS, TILES, AHEAD_OF(TY, STEPS, OUTPUTS_SLOPE), false, OUTPUTS_SLOPE, FULL><<<grid, 256, 0, stream>>>(w);
+    } else {
+        linear_walk_kernel<TY, STEPS, TILES, AHEAD_OF(TY, STEPS, STATES_SLOPE), false, STATES_SLOPE, FULL><<<grid, 256, 0, stream>>>(w);
     }
     if (!out && w.segments > 2) {
         const dim3 join(w.batch * w.heads * (uint32_t)((w.size + 255) / 256));
@@ -662,21 +652,9 @@ template <int TY, int STEPS, int COLS, bool FULL> void walk_shape(const Walk& w,
 }
 
 template <int TY> hipError_t launch_walk(const Walk& w, const Shape& s, Kind kind, bool back, hipStream_t stream) {
-    auto by_width = [&](auto steps, auto cols) {
-        constexpr int STEPS = decltype(steps)::value, COLS = decltype(cols)::value;
-        s.full ? walk_shape<TY, STEPS, COLS, true>(w, kind, back, stream) : walk_shape<TY, STEPS, COLS, false>(w, kind, back, stream);
-    };
-    constexpr std::integral_constant<int, 1> one{};
-    constexpr std::integral_constant<int, 2> two{};
-    constexpr std::integral_constant<int, 4> four{};
-    if (s.steps == 4) {
-        by_width(four, one);
-    } else if constexpr (TY != T_F32) {
-        if (s.cols == 2) s.steps == 1 ? by_width(one, two) : by_width(two, two);
-        else s.steps == 1 ? by_width(one, one) : by_width(two, one);
-    } else {
-        s.steps == 1 ? by_width(one, one) : by_width(two, one);
-    }
+    if (s.steps == 1) s.full ? walk_shape<TY, 1, true>(w, kind, back, stream) : walk_shape<TY, 1, false>(w, kind, back, stream);
+    else if (s.steps == 2) s.full ? walk_shape<TY, 2, true>(w, kind, back, stream) : walk_shape<TY, 2, false>(w, kind, back, stream);
+    else s.full ? walk_shape<TY, 4, true>(w, kind, back, stream) : walk_shape<TY, 4, false>(w, kind, back, stream);
     return hipGetLastError();
 }
 
