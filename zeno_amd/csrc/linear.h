@@ -11,7 +11,7 @@
 namespace za {
 namespace linear {
 
-constexpr int kChunk = 32;  // tokens of the grid that segments are cut on
+constexpr int kChunk = 16;  // tokens
 
 // Rows of one of the inputs. Strides are in elements: sequence, token, head.
 struct Rows {
@@ -40,7 +40,8 @@ struct Walk {
     bool out_f32;                // part sums per value head, where heads share one
     const float* first;          // the state that the walk begins with; null: zeros
     float* last;                 // the state that it ends with; null: not wanted
-    int row, col;                // strides of a state's rows and columns in memory
+    int ld;                      // a state in memory: rows of this many values, its rows or (turned) its columns
+    bool turned;
     int64_t size;                // of a state
     // A long sequence is cut into segments that are walked side by side. Between them: states (and
     // slopes, see the kernels) [batch, heads, segments - 1, size], and whether a state passes the
@@ -49,18 +50,13 @@ struct Walk {
     int segment_length;          // tokens, whole chunks
     float *starts, *slopes, *passes;
     const float* d_last;         // for the gradient of g; null: zeros
-    double* parts;               // of it: [walks]
-    uint32_t blocks;             // waves that share the columns
-    bool full;                   // dimensions as wide as the launch shape
+    double* parts;               // of it: [batch, heads, segments, blocks, 2]
+    uint32_t blocks;             // of 32 columns
 };
 
-// Launch shape: 32 `steps` rows and 32 columns of the state a wave, `blocks` waves a head.
-struct Shape {
-    int steps;
-    uint32_t blocks;
-    bool full;
-};
-Shape shape_of(int da, int dc);
+// Launch shape: a wave holds 32 times 1, 2 or 4 rows of a state; full: of exactly so many, and of whole blocks.
+inline int steps_of(int da) { return da <= 32 ? 1 : da <= 64 ? 2 : 4; }
+inline bool full_of(const Walk& w) { return w.da == 32 * steps_of(w.da) && w.dc % 32 == 0; }
 struct Segments {
     uint32_t count;
     int length;
@@ -69,10 +65,13 @@ Segments segments_of(const ZenoAmdLinearInputs& in);
 uint64_t saved_floats(const ZenoAmdLinearInputs& in);
 uint64_t workspace_floats(const ZenoAmdLinearInputs& in, bool train);
 
-enum Kind { OUTPUTS, OUTPUTS_SLOPE, STATES, STATES_SLOPE };  // SLOPE: with what the gradient of g needs
+// What a walk is for: its outputs, the gradient of g, the states between segments, or those with their slopes,
+// which the gradient of g needs.
+enum Kind { OUTPUTS, SLOPES, STATES, STATES_SLOPE };
 
 // One translation unit per element type.
-template <int TY> hipError_t launch_walk(const Walk& w, const Shape& s, Kind kind, bool back, hipStream_t stream);
+template <int TY> hipError_t launch_walk(const Walk& w, Kind kind, bool back, hipStream_t stream);
+template <int TY> hipError_t launch_gradients(const Walk& v, const Walk& k, const Walk& q, hipStream_t stream);
 template <int TY> hipError_t launch_share(const float* parts, void* out, const int64_t* stride, uint32_t batch, uint32_t length, uint32_t key_heads, uint32_t share,
                                           uint32_t dim, hipStream_t stream);
 template <int TY> hipError_t launch_step(const ZenoAmdLinearInputs& in, void* o, const int64_t* o_stride, float* state, hipStream_t stream);

@@ -33,6 +33,7 @@ __global__ __launch_bounds__(256) void linear_decay_kernel(const double* parts, 
     if (threadIdx.x == 0) d_g[h] = (float)all[0];
 }
 
+uint32_t blocks_of(uint32_t columns) { return (columns + 31) / 32; }
 int64_t bytes_of(uint32_t dtype) { return dtype == T_F32 ? 4 : 2; }
 uint64_t heads_of(const ZenoAmdLinearInputs& in) { return (uint64_t)in.batch * in.value_heads; }
 uint64_t even(uint64_t floats) { return (floats + 3) / 4 * 4; }  // 16 bytes
@@ -42,7 +43,7 @@ uint64_t states_floats(const ZenoAmdLinearInputs& in) { return even(between(in) 
 uint64_t share_floats(const ZenoAmdLinearInputs& in) {  // gradients of q (or k) by value head
     return in.key_heads == in.value_heads ? 0 : even((uint64_t)in.batch * in.length * in.value_heads * in.key_dim);
 }
-uint64_t parts_floats(const ZenoAmdLinearInputs& in) { return in.decay_gradient ? even(2 * heads_of(in) * segments_of(in).count * shape_of(in.value_dim, in.key_dim).blocks) : 0; }
+uint64_t parts_floats(const ZenoAmdLinearInputs& in) { return in.decay_gradient ? even(2 * heads_of(in) * segments_of(in).count * 2 * blocks_of(in.key_dim)) : 0; }
 
 void set_strides(int64_t* to, const int64_t* from) {
     for (int i = 0; i < 3; ++i) to[i] = from[i];
@@ -55,10 +56,9 @@ Rows rows_of(const void* at, const int64_t* stride, uint32_t share) {
     return r;
 }
 
-hipError_t launch(uint32_t dtype, const Walk& w, const Shape& s, Kind kind, bool back, hipStream_t stream) {
-    return dtype == T_F32   ? launch_walk<T_F32>(w, s, kind, back, stream)
-           : dtype == T_F16 ? launch_walk<T_F16>(w, s, kind, back, stream)
-                            : launch_walk<T_BF16>(w, s, kind, back, stream);
+hipError_t launch(uint32_t dtype, const Walk& w, Kind kind, bool back, hipStream_t stream) {
+    auto run = dtype == T_F32 ? launch_walk<T_F32> : dtype == T_F16 ? launch_walk<T_F16> : launch_walk<T_BF16>;
+    return run(w, kind, back, stream);
 }
 
 // A walk over states [key_dim, value_dim], or (turned) over them transposed.
@@ -66,8 +66,9 @@ Walk walk_of(const ZenoAmdLinearInputs& in, bool turned) {
     Walk w{};
     w.da = turned ? in.value_dim : in.key_dim;
     w.dc = turned ? in.key_dim : in.value_dim;
-    w.row = turned ? 1 : in.value_dim;
-    w.col = turned ? in.value_dim : 1;
+    w.blocks = blocks_of(w.dc);
+    w.ld = in.value_dim;
+    w.turned = turned;
     w.size = state_size(in);
     w.batch = in.batch;
     w.heads = in.value_heads;
@@ -81,10 +82,6 @@ Walk walk_of(const ZenoAmdLinearInputs& in, bool turned) {
     w.segments = s.count;
     w.segment_length = s.length;
     return w;
-}
-void set_shape(Walk& w, const Shape& s) {
-    w.blocks = s.blocks;
-    w.full = s.full;
 }
 
 std::string check_outputs(const std::vector<Memory>& inputs, const std::vector<Memory>& outputs) {
@@ -100,19 +97,11 @@ std::string check_outputs(const std::vector<Memory>& inputs, const std::vector<M
 
 }  // namespace
 
-Shape shape_of(int da, int dc) {
-    Shape s;
-    s.steps = da <= 32 ? 1 : da <= 64 ? 2 : 4;
-    s.blocks = (dc + 31) / 32;
-    s.full = da == 32 * s.steps && dc % 32 == 0;
-    return s;
-}
-
-// With fewer walks than two waves a SIMD, as many segments as make up those, of at least four chunks.
+// With fewer walks than two waves a SIMD, as many segments as make up those, of at least eight chunks.
 Segments segments_of(const ZenoAmdLinearInputs& in) {
     const int64_t chunks = ((int64_t)in.length + kChunk - 1) / kChunk;
-    const int64_t walks = (int64_t)heads_of(in) * shape_of(in.key_dim, in.value_dim).blocks;
-    int64_t want = std::min(2048 / walks, chunks / 4);
+    const int64_t walks = (int64_t)heads_of(in) * blocks_of(in.value_dim);
+    int64_t want = std::min(2048 / walks, chunks / 8);
     if (want < 2) want = 1;
     const int64_t each = (chunks + want - 1) / want;
     return Segments{(uint32_t)((chunks + each - 1) / each), (int)(each * kChunk)};
@@ -206,14 +195,10 @@ hipError_t forward(const ZenoAmdLinearInputs& in, void* o, const int64_t* o_stri
     w.starts = saved ? saved : workspace + even(between(in));
     if (w.segments > 1) {
         const bool slope = saved && in.decay_gradient;
-        const Shape s = shape_of(w.da, w.dc);
-        set_shape(w, s);
         if (slope) w.slopes = saved + states_floats(in);
-        if (const hipError_t e = launch(in.dtype, w, s, slope ? STATES_SLOPE : STATES, false, stream)) return e;
+        if (const hipError_t e = launch(in.dtype, w, slope ? STATES_SLOPE : STATES, false, stream)) return e;
     }
-    const Shape s = shape_of(w.da, w.dc);
-    set_shape(w, s);
-    return launch(in.dtype, w, s, OUTPUTS, false, stream);
+    return launch(in.dtype, w, OUTPUTS, false, stream);
 }
 
 hipError_t backward(const ZenoAmdLinearInputs& in, const float* saved, const ZenoAmdLinearGradients& grad, float* workspace, hipStream_t stream) {
@@ -232,54 +217,33 @@ hipError_t backward(const ZenoAmdLinearInputs& in, const float* saved, const Zen
         w.out_share = 1;
         w.out_f32 = share > 1;
     };
+
+    Walk wv = walk_of(in, false), wk = walk_of(in, true), wq = walk_of(in, true);
+    wv.a = k, wv.b = q, wv.c = d_o;
+    wk.a = v, wk.b = d_o, wk.c = q;
+    wq.a = d_o, wq.b = v, wq.c = k, wq.q = q;
+    wv.out = grad.d_v;
+    set_strides(wv.out_stride, grad.d_v_stride);
+    wv.out_share = 1;
+    key_out(wk, grad.d_k, grad.d_k_stride, part_k);
+    key_out(wq, grad.d_q, grad.d_q_stride, part_q);
+    wv.first = wk.first = wq.d_last = grad.d_last;
+    wv.last = grad.d_state;
+    wv.starts = wk.starts = d_starts;
+    wv.passes = passes;
+    wq.first = in.state;
+    wq.starts = const_cast<float*>(saved);
+    wq.slopes = wq.starts + states_floats(in);
+    wq.parts = reinterpret_cast<double*>(parts);
+
     hipError_t e;
-
-    // d_v, and before it what it starts its segments with
-    Walk w = walk_of(in, false);
-    w.a = k;
-    w.b = q;
-    w.c = d_o;
-    w.out = grad.d_v;
-    set_strides(w.out_stride, grad.d_v_stride);
-    w.out_share = 1;
-    w.first = grad.d_last;
-    w.last = grad.d_state;
-    w.starts = d_starts;
-    w.passes = passes;
-    Shape s = shape_of(w.da, w.dc);
-    set_shape(w, s);
-    if (w.segments > 1 && (e = launch(in.dtype, w, s, STATES, true, stream))) return e;
-    if ((e = launch(in.dtype, w, s, OUTPUTS, true, stream))) return e;
-
-    // d_k
-    w = walk_of(in, true);
-    w.a = v;
-    w.b = d_o;
-    w.c = q;
-    key_out(w, grad.d_k, grad.d_k_stride, part_k);
-    w.first = grad.d_last;
-    w.starts = d_starts;
-    s = shape_of(w.da, w.dc);
-    set_shape(w, s);
-    if ((e = launch(in.dtype, w, s, OUTPUTS, true, stream))) return e;
-
-    // d_q and d_g
-    w = walk_of(in, true);
-    w.a = d_o;
-    w.b = v;
-    w.c = k;
-    w.q = q;
-    key_out(w, grad.d_q, grad.d_q_stride, part_q);
-    w.first = in.state;
-    w.starts = const_cast<float*>(saved);
-    w.slopes = w.starts + states_floats(in);
-    w.d_last = grad.d_last;
-    w.parts = reinterpret_cast<double*>(parts);
-    s = shape_of(w.da, w.dc);
-    set_shape(w, s);
-    if ((e = launch(in.dtype, w, s, grad.d_g ? OUTPUTS_SLOPE : OUTPUTS, false, stream))) return e;
-    if (grad.d_g) linear_decay_kernel<<<in.value_heads, 256, 0, stream>>>(w.parts, in.batch, in.value_heads, w.segments * s.blocks, grad.d_g);
-
+    if (wv.segments > 1 && (e = launch(in.dtype, wv, STATES, true, stream))) return e;
+    auto gradients = in.dtype == T_F32 ? launch_gradients<T_F32> : in.dtype == T_F16 ? launch_gradients<T_F16> : launch_gradients<T_BF16>;
+    if ((e = gradients(wv, wk, wq, stream))) return e;
+    if (grad.d_g) {
+        if ((e = launch(in.dtype, wq, SLOPES, false, stream))) return e;
+        linear_decay_kernel<<<in.value_heads, 256, 0, stream>>>(wq.parts, in.batch, in.value_heads, wq.segments * 2 * wq.blocks, grad.d_g);
+    }
     if (share > 1) {
         auto add = in.dtype == T_F32 ? launch_share<T_F32> : in.dtype == T_F16 ? launch_share<T_F16> : launch_share<T_BF16>;
         if ((e = add(part_q, grad.d_q, grad.d_q_stride, in.batch, in.length, in.key_heads, share, in.key_dim, stream))) return e;

@@ -1,7 +1,7 @@
 // Kernels of linear attention with a decay for each head: walks over whole sequences, and the
 // single-token step.
 //
-// A chunk is 32 tokens (16 where registers are short). With S the state before it, a walk forward is
+// A chunk is 16 tokens. With S the state before it, a walk forward is
 //     P_ij = scale exp(g (i - j)) A_i . B_j  for j <= i with no reset after j up to i, else 0
 //     out  = P C + scale exp(g (i + 1)) A S      (the second where no reset is before or at i)
 //     S'   = exp(g L) S + sum_j exp(g (L - 1 - j)) B_j C_j^T      (L tokens; nothing across a reset)
@@ -25,6 +25,7 @@
 // A chunk that holds a value that is not finite goes token by token, so that none meets an output before
 // its token, or behind a reset, by way of the zeros in P.
 #pragma once
+#include <algorithm>
 #include <type_traits>
 
 #include "linear.h"
@@ -52,17 +53,6 @@ template <int TY> __device__ __forceinline__ Frag<Elem<TY>::parts> operand(const
     return f;
 }
 
-// Operands along the tokens of a chunk: of two tiles or of one.
-template <int TILES> struct Along;
-template <> struct Along<2> {
-    template <int P> using Op = Frag<P>;
-    template <int P> static __device__ __forceinline__ Frag<P> make(const f4* x) { return split<P>(x[0], x[1]); }
-};
-template <> struct Along<1> {
-    template <int P> using Op = Half<P>;
-    template <int P> static __device__ __forceinline__ Half<P> make(const f4* x) { return split<P>(x[0]); }
-};
-
 // Four floats at any address, the first `n` of them in bounds.
 template <bool FULL> __device__ __forceinline__ f4 load_floats(const float* at, int n) {
     if (FULL || n >= 4) return __builtin_bit_cast(f4, reinterpret_cast<const Loose<T_F32>::U*>(at)->v);
@@ -82,48 +72,44 @@ template <bool FULL> __device__ __forceinline__ void store_floats(float* at, int
     }
 }
 
-template <int TY, int STEPS, int TILES, bool AHEAD, bool BACK, int KIND, bool FULL>
-__global__ __launch_bounds__(256, 2) void linear_walk_kernel(const Walk a) {
+// One walk of one wave: of 32 columns of the state (JS 2), or of 16 of them (JS 1: tile `half` of the pair), in
+// one segment of one head.
+template <int TY, int STEPS, int JS, bool BACK, int KIND, bool FULL>
+__device__ __forceinline__ void walk(const Walk& a, const uint32_t bh, const uint32_t segment, const int block, const int half, const uint32_t unit) {
     typedef typename Elem<TY>::type E;
-    constexpr int NP = Elem<TY>::parts, C = 16 * TILES;
-    constexpr bool OUT = KIND == OUTPUTS || KIND == OUTPUTS_SLOPE, SLOPE = KIND == OUTPUTS_SLOPE || KIND == STATES_SLOPE;
-    constexpr bool GRAD = KIND == OUTPUTS_SLOPE;
+    constexpr int NP = Elem<TY>::parts, C = kChunk;
+    constexpr bool OUT = KIND == OUTPUTS, SLOPE = KIND == SLOPES || KIND == STATES_SLOPE, GRAD = KIND == SLOPES, READ = OUT || GRAD;
+    // Operands for outputs of 16 bits that are no part of a state: two parts, 2^-17 of a term, where the output is rounded
+    // by 2^-9 or 2^-12 of itself.
+    constexpr int KEPT = TY == T_F32 || GRAD ? 3 : 2;
     const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
-    const uint32_t walks = OUT ? a.segments : a.segments - 1;  // of the segments, all but the last in the walk's direction
-    const uint32_t unit = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
-    const uint32_t block = unit % a.blocks, walk = unit / a.blocks % walks, bh = unit / a.blocks / walks;
-    if (bh >= a.batch * a.heads) return;
     const int64_t b = bh / a.heads, h = bh % a.heads;
-    const uint32_t segment = !OUT && BACK ? walk + 1 : walk;
     const int begin = segment * a.segment_length, T = begin + min(a.length - begin, a.segment_length);
     const int col0 = block * 32;
     const int da = a.da, dc = a.dc - col0;
     auto row_of = [&](const Rows& x, int e) { return (const E*)x.at + b * x.stride[0] + (h / x.share) * x.stride[2] + e + 8 * g; };
-    const E* ap = OUT ? row_of(a.a, 0) : nullptr;
+    const E* ap = READ ? row_of(a.a, 0) : nullptr;
     const E* bp = row_of(a.b, 0);
     const E* cp = row_of(a.c, col0);
     const E* qp = GRAD ? row_of(a.q, col0) : nullptr;
     const uint8_t* rp = a.reset ? a.reset + b * a.reset_stride[0] : nullptr;
 
-    // ---- what a chunk reads
-    Eight<TY> ar[OUT ? TILES : 1][STEPS], br[TILES][STEPS], cr[TILES], qr[GRAD ? TILES : 1];
+    // ---- what a chunk reads: token n's dimensions 8 g to 8 g + 7 of every 32
+    Eight<TY> ar[STEPS], br[STEPS], cr, qr;
     bool cut = false, any_cut = false;
     auto fetch = [&](int t, int rows) {
         cut = rp && lane < rows && rp[(t + lane) * a.reset_stride[1]];
+        const int64_t tok = t + min(n, rows - 1);
+        const E* x = bp + tok * a.b.stride[1];
 #pragma unroll
-        for (int i = 0; i < TILES; ++i) {
-            const int64_t tok = t + min(16 * i + n, rows - 1);
-            const E* x = bp + tok * a.b.stride[1];
+        for (int s = 0; s < STEPS; ++s) br[s].template load<FULL>(x + 32 * s, da - 32 * s - 8 * g);
+        if constexpr (READ) {
+            x = ap + tok * a.a.stride[1];
 #pragma unroll
-            for (int s = 0; s < STEPS; ++s) br[i][s].template load<FULL>(x + 32 * s, da - 32 * s - 8 * g);
-            if constexpr (OUT) {
-                x = ap + tok * a.a.stride[1];
-#pragma unroll
-                for (int s = 0; s < STEPS; ++s) ar[i][s].template load<FULL>(x + 32 * s, da - 32 * s - 8 * g);
-            }
-            cr[i].template load<FULL>(cp + tok * a.c.stride[1], dc - 8 * g);
-            if constexpr (GRAD) qr[i].template load<FULL>(qp + tok * a.q.stride[1], dc - 8 * g);
+            for (int s = 0; s < STEPS; ++s) ar[s].template load<FULL>(x + 32 * s, da - 32 * s - 8 * g);
         }
+        cr.template load<FULL>(cp + tok * a.c.stride[1], dc - 8 * g);
+        if constexpr (GRAD) qr.template load<FULL>(qp + tok * a.q.stride[1], dc - 8 * g);
     };
     auto bounds = [&](int at, int& t, int& rows) {  // the chunk of the grid that `at` is in, from it (or up to it) on
         if (BACK) {
@@ -138,80 +124,74 @@ __global__ __launch_bounds__(256, 2) void linear_walk_kernel(const Walk a) {
     bounds(at, t, rows);
     fetch(t, rows);
 
-    // ---- the state, by row tiles of 16 (pairs of them make 32 rows) and two column tiles
-    f4 S[2 * STEPS][2], N[SLOPE ? 2 * STEPS : 1][2];
-    // A lane takes four values that lie side by side: of one of four rows, which four lanes then exchange, or
-    // of a column, where columns lie side by side.
-    auto place = [&](int i, int j, int& left) {
-        const int row = 32 * (i >> 1) + 8 * g + 4 * (i & 1), col = 8 * (n >> 2) + 4 * j;
-        if (a.row == 1) {
-            left = FULL ? 4 : col + (n & 3) < dc ? da - row : 0;
-            return row + (int64_t)(col0 + col + (n & 3)) * a.col;
-        }
-        left = FULL ? 4 : row + (n & 3) < da ? dc - col : 0;
-        return (int64_t)(row + (n & 3)) * a.row + col0 + col;
+    // ---- the state, by row tiles of 16 (pairs of them make 32 rows) and column tiles
+    f4 S[2 * STEPS][JS], N[SLOPE ? 2 * STEPS : 1][JS];
+    // A lane takes four values that lie side by side: of one of four rows, which four lanes then exchange, or of a
+    // column where columns lie side by side (`turned`). Places are found anew each time: kept from the walk's begin
+    // to its end they would not fit the registers.
+    auto each_four = [&](int m, auto&& access) {
+        asm volatile("" : "+v"(m));
+        const int mn = m & 15, mg = m >> 4;
+        const int mine = a.turned ? (8 * (mn >> 2) + (mn & 3)) * a.ld + 8 * mg : (8 * mg + (mn & 3)) * a.ld + 8 * (mn >> 2);
+#pragma unroll
+        for (int i = 0; i < 2 * STEPS; ++i)
+#pragma unroll
+            for (int j = 0; j < JS; ++j) {
+                const int row = 32 * (i >> 1) + 4 * (i & 1), col = 4 * (JS == 2 ? j : half);
+                const int base = a.turned ? (col0 + col) * a.ld + row : row * a.ld + col0 + col;
+                int left = 4;
+                if (!FULL) {
+                    if (a.turned) left = 8 * (mn >> 2) + (mn & 3) + col < dc ? da - row - 8 * mg : 0;
+                    else left = 8 * mg + (mn & 3) + row < da ? dc - col - 8 * (mn >> 2) : 0;
+                }
+                access(i, j, base, mine, left);
+            }
     };
     auto load_state = [&](auto& X, const float* from) {
 #pragma unroll
         for (int i = 0; i < 2 * STEPS; ++i)
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                int left;
-                const int64_t at = place(i, j, left);
-                X[i][j] = f4{0, 0, 0, 0};
-                if (from) X[i][j] = load_floats<FULL>(from + at, left);
-            }
-        if (from && a.row != 1)
-#pragma unroll
-            for (int i = 0; i < 2 * STEPS; ++i)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) X[i][j] = turn(X[i][j], lane);
-    };
-    auto store_state = [&](const auto& X, float* to) {
+            for (int j = 0; j < JS; ++j) X[i][j] = f4{0, 0, 0, 0};
+        if (!from) return;
+        each_four(lane, [&](int i, int j, int base, int mine, int left) { X[i][j] = load_floats<FULL>(from + base + mine, left); });
+        if (a.turned) return;
 #pragma unroll
         for (int i = 0; i < 2 * STEPS; ++i)
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                int left;
-                const int64_t at = place(i, j, left);
-                store_floats<FULL>(to + at, left, a.row == 1 ? X[i][j] : turn(X[i][j], lane));
-            }
+            for (int j = 0; j < JS; ++j) X[i][j] = turn(X[i][j], lane);
+    };
+    auto store_state = [&](auto& X, float* to) {
+        if (!a.turned)
+#pragma unroll
+            for (int i = 0; i < 2 * STEPS; ++i)
+#pragma unroll
+                for (int j = 0; j < JS; ++j) X[i][j] = turn(X[i][j], lane);
+        each_four(lane, [&](int i, int j, int base, int mine, int left) { store_floats<FULL>(to + base + mine, left, X[i][j]); });
     };
     const bool at_first = BACK ? segment == a.segments - 1 : segment == 0;
     const int64_t between = (int64_t)bh * (a.segments - 1) + (BACK ? segment : segment - 1);  // the start of this walk
-    load_state(S, at_first ? (a.first ? a.first + bh * a.size : nullptr) : OUT ? a.starts + between * a.size : nullptr);
-    if constexpr (SLOPE) load_state(N, OUT && !at_first ? a.slopes + between * a.size : nullptr);
+    load_state(S, at_first ? (a.first ? a.first + bh * a.size : nullptr) : READ ? a.starts + between * a.size : nullptr);
+    if constexpr (SLOPE) load_state(N, READ && !at_first ? a.slopes + between * a.size : nullptr);
 
     // ---- the head's decays. `read`: of the state to a token, `write`: of a token to the next state.
     float gh = a.g[h];
     gh = gh < -200.0f ? -200.0f : gh;  // 0 in fp32 from one token to the next
-    float near[4], far[4];  // inside a tile of 16, and between the two
-    float read[TILES], all = 0.0f;
-    f4 write[TILES];
+    float near[4], read = 0.0f, all = 0.0f;
+    f4 write;
     int measured = -1;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-        const int m = BACK ? 4 * g + r - n : n - 4 * g - r;
-        near[r] = m < 0 ? 0.0f : a.scale * decay(gh, m);
-        far[r] = a.scale * decay(gh, 16 + m);
+        near[r] = a.scale * decay(gh, max(BACK ? 4 * g + r - n : n - 4 * g - r, 0));
+        if (BACK) write[r] = a.scale * decay(gh, 4 * g + r + 1);
     }
-#pragma unroll
-    for (int i = 0; i < TILES; ++i) {
-        if (!BACK) read[i] = a.scale * decay(gh, 16 * i + n + 1);
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-            if (BACK) write[i][r] = a.scale * decay(gh, 16 * i + 4 * g + r + 1);
-    }
+    if (!BACK) read = a.scale * decay(gh, n + 1);
     auto measure = [&](int len) {  // those that depend on the chunk's length
         measured = len;
         all = decay(gh, len);
+        if (BACK) read = decay(gh, max(len - 1 - n, 0));
 #pragma unroll
-        for (int i = 0; i < TILES; ++i) {
-            if (BACK) read[i] = decay(gh, max(len - 1 - 16 * i - n, 0));
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-                if (!BACK) write[i][r] = decay(gh, max(len - 1 - 16 * i - 4 * g - r, 0));
-        }
+        for (int r = 0; r < 4; ++r)
+            if (!BACK) write[r] = decay(gh, max(len - 1 - 4 * g - r, 0));
     };
 
     // ---- unit matrices as operands: they pick dimension 8 (n / 4) + 4 i + n % 4 of a row's 32
@@ -225,27 +205,24 @@ __global__ __launch_bounds__(256, 2) void linear_walk_kernel(const Walk a) {
         }
     double dg = 0.0;
 
-    // The chunk of tokens t to t + len, in USED tiles. CUTS: there may be resets inside, in `cuts`. ODD: one token,
-    // with values that are not finite: its operands along the tokens are read one by one. No branch is inside: where
-    // one lies between a matrix instruction and the use of its result, the compiler has been seen to leave out the
-    // wait. The scheduler is kept from starting everything at once, which takes more registers than there are.
-    auto chunk = [&](auto used, auto with_cuts, auto is_odd, int t, int len, uint32_t cuts, auto&& next) {
-        constexpr int USED = decltype(used)::value;
+    // The chunk of tokens t to t + len. CUTS: there may be resets inside, in `cuts`. ODD: one token, with values
+    // that are not finite: its operands along the tokens are read one by one. No branch is inside: where one lies
+    // between a matrix instruction and the use of its result, the compiler has been seen to leave out the wait. The
+    // scheduler is kept from starting everything at once, which takes more registers than there are.
+    auto chunk = [&](auto with_cuts, auto is_odd, int t, int len, uint32_t cuts) {
         constexpr bool CUTS = decltype(with_cuts)::value, ODD = decltype(is_odd)::value;
         const f4 zero = {0, 0, 0, 0};
-        Frag<NP> af[OUT ? USED : 1][STEPS], bf[USED][STEPS], cf[USED];
-        Eight<TY> qe[GRAD ? USED : 1];
+
+        // Resets: the last one up to a token (this lane's, and those of its registers), and of the chunk.
+        int mine = -1, theirs[4], last_cut = -1, first_cut = C;
+        if constexpr (CUTS) {
+            last_cut = cuts ? 31 - __builtin_clz(cuts) : -1;
+            first_cut = cuts ? __builtin_ctz(cuts) : C;
+            mine = 31 - __clz((int)(cuts & (0xffffu >> (15 - n))));
 #pragma unroll
-        for (int i = 0; i < USED; ++i) {
-#pragma unroll
-            for (int s = 0; s < STEPS; ++s) {
-                bf[i][s] = operand(br[i][s]);
-                if constexpr (OUT) af[i][s] = operand(ar[i][s]);
-            }
-            cf[i] = operand(cr[i]);
-            if constexpr (GRAD) qe[i] = qr[i];
+            for (int r = 0; r < 4; ++r) theirs[r] = 31 - __clz((int)(cuts & (0xffffu >> (15 - 4 * g - r))));
         }
-        f4 odd_b[ODD ? 2 * STEPS : 1], odd_c[2];
+        f4 odd_b[2 * STEPS], odd_c[2];
         if constexpr (ODD) {
             const int e = 8 * (n >> 2) + (n & 3) - 8 * g;  // from this lane's place in its rows to the dimension that it stands for
 #pragma unroll
@@ -256,116 +233,80 @@ __global__ __launch_bounds__(256, 2) void linear_walk_kernel(const Walk a) {
 #pragma unroll
             for (int j = 0; j < 2; ++j) odd_c[j] = f4{g == 0 && 4 * j + e < dc ? Elem<TY>::get(cp[t * a.c.stride[1] + 4 * j + e]) : 0.0f, 0, 0, 0};
         }
-        if (AHEAD) next();
 
-        // Resets: the last one up to a token (this lane's, and those of its registers), and of the chunk.
-        int mine[USED], theirs[USED][4], last_cut = -1, first_cut = 64;
-        if constexpr (CUTS) {
-            last_cut = cuts ? 31 - __builtin_clz(cuts) : -1;
-            first_cut = cuts ? __builtin_ctz(cuts) : 64;
+        // ---- P transposed (row j = 4 g + r, column i = n), and B along the tokens
+        Frag<NP> af[STEPS];
+        Half<NP> bt[2 * STEPS];
+        f4 p = zero, y = zero;
 #pragma unroll
-            for (int i = 0; i < USED; ++i) {
-                mine[i] = 31 - __clz((int)(cuts & (0xffffffffu >> (31 - 16 * i - n))));
-#pragma unroll
-                for (int r = 0; r < 4; ++r) theirs[i][r] = 31 - __clz((int)(cuts & (0xffffffffu >> (31 - 16 * i - 4 * g - r))));
+        for (int s = 0; s < STEPS; ++s) {
+            const Frag<NP> bf = operand(br[s]);
+            if constexpr (READ) {
+                af[s] = operand(ar[s]);
+                p = mul<2>(bf, af[s], p);
             }
-        }
-
-        // ---- P transposed (row j = 16 tj + 4 g + r, column i = 16 ti + n), as operands along j
-        Half<3> alone;  // of the tokens that see one tile
-        Frag<3> both;   // of those that see two
-        float pairs = 0.0f;
-        if constexpr (OUT) {
-            f4 pt[USED][USED];
 #pragma unroll
-            for (int tj = 0; tj < USED; ++tj)
-#pragma unroll
-                for (int ti = 0; ti < USED; ++ti) {
-                    if (BACK ? tj < ti : tj > ti) continue;
-                    f4 x = zero, y = zero;
-#pragma unroll
-                    for (int s = 0; s < STEPS; ++s) x = mul<2>(bf[tj][s], af[ti][s], x);
-                    if constexpr (GRAD) y = mul<2>(cf[tj], operand(qe[ti]), y);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const int i = 16 * ti + n, j = 16 * tj + 4 * g + r;
-                        x[r] *= tj == ti ? near[r] : far[r];
-                        // A product that is not finite does not pass the zeros either.
-                        if (tj == ti) x[r] = (BACK ? j >= i : j <= i) ? x[r] : 0.0f;
-                        if (CUTS) x[r] = (BACK ? i >= theirs[tj][r] : j >= mine[ti]) ? x[r] : 0.0f;
-                        if (GRAD) pairs += (float)(i - j) * x[r] * y[r];
-                    }
-                    pt[tj][ti] = x;
-                }
-            constexpr int one = BACK ? USED - 1 : 0;
-            alone = split<3>(pt[one][one]);
-            if constexpr (USED == 2) both = split<3>(pt[0][1 - one], pt[1][1 - one]);
-        }
-        typename Along<USED>::template Op<NP> bt[2 * STEPS];
-#pragma unroll
-        for (int i = 0; i < 2 * STEPS; ++i) {
-            f4 x[USED];
-#pragma unroll
-            for (int k = 0; k < USED; ++k) x[k] = ODD ? odd_b[ODD ? i : 0] : mul<2>(bf[k][i >> 1], unit_of[i & 1], zero);
-            bt[i] = Along<USED>::template make<NP>(x);
-        }
-        f4 out[USED][2];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
+            for (int i = 0; i < 2; ++i) bt[2 * s + i] = split<NP>(ODD ? odd_b[2 * s + i] : mul<2>(bf, unit_of[i], zero));
             __builtin_amdgcn_sched_barrier(0);
-            f4 ct[USED], wc[USED];
+        }
+        const Frag<NP> cf = operand(cr);
+        Half<KEPT> P;
+        float pairs = 0.0f;
+        if constexpr (READ) {
+            if constexpr (GRAD) y = mul<2>(cf, operand(qr), zero);
 #pragma unroll
-            for (int k = 0; k < USED; ++k) ct[k] = ODD ? odd_c[j] : mul<2>(cf[k], unit_of[j], zero);
-            if constexpr (OUT) {
-                f4 slope[USED];
+            for (int r = 0; r < 4; ++r) {
+                const int i = n, j = 4 * g + r;
+                // A product that is not finite does not pass the zeros either.
+                p[r] = (BACK ? j >= i : j <= i) ? p[r] * near[r] : 0.0f;
+                if (CUTS) p[r] = (BACK ? i >= theirs[r] : j >= mine) ? p[r] : 0.0f;
+                if (GRAD) pairs += (float)(i - j) * p[r] * y[r];
+            }
+            P = split<KEPT>(p);
+        }
+        if (GRAD && JS == 1) pairs = half ? 0.0f : pairs;  // once for the two waves of these columns
+        float out[8];
 #pragma unroll
-                for (int k = 0; k < USED; ++k) out[k][j] = slope[k] = zero;
+        for (int j = 0; j < JS; ++j) {
+            __builtin_amdgcn_sched_barrier(0);
+            const f4 odd = ODD ? (JS == 2 ? odd_c[j] : half ? odd_c[1] : odd_c[0]) : zero;
+            Frag<1> pick = unit_of[JS == 2 ? j : 0];
+            if (JS == 1)
 #pragma unroll
-                for (int s = 0; s < STEPS; ++s) {
-                    const Frag<3> sf = split<3>(S[2 * s][j], S[2 * s + 1][j]);
+                for (int w = 0; w < 4; ++w) pick.p[0][w] = half ? unit_of[1].p[0][w] : unit_of[0].p[0][w];
+            const f4 ct = ODD ? odd : mul<2>(cf, pick, zero);
+            if constexpr (READ) {
+                const bool reach = !CUTS || (BACK ? n >= last_cut : mine < 0);
+                f4 x = zero;
 #pragma unroll
-                    for (int k = 0; k < USED; ++k) out[k][j] = mul<2>(sf, af[k][s], out[k][j]);
-                    if constexpr (GRAD) {
-                        const Frag<3> nf = split<3>(N[2 * s][j], N[2 * s + 1][j]);
+                for (int s = 0; s < STEPS; ++s) x = mul<2>(split<KEPT>(S[2 * s][j], S[2 * s + 1][j]), af[s], x);
 #pragma unroll
-                        for (int k = 0; k < USED; ++k) slope[k] = mul<2>(nf, af[k][s], slope[k]);
-                    }
+                for (int r = 0; r < 4; ++r) x[r] = reach ? x[r] * read : 0.0f;
+                if constexpr (GRAD) {
+                    f4 slope = zero;
+#pragma unroll
+                    for (int s = 0; s < STEPS; ++s) slope = mul<2>(split<3>(N[2 * s][j], N[2 * s + 1][j]), af[s], slope);
+                    float q[8];
+                    qr.get(q);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        pairs += ((float)(n + 1) * x[r] + (reach ? slope[r] * read : 0.0f)) * (JS == 2 ? q[4 * j + r] : half ? q[4 + r] : q[r]);
+                } else {
+                    x = mul<2>(split<NP>(ct), P, x);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) out[4 * j + r] = x[r];
                 }
-#pragma unroll
-                for (int k = 0; k < USED; ++k) {
-                    const bool reach = !CUTS || (BACK ? 16 * k + n >= last_cut : mine[k] < 0);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) out[k][j][r] = reach ? out[k][j][r] * read[k] : 0.0f;
-                    if constexpr (GRAD) {
-                        float q[8];
-                        qe[k].get(q);
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            const float x = (float)(16 * k + n + 1) * out[k][j][r] + (reach ? slope[k][r] * read[k] : 0.0f);
-                            pairs += x * q[4 * j + r];
-                        }
-                    }
-                }
-                constexpr int one = BACK ? USED - 1 : 0;
-                out[one][j] = mul<2>(split<NP>(ct[one]), alone, out[one][j]);
-                if constexpr (USED == 2) out[1 - one][j] = mul<2>(split<NP>(ct[0], ct[1]), both, out[1 - one][j]);
             }
             // ---- the state behind the chunk
             __builtin_amdgcn_sched_barrier(0);
+            f4 w;
 #pragma unroll
-            for (int k = 0; k < USED; ++k)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int at = 16 * k + 4 * g + r;
-                    wc[k][r] = !CUTS || (BACK ? at < first_cut : at >= last_cut) ? ct[k][r] * write[k][r] : 0.0f;
-                }
-            const auto wf = Along<USED>::template make<3>(wc);
+            for (int r = 0; r < 4; ++r) w[r] = !CUTS || (BACK ? 4 * g + r < first_cut : 4 * g + r >= last_cut) ? ct[r] * write[r] : 0.0f;
+            const Half<3> wf = split<3>(w);
             if constexpr (SLOPE) {
 #pragma unroll
-                for (int k = 0; k < USED; ++k)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) wc[k][r] *= (float)max(len - 1 - 16 * k - 4 * g - r, 0);
-                const auto nf = Along<USED>::template make<3>(wc);
+                for (int r = 0; r < 4; ++r) w[r] *= (float)max(len - 1 - 4 * g - r, 0);
+                const Half<3> nf = split<3>(w);
 #pragma unroll
                 for (int i = 0; i < 2 * STEPS; ++i) {
                     f4 x = (N[i][j] + S[i][j] * (float)len) * all;
@@ -381,42 +322,32 @@ __global__ __launch_bounds__(256, 2) void linear_walk_kernel(const Walk a) {
             }
         }
         if constexpr (OUT) {
-#pragma unroll
-            for (int k = 0; k < USED; ++k) {
-                const int row = 16 * k + n, e = 8 * g;
-                const float y[8] = {out[k][0][0], out[k][0][1], out[k][0][2], out[k][0][3], out[k][1][0], out[k][1][1], out[k][1][2], out[k][1][3]};
-                const int64_t to = b * a.out_stride[0] + (t + row) * a.out_stride[1] + (h / a.out_share) * a.out_stride[2] + col0 + e;
-                if (row < len) {
-                    if (a.out_f32) {
-                        Eight<T_F32> x;
-                        x.set(y);
-                        x.template store<FULL>((float*)a.out + to, dc - e);
-                    } else {
-                        Eight<TY> x;
-                        x.set(y);
-                        x.template store<FULL>((E*)a.out + to, dc - e);
-                    }
+            const int64_t to = b * a.out_stride[0] + (t + n) * a.out_stride[1] + (h / a.out_share) * a.out_stride[2] + col0 + 8 * g;
+            if (n < len) {
+                if (a.out_f32) {
+                    Eight<T_F32> x;
+                    x.set(out);
+                    x.template store<FULL>((float*)a.out + to, dc - 8 * g);
+                } else {
+                    Eight<TY> x;
+                    x.set(out);
+                    x.template store<FULL>((E*)a.out + to, dc - 8 * g);
                 }
             }
         }
         if (GRAD) dg += (double)pairs;
-        if (!AHEAD) next();
     };
 
-    // ---- the walk
-    while (BACK ? at > begin : at < T) {
+    // ---- the walk. Nothing is fetched ahead: a third wave a SIMD, for which that leaves no registers, hides more.
+    while (true) {
         int len = rows, first = t;
-        bool fine = true;
+        bool fine = cr.finite();
 #pragma unroll
-        for (int i = 0; i < TILES; ++i) {
-#pragma unroll
-            for (int s = 0; s < STEPS; ++s) {
-                fine &= br[i][s].finite();
-                if (OUT) fine &= ar[OUT ? i : 0][s].finite();
-            }
-            fine &= cr[i].finite();
-            if (GRAD) fine &= qr[GRAD ? i : 0].finite();
+        for (int s = 0; s < STEPS; ++s) {
+            fine &= br[s].finite();
+            if constexpr (READ) fine &= ar[s].finite();
         }
+        if constexpr (GRAD) fine &= qr.finite();
         uint32_t cuts = (uint32_t)__ballot(cut);
         const bool odd = __ballot(!fine) != 0;
         if (odd) {
@@ -430,99 +361,125 @@ __global__ __launch_bounds__(256, 2) void linear_walk_kernel(const Walk a) {
         }
         any_cut |= cuts != 0;
         if (len < C) {
+            const bool keep = n < len;
 #pragma unroll
-            for (int i = 0; i < TILES; ++i) {
-                const bool keep = 16 * i + n < len;
-#pragma unroll
-                for (int s = 0; s < STEPS; ++s) {
-                    br[i][s].keep(keep);
-                    if (OUT) ar[OUT ? i : 0][s].keep(keep);
-                }
-                cr[i].keep(keep);
-                if (GRAD) qr[GRAD ? i : 0].keep(keep);
+            for (int s = 0; s < STEPS; ++s) {
+                br[s].keep(keep);
+                if constexpr (READ) ar[s].keep(keep);
             }
+            cr.keep(keep);
+            if constexpr (GRAD) qr.keep(keep);
         }
         if (len != measured) measure(len);
-        const int now = first;
-        at = BACK ? first : first + len;
-        const bool more = BACK ? at > begin : at < T;
-        auto next = [&] {
-            if (more) {
-                bounds(at, t, rows);
-                fetch(t, rows);
-            }
-        };
-        constexpr std::integral_constant<int, 1> one{};
-        constexpr std::integral_constant<int, TILES> whole{};
         constexpr std::true_type yes{};
         constexpr std::false_type no{};
-        if (odd) {
-            chunk(one, yes, yes, now, len, cuts, next);
-        } else if (TILES == 2 && len <= 16) {
-            if (cuts) chunk(one, yes, no, now, len, cuts, next);
-            else chunk(one, no, no, now, len, cuts, next);
-        } else {
-            if (cuts) chunk(whole, yes, no, now, len, cuts, next);
-            else chunk(whole, no, no, now, len, cuts, next);
-        }
+        if (odd) chunk(yes, yes, first, len, cuts);
+        else if (cuts) chunk(yes, no, first, len, cuts);
+        else chunk(no, no, first, len, cuts);
+        at = BACK ? first : first + len;
+        if (BACK ? at <= begin : at >= T) break;
+        bounds(at, t, rows);
+        fetch(t, rows);
     }
 
     // ---- what it leaves
     if constexpr (OUT) {
-        if (BACK ? segment == 0 : segment == a.segments - 1) {
-            if (a.last) store_state(S, a.last + bh * a.size);
-            if constexpr (GRAD) {
-                if (a.d_last) {
-                    load_state(S, a.d_last + bh * a.size);
+        if (a.last && (BACK ? segment == 0 : segment == a.segments - 1)) store_state(S, a.last + bh * a.size);
+    } else if constexpr (GRAD) {
+        if (a.d_last && segment == a.segments - 1) {
+            load_state(S, a.d_last + bh * a.size);
 #pragma unroll
-                    for (int i = 0; i < 2 * STEPS; ++i)
+            for (int i = 0; i < 2 * STEPS; ++i)
 #pragma unroll
-                        for (int j = 0; j < 2; ++j)
+                for (int j = 0; j < JS; ++j)
 #pragma unroll
-                            for (int r = 0; r < 4; ++r) dg += S[i][j][r] == 0.0f ? 0.0 : (double)(S[i][j][r] * N[i][j][r]);
-                }
-            }
+                    for (int r = 0; r < 4; ++r) dg += S[i][j][r] == 0.0f ? 0.0 : (double)(S[i][j][r] * N[i][j][r]);
         }
-        if constexpr (GRAD) {
 #pragma unroll
-            for (int d = 32; d; d >>= 1) dg += __shfl_xor(dg, d);
-            if (lane == 0) a.parts[unit] = dg;
-        }
+        for (int d = 32; d; d >>= 1) dg += __shfl_xor(dg, d);
+        if (lane == 0) a.parts[unit] = dg;
     } else {
-        const int64_t to = (int64_t)bh * (a.segments - 1) + walk;
+        const int64_t to = (int64_t)bh * (a.segments - 1) + (BACK ? segment - 1 : segment);
         store_state(S, a.starts + to * a.size);
         if constexpr (SLOPE) store_state(N, a.slopes + to * a.size);
-        if (block == 0 && lane == 0) a.passes[to] = any_cut ? 0.0f : 1.0f;
+        if (block == 0 && half == 0 && lane == 0) a.passes[to] = any_cut ? 0.0f : 1.0f;
+    }
+}
+
+// The waves of neighbouring workgroups read the same rows: workgroups go to the eight dies in turn, so each
+// die is given a range of its own. Returns the number of this wave's work.
+__device__ __forceinline__ uint32_t unit_of_wave() {
+    const uint32_t each = gridDim.x / 8;  // the grid is a multiple of 8
+    return __builtin_amdgcn_readfirstlane(((blockIdx.x & 7) * each + (blockIdx.x >> 3)) * 4 + (threadIdx.x >> 6));
+}
+
+// Waves a SIMD that the registers are cut down to: as many as the state, its rows and their operands bear.
+constexpr int walk_waves(int type, int steps, int kind) { return steps == 4 || (steps == 2 && type == T_F32) ? 2 : 3; }
+
+template <int TY, int STEPS, int JS, bool BACK, int KIND, bool FULL>
+__global__ __launch_bounds__(256, walk_waves(TY, STEPS, KIND)) void linear_walk_kernel(const Walk a) {
+    constexpr bool READ = KIND == OUTPUTS || KIND == SLOPES;
+    const uint32_t walks = READ ? a.segments : a.segments - 1;  // of the segments, all but the last in the walk's direction
+    const uint32_t unit = unit_of_wave(), block = unit / (JS == 1 ? 2 : 1) % a.blocks, rest = unit / (JS == 1 ? 2 : 1) / a.blocks;
+    const uint32_t bh = rest / walks, segment = rest % walks + (!READ && BACK ? 1 : 0);
+    if (bh >= a.batch * a.heads) return;
+    walk<TY, STEPS, JS, BACK, KIND, FULL>(a, bh, segment, block, JS == 1 ? unit & 1 : 0, unit);
+}
+
+// All gradients but g's: the walks of d_v, d_k and d_q of a head and segment side by side, as they read the
+// same rows.
+struct Walks {
+    Walk v, k, q;
+};
+template <int TY, int STEPS, bool FULL> __global__ __launch_bounds__(256, walk_waves(TY, STEPS, OUTPUTS)) void linear_gradients_kernel(const Walks a) {
+    const uint32_t waves = a.v.blocks + a.k.blocks + a.q.blocks, unit = unit_of_wave(), rest = unit / waves;
+    const uint32_t bh = rest / a.v.segments, segment = rest % a.v.segments;
+    if (bh >= a.v.batch * a.v.heads) return;
+    const uint32_t at = unit % waves, back = a.v.blocks + a.k.blocks;
+    if (at < back) {
+        const bool v = at < a.v.blocks;
+        walk<TY, STEPS, 2, true, OUTPUTS, FULL>(v ? a.v : a.k, bh, segment, v ? at : at - a.v.blocks, 0, unit);
+    } else {
+        walk<TY, STEPS, 2, false, OUTPUTS, FULL>(a.q, bh, segment, at - back, 0, unit);
     }
 }
 
 // ---- joining segments ------------------------------------------------------------------------
 // The states between segments from what each adds: S_{p+1} = exp(g L) S_p + U_p, in place of U, where
-// the segment passes a state at all; and the slopes, N_{p+1} = exp(g L) (N_p + L S_p) + V_p. A thread a value.
+// the segment passes a state at all; and the slopes, N_{p+1} = exp(g L) (N_p + L S_p) + V_p. A thread a value;
+// eight segments' values are read at once, as each read waits for memory.
 template <bool BACK, bool SLOPE> __global__ __launch_bounds__(256) void linear_join_kernel(const Walk a) {
     const int64_t between = a.segments - 1, blocks = (a.size + 255) / 256;
     const int64_t bh = blockIdx.x / blocks, at = blockIdx.x % blocks * 256 + threadIdx.x;
     if (at >= a.size) return;
     float gh = a.g[bh % a.heads];
     gh = gh < -200.0f ? -200.0f : gh;
-    const float whole = decay(gh, a.segment_length), rest = decay(gh, a.length - between * a.segment_length);
+    const float whole = decay(gh, a.segment_length);
     float* starts = a.starts + bh * between * a.size + at;
     float* slopes = SLOPE ? a.slopes + bh * between * a.size + at : nullptr;
     const float* passes = a.passes + bh * between;
     float S = 0.0f, N = 0.0f;
-    for (int64_t k = 0; k < between; ++k) {
-        const int64_t p = BACK ? between - 1 - k : k;
-        const bool pass = k > 0 && passes[p] != 0.0f;  // nothing, NaN included, passes a reset
-        const float length = BACK && k == 0 ? a.length - between * a.segment_length : a.segment_length;
-        const float d = BACK && k == 0 ? rest : whole, before = S;
-        S = starts[p * a.size];
-        if (pass) S += d * before;
-        starts[p * a.size] = S;
-        if (SLOPE) {
-            const float n = N;
-            N = slopes[p * a.size];
-            if (pass) N += d * (n + length * before);
-            slopes[p * a.size] = N;
+    for (int64_t k0 = 0; k0 < between; k0 += 8) {
+        float U[8], V[8], pass[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            if (k0 + k >= between) continue;
+            const int64_t p = BACK ? between - 1 - k0 - k : k0 + k;
+            U[k] = starts[p * a.size];
+            if (SLOPE) V[k] = slopes[p * a.size];
+            pass[k] = passes[p];
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            if (k0 + k >= between) continue;
+            const int64_t p = BACK ? between - 1 - k0 - k : k0 + k;
+            const bool through = k0 + k > 0 && pass[k] != 0.0f;  // nothing, NaN included, passes a reset
+            if (SLOPE) {
+                N = through ? V[k] + whole * (N + (float)a.segment_length * S) : V[k];
+                slopes[p * a.size] = N;
+            }
+            S = through ? U[k] + whole * S : U[k];
+            starts[p * a.size] = S;
         }
     }
 }
@@ -620,30 +577,17 @@ __global__ __launch_bounds__(256) void linear_step_kernel(const ZenoAmdLinearInp
 }
 
 // ---- launches ------------------------------------------------------------------------------
-#ifndef TILES_OF
-#define TILES_OF(TY, STEPS) ((TY) == T_F32 ? 1 : 2)
-#endif
-#ifndef AHEAD_OF
-#define AHEAD_OF(TY, STEPS, KIND) ((STEPS) < 4 && (KIND) != OUTPUTS_SLOPE)
-#endif
+inline dim3 walk_grid(uint64_t units) { return dim3((uint32_t)((units + 31) / 32 * 8)); }  // a multiple of 8 workgroups of four waves
+
 template <int TY, int STEPS, bool FULL> void walk_shape(const Walk& w, Kind kind, bool back, hipStream_t stream) {
-    constexpr int TILES = TILES_OF(TY, STEPS);
-    const bool out = kind == OUTPUTS || kind == OUTPUTS_SLOPE;
-    const uint32_t units = w.batch * w.heads * w.blocks * (out ? w.segments : w.segments - 1);
-    const dim3 grid((units + 3) / 4);
-    if (back) {
-        if (out) linear_walk_kernel<TY, STEPS, TILES, AHEAD_OF(TY, STEPS, OUTPUTS), true, OUTPUTS, FULL><<<grid, 256, 0, stream>>>(w);
-        else linear_walk_kernel<TY, STEPS, TILES, AHEAD_OF(TY, STEPS, STATES), true, STATES, FULL><<<grid, 256, 0, stream>>>(w);
-    } else if (kind == OUTPUTS) {
-        linear_walk_kernel<TY, STEPS, TILES, AHEAD_OF(TY, STEPS, OUTPUTS), false, OUTPUTS, FULL><<<grid, 256, 0, stream>>>(w);
-    } else if (kind == STATES) {
-        linear_walk_kernel<TY, STEPS, TILES, AHEAD_OF(TY, STEPS, STATES), false, STATES, FULL><<<grid, 256, 0, stream>>>(w);
-    } else if (out) {
-        linear_walk_kernel<TY, STEPS, TILES, AHEAD_OF(TY, STEPS, OUTPUTS_SLOPE), false, OUTPUTS_SLOPE, FULL><<<grid, 256, 0, stream>>>(w);
-    } else {
-        linear_walk_kernel<TY, STEPS, TILES, AHEAD_OF(TY, STEPS, STATES_SLOPE), false, STATES_SLOPE, FULL><<<grid, 256, 0, stream>>>(w);
-    }
-    if (!out && w.segments > 2) {
+    const bool read = kind == OUTPUTS || kind == SLOPES, halves = kind == SLOPES || kind == STATES_SLOPE;
+    const dim3 grid = walk_grid((uint64_t)w.batch * w.heads * w.blocks * (read ? w.segments : w.segments - 1) * (halves ? 2 : 1));
+    if (kind == OUTPUTS) linear_walk_kernel<TY, STEPS, 2, false, OUTPUTS, FULL><<<grid, 256, 0, stream>>>(w);
+    else if (kind == SLOPES) linear_walk_kernel<TY, STEPS, 1, false, SLOPES, FULL><<<grid, 256, 0, stream>>>(w);
+    else if (kind == STATES_SLOPE) linear_walk_kernel<TY, STEPS, 1, false, STATES_SLOPE, FULL><<<grid, 256, 0, stream>>>(w);
+    else if (back) linear_walk_kernel<TY, STEPS, 2, true, STATES, FULL><<<grid, 256, 0, stream>>>(w);
+    else linear_walk_kernel<TY, STEPS, 2, false, STATES, FULL><<<grid, 256, 0, stream>>>(w);
+    if (!read && w.segments > 2) {
         const dim3 join(w.batch * w.heads * (uint32_t)((w.size + 255) / 256));
         if (back) linear_join_kernel<true, false><<<join, 256, 0, stream>>>(w);
         else if (kind == STATES) linear_join_kernel<false, false><<<join, 256, 0, stream>>>(w);
@@ -651,10 +595,23 @@ template <int TY, int STEPS, bool FULL> void walk_shape(const Walk& w, Kind kind
     }
 }
 
-template <int TY> hipError_t launch_walk(const Walk& w, const Shape& s, Kind kind, bool back, hipStream_t stream) {
-    if (s.steps == 1) s.full ? walk_shape<TY, 1, true>(w, kind, back, stream) : walk_shape<TY, 1, false>(w, kind, back, stream);
-    else if (s.steps == 2) s.full ? walk_shape<TY, 2, true>(w, kind, back, stream) : walk_shape<TY, 2, false>(w, kind, back, stream);
-    else s.full ? walk_shape<TY, 4, true>(w, kind, back, stream) : walk_shape<TY, 4, false>(w, kind, back, stream);
+template <int TY> hipError_t launch_walk(const Walk& w, Kind kind, bool back, hipStream_t stream) {
+    const int steps = steps_of(w.da);
+    const bool full = full_of(w);
+    if (steps == 1) full ? walk_shape<TY, 1, true>(w, kind, back, stream) : walk_shape<TY, 1, false>(w, kind, back, stream);
+    else if (steps == 2) full ? walk_shape<TY, 2, true>(w, kind, back, stream) : walk_shape<TY, 2, false>(w, kind, back, stream);
+    else full ? walk_shape<TY, 4, true>(w, kind, back, stream) : walk_shape<TY, 4, false>(w, kind, back, stream);
+    return hipGetLastError();
+}
+
+template <int TY> hipError_t launch_gradients(const Walk& v, const Walk& k, const Walk& q, hipStream_t stream) {
+    const Walks w{v, k, q};
+    const dim3 grid = walk_grid((uint64_t)v.batch * v.heads * v.segments * (v.blocks + k.blocks + q.blocks));
+    const int steps = std::max(steps_of(v.da), steps_of(k.da));
+    const bool full = full_of(v) && full_of(k) && steps_of(v.da) == steps_of(k.da);
+    if (steps == 1) full ? linear_gradients_kernel<TY, 1, true><<<grid, 256, 0, stream>>>(w) : linear_gradients_kernel<TY, 1, false><<<grid, 256, 0, stream>>>(w);
+    else if (steps == 2) full ? linear_gradients_kernel<TY, 2, true><<<grid, 256, 0, stream>>>(w) : linear_gradients_kernel<TY, 2, false><<<grid, 256, 0, stream>>>(w);
+    else full ? linear_gradients_kernel<TY, 4, true><<<grid, 256, 0, stream>>>(w) : linear_gradients_kernel<TY, 4, false><<<grid, 256, 0, stream>>>(w);
     return hipGetLastError();
 }
 
