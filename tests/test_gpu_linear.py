@@ -262,7 +262,9 @@ def test_a_state_that_is_not_finite_passes_no_reset():
         for bad in (float("nan"), float("inf")):
             x["state"] = torch.full_like(keep, bad)
             o, last = ours(**x)
-            assert torch.equal(o[:, t:], want[0][:, t:]) and torch.equal(last, want[1])
+            # Token by token where the reset is: the same terms in another order, each sum within the tolerance.
+            assert_near(o[:, t:], want[0][:, t:], 2 * tolerance(70, 32, 32), "o")
+            assert_near(last, want[1], 2 * tolerance(70, 32, 32), "state")
             state = torch.full_like(keep, bad)
             linear_attention_step(*(x[n][:, 0] for n in "qkv"), x["g"], state, torch.ones(1, dtype=torch.bool, device="cuda"))
             assert torch.isfinite(state).all()

@@ -22,8 +22,10 @@
 // N <- exp(g) (N + S), the state's derivative, beside the state, it is a sum over tokens of q . (A N) and
 // of products inside the chunk. No difference is taken, so heads that forget fast keep their digits.
 //
-// A chunk that holds a value that is not finite goes token by token, so that none meets an output before
-// its token, or behind a reset, by way of the zeros in P.
+// A chunk that holds a value that is not finite goes token by token on the vector units, so that none meets an output
+// before its token, or behind a reset, by way of the zeros in P, or another column by way of those in the unit matrix.
+// There is one body for the chunk: with others for resets and for odd values beside it the compiler needed 168 registers
+// and spilled where 100 do.
 #pragma once
 #include <algorithm>
 #include <type_traits>
@@ -53,6 +55,14 @@ template <int TY> __device__ __forceinline__ Frag<Elem<TY>::parts> operand(const
     return f;
 }
 
+// Four of the eight values a lane has of a row.
+template <int P> __device__ __forceinline__ Half<P> four_of(const Frag<P>& f, int i) {
+    Half<P> h;
+#pragma unroll
+    for (int p = 0; p < P; ++p) h.p[p] = i ? u2{f.p[p][2], f.p[p][3]} : u2{f.p[p][0], f.p[p][1]};
+    return h;
+}
+
 // Four floats at any address, the first `n` of them in bounds.
 template <bool FULL> __device__ __forceinline__ f4 load_floats(const float* at, int n) {
     if (FULL || n >= 4) return __builtin_bit_cast(f4, reinterpret_cast<const Loose<T_F32>::U*>(at)->v);
@@ -72,6 +82,13 @@ template <bool FULL> __device__ __forceinline__ void store_floats(float* at, int
     }
 }
 
+// This lane's number, found anew: what depends on it is then not kept in registers from use to use.
+__device__ __forceinline__ int lane_anew() {
+    int m;
+    asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(m));
+    return m;
+}
+
 // One walk of one wave: of 32 columns of the state (JS 2), or of 16 of them (JS 1: tile `half` of the pair), in
 // one segment of one head.
 template <int TY, int STEPS, int JS, bool BACK, int KIND, bool FULL>
@@ -87,11 +104,12 @@ __device__ __forceinline__ void walk(const Walk& a, const uint32_t bh, const uin
     const int begin = segment * a.segment_length, T = begin + min(a.length - begin, a.segment_length);
     const int col0 = block * 32;
     const int da = a.da, dc = a.dc - col0;
-    auto row_of = [&](const Rows& x, int e) { return (const E*)x.at + b * x.stride[0] + (h / x.share) * x.stride[2] + e + 8 * g; };
-    const E* ap = READ ? row_of(a.a, 0) : nullptr;
-    const E* bp = row_of(a.b, 0);
-    const E* cp = row_of(a.c, col0);
-    const E* qp = GRAD ? row_of(a.q, col0) : nullptr;
+    float gh = a.g[h];  // before anything else, as loads come back in order
+    auto rows_of = [&](const Rows& x) { return (const E*)x.at + b * x.stride[0] + (h / x.share) * x.stride[2]; };
+    const E* ap = READ ? rows_of(a.a) : nullptr;
+    const E* bp = rows_of(a.b);
+    const E* cp = rows_of(a.c) + col0;
+    const E* qp = GRAD ? rows_of(a.q) + col0 : nullptr;
     const uint8_t* rp = a.reset ? a.reset + b * a.reset_stride[0] : nullptr;
 
     // ---- what a chunk reads: token n's dimensions 8 g to 8 g + 7 of every 32
@@ -99,17 +117,18 @@ __device__ __forceinline__ void walk(const Walk& a, const uint32_t bh, const uin
     bool cut = false, any_cut = false;
     auto fetch = [&](int t, int rows) {
         cut = rp && lane < rows && rp[(t + lane) * a.reset_stride[1]];
-        const int64_t tok = t + min(n, rows - 1);
-        const E* x = bp + tok * a.b.stride[1];
+        const int row = min(n, rows - 1);
+        auto place = [&](const E* x, const Rows& r) { return x + t * r.stride[1] + (row * r.stride[1] + 8 * g); };
+        const E* x = place(bp, a.b);
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) br[s].template load<FULL>(x + 32 * s, da - 32 * s - 8 * g);
         if constexpr (READ) {
-            x = ap + tok * a.a.stride[1];
+            x = place(ap, a.a);
 #pragma unroll
             for (int s = 0; s < STEPS; ++s) ar[s].template load<FULL>(x + 32 * s, da - 32 * s - 8 * g);
         }
-        cr.template load<FULL>(cp + tok * a.c.stride[1], dc - 8 * g);
-        if constexpr (GRAD) qr.template load<FULL>(qp + tok * a.q.stride[1], dc - 8 * g);
+        cr.template load<FULL>(place(cp, a.c), dc - 8 * g);
+        if constexpr (GRAD) qr.template load<FULL>(place(qp, a.q), dc - 8 * g);
     };
     auto bounds = [&](int at, int& t, int& rows) {  // the chunk of the grid that `at` is in, from it (or up to it) on
         if (BACK) {
@@ -129,9 +148,8 @@ __device__ __forceinline__ void walk(const Walk& a, const uint32_t bh, const uin
     // A lane takes four values that lie side by side: of one of four rows, which four lanes then exchange, or of a
     // column where columns lie side by side (`turned`). Places are found anew each time: kept from the walk's begin
     // to its end they would not fit the registers.
-    auto each_four = [&](int m, auto&& access) {
-        asm volatile("" : "+v"(m));
-        const int mn = m & 15, mg = m >> 4;
+    auto each_four = [&](auto&& access) {
+        const int m = lane_anew(), mn = m & 15, mg = m >> 4;
         const int mine = a.turned ? (8 * (mn >> 2) + (mn & 3)) * a.ld + 8 * mg : (8 * mg + (mn & 3)) * a.ld + 8 * (mn >> 2);
 #pragma unroll
         for (int i = 0; i < 2 * STEPS; ++i)
@@ -152,88 +170,61 @@ __device__ __forceinline__ void walk(const Walk& a, const uint32_t bh, const uin
         for (int i = 0; i < 2 * STEPS; ++i)
 #pragma unroll
             for (int j = 0; j < JS; ++j) X[i][j] = f4{0, 0, 0, 0};
-        if (!from) return;
-        each_four(lane, [&](int i, int j, int base, int mine, int left) { X[i][j] = load_floats<FULL>(from + base + mine, left); });
+        if (from) each_four([&](int i, int j, int base, int mine, int left) { X[i][j] = load_floats<FULL>(from + base + mine, left); });
+    };
+    auto turn_state = [&](auto& X) {
         if (a.turned) return;
+        const int m = lane_anew();
 #pragma unroll
         for (int i = 0; i < 2 * STEPS; ++i)
 #pragma unroll
-            for (int j = 0; j < JS; ++j) X[i][j] = turn(X[i][j], lane);
+            for (int j = 0; j < JS; ++j) X[i][j] = turn(X[i][j], m);
     };
     auto store_state = [&](auto& X, float* to) {
-        if (!a.turned)
-#pragma unroll
-            for (int i = 0; i < 2 * STEPS; ++i)
-#pragma unroll
-                for (int j = 0; j < JS; ++j) X[i][j] = turn(X[i][j], lane);
-        each_four(lane, [&](int i, int j, int base, int mine, int left) { store_floats<FULL>(to + base + mine, left, X[i][j]); });
+        turn_state(X);
+        each_four([&](int i, int j, int base, int mine, int left) { store_floats<FULL>(to + base + mine, left, X[i][j]); });
     };
     const bool at_first = BACK ? segment == a.segments - 1 : segment == 0;
     const int64_t between = (int64_t)bh * (a.segments - 1) + (BACK ? segment : segment - 1);  // the start of this walk
     load_state(S, at_first ? (a.first ? a.first + bh * a.size : nullptr) : READ ? a.starts + between * a.size : nullptr);
     if constexpr (SLOPE) load_state(N, READ && !at_first ? a.slopes + between * a.size : nullptr);
 
-    // ---- the head's decays. `read`: of the state to a token, `write`: of a token to the next state.
-    float gh = a.g[h];
+    // ---- the head's decays between the tokens of a chunk of `len` with resets in `cuts`; 0 across a reset, and where
+    // a token is behind the other. `read`: of the state to a token, `write`: of a token to the next state, `all`: of
+    // the state to the next.
     gh = gh < -200.0f ? -200.0f : gh;  // 0 in fp32 from one token to the next
-    float near[4], read = 0.0f, all = 0.0f;
+    float near[4], read, all;
     f4 write;
-    int measured = -1;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        near[r] = a.scale * decay(gh, max(BACK ? 4 * g + r - n : n - 4 * g - r, 0));
-        if (BACK) write[r] = a.scale * decay(gh, 4 * g + r + 1);
-    }
-    if (!BACK) read = a.scale * decay(gh, n + 1);
-    auto measure = [&](int len) {  // those that depend on the chunk's length
+    int measured = 0;
+    uint32_t measured_cuts = 0;
+    auto measure = [&](int len, uint32_t cuts) {
         measured = len;
-        all = decay(gh, len);
-        if (BACK) read = decay(gh, max(len - 1 - n, 0));
+        measured_cuts = cuts;
+        const int m = lane_anew(), i = m & 15, j0 = 4 * (m >> 4);
+        const int last = cuts ? 31 - __builtin_clz(cuts) : -1, first = cuts ? __builtin_ctz(cuts) : C;
+        const int before = 31 - __clz((int)(cuts & (0xffffu >> (15 - i))));  // the last reset up to this lane's token
+        all = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(cuts ? 0.0f : decay(gh, len))));
+        read = BACK ? (i >= last ? decay(gh, max(len - 1 - i, 0)) : 0.0f) : before < 0 ? a.scale * decay(gh, i + 1) : 0.0f;
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-            if (!BACK) write[r] = decay(gh, max(len - 1 - 4 * g - r, 0));
+        for (int r = 0; r < 4; ++r) {
+            const int j = j0 + r, between = BACK ? 31 - __clz((int)(cuts & (0xffffu >> (15 - j)))) : before;
+            near[r] = (BACK ? j >= i && i >= between : j <= i && j >= between) ? a.scale * decay(gh, max(BACK ? j - i : i - j, 0)) : 0.0f;
+            write[r] = BACK ? (j < first ? a.scale * decay(gh, j + 1) : 0.0f) : j >= last ? decay(gh, max(len - 1 - j, 0)) : 0.0f;
+        }
     };
 
-    // ---- unit matrices as operands: they pick dimension 8 (n / 4) + 4 i + n % 4 of a row's 32
-    Frag<1> unit_of[2];
+    // A unit matrix as an operand. With four of a lane's eight values (dimensions 8 g + 4 i + 0..3 of a row's 32) it
+    // gives a tile whose column n is dimension 8 (n / 4) + 4 i + n % 4.
+    Half<1> unit_matrix;
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            const int e = 4 * i + (n & 3);
-            unit_of[i].p[0][w] = g == (n >> 2) && (e >> 1) == w ? 0x3f80u << (16 * (e & 1)) : 0u;
-        }
+    for (int w = 0; w < 2; ++w) unit_matrix.p[0][w] = g == (n >> 2) && ((n & 3) >> 1) == w ? 0x3f80u << (16 * (n & 1)) : 0u;
     double dg = 0.0;
 
-    // The chunk of tokens t to t + len. CUTS: there may be resets inside, in `cuts`. ODD: one token, with values
-    // that are not finite: its operands along the tokens are read one by one. No branch is inside: where one lies
-    // between a matrix instruction and the use of its result, the compiler has been seen to leave out the wait. The
-    // scheduler is kept from starting everything at once, which takes more registers than there are.
-    auto chunk = [&](auto with_cuts, auto is_odd, int t, int len, uint32_t cuts) {
-        constexpr bool CUTS = decltype(with_cuts)::value, ODD = decltype(is_odd)::value;
+    // The chunk of tokens t to t + len. No branch is inside: where one lies between a matrix instruction and the use of
+    // its result, the compiler has been seen to leave out the wait. The scheduler is kept from starting everything at
+    // once, which takes more registers than there are.
+    auto chunk = [&](int t, int len) {
         const f4 zero = {0, 0, 0, 0};
-
-        // Resets: the last one up to a token (this lane's, and those of its registers), and of the chunk.
-        int mine = -1, theirs[4], last_cut = -1, first_cut = C;
-        if constexpr (CUTS) {
-            last_cut = cuts ? 31 - __builtin_clz(cuts) : -1;
-            first_cut = cuts ? __builtin_ctz(cuts) : C;
-            mine = 31 - __clz((int)(cuts & (0xffffu >> (15 - n))));
-#pragma unroll
-            for (int r = 0; r < 4; ++r) theirs[r] = 31 - __clz((int)(cuts & (0xffffu >> (15 - 4 * g - r))));
-        }
-        f4 odd_b[2 * STEPS], odd_c[2];
-        if constexpr (ODD) {
-            const int e = 8 * (n >> 2) + (n & 3) - 8 * g;  // from this lane's place in its rows to the dimension that it stands for
-#pragma unroll
-            for (int i = 0; i < 2 * STEPS; ++i) {
-                const int x = 32 * (i >> 1) + 4 * (i & 1);
-                odd_b[i] = f4{g == 0 && x + e < da ? Elem<TY>::get(bp[t * a.b.stride[1] + x + e]) : 0.0f, 0, 0, 0};
-            }
-#pragma unroll
-            for (int j = 0; j < 2; ++j) odd_c[j] = f4{g == 0 && 4 * j + e < dc ? Elem<TY>::get(cp[t * a.c.stride[1] + 4 * j + e]) : 0.0f, 0, 0, 0};
-        }
-
         // ---- P transposed (row j = 4 g + r, column i = n), and B along the tokens
         Frag<NP> af[STEPS];
         Half<NP> bt[2 * STEPS];
@@ -246,7 +237,7 @@ __device__ __forceinline__ void walk(const Walk& a, const uint32_t bh, const uin
                 p = mul<2>(bf, af[s], p);
             }
 #pragma unroll
-            for (int i = 0; i < 2; ++i) bt[2 * s + i] = split<NP>(ODD ? odd_b[2 * s + i] : mul<2>(bf, unit_of[i], zero));
+            for (int i = 0; i < 2; ++i) bt[2 * s + i] = split<NP>(mul<2>(four_of(bf, i), unit_matrix, zero));
             __builtin_amdgcn_sched_barrier(0);
         }
         const Frag<NP> cf = operand(cr);
@@ -256,11 +247,8 @@ __device__ __forceinline__ void walk(const Walk& a, const uint32_t bh, const uin
             if constexpr (GRAD) y = mul<2>(cf, operand(qr), zero);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int i = n, j = 4 * g + r;
-                // A product that is not finite does not pass the zeros either.
-                p[r] = (BACK ? j >= i : j <= i) ? p[r] * near[r] : 0.0f;
-                if (CUTS) p[r] = (BACK ? i >= theirs[r] : j >= mine) ? p[r] : 0.0f;
-                if (GRAD) pairs += (float)(i - j) * p[r] * y[r];
+                p[r] = near[r] != 0.0f ? p[r] * near[r] : 0.0f;  // a product that is not finite does not pass the zeros
+                if (GRAD) pairs += (float)(n - 4 * g - r) * p[r] * y[r];
             }
             P = split<KEPT>(p);
         }
@@ -269,19 +257,17 @@ __device__ __forceinline__ void walk(const Walk& a, const uint32_t bh, const uin
 #pragma unroll
         for (int j = 0; j < JS; ++j) {
             __builtin_amdgcn_sched_barrier(0);
-            const f4 odd = ODD ? (JS == 2 ? odd_c[j] : half ? odd_c[1] : odd_c[0]) : zero;
-            Frag<1> pick = unit_of[JS == 2 ? j : 0];
+            Half<NP> cj = four_of(cf, j);
             if (JS == 1)
 #pragma unroll
-                for (int w = 0; w < 4; ++w) pick.p[0][w] = half ? unit_of[1].p[0][w] : unit_of[0].p[0][w];
-            const f4 ct = ODD ? odd : mul<2>(cf, pick, zero);
+                for (int p = 0; p < NP; ++p) cj.p[p] = half ? four_of(cf, 1).p[p] : cj.p[p];
+            const f4 ct = mul<2>(cj, unit_matrix, zero);
             if constexpr (READ) {
-                const bool reach = !CUTS || (BACK ? n >= last_cut : mine < 0);
                 f4 x = zero;
 #pragma unroll
                 for (int s = 0; s < STEPS; ++s) x = mul<2>(split<KEPT>(S[2 * s][j], S[2 * s + 1][j]), af[s], x);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) x[r] = reach ? x[r] * read : 0.0f;
+                for (int r = 0; r < 4; ++r) x[r] = read != 0.0f ? x[r] * read : 0.0f;
                 if constexpr (GRAD) {
                     f4 slope = zero;
 #pragma unroll
@@ -290,7 +276,7 @@ __device__ __forceinline__ void walk(const Walk& a, const uint32_t bh, const uin
                     qr.get(q);
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
-                        pairs += ((float)(n + 1) * x[r] + (reach ? slope[r] * read : 0.0f)) * (JS == 2 ? q[4 * j + r] : half ? q[4 + r] : q[r]);
+                        pairs += ((float)(n + 1) * x[r] + (read != 0.0f ? slope[r] * read : 0.0f)) * (JS == 2 ? q[4 * j + r] : half ? q[4 + r] : q[r]);
                 } else {
                     x = mul<2>(split<NP>(ct), P, x);
 #pragma unroll
@@ -299,30 +285,21 @@ __device__ __forceinline__ void walk(const Walk& a, const uint32_t bh, const uin
             }
             // ---- the state behind the chunk
             __builtin_amdgcn_sched_barrier(0);
-            f4 w;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) w[r] = !CUTS || (BACK ? 4 * g + r < first_cut : 4 * g + r >= last_cut) ? ct[r] * write[r] : 0.0f;
+            f4 w = ct * write;
             const Half<3> wf = split<3>(w);
             if constexpr (SLOPE) {
 #pragma unroll
                 for (int r = 0; r < 4; ++r) w[r] *= (float)max(len - 1 - 4 * g - r, 0);
                 const Half<3> nf = split<3>(w);
 #pragma unroll
-                for (int i = 0; i < 2 * STEPS; ++i) {
-                    f4 x = (N[i][j] + S[i][j] * (float)len) * all;
-                    if (CUTS) x = cuts ? zero : x;
-                    N[i][j] = mul<2>(bt[i], nf, x);
-                }
+                for (int i = 0; i < 2 * STEPS; ++i) N[i][j] = mul<2>(bt[i], nf, (N[i][j] + S[i][j] * (float)len) * all);
             }
 #pragma unroll
-            for (int i = 0; i < 2 * STEPS; ++i) {
-                f4 x = S[i][j] * all;
-                if (CUTS) x = cuts ? zero : x;
-                S[i][j] = mul<2>(bt[i], wf, x);
-            }
+            for (int i = 0; i < 2 * STEPS; ++i) S[i][j] = mul<2>(bt[i], wf, S[i][j] * all);
         }
         if constexpr (OUT) {
-            const int64_t to = b * a.out_stride[0] + (t + n) * a.out_stride[1] + (h / a.out_share) * a.out_stride[2] + col0 + 8 * g;
+            const int l = lane_anew();
+            const int64_t to = (b * a.out_stride[0] + (h / a.out_share) * a.out_stride[2] + t * a.out_stride[1] + col0) + ((l & 15) * a.out_stride[1] + 8 * (l >> 4));
             if (n < len) {
                 if (a.out_f32) {
                     Eight<T_F32> x;
@@ -338,9 +315,82 @@ __device__ __forceinline__ void walk(const Walk& a, const uint32_t bh, const uin
         if (GRAD) dg += (double)pairs;
     };
 
-    // ---- the walk. Nothing is fetched ahead: a third wave a SIMD, for which that leaves no registers, hides more.
+    // Tokens one by one, without the matrix units: of values that are not finite their zeros would make NaN where the
+    // definition has none. The state goes through memory, so that this rare path takes no registers from the other.
+    auto tokens = [&](int t, int rows, uint32_t cuts) {
+        volatile float kept[SLOPE ? 2 : 1][2 * STEPS][4][JS];
+#pragma unroll
+        for (int i = 0; i < 2 * STEPS; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int j = 0; j < JS; ++j) {
+                    kept[0][i][r][j] = S[i][j][r];
+                    if (SLOPE) kept[SLOPE][i][r][j] = N[i][j][r];
+                }
+        const int m = lane_anew();
+        const float fade = decay(gh, 1.0f);
+#pragma unroll 1
+        for (int k = 0; k < rows; ++k) {
+            const int row = BACK ? rows - 1 - k : k;
+            const int64_t tok = t + row;
+            const bool cut = cuts >> row & 1;
+            float o[JS], v[JS], slope[JS];
+            int c[JS];
+#pragma unroll
+            for (int j = 0; j < JS; ++j) {
+                c[j] = 8 * (m >> 2 & 3) + (m & 3) + 4 * (JS == 2 ? j : half);
+                v[j] = (c[j] < dc ? Elem<TY>::get(cp[tok * a.c.stride[1] + c[j]]) : 0.0f) * (BACK ? a.scale : 1.0f);
+                o[j] = slope[j] = 0.0f;
+            }
+#pragma unroll 1
+            for (int i = 0; i < 8 * STEPS; ++i) {
+                const int d = 32 * (i >> 3) + 8 * (m >> 4) + (i & 7);
+                const float B = d < da ? Elem<TY>::get(bp[tok * a.b.stride[1] + d]) : 0.0f;
+                const float A = READ && d < da ? Elem<TY>::get(ap[tok * a.a.stride[1] + d]) : 0.0f;
+#pragma unroll
+                for (int j = 0; j < JS; ++j) {
+                    float x = kept[0][i >> 2][i & 3][j];
+                    if constexpr (SLOPE) {
+                        const float y = cut ? 0.0f : fade * (kept[1][i >> 2][i & 3][j] + x);
+                        kept[1][i >> 2][i & 3][j] = y;
+                        slope[j] += y * A;
+                    }
+                    if (!BACK) x = cut ? 0.0f : fade * x;
+                    x += B * v[j];
+                    o[j] += x * A;
+                    if (BACK) x = cut ? 0.0f : fade * x;
+                    kept[0][i >> 2][i & 3][j] = x;
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < JS; ++j) {
+                o[j] += __shfl_xor(o[j], 16);
+                o[j] += __shfl_xor(o[j], 32);
+                if (OUT && m < 16 && c[j] < dc) {
+                    const int64_t to = b * a.out_stride[0] + (h / a.out_share) * a.out_stride[2] + tok * a.out_stride[1] + col0 + c[j];
+                    const float y = o[j] * (BACK ? 1.0f : a.scale);
+                    if (a.out_f32) ((float*)a.out)[to] = y;
+                    else ((E*)a.out)[to] = Elem<TY>::put(y);
+                }
+                if constexpr (GRAD)
+                    if (c[j] < dc && !cut) dg += (double)(a.scale * slope[j] * Elem<TY>::get(qp[tok * a.q.stride[1] + c[j]]));
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 2 * STEPS; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int j = 0; j < JS; ++j) {
+                    S[i][j][r] = kept[0][i][r][j];
+                    if (SLOPE) N[i][j][r] = kept[SLOPE][i][r][j];
+                }
+    };
+
+    // ---- the walk. Nothing is fetched ahead: more waves a SIMD, for which that leaves no registers, hide more.
+    bool turned = false;
     while (true) {
-        int len = rows, first = t;
         bool fine = cr.finite();
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) {
@@ -348,20 +398,11 @@ __device__ __forceinline__ void walk(const Walk& a, const uint32_t bh, const uin
             if constexpr (READ) fine &= ar[s].finite();
         }
         if constexpr (GRAD) fine &= qr.finite();
-        uint32_t cuts = (uint32_t)__ballot(cut);
-        const bool odd = __ballot(!fine) != 0;
-        if (odd) {
-            if (BACK && rows > 1) {  // the last token of the chunk first
-                first = at - 1;
-                fetch(first, 1);
-                cuts = (uint32_t)__ballot(cut);
-            }
-            cuts &= 1;
-            len = 1;
-        }
+        const uint32_t cuts = (uint32_t)__ballot(cut);
         any_cut |= cuts != 0;
-        if (len < C) {
-            const bool keep = n < len;
+        if (rows != measured || cuts != measured_cuts) measure(rows, cuts);
+        if (rows < C) {
+            const bool keep = n < rows;
 #pragma unroll
             for (int s = 0; s < STEPS; ++s) {
                 br[s].keep(keep);
@@ -370,13 +411,22 @@ __device__ __forceinline__ void walk(const Walk& a, const uint32_t bh, const uin
             cr.keep(keep);
             if constexpr (GRAD) qr.keep(keep);
         }
-        if (len != measured) measure(len);
-        constexpr std::true_type yes{};
-        constexpr std::false_type no{};
-        if (odd) chunk(yes, yes, first, len, cuts);
-        else if (cuts) chunk(yes, no, first, len, cuts);
-        else chunk(no, no, first, len, cuts);
-        at = BACK ? first : first + len;
+        if (!turned) {  // the state arrives after the first rows and decays
+            turn_state(S);
+            if constexpr (SLOPE) turn_state(N);
+            turned = true;
+        }
+        if (cuts)  // nothing of the state passes: it must not be multiplied by zero if it is not finite
+#pragma unroll
+            for (int i = 0; i < 2 * STEPS; ++i)
+#pragma unroll
+                for (int j = 0; j < JS; ++j) {
+                    fine &= finite(S[i][j]);
+                    if constexpr (SLOPE) fine &= finite(N[i][j]);
+                }
+        if (__ballot(!fine)) tokens(t, rows, cuts);
+        else chunk(t, rows);
+        at = BACK ? t : t + rows;
         if (BACK ? at <= begin : at >= T) break;
         bounds(at, t, rows);
         fetch(t, rows);
@@ -388,6 +438,7 @@ __device__ __forceinline__ void walk(const Walk& a, const uint32_t bh, const uin
     } else if constexpr (GRAD) {
         if (a.d_last && segment == a.segments - 1) {
             load_state(S, a.d_last + bh * a.size);
+            turn_state(S);
 #pragma unroll
             for (int i = 0; i < 2 * STEPS; ++i)
 #pragma unroll
@@ -414,7 +465,7 @@ __device__ __forceinline__ uint32_t unit_of_wave() {
 }
 
 // Waves a SIMD that the registers are cut down to: as many as the state, its rows and their operands bear.
-constexpr int walk_waves(int type, int steps, int kind) { return steps == 4 || (steps == 2 && type == T_F32) ? 2 : 3; }
+constexpr int walk_waves(int type, int steps, int kind) { return type == T_F32 ? (steps == 4 && (kind == OUTPUTS || kind == SLOPES) ? 1 : steps == 1 ? 3 : 2) : steps == 4 ? 2 : kind == SLOPES || type == T_F16 ? 3 : 4; }
 
 template <int TY, int STEPS, int JS, bool BACK, int KIND, bool FULL>
 __global__ __launch_bounds__(256, walk_waves(TY, STEPS, KIND)) void linear_walk_kernel(const Walk a) {
