@@ -201,15 +201,25 @@ __device__ __forceinline__ void walk(const Walk& a, const uint32_t bh, const uin
         measured = len;
         measured_cuts = cuts;
         const int m = lane_anew(), i = m & 15, j0 = 4 * (m >> 4);
-        const int last = cuts ? 31 - __builtin_clz(cuts) : -1, first = cuts ? __builtin_ctz(cuts) : C;
-        const int before = 31 - __clz((int)(cuts & (0xffffu >> (15 - i))));  // the last reset up to this lane's token
-        all = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(cuts ? 0.0f : decay(gh, len))));
-        read = BACK ? (i >= last ? decay(gh, max(len - 1 - i, 0)) : 0.0f) : before < 0 ? a.scale * decay(gh, i + 1) : 0.0f;
+        all = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(decay(gh, len))));
+        read = BACK ? decay(gh, max(len - 1 - i, 0)) : a.scale * decay(gh, i + 1);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const int j = j0 + r, between = BACK ? 31 - __clz((int)(cuts & (0xffffu >> (15 - j)))) : before;
-            near[r] = (BACK ? j >= i && i >= between : j <= i && j >= between) ? a.scale * decay(gh, max(BACK ? j - i : i - j, 0)) : 0.0f;
-            write[r] = BACK ? (j < first ? a.scale * decay(gh, j + 1) : 0.0f) : j >= last ? decay(gh, max(len - 1 - j, 0)) : 0.0f;
+            const int j = j0 + r, apart = BACK ? j - i : i - j;
+            near[r] = apart < 0 ? 0.0f : a.scale * decay(gh, max(apart, 0));
+            write[r] = BACK ? a.scale * decay(gh, j + 1) : decay(gh, max(len - 1 - j, 0));
+        }
+        if (cuts) {
+            const int last = 31 - __builtin_clz(cuts), first = __builtin_ctz(cuts);
+            auto reset_to = [&](int token) { return 31 - __clz((int)(cuts & (0xffffu >> (15 - token)))); };  // the last one up to it
+            all = 0.0f;
+            if (BACK ? i < last : reset_to(i) >= 0) read = 0.0f;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int j = j0 + r;
+                if (BACK ? j >= first : j < last) write[r] = 0.0f;
+                if (BACK ? i < reset_to(j) : j < reset_to(i)) near[r] = 0.0f;
+            }
         }
     };
 
