@@ -51,12 +51,11 @@ struct Walk {
     float *starts, *slopes, *passes;
     const float* d_last;         // for the gradient of g; null: zeros
     double* parts;               // of it: [batch, heads, segments, blocks, 2]
-    uint32_t blocks;             // of 32 columns
+    uint32_t blocks;             // waves that share the columns, set at the launch
 };
 
-// Launch shape: a wave holds 32 times 1, 2 or 4 rows of a state; full: of exactly so many, and of whole blocks.
+// A wave holds 32 times 1, 2 or 4 rows of a state.
 inline int steps_of(int da) { return da <= 32 ? 1 : da <= 64 ? 2 : 4; }
-inline bool full_of(const Walk& w) { return w.da == 32 * steps_of(w.da) && w.dc % 32 == 0; }
 struct Segments {
     uint32_t count;
     int length;
@@ -70,8 +69,8 @@ uint64_t workspace_floats(const ZenoAmdLinearInputs& in, bool train);
 enum Kind { OUTPUTS, SLOPES, STATES, STATES_SLOPE };
 
 // One translation unit per element type.
-template <int TY> hipError_t launch_walk(const Walk& w, Kind kind, bool back, hipStream_t stream);
-template <int TY> hipError_t launch_gradients(const Walk& v, const Walk& k, const Walk& q, hipStream_t stream);
+template <int TY> hipError_t launch_walk(Walk w, Kind kind, bool back, hipStream_t stream);
+template <int TY> hipError_t launch_gradients(Walk v, Walk k, Walk q, hipStream_t stream);
 template <int TY> hipError_t launch_share(const float* parts, void* out, const int64_t* stride, uint32_t batch, uint32_t length, uint32_t key_heads, uint32_t share,
                                           uint32_t dim, hipStream_t stream);
 template <int TY> hipError_t launch_step(const ZenoAmdLinearInputs& in, void* o, const int64_t* o_stride, float* state, hipStream_t stream);

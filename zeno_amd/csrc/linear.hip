@@ -66,7 +66,6 @@ Walk walk_of(const ZenoAmdLinearInputs& in, bool turned) {
     Walk w{};
     w.da = turned ? in.value_dim : in.key_dim;
     w.dc = turned ? in.key_dim : in.value_dim;
-    w.blocks = blocks_of(w.dc);
     w.ld = in.value_dim;
     w.turned = turned;
     w.size = state_size(in);
@@ -242,7 +241,7 @@ hipError_t backward(const ZenoAmdLinearInputs& in, const float* saved, const Zen
     if ((e = gradients(wv, wk, wq, stream))) return e;
     if (grad.d_g) {
         if ((e = launch(in.dtype, wq, SLOPES, false, stream))) return e;
-        linear_decay_kernel<<<in.value_heads, 256, 0, stream>>>(wq.parts, in.batch, in.value_heads, wq.segments * 2 * wq.blocks, grad.d_g);
+        linear_decay_kernel<<<in.value_heads, 256, 0, stream>>>(wq.parts, in.batch, in.value_heads, wq.segments * 2 * blocks_of(in.key_dim), grad.d_g);
     }
     if (share > 1) {
         auto add = in.dtype == T_F32 ? launch_share<T_F32> : in.dtype == T_F16 ? launch_share<T_F16> : launch_share<T_BF16>;

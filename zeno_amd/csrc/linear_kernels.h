@@ -22,12 +22,14 @@
 // N <- exp(g) (N + S), the state's derivative, beside the state, it is a sum over tokens of q . (A N) and
 // of products inside the chunk. No difference is taken, so heads that forget fast keep their digits.
 //
-// A chunk that holds a value that is not finite goes token by token on the vector units, so that none meets an output
-// before its token, or behind a reset, by way of the zeros in P, or another column by way of those in the unit matrix.
+// From a chunk on that holds a value that is not finite, a walk goes token by token on the vector units, so that none
+// meets an output before its token, or behind a reset, by way of the zeros in P, or another column by way of those in
+// the unit matrix.
 // There is one body for the chunk: with others for resets and for odd values beside it the compiler needed 168 registers
 // and spilled where 100 do.
 #pragma once
 #include <algorithm>
+#include <initializer_list>
 #include <type_traits>
 
 #include "linear.h"
@@ -89,8 +91,8 @@ __device__ __forceinline__ int lane_anew() {
     return m;
 }
 
-// One walk of one wave: of 32 columns of the state (JS 2), or of 16 of them (JS 1: tile `half` of the pair), in
-// one segment of one head.
+// One walk of one wave in one segment of one head: of 64 or 32 columns of the state (JS 4 or 2 tiles of 16), or of
+// every other four of 32 (JS 1: tile `half` of the pair).
 template <int TY, int STEPS, int JS, bool BACK, int KIND, bool FULL>
 __device__ __forceinline__ void walk(const Walk& a, const uint32_t bh, const uint32_t segment, const int block, const int half, const uint32_t unit) {
     typedef typename Elem<TY>::type E;
@@ -102,7 +104,8 @@ __device__ __forceinline__ void walk(const Walk& a, const uint32_t bh, const uin
     const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
     const int64_t b = bh / a.heads, h = bh % a.heads;
     const int begin = segment * a.segment_length, T = begin + min(a.length - begin, a.segment_length);
-    const int col0 = block * 32;
+    constexpr int U = (JS + 1) / 2;  // times 32 columns
+    const int col0 = block * 32 * U;
     const int da = a.da, dc = a.dc - col0;
     float gh = a.g[h];  // before anything else, as loads come back in order
     auto rows_of = [&](const Rows& x) { return (const E*)x.at + b * x.stride[0] + (h / x.share) * x.stride[2]; };
@@ -113,7 +116,7 @@ __device__ __forceinline__ void walk(const Walk& a, const uint32_t bh, const uin
     const uint8_t* rp = a.reset ? a.reset + b * a.reset_stride[0] : nullptr;
 
     // ---- what a chunk reads: token n's dimensions 8 g to 8 g + 7 of every 32
-    Eight<TY> ar[STEPS], br[STEPS], cr, qr;
+    Eight<TY> ar[STEPS], br[STEPS], cr[U], qr;
     bool cut = false, any_cut = false;
     auto fetch = [&](int t, int rows) {
         cut = rp && lane < rows && rp[(t + lane) * a.reset_stride[1]];
@@ -127,7 +130,9 @@ __device__ __forceinline__ void walk(const Walk& a, const uint32_t bh, const uin
 #pragma unroll
             for (int s = 0; s < STEPS; ++s) ar[s].template load<FULL>(x + 32 * s, da - 32 * s - 8 * g);
         }
-        cr.template load<FULL>(place(cp, a.c), dc - 8 * g);
+        x = place(cp, a.c);
+#pragma unroll
+        for (int u = 0; u < U; ++u) cr[u].template load<FULL>(x + 32 * u, dc - 32 * u - 8 * g);
         if constexpr (GRAD) qr.template load<FULL>(place(qp, a.q), dc - 8 * g);
     };
     auto bounds = [&](int at, int& t, int& rows) {  // the chunk of the grid that `at` is in, from it (or up to it) on
@@ -155,7 +160,7 @@ __device__ __forceinline__ void walk(const Walk& a, const uint32_t bh, const uin
         for (int i = 0; i < 2 * STEPS; ++i)
 #pragma unroll
             for (int j = 0; j < JS; ++j) {
-                const int row = 32 * (i >> 1) + 4 * (i & 1), col = 4 * (JS == 2 ? j : half);
+                const int row = 32 * (i >> 1) + 4 * (i & 1), col = JS == 1 ? 4 * half : 32 * (j >> 1) + 4 * (j & 1);
                 const int base = a.turned ? (col0 + col) * a.ld + row : row * a.ld + col0 + col;
                 int left = 4;
                 if (!FULL) {
@@ -178,7 +183,10 @@ __device__ __forceinline__ void walk(const Walk& a, const uint32_t bh, const uin
 #pragma unroll
         for (int i = 0; i < 2 * STEPS; ++i)
 #pragma unroll
-            for (int j = 0; j < JS; ++j) X[i][j] = turn(X[i][j], m);
+            for (int j = 0; j < JS; ++j) {
+                X[i][j] = turn(X[i][j], m);
+                __builtin_amdgcn_sched_barrier(0);
+            }
     };
     auto store_state = [&](auto& X, float* to) {
         turn_state(X);
@@ -195,8 +203,8 @@ __device__ __forceinline__ void walk(const Walk& a, const uint32_t bh, const uin
     gh = gh < -200.0f ? -200.0f : gh;  // 0 in fp32 from one token to the next
     float near[4], read, all;
     f4 write;
-    int measured = 0;
-    uint32_t measured_cuts = 0;
+    int measured;
+    uint32_t measured_cuts;
     auto measure = [&](int len, uint32_t cuts) {
         measured = len;
         measured_cuts = cuts;
@@ -250,11 +258,13 @@ __device__ __forceinline__ void walk(const Walk& a, const uint32_t bh, const uin
             for (int i = 0; i < 2; ++i) bt[2 * s + i] = split<NP>(mul<2>(four_of(bf, i), unit_matrix, zero));
             __builtin_amdgcn_sched_barrier(0);
         }
-        const Frag<NP> cf = operand(cr);
+        Frag<NP> cf[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) cf[u] = operand(cr[u]);
         Half<KEPT> P;
         float pairs = 0.0f;
         if constexpr (READ) {
-            if constexpr (GRAD) y = mul<2>(cf, operand(qr), zero);
+            if constexpr (GRAD) y = mul<2>(cf[0], operand(qr), zero);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 p[r] = near[r] != 0.0f ? p[r] * near[r] : 0.0f;  // a product that is not finite does not pass the zeros
@@ -263,14 +273,14 @@ __device__ __forceinline__ void walk(const Walk& a, const uint32_t bh, const uin
             P = split<KEPT>(p);
         }
         if (GRAD && JS == 1) pairs = half ? 0.0f : pairs;  // once for the two waves of these columns
-        float out[8];
+        float out[U][8];
 #pragma unroll
         for (int j = 0; j < JS; ++j) {
             __builtin_amdgcn_sched_barrier(0);
-            Half<NP> cj = four_of(cf, j);
+            Half<NP> cj = four_of(cf[j >> 1], j & 1);
             if (JS == 1)
 #pragma unroll
-                for (int p = 0; p < NP; ++p) cj.p[p] = half ? four_of(cf, 1).p[p] : cj.p[p];
+                for (int p = 0; p < NP; ++p) cj.p[p] = half ? four_of(cf[0], 1).p[p] : cj.p[p];
             const f4 ct = mul<2>(cj, unit_matrix, zero);
             if constexpr (READ) {
                 f4 x = zero;
@@ -286,11 +296,11 @@ __device__ __forceinline__ void walk(const Walk& a, const uint32_t bh, const uin
                     qr.get(q);
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
-                        pairs += ((float)(n + 1) * x[r] + (read != 0.0f ? slope[r] * read : 0.0f)) * (JS == 2 ? q[4 * j + r] : half ? q[4 + r] : q[r]);
+                        pairs += ((float)(n + 1) * x[r] + (read != 0.0f ? slope[r] * read : 0.0f)) * (half ? q[4 + r] : q[r]);
                 } else {
                     x = mul<2>(split<NP>(ct), P, x);
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) out[4 * j + r] = x[r];
+                    for (int r = 0; r < 4; ++r) out[j >> 1][4 * (j & 1) + r] = x[r];
                 }
             }
             // ---- the state behind the chunk
@@ -310,24 +320,28 @@ __device__ __forceinline__ void walk(const Walk& a, const uint32_t bh, const uin
         if constexpr (OUT) {
             const int l = lane_anew();
             const int64_t to = (b * a.out_stride[0] + (h / a.out_share) * a.out_stride[2] + t * a.out_stride[1] + col0) + ((l & 15) * a.out_stride[1] + 8 * (l >> 4));
-            if (n < len) {
-                if (a.out_f32) {
-                    Eight<T_F32> x;
-                    x.set(out);
-                    x.template store<FULL>((float*)a.out + to, dc - 8 * g);
-                } else {
-                    Eight<TY> x;
-                    x.set(out);
-                    x.template store<FULL>((E*)a.out + to, dc - 8 * g);
+            if (n < len)
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    if (a.out_f32) {
+                        Eight<T_F32> x;
+                        x.set(out[u]);
+                        x.template store<FULL>((float*)a.out + to + 32 * u, dc - 32 * u - 8 * g);
+                    } else {
+                        Eight<TY> x;
+                        x.set(out[u]);
+                        x.template store<FULL>((E*)a.out + to + 32 * u, dc - 32 * u - 8 * g);
+                    }
                 }
-            }
         }
         if (GRAD) dg += (double)pairs;
     };
 
-    // Tokens one by one, without the matrix units: of values that are not finite their zeros would make NaN where the
-    // definition has none. The state goes through memory, so that this rare path takes no registers from the other.
-    auto tokens = [&](int t, int rows, uint32_t cuts) {
+    // The rest of the walk token by token, without the matrix units: of values that are not finite their zeros would
+    // make NaN where the definition has none. The state goes through memory and the walk does not come back from
+    // here, so that this rare path takes no registers from the other (with a way back each chunk moved the whole state
+    // to other registers).
+    auto tokens = [&](int from, int to) {  // in order of time
         volatile float kept[SLOPE ? 2 : 1][2 * STEPS][4][JS];
 #pragma unroll
         for (int i = 0; i < 2 * STEPS; ++i)
@@ -341,15 +355,15 @@ __device__ __forceinline__ void walk(const Walk& a, const uint32_t bh, const uin
         const int m = lane_anew();
         const float fade = decay(gh, 1.0f);
 #pragma unroll 1
-        for (int k = 0; k < rows; ++k) {
-            const int row = BACK ? rows - 1 - k : k;
-            const int64_t tok = t + row;
-            const bool cut = cuts >> row & 1;
+        for (int k = from; k < to; ++k) {
+            const int64_t tok = BACK ? from + to - 1 - k : k;
+            const bool cut = rp && rp[tok * a.reset_stride[1]];
+            any_cut |= cut;
             float o[JS], v[JS], slope[JS];
             int c[JS];
 #pragma unroll
             for (int j = 0; j < JS; ++j) {
-                c[j] = 8 * (m >> 2 & 3) + (m & 3) + 4 * (JS == 2 ? j : half);
+                c[j] = 8 * (m >> 2 & 3) + (m & 3) + (JS == 1 ? 4 * half : 32 * (j >> 1) + 4 * (j & 1));
                 v[j] = (c[j] < dc ? Elem<TY>::get(cp[tok * a.c.stride[1] + c[j]]) : 0.0f) * (BACK ? a.scale : 1.0f);
                 o[j] = slope[j] = 0.0f;
             }
@@ -399,33 +413,20 @@ __device__ __forceinline__ void walk(const Walk& a, const uint32_t bh, const uin
     };
 
     // ---- the walk. Nothing is fetched ahead: more waves a SIMD, for which that leaves no registers, hide more.
-    bool turned = false;
-    while (true) {
-        bool fine = cr.finite();
+    uint32_t cuts = (uint32_t)__ballot(cut);
+    measure(rows, cuts);
+    turn_state(S);  // which has arrived by now
+    if constexpr (SLOPE) turn_state(N);
+    auto is_fine = [&] {
+        bool fine = true;
+#pragma unroll
+        for (int u = 0; u < U; ++u) fine &= cr[u].finite();
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) {
             fine &= br[s].finite();
             if constexpr (READ) fine &= ar[s].finite();
         }
         if constexpr (GRAD) fine &= qr.finite();
-        const uint32_t cuts = (uint32_t)__ballot(cut);
-        any_cut |= cuts != 0;
-        if (rows != measured || cuts != measured_cuts) measure(rows, cuts);
-        if (rows < C) {
-            const bool keep = n < rows;
-#pragma unroll
-            for (int s = 0; s < STEPS; ++s) {
-                br[s].keep(keep);
-                if constexpr (READ) ar[s].keep(keep);
-            }
-            cr.keep(keep);
-            if constexpr (GRAD) qr.keep(keep);
-        }
-        if (!turned) {  // the state arrives after the first rows and decays
-            turn_state(S);
-            if constexpr (SLOPE) turn_state(N);
-            turned = true;
-        }
         if (cuts)  // nothing of the state passes: it must not be multiplied by zero if it is not finite
 #pragma unroll
             for (int i = 0; i < 2 * STEPS; ++i)
@@ -434,13 +435,35 @@ __device__ __forceinline__ void walk(const Walk& a, const uint32_t bh, const uin
                     fine &= finite(S[i][j]);
                     if constexpr (SLOPE) fine &= finite(N[i][j]);
                 }
-        if (__ballot(!fine)) tokens(t, rows, cuts);
-        else chunk(t, rows);
+        return __ballot(!fine) == 0;
+    };
+    bool more = true;
+    bool fine = is_fine();
+    while (more && fine) {  // with one way out, else the state moves to other registers in every round
+        any_cut |= cuts != 0;
+        if (rows < C) {
+            const bool keep = n < rows;
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s) {
+                br[s].keep(keep);
+                if constexpr (READ) ar[s].keep(keep);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) cr[u].keep(keep);
+            if constexpr (GRAD) qr.keep(keep);
+        }
+        chunk(t, rows);
         at = BACK ? t : t + rows;
-        if (BACK ? at <= begin : at >= T) break;
-        bounds(at, t, rows);
-        fetch(t, rows);
+        more = BACK ? at > begin : at < T;
+        if (more) {
+            bounds(at, t, rows);
+            fetch(t, rows);
+            cuts = (uint32_t)__ballot(cut);
+            if (rows != measured || cuts != measured_cuts) measure(rows, cuts);
+            fine = is_fine();
+        }
     }
+    if (more) tokens(BACK ? begin : t, BACK ? at : T);
 
     // ---- what it leaves
     if constexpr (OUT) {
@@ -475,10 +498,19 @@ __device__ __forceinline__ uint32_t unit_of_wave() {
 }
 
 // Waves a SIMD that the registers are cut down to: as many as the state, its rows and their operands bear.
-constexpr int walk_waves(int type, int steps, int kind) { return type == T_F32 ? (steps == 4 && (kind == OUTPUTS || kind == SLOPES) ? 1 : steps == 1 ? 3 : 2) : steps == 4 ? 2 : kind == SLOPES || type == T_F16 ? 3 : 4; }
+#ifndef WIDE
+#define WIDE 32
+#endif
+constexpr int walk_waves(int type, int steps, int js, int kind) {
+#ifdef WV
+    if (steps == 2 && type == T_BF16) return WV;
+#endif
+    if (type == T_F32) return steps == 4 && (kind == OUTPUTS || kind == SLOPES) ? 1 : steps == 1 ? 3 : 2;
+    return steps == 4 ? 2 : js == 4 || kind == SLOPES || type == T_F16 ? 3 : 4;
+}
 
 template <int TY, int STEPS, int JS, bool BACK, int KIND, bool FULL>
-__global__ __launch_bounds__(256, walk_waves(TY, STEPS, KIND)) void linear_walk_kernel(const Walk a) {
+__global__ __launch_bounds__(256, walk_waves(TY, STEPS, JS, KIND)) void linear_walk_kernel(const Walk a) {
     constexpr bool READ = KIND == OUTPUTS || KIND == SLOPES;
     const uint32_t walks = READ ? a.segments : a.segments - 1;  // of the segments, all but the last in the walk's direction
     const uint32_t unit = unit_of_wave(), block = unit / (JS == 1 ? 2 : 1) % a.blocks, rest = unit / (JS == 1 ? 2 : 1) / a.blocks;
@@ -492,16 +524,16 @@ __global__ __launch_bounds__(256, walk_waves(TY, STEPS, KIND)) void linear_walk_
 struct Walks {
     Walk v, k, q;
 };
-template <int TY, int STEPS, bool FULL> __global__ __launch_bounds__(256, walk_waves(TY, STEPS, OUTPUTS)) void linear_gradients_kernel(const Walks a) {
+template <int TY, int STEPS, int JS, bool FULL> __global__ __launch_bounds__(256, walk_waves(TY, STEPS, JS, OUTPUTS)) void linear_gradients_kernel(const Walks a) {
     const uint32_t waves = a.v.blocks + a.k.blocks + a.q.blocks, unit = unit_of_wave(), rest = unit / waves;
     const uint32_t bh = rest / a.v.segments, segment = rest % a.v.segments;
     if (bh >= a.v.batch * a.v.heads) return;
     const uint32_t at = unit % waves, back = a.v.blocks + a.k.blocks;
     if (at < back) {
         const bool v = at < a.v.blocks;
-        walk<TY, STEPS, 2, true, OUTPUTS, FULL>(v ? a.v : a.k, bh, segment, v ? at : at - a.v.blocks, 0, unit);
+        walk<TY, STEPS, JS, true, OUTPUTS, FULL>(v ? a.v : a.k, bh, segment, v ? at : at - a.v.blocks, 0, unit);
     } else {
-        walk<TY, STEPS, 2, false, OUTPUTS, FULL>(a.q, bh, segment, at - back, 0, unit);
+        walk<TY, STEPS, JS, false, OUTPUTS, FULL>(a.q, bh, segment, at - back, 0, unit);
     }
 }
 
@@ -640,39 +672,65 @@ __global__ __launch_bounds__(256) void linear_step_kernel(const ZenoAmdLinearInp
 // ---- launches ------------------------------------------------------------------------------
 inline dim3 walk_grid(uint64_t units) { return dim3((uint32_t)((units + 31) / 32 * 8)); }  // a multiple of 8 workgroups of four waves
 
-template <int TY, int STEPS, bool FULL> void walk_shape(const Walk& w, Kind kind, bool back, hipStream_t stream) {
-    const bool read = kind == OUTPUTS || kind == SLOPES, halves = kind == SLOPES || kind == STATES_SLOPE;
-    const dim3 grid = walk_grid((uint64_t)w.batch * w.heads * w.blocks * (read ? w.segments : w.segments - 1) * (halves ? 2 : 1));
-    if (kind == OUTPUTS) linear_walk_kernel<TY, STEPS, 2, false, OUTPUTS, FULL><<<grid, 256, 0, stream>>>(w);
-    else if (kind == SLOPES) linear_walk_kernel<TY, STEPS, 1, false, SLOPES, FULL><<<grid, 256, 0, stream>>>(w);
-    else if (kind == STATES_SLOPE) linear_walk_kernel<TY, STEPS, 1, false, STATES_SLOPE, FULL><<<grid, 256, 0, stream>>>(w);
-    else if (back) linear_walk_kernel<TY, STEPS, 2, true, STATES, FULL><<<grid, 256, 0, stream>>>(w);
-    else linear_walk_kernel<TY, STEPS, 2, false, STATES, FULL><<<grid, 256, 0, stream>>>(w);
+// Runs launch(steps, js, full) with the launch shape as constants, and sets the walks' number of blocks: waves of
+// 64 columns where the registers bear them and a walk has more than 32. (Waves of 32 read and multiply A and B twice:
+// WAVE_FIGURES.)
+template <int TY, class F> void by_shape(int steps, std::initializer_list<Walk*> walks, F&& launch) {
+    auto by_columns = [&](auto s) {
+        constexpr int STEPS = decltype(s)::value;
+        int most = 0;
+        for (const Walk* w : walks) most = std::max(most, w->dc);
+        auto run = [&](auto js) {
+            constexpr int width = 16 * decltype(js)::value;
+            bool full = true;
+            for (Walk* w : walks) {
+                w->blocks = (w->dc + width - 1) / width;
+                full = full && w->da == 32 * STEPS && w->dc % width == 0;
+            }
+            full ? launch(s, js, std::true_type{}) : launch(s, js, std::false_type{});
+        };
+        if constexpr (STEPS < 4) {
+            if (most > WIDE) return run(std::integral_constant<int, 4>{});
+        }
+        run(std::integral_constant<int, 2>{});
+    };
+    if (steps == 1) by_columns(std::integral_constant<int, 1>{});
+    else if (steps == 2) by_columns(std::integral_constant<int, 2>{});
+    else by_columns(std::integral_constant<int, 4>{});
+}
+
+template <int TY> hipError_t launch_walk(Walk w, Kind kind, bool back, hipStream_t stream) {
+    const bool read = kind == OUTPUTS || kind == SLOPES;
+    by_shape<TY>(steps_of(w.da), {&w}, [&](auto steps, auto js, auto is_full) {
+        constexpr int STEPS = decltype(steps)::value, JS = decltype(js)::value;
+        constexpr bool FULL = decltype(is_full)::value;
+        const uint64_t walks = (uint64_t)w.batch * w.heads * (read ? w.segments : w.segments - 1);
+        if (kind == SLOPES || kind == STATES_SLOPE) {
+            w.blocks = (w.dc + 31) / 32;
+            const dim3 grid = walk_grid(walks * w.blocks * 2);
+            if (read) linear_walk_kernel<TY, STEPS, 1, false, SLOPES, FULL><<<grid, 256, 0, stream>>>(w);
+            else linear_walk_kernel<TY, STEPS, 1, false, STATES_SLOPE, FULL><<<grid, 256, 0, stream>>>(w);
+            return;
+        }
+        const dim3 grid = walk_grid(walks * w.blocks);
+        if (kind == OUTPUTS) linear_walk_kernel<TY, STEPS, JS, false, OUTPUTS, FULL><<<grid, 256, 0, stream>>>(w);
+        else if (back) linear_walk_kernel<TY, STEPS, JS, true, STATES, FULL><<<grid, 256, 0, stream>>>(w);
+        else linear_walk_kernel<TY, STEPS, JS, false, STATES, FULL><<<grid, 256, 0, stream>>>(w);
+    });
     if (!read && w.segments > 2) {
         const dim3 join(w.batch * w.heads * (uint32_t)((w.size + 255) / 256));
         if (back) linear_join_kernel<true, false><<<join, 256, 0, stream>>>(w);
         else if (kind == STATES) linear_join_kernel<false, false><<<join, 256, 0, stream>>>(w);
         else linear_join_kernel<false, true><<<join, 256, 0, stream>>>(w);
     }
-}
-
-template <int TY> hipError_t launch_walk(const Walk& w, Kind kind, bool back, hipStream_t stream) {
-    const int steps = steps_of(w.da);
-    const bool full = full_of(w);
-    if (steps == 1) full ? walk_shape<TY, 1, true>(w, kind, back, stream) : walk_shape<TY, 1, false>(w, kind, back, stream);
-    else if (steps == 2) full ? walk_shape<TY, 2, true>(w, kind, back, stream) : walk_shape<TY, 2, false>(w, kind, back, stream);
-    else full ? walk_shape<TY, 4, true>(w, kind, back, stream) : walk_shape<TY, 4, false>(w, kind, back, stream);
     return hipGetLastError();
 }
 
-template <int TY> hipError_t launch_gradients(const Walk& v, const Walk& k, const Walk& q, hipStream_t stream) {
-    const Walks w{v, k, q};
-    const dim3 grid = walk_grid((uint64_t)v.batch * v.heads * v.segments * (v.blocks + k.blocks + q.blocks));
-    const int steps = std::max(steps_of(v.da), steps_of(k.da));
-    const bool full = full_of(v) && full_of(k) && steps_of(v.da) == steps_of(k.da);
-    if (steps == 1) full ? linear_gradients_kernel<TY, 1, true><<<grid, 256, 0, stream>>>(w) : linear_gradients_kernel<TY, 1, false><<<grid, 256, 0, stream>>>(w);
-    else if (steps == 2) full ? linear_gradients_kernel<TY, 2, true><<<grid, 256, 0, stream>>>(w) : linear_gradients_kernel<TY, 2, false><<<grid, 256, 0, stream>>>(w);
-    else full ? linear_gradients_kernel<TY, 4, true><<<grid, 256, 0, stream>>>(w) : linear_gradients_kernel<TY, 4, false><<<grid, 256, 0, stream>>>(w);
+template <int TY> hipError_t launch_gradients(Walk v, Walk k, Walk q, hipStream_t stream) {
+    by_shape<TY>(std::max(steps_of(v.da), steps_of(k.da)), {&v, &k, &q}, [&](auto steps, auto js, auto full) {
+        const dim3 grid = walk_grid((uint64_t)v.batch * v.heads * v.segments * (v.blocks + k.blocks + q.blocks));
+        linear_gradients_kernel<TY, decltype(steps)::value, decltype(js)::value, decltype(full)::value><<<grid, 256, 0, stream>>>(Walks{v, k, q});
+    });
     return hipGetLastError();
 }
 
