@@ -11,7 +11,7 @@
 namespace za {
 namespace linear {
 
-constexpr int kChunk = 16;  // tokens
+constexpr int kChunk = 32;  // tokens, at most: segments are multiples of it
 
 // Rows of one of the inputs. Strides are in elements: sequence, token, head.
 struct Rows {

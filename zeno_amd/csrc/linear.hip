@@ -96,11 +96,12 @@ std::string check_outputs(const std::vector<Memory>& inputs, const std::vector<M
 
 }  // namespace
 
-// With fewer walks than two waves a SIMD, as many segments as make up those, of at least eight chunks.
+// With fewer walks than two waves a SIMD, as many segments as make up those, of at least four chunks.
 Segments segments_of(const ZenoAmdLinearInputs& in) {
     const int64_t chunks = ((int64_t)in.length + kChunk - 1) / kChunk;
     const int64_t walks = (int64_t)heads_of(in) * blocks_of(in.value_dim);
-    int64_t want = std::min(2048 / walks, chunks / 8);
+    static const int target = getenv("ZT") ? atoi(getenv("ZT")) : 2048, least = getenv("ZL") ? atoi(getenv("ZL")) : 4;
+    int64_t want = std::min(target / walks, chunks / least);
     if (want < 2) want = 1;
     const int64_t each = (chunks + want - 1) / want;
     return Segments{(uint32_t)((chunks + each - 1) / each), (int)(each * kChunk)};

@@ -1,7 +1,7 @@
 // Kernels of linear attention with a decay for each head: walks over whole sequences, and the
 // single-token step.
 //
-// A chunk is 16 tokens. With S the state before it, a walk forward is
+// A chunk is one or two tiles of 16 tokens. With S the state before it, a walk forward is
 //     P_ij = scale exp(g (i - j)) A_i . B_j  for j <= i with no reset after j up to i, else 0
 //     out  = P C + scale exp(g (i + 1)) A S      (the second where no reset is before or at i)
 //     S'   = exp(g L) S + sum_j exp(g (L - 1 - j)) B_j C_j^T      (L tokens; nothing across a reset)
@@ -57,12 +57,48 @@ template <int TY> __device__ __forceinline__ Frag<Elem<TY>::parts> operand(const
     return f;
 }
 
-// Four of the eight values a lane has of a row.
+// A row's eight values as an operand for products with other rows: 16-bit types as they are, for the matrix
+// instructions of their own type, float32 in three parts.
+template <int TY> struct Own {
+    static constexpr int parts = TY == T_F32 ? 3 : 1;
+    static constexpr uint32_t one = TY == T_F16 ? 0x3c00u : 0x3f80u;  // of the parts' type
+    typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+    typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+    static __device__ __forceinline__ Frag<parts> make(const Eight<TY>& x) {
+        if constexpr (TY == T_F32) return operand(x);
+        else return Frag<1>{{x.a[0]}};
+    }
+    template <int PB> static __device__ __forceinline__ f4 product(const Frag<parts>& a, const Frag<PB>& b, f4 acc) {
+        if constexpr (TY == T_F16) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a.p[0]), __builtin_bit_cast(h8, b.p[0]), acc, 0, 0, 0);
+        else return mul<2>(a, b, acc);
+    }
+    // Four of a lane's eight, with 16 along the contraction.
+    static __device__ __forceinline__ f4 product(const Half<parts>& a, const Half<1>& b, f4 acc) {
+        if constexpr (TY == T_F16) return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(h4, a.p[0]), __builtin_bit_cast(h4, b.p[0]), acc, 0, 0, 0);
+        else return mul<2>(a, b, acc);
+    }
+};
 template <int P> __device__ __forceinline__ Half<P> four_of(const Frag<P>& f, int i) {
     Half<P> h;
 #pragma unroll
     for (int p = 0; p < P; ++p) h.p[p] = i ? u2{f.p[p][2], f.p[p][3]} : u2{f.p[p][0], f.p[p][1]};
     return h;
+}
+// acc[i] + A[i] B, the smallest part products first, those of one weight side by side as they do not wait for one another.
+template <int N, class A, class B> __device__ __forceinline__ void mul_each(const A* a, const B& b, f4* acc) {
+    constexpr int PA = sizeof(a->p) / sizeof(a->p[0]), PB = sizeof(b.p) / sizeof(b.p[0]);
+#pragma unroll
+    for (int s = 2; s >= 0; --s)
+#pragma unroll
+        for (int x = 0; x < PA; ++x)
+            if (s - x >= 0 && s - x < PB)
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    if constexpr (sizeof(a->p[0]) == 16)
+                        acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8, a[i].p[x]), __builtin_bit_cast(bf8, b.p[s - x]), acc[i], 0, 0, 0);
+                    else
+                        acc[i] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s4, a[i].p[x]), __builtin_bit_cast(s4, b.p[s - x]), acc[i], 0, 0, 0);
+                }
 }
 
 // Four floats at any address, the first `n` of them in bounds.
@@ -91,12 +127,23 @@ __device__ __forceinline__ int lane_anew() {
     return m;
 }
 
+// Operands along the tokens of a chunk: of two tiles or of one.
+template <int TILES> struct Along;
+template <> struct Along<2> {
+    template <int P> using Op = Frag<P>;
+    template <int P> static __device__ __forceinline__ Frag<P> make(const f4* x) { return split<P>(x[0], x[1]); }
+};
+template <> struct Along<1> {
+    template <int P> using Op = Half<P>;
+    template <int P> static __device__ __forceinline__ Half<P> make(const f4* x) { return split<P>(x[0]); }
+};
+
 // One walk of one wave in one segment of one head: of 64 or 32 columns of the state (JS 4 or 2 tiles of 16), or of
 // every other four of 32 (JS 1: tile `half` of the pair).
-template <int TY, int STEPS, int JS, bool BACK, int KIND, bool FULL>
+template <int TY, int STEPS, int TILES, int JS, bool BACK, int KIND, bool FULL>
 __device__ __forceinline__ void walk(const Walk& a, const uint32_t bh, const uint32_t segment, const int block, const int half, const uint32_t unit) {
     typedef typename Elem<TY>::type E;
-    constexpr int NP = Elem<TY>::parts, C = kChunk;
+    constexpr int NP = Elem<TY>::parts, C = 16 * TILES;
     constexpr bool OUT = KIND == OUTPUTS, SLOPE = KIND == SLOPES || KIND == STATES_SLOPE, GRAD = KIND == SLOPES, READ = OUT || GRAD;
     // Operands for outputs of 16 bits that are no part of a state: two parts, 2^-17 of a term, where the output is rounded
     // by 2^-9 or 2^-12 of itself.
@@ -115,25 +162,28 @@ __device__ __forceinline__ void walk(const Walk& a, const uint32_t bh, const uin
     const E* qp = GRAD ? rows_of(a.q) + col0 : nullptr;
     const uint8_t* rp = a.reset ? a.reset + b * a.reset_stride[0] : nullptr;
 
-    // ---- what a chunk reads: token n's dimensions 8 g to 8 g + 7 of every 32
-    Eight<TY> ar[STEPS], br[STEPS], cr[U], qr;
+    // ---- what a chunk reads: dimensions 8 g to 8 g + 7 of every 32, of token n of each tile of 16
+    Eight<TY> ar[TILES][STEPS], br[TILES][STEPS], cr[TILES][U], qr[TILES];
     bool cut = false, any_cut = false;
     auto fetch = [&](int t, int rows) {
         cut = rp && lane < rows && rp[(t + lane) * a.reset_stride[1]];
-        const int row = min(n, rows - 1);
-        auto place = [&](const E* x, const Rows& r) { return x + t * r.stride[1] + (row * r.stride[1] + 8 * g); };
-        const E* x = place(bp, a.b);
 #pragma unroll
-        for (int s = 0; s < STEPS; ++s) br[s].template load<FULL>(x + 32 * s, da - 32 * s - 8 * g);
-        if constexpr (READ) {
-            x = place(ap, a.a);
+        for (int k = 0; k < TILES; ++k) {
+            const int row = min(16 * k + n, rows - 1);
+            auto place = [&](const E* x, const Rows& r) { return x + t * r.stride[1] + (row * r.stride[1] + 8 * g); };
+            const E* x = place(bp, a.b);
 #pragma unroll
-            for (int s = 0; s < STEPS; ++s) ar[s].template load<FULL>(x + 32 * s, da - 32 * s - 8 * g);
+            for (int s = 0; s < STEPS; ++s) br[k][s].template load<FULL>(x + 32 * s, da - 32 * s - 8 * g);
+            if constexpr (READ) {
+                x = place(ap, a.a);
+#pragma unroll
+                for (int s = 0; s < STEPS; ++s) ar[k][s].template load<FULL>(x + 32 * s, da - 32 * s - 8 * g);
+            }
+            x = place(cp, a.c);
+#pragma unroll
+            for (int u = 0; u < U; ++u) cr[k][u].template load<FULL>(x + 32 * u, dc - 32 * u - 8 * g);
+            if constexpr (GRAD) qr[k].template load<FULL>(place(qp, a.q), dc - 8 * g);
         }
-        x = place(cp, a.c);
-#pragma unroll
-        for (int u = 0; u < U; ++u) cr[u].template load<FULL>(x + 32 * u, dc - 32 * u - 8 * g);
-        if constexpr (GRAD) qr.template load<FULL>(place(qp, a.q), dc - 8 * g);
     };
     auto bounds = [&](int at, int& t, int& rows) {  // the chunk of the grid that `at` is in, from it (or up to it) on
         if (BACK) {
@@ -201,33 +251,54 @@ __device__ __forceinline__ void walk(const Walk& a, const uint32_t bh, const uin
     // a token is behind the other. `read`: of the state to a token, `write`: of a token to the next state, `all`: of
     // the state to the next.
     gh = gh < -200.0f ? -200.0f : gh;  // 0 in fp32 from one token to the next
-    float near[4], read, all;
-    f4 write;
+    constexpr int tile_pairs = TILES == 2 ? 3 : 1;  // each tile with itself, and the first with the second
+    float near[tile_pairs][4], read[TILES], all;
+    f4 write[TILES];
     int measured;
     uint32_t measured_cuts;
     auto measure = [&](int len, uint32_t cuts) {
         measured = len;
         measured_cuts = cuts;
-        const int m = lane_anew(), i = m & 15, j0 = 4 * (m >> 4);
+        const int m = lane_anew(), i0 = m & 15, j0 = 4 * (m >> 4);
         all = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(decay(gh, len))));
-        read = BACK ? decay(gh, max(len - 1 - i, 0)) : a.scale * decay(gh, i + 1);
+#pragma unroll
+        for (int k = 0; k < TILES; ++k) {
+            const int i = 16 * k + i0;
+            read[k] = BACK ? decay(gh, max(len - 1 - i, 0)) : a.scale * decay(gh, i + 1);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int j = 16 * k + j0 + r;
+                write[k][r] = BACK ? a.scale * decay(gh, j + 1) : decay(gh, max(len - 1 - j, 0));
+            }
+        }
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const int j = j0 + r, apart = BACK ? j - i : i - j;
-            near[r] = apart < 0 ? 0.0f : a.scale * decay(gh, max(apart, 0));
-            write[r] = BACK ? a.scale * decay(gh, j + 1) : decay(gh, max(len - 1 - j, 0));
+            const int apart = BACK ? j0 + r - i0 : i0 - j0 - r;
+            near[0][r] = apart < 0 ? 0.0f : a.scale * decay(gh, max(apart, 0));
+            if constexpr (TILES == 2) {
+                near[1][r] = near[0][r];
+                near[2][r] = a.scale * decay(gh, 16 + apart);
+            }
         }
         if (cuts) {
             const int last = 31 - __builtin_clz(cuts), first = __builtin_ctz(cuts);
-            auto reset_to = [&](int token) { return 31 - __clz((int)(cuts & (0xffffu >> (15 - token)))); };  // the last one up to it
+            auto reset_to = [&](int token) { return 31 - __clz((int)(cuts & (0xffffffffu >> (31 - token)))); };  // the last one up to it
             all = 0.0f;
-            if (BACK ? i < last : reset_to(i) >= 0) read = 0.0f;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int j = j0 + r;
-                if (BACK ? j >= first : j < last) write[r] = 0.0f;
-                if (BACK ? i < reset_to(j) : j < reset_to(i)) near[r] = 0.0f;
+            for (int k = 0; k < TILES; ++k) {
+                const int i = 16 * k + i0;
+                if (BACK ? i < last : reset_to(i) >= 0) read[k] = 0.0f;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int j = 16 * k + j0 + r;
+                    if (BACK ? j >= first : j < last) write[k][r] = 0.0f;
+                    if (BACK ? i < reset_to(j) : j < reset_to(i)) near[k][r] = 0.0f;
+                }
             }
+            if constexpr (TILES == 2)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (BACK ? i0 < reset_to(16 + j0 + r) : j0 + r < reset_to(16 + i0)) near[2][r] = 0.0f;
         }
     };
 
@@ -235,102 +306,208 @@ __device__ __forceinline__ void walk(const Walk& a, const uint32_t bh, const uin
     // gives a tile whose column n is dimension 8 (n / 4) + 4 i + n % 4.
     Half<1> unit_matrix;
 #pragma unroll
-    for (int w = 0; w < 2; ++w) unit_matrix.p[0][w] = g == (n >> 2) && ((n & 3) >> 1) == w ? 0x3f80u << (16 * (n & 1)) : 0u;
+    for (int w = 0; w < 2; ++w) unit_matrix.p[0][w] = g == (n >> 2) && ((n & 3) >> 1) == w ? Own<TY>::one << (16 * (n & 1)) : 0u;
     double dg = 0.0;
+
+    // The chunk's rows as operands, and the products of A's with B's, row j = 16 tj + 4 g + r, column i = 16 ti + n: P without
+    // its decays. Returns whether all that was read is finite, which these products tell, and sums of rows where they do
+    // not. (A look at every value was a third of a chunk's vector instructions.)
+    Frag<Own<TY>::parts> ao[TILES][STEPS], bo[TILES][STEPS], co[TILES][U];
+    f4 p[tile_pairs];
+    auto products = [&](int rows, uint32_t cuts) {
+        const f4 zero = {0, 0, 0, 0};
+        if (rows < C)
+#pragma unroll
+            for (int k = 0; k < TILES; ++k) {
+                const bool keep = 16 * k + n < rows;
+#pragma unroll
+                for (int s = 0; s < STEPS; ++s) {
+                    br[k][s].keep(keep);
+                    if constexpr (READ) ar[k][s].keep(keep);
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u) cr[k][u].keep(keep);
+                if constexpr (GRAD) qr[k].keep(keep);
+            }
+        Frag<1> ones;
+        ones.p[0] = u4{Own<TY>::one * 0x10001u, Own<TY>::one * 0x10001u, Own<TY>::one * 0x10001u, Own<TY>::one * 0x10001u};
+        bool fine = true;
+#pragma unroll
+        for (int k = 0; k < tile_pairs; ++k) p[k] = zero;
+#pragma unroll
+        for (int k = 0; k < TILES; ++k) {
+            f4 sums = zero;
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s) {
+                bo[k][s] = Own<TY>::make(br[k][s]);
+                if constexpr (READ) {
+                    ao[k][s] = Own<TY>::make(ar[k][s]);
+                    p[k] = Own<TY>::product(bo[k][s], ao[k][s], p[k]);
+                } else {
+                    sums = Own<TY>::product(bo[k][s], ones, sums);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                co[k][u] = Own<TY>::make(cr[k][u]);
+                sums = Own<TY>::product(co[k][u], ones, sums);
+            }
+            if constexpr (GRAD) sums = Own<TY>::product(Own<TY>::make(qr[k]), ones, sums);
+            fine &= finite(sums);
+        }
+        if constexpr (READ && TILES == 2)
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s) p[2] = Own<TY>::product(bo[BACK ? 1 : 0][s], ao[BACK ? 0 : 1][s], p[2]);
+        if constexpr (READ)
+#pragma unroll
+            for (int k = 0; k < tile_pairs; ++k) fine &= finite(p[k]);
+        if (cuts)  // nothing of the state passes: it must not be multiplied by zero if it is not finite
+#pragma unroll
+            for (int i = 0; i < 2 * STEPS; ++i)
+#pragma unroll
+                for (int j = 0; j < JS; ++j) {
+                    fine &= finite(S[i][j]);
+                    if constexpr (SLOPE) fine &= finite(N[i][j]);
+                }
+        return __ballot(!fine) == 0;
+    };
 
     // The chunk of tokens t to t + len. No branch is inside: where one lies between a matrix instruction and the use of
     // its result, the compiler has been seen to leave out the wait. The scheduler is kept from starting everything at
     // once, which takes more registers than there are.
     auto chunk = [&](int t, int len) {
         const f4 zero = {0, 0, 0, 0};
-        // ---- P transposed (row j = 4 g + r, column i = n), and B along the tokens
-        Frag<NP> af[STEPS];
-        Half<NP> bt[2 * STEPS];
-        f4 p = zero, y = zero;
+        // ---- B along the tokens, P
+        typename Along<TILES>::template Op<NP> bt[2 * STEPS];
 #pragma unroll
-        for (int s = 0; s < STEPS; ++s) {
-            const Frag<NP> bf = operand(br[s]);
-            if constexpr (READ) {
-                af[s] = operand(ar[s]);
-                p = mul<2>(bf, af[s], p);
-            }
+        for (int i = 0; i < 2 * STEPS; ++i) {
+            f4 x[TILES];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) bt[2 * s + i] = split<NP>(mul<2>(four_of(bf, i), unit_matrix, zero));
-            __builtin_amdgcn_sched_barrier(0);
+            for (int k = 0; k < TILES; ++k) x[k] = Own<TY>::product(four_of(bo[k][i >> 1], i & 1), unit_matrix, zero);
+            bt[i] = Along<TILES>::template make<NP>(x);
+            if (i & 1) __builtin_amdgcn_sched_barrier(0);
         }
-        Frag<NP> cf[U];
+        Frag<NP> af[TILES][STEPS];
+        if constexpr (READ)
 #pragma unroll
-        for (int u = 0; u < U; ++u) cf[u] = operand(cr[u]);
-        Half<KEPT> P;
+            for (int k = 0; k < TILES; ++k)
+#pragma unroll
+                for (int s = 0; s < STEPS; ++s) {
+                    if constexpr (TY == T_F16) af[k][s] = operand(ar[k][s]);
+                    else af[k][s] = ao[k][s];
+                }
+        constexpr int one = BACK ? TILES - 1 : 0;  // the tile whose tokens see no other
+        Half<KEPT> alone;
+        Frag<KEPT> both;
         float pairs = 0.0f;
         if constexpr (READ) {
-            if constexpr (GRAD) y = mul<2>(cf[0], operand(qr), zero);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                p[r] = near[r] != 0.0f ? p[r] * near[r] : 0.0f;  // a product that is not finite does not pass the zeros
-                if (GRAD) pairs += (float)(n - 4 * g - r) * p[r] * y[r];
+            for (int k = 0; k < tile_pairs; ++k) {
+                f4 y = zero;
+                const int ti = k < 2 ? k : BACK ? 0 : 1, tj = k < 2 ? k : 1 - ti;
+                if constexpr (GRAD) y = Own<TY>::product(co[tj][0], Own<TY>::make(qr[ti]), zero);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    p[k][r] *= near[k][r];
+                    if (GRAD) pairs += (float)(16 * (ti - tj) + n - 4 * g - r) * p[k][r] * y[r];
+                }
             }
-            P = split<KEPT>(p);
+            alone = split<KEPT>(p[one]);
+            if constexpr (TILES == 2) both = BACK ? split<KEPT>(p[0], p[2]) : split<KEPT>(p[2], p[1]);
         }
         if (GRAD && JS == 1) pairs = half ? 0.0f : pairs;  // once for the two waves of these columns
-        float out[U][8];
+        float out[TILES][U][8];
 #pragma unroll
         for (int j = 0; j < JS; ++j) {
             __builtin_amdgcn_sched_barrier(0);
-            Half<NP> cj = four_of(cf[j >> 1], j & 1);
-            if (JS == 1)
+            f4 ct[TILES];
 #pragma unroll
-                for (int p = 0; p < NP; ++p) cj.p[p] = half ? four_of(cf[0], 1).p[p] : cj.p[p];
-            const f4 ct = mul<2>(cj, unit_matrix, zero);
+            for (int k = 0; k < TILES; ++k) {
+                auto cj = four_of(co[k][j >> 1], j & 1);
+                if (JS == 1)
+#pragma unroll
+                    for (int p = 0; p < Own<TY>::parts; ++p) cj.p[p] = half ? four_of(co[k][0], 1).p[p] : cj.p[p];
+                ct[k] = Own<TY>::product(cj, unit_matrix, zero);
+            }
             if constexpr (READ) {
-                f4 x = zero;
+                f4 x[TILES], slope[TILES];
 #pragma unroll
-                for (int s = 0; s < STEPS; ++s) x = mul<2>(split<KEPT>(S[2 * s][j], S[2 * s + 1][j]), af[s], x);
+                for (int k = 0; k < TILES; ++k) x[k] = slope[k] = zero;
 #pragma unroll
-                for (int r = 0; r < 4; ++r) x[r] = read != 0.0f ? x[r] * read : 0.0f;
-                if constexpr (GRAD) {
-                    f4 slope = zero;
+                for (int s = 0; s < STEPS; ++s) {
+                    const Frag<KEPT> sf = split<KEPT>(S[2 * s][j], S[2 * s + 1][j]);
 #pragma unroll
-                    for (int s = 0; s < STEPS; ++s) slope = mul<2>(split<3>(N[2 * s][j], N[2 * s + 1][j]), af[s], slope);
-                    float q[8];
-                    qr.get(q);
+                    for (int k = 0; k < TILES; ++k) x[k] = mul<2>(sf, af[k][s], x[k]);
+                    if constexpr (GRAD) {
+                        const Frag<3> nf = split<3>(N[2 * s][j], N[2 * s + 1][j]);
 #pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        pairs += ((float)(n + 1) * x[r] + (read != 0.0f ? slope[r] * read : 0.0f)) * (half ? q[4 + r] : q[r]);
-                } else {
-                    x = mul<2>(split<NP>(ct), P, x);
+                        for (int k = 0; k < TILES; ++k) slope[k] = mul<2>(nf, af[k][s], slope[k]);
+                    }
+                }
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) out[j >> 1][4 * (j & 1) + r] = x[r];
+                for (int k = 0; k < TILES; ++k) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) x[k][r] = read[k] != 0.0f ? x[k][r] * read[k] : 0.0f;
+                    if constexpr (GRAD) {
+                        float q[8];
+                        qr[k].get(q);
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            pairs += ((float)(16 * k + n + 1) * x[k][r] + (read[k] != 0.0f ? slope[k][r] * read[k] : 0.0f)) * (half ? q[4 + r] : q[r]);
+                    }
+                }
+                if constexpr (OUT) {
+                    x[one] = mul<2>(split<NP>(ct[one]), alone, x[one]);
+                    if constexpr (TILES == 2) x[1 - one] = mul<2>(split<NP>(ct[0], ct[1]), both, x[1 - one]);
+#pragma unroll
+                    for (int k = 0; k < TILES; ++k)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) out[k][j >> 1][4 * (j & 1) + r] = x[k][r];
                 }
             }
             // ---- the state behind the chunk
             __builtin_amdgcn_sched_barrier(0);
-            f4 w = ct * write;
-            const Half<3> wf = split<3>(w);
+#pragma unroll
+            for (int k = 0; k < TILES; ++k) ct[k] *= write[k];
+            const auto wf = Along<TILES>::template make<3>(ct);
             if constexpr (SLOPE) {
 #pragma unroll
-                for (int r = 0; r < 4; ++r) w[r] *= (float)max(len - 1 - 4 * g - r, 0);
-                const Half<3> nf = split<3>(w);
+                for (int k = 0; k < TILES; ++k)
 #pragma unroll
-                for (int i = 0; i < 2 * STEPS; ++i) N[i][j] = mul<2>(bt[i], nf, (N[i][j] + S[i][j] * (float)len) * all);
+                    for (int r = 0; r < 4; ++r) ct[k][r] *= (float)max(len - 1 - 16 * k - 4 * g - r, 0);
+                const auto nf = Along<TILES>::template make<3>(ct);
+                f4 x[2 * STEPS];
+#pragma unroll
+                for (int i = 0; i < 2 * STEPS; ++i) x[i] = (N[i][j] + S[i][j] * (float)len) * all;
+                mul_each<2 * STEPS>(bt, nf, x);
+#pragma unroll
+                for (int i = 0; i < 2 * STEPS; ++i) N[i][j] = x[i];
             }
+            f4 x[2 * STEPS];
 #pragma unroll
-            for (int i = 0; i < 2 * STEPS; ++i) S[i][j] = mul<2>(bt[i], wf, S[i][j] * all);
-        }
-        if constexpr (OUT) {
-            const int l = lane_anew();
-            const int64_t to = (b * a.out_stride[0] + (h / a.out_share) * a.out_stride[2] + t * a.out_stride[1] + col0) + ((l & 15) * a.out_stride[1] + 8 * (l >> 4));
-            if (n < len)
+            for (int i = 0; i < 2 * STEPS; ++i) x[i] = S[i][j] * all;
+            mul_each<2 * STEPS>(bt, wf, x);
 #pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    if (a.out_f32) {
-                        Eight<T_F32> x;
-                        x.set(out[u]);
-                        x.template store<FULL>((float*)a.out + to + 32 * u, dc - 32 * u - 8 * g);
-                    } else {
-                        Eight<TY> x;
-                        x.set(out[u]);
-                        x.template store<FULL>((E*)a.out + to + 32 * u, dc - 32 * u - 8 * g);
+            for (int i = 0; i < 2 * STEPS; ++i) S[i][j] = x[i];
+            // ---- 32 columns of the outputs
+            if constexpr (OUT)
+                if (j & 1) {
+                    const int l = lane_anew(), u = j >> 1;
+#pragma unroll
+                    for (int k = 0; k < TILES; ++k) {
+                        const int row = 16 * k + (l & 15);
+                        const int64_t to = (b * a.out_stride[0] + (h / a.out_share) * a.out_stride[2] + t * a.out_stride[1] + col0 + 32 * u) + (row * a.out_stride[1] + 8 * (l >> 4));
+                        if (row < len) {
+                            if (a.out_f32) {
+                                Eight<T_F32> x;
+                                x.set(out[k][u]);
+                                x.template store<FULL>((float*)a.out + to, dc - 32 * u - 8 * g);
+                            } else {
+                                Eight<TY> x;
+                                x.set(out[k][u]);
+                                x.template store<FULL>((E*)a.out + to, dc - 32 * u - 8 * g);
+                            }
+                        }
                     }
                 }
         }
@@ -417,41 +594,10 @@ __device__ __forceinline__ void walk(const Walk& a, const uint32_t bh, const uin
     measure(rows, cuts);
     turn_state(S);  // which has arrived by now
     if constexpr (SLOPE) turn_state(N);
-    auto is_fine = [&] {
-        bool fine = true;
-#pragma unroll
-        for (int u = 0; u < U; ++u) fine &= cr[u].finite();
-#pragma unroll
-        for (int s = 0; s < STEPS; ++s) {
-            fine &= br[s].finite();
-            if constexpr (READ) fine &= ar[s].finite();
-        }
-        if constexpr (GRAD) fine &= qr.finite();
-        if (cuts)  // nothing of the state passes: it must not be multiplied by zero if it is not finite
-#pragma unroll
-            for (int i = 0; i < 2 * STEPS; ++i)
-#pragma unroll
-                for (int j = 0; j < JS; ++j) {
-                    fine &= finite(S[i][j]);
-                    if constexpr (SLOPE) fine &= finite(N[i][j]);
-                }
-        return __ballot(!fine) == 0;
-    };
     bool more = true;
-    bool fine = is_fine();
+    bool fine = products(rows, cuts);
     while (more && fine) {  // with one way out, else the state moves to other registers in every round
         any_cut |= cuts != 0;
-        if (rows < C) {
-            const bool keep = n < rows;
-#pragma unroll
-            for (int s = 0; s < STEPS; ++s) {
-                br[s].keep(keep);
-                if constexpr (READ) ar[s].keep(keep);
-            }
-#pragma unroll
-            for (int u = 0; u < U; ++u) cr[u].keep(keep);
-            if constexpr (GRAD) qr.keep(keep);
-        }
         chunk(t, rows);
         at = BACK ? t : t + rows;
         more = BACK ? at > begin : at < T;
@@ -460,7 +606,7 @@ __device__ __forceinline__ void walk(const Walk& a, const uint32_t bh, const uin
             fetch(t, rows);
             cuts = (uint32_t)__ballot(cut);
             if (rows != measured || cuts != measured_cuts) measure(rows, cuts);
-            fine = is_fine();
+            fine = products(rows, cuts);
         }
     }
     if (more) tokens(BACK ? begin : t, BACK ? at : T);
@@ -498,25 +644,26 @@ __device__ __forceinline__ uint32_t unit_of_wave() {
 }
 
 // Waves a SIMD that the registers are cut down to: as many as the state, its rows and their operands bear.
-#ifndef WIDE
-#define WIDE 32
+#ifndef TALL_OK
+#define TALL_OK(TY, STEPS, JS) ((TY) == T_BF16 || ((TY) == T_F16 && (STEPS) == 1))
 #endif
-constexpr int walk_waves(int type, int steps, int js, int kind) {
-#ifdef WV
-    if (steps == 2 && type == T_BF16) return WV;
+#ifndef WV
+#define WV 2
 #endif
+constexpr int walk_waves(int type, int steps, int tiles, int js, int kind) {
+    if (tiles == 2) return steps == 4 ? 2 : WV;
     if (type == T_F32) return steps == 4 && (kind == OUTPUTS || kind == SLOPES) ? 1 : steps == 1 ? 3 : 2;
-    return steps == 4 ? 2 : js == 4 || kind == SLOPES || type == T_F16 ? 3 : 4;
+    return steps == 4 ? 2 : js == 4 && steps == 2 ? 2 : kind == SLOPES || type == T_F16 ? 3 : 4;
 }
 
-template <int TY, int STEPS, int JS, bool BACK, int KIND, bool FULL>
-__global__ __launch_bounds__(256, walk_waves(TY, STEPS, JS, KIND)) void linear_walk_kernel(const Walk a) {
+template <int TY, int STEPS, int TILES, int JS, bool BACK, int KIND, bool FULL>
+__global__ __launch_bounds__(256, walk_waves(TY, STEPS, TILES, JS, KIND)) void linear_walk_kernel(const Walk a) {
     constexpr bool READ = KIND == OUTPUTS || KIND == SLOPES;
     const uint32_t walks = READ ? a.segments : a.segments - 1;  // of the segments, all but the last in the walk's direction
     const uint32_t unit = unit_of_wave(), block = unit / (JS == 1 ? 2 : 1) % a.blocks, rest = unit / (JS == 1 ? 2 : 1) / a.blocks;
     const uint32_t bh = rest / walks, segment = rest % walks + (!READ && BACK ? 1 : 0);
     if (bh >= a.batch * a.heads) return;
-    walk<TY, STEPS, JS, BACK, KIND, FULL>(a, bh, segment, block, JS == 1 ? unit & 1 : 0, unit);
+    walk<TY, STEPS, TILES, JS, BACK, KIND, FULL>(a, bh, segment, block, JS == 1 ? unit & 1 : 0, unit);
 }
 
 // All gradients but g's: the walks of d_v, d_k and d_q of a head and segment side by side, as they read the
@@ -524,16 +671,16 @@ __global__ __launch_bounds__(256, walk_waves(TY, STEPS, JS, KIND)) void linear_w
 struct Walks {
     Walk v, k, q;
 };
-template <int TY, int STEPS, int JS, bool FULL> __global__ __launch_bounds__(256, walk_waves(TY, STEPS, JS, OUTPUTS)) void linear_gradients_kernel(const Walks a) {
+template <int TY, int STEPS, int TILES, int JS, bool FULL> __global__ __launch_bounds__(256, walk_waves(TY, STEPS, TILES, JS, OUTPUTS)) void linear_gradients_kernel(const Walks a) {
     const uint32_t waves = a.v.blocks + a.k.blocks + a.q.blocks, unit = unit_of_wave(), rest = unit / waves;
     const uint32_t bh = rest / a.v.segments, segment = rest % a.v.segments;
     if (bh >= a.v.batch * a.v.heads) return;
     const uint32_t at = unit % waves, back = a.v.blocks + a.k.blocks;
     if (at < back) {
         const bool v = at < a.v.blocks;
-        walk<TY, STEPS, JS, true, OUTPUTS, FULL>(v ? a.v : a.k, bh, segment, v ? at : at - a.v.blocks, 0, unit);
+        walk<TY, STEPS, TILES, JS, true, OUTPUTS, FULL>(v ? a.v : a.k, bh, segment, v ? at : at - a.v.blocks, 0, unit);
     } else {
-        walk<TY, STEPS, JS, false, OUTPUTS, FULL>(a.q, bh, segment, at - back, 0, unit);
+        walk<TY, STEPS, TILES, JS, false, OUTPUTS, FULL>(a.q, bh, segment, at - back, 0, unit);
     }
 }
 
@@ -676,10 +823,15 @@ inline dim3 walk_grid(uint64_t units) { return dim3((uint32_t)((units + 31) / 32
 // 64 columns where the registers bear them and a walk has more than 32. (Waves of 32 read and multiply A and B twice:
 // WAVE_FIGURES.)
 template <int TY, class F> void by_shape(int steps, std::initializer_list<Walk*> walks, F&& launch) {
+    const int length = (*walks.begin())->length;
     auto by_columns = [&](auto s) {
         constexpr int STEPS = decltype(s)::value;
         int most = 0;
-        for (const Walk* w : walks) most = std::max(most, w->dc);
+        uint64_t waves = 0;  // of 64 columns
+        for (const Walk* w : walks) {
+            most = std::max(most, w->dc);
+            waves += (uint64_t)w->batch * w->heads * w->segments * ((w->dc + 63) / 64);
+        }
         auto run = [&](auto js) {
             constexpr int width = 16 * decltype(js)::value;
             bool full = true;
@@ -687,10 +839,14 @@ template <int TY, class F> void by_shape(int steps, std::initializer_list<Walk*>
                 w->blocks = (w->dc + width - 1) / width;
                 full = full && w->da == 32 * STEPS && w->dc % width == 0;
             }
-            full ? launch(s, js, std::true_type{}) : launch(s, js, std::false_type{});
+            auto by_tiles = [&](auto tiles) { full ? launch(s, tiles, js, std::true_type{}) : launch(s, tiles, js, std::false_type{}); };
+            if constexpr (TALL_OK(TY, STEPS, decltype(js)::value)) {
+                if (length > 16) return by_tiles(std::integral_constant<int, 2>{});
+            }
+            by_tiles(std::integral_constant<int, 1>{});
         };
         if constexpr (STEPS < 4) {
-            if (most > WIDE) return run(std::integral_constant<int, 4>{});
+            if (most > 32 && waves >= 2048) return run(std::integral_constant<int, 4>{});
         }
         run(std::integral_constant<int, 2>{});
     };
@@ -701,21 +857,21 @@ template <int TY, class F> void by_shape(int steps, std::initializer_list<Walk*>
 
 template <int TY> hipError_t launch_walk(Walk w, Kind kind, bool back, hipStream_t stream) {
     const bool read = kind == OUTPUTS || kind == SLOPES;
-    by_shape<TY>(steps_of(w.da), {&w}, [&](auto steps, auto js, auto is_full) {
-        constexpr int STEPS = decltype(steps)::value, JS = decltype(js)::value;
+    by_shape<TY>(steps_of(w.da), {&w}, [&](auto steps, auto tiles, auto js, auto is_full) {
+        constexpr int STEPS = decltype(steps)::value, TILES = decltype(tiles)::value, JS = decltype(js)::value;
         constexpr bool FULL = decltype(is_full)::value;
         const uint64_t walks = (uint64_t)w.batch * w.heads * (read ? w.segments : w.segments - 1);
         if (kind == SLOPES || kind == STATES_SLOPE) {
             w.blocks = (w.dc + 31) / 32;
             const dim3 grid = walk_grid(walks * w.blocks * 2);
-            if (read) linear_walk_kernel<TY, STEPS, 1, false, SLOPES, FULL><<<grid, 256, 0, stream>>>(w);
-            else linear_walk_kernel<TY, STEPS, 1, false, STATES_SLOPE, FULL><<<grid, 256, 0, stream>>>(w);
+            if (read) linear_walk_kernel<TY, STEPS, 1, 1, false, SLOPES, FULL><<<grid, 256, 0, stream>>>(w);
+            else linear_walk_kernel<TY, STEPS, TILES, 1, false, STATES_SLOPE, FULL><<<grid, 256, 0, stream>>>(w);
             return;
         }
         const dim3 grid = walk_grid(walks * w.blocks);
-        if (kind == OUTPUTS) linear_walk_kernel<TY, STEPS, JS, false, OUTPUTS, FULL><<<grid, 256, 0, stream>>>(w);
-        else if (back) linear_walk_kernel<TY, STEPS, JS, true, STATES, FULL><<<grid, 256, 0, stream>>>(w);
-        else linear_walk_kernel<TY, STEPS, JS, false, STATES, FULL><<<grid, 256, 0, stream>>>(w);
+        if (kind == OUTPUTS) linear_walk_kernel<TY, STEPS, TILES, JS, false, OUTPUTS, FULL><<<grid, 256, 0, stream>>>(w);
+        else if (back) linear_walk_kernel<TY, STEPS, TILES, JS, true, STATES, FULL><<<grid, 256, 0, stream>>>(w);
+        else linear_walk_kernel<TY, STEPS, TILES, JS, false, STATES, FULL><<<grid, 256, 0, stream>>>(w);
     });
     if (!read && w.segments > 2) {
         const dim3 join(w.batch * w.heads * (uint32_t)((w.size + 255) / 256));
@@ -727,9 +883,9 @@ template <int TY> hipError_t launch_walk(Walk w, Kind kind, bool back, hipStream
 }
 
 template <int TY> hipError_t launch_gradients(Walk v, Walk k, Walk q, hipStream_t stream) {
-    by_shape<TY>(std::max(steps_of(v.da), steps_of(k.da)), {&v, &k, &q}, [&](auto steps, auto js, auto full) {
+    by_shape<TY>(std::max(steps_of(v.da), steps_of(k.da)), {&v, &k, &q}, [&](auto steps, auto tiles, auto js, auto full) {
         const dim3 grid = walk_grid((uint64_t)v.batch * v.heads * v.segments * (v.blocks + k.blocks + q.blocks));
-        linear_gradients_kernel<TY, decltype(steps)::value, decltype(js)::value, decltype(full)::value><<<grid, 256, 0, stream>>>(Walks{v, k, q});
+        linear_gradients_kernel<TY, decltype(steps)::value, decltype(tiles)::value, decltype(js)::value, decltype(full)::value><<<grid, 256, 0, stream>>>(Walks{v, k, q});
     });
     return hipGetLastError();
 }
