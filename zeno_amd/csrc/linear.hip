@@ -100,7 +100,7 @@ std::string check_outputs(const std::vector<Memory>& inputs, const std::vector<M
 Segments segments_of(const ZenoAmdLinearInputs& in) {
     const int64_t chunks = ((int64_t)in.length + kChunk - 1) / kChunk;
     const int64_t walks = (int64_t)heads_of(in) * blocks_of(in.value_dim);
-    static const int target = getenv("ZT") ? atoi(getenv("ZT")) : 2048, least = getenv("ZL") ? atoi(getenv("ZL")) : 4;
+    static const int target = getenv("ZT") ? atoi(getenv("ZT")) : 2048, least = getenv("ZL") ? atoi(getenv("ZL")) : 2;
     int64_t want = std::min(target / walks, chunks / least);
     if (want < 2) want = 1;
     const int64_t each = (chunks + want - 1) / want;

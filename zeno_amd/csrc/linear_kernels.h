@@ -361,7 +361,8 @@ __device__ __forceinline__ void walk(const Walk& a, const uint32_t bh, const uin
         if constexpr (READ)
 #pragma unroll
             for (int k = 0; k < tile_pairs; ++k) fine &= finite(p[k]);
-        if (cuts)  // nothing of the state passes: it must not be multiplied by zero if it is not finite
+        if (cuts) {  // nothing of the state passes: it must not be multiplied by zero if it is not finite
+            asm volatile("");  // a branch, not a look at every chunk
 #pragma unroll
             for (int i = 0; i < 2 * STEPS; ++i)
 #pragma unroll
@@ -369,6 +370,7 @@ __device__ __forceinline__ void walk(const Walk& a, const uint32_t bh, const uin
                     fine &= finite(S[i][j]);
                     if constexpr (SLOPE) fine &= finite(N[i][j]);
                 }
+        }
         return __ballot(!fine) == 0;
     };
 
