@@ -638,43 +638,38 @@ __device__ __forceinline__ void walk(const Walk& a, const uint32_t bh, const uin
     }
 }
 
-// The waves of neighbouring workgroups read the same rows: workgroups go to the eight dies in turn, so each
-// die is given a range of its own. Returns the number of this wave's work.
-__device__ __forceinline__ uint32_t unit_of_wave() {
+// Waves read the rows that their neighbours read, and workgroups go to the eight dies in turn: each die is given a
+// range of its own. Returns the number of this wave's work.
+template <int WAVES> __device__ __forceinline__ uint32_t unit_of_wave() {
     const uint32_t each = gridDim.x / 8;  // the grid is a multiple of 8
-    return __builtin_amdgcn_readfirstlane(((blockIdx.x & 7) * each + (blockIdx.x >> 3)) * 4 + (threadIdx.x >> 6));
+    return __builtin_amdgcn_readfirstlane(((blockIdx.x & 7) * each + (blockIdx.x >> 3)) * WAVES + (threadIdx.x >> 6));
 }
 
-// Waves a SIMD that the registers are cut down to: as many as the state, its rows and their operands bear.
-#ifndef TALL_OK
-#define TALL_OK(TY, STEPS, JS) ((TY) == T_BF16 || ((TY) == T_F16 && (STEPS) == 1))
-#endif
-#ifndef WV
-#define WV 2
-#endif
+// Waves a SIMD that the registers are cut down to: as many as the state, its rows and their operands bear without
+// spilling, which costs more than a wave gains (27 registers spilled: 415 us, none 306; 16384 sequences of 16, two heads of 64 x 64).
 constexpr int walk_waves(int type, int steps, int tiles, int js, int kind) {
-    if (tiles == 2) return steps == 4 ? 2 : WV;
     if (type == T_F32) return steps == 4 && (kind == OUTPUTS || kind == SLOPES) ? 1 : steps == 1 ? 3 : 2;
-    return steps == 4 ? 2 : js == 4 && steps == 2 ? 2 : kind == SLOPES || type == T_F16 ? 3 : 4;
+    return tiles == 2 || steps == 4 || (js == 4 && steps == 2) ? 2 : kind == SLOPES || type == T_F16 ? 3 : 4;
 }
 
 template <int TY, int STEPS, int TILES, int JS, bool BACK, int KIND, bool FULL>
 __global__ __launch_bounds__(256, walk_waves(TY, STEPS, TILES, JS, KIND)) void linear_walk_kernel(const Walk a) {
     constexpr bool READ = KIND == OUTPUTS || KIND == SLOPES;
     const uint32_t walks = READ ? a.segments : a.segments - 1;  // of the segments, all but the last in the walk's direction
-    const uint32_t unit = unit_of_wave(), block = unit / (JS == 1 ? 2 : 1) % a.blocks, rest = unit / (JS == 1 ? 2 : 1) / a.blocks;
+    const uint32_t unit = unit_of_wave<4>(), block = unit / (JS == 1 ? 2 : 1) % a.blocks, rest = unit / (JS == 1 ? 2 : 1) / a.blocks;
     const uint32_t bh = rest / walks, segment = rest % walks + (!READ && BACK ? 1 : 0);
     if (bh >= a.batch * a.heads) return;
     walk<TY, STEPS, TILES, JS, BACK, KIND, FULL>(a, bh, segment, block, JS == 1 ? unit & 1 : 0, unit);
 }
 
 // All gradients but g's: the walks of d_v, d_k and d_q of a head and segment side by side, as they read the
-// same rows.
+// same rows: of 4096 sequences of 32 tokens, four heads of 64 x 64, in bfloat16, 366 us, and one after the other 490.
+// A workgroup is one wave, as the three take unlike times (workgroups of four: 400 us).
 struct Walks {
     Walk v, k, q;
 };
-template <int TY, int STEPS, int TILES, int JS, bool FULL> __global__ __launch_bounds__(256, walk_waves(TY, STEPS, TILES, JS, OUTPUTS)) void linear_gradients_kernel(const Walks a) {
-    const uint32_t waves = a.v.blocks + a.k.blocks + a.q.blocks, unit = unit_of_wave(), rest = unit / waves;
+template <int TY, int STEPS, int TILES, int JS, bool FULL> __global__ __launch_bounds__(64, walk_waves(TY, STEPS, TILES, JS, OUTPUTS)) void linear_gradients_kernel(const Walks a) {
+    const uint32_t waves = a.v.blocks + a.k.blocks + a.q.blocks, unit = unit_of_wave<1>(), rest = unit / waves;
     const uint32_t bh = rest / a.v.segments, segment = rest % a.v.segments;
     if (bh >= a.v.batch * a.v.heads) return;
     const uint32_t at = unit % waves, back = a.v.blocks + a.k.blocks;
@@ -819,42 +814,50 @@ __global__ __launch_bounds__(256) void linear_step_kernel(const ZenoAmdLinearInp
 }
 
 // ---- launches ------------------------------------------------------------------------------
-inline dim3 walk_grid(uint64_t units) { return dim3((uint32_t)((units + 31) / 32 * 8)); }  // a multiple of 8 workgroups of four waves
+inline dim3 walk_grid(uint64_t units, int waves) { return dim3((uint32_t)((units + 8 * waves - 1) / (8 * waves) * 8)); }
 
-// Runs launch(steps, js, full) with the launch shape as constants, and sets the walks' number of blocks: waves of
-// 64 columns where the registers bear them and a walk has more than 32. (Waves of 32 read and multiply A and B twice:
-// WAVE_FIGURES.)
+// Runs launch(steps, tiles, js, full) with the launch shape as constants, and sets the walks' number of blocks.
+// Waves of 64 columns where the registers bear them and enough of them come of it for two a SIMD: they read and multiply
+// A and B once where two of 32 do it twice (4096 sequences of 32, four heads of 64 x 64, bfloat16: 178 us, 192; but 19 of
+// 333 tokens, four heads of 24 x 48 with gradients: 213, 174). Chunks of two tiles where the registers bear them: what
+// is done to the state, its parts as operands and its decay, is done for 32 tokens at once (the same 4096 sequences with
+// gradients: 552, 579).
 template <int TY, class F> void by_shape(int steps, std::initializer_list<Walk*> walks, F&& launch) {
-    const int length = (*walks.begin())->length;
-    auto by_columns = [&](auto s) {
+    constexpr std::integral_constant<int, 1> one{};
+    constexpr std::integral_constant<int, 2> two{};
+    constexpr std::integral_constant<int, 4> four{};
+    int most = 0;
+    uint64_t waves = 0;  // of 64 columns
+    for (const Walk* w : walks) {
+        most = std::max(most, w->dc);
+        waves += (uint64_t)w->batch * w->heads * w->segments * ((w->dc + 63) / 64);
+    }
+    const bool wide = most > 32 && waves >= 2048, tall = (*walks.begin())->length > 16;
+    auto by_steps = [&](auto s) {
         constexpr int STEPS = decltype(s)::value;
-        int most = 0;
-        uint64_t waves = 0;  // of 64 columns
-        for (const Walk* w : walks) {
-            most = std::max(most, w->dc);
-            waves += (uint64_t)w->batch * w->heads * w->segments * ((w->dc + 63) / 64);
-        }
-        auto run = [&](auto js) {
+        auto by_full = [&](auto tiles, auto js) {
             constexpr int width = 16 * decltype(js)::value;
             bool full = true;
             for (Walk* w : walks) {
                 w->blocks = (w->dc + width - 1) / width;
                 full = full && w->da == 32 * STEPS && w->dc % width == 0;
             }
-            auto by_tiles = [&](auto tiles) { full ? launch(s, tiles, js, std::true_type{}) : launch(s, tiles, js, std::false_type{}); };
-            if constexpr (TALL_OK(TY, STEPS, decltype(js)::value)) {
-                if (length > 16) return by_tiles(std::integral_constant<int, 2>{});
+            full ? launch(s, tiles, js, std::true_type{}) : launch(s, tiles, js, std::false_type{});
+        };
+        auto by_tiles = [&](auto js) {
+            if constexpr (TY == T_BF16 || (TY == T_F16 && STEPS == 1)) {
+                if (tall) return by_full(two, js);
             }
-            by_tiles(std::integral_constant<int, 1>{});
+            by_full(one, js);
         };
         if constexpr (STEPS < 4) {
-            if (most > 32 && waves >= 2048) return run(std::integral_constant<int, 4>{});
+            if (wide) return by_tiles(four);
         }
-        run(std::integral_constant<int, 2>{});
+        by_tiles(two);
     };
-    if (steps == 1) by_columns(std::integral_constant<int, 1>{});
-    else if (steps == 2) by_columns(std::integral_constant<int, 2>{});
-    else by_columns(std::integral_constant<int, 4>{});
+    if (steps == 1) by_steps(one);
+    else if (steps == 2) by_steps(two);
+    else by_steps(four);
 }
 
 template <int TY> hipError_t launch_walk(Walk w, Kind kind, bool back, hipStream_t stream) {
@@ -865,12 +868,12 @@ template <int TY> hipError_t launch_walk(Walk w, Kind kind, bool back, hipStream
         const uint64_t walks = (uint64_t)w.batch * w.heads * (read ? w.segments : w.segments - 1);
         if (kind == SLOPES || kind == STATES_SLOPE) {
             w.blocks = (w.dc + 31) / 32;
-            const dim3 grid = walk_grid(walks * w.blocks * 2);
+            const dim3 grid = walk_grid(walks * w.blocks * 2, 4);
             if (read) linear_walk_kernel<TY, STEPS, 1, 1, false, SLOPES, FULL><<<grid, 256, 0, stream>>>(w);
             else linear_walk_kernel<TY, STEPS, TILES, 1, false, STATES_SLOPE, FULL><<<grid, 256, 0, stream>>>(w);
             return;
         }
-        const dim3 grid = walk_grid(walks * w.blocks);
+        const dim3 grid = walk_grid(walks * w.blocks, 4);
         if (kind == OUTPUTS) linear_walk_kernel<TY, STEPS, TILES, JS, false, OUTPUTS, FULL><<<grid, 256, 0, stream>>>(w);
         else if (back) linear_walk_kernel<TY, STEPS, TILES, JS, true, STATES, FULL><<<grid, 256, 0, stream>>>(w);
         else linear_walk_kernel<TY, STEPS, TILES, JS, false, STATES, FULL><<<grid, 256, 0, stream>>>(w);
@@ -886,8 +889,8 @@ template <int TY> hipError_t launch_walk(Walk w, Kind kind, bool back, hipStream
 
 template <int TY> hipError_t launch_gradients(Walk v, Walk k, Walk q, hipStream_t stream) {
     by_shape<TY>(std::max(steps_of(v.da), steps_of(k.da)), {&v, &k, &q}, [&](auto steps, auto tiles, auto js, auto full) {
-        const dim3 grid = walk_grid((uint64_t)v.batch * v.heads * v.segments * (v.blocks + k.blocks + q.blocks));
-        linear_gradients_kernel<TY, decltype(steps)::value, decltype(tiles)::value, decltype(js)::value, decltype(full)::value><<<grid, 256, 0, stream>>>(Walks{v, k, q});
+        const dim3 grid = walk_grid((uint64_t)v.batch * v.heads * v.segments * (v.blocks + k.blocks + q.blocks), 1);
+        linear_gradients_kernel<TY, decltype(steps)::value, decltype(tiles)::value, decltype(js)::value, decltype(full)::value><<<grid, 64, 0, stream>>>(Walks{v, k, q});
     });
     return hipGetLastError();
 }
