@@ -120,11 +120,12 @@ template <bool FULL> __device__ __forceinline__ void store_floats(float* at, int
     }
 }
 
-// This lane's number, found anew: what depends on it is then not kept in registers from use to use.
+// This lane's number, found anew: what depends on it is then not kept in registers from use to use. (The empty asm hides
+// where the zero comes from; it holds no instruction, so the compiler's waits stay right.)
 __device__ __forceinline__ int lane_anew() {
-    int m;
-    asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(m));
-    return m;
+    uint32_t zero = 0;
+    asm volatile("" : "+v"(zero));
+    return (int)__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, zero));
 }
 
 // Operands along the tokens of a chunk: of two tiles or of one.
