@@ -43,32 +43,18 @@ gradients of tokens up to its own only, through o, and none beyond a reset.
 """
 from __future__ import annotations
 
-import contextlib
-import ctypes as C
 from typing import Optional, Tuple
 
 import torch
 
 from . import _lib as L
-
-L.one_runtime()
-
-_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
-_S3 = C.c_int64 * 3
-_HERE = contextlib.nullcontext()
-_written = torch.autograd.graph.increment_version
-
-
-def _fail(rc: int, what: str) -> None:
-    if rc == -6:
-        raise ValueError(L.last_error())
-    raise RuntimeError(f"{what} failed: {rc}: {L.last_error()}")
+from ._torch import DTYPES, S3, dense_like, fail, on, pointer, row, space as bytes_for, stream, written
 
 
 def _check(q, k, v, g, beta, reset, state, lead: int) -> None:
     """Shapes, types and devices; `lead` is the number of dimensions before the heads."""
     dtype, device, qs, vs, gs = q.dtype, q.device, q.shape, v.shape, g.shape
-    if dtype not in _DTYPES:
+    if dtype not in DTYPES:
         raise TypeError(f"q, k and v must be float32, float16 or bfloat16, not {dtype}")
     if len(qs) != lead + 2 or len(vs) != lead + 2:
         raise ValueError(f"q and v must have {lead + 2} dimensions, not {len(qs)} and {len(vs)}")
@@ -111,10 +97,6 @@ def _check_step(v, state, out) -> None:
         raise ValueError(f"out must be like v: {tuple(v.shape)}, {v.dtype}, on {v.device}, its last dimension contiguous")
 
 
-def _row(x: torch.Tensor) -> torch.Tensor:
-    return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
-
-
 def _inputs(q, k, v, g, beta, reset, state, scale, normalize) -> L.ZenoAmdDeltaInputs:
     qs, ks, vs, gs, bs = q.stride(), k.stride(), v.stride(), g.stride(), beta.stride()
     rs = (0, 0) if reset is None else reset.stride()
@@ -127,28 +109,15 @@ def _inputs(q, k, v, g, beta, reset, state, scale, normalize) -> L.ZenoAmdDeltaI
         rs = (rs[0], 0)
     _, hv, dv = v.shape[-3:]
     return L.ZenoAmdDeltaInputs(
-        _DTYPES[q.dtype], b, t, hk, hv, dk, dv, normalize, scale,
+        DTYPES[q.dtype], b, t, hk, hv, dk, dv, normalize, scale,
         q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(),
         None if reset is None else reset.data_ptr(), None if state is None else state.data_ptr(), qs, ks, vs, gs, bs, rs)
-
-
-def _space(n: int, x: torch.Tensor) -> Optional[torch.Tensor]:
-    return torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
-
-
-def _stream(x: torch.Tensor) -> int:
-    return torch.cuda.current_stream(x.device).cuda_stream
-
-
-def _on(x: torch.Tensor):
-    """The context in which x's device is the current one, as the library's calls need it."""
-    return _HERE if torch.cuda.current_device() == x.device.index else torch.cuda.device(x.device)
 
 
 class _GatedDelta(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, g, beta, reset, state, scale, normalize, train):
-        with _on(q):
+        with on(q):
             lib = L.load()
             a = _inputs(q, k, v, g, beta, reset, state, scale, normalize)
             o = torch.empty_like(v)  # v's order of dimensions: time-major in, time-major out
@@ -156,11 +125,11 @@ class _GatedDelta(torch.autograd.Function):
                 o = torch.empty(v.shape, dtype=v.dtype, device=v.device)
             last = torch.empty((q.shape[0], v.shape[2], q.shape[3], v.shape[3]), dtype=torch.float32, device=q.device)
             saved = torch.empty(max(lib.zeno_amd_delta_saved_bytes(a), 1), dtype=torch.uint8, device=q.device) if train else None
-            space = _space(lib.zeno_amd_delta_workspace_bytes(a), q)
-            rc = lib.zeno_amd_delta_forward(a, o.data_ptr(), _S3(*o.stride()[:3]), last.data_ptr(),
-                                            None if saved is None else saved.data_ptr(), None if space is None else space.data_ptr(), _stream(q))
+            space = bytes_for(lib.zeno_amd_delta_workspace_bytes(a), q)
+            rc = lib.zeno_amd_delta_forward(a, o.data_ptr(), S3(*o.stride()[:3]), last.data_ptr(),
+                                            None if saved is None else saved.data_ptr(), None if space is None else space.data_ptr(), stream(q))
             if rc:
-                _fail(rc, "gated_delta")
+                fail(rc, "gated_delta")
         if train:
             ctx.save_for_backward(q, k, v, g, beta, reset, state, last, saved)
             ctx.scale, ctx.normalize = scale, normalize
@@ -173,31 +142,25 @@ class _GatedDelta(torch.autograd.Function):
         q, k, v, g, beta, reset, state, last, saved = ctx.saved_tensors
         if d_o is None and d_last is None:
             return (None,) * 10
-        with _on(q):
+        with on(q):
             lib = L.load()
             a = _inputs(q, k, v, g, beta, reset, state, ctx.scale, ctx.normalize)
-            d_o = torch.zeros_like(v) if d_o is None else _row(d_o)
+            d_o = torch.zeros_like(v) if d_o is None else row(d_o)
             d_last = None if d_last is None else d_last.contiguous()
-            d_q, d_k, d_v = (_dense_like(x) for x in (q, k, v))
-            d_g, d_beta = _dense_like(g), _dense_like(beta)
+            d_q, d_k, d_v = (dense_like(x) for x in (q, k, v))
+            d_g, d_beta = torch.empty_like(g), torch.empty_like(beta)
             d_state = torch.empty_like(state) if state is not None and ctx.needs_input_grad[6] else None
-            space = _space(lib.zeno_amd_delta_workspace_bytes(a), q)
+            space = bytes_for(lib.zeno_amd_delta_workspace_bytes(a), q)
             grads = L.ZenoAmdDeltaGradients(
-                d_o.data_ptr(), _S3(*d_o.stride()[:3]), None if d_last is None else d_last.data_ptr(),
+                d_o.data_ptr(), S3(*d_o.stride()[:3]), None if d_last is None else d_last.data_ptr(),
                 d_q.data_ptr(), d_k.data_ptr(), d_v.data_ptr(), d_g.data_ptr(), d_beta.data_ptr(),
                 None if d_state is None else d_state.data_ptr(),
-                *(_S3(*x.stride()[:3]) for x in (d_q, d_k, d_v, d_g, d_beta)))
+                *(S3(*x.stride()[:3]) for x in (d_q, d_k, d_v, d_g, d_beta)))
             rc = lib.zeno_amd_delta_backward(a, last.data_ptr(), saved.data_ptr(), grads, None if space is None else space.data_ptr(),
-                                             _stream(q))
+                                             stream(q))
             if rc:
-                _fail(rc, "gated_delta's gradients")
+                fail(rc, "gated_delta's gradients")
         return d_q, d_k, d_v, d_g, d_beta, None, d_state, None, None, None
-
-
-def _dense_like(x: torch.Tensor) -> torch.Tensor:
-    """Memory for x's gradient in x's order of dimensions, each value at a place of its own."""
-    y = torch.empty_like(x)
-    return y if y.stride(-1) == 1 or x.shape[-1] == 1 or x.dim() == 3 else torch.empty(x.shape, dtype=x.dtype, device=x.device)
 
 
 def gated_delta(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, beta: torch.Tensor,
@@ -207,7 +170,7 @@ def gated_delta(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tens
     state after the last token, a new tensor. Differentiable in q, k, v, g, beta and state."""
     _check(q, k, v, g, beta, reset, state, 2)
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
-    q, k, v = _row(q), _row(k), _row(v)
+    q, k, v = row(q), row(k), row(v)
     state = None if state is None else state.contiguous()
     train = torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in (q, k, v, g, beta, state))
     return _GatedDelta.apply(q, k, v, g, beta, reset, state, scale, bool(normalize), train)
@@ -222,17 +185,17 @@ def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
     gated_delta on the recorded rollout."""
     _check(q, k, v, g, beta, reset, state, 1)
     _check_step(v, state, out)
-    q, k, v = _row(q), _row(k), _row(v)
+    q, k, v = row(q), row(k), row(v)
     if out is None:
         out = torch.empty_like(v, memory_format=torch.contiguous_format)
-    with _on(q):
+    with on(q):
         a = _inputs(q, k, v, g, beta, reset, state, q.shape[-1] ** -0.5 if scale is None else float(scale), bool(normalize))
         os = out.stride()
-        rc = L.load().zeno_amd_delta_step(a, out.data_ptr(), _S3(os[0], 0, os[1]), state.data_ptr(), _stream(q))
+        rc = L.load().zeno_amd_delta_step(a, out.data_ptr(), S3(os[0], 0, os[1]), state.data_ptr(), stream(q))
         if rc:
-            _fail(rc, "gated_delta_step")
-    _written(state)  # autograd refuses a backward pass that needs what was here
-    _written(out)
+            fail(rc, "gated_delta_step")
+    written(state)  # autograd refuses a backward pass that needs what was here
+    written(out)
     return out
 
 
@@ -256,29 +219,31 @@ def _linear_inputs(q, k, v, g, reset, state, scale, learned) -> L.ZenoAmdLinearI
         rs = (rs[0], 0)
     _, hv, dv = v.shape[-3:]
     return L.ZenoAmdLinearInputs(
-        _DTYPES[q.dtype], b, t, hk, hv, dk, dv, learned, scale, q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(),
+        DTYPES[q.dtype], b, t, hk, hv, dk, dv, learned, scale, q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(),
         None if reset is None else reset.data_ptr(), None if state is None else state.data_ptr(), qs, ks, vs, rs)
+
+
+def _linear_forward(q, k, v, g, reset, state, scale, learned, train):
+    with on(q):
+        lib = L.load()
+        a = _linear_inputs(q, k, v, g, reset, state, scale, learned)
+        o = dense_like(v)  # v's order of dimensions: time-major in, time-major out
+        last = torch.empty((q.shape[0], v.shape[2], q.shape[3], v.shape[3]), dtype=torch.float32, device=q.device)
+        saved = bytes_for(lib.zeno_amd_linear_saved_bytes(a), q) if train else None
+        space = bytes_for(lib.zeno_amd_linear_workspace_bytes(a, 0), q)
+        rc = lib.zeno_amd_linear_forward(a, o.data_ptr(), S3(*o.stride()[:3]), last.data_ptr(), pointer(saved), pointer(space), stream(q))
+        if rc:
+            fail(rc, "linear_attention")
+    return o, last, saved
 
 
 class _LinearAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, g, reset, state, scale, train):
-        learned = train and g.requires_grad
-        with _on(q):
-            lib = L.load()
-            a = _linear_inputs(q, k, v, g, reset, state, scale, learned)
-            o = _dense_like(v)  # v's order of dimensions: time-major in, time-major out
-            last = torch.empty((q.shape[0], v.shape[2], q.shape[3], v.shape[3]), dtype=torch.float32, device=q.device)
-            saved = _space(lib.zeno_amd_linear_saved_bytes(a), q) if train else None
-            space = _space(lib.zeno_amd_linear_workspace_bytes(a, 0), q)
-            rc = lib.zeno_amd_linear_forward(a, o.data_ptr(), _S3(*o.stride()[:3]), last.data_ptr(), None if saved is None else saved.data_ptr(),
-                                             None if space is None else space.data_ptr(), _stream(q))
-            if rc:
-                _fail(rc, "linear_attention")
-        if train:
-            ctx.save_for_backward(q, k, v, g, reset, state, saved)
-            ctx.scale, ctx.learned = scale, learned
-            ctx.set_materialize_grads(False)
+    def forward(ctx, q, k, v, g, reset, state, scale):
+        ctx.scale, ctx.learned = scale, g.requires_grad
+        o, last, saved = _linear_forward(q, k, v, g, reset, state, scale, ctx.learned, True)
+        ctx.save_for_backward(q, k, v, g, reset, state, saved)
+        ctx.set_materialize_grads(False)
         return o, last
 
     @staticmethod
@@ -286,24 +251,23 @@ class _LinearAttention(torch.autograd.Function):
     def backward(ctx, d_o, d_last):
         q, k, v, g, reset, state, saved = ctx.saved_tensors
         if d_o is None and d_last is None:
-            return (None,) * 8
-        with _on(q):
+            return (None,) * 7
+        with on(q):
             lib = L.load()
             a = _linear_inputs(q, k, v, g, reset, state, ctx.scale, ctx.learned)
-            d_o = torch.zeros_like(v) if d_o is None else _row(d_o)
+            d_o = torch.zeros_like(v) if d_o is None else row(d_o)
             d_last = None if d_last is None else d_last.contiguous()
-            d_q, d_k, d_v = (_dense_like(x) for x in (q, k, v))
+            d_q, d_k, d_v = (dense_like(x) for x in (q, k, v))
             d_g = torch.empty_like(g) if ctx.learned else None
             d_state = torch.empty_like(state) if state is not None and ctx.needs_input_grad[5] else None
-            space = _space(lib.zeno_amd_linear_workspace_bytes(a, 1), q)
+            space = bytes_for(lib.zeno_amd_linear_workspace_bytes(a, 1), q)
             grads = L.ZenoAmdLinearGradients(
-                d_o.data_ptr(), _S3(*d_o.stride()[:3]), None if d_last is None else d_last.data_ptr(), d_q.data_ptr(), d_k.data_ptr(), d_v.data_ptr(),
-                None if d_g is None else d_g.data_ptr(), None if d_state is None else d_state.data_ptr(),
-                *(_S3(*x.stride()[:3]) for x in (d_q, d_k, d_v)))
-            rc = lib.zeno_amd_linear_backward(a, None if saved is None else saved.data_ptr(), grads, None if space is None else space.data_ptr(), _stream(q))
+                d_o.data_ptr(), S3(*d_o.stride()[:3]), pointer(d_last), d_q.data_ptr(), d_k.data_ptr(), d_v.data_ptr(), pointer(d_g), pointer(d_state),
+                *(S3(*x.stride()[:3]) for x in (d_q, d_k, d_v)))
+            rc = lib.zeno_amd_linear_backward(a, pointer(saved), grads, pointer(space), stream(q))
             if rc:
-                _fail(rc, "linear_attention's gradients")
-        return d_q, d_k, d_v, d_g, None, d_state, None, None
+                fail(rc, "linear_attention's gradients")
+        return d_q, d_k, d_v, d_g, None, d_state, None
 
 
 def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, reset: Optional[torch.Tensor] = None,
@@ -312,10 +276,11 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
     state after the last token, a new tensor. Differentiable in q, k, v, g and state."""
     _check_linear(q, k, v, g, reset, state, 2)
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
-    q, k, v, g = _row(q), _row(k), _row(v), g.contiguous()
+    q, k, v, g = row(q), row(k), row(v), g.contiguous()
     state = None if state is None else state.contiguous()
-    train = torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in (q, k, v, g, state))
-    return _LinearAttention.apply(q, k, v, g, reset, state, scale, train)
+    if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in (q, k, v, g, state)):
+        return _LinearAttention.apply(q, k, v, g, reset, state, scale)
+    return _linear_forward(q, k, v, g, reset, state, scale, False, False)[:2]
 
 
 def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, state: torch.Tensor,
@@ -324,15 +289,15 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: 
     reset [B]. `state`, `out` and gradients are as gated_delta_step has them."""
     _check_linear(q, k, v, g, reset, state, 1)
     _check_step(v, state, out)
-    q, k, v, g = _row(q), _row(k), _row(v), g.contiguous()
+    q, k, v, g = row(q), row(k), row(v), g.contiguous()
     if out is None:
         out = torch.empty_like(v, memory_format=torch.contiguous_format)
-    with _on(q):
+    with on(q):
         a = _linear_inputs(q, k, v, g, reset, state, q.shape[-1] ** -0.5 if scale is None else float(scale), False)
         os = out.stride()
-        rc = L.load().zeno_amd_linear_step(a, out.data_ptr(), _S3(os[0], 0, os[1]), state.data_ptr(), _stream(q))
+        rc = L.load().zeno_amd_linear_step(a, out.data_ptr(), S3(os[0], 0, os[1]), state.data_ptr(), stream(q))
         if rc:
-            _fail(rc, "linear_attention_step")
-    _written(state)  # autograd refuses a backward pass that needs what was here
-    _written(out)
+            fail(rc, "linear_attention_step")
+    written(state)  # autograd refuses a backward pass that needs what was here
+    written(out)
     return out

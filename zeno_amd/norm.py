@@ -16,99 +16,79 @@ gradients are rounded once, and are the same from run to run.
 """
 from __future__ import annotations
 
-from typing import Optional, Tuple, Union
-
 import ctypes as C
+from typing import Optional, Tuple, Union
 
 import torch
 
 from . import _lib as L
+from ._torch import DTYPES, S3, dense_like, fail, on, pointer, row, space, stream
 
-L.one_runtime()
-
-_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
-_S3 = C.c_int64 * 3
 _U3 = C.c_uint32 * 3
-
-
-def _fail(rc: int, what: str) -> None:
-    if rc == -6:
-        raise ValueError(L.last_error())
-    raise RuntimeError(f"{what} failed: {rc}: {L.last_error()}")
-
-
-def _row(x: torch.Tensor) -> torch.Tensor:
-    return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
-
-
-def _like(x: torch.Tensor) -> torch.Tensor:
-    """Memory in x's order of dimensions, each value at a place of its own, rows contiguous."""
-    y = torch.empty_like(x)
-    return y if y.stride(-1) == 1 or x.shape[-1] == 1 else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+_NONE = S3()
 
 
 def _strides(x: Optional[torch.Tensor]):
     if x is None:
-        return _S3()
-    s = x.stride()[:-1]
-    return _S3(*(0,) * (3 - len(s)), *s)
+        return _NONE
+    s = x.stride()
+    return S3(s[0], s[1], s[2]) if len(s) == 4 else S3(0, s[0], s[1]) if len(s) == 3 else S3(0, 0, s[0]) if len(s) == 2 else _NONE
 
 
 def _inputs(x, residual, weight, bias, eps) -> L.ZenoAmdNormInputs:
-    rows = x.shape[:-1]
-    w = weight if weight is not None else bias
+    shape, dtype = x.shape, DTYPES[x.dtype]
+    w = bias if weight is None else weight
     return L.ZenoAmdNormInputs(
-        _DTYPES[x.dtype], _DTYPES[x.dtype if w is None else w.dtype], _U3(*(1,) * (3 - len(rows)), *rows), x.shape[-1], eps, x.data_ptr(),
-        None if residual is None else residual.data_ptr(), None if weight is None else weight.data_ptr(),
-        None if bias is None else bias.data_ptr(), _strides(x), _strides(residual))
+        dtype, dtype if w is None else DTYPES[w.dtype], _U3(*(1,) * (4 - len(shape)), *shape[:-1]), shape[-1], eps, x.data_ptr(), pointer(residual),
+        pointer(weight), pointer(bias), _strides(x), _strides(residual))
+
+
+def _forward(x, weight, bias, residual, eps):
+    with on(x):
+        y = dense_like(x)
+        total = None if residual is None else dense_like(x)
+        rc = L.load().zeno_amd_norm_forward(_inputs(x, residual, weight, bias, eps), y.data_ptr(), _strides(y), pointer(total), _strides(total), stream(x))
+        if rc:
+            fail(rc, "layer_norm")
+    return y, total
 
 
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, eps):
-        with torch.cuda.device(x.device):
-            y = _like(x)
-            total = None if residual is None else _like(x)
-            rc = L.load().zeno_amd_norm_forward(_inputs(x, residual, weight, bias, eps), y.data_ptr(), _strides(y),
-                                                None if total is None else total.data_ptr(), _strides(total),
-                                                torch.cuda.current_stream(x.device).cuda_stream)
-            if rc:
-                _fail(rc, "layer_norm")
-        if any(ctx.needs_input_grad):
-            ctx.save_for_backward(x if total is None else total, weight, bias)
-            ctx.eps = eps
-            ctx.set_materialize_grads(False)
+        y, total = _forward(x, weight, bias, residual, eps)
+        ctx.save_for_backward(x if total is None else total, weight, bias)
+        ctx.eps = eps
+        ctx.set_materialize_grads(False)
         return y if total is None else (y, total)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_y, d_sum=None):
-        s, weight, bias = ctx.saved_tensors
-        want_x, want_weight, want_bias, want_residual = ctx.needs_input_grad[:4]
         if d_y is None and d_sum is None:
             return (None,) * 5
-        with torch.cuda.device(s.device):
+        s, weight, bias = ctx.saved_tensors
+        want_x, want_weight, want_bias, want_residual = ctx.needs_input_grad[:4]
+        with on(s):
             lib = L.load()
-            d_y = torch.zeros_like(s) if d_y is None else _row(d_y)
-            d_sum = None if d_sum is None else _row(d_sum)
+            d_y = torch.zeros_like(s) if d_y is None else row(d_y)
+            d_sum = None if d_sum is None else row(d_sum)
             a = _inputs(s, None, weight, bias, ctx.eps)
-            d_x = _like(s) if want_x or want_residual else None
+            d_x = dense_like(s) if want_x or want_residual else None
             d_weight = torch.empty_like(weight) if want_weight else None
             d_bias = torch.empty_like(bias) if want_bias else None
-            space = None
-            if want_weight or want_bias:
-                space = torch.empty(lib.zeno_amd_norm_workspace_bytes(a), dtype=torch.uint8, device=s.device)
-            grads = L.ZenoAmdNormGradients(d_y.data_ptr(), *(None if z is None else z.data_ptr() for z in (d_sum, d_x, d_weight, d_bias)),
+            parts = space(lib.zeno_amd_norm_workspace_bytes(a), s) if want_weight or want_bias else None
+            grads = L.ZenoAmdNormGradients(d_y.data_ptr(), pointer(d_sum), pointer(d_x), pointer(d_weight), pointer(d_bias),
                                            _strides(d_y), _strides(d_sum), _strides(d_x))
-            rc = lib.zeno_amd_norm_backward(a, grads, None if space is None else space.data_ptr(), torch.cuda.current_stream(s.device).cuda_stream)
+            rc = lib.zeno_amd_norm_backward(a, grads, pointer(parts), stream(s))
             if rc:
-                _fail(rc, "layer_norm's gradients")
+                fail(rc, "layer_norm's gradients")
         return d_x if want_x else None, d_weight, d_bias, d_x if want_residual else None, None
 
 
 def _check(x, weight, bias, residual) -> None:
     dtype, shape, device = x.dtype, x.shape, x.device
-    if dtype not in _DTYPES:
+    if dtype not in DTYPES:
         raise TypeError(f"x must be float32, float16 or bfloat16, not {dtype}")
     if not shape or 0 in shape:
         raise ValueError(f"x must hold rows of features, not {tuple(shape)}")
@@ -143,7 +123,12 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
         residual = None if residual is None else residual.flatten(0, len(shape) - 4)
     weight = None if weight is None else weight.contiguous()
     bias = None if bias is None else bias.contiguous()
-    out = _LayerNorm.apply(_row(x), weight, bias, None if residual is None else _row(residual), float(eps))
+    x, residual = row(x), None if residual is None else row(residual)
+    if torch.is_grad_enabled() and any(z is not None and z.requires_grad for z in (x, weight, bias, residual)):
+        out = _LayerNorm.apply(x, weight, bias, residual, float(eps))
+    else:
+        y, total = _forward(x, weight, bias, residual, float(eps))
+        out = y if total is None else (y, total)
     if len(shape) > 4:
         return out.view(shape) if residual is None else tuple(y.view(shape) for y in out)
     return out
