@@ -76,6 +76,79 @@ def decay_size(x, h, do, ds, scale):
     return float(torch.autograd.grad(total, one["g"])[0])
 
 
+# Batches large enough for waves of 64 columns (2048 of them), one chunk or several, whole and odd dimensions, shared heads;
+# and, the last two, for walks of gradients that are wide where the forward's are not.
+MANY = [(2048, 9, 1, 1, 64, 64), (1030, 37, 1, 2, 33, 63), (700, 33, 3, 3, 64, 64), (520, 20, 2, 4, 24, 40), (2050, 3, 1, 1, 32, 48), (1030, 17, 1, 1, 20, 100),
+        (700, 40, 1, 1, 64, 33), (720, 18, 1, 1, 63, 16)]
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("shape", MANY, ids=str)
+def test_many_sequences(shape, dtype):
+    check_train(inputs(*shape, dtype, seed=sum(shape)))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_many_sequences_with_values_that_are_not_finite(bad, dtype):
+    """Waves of 64 columns: one sequence has such a value, between resets; no other row of it and no other
+    sequence or head is reached."""
+    from zeno_amd.memory import linear_attention as ours
+
+    b, t, h, d = 1024, 44, 2, 64
+    x = inputs(b, t, 1, h, d, d, dtype, seed=14, resets=0.05)
+    x["reset"][:, 12] = x["reset"][:, 30] = True
+    x["state"][7, 1] = bad  # and a state, up to its first reset
+    spoilt = {n: y.clone() for n, y in x.items()}
+    spoilt["v"][500, 20, 1, 40] = bad
+    spoilt["k"][501, 20, 0, 3] = bad
+    spoilt["q"][502, 20, 0, 63] = bad
+    tol = 2 * HALF_ULP[dtype] + 2 * tolerance(t, d, d)
+    results = []
+    for y in (x, spoilt):
+        dev = {n: z.cuda().requires_grad_(z.is_floating_point() and n != "g") for n, z in y.items()}
+        o, s = ours(**dev)
+        results.append([o, s, *torch.autograd.grad(o.float().square().sum() + s.square().sum(), [dev[n] for n in "qkv"])])
+    clean, other = results
+    apart = torch.ones(b, t, dtype=torch.bool)
+    apart[500:503, 12:30] = False
+    apart[7, :12] = False
+    for n, p, r in zip(("o", "state", "q", "k", "v"), other, clean):
+        p, r = p.cpu(), r.cpu()
+        if n == "state":
+            assert_near(p, r, tol, n)
+            continue
+        # The squares' gradient is 2 o, so that its rounding comes on top.
+        assert_near(p[apart], r[apart], tol if n == "o" else 4 * tol, n)
+    o, ref = other[0].cpu(), clean[0].cpu()
+    assert torch.isfinite(ref[500:503]).all()
+    for c in (slice(0, 40), slice(41, 64)):
+        assert_near(o[500, :, 1, c], ref[500, :, 1, c], tol, "other columns")
+    assert_near(o[500, :, 0], ref[500, :, 0], tol, "the other head")
+    assert_near(o[502, 21:], ref[502, 21:], tol, "behind a query")
+    assert not torch.isfinite(o[500, 20, 1, 40]) and not torch.isfinite(o[501, 20]).all() and not torch.isfinite(o[502, 20]).any()
+
+
+def test_small_half_precision_values():
+    """float16 rows below its smallest normal value: products are of the values themselves."""
+    x = inputs(3, 70, 1, 2, 64, 64, torch.float16, seed=21, resets=0.05)
+    for n in "qk":
+        x[n] = (x[n].float() * 2.0 ** -18).half()  # 64 steps of 2^-24
+    x["state"] *= 2.0 ** -18
+    from zeno_amd.memory import linear_attention as ours
+
+    # The scale brings the outputs back to normal values, of which half a step is the rounding.
+    o, s = ours(**on_gpu(x), scale=2.0 ** 32)
+    want, last = definition(**x, scale=2.0 ** 32)
+    assert_near(o, want, HALF_ULP[torch.float16] + tolerance(70, 64, 64), "o")
+    assert_near(s, last, tolerance(70, 64, 64), "state")
+
+
+def test_many_heads_of_long_sequences_are_not_cut():
+    """As many waves as fill the device: no segments, and many chunks to a walk."""
+    check_train(inputs(128, 300, 2, 16, 8, 16, torch.bfloat16, seed=31, resets=0.01))
+
+
 # (batch, length, key heads, value heads, key_dim, value_dim): every launch shape of every type,
 # lengths around the chunks of 16 and 32 and of one and several segments, odd dimensions
 SHAPES = [(2, 1, 1, 1, 8, 8), (3, 15, 2, 2, 16, 24), (2, 16, 1, 2, 64, 64), (2, 17, 2, 2, 32, 32), (3, 31, 1, 1, 32, 64), (2, 32, 1, 2, 64, 32), (2, 33, 2, 6, 33, 65),

@@ -117,8 +117,10 @@ std::string check_sizes(const ZenoAmdLinearInputs& in, bool step) {
     if (in.value_heads % in.key_heads) return "value_heads is not a multiple of key_heads";
     if (!in.key_dim || in.key_dim > ZENO_AMD_LINEAR_MAX_DIM || !in.value_dim || in.value_dim > ZENO_AMD_LINEAR_MAX_DIM)
         return "key_dim and value_dim must be 1 to " + std::to_string(ZENO_AMD_LINEAR_MAX_DIM);
-    // A launch takes less than 2^32 threads: up to four waves for each sequence and head.
-    if (in.length > 0x7fffff00u || heads_of(in) > 0xffffff00ull / 256) return "too many sequences or tokens";
+    // A launch takes less than 2^32 threads, and is rounded up to 32 waves. Each sequence and head is up to four waves, and
+    // with dimensions over 64 twelve (three gradients, four waves of 32 columns each).
+    const uint64_t waves = std::max(in.key_dim, in.value_dim) > 64 ? 12 : 4;
+    if (in.length > 0x7fffff00u || heads_of(in) > ((1ull << 32) / 64 - 32) / waves) return "too many sequences or tokens";
     if (step && in.length != 1) return "a step takes one token";
     return "";
 }
