@@ -4,7 +4,8 @@ The scene's sensors give positions and velocities of the cart and the pole; the 
 two positions, so it has to remember what it saw to know how fast they move. Its memory layer is
 the gated delta rule: `gated_delta_step` advances every environment's state beside each step of
 the simulation, `gated_delta` runs the recorded rollout and its gradients, and `orthogonalize`
-makes the update of the policy's matrices.
+makes the update of the policy's matrices. With `--memory linear` the layer is linear attention,
+`linear_attention_step` and `linear_attention`, each head's output normalised by `layer_norm`.
 
     python examples/memory_policy.py --envs 1024 --updates 100
 
@@ -19,7 +20,8 @@ import torch
 
 sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 from zeno_amd import make  # noqa: E402
-from zeno_amd.memory import gated_delta, gated_delta_step  # noqa: E402
+from zeno_amd.memory import gated_delta, gated_delta_step, linear_attention, linear_attention_step  # noqa: E402
+from zeno_amd.norm import layer_norm  # noqa: E402
 from zeno_amd.optim import orthogonalize  # noqa: E402
 
 HEADS, DIM, HIDDEN = 2, 32, 64
@@ -30,7 +32,7 @@ FALLEN, OFF_RAIL = 0.6, 4.0
 class Policy:
     """Positions -> features -> memory -> mean action, as plain tensors."""
 
-    def __init__(self, seed: int):
+    def __init__(self, seed: int, memory: str = "delta"):
         g = torch.Generator(device="cuda").manual_seed(seed)
 
         def matrix(rows, cols, gain=1.0):
@@ -39,16 +41,39 @@ class Policy:
         wide = HEADS * DIM
         self.matrices = {"seen": matrix(len(SEEN), HIDDEN, 2.0), "qkv": matrix(HIDDEN, 3 * wide), "gates": matrix(HIDDEN, 2 * HEADS),
                          "act": matrix(HIDDEN + wide, 1, 0.1)}
+        if memory == "linear":
+            del self.matrices["gates"]
+        self.decays = -torch.exp(torch.linspace(-4.0, -1.0, HEADS, device="cuda"))  # linear attention's: slow and fast heads
+        self.linear = memory == "linear"
         self.momenta = {n: torch.zeros_like(w) for n, w in self.matrices.items()}
 
     def project(self, seen):
         """What the memory layer takes, for one token or a whole rollout."""
         x = torch.tanh(seen @ self.matrices["seen"])
         q, k, v = (y.unflatten(-1, (HEADS, DIM)) for y in (x @ self.matrices["qkv"]).split(HEADS * DIM, -1))
+        if self.linear:
+            return x, q, k, v
         g, beta = (x @ self.matrices["gates"]).split(HEADS, -1)
         return x, q, k, v, torch.nn.functional.logsigmoid(g + 3.0), torch.sigmoid(beta)
 
+    def remember(self, token, state, reset):
+        """One token of every environment; the state is advanced in place."""
+        if self.linear:
+            return linear_attention_step(*token, self.decays, state, reset)
+        return gated_delta_step(*token, state, reset, normalize=True)
+
+    def recall(self, tokens, begins, first):
+        """The whole rollout, time-major."""
+        tokens, begins = [y.transpose(0, 1) for y in tokens], begins.transpose(0, 1)
+        if self.linear:
+            o, _ = linear_attention(*tokens, self.decays, begins, first)
+        else:
+            o, _ = gated_delta(*tokens, begins, first, normalize=True)
+        return o.transpose(0, 1)
+
     def mean(self, x, o):
+        if self.linear:
+            o = layer_norm(o, eps=1e-2)
         return (torch.cat([x, o.flatten(-2)], -1) @ self.matrices["act"])[..., 0]
 
     def update(self, grads, rate):
@@ -58,12 +83,12 @@ class Policy:
                 w.sub_(rate * max(1.0, w.shape[0] / w.shape[1]) ** 0.5 * orthogonalize(m))
 
 
-def train(envs: int, updates: int, length: int, seed: int = 0, rate: float = 0.03, noise: float = 0.5, log=print):
+def train(envs: int, updates: int, length: int, seed: int = 0, rate: float = 0.03, noise: float = 0.5, log=print, memory: str = "delta"):
     """Returns the mean length of the episodes that ended during each update, and how far the
-    rollout's outputs, as they were acted, are from those the training pass computes."""
+    rollout's outputs, as they were acted, are from those the training pass computes, of the largest where it is over 1."""
     torch.manual_seed(seed)
     rng = torch.Generator(device="cuda").manual_seed(seed + 1)
-    policy, env = Policy(seed), make("cartpole", num_envs=envs)
+    policy, env = Policy(seed, memory), make("cartpole", num_envs=envs)
     obs = env.reset()
     state = torch.zeros(envs, HEADS, DIM, DIM, device="cuda")
     began = np.ones(envs, dtype=bool)  # this step begins an episode
@@ -76,7 +101,7 @@ def train(envs: int, updates: int, length: int, seed: int = 0, rate: float = 0.0
                 s = torch.from_numpy(obs[:, SEEN]).cuda()
                 reset = torch.from_numpy(began).cuda()
                 x, *token = policy.project(s)
-                o = gated_delta_step(*token, state, reset, normalize=True)
+                o = policy.remember(token, state, reset)
                 act = policy.mean(x, o) + noise * torch.randn(envs, generator=rng, device="cuda")
                 seen.append(s), begins.append(reset), actions.append(act), outputs.append(o)
                 obs = env.step(act.clamp(-1, 1).cpu().numpy()[:, None])[0]
@@ -99,9 +124,8 @@ def train(envs: int, updates: int, length: int, seed: int = 0, rate: float = 0.0
         advantage = (returns - returns.mean(1, keepdim=True)) / (returns.std() + 1e-6)
 
         x, *tokens = policy.project(seen)
-        o, _ = gated_delta(*(y.transpose(0, 1) for y in tokens), begins.transpose(0, 1), first, normalize=True)
-        o = o.transpose(0, 1)
-        apart = max(apart, float((o.detach() - torch.stack(outputs)).abs().max()))
+        o = policy.recall(tokens, begins, first)
+        apart = max(apart, float((o.detach() - torch.stack(outputs)).abs().max() / o.detach().abs().max().clamp(min=1.0)))
         loss = (0.5 * ((actions - policy.mean(x, o)) / noise).square() * advantage).mean()
         policy.update(torch.autograd.grad(loss, list(policy.matrices.values())), rate * (1.0 - step / updates))
         history.append(float(np.mean(lengths)) if lengths else float(age.mean()))
@@ -117,5 +141,6 @@ if __name__ == "__main__":
     ap.add_argument("--updates", type=int, default=100)
     ap.add_argument("--length", type=int, default=128)
     ap.add_argument("--seed", type=int, default=0)
+    ap.add_argument("--memory", choices=("delta", "linear"), default="delta")
     a = ap.parse_args()
-    train(a.envs, a.updates, a.length, a.seed)
+    train(a.envs, a.updates, a.length, a.seed, memory=a.memory)
