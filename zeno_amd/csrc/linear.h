@@ -71,8 +71,7 @@ enum Kind { OUTPUTS, SLOPES, STATES, STATES_SLOPE };
 // One translation unit per element type.
 template <int TY> hipError_t launch_walk(Walk w, Kind kind, bool back, hipStream_t stream);
 template <int TY> hipError_t launch_gradients(Walk v, Walk k, Walk q, hipStream_t stream);
-template <int TY> hipError_t launch_share(const float* parts, void* out, const int64_t* stride, uint32_t batch, uint32_t length, uint32_t key_heads, uint32_t share,
-                                          uint32_t dim, hipStream_t stream);
+template <int TY> hipError_t launch_share(const ZenoAmdLinearInputs& in, const float* part_q, const float* part_k, const ZenoAmdLinearGradients& grad, hipStream_t stream);
 template <int TY> hipError_t launch_step(const ZenoAmdLinearInputs& in, void* o, const int64_t* o_stride, float* state, hipStream_t stream);
 
 // Of the single step: a wave holds all rows of 4 `lanes` columns of a head.

@@ -247,8 +247,7 @@ hipError_t backward(const ZenoAmdLinearInputs& in, const float* saved, const Zen
     }
     if (share > 1) {
         auto add = in.dtype == T_F32 ? launch_share<T_F32> : in.dtype == T_F16 ? launch_share<T_F16> : launch_share<T_BF16>;
-        if ((e = add(part_q, grad.d_q, grad.d_q_stride, in.batch, in.length, in.key_heads, share, in.key_dim, stream))) return e;
-        if ((e = add(part_k, grad.d_k, grad.d_k_stride, in.batch, in.length, in.key_heads, share, in.key_dim, stream))) return e;
+        return add(in, part_q, part_k, grad, stream);
     }
     return hipGetLastError();
 }

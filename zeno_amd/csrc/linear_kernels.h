@@ -253,7 +253,7 @@ __device__ __forceinline__ void walk(const Walk& a, const uint32_t bh, const uin
 
     // ---- the head's decays between the tokens of a chunk of `len` with resets in `cuts`; 0 across a reset, and where
     // a token is behind the other. `read`: of the state to a token, `write`: of a token to the next state, `all`: of
-    // the state to the next.
+    // the state to the next. None is over more than `len` tokens: behind the last token zeros are multiplied by them, which must not be infinite.
     gh = gh < -200.0f ? -200.0f : gh;  // 0 in fp32 from one token to the next
     constexpr int tile_pairs = TILES == 2 ? 3 : 1;  // each tile with itself, and the first with the second
     float near[tile_pairs][4], read[TILES], all;
@@ -268,20 +268,20 @@ __device__ __forceinline__ void walk(const Walk& a, const uint32_t bh, const uin
 #pragma unroll
         for (int k = 0; k < TILES; ++k) {
             const int i = 16 * k + i0;
-            read[k] = BACK ? decay(gh, max(len - 1 - i, 0)) : a.scale * decay(gh, i + 1);
+            read[k] = BACK ? decay(gh, max(len - 1 - i, 0)) : a.scale * decay(gh, min(i + 1, len));
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int j = 16 * k + j0 + r;
-                write[k][r] = BACK ? a.scale * decay(gh, j + 1) : decay(gh, max(len - 1 - j, 0));
+                write[k][r] = BACK ? a.scale * decay(gh, min(j + 1, len)) : decay(gh, max(len - 1 - j, 0));
             }
         }
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int apart = BACK ? j0 + r - i0 : i0 - j0 - r;
-            near[0][r] = apart < 0 ? 0.0f : a.scale * decay(gh, max(apart, 0));
+            near[0][r] = apart < 0 ? 0.0f : a.scale * decay(gh, min(max(apart, 0), len));
             if constexpr (TILES == 2) {
                 near[1][r] = near[0][r];
-                near[2][r] = a.scale * decay(gh, 16 + apart);
+                near[2][r] = a.scale * decay(gh, min(16 + apart, len));
             }
         }
         if (cuts) {
@@ -726,18 +726,25 @@ template <bool BACK, bool SLOPE> __global__ __launch_bounds__(256) void linear_j
     }
 }
 
-// Sums the value heads of each key head, in their order; a thread a value, several where there are more
-// than 2^28 (a launch takes less than 2^32 threads). Bound by memory, of which the parts in fp32 are most.
-template <int TY>
-__global__ __launch_bounds__(256) void linear_share_kernel(const float* parts, void* out, int64_t s0, int64_t s1, int64_t s2, int64_t all, uint32_t length, uint32_t heads,
-                                                           uint32_t share, uint32_t dim) {
+// Sums the value heads of each key head, in their order, for q and for k (blockIdx.y); a thread a value, several where there
+// are more than 2^28 (a launch takes less than 2^32 threads). Bound by memory, of which the parts in fp32 are most.
+struct Shared {
+    const float* parts[2];
+    void* out[2];
+    int64_t stride[2][3], all;
+    uint32_t length, heads, share, dim;
+};
+template <int TY> __global__ __launch_bounds__(256) void linear_share_kernel(const Shared a) {
     typedef typename Elem<TY>::type E;
-    for (int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x; id < all; id += (int64_t)gridDim.x * 256) {
-        const int64_t x = id % dim, h = id / dim % heads, bt = id / dim / heads;
-        const float* from = parts + (bt * heads + h) * share * dim + x;
+    const float* parts = a.parts[blockIdx.y];
+    E* out = (E*)a.out[blockIdx.y];
+    const int64_t* stride = a.stride[blockIdx.y];
+    for (int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x; id < a.all; id += (int64_t)gridDim.x * 256) {
+        const int64_t x = id % a.dim, h = id / a.dim % a.heads, bt = id / a.dim / a.heads;
+        const float* from = parts + (bt * a.heads + h) * a.share * a.dim + x;
         float sum = 0.0f;
-        for (uint32_t s = 0; s < share; ++s) sum += from[(int64_t)s * dim];
-        ((E*)out)[bt / length * s0 + bt % length * s1 + h * s2 + x] = Elem<TY>::put(sum);
+        for (uint32_t s = 0; s < a.share; ++s) sum += from[(int64_t)s * a.dim];
+        out[bt / a.length * stride[0] + bt % a.length * stride[1] + h * stride[2] + x] = Elem<TY>::put(sum);
     }
 }
 
@@ -904,10 +911,13 @@ template <int TY> hipError_t launch_gradients(Walk v, Walk k, Walk q, hipStream_
     return hipGetLastError();
 }
 
-template <int TY> hipError_t launch_share(const float* parts, void* out, const int64_t* stride, uint32_t batch, uint32_t length, uint32_t key_heads, uint32_t share,
-                                          uint32_t dim, hipStream_t stream) {
-    const int64_t all = (int64_t)batch * length * key_heads * dim, blocks = (all + 255) / 256, most = 1 << 20;
-    linear_share_kernel<TY><<<dim3((uint32_t)(blocks < most ? blocks : most)), 256, 0, stream>>>(parts, out, stride[0], stride[1], stride[2], all, length, key_heads, share, dim);
+template <int TY> hipError_t launch_share(const ZenoAmdLinearInputs& in, const float* part_q, const float* part_k, const ZenoAmdLinearGradients& grad, hipStream_t stream) {
+    Shared a{{part_q, part_k}, {grad.d_q, grad.d_k}, {}, (int64_t)in.batch * in.length * in.key_heads * in.key_dim, in.length, in.key_heads, in.value_heads / in.key_heads, in.key_dim};
+    for (int i = 0; i < 3; ++i) {
+        a.stride[0][i] = grad.d_q_stride[i];
+        a.stride[1][i] = grad.d_k_stride[i];
+    }
+    linear_share_kernel<TY><<<dim3((uint32_t)std::min<int64_t>((a.all + 255) / 256, 1 << 20), 2), 256, 0, stream>>>(a);
     return hipGetLastError();
 }
 
