@@ -9,6 +9,10 @@
 // The backward pass finds mean and r again from s, which it has to read anyway: two sums of values
 // in registers for 8 bytes a row less each way.
 //
+// Bound by memory. Forward, bfloat16: 524288 rows of 64 23 us, 131072 of 512 44, 16384 of 4096 45, that is 5.8 to 6.1 TB/s;
+// 65536 of 1000 in float32 106, 4.9. Gradients, whose sums by column hold twice the registers and so fewer waves: 131072 of
+// 512 89 us, 4.5 TB/s; 65536 of 1000 in float32 163, 4.8; 8192 of 8192 116, 3.5 (two barriers a row of 1024 threads).
+//
 // A row is held in registers by LANES lanes of a wave (or by a workgroup), V vectors of eight
 // elements each, so memory is read once. A lane keeps its columns from row to row: the weights stay
 // in registers and the sums of dw and db too, until each workgroup writes its own and a second
