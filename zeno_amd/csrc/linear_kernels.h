@@ -9,9 +9,9 @@
 // they are a table in registers that is made once.
 //
 // A wave owns 32 or 64 columns of the state, all of its rows, and works alone: no LDS, no barrier. That leaves no
-// wait but for memory, and the vector instructions bound it: they are issued 70 % of the time in 16384 tokens of 8 heads of
-// 128 x 128 (the matrix units work 15 % of it), the rest being waits for rows. Many short sequences are bound by memory:
-// 16384 of 16 tokens, two heads of 64 x 64, bfloat16: 1.34 GB in 275 to 294 us, 4.6 to 4.9 TB/s.
+// wait but for memory, and the vector instructions bound it: of 16384 tokens of 8 heads of 128 x 128, float16, each of a SIMD's two
+// waves issues them 37 % of its time and keeps the matrix units busy for 24 % (outputs 87 us). Many short sequences are bound by
+// memory: 16384 of 16 tokens, two heads of 64 x 64, bfloat16: 1.34 GB in 267 us, 5.0 TB/s.
 // Rows are read as they lie, 16 bytes a lane: lane (n, g) has row n's dimensions 8 g to 8 g + 7 of
 // every 32. That is an operand of the matrix units as it is, for contractions along the dimensions.
 // The other operands come from results without an exchange: a result tile has its rows in registers and
