@@ -141,6 +141,23 @@ def test_captured_and_replayed(t):
         assert all(torch.equal(p, q) for p, q in zip(out, eager)), i
 
 
+def test_tangents_are_refused():
+    """Forward-mode differentiation, which the operators do not have, is an error and no result without a tangent."""
+    import torch.autograd.forward_ad as forward
+
+    from zeno_amd.memory import linear_attention
+    from zeno_amd.norm import layer_norm
+
+    q = torch.randn(1, 4, 1, 8, device="cuda")
+    with forward.dual_level():
+        dual = forward.make_dual(q, torch.ones_like(q))
+        with pytest.raises(RuntimeError):
+            linear_attention(dual, q, q, torch.zeros(1, device="cuda"))
+        with pytest.raises(RuntimeError):
+            layer_norm(dual)
+    assert torch.isfinite(layer_norm(q)).all()
+
+
 def test_the_example_with_linear_attention():
     spec = importlib.util.spec_from_file_location("memory_policy", Path(__file__).resolve().parents[1] / "examples" / "memory_policy.py")
     example = importlib.util.module_from_spec(spec)

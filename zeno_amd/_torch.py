@@ -47,5 +47,10 @@ def on(x: torch.Tensor):
     return _HERE if torch.cuda.current_device() == x.device.index else torch.cuda.device(x.device)
 
 
+def differentiated(*operands: Optional[torch.Tensor]) -> bool:
+    """Whether a call has to go through autograd: for gradients, or to be refused where tangents are carried forward."""
+    return (torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in operands)) or torch.autograd.forward_ad._current_level >= 0
+
+
 def pointer(x: Optional[torch.Tensor]) -> Optional[int]:
     return None if x is None else x.data_ptr()

@@ -48,7 +48,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib as L
-from ._torch import DTYPES, S3, dense_like, fail, on, pointer, row, space as bytes_for, stream, written
+from ._torch import DTYPES, S3, dense_like, differentiated, fail, on, pointer, row, space as bytes_for, stream, written
 
 
 def _check(q, k, v, g, beta, reset, state, lead: int) -> None:
@@ -278,7 +278,7 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
     q, k, v, g = row(q), row(k), row(v), g.contiguous()
     state = None if state is None else state.contiguous()
-    if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in (q, k, v, g, state)):
+    if differentiated(q, k, v, g, state):
         return _LinearAttention.apply(q, k, v, g, reset, state, scale)
     return _linear_forward(q, k, v, g, reset, state, scale, False, False)[:2]
 

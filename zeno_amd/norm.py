@@ -24,7 +24,7 @@ from typing import Optional, Tuple, Union
 import torch
 
 from . import _lib as L
-from ._torch import DTYPES, S3, dense_like, fail, on, pointer, row, space, stream
+from ._torch import DTYPES, S3, dense_like, differentiated, fail, on, pointer, row, space, stream
 
 _U3 = C.c_uint32 * 3
 _NONE = S3()
@@ -126,7 +126,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     weight = None if weight is None else weight.contiguous()
     bias = None if bias is None else bias.contiguous()
     x, residual = row(x), None if residual is None else row(residual)
-    if torch.is_grad_enabled() and any(z is not None and z.requires_grad for z in (x, weight, bias, residual)):
+    if differentiated(x, weight, bias, residual):
         out = _LayerNorm.apply(x, weight, bias, residual, float(eps))
     else:
         y, total = _forward(x, weight, bias, residual, float(eps))
