@@ -56,6 +56,11 @@ struct Walk {
 
 // A wave holds 32 times 1, 2 or 4 rows of a state.
 inline int steps_of(int da) { return da <= 32 ? 1 : da <= 64 ? 2 : 4; }
+// Tiles of 16 columns of a wave of the decays' gradient, which carries the state and its slope, where `waves` of 32 columns would
+// do. Two where they fill two a SIMD and the registers bear it: 4096 sequences of 32 tokens, four heads of 64 x 64, bfloat16: 233 us,
+// with one 271; 300 of 200, float32: 154, 179. With fewer waves one (19 of 333, four heads of 24 x 48, float32: 25 us, 36), and with
+// 32 rows (300 of 200, 32 x 32, bfloat16: 37, 39); with 128 rows two spill 145 registers.
+constexpr int slope_tiles(int steps, uint64_t waves) { return steps == 2 && waves >= 2048 ? 2 : 1; }
 struct Segments {
     uint32_t count;
     int length;

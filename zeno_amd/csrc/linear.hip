@@ -17,16 +17,26 @@ using mma::T_F32;
 
 namespace {
 
-// The gradient of g: the walks' parts of each head, in order, in 64 bits.
-__global__ __launch_bounds__(256) void linear_decay_kernel(const double* parts, uint32_t batch, uint32_t heads, uint32_t each, float* d_g) {
-    __shared__ double all[256];
+// The gradient of g: the walks' parts of each head, in order, in 64 bits. Bound by the wait for each read, so eight are
+// read at once, by as many threads as a workgroup has.
+__global__ __launch_bounds__(1024) void linear_decay_kernel(const double* parts, uint32_t batch, uint32_t heads, uint32_t each, float* d_g) {
+    __shared__ double all[1024];
     const uint32_t h = blockIdx.x;
     const int64_t n = (int64_t)batch * each;
     double sum = 0.0;
-    for (int64_t i = threadIdx.x; i < n; i += 256) sum += parts[(i / each * heads + h) * each + i % each];
+    for (int64_t i = threadIdx.x; i < n; i += 8 * 1024) {
+        double x[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int64_t at = i + 1024 * k;
+            x[k] = at < n ? parts[(at / each * heads + h) * each + at % each] : 0.0;
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) sum += x[k];
+    }
     all[threadIdx.x] = sum;
     __syncthreads();
-    for (int d = 128; d; d >>= 1) {
+    for (int d = 512; d; d >>= 1) {
         if ((int)threadIdx.x < d) all[threadIdx.x] += all[threadIdx.x + d];
         __syncthreads();
     }
@@ -43,7 +53,11 @@ uint64_t states_floats(const ZenoAmdLinearInputs& in) { return even(between(in) 
 uint64_t share_floats(const ZenoAmdLinearInputs& in) {  // gradients of q (or k) by value head
     return in.key_heads == in.value_heads ? 0 : even((uint64_t)in.batch * in.length * in.value_heads * in.key_dim);
 }
-uint64_t parts_floats(const ZenoAmdLinearInputs& in) { return in.decay_gradient ? even(2 * heads_of(in) * segments_of(in).count * 2 * blocks_of(in.key_dim)) : 0; }
+uint32_t slope_waves(const ZenoAmdLinearInputs& in) {  // of a head and segment
+    const uint32_t blocks = blocks_of(in.key_dim);
+    return 2 / slope_tiles(steps_of(in.value_dim), heads_of(in) * segments_of(in).count * blocks) * blocks;
+}
+uint64_t parts_floats(const ZenoAmdLinearInputs& in) { return in.decay_gradient ? even(2 * heads_of(in) * segments_of(in).count * slope_waves(in)) : 0; }
 
 void set_strides(int64_t* to, const int64_t* from) {
     for (int i = 0; i < 3; ++i) to[i] = from[i];
@@ -243,7 +257,7 @@ hipError_t backward(const ZenoAmdLinearInputs& in, const float* saved, const Zen
     if ((e = gradients(wv, wk, wq, stream))) return e;
     if (grad.d_g) {
         if ((e = launch(in.dtype, wq, SLOPES, false, stream))) return e;
-        linear_decay_kernel<<<in.value_heads, 256, 0, stream>>>(wq.parts, in.batch, in.value_heads, wq.segments * 2 * blocks_of(in.key_dim), grad.d_g);
+        linear_decay_kernel<<<in.value_heads, 1024, 0, stream>>>(wq.parts, in.batch, in.value_heads, wq.segments * slope_waves(in), grad.d_g);
     }
     if (share > 1) {
         auto add = in.dtype == T_F32 ? launch_share<T_F32> : in.dtype == T_F16 ? launch_share<T_F16> : launch_share<T_BF16>;

@@ -459,7 +459,7 @@ __device__ __forceinline__ void walk(const Walk& a, const uint32_t bh, const uin
                         qr[k].get(q);
 #pragma unroll
                         for (int r = 0; r < 4; ++r)
-                            pairs += ((float)(16 * k + n + 1) * x[k][r] + (read[k] != 0.0f ? slope[k][r] * read[k] : 0.0f)) * (half ? q[4 + r] : q[r]);
+                            pairs += ((float)(16 * k + n + 1) * x[k][r] + (read[k] != 0.0f ? slope[k][r] * read[k] : 0.0f)) * (JS == 1 ? half ? q[4 + r] : q[r] : q[4 * (j & 1) + r]);
                     }
                 }
                 if constexpr (OUT) {
@@ -653,6 +653,7 @@ template <int WAVES> __device__ __forceinline__ uint32_t unit_of_wave() {
 // spilling, which costs more than a wave gains (27 registers spilled: 415 us, none 306; 16384 sequences of 16, two heads of 64 x 64).
 constexpr int walk_waves(int type, int steps, int tiles, int js, int kind) {
     if (type == T_F32) return steps == 4 && (kind == OUTPUTS || kind == SLOPES) ? 1 : steps == 1 ? 3 : 2;
+    if (js == 2 && kind == SLOPES) return 2;
     return tiles == 2 || steps == 4 || (js == 4 && steps == 2) ? 2 : kind == SLOPES || type == T_F16 ? 3 : 4;
 }
 
@@ -881,6 +882,11 @@ template <int TY> hipError_t launch_walk(Walk w, Kind kind, bool back, hipStream
         const uint64_t walks = (uint64_t)w.batch * w.heads * (read ? w.segments : w.segments - 1);
         if (kind == SLOPES || kind == STATES_SLOPE) {
             w.blocks = (w.dc + 31) / 32;
+            if constexpr (STEPS == 2)
+                if (read && slope_tiles(STEPS, walks * w.blocks) == 2) {
+                    linear_walk_kernel<TY, STEPS, 1, 2, false, SLOPES, FULL><<<walk_grid(walks * w.blocks, 4), 256, 0, stream>>>(w);
+                    return;
+                }
             const dim3 grid = walk_grid(walks * w.blocks * 2, 4);
             if (read) linear_walk_kernel<TY, STEPS, 1, 1, false, SLOPES, FULL><<<grid, 256, 0, stream>>>(w);
             else linear_walk_kernel<TY, STEPS, TILES, 1, false, STATES_SLOPE, FULL><<<grid, 256, 0, stream>>>(w);
