@@ -50,17 +50,17 @@ struct Walk {
     int segment_length;          // tokens, whole chunks
     float *starts, *slopes, *passes;
     const float* d_last;         // for the gradient of g; null: zeros
-    double* parts;               // of it: [batch, heads, segments, blocks, 2]
+    double* parts;               // of it: [batch, heads, segments, waves]
     uint32_t blocks;             // waves that share the columns, set at the launch
 };
 
 // A wave holds 32 times 1, 2 or 4 rows of a state.
 inline int steps_of(int da) { return da <= 32 ? 1 : da <= 64 ? 2 : 4; }
-// Tiles of 16 columns of a wave of the decays' gradient, which carries the state and its slope, where `waves` of 32 columns would
-// do. Two where they fill two a SIMD and the registers bear it: 4096 sequences of 32 tokens, four heads of 64 x 64, bfloat16: 233 us,
-// with one 271; 300 of 200, float32: 154, 179. With fewer waves one (19 of 333, four heads of 24 x 48, float32: 25 us, 36), and with
-// 32 rows (300 of 200, 32 x 32, bfloat16: 37, 39); with 128 rows two spill 145 registers.
-constexpr int slope_tiles(int steps, uint64_t waves) { return steps == 2 && waves >= 2048 ? 2 : 1; }
+// Tiles of 16 columns of a wave of the decays' gradient, which carries the state and its slope; `js` is of the waves beside it. Two
+// where there are many waves and the registers bear it: by themselves those of 4096 sequences of 32 tokens, four heads of
+// 64 x 64, bfloat16, take 233 us, with one tile 271; of 300 of 200, float32, 154 and 179. With few waves one (19 of 333, four heads of
+// 24 x 48, float32: 25 us, 36), and with 32 rows (300 of 200, 32 x 32, bfloat16: 37, 39); with 128 rows two spill 145 registers.
+constexpr int slope_tiles(int steps, int js) { return steps == 2 && js == 4 ? 2 : 1; }
 struct Segments {
     uint32_t count;
     int length;
@@ -75,7 +75,7 @@ enum Kind { OUTPUTS, SLOPES, STATES, STATES_SLOPE };
 
 // One translation unit per element type.
 template <int TY> hipError_t launch_walk(Walk w, Kind kind, bool back, hipStream_t stream);
-template <int TY> hipError_t launch_gradients(Walk v, Walk k, Walk q, hipStream_t stream);
+template <int TY> hipError_t launch_gradients(Walk v, Walk k, Walk q, uint32_t* slopes, hipStream_t stream);
 template <int TY> hipError_t launch_share(const ZenoAmdLinearInputs& in, const float* part_q, const float* part_k, const ZenoAmdLinearGradients& grad, hipStream_t stream);
 template <int TY> hipError_t launch_step(const ZenoAmdLinearInputs& in, void* o, const int64_t* o_stride, float* state, hipStream_t stream);
 

@@ -53,11 +53,7 @@ uint64_t states_floats(const ZenoAmdLinearInputs& in) { return even(between(in) 
 uint64_t share_floats(const ZenoAmdLinearInputs& in) {  // gradients of q (or k) by value head
     return in.key_heads == in.value_heads ? 0 : even((uint64_t)in.batch * in.length * in.value_heads * in.key_dim);
 }
-uint32_t slope_waves(const ZenoAmdLinearInputs& in) {  // of a head and segment
-    const uint32_t blocks = blocks_of(in.key_dim);
-    return 2 / slope_tiles(steps_of(in.value_dim), heads_of(in) * segments_of(in).count * blocks) * blocks;
-}
-uint64_t parts_floats(const ZenoAmdLinearInputs& in) { return in.decay_gradient ? even(2 * heads_of(in) * segments_of(in).count * slope_waves(in)) : 0; }
+uint64_t parts_floats(const ZenoAmdLinearInputs& in) { return in.decay_gradient ? even(2 * heads_of(in) * segments_of(in).count * 2 * blocks_of(in.key_dim)) : 0; }
 
 void set_strides(int64_t* to, const int64_t* from) {
     for (int i = 0; i < 3; ++i) to[i] = from[i];
@@ -132,8 +128,8 @@ std::string check_sizes(const ZenoAmdLinearInputs& in, bool step) {
     if (!in.key_dim || in.key_dim > ZENO_AMD_LINEAR_MAX_DIM || !in.value_dim || in.value_dim > ZENO_AMD_LINEAR_MAX_DIM)
         return "key_dim and value_dim must be 1 to " + std::to_string(ZENO_AMD_LINEAR_MAX_DIM);
     // A launch takes less than 2^32 threads, and is rounded up to 32 waves. Each sequence and head is up to four waves, and
-    // with dimensions over 64 twelve (three gradients, four waves of 32 columns each).
-    const uint64_t waves = std::max(in.key_dim, in.value_dim) > 64 ? 12 : 4;
+    // with dimensions over 64 twenty (three gradients, four waves of 32 columns each, and the decays', eight of 16).
+    const uint64_t waves = std::max(in.key_dim, in.value_dim) > 64 ? 20 : 5;
     if (in.length > 0x7fffff00u || heads_of(in) > ((1ull << 32) / 64 - 32) / waves) return "too many sequences or tokens";
     if (step && in.length != 1) return "a step takes one token";
     return "";
@@ -249,16 +245,14 @@ hipError_t backward(const ZenoAmdLinearInputs& in, const float* saved, const Zen
     wq.first = in.state;
     wq.starts = const_cast<float*>(saved);
     wq.slopes = wq.starts + states_floats(in);
-    wq.parts = reinterpret_cast<double*>(parts);
+    wq.parts = grad.d_g ? reinterpret_cast<double*>(parts) : nullptr;
 
     hipError_t e;
     if (wv.segments > 1 && (e = launch(in.dtype, wv, STATES, true, stream))) return e;
     auto gradients = in.dtype == T_F32 ? launch_gradients<T_F32> : in.dtype == T_F16 ? launch_gradients<T_F16> : launch_gradients<T_BF16>;
-    if ((e = gradients(wv, wk, wq, stream))) return e;
-    if (grad.d_g) {
-        if ((e = launch(in.dtype, wq, SLOPES, false, stream))) return e;
-        linear_decay_kernel<<<in.value_heads, 1024, 0, stream>>>(wq.parts, in.batch, in.value_heads, wq.segments * slope_waves(in), grad.d_g);
-    }
+    uint32_t slopes;
+    if ((e = gradients(wv, wk, wq, &slopes, stream))) return e;
+    if (grad.d_g) linear_decay_kernel<<<in.value_heads, 1024, 0, stream>>>(wq.parts, in.batch, in.value_heads, wq.segments * slopes, grad.d_g);
     if (share > 1) {
         auto add = in.dtype == T_F32 ? launch_share<T_F32> : in.dtype == T_F16 ? launch_share<T_F16> : launch_share<T_BF16>;
         return add(in, part_q, part_k, grad, stream);

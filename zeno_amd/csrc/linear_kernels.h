@@ -656,10 +656,13 @@ constexpr int walk_waves(int type, int steps, int tiles, int js, int kind) {
     if (js == 2 && kind == SLOPES) return 2;
     return tiles == 2 || steps == 4 || (js == 4 && steps == 2) ? 2 : kind == SLOPES || type == T_F16 ? 3 : 4;
 }
+constexpr int gradient_waves(int type, int steps, int tiles, int js, bool learned) {
+    return learned ? std::min(walk_waves(type, steps, tiles, js, OUTPUTS), walk_waves(type, steps, 1, slope_tiles(steps, js), SLOPES)) : walk_waves(type, steps, tiles, js, OUTPUTS);
+}
 
 template <int TY, int STEPS, int TILES, int JS, bool BACK, int KIND, bool FULL>
 __global__ __launch_bounds__(256, walk_waves(TY, STEPS, TILES, JS, KIND)) void linear_walk_kernel(const Walk a) {
-    constexpr bool READ = KIND == OUTPUTS || KIND == SLOPES;
+    constexpr bool READ = KIND == OUTPUTS;
     const uint32_t walks = READ ? a.segments : a.segments - 1;  // of the segments, all but the last in the walk's direction
     const uint32_t unit = unit_of_wave<4>(), block = unit / (JS == 1 ? 2 : 1) % a.blocks, rest = unit / (JS == 1 ? 2 : 1) / a.blocks;
     const uint32_t bh = rest / walks, segment = rest % walks + (!READ && BACK ? 1 : 0);
@@ -667,22 +670,29 @@ __global__ __launch_bounds__(256, walk_waves(TY, STEPS, TILES, JS, KIND)) void l
     walk<TY, STEPS, TILES, JS, BACK, KIND, FULL>(a, bh, segment, block, JS == 1 ? unit & 1 : 0, unit);
 }
 
-// All gradients but g's: the walks of d_v, d_k and d_q of a head and segment side by side, as they read the
-// same rows: of 4096 sequences of 32 tokens, four heads of 64 x 64, in bfloat16, 366 us, and one after the other 490.
-// A workgroup is one wave, as the three take unlike times (workgroups of four: 400 us).
+// All gradients: the walks of d_v, d_k and d_q of a head and segment side by side, as they read the same rows: of 4096
+// sequences of 32 tokens, four heads of 64 x 64, in bfloat16, 366 us, and one after the other 490. Where the decays are learned
+// the walk of their gradient too: 520 us, by itself behind the others 366 and 235; 19 sequences of 333, four heads of 24 x 48, float32:
+// 36, and 34 and 25. A workgroup is one wave, as the walks take unlike times (workgroups of four, the first three: 400 us).
 struct Walks {
     Walk v, k, q;
+    uint32_t slopes;  // waves of the decays' gradient, for each head and segment
 };
-template <int TY, int STEPS, int TILES, int JS, bool FULL> __global__ __launch_bounds__(64, walk_waves(TY, STEPS, TILES, JS, OUTPUTS)) void linear_gradients_kernel(const Walks a) {
-    const uint32_t waves = a.v.blocks + a.k.blocks + a.q.blocks, unit = unit_of_wave<1>(), rest = unit / waves;
+template <int TY, int STEPS, int TILES, int JS, bool FULL, bool LEARNED>
+__global__ __launch_bounds__(64, gradient_waves(TY, STEPS, TILES, JS, LEARNED)) void linear_gradients_kernel(const Walks a) {
+    const uint32_t back = a.v.blocks + a.k.blocks, outputs = back + a.q.blocks, waves = outputs + (LEARNED ? a.slopes : 0), unit = unit_of_wave<1>(), rest = unit / waves;
     const uint32_t bh = rest / a.v.segments, segment = rest % a.v.segments;
     if (bh >= a.v.batch * a.v.heads) return;
-    const uint32_t at = unit % waves, back = a.v.blocks + a.k.blocks;
+    const uint32_t at = unit % waves;
     if (at < back) {
         const bool v = at < a.v.blocks;
-        walk<TY, STEPS, TILES, JS, true, OUTPUTS, FULL>(v ? a.v : a.k, bh, segment, v ? at : at - a.v.blocks, 0, unit);
+        walk<TY, STEPS, TILES, JS, true, OUTPUTS, FULL>(v ? a.v : a.k, bh, segment, v ? at : at - a.v.blocks, 0, 0);
+    } else if (!LEARNED || at < outputs) {
+        walk<TY, STEPS, TILES, JS, false, OUTPUTS, FULL>(a.q, bh, segment, at - back, 0, 0);
     } else {
-        walk<TY, STEPS, TILES, JS, false, OUTPUTS, FULL>(a.q, bh, segment, at - back, 0, unit);
+        constexpr int SJ = slope_tiles(STEPS, JS);
+        const uint32_t s = at - outputs;
+        walk<TY, STEPS, 1, SJ, false, SLOPES, FULL>(a.q, bh, segment, SJ == 1 ? s / 2 : s, SJ == 1 ? s & 1 : 0, rest * a.slopes + s);
     }
 }
 
@@ -875,21 +885,14 @@ template <int TY, class F> void by_shape(int steps, std::initializer_list<Walk*>
 }
 
 template <int TY> hipError_t launch_walk(Walk w, Kind kind, bool back, hipStream_t stream) {
-    const bool read = kind == OUTPUTS || kind == SLOPES;
+    const bool read = kind == OUTPUTS;
     by_shape<TY>(steps_of(w.da), {&w}, [&](auto steps, auto tiles, auto js, auto is_full) {
         constexpr int STEPS = decltype(steps)::value, TILES = decltype(tiles)::value, JS = decltype(js)::value;
         constexpr bool FULL = decltype(is_full)::value;
         const uint64_t walks = (uint64_t)w.batch * w.heads * (read ? w.segments : w.segments - 1);
-        if (kind == SLOPES || kind == STATES_SLOPE) {
+        if (kind == STATES_SLOPE) {
             w.blocks = (w.dc + 31) / 32;
-            if constexpr (STEPS == 2)
-                if (read && slope_tiles(STEPS, walks * w.blocks) == 2) {
-                    linear_walk_kernel<TY, STEPS, 1, 2, false, SLOPES, FULL><<<walk_grid(walks * w.blocks, 4), 256, 0, stream>>>(w);
-                    return;
-                }
-            const dim3 grid = walk_grid(walks * w.blocks * 2, 4);
-            if (read) linear_walk_kernel<TY, STEPS, 1, 1, false, SLOPES, FULL><<<grid, 256, 0, stream>>>(w);
-            else linear_walk_kernel<TY, STEPS, TILES, 1, false, STATES_SLOPE, FULL><<<grid, 256, 0, stream>>>(w);
+            linear_walk_kernel<TY, STEPS, TILES, 1, false, STATES_SLOPE, FULL><<<walk_grid(walks * w.blocks * 2, 4), 256, 0, stream>>>(w);
             return;
         }
         const dim3 grid = walk_grid(walks * w.blocks, 4);
@@ -909,10 +912,16 @@ template <int TY> hipError_t launch_walk(Walk w, Kind kind, bool back, hipStream
     return hipGetLastError();
 }
 
-template <int TY> hipError_t launch_gradients(Walk v, Walk k, Walk q, hipStream_t stream) {
+// Sets `slopes` to the waves of each head and segment that leave a part of the decays' gradient.
+template <int TY> hipError_t launch_gradients(Walk v, Walk k, Walk q, uint32_t* slopes, hipStream_t stream) {
     by_shape<TY>(std::max(steps_of(v.da), steps_of(k.da)), {&v, &k, &q}, [&](auto steps, auto tiles, auto js, auto full) {
-        const dim3 grid = walk_grid((uint64_t)v.batch * v.heads * v.segments * (v.blocks + k.blocks + q.blocks), 1);
-        linear_gradients_kernel<TY, decltype(steps)::value, decltype(tiles)::value, decltype(js)::value, decltype(full)::value><<<grid, 64, 0, stream>>>(Walks{v, k, q});
+        constexpr int STEPS = decltype(steps)::value, TILES = decltype(tiles)::value, JS = decltype(js)::value;
+        constexpr bool FULL = decltype(full)::value;
+        *slopes = q.parts ? (q.dc + 31) / 32 * (2 / slope_tiles(STEPS, JS)) : 0;
+        const Walks all{v, k, q, *slopes};
+        const dim3 grid = walk_grid((uint64_t)v.batch * v.heads * v.segments * (v.blocks + k.blocks + q.blocks + *slopes), 1);
+        if (q.parts) linear_gradients_kernel<TY, STEPS, TILES, JS, FULL, true><<<grid, 64, 0, stream>>>(all);
+        else linear_gradients_kernel<TY, STEPS, TILES, JS, FULL, false><<<grid, 64, 0, stream>>>(all);
     });
     return hipGetLastError();
 }
