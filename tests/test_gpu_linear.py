@@ -458,3 +458,34 @@ def test_refusals():
     v = token[2].clone()
     want = linear_attention_step(*token, x["g"], x["state"])
     assert linear_attention_step(token[0], token[1], v, x["g"], s, out=v) is v and torch.equal(v, want)
+
+
+def test_places_behind_2_31_elements():
+    """One sequence whose values, and wide rows whose strides, go beyond 2^31 elements: the last tokens agree with a short call's."""
+    from zeno_amd.memory import linear_attention as ours
+
+    t, part = (1 << 22) + 70, 200
+    r = torch.Generator(device="cuda").manual_seed(2)
+    wide = torch.empty(1, t, 2, 8 + 8 + 256, dtype=torch.float16, device="cuda")  # 2^31 elements and more; the heads are slices of it
+    q, k, v = wide[..., :8], wide[..., 8:16], wide[..., 16:48]
+    for x in (q, k, v):
+        x.copy_(torch.randn(x.shape, generator=r, device="cuda", dtype=torch.float16))
+    assert wide.numel() > 1 << 31
+    g = torch.tensor([-1.0, -0.7], device="cuda")
+    reset = torch.zeros(1, t, dtype=torch.bool, device="cuda")
+    reset[0, t - part] = True
+    leaves = [x.detach().requires_grad_() for x in (q, k, v)]
+    o, last = ours(*leaves, g, reset)
+    tail = [x[:, t - part:].clone().requires_grad_() for x in (q, k, v)]
+    want, end = ours(*tail, g)
+    tol = 2 * HALF_ULP[torch.float16] + 2 * tolerance(part, 8, 32)
+    assert_near(o[:, t - part:], want, tol, "o")
+    assert_near(last, end, 2 * tolerance(part, 8, 32), "state")
+    d_o = torch.zeros_like(o)
+    d_o[:, t - part:] = torch.randn(want.shape, generator=r, device="cuda", dtype=torch.float16)
+    got = torch.autograd.grad(o, leaves, d_o)
+    ref = torch.autograd.grad(want, tail, d_o[:, t - part:].contiguous())
+    for n, a, b in zip("qkv", got, ref):
+        assert a.abs().sum(dtype=torch.float64).isfinite()
+        assert_near(a[:, t - part:], b, tol, "gradient of " + n)
+        assert not a[:, :t - part].any(), n

@@ -284,3 +284,20 @@ def test_refusals():
     h = x.half()
     with pytest.raises(TypeError):  # two types
         layer_norm(h, h[0], x[0])
+
+
+def test_places_behind_2_31_elements():
+    """Rows of a wide tensor beyond 2^31 elements: the last ones agree with a short call's."""
+    from zeno_amd.norm import layer_norm
+
+    wide = torch.empty((1 << 20) + 3, 2112, dtype=torch.float16, device="cuda")
+    x = wide[:, 5:37]
+    x.copy_(torch.randn(x.shape, device="cuda"))
+    assert x.stride(0) * (len(x) - 1) > 1 << 31
+    leaf = x.detach().requires_grad_()
+    y = layer_norm(leaf)
+    assert torch.equal(y[-70:], layer_norm(x[-70:].clone()))
+    d = torch.randn_like(y)
+    tail = x[-70:].clone().requires_grad_()
+    (got,), (want,) = torch.autograd.grad(y, leaf, d), torch.autograd.grad(layer_norm(tail), tail, d[-70:].contiguous())
+    assert torch.equal(got[-70:], want)
