@@ -77,9 +77,9 @@ def decay_size(x, h, do, ds, scale):
 
 
 # Batches large enough for waves of 64 columns (2048 of them), one chunk or several, whole and odd dimensions, shared heads;
-# and, the last two, for walks of gradients that are wide where the forward's are not.
+# among them some whose gradients' walks, or whose values, leave such waves half idle and are given waves of 32.
 MANY = [(2048, 9, 1, 1, 64, 64), (1030, 37, 1, 2, 33, 63), (700, 33, 3, 3, 64, 64), (520, 20, 2, 4, 24, 40), (2050, 3, 1, 1, 32, 48), (1030, 17, 1, 1, 20, 100),
-        (700, 40, 1, 1, 64, 33), (720, 18, 1, 1, 63, 16)]
+        (700, 40, 1, 1, 64, 33), (720, 18, 1, 1, 63, 16), (1030, 20, 1, 1, 64, 80), (1000, 34, 1, 2, 32, 64)]
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)

@@ -106,7 +106,7 @@ def test_gradients_that_overlap(lib, change, words):
     refused(lib.zeno_amd_linear_backward(operands(), None, gradients(**change), 16 * MIB, None), words)
 
 
-@pytest.mark.parametrize("dims, waves", [((64, 64), 5), ((8, 65), 20), ((128, 128), 20), ((65, 1), 20)])
+@pytest.mark.parametrize("dims, waves", [((64, 64), 9), ((64, 32), 9), ((8, 65), 20), ((128, 128), 20), ((65, 1), 20)])
 def test_launches(lib, dims, waves):
     """Less than 2^32 threads, 64 to a wave, also of the gradients of one token."""
     most = ((1 << 26) - 32) // waves

@@ -127,9 +127,10 @@ std::string check_sizes(const ZenoAmdLinearInputs& in, bool step) {
     if (in.value_heads % in.key_heads) return "value_heads is not a multiple of key_heads";
     if (!in.key_dim || in.key_dim > ZENO_AMD_LINEAR_MAX_DIM || !in.value_dim || in.value_dim > ZENO_AMD_LINEAR_MAX_DIM)
         return "key_dim and value_dim must be 1 to " + std::to_string(ZENO_AMD_LINEAR_MAX_DIM);
-    // A launch takes less than 2^32 threads, and is rounded up to 32 waves. Each sequence and head is up to four waves, and
-    // with dimensions over 64 twenty (three gradients, four waves of 32 columns each, and the decays', eight of 16).
-    const uint64_t waves = std::max(in.key_dim, in.value_dim) > 64 ? 20 : 5;
+    // A launch takes less than 2^32 threads, and is rounded up to 32 waves. Most is what gradients take of a sequence and head, with
+    // waves of 32 columns for three and of 16 for the decays': 4 + 4 + 4 + 8, and with dimensions to 64 and 32 values 1 + 2 + 2 + 4
+    // (64 x 64 has waves of 64 where there are many).
+    const uint64_t waves = std::max(in.key_dim, in.value_dim) > 64 ? 20 : 9;
     if (in.length > 0x7fffff00u || heads_of(in) > ((1ull << 32) / 64 - 32) / waves) return "too many sequences or tokens";
     if (step && in.length != 1) return "a step takes one token";
     return "";

@@ -842,21 +842,22 @@ inline dim3 walk_grid(uint64_t units, int waves) { return dim3((uint32_t)((units
 
 // Runs launch(steps, tiles, js, full) with the launch shape as constants, and sets the walks' number of blocks.
 // Waves of 64 columns where the registers bear them and enough of them come of it for two a SIMD: they read and multiply
-// A and B once where two of 32 do it twice (4096 sequences of 32, four heads of 64 x 64, bfloat16: 178 us, 192; but 19 of
-// 333 tokens, four heads of 24 x 48 with gradients: 213, 174). Chunks of two tiles where the registers bear them: what
-// is done to the state, its parts as operands and its decay, is done for 32 tokens at once (the same 4096 sequences with
-// gradients: 552, 579).
+// A and B once where two of 32 do it twice (4096 sequences of 32, four heads of 64 x 64, bfloat16: 178 us, 192; with gradients, float32:
+// 748, 876; but 19 of 333 tokens, four heads of 24 x 48 with gradients: 213, 174), and where none of the 64 is idle that
+// 32 would spare (gradients of 1000 sequences of 64, four heads of 32 x 64, float16: 203 us, 161). Chunks of two tiles where
+// the registers bear them: what is done to the state, its parts as operands and its decay, is done for 32 tokens at once
+// (the same 4096 sequences with gradients: 552, 579).
 template <int TY, class F> void by_shape(int steps, std::initializer_list<Walk*> walks, F&& launch) {
     constexpr std::integral_constant<int, 1> one{};
     constexpr std::integral_constant<int, 2> two{};
     constexpr std::integral_constant<int, 4> four{};
-    int most = 0;
-    uint64_t waves = 0;  // of 64 columns
+    int blocks = 0, halves = 0;  // of 64 columns and of 32
     for (const Walk* w : walks) {
-        most = std::max(most, w->dc);
-        waves += (uint64_t)w->batch * w->heads * w->segments * ((w->dc + 63) / 64);
+        blocks += (w->dc + 63) / 64;
+        halves += (w->dc + 31) / 32;
     }
-    const bool wide = most > 32 && waves >= 2048, tall = (*walks.begin())->length > 16;
+    const Walk& w0 = **walks.begin();
+    const bool wide = 2 * blocks == halves && (uint64_t)w0.batch * w0.heads * w0.segments * blocks >= 2048, tall = w0.length > 16;
     auto by_steps = [&](auto s) {
         constexpr int STEPS = decltype(s)::value;
         auto by_full = [&](auto tiles, auto js) {
@@ -917,11 +918,13 @@ template <int TY> hipError_t launch_gradients(Walk v, Walk k, Walk q, uint32_t* 
     by_shape<TY>(std::max(steps_of(v.da), steps_of(k.da)), {&v, &k, &q}, [&](auto steps, auto tiles, auto js, auto full) {
         constexpr int STEPS = decltype(steps)::value, TILES = decltype(tiles)::value, JS = decltype(js)::value;
         constexpr bool FULL = decltype(full)::value;
-        *slopes = q.parts ? (q.dc + 31) / 32 * (2 / slope_tiles(STEPS, JS)) : 0;
-        const Walks all{v, k, q, *slopes};
-        const dim3 grid = walk_grid((uint64_t)v.batch * v.heads * v.segments * (v.blocks + k.blocks + q.blocks + *slopes), 1);
-        if (q.parts) linear_gradients_kernel<TY, STEPS, TILES, JS, FULL, true><<<grid, 64, 0, stream>>>(all);
-        else linear_gradients_kernel<TY, STEPS, TILES, JS, FULL, false><<<grid, 64, 0, stream>>>(all);
+        if constexpr (STEPS > 1 || JS == 2) {  // with 32 rows at most there are 32 columns at most
+            *slopes = q.parts ? (q.dc + 31) / 32 * (2 / slope_tiles(STEPS, JS)) : 0;
+            const Walks all{v, k, q, *slopes};
+            const dim3 grid = walk_grid((uint64_t)v.batch * v.heads * v.segments * (v.blocks + k.blocks + q.blocks + *slopes), 1);
+            if (q.parts) linear_gradients_kernel<TY, STEPS, TILES, JS, FULL, true><<<grid, 64, 0, stream>>>(all);
+            else linear_gradients_kernel<TY, STEPS, TILES, JS, FULL, false><<<grid, 64, 0, stream>>>(all);
+        }
     });
     return hipGetLastError();
 }
