@@ -17,7 +17,8 @@
 // The other operands come from results without an exchange: a result tile has its rows in registers and
 // its columns in lanes, as operands have their contraction index and their other one. So P is computed
 // transposed and is then an operand along its tokens; the state's tiles are operands along its rows; and
-// B and C along the tokens are their rows' product with a unit matrix. To let eight contiguous dimensions
+// B and C along the tokens are their rows' product with a unit matrix. P and the state are operands in three parts, so all
+// of fp32, in every type (two, 2^-17 of a term, took up to 20 % less, but where terms cancel that is no small part of the sum). To let eight contiguous dimensions
 // meet the four registers of two tiles, row 4 g + r of tile h of a pair stands for dimension 8 g + 4 h + r.
 // Outputs are computed transposed, so that a lane has eight contiguous columns of its token.
 //
@@ -149,9 +150,6 @@ __device__ __forceinline__ void walk(const Walk& a, const uint32_t bh, const uin
     typedef typename Elem<TY>::type E;
     constexpr int NP = Elem<TY>::parts, C = 16 * TILES;
     constexpr bool OUT = KIND == OUTPUTS, SLOPE = KIND == SLOPES || KIND == STATES_SLOPE, GRAD = KIND == SLOPES, READ = OUT || GRAD;
-    // Operands for outputs of 16 bits that are no part of a state: two parts, 2^-17 of a term, where the output is rounded
-    // by 2^-9 or 2^-12 of itself.
-    constexpr int KEPT = TY == T_F32 || GRAD ? 3 : 2;
     const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
     const int64_t b = bh / a.heads, h = bh % a.heads;
     const int begin = segment * a.segment_length, T = begin + min(a.length - begin, a.segment_length);
@@ -403,8 +401,8 @@ __device__ __forceinline__ void walk(const Walk& a, const uint32_t bh, const uin
                     else af[k][s] = ao[k][s];
                 }
         constexpr int one = BACK ? TILES - 1 : 0;  // the tile whose tokens see no other
-        Half<KEPT> alone;
-        Frag<KEPT> both;
+        Half<3> alone;
+        Frag<3> both;
         float pairs = 0.0f;
         if constexpr (READ) {
 #pragma unroll
@@ -418,8 +416,8 @@ __device__ __forceinline__ void walk(const Walk& a, const uint32_t bh, const uin
                     if (GRAD) pairs += (float)(16 * (ti - tj) + n - 4 * g - r) * p[k][r] * y[r];
                 }
             }
-            alone = split<KEPT>(p[one]);
-            if constexpr (TILES == 2) both = BACK ? split<KEPT>(p[0], p[2]) : split<KEPT>(p[2], p[1]);
+            alone = split<3>(p[one]);
+            if constexpr (TILES == 2) both = BACK ? split<3>(p[0], p[2]) : split<3>(p[2], p[1]);
         }
         if (GRAD && JS == 1) pairs = half ? 0.0f : pairs;  // once for the two waves of these columns
         float out[TILES][U][8];
@@ -441,7 +439,7 @@ __device__ __forceinline__ void walk(const Walk& a, const uint32_t bh, const uin
                 for (int k = 0; k < TILES; ++k) x[k] = slope[k] = zero;
 #pragma unroll
                 for (int s = 0; s < STEPS; ++s) {
-                    const Frag<KEPT> sf = split<KEPT>(S[2 * s][j], S[2 * s + 1][j]);
+                    const Frag<3> sf = split<3>(S[2 * s][j], S[2 * s + 1][j]);
 #pragma unroll
                     for (int k = 0; k < TILES; ++k) x[k] = mul<2>(sf, af[k][s], x[k]);
                     if constexpr (GRAD) {
@@ -846,8 +844,9 @@ inline dim3 walk_grid(uint64_t units, int waves) { return dim3((uint32_t)((units
 // 748, 876; but 19 of 333 tokens, four heads of 24 x 48 with gradients: 213, 174), and where none of the 64 is idle that
 // 32 would spare (gradients of 1000 sequences of 64, four heads of 32 x 64, float16: 203 us, 161). Chunks of two tiles where
 // the registers bear them: what is done to the state, its parts as operands and its decay, is done for 32 tokens at once
-// (the same 4096 sequences with gradients: 552, 579).
-template <int TY, class F> void by_shape(int steps, std::initializer_list<Walk*> walks, F&& launch) {
+// (the same 4096 sequences with gradients: 552, 579). With 128 rows those of the states between segments do, those of the outputs
+// do not (2 of 4096 tokens, 8 heads of 128 x 128, bfloat16: outputs 44 us and gradients 163; two tiles, 63 and 261 registers spilled: 53 and 191).
+template <int TY, class F> void by_shape(int steps, std::initializer_list<Walk*> walks, bool outputs, F&& launch) {
     constexpr std::integral_constant<int, 1> one{};
     constexpr std::integral_constant<int, 2> two{};
     constexpr std::integral_constant<int, 4> four{};
@@ -871,7 +870,7 @@ template <int TY, class F> void by_shape(int steps, std::initializer_list<Walk*>
         };
         auto by_tiles = [&](auto js) {
             if constexpr (TY == T_BF16 || (TY == T_F16 && STEPS == 1)) {
-                if (tall) return by_full(two, js);
+                if (tall && !(STEPS == 4 && outputs)) return by_full(two, js);
             }
             by_full(one, js);
         };
@@ -887,7 +886,7 @@ template <int TY, class F> void by_shape(int steps, std::initializer_list<Walk*>
 
 template <int TY> hipError_t launch_walk(Walk w, Kind kind, bool back, hipStream_t stream) {
     const bool read = kind == OUTPUTS;
-    by_shape<TY>(steps_of(w.da), {&w}, [&](auto steps, auto tiles, auto js, auto is_full) {
+    by_shape<TY>(steps_of(w.da), {&w}, read, [&](auto steps, auto tiles, auto js, auto is_full) {
         constexpr int STEPS = decltype(steps)::value, TILES = decltype(tiles)::value, JS = decltype(js)::value;
         constexpr bool FULL = decltype(is_full)::value;
         const uint64_t walks = (uint64_t)w.batch * w.heads * (read ? w.segments : w.segments - 1);
@@ -898,7 +897,7 @@ template <int TY> hipError_t launch_walk(Walk w, Kind kind, bool back, hipStream
         }
         const dim3 grid = walk_grid(walks * w.blocks, 4);
         if (kind == OUTPUTS) {
-            linear_walk_kernel<TY, STEPS, TILES, JS, false, OUTPUTS, FULL><<<grid, 256, 0, stream>>>(w);
+            if constexpr (STEPS < 4 || TILES == 1) linear_walk_kernel<TY, STEPS, TILES, JS, false, OUTPUTS, FULL><<<grid, 256, 0, stream>>>(w);
         } else if constexpr (JS == 2) {  // segments come of too few waves for 64 columns
             if (back) linear_walk_kernel<TY, STEPS, TILES, 2, true, STATES, FULL><<<grid, 256, 0, stream>>>(w);
             else linear_walk_kernel<TY, STEPS, TILES, 2, false, STATES, FULL><<<grid, 256, 0, stream>>>(w);
@@ -915,10 +914,10 @@ template <int TY> hipError_t launch_walk(Walk w, Kind kind, bool back, hipStream
 
 // Sets `slopes` to the waves of each head and segment that leave a part of the decays' gradient.
 template <int TY> hipError_t launch_gradients(Walk v, Walk k, Walk q, uint32_t* slopes, hipStream_t stream) {
-    by_shape<TY>(std::max(steps_of(v.da), steps_of(k.da)), {&v, &k, &q}, [&](auto steps, auto tiles, auto js, auto full) {
+    by_shape<TY>(std::max(steps_of(v.da), steps_of(k.da)), {&v, &k, &q}, true, [&](auto steps, auto tiles, auto js, auto full) {
         constexpr int STEPS = decltype(steps)::value, TILES = decltype(tiles)::value, JS = decltype(js)::value;
         constexpr bool FULL = decltype(full)::value;
-        if constexpr (STEPS > 1 || JS == 2) {  // with 32 rows at most there are 32 columns at most
+        if constexpr ((STEPS > 1 || JS == 2) && (STEPS < 4 || TILES == 1)) {  // with 32 rows at most there are 32 columns at most
             *slopes = q.parts ? (q.dc + 31) / 32 * (2 / slope_tiles(STEPS, JS)) : 0;
             const Walks all{v, k, q, *slopes};
             const dim3 grid = walk_grid((uint64_t)v.batch * v.heads * v.segments * (v.blocks + k.blocks + q.blocks + *slopes), 1);
