@@ -6,6 +6,7 @@ import ctypes as C
 from typing import Optional
 
 import torch
+from torch.fx.experimental.proxy_tensor import get_proxy_mode
 
 from . import _lib as L
 
@@ -42,14 +43,30 @@ def stream(x: torch.Tensor) -> int:
     return torch._C._cuda_getCurrentRawStream(x.device.index)
 
 
+def refuse_graph() -> None:
+    """Where make_fx records torch's operations: a graph of them has the memory that a call allocates and not the call. (It
+    always sets a function mode, which is quicker to see.)"""
+    if torch._C._len_torch_function_stack() and get_proxy_mode() is not None:
+        raise RuntimeError("the library's calls are no torch operations and cannot be recorded into a graph of those")
+
+
 def on(x: torch.Tensor):
     """The context in which x's device is the current one, as the library's calls need it."""
+    refuse_graph()
     return _HERE if torch.cuda.current_device() == x.device.index else torch.cuda.device(x.device)
 
 
 def differentiated(*operands: Optional[torch.Tensor]) -> bool:
-    """Whether a call has to go through autograd: for gradients, or to be refused where tangents are carried forward."""
-    return (torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in operands)) or torch.autograd.forward_ad._current_level >= 0
+    """Whether a call has to go through autograd: for gradients, to be refused where tangents are carried forward, or
+    to be in a trace as a call, which without a function of autograd's would have the memory alone that it allocates."""
+    return ((torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in operands)) or torch.autograd.forward_ad._current_level >= 0
+            or torch._C._get_tracing_state() is not None)
+
+
+def refuse_trace(what: str) -> None:
+    """For calls that are no function of autograd's, of which a trace has nothing."""
+    if torch._C._get_tracing_state() is not None:
+        raise RuntimeError(f"{what} writes memory that a trace does not see: it cannot be traced")
 
 
 def pointer(x: Optional[torch.Tensor]) -> Optional[int]:

@@ -10,6 +10,8 @@ brings a query, a key, a value, the log of a decay and a strength, and
 ``gated_delta_step`` advances every environment's state by one token in place, beside a step of
 the simulation; ``gated_delta`` runs whole sequences (rollouts, recorded episodes) and has
 gradients for every input. Both take torch tensors on the GPU and run on torch's current stream.
+``torch.jit.trace`` records calls over whole sequences as calls; steps, and graphs of torch's own operations
+(make_fx), which would have nothing of either, are refused.
 
 Arguments, for B sequences (environments) of T tokens, Hk key heads and Hv value heads (a
 multiple of Hk; value head h reads key head h // (Hv // Hk)):
@@ -48,7 +50,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib as L
-from ._torch import DTYPES, S3, dense_like, differentiated, fail, on, pointer, row, space as bytes_for, stream, written
+from ._torch import DTYPES, S3, dense_like, differentiated, fail, on, pointer, refuse_trace, row, space as bytes_for, stream, written
 
 
 def _check(q, k, v, g, beta, reset, state, lead: int) -> None:
@@ -89,6 +91,7 @@ def _check(q, k, v, g, beta, reset, state, lead: int) -> None:
 
 def _check_step(v, state, out) -> None:
     """What a step writes in place."""
+    refuse_trace("a step")
     if not state.is_contiguous():
         raise ValueError("state must be contiguous: it is advanced in place")
     if (state.requires_grad or (out is not None and out.requires_grad)) and torch.is_grad_enabled():
@@ -207,6 +210,10 @@ def _check_linear(q, k, v, g, reset, state, lead: int) -> None:
     _check(q, k, v, each, each, reset, state, lead)
 
 
+def _scale(q, scale: Optional[float]) -> float:
+    return int(q.shape[-1]) ** -0.5 if scale is None else float(scale)  # an int: in a trace a size is a tensor, whose power has fp32's digits
+
+
 def _linear_inputs(q, k, v, g, reset, state, scale, learned) -> L.ZenoAmdLinearInputs:
     qs, ks, vs = q.stride(), k.stride(), v.stride()
     rs = (0, 0) if reset is None else reset.stride()
@@ -219,7 +226,7 @@ def _linear_inputs(q, k, v, g, reset, state, scale, learned) -> L.ZenoAmdLinearI
         rs = (rs[0], 0)
     _, hv, dv = v.shape[-3:]
     return L.ZenoAmdLinearInputs(
-        DTYPES[q.dtype], b, t, hk, hv, dk, dv, learned, scale, q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(),
+        DTYPES[q.dtype], b, t, hk, hv, dk, dv, learned, _scale(q, scale), q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(),
         None if reset is None else reset.data_ptr(), None if state is None else state.data_ptr(), qs, ks, vs, rs)
 
 
@@ -275,7 +282,6 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
     """Linear attention over whole sequences. Returns o [B, T, Hv, value_dim] in the type of v and the
     state after the last token, a new tensor. Differentiable in q, k, v, g and state."""
     _check_linear(q, k, v, g, reset, state, 2)
-    scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
     q, k, v, g = row(q), row(k), row(v), g.contiguous()
     state = None if state is None else state.contiguous()
     if differentiated(q, k, v, g, state):
@@ -293,7 +299,7 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: 
     if out is None:
         out = torch.empty_like(v, memory_format=torch.contiguous_format)
     with on(q):
-        a = _linear_inputs(q, k, v, g, reset, state, q.shape[-1] ** -0.5 if scale is None else float(scale), False)
+        a = _linear_inputs(q, k, v, g, reset, state, scale, False)
         os = out.stride()
         rc = L.load().zeno_amd_linear_step(a, out.data_ptr(), S3(os[0], 0, os[1]), state.data_ptr(), stream(q))
         if rc:

@@ -4,7 +4,7 @@
 
 over the last dimension, where s is x or, with a residual, x + residual rounded to its type: a
 block's output and the stream it is added to, in one pass. Runs on torch's current stream and has
-gradients for every input.
+gradients for every input; a trace records it as a call.
 
     x, residual    [..., dim]   float32, float16 or bfloat16, any strides
     weight, bias   [dim]        x's type or float32; None: 1 and 0

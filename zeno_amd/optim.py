@@ -16,8 +16,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib as L
-
-L.one_runtime()
+from ._torch import on, refuse_graph, refuse_trace
 
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _S3 = C.c_int64 * 3
@@ -30,6 +29,8 @@ def orthogonalize(update: torch.Tensor, steps: int = 5, coefficients: Tuple[floa
     bfloat16, on the GPU, of any strides. Returns matrices of its shape and type (`out` if given;
     out=update works in place). Results of every type are as exact as fp32 products give them,
     rounded once. Runs on torch's current stream."""
+    refuse_trace("orthogonalize")
+    refuse_graph()
     if update.dtype not in _DTYPES:
         raise TypeError(f"update must be float32, float16 or bfloat16, not {update.dtype}")
     if update.dim() < 2 or update.numel() == 0:
@@ -46,7 +47,7 @@ def orthogonalize(update: torch.Tensor, steps: int = 5, coefficients: Tuple[floa
         raise ValueError(f"out must be like update: {tuple(update.shape)}, {update.dtype}, on {update.device}")
     x = update.reshape(-1, *update.shape[-2:])
     y = out.view(-1, *update.shape[-2:])
-    with torch.cuda.device(update.device):
+    with on(update):
         lib = L.load()
         a = L.ZenoAmdOrthogonalize(_DTYPES[x.dtype], *x.shape, steps, *coefficients, eps, x.data_ptr(), _S3(*x.stride()),
                                    y.data_ptr(), _S3(*y.stride()))
