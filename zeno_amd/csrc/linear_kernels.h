@@ -28,7 +28,7 @@
 //
 // From a chunk on that holds a value that is not finite, a walk goes token by token on the vector units, so that none
 // meets an output before its token, or behind a reset, by way of the zeros in P, or another column by way of those in
-// the unit matrix.
+// the unit matrix. So do heads whose decays are so far above one that a chunk's would pass fp32's range.
 // There is one body for the chunk: with others for resets and for odd values beside it the compiler needed 168 registers
 // and spilled where 100 do.
 #pragma once
@@ -51,6 +51,22 @@ __device__ __forceinline__ float decay(float g, float m) {
     const float e = __builtin_fmaf(x, l2e, -p) + __builtin_fmaf(x, rest, low * l2e);
     return __builtin_amdgcn_exp2f(p) * __builtin_fmaf(e, ln2, 1.0f);
 }
+
+// x exp(g m) as part of it times a power of two: where exp(g m) passes fp32's range a zero stays zero, and a small x is no
+// infinity before its time.
+struct Grown {
+    float part;
+    int twos;
+    __device__ __forceinline__ Grown(float g, float m) {
+        constexpr float l2e = 1.44269504f, rest = 1.92596303e-8f, ln2 = 0.693147181f;
+        const float x = g * m, low = __builtin_fmaf(g, m, -x), p = x * l2e, e = __builtin_fmaf(x, l2e, -p) + __builtin_fmaf(x, rest, low * l2e);
+        const bool far = fabsf(p) > 600.0f;  // all of fp32's range and its like below zero
+        const float whole = far ? copysignf(600.0f, p) : ceilf(p);
+        part = far ? 0.5f : __builtin_amdgcn_exp2f(p - whole - 1.0f) * __builtin_fmaf(e, ln2, 1.0f);
+        twos = (int)whole + 1;
+    }
+    __device__ __forceinline__ float operator()(float x) const { return __builtin_ldexpf(x * part, twos); }
+};
 
 template <int TY> __device__ __forceinline__ Frag<Elem<TY>::parts> operand(const Eight<TY>& x) {
     uint32_t w[4][Elem<TY>::parts];
@@ -519,7 +535,7 @@ __device__ __forceinline__ void walk(const Walk& a, const uint32_t bh, const uin
     };
 
     // The rest of the walk token by token, without the matrix units: of values that are not finite their zeros would
-    // make NaN where the definition has none. The state goes through memory and the walk does not come back from
+    // make NaN where the definition has none, and heads that grow fast have no table of decays. The state goes through memory and the walk does not come back from
     // here, so that this rare path takes no registers from the other (with a way back each chunk moved the whole state
     // to other registers).
     auto tokens = [&](int from, int to) {  // in order of time
@@ -534,7 +550,7 @@ __device__ __forceinline__ void walk(const Walk& a, const uint32_t bh, const uin
                     if (SLOPE) kept[SLOPE][i][r][j] = N[i][j][r];
                 }
         const int m = lane_anew();
-        const float fade = decay(gh, 1.0f);
+        const Grown next(gh, 1.0f);
 #pragma unroll 1
         for (int k = from; k < to; ++k) {
             const int64_t tok = BACK ? from + to - 1 - k : k;
@@ -557,14 +573,14 @@ __device__ __forceinline__ void walk(const Walk& a, const uint32_t bh, const uin
                 for (int j = 0; j < JS; ++j) {
                     float x = kept[0][i >> 2][i & 3][j];
                     if constexpr (SLOPE) {
-                        const float y = cut ? 0.0f : fade * (kept[1][i >> 2][i & 3][j] + x);
+                        const float y = cut ? 0.0f : next(kept[1][i >> 2][i & 3][j] + x);
                         kept[1][i >> 2][i & 3][j] = y;
                         slope[j] += y * A;
                     }
-                    if (!BACK) x = cut ? 0.0f : fade * x;
+                    if (!BACK) x = cut ? 0.0f : next(x);
                     x += B * v[j];
                     o[j] += x * A;
-                    if (BACK) x = cut ? 0.0f : fade * x;
+                    if (BACK) x = cut ? 0.0f : next(x);
                     kept[0][i >> 2][i & 3][j] = x;
                 }
             }
@@ -599,7 +615,10 @@ __device__ __forceinline__ void walk(const Walk& a, const uint32_t bh, const uin
     turn_state(S);  // which has arrived by now
     if constexpr (SLOPE) turn_state(N);
     bool more = true;
-    bool fine = products(rows, cuts);
+    // A head that grows by more than exp(40) in a chunk goes token by token from the start: the chunk's decays, of which only
+    // zeros meet some, must be no infinities, and leave room for the products that they are multiplied with.
+    const bool steep = __ballot(gh * (float)min(C, a.length) > 40.0f) != 0;
+    bool fine = products(rows, cuts) && !steep;
     while (more && fine) {  // with one way out, else the state moves to other registers in every round
         any_cut |= cuts != 0;
         chunk(t, rows);
@@ -705,7 +724,7 @@ template <bool BACK, bool SLOPE> __global__ __launch_bounds__(256) void linear_j
     if (at >= a.size) return;
     float gh = a.g[bh % a.heads];
     gh = gh < -200.0f ? -200.0f : gh;
-    const float whole = decay(gh, a.segment_length);
+    const Grown whole(gh, a.segment_length);
     float* starts = a.starts + bh * between * a.size + at;
     float* slopes = SLOPE ? a.slopes + bh * between * a.size + at : nullptr;
     const float* passes = a.passes + bh * between;
@@ -726,10 +745,10 @@ template <bool BACK, bool SLOPE> __global__ __launch_bounds__(256) void linear_j
             const int64_t p = BACK ? between - 1 - k0 - k : k0 + k;
             const bool through = k0 + k > 0 && pass[k] != 0.0f;  // nothing, NaN included, passes a reset
             if (SLOPE) {
-                N = through ? V[k] + whole * (N + (float)a.segment_length * S) : V[k];
+                N = through ? V[k] + whole(N + (float)a.segment_length * S) : V[k];
                 slopes[p * a.size] = N;
             }
-            S = through ? U[k] + whole * S : U[k];
+            S = through ? U[k] + whole(S) : U[k];
             starts[p * a.size] = S;
         }
     }
@@ -777,7 +796,8 @@ __global__ __launch_bounds__(256) void linear_step_kernel(const ZenoAmdLinearInp
     const E* k = (const E*)in.k + b * in.k_stride[0] + hk * in.k_stride[2] + row0;
     const E* v = (const E*)in.v + b * in.v_stride[0] + h * in.v_stride[2] + col;
     const bool first = in.reset && in.reset[b * in.reset_stride[0]];
-    const float a = first ? 0.0f : expf(in.g[h]);
+    const float g = in.g[h];
+    float a = first ? 0.0f : expf(g);
     float* s = state + bh * dk * dv + (int64_t)row0 * dv + col;
     f4 S[ROWS];
 #pragma unroll
@@ -802,6 +822,14 @@ __global__ __launch_bounds__(256) void linear_step_kernel(const ZenoAmdLinearInp
     }
 #pragma unroll
     for (int c = 0; c < 4; ++c) vv[c] = col + c < dv ? Elem<TY>::get(v[c]) : 0.0f;
+    if (g > 80.0f && !first) {  // exp(g) may pass fp32's range
+        const Grown grown(g, 1.0f);
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) S[i][c] = grown(S[i][c]);
+        a = 1.0f;
+    }
     float kq = 0.0f;
     f4 sq = {0, 0, 0, 0};
 #pragma unroll

@@ -40,7 +40,8 @@ Linear attention with a decay for each head is the same without the correction a
 ``linear_attention_step`` and ``linear_attention`` take q, k, v, reset and state as above and g [Hv] float32. It
 costs less than the delta rule, as tokens do not wait for one another inside a sequence, but what is stored under a
 key is added to, not replaced. Its outputs grow with the state: ``zeno_amd.norm.layer_norm`` over each head's
-output usually follows. Values that are not finite are kept apart as above, in the gradients too: a NaN reaches
+output usually follows. g may be above zero: what the definition keeps within fp32 is, whatever the decays of many
+tokens would come to. Values that are not finite are kept apart as above, in the gradients too: a NaN reaches
 gradients of tokens up to its own only, through o, and none beyond a reset.
 """
 from __future__ import annotations
