@@ -69,5 +69,12 @@ def refuse_trace(what: str) -> None:
         raise RuntimeError(f"{what} writes memory that a trace does not see: it cannot be traced")
 
 
+def refuse_tangents(*operands: Optional[torch.Tensor]) -> None:
+    """For calls that are no function of autograd's, which would refuse them."""
+    forward = torch.autograd.forward_ad
+    if forward._current_level >= 0 and any(x is not None and forward.unpack_dual(x).tangent is not None for x in operands):
+        raise RuntimeError("an operand carries a tangent forward, of which a call without derivatives would make nothing")
+
+
 def pointer(x: Optional[torch.Tensor]) -> Optional[int]:
     return None if x is None else x.data_ptr()

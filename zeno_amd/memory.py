@@ -51,7 +51,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib as L
-from ._torch import DTYPES, S3, dense_like, differentiated, fail, on, pointer, refuse_trace, row, space as bytes_for, stream, written
+from ._torch import DTYPES, S3, dense_like, differentiated, fail, on, pointer, refuse_tangents, refuse_trace, row, space as bytes_for, stream, written
 
 
 def _check(q, k, v, g, beta, reset, state, lead: int) -> None:
@@ -185,9 +185,10 @@ def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
                      normalize: bool = False, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """One token for every sequence: q, k [B, Hk, key_dim], v [B, Hv, value_dim], g, beta
     [B, Hv], reset [B]. `state` (contiguous, refused if autograd follows it) is advanced in place; returns o [B, Hv, value_dim]
-    (`out` if given; it may be v, but overlap nothing else that the step reads or writes). Without gradients, even where an operand asks for them: training runs
-    gated_delta on the recorded rollout."""
+    (`out` if given; it may be v, but overlap nothing else that the step reads or writes). Without gradients, even where an operand asks for them (one that
+    carries a tangent forward is refused): training runs gated_delta on the recorded rollout."""
     _check(q, k, v, g, beta, reset, state, 1)
+    refuse_tangents(q, k, v, g, beta, state, out)
     _check_step(v, state, out)
     q, k, v = row(q), row(k), row(v)
     if out is None:
@@ -295,6 +296,7 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: 
     """One token of linear attention for every sequence: q, k [B, Hk, key_dim], v [B, Hv, value_dim], g [Hv],
     reset [B]. `state`, `out` and gradients are as gated_delta_step has them."""
     _check_linear(q, k, v, g, reset, state, 1)
+    refuse_tangents(q, k, v, g, state, out)
     _check_step(v, state, out)
     q, k, v, g = row(q), row(k), row(v), g.contiguous()
     if out is None:
