@@ -85,7 +85,8 @@ class Policy:
 
 def train(envs: int, updates: int, length: int, seed: int = 0, rate: float = 0.03, noise: float = 0.5, log=print, memory: str = "delta"):
     """Returns the mean length of the episodes that ended during each update, and how far the
-    rollout's outputs, as they were acted, are from those the training pass computes, of the largest where it is over 1."""
+    rollout's outputs, as they were acted, are from those the training pass computes (of linear attention, whose
+    outputs grow, as a share of the largest where that is over 1)."""
     torch.manual_seed(seed)
     rng = torch.Generator(device="cuda").manual_seed(seed + 1)
     policy, env = Policy(seed, memory), make("cartpole", num_envs=envs)
@@ -125,7 +126,8 @@ def train(envs: int, updates: int, length: int, seed: int = 0, rate: float = 0.0
 
         x, *tokens = policy.project(seen)
         o = policy.recall(tokens, begins, first)
-        apart = max(apart, float((o.detach() - torch.stack(outputs)).abs().max() / o.detach().abs().max().clamp(min=1.0)))
+        size = o.detach().abs().max().clamp(min=1.0) if policy.linear else 1.0
+        apart = max(apart, float((o.detach() - torch.stack(outputs)).abs().max() / size))
         loss = (0.5 * ((actions - policy.mean(x, o)) / noise).square() * advantage).mean()
         policy.update(torch.autograd.grad(loss, list(policy.matrices.values())), rate * (1.0 - step / updates))
         history.append(float(np.mean(lengths)) if lengths else float(age.mean()))
