@@ -41,8 +41,9 @@ Linear attention with a decay for each head is the same without the correction a
 costs less than the delta rule, as tokens do not wait for one another inside a sequence, but what is stored under a
 key is added to, not replaced. Its outputs grow with the state: ``zeno_amd.norm.layer_norm`` over each head's
 output usually follows. g may be above zero: what the definition keeps within fp32 is, whatever the decays of many
-tokens would come to. Values that are not finite are kept apart as above, in the gradients too: a NaN reaches
-gradients of tokens up to its own only, through o, and none beyond a reset.
+tokens would come to. Values that are not finite are kept apart as above, in the gradients too:
+one in the gradient of o or in q reaches the gradients of k and v at tokens up to its own, one in k or v those of q from its
+token on and its own token's of v or k; none passes a reset, but into the gradient of g, which is a sum over all.
 """
 from __future__ import annotations
 
