@@ -36,7 +36,6 @@ struct Walk {
     int64_t reset_stride[2];
     void* out;
     int64_t out_stride[3];
-    uint32_t out_share;
     bool out_f32;                // part sums per value head, where heads share one
     const float* first;          // the state that the walk begins with; null: zeros
     float* last;                 // the state that it ends with; null: not wanted

@@ -200,7 +200,6 @@ hipError_t forward(const ZenoAmdLinearInputs& in, void* o, const int64_t* o_stri
     w.c = rows_of(in.v, in.v_stride, 1);
     w.out = o;
     set_strides(w.out_stride, o_stride);
-    w.out_share = 1;
     w.first = in.state;
     w.last = last;
     w.passes = workspace;
@@ -226,7 +225,6 @@ hipError_t backward(const ZenoAmdLinearInputs& in, const float* saved, const Zen
     auto key_out = [&](Walk& w, void* to, const int64_t* stride, float* part) {
         w.out = share > 1 ? part : to;
         set_strides(w.out_stride, share > 1 ? part_stride : stride);
-        w.out_share = 1;
         w.out_f32 = share > 1;
     };
 
@@ -236,7 +234,6 @@ hipError_t backward(const ZenoAmdLinearInputs& in, const float* saved, const Zen
     wq.a = d_o, wq.b = v, wq.c = k, wq.q = q;
     wv.out = grad.d_v;
     set_strides(wv.out_stride, grad.d_v_stride);
-    wv.out_share = 1;
     key_out(wk, grad.d_k, grad.d_k_stride, part_k);
     key_out(wq, grad.d_q, grad.d_q_stride, part_q);
     wv.first = wk.first = wq.d_last = grad.d_last;

@@ -516,7 +516,7 @@ __device__ __forceinline__ void walk(const Walk& a, const uint32_t bh, const uin
 #pragma unroll
                     for (int k = 0; k < TILES; ++k) {
                         const int row = 16 * k + (l & 15);
-                        const int64_t to = (b * a.out_stride[0] + (h / a.out_share) * a.out_stride[2] + t * a.out_stride[1] + col0 + 32 * u) + (row * a.out_stride[1] + 8 * (l >> 4));
+                        const int64_t to = (b * a.out_stride[0] + h * a.out_stride[2] + t * a.out_stride[1] + col0 + 32 * u) + (row * a.out_stride[1] + 8 * (l >> 4));
                         if (row < len) {
                             if (a.out_f32) {
                                 Eight<T_F32> x;
@@ -589,7 +589,7 @@ __device__ __forceinline__ void walk(const Walk& a, const uint32_t bh, const uin
                 o[j] += __shfl_xor(o[j], 16);
                 o[j] += __shfl_xor(o[j], 32);
                 if (OUT && m < 16 && c[j] < dc) {
-                    const int64_t to = b * a.out_stride[0] + (h / a.out_share) * a.out_stride[2] + tok * a.out_stride[1] + col0 + c[j];
+                    const int64_t to = b * a.out_stride[0] + h * a.out_stride[2] + tok * a.out_stride[1] + col0 + c[j];
                     const float y = o[j] * (BACK ? 1.0f : a.scale);
                     if (a.out_f32) ((float*)a.out)[to] = y;
                     else ((E*)a.out)[to] = Elem<TY>::put(y);
