@@ -53,6 +53,12 @@ struct Walk {
     uint32_t blocks;             // waves that share the columns, set at the launch
 };
 
+// Two waves a SIMD. Sequences are cut into segments for as many waves (of 32 columns) at most, and waves of 64 columns are
+// taken where there are as many of those, which fill their columns: never of a sequence that is cut, so the states between
+// segments have no kernel for them.
+constexpr int kWaves = 2048;
+inline bool wide(uint64_t walks, int blocks, int halves) { return 2 * blocks == halves && walks * blocks >= kWaves; }  // of 64 columns and of 32
+
 // A wave holds 32 times 1, 2 or 4 rows of a state.
 inline int steps_of(int da) { return da <= 32 ? 1 : da <= 64 ? 2 : 4; }
 // Tiles of 16 columns of a wave of the decays' gradient, which carries the state and its slope; `js` is of the waves beside it. Two

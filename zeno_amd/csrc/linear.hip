@@ -112,7 +112,7 @@ std::string check_outputs(const std::vector<Memory>& inputs, const std::vector<M
 Segments segments_of(const ZenoAmdLinearInputs& in) {
     const int64_t chunks = ((int64_t)in.length + kChunk - 1) / kChunk;
     const int64_t waves = (int64_t)heads_of(in) * blocks_of(in.value_dim);
-    const int64_t want = std::max<int64_t>(std::min(2048 / waves, chunks / 2), 1), each = (chunks + want - 1) / want;
+    const int64_t want = std::max<int64_t>(std::min(kWaves / waves, chunks / 2), 1), each = (chunks + want - 1) / want;
     return Segments{(uint32_t)((chunks + each - 1) / each), (int)(each * kChunk)};
 }
 

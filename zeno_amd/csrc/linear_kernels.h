@@ -884,7 +884,7 @@ template <int TY, class F> void by_shape(int steps, std::initializer_list<Walk*>
         halves += (w->dc + 31) / 32;
     }
     const Walk& w0 = **walks.begin();
-    const bool wide = 2 * blocks == halves && (uint64_t)w0.batch * w0.heads * w0.segments * blocks >= 2048, tall = w0.length > 16;
+    const bool four_tiles = wide((uint64_t)w0.batch * w0.heads * w0.segments, blocks, halves), tall = w0.length > 16;
     auto by_steps = [&](auto s) {
         constexpr int STEPS = decltype(s)::value;
         auto by_full = [&](auto tiles, auto js) {
@@ -903,7 +903,7 @@ template <int TY, class F> void by_shape(int steps, std::initializer_list<Walk*>
             by_full(one, js);
         };
         if constexpr (STEPS < 4) {
-            if (wide) return by_tiles(four);
+            if (four_tiles) return by_tiles(four);
         }
         by_tiles(two);
     };
@@ -914,23 +914,26 @@ template <int TY, class F> void by_shape(int steps, std::initializer_list<Walk*>
 
 template <int TY> hipError_t launch_walk(Walk w, Kind kind, bool back, hipStream_t stream) {
     const bool read = kind == OUTPUTS;
+    hipError_t shape = hipErrorInvalidValue;  // of no kernel
     by_shape<TY>(steps_of(w.da), {&w}, read, [&](auto steps, auto tiles, auto js, auto is_full) {
         constexpr int STEPS = decltype(steps)::value, TILES = decltype(tiles)::value, JS = decltype(js)::value;
         constexpr bool FULL = decltype(is_full)::value;
         const uint64_t walks = (uint64_t)w.batch * w.heads * (read ? w.segments : w.segments - 1);
+        auto run = [&](auto kernel, uint64_t waves) {
+            kernel<<<walk_grid(waves, 4), 256, 0, stream>>>(w);
+            shape = hipSuccess;
+        };
         if (kind == STATES_SLOPE) {
             w.blocks = (w.dc + 31) / 32;
-            linear_walk_kernel<TY, STEPS, TILES, 1, false, STATES_SLOPE, FULL><<<walk_grid(walks * w.blocks * 2, 4), 256, 0, stream>>>(w);
-            return;
-        }
-        const dim3 grid = walk_grid(walks * w.blocks, 4);
-        if (kind == OUTPUTS) {
-            if constexpr (STEPS < 4 || TILES == 1) linear_walk_kernel<TY, STEPS, TILES, JS, false, OUTPUTS, FULL><<<grid, 256, 0, stream>>>(w);
-        } else if constexpr (JS == 2) {  // segments come of too few waves for 64 columns
-            if (back) linear_walk_kernel<TY, STEPS, TILES, 2, true, STATES, FULL><<<grid, 256, 0, stream>>>(w);
-            else linear_walk_kernel<TY, STEPS, TILES, 2, false, STATES, FULL><<<grid, 256, 0, stream>>>(w);
+            run(linear_walk_kernel<TY, STEPS, TILES, 1, false, STATES_SLOPE, FULL>, walks * w.blocks * 2);
+        } else if (kind == OUTPUTS) {
+            if constexpr (STEPS < 4 || TILES == 1) run(linear_walk_kernel<TY, STEPS, TILES, JS, false, OUTPUTS, FULL>, walks * w.blocks);
+        } else if constexpr (JS == 2) {
+            if (back) run(linear_walk_kernel<TY, STEPS, TILES, 2, true, STATES, FULL>, walks * w.blocks);
+            else run(linear_walk_kernel<TY, STEPS, TILES, 2, false, STATES, FULL>, walks * w.blocks);
         }
     });
+    if (shape != hipSuccess) return shape;
     if (!read && w.segments > 2) {
         const dim3 join(w.batch * w.heads * (uint32_t)((w.size + 255) / 256));
         if (back) linear_join_kernel<true, false><<<join, 256, 0, stream>>>(w);
@@ -942,6 +945,7 @@ template <int TY> hipError_t launch_walk(Walk w, Kind kind, bool back, hipStream
 
 // Sets `slopes` to the waves of each head and segment that leave a part of the decays' gradient.
 template <int TY> hipError_t launch_gradients(Walk v, Walk k, Walk q, uint32_t* slopes, hipStream_t stream) {
+    hipError_t shape = hipErrorInvalidValue;  // of no kernel
     by_shape<TY>(std::max(steps_of(v.da), steps_of(k.da)), {&v, &k, &q}, true, [&](auto steps, auto tiles, auto js, auto full) {
         constexpr int STEPS = decltype(steps)::value, TILES = decltype(tiles)::value, JS = decltype(js)::value;
         constexpr bool FULL = decltype(full)::value;
@@ -951,9 +955,10 @@ template <int TY> hipError_t launch_gradients(Walk v, Walk k, Walk q, uint32_t* 
             const dim3 grid = walk_grid((uint64_t)v.batch * v.heads * v.segments * (v.blocks + k.blocks + q.blocks + *slopes), 1);
             if (q.parts) linear_gradients_kernel<TY, STEPS, TILES, JS, FULL, true><<<grid, 64, 0, stream>>>(all);
             else linear_gradients_kernel<TY, STEPS, TILES, JS, FULL, false><<<grid, 64, 0, stream>>>(all);
+            shape = hipSuccess;
         }
     });
-    return hipGetLastError();
+    return shape != hipSuccess ? shape : hipGetLastError();
 }
 
 template <int TY> hipError_t launch_share(const ZenoAmdLinearInputs& in, const float* part_q, const float* part_k, const ZenoAmdLinearGradients& grad, hipStream_t stream) {
