@@ -411,8 +411,9 @@ typedef struct {
 int zeno_amd_linear_forward(const ZenoAmdLinearInputs* in, void* o, const int64_t* o_stride, float* last, void* saved, void* workspace, void* stream);
 
 /* Gradients of a zeno_amd_linear_forward call with the same inputs, which left `saved`. `workspace`:
- * zeno_amd_linear_workspace_bytes(in, 1) bytes. The gradient of g keeps fp32's digits relative to its own
- * size for heads that forget fast too. All sums are in a fixed order: results are bitwise reproducible. */
+ * zeno_amd_linear_workspace_bytes(in, 1) bytes. The gradient of g is a sum of terms that have fp32's digits each,
+ * and of no differences of larger numbers: relative to the sizes of its terms it has them, for heads that forget fast
+ * too. All sums are in a fixed order: results are bitwise reproducible. */
 int zeno_amd_linear_backward(const ZenoAmdLinearInputs* in, const void* saved, const ZenoAmdLinearGradients* grad, void* workspace, void* stream);
 
 uint64_t zeno_amd_linear_saved_bytes(const ZenoAmdLinearInputs* in);  /* 0 also for invalid inputs */

@@ -106,9 +106,9 @@ std::string check_outputs(const std::vector<Memory>& inputs, const std::vector<M
 
 }  // namespace
 
-// With fewer waves than two a SIMD, as many segments as make up those, of at least two chunks of 32. (One sequence of
-// 16384, 8 heads of 128 x 128, float16: 157 us, with one wave a SIMD 189, with four 182; 2 of 4096 with gradients, bfloat16: 309,
-// 298 and 391; 19 of 333 tokens, four heads of 24 x 48, float32, with gradients: 102, in segments of at least four chunks 138.)
+// With fewer waves than two a SIMD, as many segments as make up those, of at least two chunks of 32. (Kernels of one sequence of
+// 16384, 8 heads of 128 x 128, float16: 168 us, with one wave a SIMD 200, with four 193; of 2 of 4096 with gradients, bfloat16: 305,
+// 299 and 391; of 19 of 333 tokens, four heads of 24 x 48, float32, with gradients: 101, in segments of at least four chunks 139.)
 Segments segments_of(const ZenoAmdLinearInputs& in) {
     const int64_t chunks = ((int64_t)in.length + kChunk - 1) / kChunk;
     const int64_t waves = (int64_t)heads_of(in) * blocks_of(in.value_dim);

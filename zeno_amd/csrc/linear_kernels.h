@@ -10,8 +10,8 @@
 //
 // A wave owns 32 or 64 columns of the state, all of its rows, and works alone: no LDS, no barrier. That leaves no
 // wait but for memory, and the vector instructions bound it: of 16384 tokens of 8 heads of 128 x 128, float16, each of a SIMD's two
-// waves issues them 37 % of its time and keeps the matrix units busy for 24 % (outputs 87 us). Many short sequences are bound by
-// memory: 16384 of 16 tokens, two heads of 64 x 64, bfloat16: 1.34 GB in 267 us, 5.0 TB/s.
+// waves issues them 40 % of its time and keeps the matrix units busy for 23 % (outputs 95 us). Many short sequences are bound by
+// memory: 16384 of 16 tokens, two heads of 64 x 64, bfloat16: 1.34 GB in 269 us, 5.0 TB/s.
 // Rows are read as they lie, 16 bytes a lane: lane (n, g) has row n's dimensions 8 g to 8 g + 7 of
 // every 32. That is an operand of the matrix units as it is, for contractions along the dimensions.
 // The other operands come from results without an exchange: a result tile has its rows in registers and
@@ -392,8 +392,9 @@ __device__ __forceinline__ void walk(const Walk& a, const uint32_t bh, const uin
         return __ballot(!fine) == 0;
     };
 
-    // The chunk of tokens t to t + len. No branch is inside: where one lies between a matrix instruction and the use of
-    // its result, the compiler has been seen to leave out the wait. The scheduler is kept from starting everything at
+    // The chunk of tokens t to t + len. But for the stores of 32 columns, between the products of two column tiles, no branch is
+    // inside: where one lies between a matrix instruction and the use of its result, the compiler has been seen to leave out
+    // the wait (tests/test_matrix_waits.py follows every path of what it made). The scheduler is kept from starting everything at
     // once, which takes more registers than there are.
     auto chunk = [&](int t, int len) {
         const f4 zero = {0, 0, 0, 0};
@@ -688,9 +689,11 @@ __global__ __launch_bounds__(256, walk_waves(TY, STEPS, TILES, JS, KIND)) void l
 }
 
 // All gradients: the walks of d_v, d_k and d_q of a head and segment side by side, as they read the same rows: of 4096
-// sequences of 32 tokens, four heads of 64 x 64, in bfloat16, 366 us, and one after the other 490. Where the decays are learned
-// the walk of their gradient too: 520 us, by itself behind the others 366 and 235; 19 sequences of 333, four heads of 24 x 48, float32:
-// 36, and 34 and 25. A workgroup is one wave, as the walks take unlike times (workgroups of four, the first three: 400 us).
+// sequences of 32 tokens, four heads of 64 x 64, in bfloat16, 346 us (one after the other 490 where this took 366). Where the decays are
+// learned the walk of their gradient too: 471 us (behind the others 366 and 235, this 520); 19 sequences of 333, four heads of 24 x 48,
+// float32: 35 (34 and 25, this 36). A workgroup is one wave, as the walks take unlike times (of four, the first three: 400, this 366).
+// Bound by neither of memory and instructions: caches hold the second and third readings (788 MB read, 462 written, what they
+// cannot be without is 804 and 470), which flow at 3.6 TB/s, as a wave reads, multiplies, stores and ends, and two a SIMD overlap.
 struct Walks {
     Walk v, k, q;
     uint32_t slopes;  // waves of the decays' gradient, for each head and segment
@@ -717,7 +720,7 @@ __global__ __launch_bounds__(64, gradient_waves(TY, STEPS, TILES, JS, LEARNED)) 
 // The states between segments from what each adds: S_{p+1} = exp(g L) S_p + U_p, in place of U, where
 // the segment passes a state at all; and the slopes, N_{p+1} = exp(g L) (N_p + L S_p) + V_p. A thread a value;
 // eight segments' values are read at once, as each read waits for memory. Bound by those waits: 64 segments of 8 heads of
-// 128 x 128, 33 MB read and written: 14 us, 4.8 TB/s of which caches hold most; with slopes and 32 segments of 16 heads 23.
+// 128 x 128, 33 MB read and written: 14 us, 4.8 TB/s of which caches hold most; with slopes and 32 segments of 16 heads 21.
 template <bool BACK, bool SLOPE> __global__ __launch_bounds__(256) void linear_join_kernel(const Walk a) {
     const int64_t between = a.segments - 1, blocks = (a.size + 255) / 256;
     const int64_t bh = blockIdx.x / blocks, at = blockIdx.x % blocks * 256 + threadIdx.x;
@@ -779,7 +782,7 @@ template <int TY> __global__ __launch_bounds__(256) void linear_share_kernel(con
 // ---- one token -----------------------------------------------------------------------------
 // The state is read once and written once. A wave holds all rows of 4 LANES columns, 16 (or 4) rows and 4
 // columns a lane:  o = scale (a S^T q + (k . q) v),  S <- a S + k v^T.  LANES lanes lie along the
-// columns, 64 / LANES along the rows. Bound by memory: 4096 sequences of four heads of 64 x 64, 0.55 GB of state in 121 us,
+// columns, 64 / LANES along the rows. Bound by memory: 4096 sequences of four heads of 64 x 64, 0.55 GB of state in 118 us,
 // 4.6 TB/s.
 template <int TY, int LANES, int ROWS, bool VEC>
 __global__ __launch_bounds__(256) void linear_step_kernel(const ZenoAmdLinearInputs in, void* out, int64_t o_batch, int64_t o_head, float* state) {
@@ -868,12 +871,12 @@ inline dim3 walk_grid(uint64_t units, int waves) { return dim3((uint32_t)((units
 
 // Runs launch(steps, tiles, js, full) with the launch shape as constants, and sets the walks' number of blocks.
 // Waves of 64 columns where the registers bear them and enough of them come of it for two a SIMD: they read and multiply
-// A and B once where two of 32 do it twice (4096 sequences of 32, four heads of 64 x 64, bfloat16: 178 us, 192; with gradients, float32:
-// 748, 876; but 19 of 333 tokens, four heads of 24 x 48 with gradients: 213, 174), and where none of the 64 is idle that
-// 32 would spare (gradients of 1000 sequences of 64, four heads of 32 x 64, float16: 203 us, 161). Chunks of two tiles where
+// A and B once where two of 32 do it twice (4096 sequences of 32, four heads of 64 x 64, bfloat16: 167 us, 191; with gradients, float32:
+// 667, 778; but 100 of them with gradients, bfloat16: 30, 25), and where none of the 64 is idle that
+// 32 would spare (gradients of 1000 sequences of 64, four heads of 32 x 64, float16: 163 us, 106). Chunks of two tiles where
 // the registers bear them: what is done to the state, its parts as operands and its decay, is done for 32 tokens at once
-// (the same 4096 sequences with gradients: 552, 579). With 128 rows those of the states between segments do, those of the outputs
-// do not (2 of 4096 tokens, 8 heads of 128 x 128, bfloat16: outputs 44 us and gradients 163; two tiles, 63 and 261 registers spilled: 53 and 191).
+// (the same 4096 sequences with gradients, bfloat16: 517, 588). With 128 rows those of the states between segments do, those of the outputs
+// do not (2 of 4096 tokens, 8 heads of 128 x 128, bfloat16: outputs 43 us and gradients 159; two tiles, 63 and 261 registers spilled: 53 and 191).
 template <int TY, class F> void by_shape(int steps, std::initializer_list<Walk*> walks, bool outputs, F&& launch) {
     constexpr std::integral_constant<int, 1> one{};
     constexpr std::integral_constant<int, 2> two{};

@@ -72,8 +72,10 @@ void set_strides(int64_t* to, const int64_t* from) {
 // A row of up to 1024 features is held by part of a wave or a wave, one or two vectors a lane; a wider
 // one by a workgroup. Of 65536 rows of 1024, bfloat16, the norm takes 43 us and the gradients 95, by a workgroup of 256 to the row 85
 // and 154; of 16384 rows of 4096 by 256 threads 45 and 100, by 1024 95 and 179; of 524288 rows of 64 by 8 lanes 23 us, by 16 39.
-// Workgroups as fill the device several times over, each with several rows, as each reads the weights and leaves sums: of
-// 131072 rows of 512 the gradients take 89 us, with half as many 122, with twice as many 93.
+// Workgroups as fill the device several times over, each with several rows, as each reads the weights and leaves sums. Gradients
+// (us; with half as many, with twice as many): 131072 rows of 512 86 (122, 92), 32768 of 2048 88 (119, 93), 8192 of 8192 116 (200,
+// 121), 65536 of 1024 95 (87, 90), 16384 of 4096 101 (93, 99), 524288 of 64 71 (68, 71), 131072 of 200 73 (70, 71); float32: 16384 of
+// 2500 177 (160, 152), 65536 of 1000 162 (155, 166).
 Shape shape_of(const ZenoAmdNormInputs& in, bool train) {
     Shape s;
     const uint32_t n = in.dim;

@@ -9,9 +9,12 @@
 // The backward pass finds mean and r again from s, which it has to read anyway: two sums of values
 // in registers for 8 bytes a row less each way.
 //
-// Bound by memory. Forward, bfloat16: 524288 rows of 64 23 us, 131072 of 512 44, 16384 of 4096 45, that is 5.8 to 6.1 TB/s;
-// 65536 of 1000 in float32 106, 4.9. Gradients, whose sums by column hold twice the registers and so fewer waves: 131072 of
-// 512 89 us, 4.5 TB/s; 65536 of 1000 in float32 163, 4.8; 8192 of 8192 116, 3.5 (two barriers a row of 1024 threads).
+// Bound by memory. Forward, bfloat16: 524288 rows of 64 23 us, 131072 of 512 45, 16384 of 4096 45, that is 5.7 to 6.0 TB/s;
+// 65536 of 1000 in float32 106, 4.9. Narrower rows less, 524288 of 32 22 us, 3.1. Gradients, whose sums by column hold twice
+// the registers and so fewer waves: 131072 of 512 86 us, 4.7 TB/s; 65536 of 1000 in float32 162, 4.8; 16384 of 4096 101, 4.0; 8192 of
+// 8192 116, 3.5 (two barriers a row of 1024 threads). Those of narrow rows are bound by waits, for a row's two reads and then for sums across
+// lanes that follow on one another, with no other row in flight: 524288 of 64 71 us, 2.8 TB/s, 131072 of 200 73, 2.2, 524288 of 32 71,
+// 1.4; and 16384 of 2500 in float32 177, 2.8, fill 61 % of their lanes' 4096 places.
 //
 // A row is held in registers by LANES lanes of a wave (or by a workgroup), V vectors of eight
 // elements each, so memory is read once. A lane keeps its columns from row to row: the weights stay

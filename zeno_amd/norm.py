@@ -12,8 +12,8 @@ gradients for every input; a trace records it as a call.
 dim is 1 to 16384; a row of x may begin anywhere (a slice of wider rows needs no copy), its features
 are contiguous or x is copied first. Each head's output [..., heads, dim] is normalised by the same
 call. Sums and statistics are fp32, in the gradients of the weight and the bias too; results and
-gradients are rounded once, and are the same from run to run. Squares of a row's distances from its mean
-have to stay in fp32's range (distances below 1e17 do, whatever dim is); a NaN or an infinity spoils its own row, and of the gradients
+gradients are rounded once, and are the same from run to run. The sum of a row's values and of the
+squares of their distances from its mean have to stay in fp32's range (values below 1e34 and distances below 1e17 do, whatever dim is); a NaN or an infinity spoils its own row, and of the gradients
 its row's and those of the weight and the bias.
 """
 from __future__ import annotations
